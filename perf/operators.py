@@ -359,8 +359,9 @@ def _plain_q8(x):
     xp = torch.cat([x, torch.zeros(r, pad, device=x.device)], 1).view(r, -1, Q_BLOCK)
     top = xp.abs().max(2, keepdim=True).values
     tiny = top < 2.0 ** -100
-    inv = torch.where(tiny, torch.zeros_like(top), 127.0 / top)
-    return (torch.round(xp * inv) * (top / 127.0)).view(r, c + pad)[:, :c]
+    full = torch.full_like(top, 127.0)  # a tensor: dividing by a number multiplies by its reciprocal
+    inv = torch.where(tiny, torch.zeros_like(top), full / top)
+    return (torch.round(xp * inv) * (top / full)).view(r, c + pad)[:, :c]
 
 
 def _plain_swiglu8(st):
@@ -539,8 +540,9 @@ def _exact_swiglu8(st):
         out = torch.empty(t.shape, dtype=torch.float64, device=t.device)
         for blk, dst in zip(t.split(Q_BLOCK, dim=1), out.split(Q_BLOCK, dim=1)):
             top = blk.abs().amax(1, keepdim=True)
-            inv = torch.where(top < 2.0 ** -100, torch.zeros_like(top), 127.0 / top)
-            dst.copy_(torch.round(blk * inv).to(torch.float64) * (top / 127.0).to(torch.float64))
+            most = torch.full_like(top, 127.0)
+            inv = torch.where(top < 2.0 ** -100, torch.zeros_like(top), torch.div(most, top))
+            dst.copy_(torch.round(blk * inv).to(torch.float64) * torch.div(top, most).to(torch.float64))
         return out
 
     g, u, dy = (st[n].detach().to(torch.float64) for n in ("gate", "up", "dy"))
