@@ -42,6 +42,7 @@ class SoupError(RuntimeError):
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_f = ctypes.c_float
+c_d = ctypes.c_double
 c_vp = ctypes.c_void_p
 c_sz = ctypes.c_size_t
 P_I64 = ctypes.POINTER(ctypes.c_int64)
@@ -89,6 +90,31 @@ _SIGNATURES = {
     "soup_attention_bwd": (c_int, [c_vp, P_I64, c_vp, P_I64, c_vp, P_I64, c_vp, c_vp, c_vp, c_i64,
                                    c_i64, c_i64, c_i64, c_i64, c_f, c_int, c_vp, c_vp, c_vp, c_vp,
                                    c_sz, c_vp]),
+    "soup_attention_window_fwd": (c_int, [c_vp, P_I64, c_vp, P_I64, c_vp, P_I64, c_i64, c_i64, c_i64,
+                                          c_i64, c_i64, c_f, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "soup_attention_window_bwd": (c_int, [c_vp, P_I64, c_vp, P_I64, c_vp, P_I64, c_vp, c_vp, c_vp, c_i64,
+                                          c_i64, c_i64, c_i64, c_i64, c_f, c_i64, c_i64, c_vp, c_vp, c_vp,
+                                          c_vp, c_sz, c_vp]),
+    "soup_head_logps_state_bytes": (c_sz, [c_i64, c_i64, c_i64]),
+    "soup_head_logps_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_int]),
+    "soup_head_logps_fwd": (c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_i64, c_i64, c_i64, c_i64,
+                                    c_vp, c_vp, c_vp, c_sz, c_vp, c_sz, c_vp]),
+    "soup_head_logps_bwd": (c_int, [c_vp, c_sz, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,
+                                    c_i64, c_i64, c_vp, c_int, c_vp, c_int, c_int, c_vp, c_sz, c_vp]),
+    "soup_preference_loss_workspace_bytes": (c_sz, [c_i64, c_i64]),
+    "soup_preference_loss_fwd": (c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_i64, c_i64, c_i64, c_i64,
+                                         c_d, c_d, c_int, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "soup_preference_loss_bwd": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp]),
+    "soup_policy_loss_workspace_bytes": (c_sz, [c_i64, c_i64]),
+    "soup_policy_loss_fwd": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64,
+                                     c_i64, c_i64, c_d, c_d, c_f, c_int, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                     c_vp, c_sz, c_vp]),
+    "soup_policy_loss_bwd": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp]),
+    "soup_swiglu_q8_fwd": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp,
+                                   c_i64, c_i64, c_i64, c_int, c_vp]),
+    "soup_swiglu_q8_bwd": (c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,
+                                   c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]),
+    "soup_q8_quantize": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]),
     "soup_nf4_quantize": (c_int, [c_vp, c_i64, c_int, c_int, ctypes.POINTER(c_f), c_vp, c_vp, c_vp]),
     "soup_nf4_dequant": (c_int, [c_vp, c_vp, c_i64, c_int, ctypes.POINTER(c_f), c_vp, c_int, c_vp]),
     "soup_gemm_stream_k_workspace_bytes": (c_sz, []),

@@ -177,7 +177,36 @@ struct AttnArgs {
   float* lse;            // [B, H, S_pad] natural-log log-sum-exp of scale * q.k, rows
                          // padded to S_pad = S rounded up to 128 (padding not written)
   uint64_t wait_ns;
+  int window, sinks;     // kWin kernels only: 1 <= window <= S, 0 <= sinks <= S
 };
+
+// Sliding window with sinks (the kernels' kWin form, always causal): query q
+// sees key k iff k <= q and (q - k < window or k < sinks). The key tiles that
+// a run of queries starting at q0 needs, in the order the kernels take them:
+// the sink tiles that lie before the window's first tile, then the window's
+// tiles up to the diagonal. Tiles outside the list are never loaded, so the
+// work is (window + sinks) keys a query instead of the whole prefix.
+struct KeyTiles {
+  int n_sink, lo;  // leading sink tiles; first tile of the window
+  __device__ __forceinline__ int at(int j) const { return j < n_sink ? j : lo + (j - n_sink); }
+};
+__device__ __forceinline__ KeyTiles key_tiles(int q0, int window, int sinks) {
+  KeyTiles t;
+  const int first = q0 - window + 1;
+  t.lo = first > 0 ? first / kTile : 0;
+  const int ns = (sinks + kTile - 1) / kTile;
+  t.n_sink = ns < t.lo ? ns : t.lo;
+  return t;
+}
+// (q, k) outside the window and not a sink
+__device__ __forceinline__ bool win_hidden(int q, int key, int window, int sinks) {
+  return q - key >= window && key >= sinks;
+}
+// Some pair of the tile of keys [k0, k0 + 128) and the queries up to q_max is
+// hidden by the window.
+__device__ __forceinline__ bool win_edge(int q_max, int k0, int window, int sinks) {
+  return q_max - k0 >= window && k0 + kTile > sinks;
+}
 
 // D (TMEM) [+]= A (TMEM, M rows in lanes, two bf16 of K per 32-bit column) x B (smem descriptor).
 __device__ __forceinline__ void tc_mma_bf16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
@@ -288,6 +317,7 @@ __device__ __noinline__ void rescale_o_row(uint32_t o_t, float alpha) {
   }
 }
 
+template <bool kWin>
 __global__ void __launch_bounds__(kFwdThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                     const __grid_constant__ CUtensorMap tma_v, AttnArgs a, int* err) {
@@ -323,8 +353,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const int b = bh / a.H, h = bh % a.H;
   const int hk = h / (a.H / a.Hk);
   // key tiles each query tile attends to (B's are a superset of A's)
-  const int nkv_a = a.causal ? 2 * pr + 1 : nq;
-  const int nkv_b = a.causal ? (2 * pr + 2 < nq ? 2 * pr + 2 : nq) : nq;
+  KeyTiles kt{0, 0};
+  if (kWin) kt = key_tiles(2 * pr * kTile, a.window, a.sinks);
+  const int skip = kWin ? kt.lo - kt.n_sink : 0;  // tiles of the prefix not in the list
+  const int nkv_a = (a.causal ? 2 * pr + 1 : nq) - skip;
+  const int nkv_b = (a.causal ? (2 * pr + 2 < nq ? 2 * pr + 2 : nq) : nq) - skip;
   const uint64_t wait_ns = a.wait_ns;
 
   if (threadIdx.x == 0) {
@@ -368,21 +401,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       int issued_k = 0, issued_v = 0;
       for (int j = 0; j < nkv_b; ++j) {
         const int sk = j % kKStages, sv = j % kVStages;
+        const int key0 = (kWin ? kt.at(j) : j) * kTile;
         if (!bounded_wait(k_empty(sk), ((j / kKStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t kd = sbase + L::kK + sk * kTileBytes;
         mbar_arrive_expect_tx(k_full(sk), kTileBytes);
-        tma_load_4d(kd, &tma_k, k_full(sk), 0, j * kTile, hk, b);
-        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, j * kTile, hk, b);
+        tma_load_4d(kd, &tma_k, k_full(sk), 0, key0, hk, b);
+        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, key0, hk, b);
         ++issued_k;
         if (!bounded_wait(v_empty(sv), ((j / kVStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t vd = sbase + L::kV + sv * kTileBytes;
         mbar_arrive_expect_tx(v_full(sv), kTileBytes);
-        tma_load_4d(vd, &tma_v, v_full(sv), 0, j * kTile, hk, b);
-        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, j * kTile, hk, b);
+        tma_load_4d(vd, &tma_v, v_full(sv), 0, key0, hk, b);
+        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, key0, hk, b);
         ++issued_v;
       }
       // let every issued copy land before the CTA may leave (bounded)
@@ -476,12 +510,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint64_t sl2 = f2_pack(a.scale_log2, a.scale_log2);
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
-    // -inf for keys beyond the sequence and (causal) keys after the query
+    // -inf for keys beyond the sequence, (causal) keys after the query and, with a
+    // window, keys before it that are no sinks
     auto mask32 = [&](float (&v)[32], int key0) {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const int key = key0 + i;
-        if (key >= a.S || (a.causal && key > q)) v[i] = -INFINITY;
+        if (key >= a.S || (a.causal && key > q) ||
+            (kWin && win_hidden(q, key, a.window, a.sinks)))
+          v[i] = -INFINITY;
       }
     };
     auto max32 = [&](const float (&v)[32]) -> float {
@@ -517,8 +554,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (lane == 0) w = bounded_wait(s_full(x), j & 1, abort_flag, err, kErrAttnSoftmax, wait_ns);
       if (!(ok = warp_ok(w))) break;
       tc_fence_after();
-      const int k0 = j * kTile;
-      const bool edge = (k0 + kTile > a.S) || (a.causal && j == qt);
+      const int jt = kWin ? kt.at(j) : j;
+      const int k0 = jt * kTile;
+      const bool edge = (k0 + kTile > a.S) || (a.causal && jt == qt) ||
+                        (kWin && win_edge(qt * kTile + kTile - 1, k0, a.window, a.sinks));
       // pass 1: the row maximum of the raw logits (the scale is positive): keys
       // 0-63, then keys 64-127, which stay in registers
       float s[kHalf];
@@ -548,7 +587,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         m_used = mt;
         rescale = true;
       }
-      const uint64_t nm2 = f2_pack(-m_used, -m_used);
+      // a window may hide a row's whole first tiles: its maximum is then still
+      // -inf, and the exponent offset 0 keeps exp2(-inf + 0) = 0 (not NaN)
+      const float nm = kWin && m_used == -INFINITY ? 0.f : -m_used;
+      const uint64_t nm2 = f2_pack(nm, nm);
       // the previous tile's P V product has read the P buffer, and O_X is stable
       if (j > 0) {
         if (lane == 0) w = bounded_wait(pv_done(x), (j - 1) & 1, abort_flag, err, kErrAttnSoftmax,
@@ -705,6 +747,7 @@ struct BwdArgs {
   float* dv_part;
   bf16* dq;           // dQ kernel: [B, S, H, D]
   uint64_t wait_ns;
+  int window, sinks;  // kWin kernels only
 };
 
 // dK / dV partials of one query head for one 128-key tile, stepping through its
@@ -788,6 +831,7 @@ __device__ __forceinline__ void store_row_tile(uint8_t* tile, int r, const uint3
 // Maps: K / V over [B, Hk, S, D] (128-row boxes), Q over [B, H, S, D] and dO
 // over [B, S, H, D] viewed as [B, H, S, D] (strides S*H*D, D, H*D), both with
 // 64-row boxes.
+template <bool kWin>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tma_q,
                          const __grid_constant__ CUtensorMap tma_k,
@@ -824,7 +868,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int hk = h / (a.H / a.Hk);
   const int k0 = kt * kTile;
   const int step_first = a.causal ? kt * (kTile / kQStep) : 0;
-  const int n = nq64 - step_first;
+  // the last query that sees a key of this tile: through the window, or any when
+  // the tile holds a sink
+  int n = nq64 - step_first;
+  if (kWin && k0 >= a.sinks) {
+    const int last = (k0 + kTile - 1 + a.window - 1) / kQStep;
+    n = (last < nq64 - 1 ? last : nq64 - 1) - step_first + 1;
+  }
   const int64_t s_pad = (int64_t)nq * kTile;
   const uint64_t wait_ns = a.wait_ns;
 
@@ -981,7 +1031,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const float* vnl = reinterpret_cast<const float*>(smem + L::kVec + st * 2 * kQStep * 4) + cb;
       const float* vD = vnl + kQStep;
       const int qs = (step_first + i) * kQStep;
-      const bool edge = (qs + kQStep > a.S) || (a.causal && qs < k0 + kTile);
+      const bool edge = (qs + kQStep > a.S) || (a.causal && qs < k0 + kTile) ||
+                        (kWin && win_edge(qs + kQStep - 1, k0, a.window, a.sinks));
       uint32_t pw[16], dw[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
@@ -1000,7 +1051,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int q = q0 + e + u;
-            if (q >= a.S || (a.causal && q < key)) p[u] = d[u] = 0.f;
+            if (q >= a.S || (a.causal && q < key) ||
+                (kWin && win_hidden(q, key, a.window, a.sinks)))
+              p[u] = d[u] = 0.f;
           }
         }
         pw[e >> 1] = pack_bf16(p[0], p[1]);
@@ -1094,6 +1147,7 @@ struct DqSmem {
 };
 static_assert(DqSmem::kUsed + 128 <= 232448, "attention dQ shared memory exceeds 227 KB");
 
+template <bool kWin>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tma_q,
                        const __grid_constant__ CUtensorMap tma_k,
@@ -1128,7 +1182,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int b = bh / a.H, h = bh % a.H;
   const int hk = h / (a.H / a.Hk);
   const int q0 = qt * kTile;
-  const int n = a.causal ? qt + 1 : nq;
+  KeyTiles kt{0, 0};
+  if (kWin) kt = key_tiles(q0, a.window, a.sinks);
+  const int n = (a.causal ? qt + 1 : nq) - (kWin ? kt.lo - kt.n_sink : 0);
   const uint64_t wait_ns = a.wait_ns;
 
   if (threadIdx.x == 0) {
@@ -1169,21 +1225,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int issued_k = 0, issued_v = 0;
       for (int j = 0; j < n; ++j) {
         const int sk = j % kDqKStages, sv = j % kDqVStages;
+        const int key0 = (kWin ? kt.at(j) : j) * kTile;
         if (!bounded_wait(k_empty(sk), ((j / kDqKStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t kd = sbase + L::kK + sk * kTileBytes;
         mbar_arrive_expect_tx(k_full(sk), kTileBytes);
-        tma_load_4d(kd, &tma_k, k_full(sk), 0, j * kTile, hk, b);
-        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, j * kTile, hk, b);
+        tma_load_4d(kd, &tma_k, k_full(sk), 0, key0, hk, b);
+        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, key0, hk, b);
         ++issued_k;
         if (!bounded_wait(v_empty(sv), ((j / kDqVStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t vd = sbase + L::kV + sv * kTileBytes;
         mbar_arrive_expect_tx(v_full(sv), kTileBytes);
-        tma_load_4d(vd, &tma_v, v_full(sv), 0, j * kTile, hk, b);
-        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, j * kTile, hk, b);
+        tma_load_4d(vd, &tma_v, v_full(sv), 0, key0, hk, b);
+        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, key0, hk, b);
         ++issued_v;
       }
       uint64_t t0 = tc::globaltimer();
@@ -1283,8 +1340,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(st_empty);  // the next tile's S / dP may overwrite them
-      const int k0 = j * kTile + cb;
-      const bool edge = (j * kTile + kTile > a.S) || (a.causal && j == qt);
+      const int jt = kWin ? kt.at(j) : j;
+      const int k0 = jt * kTile + cb;
+      const bool edge = (jt * kTile + kTile > a.S) || (a.causal && jt == qt) ||
+                        (kWin && win_edge(q0 + kTile - 1, jt * kTile, a.window, a.sinks));
       uint32_t dw[kHalf / 2];
 #pragma unroll
       for (int e = 0; e < kHalf; e += 2) {
@@ -1295,8 +1354,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0, d1);
         if (edge) {
           const int key = k0 + e;
-          if (key >= a.S || (a.causal && key > q)) d0 = 0.f;
-          if (key + 1 >= a.S || (a.causal && key + 1 > q)) d1 = 0.f;
+          if (key >= a.S || (a.causal && key > q) ||
+              (kWin && win_hidden(q, key, a.window, a.sinks)))
+            d0 = 0.f;
+          if (key + 1 >= a.S || (a.causal && key + 1 > q) ||
+              (kWin && win_hidden(q, key + 1, a.window, a.sinks)))
+            d1 = 0.f;
         }
         dw[e >> 1] = pack_bf16(d0, d1);
       }
@@ -1447,31 +1510,31 @@ static int set_smem(K kern, int bytes, bool* done) {
   return SOUP_OK;
 }
 
-}  // namespace attn
-}  // namespace soup
+static void fn_error(const char* fn, const char* text) {
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: %s", fn, text);
+  set_last_error(msg);
+}
 
-using namespace soup;
-using namespace soup::attn;
-
-extern "C" {
-
-int soup_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
-                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                       int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
-                       int64_t head_dim, float scale, int causal, void* out, float* lse,
-                       void* stream) {
+// The forward of both forms: window 0 is the plain one. `fn` names the entry
+// point in error messages.
+static int attention_fwd(const char* fn, const void* q, const int64_t* q_strides, const void* k,
+                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
+                         int64_t head_dim, float scale, int causal, int64_t window, int64_t sinks,
+                         void* out, float* lse, void* stream) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || seq <= 0 || heads % kv_heads != 0 ||
       batch * heads > (1 << 20) || seq > (1 << 24) || !out || !lse || !(scale > 0.f)) {
-    set_last_error("soup_attention_fwd: bad arguments");
+    fn_error(fn, "bad arguments");
     return SOUP_ERR_INVALID;
   }
   if (head_dim != kHeadDim) {
-    set_last_error("soup_attention_fwd: head_dim must be 128");
+    fn_error(fn, "head_dim must be 128");
     return SOUP_ERR_UNSUPPORTED;
   }
   if (!bhsd_ok(q, q_strides) || !bhsd_ok(k, k_strides) || !bhsd_ok(v, v_strides) ||
       !aligned16(out)) {
-    set_last_error("soup_attention_fwd: q/k/v need 16-byte aligned bases and strides that are "
+    fn_error(fn, "q/k/v need 16-byte aligned bases and strides that are "
                    "multiples of 8 elements (last dimension contiguous)");
     return SOUP_ERR_UNSUPPORTED;
   }
@@ -1485,51 +1548,45 @@ int soup_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
   if ((rc = make_bhsd_map(&mq, q, q_strides, batch, heads, seq, "q"))) return rc;
   if ((rc = make_bhsd_map(&mk, k, k_strides, batch, kv_heads, seq, "k"))) return rc;
   if ((rc = make_bhsd_map(&mv, v, v_strides, batch, kv_heads, seq, "v"))) return rc;
-  static bool smem_set[64] = {false};
-  if ((rc = set_smem(attn_fwd_kernel, FwdSmem::kBytes, smem_set))) return rc;
+  static bool smem_set[2][64] = {};
+  auto kern = window ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
+  if ((rc = set_smem(kern, FwdSmem::kBytes, smem_set[window ? 1 : 0]))) return rc;
   AttnArgs a{(int)batch, (int)heads, (int)kv_heads, (int)seq, scale * 1.4426950408889634f,
-             causal ? 1 : 0, static_cast<bf16*>(out), lse, 0};
+             causal ? 1 : 0, static_cast<bf16*>(out), lse, 0, (int)(window < seq ? window : seq),
+             (int)(sinks < seq ? sinks : seq)};
   a.wait_ns = wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs;
   const int64_t npair = ((seq + kTile - 1) / kTile + 1) / 2;
-  return cuda_status(launch_pdl(attn_fwd_kernel, dim3((unsigned)(batch * heads * npair)),
+  return cuda_status(launch_pdl(kern, dim3((unsigned)(batch * heads * npair)),
                                 dim3(kFwdThreads), FwdSmem::kBytes, as_stream(stream), mq, mk, mv,
                                 a, err));
 }
 
-size_t soup_attention_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t seq) {
-  if (batch <= 0 || heads <= 0 || seq <= 0) return 0;
-  const size_t s_pad = (size_t)((seq + kTile - 1) / kTile * kTile);
-  const size_t dvec = (size_t)batch * heads * s_pad * 4;
-  const size_t part = (size_t)batch * heads * seq * kHeadDim * 4;
-  return 2 * ((dvec + 255) / 256 * 256) + 2 * ((part + 255) / 256 * 256);
-}
-
-int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
-                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                       const void* out, const void* dout, const float* lse, int64_t batch,
-                       int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim, float scale,
-                       int causal, void* dq, void* dk, void* dv, void* workspace,
-                       size_t workspace_bytes, void* stream) {
+static int attention_bwd(const char* fn, const void* q, const int64_t* q_strides, const void* k,
+                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                         const void* out, const void* dout, const float* lse, int64_t batch,
+                         int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim, float scale,
+                         int causal, int64_t window, int64_t sinks, void* dq, void* dk, void* dv,
+                         void* workspace, size_t workspace_bytes, void* stream) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || seq <= 0 || heads % kv_heads != 0 ||
       batch * heads > (1 << 20) || seq > (1 << 24) || !out || !dout || !lse || !dq || !dk || !dv ||
       !workspace || !(scale > 0.f)) {
-    set_last_error("soup_attention_bwd: bad arguments");
+    fn_error(fn, "bad arguments");
     return SOUP_ERR_INVALID;
   }
   if (head_dim != kHeadDim) {
-    set_last_error("soup_attention_bwd: head_dim must be 128");
+    fn_error(fn, "head_dim must be 128");
     return SOUP_ERR_UNSUPPORTED;
   }
   if (!bhsd_ok(q, q_strides) || !bhsd_ok(k, k_strides) || !bhsd_ok(v, v_strides) ||
       !aligned16(out) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
       !aligned16(lse)) {
-    set_last_error("soup_attention_bwd: operands need 16-byte aligned bases and strides that are "
+    fn_error(fn, "operands need 16-byte aligned bases and strides that are "
                    "multiples of 8 elements");
     return SOUP_ERR_UNSUPPORTED;
   }
   const size_t need = soup_attention_bwd_workspace_bytes(batch, heads, seq);
   if (workspace_bytes < need || !aligned16(workspace)) {
-    set_last_error("soup_attention_bwd: workspace too small or misaligned");
+    fn_error(fn, "workspace too small or misaligned");
     return SOUP_ERR_WORKSPACE;
   }
   int* err = device_err_ptr();
@@ -1554,9 +1611,11 @@ int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
   if ((rc = make_bhsd_map(&mdo, dout, do_strides, batch, heads, seq, "dout"))) return rc;
   if ((rc = make_bhsd_map(&mq64, q, q_strides, batch, heads, seq, "q", kQStep))) return rc;
   if ((rc = make_bhsd_map(&mdo64, dout, do_strides, batch, heads, seq, "dout", kQStep))) return rc;
-  static bool dkdv_set[64] = {false}, dq_set[64] = {false};
-  if ((rc = set_smem(attn_bwd_dkdv_kernel, DkvSmem::kBytes, dkdv_set))) return rc;
-  if ((rc = set_smem(attn_bwd_dq_kernel, DqSmem::kBytes, dq_set))) return rc;
+  static bool dkdv_set[2][64] = {}, dq_set[2][64] = {};
+  auto dkdv = window ? attn_bwd_dkdv_kernel<true> : attn_bwd_dkdv_kernel<false>;
+  auto dqk = window ? attn_bwd_dq_kernel<true> : attn_bwd_dq_kernel<false>;
+  if ((rc = set_smem(dkdv, DkvSmem::kBytes, dkdv_set[window ? 1 : 0]))) return rc;
+  if ((rc = set_smem(dqk, DqSmem::kBytes, dq_set[window ? 1 : 0]))) return rc;
   cudaStream_t st = as_stream(stream);
   const int B = (int)batch, H = (int)heads, Hk = (int)kv_heads, S = (int)seq;
   const int64_t rows = (int64_t)B * S * H;
@@ -1567,14 +1626,15 @@ int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
                                    static_cast<const bf16*>(out), lse, B, H, S, dvec, nl2))))
     return rc;
   BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, causal ? 1 : 0, lse, dvec, nl2,
-            dk_part, dv_part, static_cast<bf16*>(dq), 0};
+            dk_part, dv_part, static_cast<bf16*>(dq), 0, (int)(window < seq ? window : seq),
+            (int)(sinks < seq ? sinks : seq)};
   a.wait_ns = wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs;
   const int nt = (S + kTile - 1) / kTile;
-  if ((rc = cuda_status(launch_pdl(attn_bwd_dkdv_kernel, dim3((unsigned)(B * H * nt)),
+  if ((rc = cuda_status(launch_pdl(dkdv, dim3((unsigned)(B * H * nt)),
                                    dim3(kBwdThreads), DkvSmem::kBytes, st, mq64, mk, mv, mdo64, a,
                                    err))))
     return rc;
-  if ((rc = cuda_status(launch_pdl(attn_bwd_dq_kernel, dim3((unsigned)(B * H * nt)),
+  if ((rc = cuda_status(launch_pdl(dqk, dim3((unsigned)(B * H * nt)),
                                    dim3(kBwdThreads), DqSmem::kBytes, st, mq, mk, mv, mdo, a, err))))
     return rc;
   const int64_t n4 = (int64_t)B * S * Hk * (kHeadDim / 4);
@@ -1583,6 +1643,70 @@ int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
   return cuda_status(launch_pdl(attn_bwd_group_sum_kernel, dim3(blocks), dim3(256), 0, st,
                                 (const float*)dk_part, (const float*)dv_part, B, H, Hk, S,
                                 static_cast<bf16*>(dk), static_cast<bf16*>(dv)));
+}
+
+}  // namespace attn
+}  // namespace soup
+
+using namespace soup;
+using namespace soup::attn;
+
+extern "C" {
+
+int soup_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
+                       int64_t head_dim, float scale, int causal, void* out, float* lse,
+                       void* stream) {
+  return attention_fwd("soup_attention_fwd", q, q_strides, k, k_strides, v, v_strides, batch, heads,
+                       kv_heads, seq, head_dim, scale, causal, 0, 0, out, lse, stream);
+}
+
+size_t soup_attention_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t seq) {
+  if (batch <= 0 || heads <= 0 || seq <= 0) return 0;
+  const size_t s_pad = (size_t)((seq + kTile - 1) / kTile * kTile);
+  const size_t dvec = (size_t)batch * heads * s_pad * 4;
+  const size_t part = (size_t)batch * heads * seq * kHeadDim * 4;
+  return 2 * ((dvec + 255) / 256 * 256) + 2 * ((part + 255) / 256 * 256);
+}
+
+int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       const void* out, const void* dout, const float* lse, int64_t batch,
+                       int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim, float scale,
+                       int causal, void* dq, void* dk, void* dv, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  return attention_bwd("soup_attention_bwd", q, q_strides, k, k_strides, v, v_strides, out, dout, lse,
+                       batch, heads, kv_heads, seq, head_dim, scale, causal, 0, 0, dq, dk, dv,
+                       workspace, workspace_bytes, stream);
+}
+
+int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
+                              int64_t head_dim, float scale, int64_t window, int64_t sinks,
+                              void* out, float* lse, void* stream) {
+  if (window <= 0 || sinks < 0) {
+    set_last_error("soup_attention_window_fwd: window must be positive and sinks not negative");
+    return SOUP_ERR_INVALID;
+  }
+  return attention_fwd("soup_attention_window_fwd", q, q_strides, k, k_strides, v, v_strides, batch,
+                       heads, kv_heads, seq, head_dim, scale, 1, window, sinks, out, lse, stream);
+}
+
+int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                              const void* out, const void* dout, const float* lse, int64_t batch,
+                              int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim,
+                              float scale, int64_t window, int64_t sinks, void* dq, void* dk,
+                              void* dv, void* workspace, size_t workspace_bytes, void* stream) {
+  if (window <= 0 || sinks < 0) {
+    set_last_error("soup_attention_window_bwd: window must be positive and sinks not negative");
+    return SOUP_ERR_INVALID;
+  }
+  return attention_bwd("soup_attention_window_bwd", q, q_strides, k, k_strides, v, v_strides, out,
+                       dout, lse, batch, heads, kv_heads, seq, head_dim, scale, 1, window, sinks,
+                       dq, dk, dv, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -492,7 +492,8 @@ struct EpiCE {
     int64_t vocab_offset;  // first vocabulary row of this weight shard (0 unsharded)
     int M, N;
     int tma;  // logits stored through tma_c
-    const float* shift;  // [M] or nullptr (store the logits themselves)
+    const float* shift;  // [M] or nullptr (store the logits themselves); with shift and
+                         // no logits buffer: the shifted sums alone
     int* flag;           // set to 1 when a row's maximum exceeds shift + kShiftGap
     int onehot;          // shift = lse: store E - 1 at the target column (= p - 1)
     int has_ignore;      // rows whose target is ignore_index store E = 0 (statistics kept)
@@ -600,7 +601,7 @@ struct EpiCE {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = 0.f;
       }
-      store(p, tmc, stage, lane, nstore, v, col0, row0);
+      if (p.logits) store(p, tmc, stage, lane, nstore, v, col0, row0);
     }
     if (row_ok) {
       float s0, s1, w0, w1;
@@ -624,7 +625,7 @@ struct EpiCE {
                                               int quarter, int lane, uint32_t taddr, uint8_t* stage,
                                               int group, int ngroups) {
     const int row0 = row_base + quarter * 32;
-    if (p.logits && p.shift) {
+    if (p.shift) {
       tile_shifted(p, tmc, row0, nt, lane, taddr, stage, group, ngroups);
       return;
     }
@@ -863,7 +864,7 @@ static int sk_min_saved() { return g_sk_min_saved.load(std::memory_order_relaxed
 static int plan_stream_k(Sched& sched, int max_cl, int dev) {
   const int tiles = sched.m_tiles * sched.n_tiles;
   const int whole = tiles < max_cl ? tiles : max_cl;
-  if (sched.splits != 1 || sched.withhold >= 0 || tiles % max_cl == 0) return whole;
+  if (sched.splits != 1 || sched.withhold >= 0 || sched.no_sk || tiles % max_cl == 0) return whole;
   SkWorkspace ws;
   {
     std::lock_guard<std::mutex> lock(cache_mutex());
@@ -1230,6 +1231,109 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ ws, int splits, i
   }
 }
 
+// --------------------------------------------- per-token log-probabilities --
+// After the logits GEMM, per row: merge the tile records, then
+//   logp = z_t - lse, entropy = lse - sum z p
+// and, when E is kept for a backward, rscale = exp(c - lse) and
+// E[t] = (p_t - 1) exp(lse - c), so that -g * rscale * E is the row of
+// d(sum g logp) / d logits = g (onehot - softmax). Rows whose target is
+// ignore_index give 0; a target outside the vocabulary or a row without a
+// finite logit gives NaN. The merge is that of ce_stats_kernel: 8 rows per
+// block of 512 threads, 64 partial states a row joined in a fixed order.
+__global__ void __launch_bounds__(512, 2) logps_stats_kernel(
+    const float4* __restrict__ partials, int n_parts, const float* __restrict__ zt,
+    const int64_t* __restrict__ targets, int rows, int vocab, int64_t ignore_index,
+    float* __restrict__ logps, float* __restrict__ entropies, bf16* __restrict__ E, int64_t ld_e,
+    float* __restrict__ shift, float* __restrict__ rscale, const int* __restrict__ flag) {
+  constexpr int kGroups = 512 / kStatRows;
+  __shared__ SoftmaxState part[kGroups][kStatRows + 1];
+  __shared__ SoftmaxState part2[8][kStatRows + 1];
+  const int r0 = blockIdx.x * kStatRows;
+  const int lr = threadIdx.x % kStatRows, g = threadIdx.x / kStatRows;
+  {
+    const int row = r0 + lr;
+    SoftmaxState st = sm_init();
+    if (row < rows) {
+      for (int j0 = g; j0 < n_parts; j0 += kStatBatch * kGroups) {
+        float4 p[kStatBatch];
+#pragma unroll
+        for (int i = 0; i < kStatBatch; ++i) {
+          const int j = j0 + i * kGroups;
+          p[i] = j < n_parts ? partials[(int64_t)j * rows + row]
+                             : make_float4(-INFINITY, 0.f, 0.f, __int_as_float(0x7fffffff));
+        }
+#pragma unroll
+        for (int i = 0; i < kStatBatch; ++i)
+          st = sm_merge(st, SoftmaxState{p[i].x, p[i].y, p[i].z, __float_as_int(p[i].w)});
+      }
+    }
+    part[g][lr] = st;
+  }
+  __syncthreads();
+  if (threadIdx.x < 8 * kStatRows) {
+    const int sub = threadIdx.x / kStatRows;
+    SoftmaxState st = part[sub * (kGroups / 8)][lr];
+    for (int i = 1; i < kGroups / 8; ++i) st = sm_merge(st, part[sub * (kGroups / 8) + i][lr]);
+    part2[sub][lr] = st;
+  }
+  __syncthreads();
+  const int row = r0 + threadIdx.x;
+  if (threadIdx.x >= kStatRows || row >= rows) return;
+  SoftmaxState r = part2[0][threadIdx.x];
+  for (int i = 1; i < 8; ++i) r = sm_merge(r, part2[i][threadIdx.x]);
+  const int64_t t = targets[row];
+  const bool ignored = t == ignore_index;
+  const bool in_range = t >= 0 && t < vocab;
+  const float lse = r.m == -INFINITY ? NAN : r.m + logf(r.s);
+  const float z_t = in_range ? zt[row] : NAN;
+  logps[row] = ignored ? 0.f : z_t - lse;
+  if (entropies) entropies[row] = ignored ? 0.f : fmaxf(0.f, lse - r.w / r.s);
+  if (!E) return;
+  float sc = 0.f;
+  const bool flagged = *flag != 0;
+  const float c = shift[row];
+  if (!ignored) {
+    if (flagged) {
+      sc = 1.f;
+    } else {
+      sc = fast_exp2((c - lse) * kLog2e);
+      if (in_range) {
+        const float q = fast_exp2((z_t - lse) * kLog2e) - 1.f;
+        E[(int64_t)row * ld_e + t] = __float2bfloat16_rn(q * fast_exp2((lse - c) * kLog2e));
+      }
+    }
+  }
+  if (flagged) shift[row] = lse;  // every row: the fallback GEMM reads it
+  rscale[row] = sc;
+}
+
+// Backward row factors rs[row] = -dlogps[row] * rscale[row] (0 for ignored rows,
+// whatever their dlogps hold) and, with hs set, hs[row] = rs[row] * hidden[row].
+// One warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) logps_grad_rows_kernel(
+    const float* __restrict__ dlogps, const float* __restrict__ rscale,
+    const int64_t* __restrict__ targets, int64_t ignore_index, int rows,
+    const T* __restrict__ hidden, int64_t h_ld, int dim, float* __restrict__ rs,
+    bf16* __restrict__ hs) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const float sc = targets[row] == ignore_index ? 0.f : -dlogps[row] * rscale[row];
+  if (lane == 0) rs[row] = sc;
+  if (!hs) return;
+  const T* hrow = hidden + (int64_t)row * h_ld;
+  bf16* orow = hs + (int64_t)row * dim;
+  for (int k = lane * 8; k < dim; k += 256) {
+    const Vec16<T> a = ld16(hrow + k);
+    Vec16<bf16> o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)  // a row of weight 0 may hold anything
+      o.v[e] = __float2bfloat16_rn(sc == 0.f ? 0.f : sc * Cvt<T>::to_f(a.v[e]));
+    st16(orow + k, o);
+  }
+}
+
 // ------------------------------------------------- vocab-parallel kernels ---
 // Per row (one warp each): merge this shard's tile states into one record
 // {max, sum exp, sum z*exp, global argmax (int bits), target logit or 0}.
@@ -1421,7 +1525,7 @@ static CEWorkspace ce_layout(int64_t rows, int64_t vocab, int64_t dim) {
 // otherwise the GEMM epilogue writes dH directly. dh_dtype: SOUP_BF16 or SOUP_F32.
 static int dx_gemm(const bf16* L, int64_t ld_logits, const void* weight, int64_t w_ld, int M, int V,
                    int D, int splits, float* splitk, void* dh, int dh_dtype, cudaStream_t stream,
-                   int gemm_stage = -1, const float* row_scale = nullptr) {
+                   int gemm_stage = -1, const float* row_scale = nullptr, int no_sk = 0) {
   CUtensorMap ma, mb;
   int rc;
   if ((rc = make_operand_map(&ma, L, false, M, V, ld_logits, BM))) return rc;
@@ -1431,6 +1535,7 @@ static int dx_gemm(const bf16* L, int64_t ld_logits, const void* weight, int64_t
   // order) leaves the end of dL / E and of W in L2; the last split run is then
   // the vocab's start, where the dW GEMM begins
   sc.rev_split = 1;
+  sc.no_sk = no_sk;
   const bool bf = dh_dtype == SOUP_BF16;
   if (splits == 1) {
     const int vec = (aligned16(dh) && (D * (bf ? 2 : 4)) % 16 == 0) ? 1 : 0;
@@ -1461,12 +1566,13 @@ static int dx_gemm(const bf16* L, int64_t ld_logits, const void* weight, int64_t
 // already scaled by the row factors) read MN-major, B = hidden MN-major.
 static int dweight_gemm(const bf16* L, int64_t ld_logits, const void* hidden, int64_t h_ld, int M,
                         int V, int D, const float* scale, void* dweight, int dw_dtype,
-                        int accumulate, cudaStream_t stream) {
+                        int accumulate, cudaStream_t stream, int no_sk = 0) {
   CUtensorMap ma, mb;
   int rc;
   if ((rc = make_operand_map(&ma, L, true, V, M, ld_logits, 64))) return rc;
   if ((rc = make_operand_map(&mb, hidden, true, D, M, h_ld, 64))) return rc;
   Sched sc{m_tiles(V), (D + kBN - 1) / kBN, 1, (M + BK - 1) / BK, 1};
+  sc.no_sk = no_sk;
   const int es = dw_dtype == SOUP_BF16 ? 2 : 4;
   const int vec = (aligned16(dweight) && (D * es) % 16 == 0) ? 1 : 0;
   CUtensorMap mc = ma;
@@ -1475,6 +1581,38 @@ static int dweight_gemm(const bf16* L, int64_t ld_logits, const void* hidden, in
   EpiStore<kBN>::Params ep{dweight, D, 0, scale, 1.f, dw_dtype == SOUP_BF16 ? 1 : 0,
                            accumulate ? 1 : 0, vec, V, D, nullptr, tma};
   return launch_gemm<true, true, EpiStore<kBN>>(ma, mb, mc, sc, ep, stream);
+}
+
+// Buffers of the per-token log-probabilities: `state` lives from the forward to
+// the backward (the exponentials and their row factors), the workspaces only
+// for one call each.
+struct LogpsLayout {
+  CEWorkspace ce;
+  size_t st_rscale, st_total;                           // state: E at 0
+  size_t fw_partials, fw_zt, fw_shift, fw_flag, fw_total;  // forward workspace
+  size_t bw_splitk, bw_rs, bw_hs, bw_total;             // backward workspace
+};
+static LogpsLayout logps_layout(int64_t rows, int64_t vocab, int64_t dim) {
+  LogpsLayout l;
+  l.ce = ce_layout(rows, vocab, dim);
+  size_t off = align_up((size_t)rows * l.ce.ld_logits * 2, 256);
+  l.st_rscale = off;
+  l.st_total = align_up(off + (size_t)rows * 4, 256);
+  l.fw_partials = 0;
+  off = align_up((size_t)l.ce.n_parts * rows * 16, 256);
+  l.fw_zt = off;
+  off = align_up(off + (size_t)rows * 4, 256);
+  l.fw_shift = off;
+  off = align_up(off + (size_t)rows * 4, 256);
+  l.fw_flag = off;
+  l.fw_total = align_up(off + 4, 256);
+  l.bw_splitk = 0;
+  off = align_up((size_t)l.ce.splits * rows * dim * 4, 256);
+  l.bw_rs = off;
+  off = align_up(off + (size_t)rows * 4, 256);
+  l.bw_hs = off;
+  l.bw_total = align_up(off + (size_t)rows * dim * 2, 256);
+  return l;
 }
 
 // Launch helpers shared by the entry points below (operand type T of the
@@ -1834,6 +1972,138 @@ int soup_ce_vp_backward(void* workspace, size_t workspace_bytes, const void* hid
   if (dweight_shard)
     return dweight_gemm(L, w.ld_logits, hs, D, M, V, D, nullptr, dweight_shard, dw_dtype,
                         accumulate_dw, stream);
+  return SOUP_OK;
+}
+
+// ------------------------------------------------ per-token log-probabilities
+static bool logps_sizes_ok(int64_t rows, int64_t vocab, int64_t dim) {
+  return rows > 0 && vocab > 0 && dim > 0 && rows <= (1 << 30) && vocab <= (1 << 30) &&
+         dim <= (1 << 24);
+}
+
+size_t soup_head_logps_state_bytes(int64_t rows, int64_t vocab, int64_t dim) {
+  return logps_sizes_ok(rows, vocab, dim) ? logps_layout(rows, vocab, dim).st_total : 0;
+}
+
+size_t soup_head_logps_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int backward) {
+  if (!logps_sizes_ok(rows, vocab, dim)) return 0;
+  const LogpsLayout l = logps_layout(rows, vocab, dim);
+  return backward ? l.bw_total : l.fw_total;
+}
+
+int soup_head_logps_fwd(const void* hidden, int64_t h_ld, const void* weight, int64_t w_ld,
+                        int in_dtype, const int64_t* targets, int64_t rows, int64_t vocab,
+                        int64_t dim, int64_t ignore_index, float* logps, float* entropies,
+                        void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
+                        void* stream_) {
+  if (!hidden || !weight || !targets || !logps || !workspace || !logps_sizes_ok(rows, vocab, dim) ||
+      h_ld < dim || w_ld < dim) {
+    set_last_error("soup_head_logps_fwd: bad arguments");
+    return SOUP_ERR_INVALID;
+  }
+  int rc = check_in_dtype("soup_head_logps_fwd", in_dtype, nullptr, false);
+  if (rc) return rc;
+  const bool f16 = in_dtype == SOUP_F16;
+  if (!tma_ok(hidden, h_ld) || !tma_ok(weight, w_ld) || (dim % 8) != 0) {
+    set_last_error("soup_head_logps_fwd: hidden/weight need 16-byte aligned rows and dim % 8 == 0");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  const LogpsLayout l = logps_layout(rows, vocab, dim);
+  if (workspace_bytes < l.fw_total || !aligned16(workspace) ||
+      (state && (state_bytes < l.st_total || !aligned16(state)))) {
+    set_last_error("soup_head_logps_fwd: state or workspace too small or misaligned");
+    return SOUP_ERR_WORKSPACE;
+  }
+  cudaStream_t stream = as_stream(stream_);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float4* partials = reinterpret_cast<float4*>(ws + l.fw_partials);
+  float* zt = reinterpret_cast<float*>(ws + l.fw_zt);
+  float* shift = reinterpret_cast<float*>(ws + l.fw_shift);
+  int* flag = reinterpret_cast<int*>(ws + l.fw_flag);
+  uint8_t* st = static_cast<uint8_t*>(state);
+  bf16* E = reinterpret_cast<bf16*>(st);
+  float* rscale = state ? reinterpret_cast<float*>(st + l.st_rscale) : nullptr;
+  const int M = static_cast<int>(rows), V = static_cast<int>(vocab), D = static_cast<int>(dim);
+  // the same sums with and without the stored exponentials: a policy's
+  // log-probabilities are bit-identical in sampling and in training
+  rc = f16 ? launch_shift<__half>(hidden, h_ld, weight, w_ld, targets, M, V, D, 0, shift, flag, stream)
+           : launch_shift<bf16>(hidden, h_ld, weight, w_ld, targets, M, V, D, 0, shift, flag, stream);
+  if (rc) return rc;
+  CUtensorMap ma, mb, mc;
+  Sched sc{m_tiles(M), l.ce.n_vtiles, 1, (D + BK - 1) / BK, 0};
+  sc.ab_f16 = f16 ? 1 : 0;
+  sc.no_sk = 1;
+  if ((rc = make_operand_map(&ma, hidden, false, rows, dim, h_ld, BM, f16))) return rc;
+  if ((rc = make_operand_map(&mb, weight, false, vocab, dim, w_ld, b_box_rows(), f16))) return rc;
+  mc = ma;
+  EpiCE<kBN>::Params ep{targets, partials, zt, E, l.ce.ld_logits, 0, M, V, 0, shift, flag, 0, 1,
+                        ignore_index};
+  ep.tma = (state && make_store_map(&mc, E, V, M, l.ce.ld_logits) == SOUP_OK) ? 1 : 0;
+  if ((rc = launch_gemm<false, false, EpiCE<kBN>>(ma, mb, mc, sc, ep, stream))) return rc;
+  logps_stats_kernel<<<(M + kStatRows - 1) / kStatRows, 512, 0, stream>>>(
+      partials, l.ce.n_parts, zt, targets, M, V, ignore_index, logps, entropies, E, l.ce.ld_logits,
+      shift, rscale, flag);
+  if ((rc = launch_status()) || !state) return rc;
+  // overflow fallback as in soup_ce_linear: the same GEMM with shift = lse
+  sc.gate = flag;
+  ep.onehot = 1;
+  return launch_gemm<false, false, EpiCE<kBN>>(ma, mb, mc, sc, ep, stream);
+}
+
+int soup_head_logps_bwd(const void* state, size_t state_bytes, const void* hidden, int64_t h_ld,
+                        int in_dtype, const void* weight_bwd, int64_t wb_ld, const int64_t* targets,
+                        const float* dlogps, int64_t rows, int64_t vocab, int64_t dim,
+                        int64_t ignore_index, void* dhidden, int dh_dtype, void* dweight,
+                        int dw_dtype, int accumulate_dw, void* workspace, size_t workspace_bytes,
+                        void* stream_) {
+  if (!state || !targets || !dlogps || !workspace || !logps_sizes_ok(rows, vocab, dim) ||
+      (!dhidden && !dweight) || (dhidden && (!weight_bwd || wb_ld < dim)) ||
+      (dweight && (!hidden || h_ld < dim))) {
+    set_last_error("soup_head_logps_bwd: bad arguments");
+    return SOUP_ERR_INVALID;
+  }
+  int rc = check_in_dtype("soup_head_logps_bwd", in_dtype, nullptr, false);
+  if (rc) return rc;
+  if ((dweight && dw_dtype != SOUP_F32 && dw_dtype != SOUP_BF16) ||
+      (dhidden && dh_dtype != SOUP_F32 && dh_dtype != SOUP_BF16)) {
+    set_last_error("soup_head_logps_bwd: gradient dtypes must be F32 or BF16");
+    return SOUP_ERR_INVALID;
+  }
+  if ((dweight && !tma_ok(hidden, h_ld)) || (dhidden && !tma_ok(weight_bwd, wb_ld)) ||
+      (dim % 8) != 0) {
+    set_last_error("soup_head_logps_bwd: hidden/weight need 16-byte aligned rows and dim % 8 == 0");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  const LogpsLayout l = logps_layout(rows, vocab, dim);
+  if (state_bytes < l.st_total || !aligned16(state) || workspace_bytes < l.bw_total ||
+      !aligned16(workspace)) {
+    set_last_error("soup_head_logps_bwd: state or workspace too small or misaligned");
+    return SOUP_ERR_WORKSPACE;
+  }
+  cudaStream_t stream = as_stream(stream_);
+  const uint8_t* st = static_cast<const uint8_t*>(state);
+  const bf16* E = reinterpret_cast<const bf16*>(st);
+  const float* rscale = reinterpret_cast<const float*>(st + l.st_rscale);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* splitk = reinterpret_cast<float*>(ws + l.bw_splitk);
+  float* rs = reinterpret_cast<float*>(ws + l.bw_rs);
+  bf16* hs = reinterpret_cast<bf16*>(ws + l.bw_hs);
+  const int M = static_cast<int>(rows), V = static_cast<int>(vocab), D = static_cast<int>(dim);
+  if (in_dtype == SOUP_F16)
+    logps_grad_rows_kernel<__half><<<(M + 7) / 8, 256, 0, stream>>>(
+        dlogps, rscale, targets, ignore_index, M, static_cast<const __half*>(hidden), h_ld, D, rs,
+        dweight ? hs : nullptr);
+  else
+    logps_grad_rows_kernel<bf16><<<(M + 7) / 8, 256, 0, stream>>>(
+        dlogps, rscale, targets, ignore_index, M, static_cast<const bf16*>(hidden), h_ld, D, rs,
+        dweight ? hs : nullptr);
+  if ((rc = launch_status())) return rc;
+  if (dhidden && (rc = dx_gemm(E, l.ce.ld_logits, weight_bwd, wb_ld, M, V, D, l.ce.splits, splitk,
+                               dhidden, dh_dtype, stream, -1, rs, 1)))
+    return rc;
+  if (dweight)
+    return dweight_gemm(E, l.ce.ld_logits, hs, D, M, V, D, nullptr, dweight, dw_dtype, accumulate_dw,
+                        stream, 1);
   return SOUP_OK;
 }
 

@@ -277,6 +277,9 @@ struct Sched {
   int withhold = -1;
   // 1: A and B are fp16 (kind::f16 with the f16 operand format) instead of bf16
   int ab_f16 = 0;
+  // 1: no stream-K tail, so the launch shares no scratch with others and may run
+  // beside GEMMs of other streams
+  int no_sk = 0;
   __device__ __forceinline__ uint64_t limit() const { return wait_ns ? wait_ns : kWaitNs; }
   // the instruction descriptor with the operand format of this launch
   __device__ __forceinline__ uint32_t idesc(uint32_t bf16_desc) const {

@@ -1,7 +1,10 @@
 """sm_100a fused ops behind the reference's kernel-package names.
 
-Mirrors the export list of the reference's ``solution/kernels/__init__.py:3-51``.
+Mirrors the export list of the reference's ``solution/kernels/__init__.py:3-51``,
+and adds the operators of preference and policy tuning (no counterpart there).
 """
+
+from .attention import window_attention
 
 from .chunked_ce import (
     _chunked_cross_entropy_fused_kernel,
@@ -32,7 +35,11 @@ from .swiglu import (
     FastSwiGLUFunction,
     fast_swiglu,
     patch_qwen2_mlp,
+    quantize_8bit,
+    swiglu_8bit,
 )
+from .token_logps import head_token_logps
+from .tuning_loss import policy_loss, preference_loss
 
 __all__ = [
     "_chunked_cross_entropy_fused_kernel",
@@ -57,4 +64,10 @@ __all__ = [
     "FastSwiGLUFunction",
     "fast_swiglu",
     "patch_qwen2_mlp",
+    "head_token_logps",
+    "preference_loss",
+    "policy_loss",
+    "window_attention",
+    "swiglu_8bit",
+    "quantize_8bit",
 ]

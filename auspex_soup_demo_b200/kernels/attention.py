@@ -10,16 +10,22 @@ the QLoRA step:
   [B, S, H, D] projections are read in place) -> out [B, S, H, 128] bf16 (the
   layout the o_proj consumes, no transpose copy) and the row log-sum-exp for
   the backward;
+* :func:`window_attention` - the same with a sliding window and a few first
+  tokens that stay visible (sinks), forward and backward;
 * :func:`soup_attention` - an attention function with transformers'
   ``AttentionInterface`` signature, registered under the name ``"soup_b200"``
   by :func:`register`. Calls the kernels have no form for (an attention mask,
   dropout, a head dim other than 128, non-bf16 or CPU tensors) go to
-  transformers' SDPA function unchanged.
+  transformers' SDPA function unchanged. Layers with a ``sliding_window`` (and,
+  optionally, ``config.attention_sink_tokens``) take :func:`window_attention`.
 """
 
 from __future__ import annotations
 
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -31,16 +37,16 @@ def _strides(t: torch.Tensor):
     return _lib.i64_array([t.stride(0), t.stride(1), t.stride(2)])
 
 
-def _check(q, k, v):
+def _check(q, k, v, any_stride: bool = False):
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("attention: q, k, v must be [B, heads, S, D]")
     B, H, S, D = q.shape
     if k.shape != v.shape or k.shape[0] != B or k.shape[2] != S or k.shape[3] != D:
         raise ValueError(f"attention: shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
-    if H % k.shape[1]:
+    if k.shape[1] == 0 or H % k.shape[1]:
         raise ValueError("attention: query heads must be a multiple of the KV heads")
     for t in (q, k, v):
-        if t.dtype != torch.bfloat16 or not t.is_cuda or t.stride(-1) != 1:
+        if t.dtype != torch.bfloat16 or not t.is_cuda or (t.stride(-1) != 1 and not any_stride):
             raise ValueError("attention: q, k, v must be bf16 CUDA tensors with a contiguous last dim")
     return B, H, k.shape[1], S, D
 
@@ -108,6 +114,86 @@ def flash_attention(q, k, v, scale: float, causal: bool = True):
     return FlashAttentionFunction.apply(q, k, v, scale, causal)
 
 
+def _kernel_layout(t: torch.Tensor):
+    """(t, element strides) in a form the tensor maps can read: 16-byte aligned,
+    positive strides that are multiples of 8. Dimensions of size 1 take any
+    stride; anything else is copied."""
+    def strides(x):
+        full = (x.shape[1] * x.shape[2] * x.shape[3], x.shape[2] * x.shape[3], x.shape[3])
+        return [full[i] if x.shape[i] == 1 else x.stride(i) for i in range(3)]
+
+    st = strides(t)
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(v <= 0 or v % 8 for v in st):
+        t = t.clone(memory_format=torch.contiguous_format)
+        st = strides(t)
+    return t, _lib.i64_array(st)
+
+
+class WindowAttentionFunction(torch.autograd.Function):
+    """out [B, S, H, D] of :func:`window_attention`; backward recomputes P from the
+    saved log-sum-exp."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale: float, window: int, sinks: int):
+        B, H, S, D = q.shape
+        Hk = k.shape[1]
+        (q, qs), (k, ks), (v, vs) = (_kernel_layout(t.detach()) for t in (q, k, v))
+        out = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device)
+        lse = torch.empty(B, H, _s_pad(S), dtype=torch.float32, device=q.device)
+        _lib.call("soup_attention_window_fwd", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
+                  vs, B, H, Hk, S, D, scale, window, sinks, out.data_ptr(), lse.data_ptr(),
+                  _lib.stream_of(q))
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.args = (scale, window, sinks)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        scale, window, sinks = ctx.args
+        B, H, S, D = q.shape
+        Hk = k.shape[1]
+        dout = dout.to(torch.bfloat16).contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        dq = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device)
+        dk = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
+        dv = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
+        nbytes = _lib.lib().soup_attention_bwd_workspace_bytes(B, H, S)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        (_, qs), (_, ks), (_, vs) = (_kernel_layout(t) for t in (q, k, v))
+        _lib.call("soup_attention_window_bwd", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
+                  vs, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), B, H, Hk, S, D, scale, window,
+                  sinks, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes,
+                  _lib.stream_of(q))
+        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None, None
+
+
+def window_attention(q, k, v, scale: float, window: int, sinks: int = 0) -> torch.Tensor:
+    """out [B, S, H, D] of causal grouped-query attention in which query i sees
+    key j iff j <= i and (i - j < window or j < sinks).
+
+    q [B, H, S, 128], k and v [B, Hk, S, 128] bf16 CUDA tensors, H a multiple of
+    Hk, any strides (layouts the kernels cannot read in place are copied);
+    window >= 1, sinks >= 0, either may exceed S. Time and memory traffic grow
+    with S (window + sinks), not with S^2. Differentiable in q, k and v.
+    """
+    B, H, Hk, S, D = _check(q, k, v, any_stride=True)
+    if D != HEAD_DIM:
+        raise ValueError(f"window_attention: head dim must be {HEAD_DIM}, got {D}")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("window_attention: q, k and v must be on one device")
+    if min(B, H, Hk, S) == 0:
+        raise ValueError(f"window_attention: empty input, q {tuple(q.shape)} k {tuple(k.shape)}")
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window_attention: window must be >= 1 and sinks >= 0, got {window}, {sinks}")
+    if not (math.isfinite(scale) and scale > 0):
+        raise ValueError("window_attention: scale must be positive and finite")
+    return WindowAttentionFunction.apply(q, k, v, float(scale), min(window, S), min(sinks, S))
+
+
 def _supported(module, query, key, value, attention_mask, dropout) -> bool:
     return (attention_mask is None and not dropout and query.is_cuda
             and query.dtype == key.dtype == value.dtype == torch.bfloat16
@@ -121,9 +207,25 @@ def soup_attention(module, query, key, value, attention_mask, dropout: float = 0
                    scaling=None, is_causal=None, **kwargs):
     """transformers ``AttentionInterface`` function: (attn_output [B, S, H, D], None).
 
-    Causal when the module is (and the query is longer than one token), as
+    A ``sliding_window`` (transformers passes the layer's) limits each query to its
+    last ``sliding_window`` keys, plus the first ``attention_sink_tokens`` of the
+    sequence when the module's config sets that. Causal when the module is (and the query is longer than one token), as
     transformers' SDPA path decides (``integrations/sdpa_attention.py``). Calls
     outside the kernels' form go to transformers' SDPA function."""
+    window = kwargs.get("sliding_window")
+    if window is not None and query.shape[2] == key.shape[2]:
+        # transformers builds no mask for an attention function of its own registry
+        # entry, so the window is this function's to apply
+        causal = is_causal if is_causal is not None else getattr(module, "is_causal", True)
+        sinks = int(getattr(getattr(module, "config", None), "attention_sink_tokens", 0) or 0)
+        if causal and attention_mask is None and window < query.shape[2]:
+            scale = scaling if scaling is not None else query.shape[-1] ** -0.5
+            if (not dropout and query.is_cuda and query.shape[-1] == HEAD_DIM
+                    and query.dtype == key.dtype == value.dtype == torch.bfloat16):
+                return window_attention(query, key, value, float(scale), window, sinks), None
+            i = torch.arange(query.shape[2], device=query.device)
+            dist = i[:, None] - i[None, :]
+            attention_mask = ((dist >= 0) & ((dist < window) | (i[None, :] < sinks)))[None, None]
     if not _supported(module, query, key, value, attention_mask, dropout):
         from transformers.integrations.sdpa_attention import sdpa_attention_forward
 

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 import torch.utils.checkpoint
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ._shim import LaunchShim
@@ -78,6 +79,100 @@ def fast_swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return FastSwiGLUFunction.apply(gate, up)
 
 
+# ---- SwiGLU with gate and up kept in 8 bits --------------------------------------
+Q8_BLOCK = 64  # consecutive columns that share one fp32 scale
+
+
+def _rows_8bit(t: torch.Tensor, n: int) -> torch.Tensor:
+    t2 = _rows(t, n)
+    return t2 if t2.shape[0] < 2 or t2.stride(0) >= n else t2.contiguous()
+
+
+def _ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def quantize_8bit(x2: torch.Tensor):
+    """(codes int8 [rows, n], scales fp32 [rows, ceil(n / 64)]) of a CUDA tensor
+    [rows, n]: per 64 consecutive columns scale = absmax / 127 and
+    code = round(x * (127 / absmax)); the kept value is code * scale."""
+    x2 = _rows_8bit(x2.detach(), x2.shape[-1])
+    rows, n = x2.shape
+    codes = torch.empty(rows, n, dtype=torch.int8, device=x2.device)
+    scales = torch.empty(rows, -(-n // Q8_BLOCK), dtype=torch.float32, device=x2.device)
+    _lib.call("soup_q8_quantize", x2.device, x2.data_ptr(), _ld(x2), codes.data_ptr(), n,
+              scales.data_ptr(), scales.shape[1], rows, n, _lib.dtype_code(x2.dtype), _lib.stream_of(x2))
+    return codes, scales
+
+
+def swiglu_8bit_backward(dy2, g_codes, u_codes, g_scales, u_scales, dg, du, h=None) -> None:
+    """dg, du (and, when given, h = silu(g) u) at the kept values; every tensor
+    [rows, n] (scales [rows, n / 64 rounded up]), the codes of gate and up with
+    one row stride, their scales with one row stride."""
+    rows, n = dy2.shape
+    _lib.call("soup_swiglu_q8_bwd", dy2.device, dy2.data_ptr(), _ld(dy2), g_codes.data_ptr(),
+              u_codes.data_ptr(), _ld(g_codes), g_scales.data_ptr(), u_scales.data_ptr(), _ld(g_scales),
+              dg.data_ptr(), _ld(dg), du.data_ptr(), _ld(du), _lib.ptr(h), 0 if h is None else _ld(h),
+              rows, n, _lib.dtype_code(dy2.dtype), _lib.stream_of(dy2))
+
+
+class SwiGLU8BitFunction(torch.autograd.Function):
+    """silu(gate) * up whose backward reads gate and up from 8-bit codes."""
+
+    @staticmethod
+    def forward(ctx, gate: torch.Tensor, up: torch.Tensor):
+        n = gate.shape[-1]
+        g2, u2 = _rows_8bit(gate.detach(), n), _rows_8bit(up.detach(), n)
+        rows = g2.shape[0]
+        out = torch.empty(rows, n, dtype=gate.dtype, device=gate.device)
+        codes = torch.empty(2, rows, n, dtype=torch.int8, device=gate.device)
+        scales = torch.empty(2, rows, -(-n // Q8_BLOCK), dtype=torch.float32, device=gate.device)
+        _lib.call("soup_swiglu_q8_fwd", gate.device, g2.data_ptr(), _ld(g2), u2.data_ptr(), _ld(u2),
+                  out.data_ptr(), n, codes.data_ptr(), codes[1].data_ptr(), n, scales.data_ptr(),
+                  scales[1].data_ptr(), scales.shape[2], rows, n, _lib.dtype_code(gate.dtype),
+                  _lib.stream_of(g2))
+        ctx.save_for_backward(codes, scales)
+        ctx.dtype = gate.dtype
+        return out.view(gate.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy: torch.Tensor):
+        codes, scales = ctx.saved_tensors
+        _, rows, n = codes.shape
+        dy2 = _rows_8bit(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype), n)
+        dg = torch.empty(rows, n, dtype=ctx.dtype, device=dy.device)
+        du = torch.empty_like(dg)
+        swiglu_8bit_backward(dy2, codes[0], codes[1], scales[0], scales[1], dg, du)
+        return dg.view(dy.shape), du.view(dy.shape)
+
+
+def swiglu_8bit(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
+    """silu(gate) * up, keeping gate and up for the backward as 8-bit codes (1.0625
+    bytes an element instead of the dtype's 2 or 4; see :func:`quantize_8bit`).
+
+    The output is that of the exact gate and up; the gradients are SwiGLU's at the
+    kept values, each within absmax / 254 of its block of 64 columns. An infinity
+    or NaN makes its whole block's gradient NaN. Same shapes and dtypes (fp32, fp16,
+    bf16) on one CUDA device.
+    """
+    if gate.shape != up.shape or gate.dim() == 0 or gate.shape[-1] == 0:
+        raise ValueError(f"swiglu_8bit: gate {tuple(gate.shape)} and up {tuple(up.shape)}")
+    if gate.dtype != up.dtype:
+        raise TypeError(f"swiglu_8bit: gate and up dtypes differ: {gate.dtype} vs {up.dtype}")
+    _lib.dtype_code(gate.dtype)
+    if not gate.is_cuda or up.device != gate.device:
+        raise ValueError("swiglu_8bit: gate and up must be on one CUDA device")
+    if gate.numel() == 0:
+        return gate * up
+    return SwiGLU8BitFunction.apply(gate, up)
+
+
+#: Keep the MLP's gate and up in 8 bits from forward to backward instead of
+#: recomputing them (takes precedence over RECOMPUTE in training): 2.1 bytes per
+#: token and intermediate column, no second gate/up GEMM.
+CHECKPOINT_8BIT = False
+
 #: Recompute gate/up + SwiGLU in backward (the reference's selective recompute,
 #: ``swiglu.py:197-214``). False keeps the activations instead: more memory
 #: (2 x tokens x intermediate bf16 per layer), no second gate/up GEMM pass.
@@ -106,14 +201,17 @@ def patch_qwen2_mlp():
         act = getattr(getattr(self, "config", None), "hidden_act", "silu")
         if act != "silu" or not x.is_cuda:
             return original_forward(self, x)
-        recompute = (RECOMPUTE and self.training and torch.is_grad_enabled()
-                     and getattr(x, "requires_grad", False))
+        with_grad = self.training and torch.is_grad_enabled() and getattr(x, "requires_grad", False)
+        keep8 = CHECKPOINT_8BIT and with_grad
+        recompute = RECOMPUTE and with_grad and not keep8
         group = getattr(self.gate_proj, "lora_group", None)
         if (group is not None and group.kind == "gate_up" and group.members[0] is self.gate_proj
                 and group.members[1] is self.up_proj and group.usable(x)):
             # gate/up as one GEMM feeding the fused SwiGLU; same recompute policy
             # (without recompute the SwiGLU backward joins down_proj's dX GEMM)
-            return group.mlp(x, self.down_proj, recompute)
+            return group.mlp(x, self.down_proj, recompute, keep8)
+        if keep8:
+            return self.down_proj(swiglu_8bit(self.gate_proj(x), self.up_proj(x)))
         if not recompute:
             return self.down_proj(fast_swiglu(self.gate_proj(x), self.up_proj(x)))
 

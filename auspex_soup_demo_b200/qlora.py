@@ -617,15 +617,17 @@ class LoRAProjectionGroup:
         recompute of the MLP, solution/kernels/swiglu.py:197-214)."""
         return _LoRAGateUpFn.apply(x, self, bool(recompute), *self.params())
 
-    def mlp(self, x: torch.Tensor, down, recompute: bool) -> torch.Tensor:
+    def mlp(self, x: torch.Tensor, down, recompute: bool, keep8: bool = False) -> torch.Tensor:
         """down(silu(gate(x)) * up(x)) for a gate/up group; one Function with the
         SwiGLU backward fused into down's input-gradient GEMM (FUSE_MLP_BACKWARD)
-        when the activations are kept, bf16, and down is an ungrouped LoRA linear."""
+        when the activations are kept, bf16, and down is an ungrouped LoRA linear.
+        ``keep8`` keeps [g | u] of that form in 8 bits (and h not at all); a form the
+        one Function does not take then recomputes instead."""
         if (FUSE_MLP_BACKWARD and not recompute and self.interleaved
                 and isinstance(down, _LoRABase) and down.lora_group is None
                 and x.dtype == torch.bfloat16 and down.in_features == self.outs[0]):
-            return _LoRAMLPFn.apply(x, self, down, down.lora_A, down.lora_B, *self.params())
-        return down(self.swiglu(x, recompute))
+            return _LoRAMLPFn.apply(x, self, down, keep8, down.lora_A, down.lora_B, *self.params())
+        return down(self.swiglu(x, recompute or keep8))
 
 
 def _group_gemm(group: LoRAProjectionGroup, x2: torch.Tensor, w: torch.Tensor, As16, Bblk,
@@ -886,11 +888,14 @@ class _LoRAMLPFn(torch.autograd.Function):
     (soup_gemm_bf16_lora_swiglu), then down's GEMM as in _LoRALinearFn. Backward:
     dxa_down = dout B_down, then [dg | du] = SwiGLU'(dout W_down + dxa_down As_down)
     in place of [g | u] (soup_gemm_bf16_lora_dswiglu: dh never reaches memory),
-    down's LoRA gradients, then the gate/up group backward.
+    down's LoRA gradients, then the gate/up group backward. With ``keep8`` the
+    forward keeps [g | u] as 8-bit codes and drops h; the backward takes dh from
+    down's GEMM and one pass over the codes gives [dg | du] and h again
+    (soup_swiglu_q8_bwd): 2.1 instead of 6 bytes per token and column kept.
     """
 
     @staticmethod
-    def forward(ctx, x, group, down, A_d, B_d, *params):
+    def forward(ctx, x, group, down, keep8, A_d, B_d, *params):
         k = group.in_features
         inter = group.outs[0]
         x2 = x.reshape(-1, k)
@@ -926,7 +931,14 @@ class _LoRAMLPFn(torch.autograd.Function):
         else:
             out = F.linear(h, w_d, bias_d)
             out.addmm_(xa_d, b16_d.t())
-        ctx.save_for_backward(x2, xa, As16, Bblk, y, h, xa_d, as16_d, b16_d, xaT, xa_dT, bt16_d)
+        if keep8:
+            from .kernels.swiglu import quantize_8bit
+
+            kept = quantize_8bit(y.view(-1, 2 * IL_BLOCK))
+        else:
+            kept = (y, h)
+        ctx.keep8 = keep8
+        ctx.save_for_backward(x2, xa, As16, Bblk, *kept, xa_d, as16_d, b16_d, xaT, xa_dT, bt16_d)
         ctx.w = _keep(w)
         ctx.w_d = _keep(w_d)
         ctx.group = group
@@ -936,7 +948,7 @@ class _LoRAMLPFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        from .kernels.swiglu import swiglu_backward
+        from .kernels.swiglu import swiglu_8bit_backward, swiglu_backward
 
         x2, xa, As16, Bblk, y, h, xa_d, as16_d, b16_d, xaT, xa_dT, bt16_d = ctx.saved_tensors
         group, down = ctx.group, ctx.down
@@ -952,7 +964,22 @@ class _LoRAMLPFn(torch.autograd.Function):
             dxa_d, dxa_dT = _rank_product(d2, bt16_d if bt16_d is not None else b16_d.t().contiguous())
         else:
             dxa_d, dxa_dT = d2 @ b16_d, None
-        if _fused_ok(d2.shape[1], d2, w_d, dxa_d, as16_d, y):
+        if ctx.keep8:
+            codes, scales = y, h  # of [g | u] as [rows * blocks, 2 * IL_BLOCK]
+            m, inter = d2.shape[0], group.outs[0]
+            dh = torch.empty(m, inter, device=d2.device, dtype=d2.dtype)
+            if _fused_ok(d2.shape[1], d2, w_d, dxa_d, as16_d, n=inter):
+                lora_gemm(d2, w_d, True, dxa_d, as16_d, dh)
+            else:
+                torch.mm(d2, w_d, out=dh)
+                dh.addmm_(dxa_d, as16_d)
+            dy = torch.empty(m, group.n_total, device=d2.device, dtype=d2.dtype)
+            h = torch.empty_like(dh)
+            dg, du = _gu_views(group, dy)
+            sb = scales.shape[1] // 2
+            swiglu_8bit_backward(dh.view(dg.shape), codes[:, :IL_BLOCK], codes[:, IL_BLOCK:],
+                                 scales[:, :sb], scales[:, sb:], dg, du, h.view(dg.shape))
+        elif _fused_ok(d2.shape[1], d2, w_d, dxa_d, as16_d, y):
             dswiglu_gemm(d2, w_d, dxa_d, as16_d, y)
             dy = y  # [dg | du] over [g | u]
         else:
@@ -963,12 +990,12 @@ class _LoRAMLPFn(torch.autograd.Function):
             dg, du = _gu_views(group, dy)
             swiglu_backward(dh.view(g.shape[0], g.shape[1]), g, u, dg=dg, du=du)
         gA_d, gB_d = _lora_grads(down.lora_A, down.lora_B, h, d2, xa_d, xa_dT, dxa_d, dxa_dT, down.scaling,
-                                 ctx.needs_input_grad[3], ctx.needs_input_grad[4])
+                                 ctx.needs_input_grad[4], ctx.needs_input_grad[5])
         dx, grads = _group_backward(group, dy, x2, xa, w, As16, Bblk, ctx.needs_input_grad[0],
-                                    ctx.needs_input_grad[5:], xaT)
+                                    ctx.needs_input_grad[6:], xaT)
         if dx is not None:
             dx = dx.view(*ctx.lead, x2.shape[1])
-        return (dx, None, None, gA_d, gB_d, *grads)
+        return (dx, None, None, None, gA_d, gB_d, *grads)
 
 
 def group_projections(model, kinds=("qkv", "gate_up")):
@@ -1174,9 +1201,7 @@ class QLoRATrainer:
             dist.all_reduce(self.flat_grad, op=dist.ReduceOp.SUM)
             self.flat_grad.mul_(1.0 / self.world)
 
-    def step(self, input_ids: torch.Tensor, labels: torch.Tensor, denominator: float):
-        self.flat_grad.zero_()
-        self._refresh_param16()  # the factors may have been changed outside the trainer
+    def _hidden(self, input_ids: torch.Tensor) -> torch.Tensor:
         # Batches here are unpadded single sequences, so the attention mask is
         # exactly the causal pattern. Handing transformers a prepared "no mask"
         # keeps SDPA on is_causal with grouped K/V heads also while a CUDA graph
@@ -1185,9 +1210,56 @@ class QLoRATrainer:
         # SDPA expand K/V to every query head and use a masked kernel (about 3x
         # slower on B200 at S=2048).
         out = self.body(input_ids=input_ids, attention_mask=self._no_mask)
-        hidden = out.last_hidden_state if hasattr(out, "last_hidden_state") else out[0]
+        return out.last_hidden_state if hasattr(out, "last_hidden_state") else out[0]
+
+    def _begin_step(self):
+        self.flat_grad.zero_()
+        self._refresh_param16()  # the factors may have been changed outside the trainer
+
+    def step(self, input_ids: torch.Tensor, labels: torch.Tensor, denominator: float):
+        self._begin_step()
+        hidden = self._hidden(input_ids)
         loss, entropy, token_loss, correct = self.loss_fn.apply(
             hidden, self.model.lm_head, labels, self.chunk, denominator, -100, True)
+        self._end_step(loss)
+        return loss.detach(), correct
+
+    def token_logps(self, input_ids: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+        """Log-probabilities [B, S] of the labels (:func:`causal_labels` of the ids,
+        unscored positions set to -100) without a gradient. Before the first step
+        they are the base model's (LoRA's B starts at 0): the reference of
+        :meth:`preference_step` and :meth:`policy_step`."""
+        from .kernels import head_token_logps
+
+        with torch.no_grad():
+            self._refresh_param16()
+            return head_token_logps(self._hidden(input_ids), self.model.lm_head, labels)[0]
+
+    def preference_step(self, input_ids: torch.Tensor, labels: torch.Tensor, ref_logps, **options):
+        """One step on P preference pairs: ids and labels [2P, S], chosen answers
+        first; options as in :func:`kernels.preference_loss`. Returns (loss, chosen
+        rewards, rejected rewards)."""
+        from .kernels import head_token_logps, preference_loss
+
+        self._begin_step()
+        logps, _ = head_token_logps(self._hidden(input_ids), self.model.lm_head, labels)
+        loss, chosen, rejected = preference_loss(logps, ref_logps, labels, **options)
+        self._end_step(loss)
+        return loss.detach(), chosen, rejected
+
+    def policy_step(self, input_ids: torch.Tensor, labels: torch.Tensor, advantages: torch.Tensor,
+                    **options):
+        """One step on sampled answers with advantages [B] or [B, S]; options as in
+        :func:`kernels.policy_loss`. Returns (loss, mean KL, clipped share)."""
+        from .kernels import head_token_logps, policy_loss
+
+        self._begin_step()
+        logps, _ = head_token_logps(self._hidden(input_ids), self.model.lm_head, labels)
+        loss, kl, clipped = policy_loss(logps, advantages, labels, **options)
+        self._end_step(loss)
+        return loss.detach(), kl, clipped
+
+    def _end_step(self, loss: torch.Tensor):
         loss.backward()
         if self.ddp:
             self._allreduce_grads()
@@ -1197,7 +1269,6 @@ class QLoRATrainer:
         else:
             self.opt.step()
             self._refresh_param16()  # forwards outside the trainer see the updated factors
-        return loss.detach(), correct
 
     def _adamw_step(self):
         self.step_t.add_(1.0)

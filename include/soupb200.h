@@ -110,6 +110,32 @@ int soup_swiglu_bwd(const void* dy, int64_t dy_row_stride, const void* gate,
                     int64_t dgate_row_stride, void* dup, int64_t dup_row_stride, int64_t rows,
                     int64_t cols, int dtype, void* stream);
 
+/* ---- SwiGLU with its inputs kept in 8 bits ----------------------------------
+ * Extends swiglu.py:20-95 (whose backward reads gate and up as they were). A kept
+ * [rows, cols] tensor is one signed byte per element (row stride codes_row_stride)
+ * and one fp32 scale per 64 consecutive columns of a row (row stride
+ * scales_row_stride >= ceil(cols / 64)): scale = absmax / 127, code = rint(x *
+ * (127 / absmax)), value = code * scale, fp32 operations rounded to nearest. A
+ * block with absmax < 2^-100 stands for zeros, one with an infinity or NaN for
+ * NaN. The forward computes out = silu(gate) up from the exact inputs and writes
+ * both codes; the backward is soup_swiglu_bwd's formula at the kept values, and
+ * with h != NULL also writes h = silu(gate) up of the kept values (what a
+ * following projection's weight gradient multiplies). soup_q8_quantize writes the
+ * codes of one tensor alone. dtype: F32, F16 or BF16 for every non-code tensor. */
+int soup_swiglu_q8_fwd(const void* gate, int64_t gate_row_stride, const void* up,
+                       int64_t up_row_stride, void* out, int64_t out_row_stride, int8_t* gate_codes,
+                       int8_t* up_codes, int64_t codes_row_stride, float* gate_scales,
+                       float* up_scales, int64_t scales_row_stride, int64_t rows, int64_t cols,
+                       int dtype, void* stream);
+int soup_swiglu_q8_bwd(const void* dy, int64_t dy_row_stride, const int8_t* gate_codes,
+                       const int8_t* up_codes, int64_t codes_row_stride, const float* gate_scales,
+                       const float* up_scales, int64_t scales_row_stride, void* dgate,
+                       int64_t dgate_row_stride, void* dup, int64_t dup_row_stride, void* h,
+                       int64_t h_row_stride, int64_t rows, int64_t cols, int dtype, void* stream);
+int soup_q8_quantize(const void* x, int64_t x_row_stride, int8_t* codes, int64_t codes_row_stride,
+                     float* scales, int64_t scales_row_stride, int64_t rows, int64_t cols, int dtype,
+                     void* stream);
+
 /* ---- RoPE (rotate-half) ----------------------------------------------------
  * Replaces solution/kernels/rope.py:20-67 (_fused_rope_2d_fwd_kernel) and the
  * two launches of patch_qwen2_rope (rope.py:217-218): Q and K in one launch.
@@ -217,6 +243,90 @@ int soup_ce_vp_backward(void* workspace, size_t workspace_bytes, const void* hid
                         void* dhidden_partial, int dh_dtype, void* dweight_shard, int dw_dtype,
                         int accumulate_dw, void* stream);
 
+/* ---- Per-token log-probabilities of the lm_head ----------------------------
+ * No counterpart in the reference (it trains on the summed cross-entropy only).
+ * logps[i] = z_i[t_i] - lse(z_i) for the logits z_i = hidden_i W^T of target
+ * t_i, and the softmax entropy (entropies may be NULL); both 0 where the target
+ * is ignore_index, and logps NaN where it is outside [0, vocab). Operand types and
+ * row rules as for soup_ce_linear. With `state` (soup_head_logps_state_bytes)
+ * the forward keeps the row-shifted exponentials that the backward multiplies;
+ * without it (NULL) no [rows, vocab] buffer is written.
+ * The backward takes one weight per token, dlogps[i] = dL/dlogps[i] (not read
+ * where the target is ignore_index), and the state of a forward with the same
+ * hidden, weight and targets; it does not change the state, so it may run more
+ * than once. weight_bwd: the weight itself for BF16 operands, a bf16 copy of it
+ * for F16. dhidden [rows, dim] and dweight [vocab, dim] (either may be NULL) are
+ * F32 or BF16; accumulate_dw != 0 adds to dweight. The calls use no scratch but
+ * the given buffers, so calls on different streams are independent. */
+size_t soup_head_logps_state_bytes(int64_t rows, int64_t vocab, int64_t dim);
+size_t soup_head_logps_workspace_bytes(int64_t rows, int64_t vocab, int64_t dim, int backward);
+int soup_head_logps_fwd(const void* hidden, int64_t h_ld, const void* weight, int64_t w_ld,
+                        int in_dtype, const int64_t* targets, int64_t rows, int64_t vocab,
+                        int64_t dim, int64_t ignore_index, float* logps, float* entropies,
+                        void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
+                        void* stream);
+int soup_head_logps_bwd(const void* state, size_t state_bytes, const void* hidden, int64_t h_ld,
+                        int in_dtype, const void* weight_bwd, int64_t wb_ld, const int64_t* targets,
+                        const float* dlogps, int64_t rows, int64_t vocab, int64_t dim,
+                        int64_t ignore_index, void* dhidden, int dh_dtype, void* dweight,
+                        int dw_dtype, int accumulate_dw, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* ---- Preference loss (paired log ratios) ------------------------------------
+ * No counterpart in the reference. Sequences 0 .. pairs-1 of logps [2 pairs, seq]
+ * (fp32, row stride lp_ld) are the chosen answers, pairs .. 2 pairs-1 the rejected
+ * ones in the same order; tokens whose label is ignore_index do not count and
+ * their values are not used. With r_n = sum over the counted tokens of
+ * (logps - ref) of sequence n and h = r_chosen - r_rejected:
+ *   SOUP_PREF_SIGMOID  -(1 - e) log sigmoid(beta h) - e log sigmoid(-beta h), e =
+ *                      label_smoothing in [0, 0.5)
+ *   SOUP_PREF_HINGE    max(0, 1 - beta h)
+ *   SOUP_PREF_IPO      (h' - 1/(2 beta))^2, h' from r_n / (counted tokens of n)
+ * ref_mode 0: no reference (ref NULL); 1: ref [2 pairs, seq] per token (row stride
+ * ref_ld); 2: ref [2 pairs], already summed. loss[1] = mean over the pairs,
+ * rewards[2 pairs] = beta r_n, coef[2 pairs] = dloss / dlogps of a counted token.
+ * The backward writes dlogps [2 pairs, seq] (contiguous) = grad_loss[0] * coef[n]
+ * for counted tokens, 0 for the others. Reproducible (fixed order, no atomics). */
+#define SOUP_PREF_SIGMOID 0
+#define SOUP_PREF_HINGE 1
+#define SOUP_PREF_IPO 2
+size_t soup_preference_loss_workspace_bytes(int64_t pairs, int64_t seq);
+int soup_preference_loss_fwd(const float* logps, int64_t lp_ld, const float* ref, int64_t ref_ld,
+                             int ref_mode, const int64_t* labels, int64_t lab_ld, int64_t pairs,
+                             int64_t seq, int64_t ignore_index, double beta, double label_smoothing,
+                             int loss_type, float* loss, float* rewards, float* coef,
+                             void* workspace, size_t workspace_bytes, void* stream);
+int soup_preference_loss_bwd(const float* grad_loss, const float* coef, const int64_t* labels,
+                             int64_t lab_ld, int64_t pairs, int64_t seq, int64_t ignore_index,
+                             float* dlogps, void* stream);
+
+/* ---- Policy loss (clipped importance ratio, KL term) -------------------------
+ * No counterpart in the reference. Per counted token (label != ignore_index) of
+ * logps [batch, seq]: r = exp(logps - old), A the advantage,
+ *   L = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1),
+ *   d = ref - logps
+ * old_logps NULL: the policy's own log-probabilities (r = 1, dL/dlogps = -A);
+ * ref_logps NULL: no KL term. advantages [batch] (adv_ld 0) or [batch, seq].
+ * SOUP_POLICY_TOKEN: sum over all counted tokens / their number;
+ * SOUP_POLICY_SEQUENCE: mean over the batch of each sequence's mean (a sequence
+ * without counted tokens contributes 0). loss[1]; kl[1] = mean over counted tokens
+ * of e^d - d - 1; clipped[1] = share of counted tokens whose clipped branch is the
+ * smaller one; factor[batch] = weight of a token of each sequence. tok_grad
+ * [batch, seq] (contiguous, NULL: no backward) receives each token's unweighted
+ * gradient, which the backward scales: dlogps = grad_loss[0] factor[n] tok_grad. */
+#define SOUP_POLICY_TOKEN 0
+#define SOUP_POLICY_SEQUENCE 1
+size_t soup_policy_loss_workspace_bytes(int64_t batch, int64_t seq);
+int soup_policy_loss_fwd(const float* logps, int64_t lp_ld, const float* old_logps, int64_t old_ld,
+                         const float* ref_logps, int64_t ref_ld, const float* advantages,
+                         int64_t adv_ld, const int64_t* labels, int64_t lab_ld, int64_t batch,
+                         int64_t seq, int64_t ignore_index, double clip_low, double clip_high,
+                         float kl_coef, int reduction, float* loss, float* kl, float* clipped,
+                         float* factor, float* tok_grad, void* workspace, size_t workspace_bytes,
+                         void* stream);
+int soup_policy_loss_bwd(const float* grad_loss, const float* factor, const float* tok_grad,
+                         int64_t batch, int64_t seq, float* dlogps, void* stream);
+
 /* Stage timing for measurement: while set (n > 0), each soup_ce_linear call on
  * this host thread records events[i] on its stream after stage i:
  * 0 row shifts + logits GEMM, 1 row statistics (+ the gated fallback GEMM),
@@ -255,6 +365,24 @@ int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
                        int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim, float scale,
                        int causal, void* dq, void* dk, void* dv, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* The same attention with a sliding window and sinks: query i sees key j iff
+ * j <= i and (i - j < window or j < sinks), window >= 1, sinks >= 0 (either may
+ * exceed seq). Only key tiles that hold a visible key are read: the cost is
+ * proportional to seq (window + sinks). Buffers, layouts, strides and the
+ * backward's workspace as for soup_attention_fwd / soup_attention_bwd. No kernel
+ * in the reference (transformers masks SDPA for its sliding-window layers). */
+int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
+                              int64_t head_dim, float scale, int64_t window, int64_t sinks,
+                              void* out, float* lse, void* stream);
+int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                              const void* out, const void* dout, const float* lse, int64_t batch,
+                              int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim,
+                              float scale, int64_t window, int64_t sinks, void* dq, void* dk,
+                              void* dv, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- NF4 base weights for the QLoRA step ------------------------------------
  * No kernel in the reference: there the 4-bit base layers come from

@@ -1,0 +1,193 @@
+"""CPU checks of the preference / policy tuning operators: what they refuse, before
+any kernel runs, and the key tile lists of the window attention kernels."""
+
+import math
+
+import pytest
+import torch
+
+from auspex_soup_demo_b200 import _lib, kernels
+
+
+def _cpu(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+LAB = torch.zeros(4, 6, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("call,error", [
+    # CPU tensors
+    (lambda: kernels.preference_loss(_cpu(4, 6), None, LAB), ValueError),
+    (lambda: kernels.policy_loss(_cpu(4, 6), _cpu(4), LAB), ValueError),
+    (lambda: kernels.head_token_logps(_cpu(4, 8), _cpu(9, 8), LAB[0, :4]), ValueError),
+    (lambda: kernels.swiglu_8bit(_cpu(4, 8), _cpu(4, 8)), ValueError),
+    (lambda: kernels.window_attention(*[_cpu(1, 1, 4, 128, dtype=torch.bfloat16)] * 3, 1.0, 2), ValueError),
+    # shapes
+    (lambda: kernels.preference_loss(_cpu(4), None, LAB[0, :4]), ValueError),
+    (lambda: kernels.preference_loss(_cpu(4, 0), None, LAB[:, :0]), ValueError),
+    (lambda: kernels.preference_loss(_cpu(4, 5), None, LAB), ValueError),
+    (lambda: kernels.policy_loss(_cpu(0, 6), _cpu(0), LAB[:0]), ValueError),
+    (lambda: kernels.head_token_logps(_cpu(4, 8), _cpu(9, 16), LAB[0, :4]), ValueError),
+    (lambda: kernels.head_token_logps(_cpu(4, 8), _cpu(9, 8), LAB[0, :3]), ValueError),
+    (lambda: kernels.head_token_logps(_cpu(4, 8), object(), LAB[0, :4]), ValueError),
+    (lambda: kernels.swiglu_8bit(_cpu(4, 8), _cpu(4, 7)), ValueError),
+    (lambda: kernels.swiglu_8bit(_cpu(4, 0), _cpu(4, 0)), ValueError),
+    (lambda: kernels.window_attention(_cpu(4, 128), _cpu(4, 128), _cpu(4, 128), 1.0, 2), ValueError),
+    # types
+    (lambda: kernels.preference_loss(_cpu(4, 6, dtype=torch.float64), None, LAB), TypeError),
+    (lambda: kernels.preference_loss(_cpu(4, 6), None, _cpu(4, 6)), TypeError),
+    (lambda: kernels.policy_loss(_cpu(4, 6, dtype=torch.bfloat16), _cpu(4), LAB), TypeError),
+    (lambda: kernels.policy_loss(_cpu(4, 6), _cpu(4), LAB.bool()), TypeError),
+    (lambda: kernels.head_token_logps(_cpu(4, 8), _cpu(9, 8), _cpu(4)), TypeError),
+    (lambda: kernels.head_token_logps(_cpu(4, 8, dtype=torch.float64), _cpu(9, 8), LAB[0, :4]), TypeError),
+    (lambda: kernels.swiglu_8bit(_cpu(4, 8), _cpu(4, 8, dtype=torch.float16)), TypeError),
+    (lambda: kernels.swiglu_8bit(*[_cpu(4, 8, dtype=torch.int32)] * 2), TypeError),
+])
+def test_refusals(call, error):
+    with pytest.raises(error):
+        call()
+
+
+class _Cuda:
+    """Stands for a CUDA tensor where only the argument checks look at it."""
+
+    def __init__(self, t):
+        self.t = t
+        self.is_cuda = True
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(beta=0.0), dict(beta=-1.0), dict(beta=math.nan), dict(beta=math.inf), dict(label_smoothing=0.5),
+    dict(label_smoothing=-0.1), dict(loss_type="hinge", label_smoothing=0.1), dict(loss_type="other"),
+    dict(ref=_cpu(4, 5)), dict(ref=_cpu(3)), dict(ref=_cpu(4, 6).requires_grad_(True)),
+])
+def test_preference_options(kw):
+    kw = dict(kw)
+    ref = kw.pop("ref", None)
+    with pytest.raises(ValueError):
+        kernels.preference_loss(_Cuda(_cpu(4, 6)), ref, LAB, **kw)
+
+
+def test_preference_odd_rows():
+    with pytest.raises(ValueError, match="as many chosen as rejected"):
+        kernels.preference_loss(_Cuda(_cpu(3, 6)), None, LAB[:3])
+
+
+@pytest.mark.parametrize("kw", [
+    dict(clip_low=1.0), dict(clip_low=-0.1), dict(clip_high=-0.1), dict(clip_high=math.inf),
+    dict(clip_high=math.nan), dict(kl_coef=0.1), dict(kl_coef=-1.0, ref_logps=_cpu(4, 6)),
+    dict(reduction="mean"), dict(old_logps=_cpu(4, 5)), dict(ref_logps=_cpu(4)), dict(adv=_cpu(6)),
+    dict(old_logps=_cpu(4, 6).requires_grad_(True)),
+])
+def test_policy_options(kw):
+    kw = dict(kw)
+    adv = kw.pop("adv", _cpu(4))
+    with pytest.raises(ValueError):
+        kernels.policy_loss(_Cuda(_cpu(4, 6)), adv, LAB, **kw)
+
+
+@pytest.mark.parametrize("scale,window,sinks", [(0.0, 4, 0), (math.nan, 4, 0), (math.inf, 4, 0),
+                                                (1.0, 0, 0), (1.0, -3, 0), (1.0, 4, -1)])
+def test_window_options(scale, window, sinks):
+    t = _Cuda(_cpu(1, 2, 4, 128, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        kernels.window_attention(t, t, t, scale, window, sinks)
+
+
+def test_window_head_dim_and_groups():
+    t = _Cuda(_cpu(1, 2, 4, 64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="head dim"):
+        kernels.window_attention(t, t, t, 1.0, 4)
+    q, k = (_Cuda(_cpu(1, h, 4, 128, dtype=torch.bfloat16)) for h in (3, 2))
+    with pytest.raises(ValueError, match="multiple"):
+        kernels.window_attention(q, k, k, 1.0, 4)
+
+
+def test_entry_points_refuse_bad_arguments():
+    lib = _lib.lib()
+    p, st = 256, _lib.i64_array([128, 128, 128])  # a pointer that no check follows
+    bad = _lib.SOUP_ERR_INVALID
+    assert lib.soup_attention_window_fwd(p, st, p, st, p, st, 1, 1, 1, 4, 128, 1.0, 0, 0, p, p, 0) == bad
+    assert lib.soup_attention_window_bwd(p, st, p, st, p, st, p, p, p, 1, 1, 1, 4, 128, 1.0, 3, -1, p, p, p,
+                                         p, 1 << 20, 0) == bad
+    assert lib.soup_attention_window_fwd(p, st, p, st, p, st, 1, 1, 1, 4, 64, 1.0, 3, 0, p, p,
+                                         0) == _lib.SOUP_ERR_UNSUPPORTED
+    assert b"soup_attention_window_fwd" in lib.soup_last_error()
+    f = lib.soup_preference_loss_fwd
+    ok = [p, 6, p, 6, 1, p, 6, 2, 6, -100, 0.1, 0.0, 0, p, p, p, p, 1 << 20, 0]
+    for i, v in ((0, 0), (1, 5), (2, 0), (3, 5), (4, 3), (6, 5), (7, 0), (8, 0), (10, 0.0), (11, 0.5),
+                 (12, 3), (13, 0), (16, 0)):
+        a = list(ok)
+        a[i] = v
+        assert f(*a) == bad, i
+    a = list(ok)
+    a[17] = 16
+    assert f(*a) == _lib.SOUP_ERR_WORKSPACE
+    f = lib.soup_policy_loss_fwd
+    ok = [p, 6, p, 6, p, 6, p, 0, p, 6, 2, 6, -100, 0.2, 0.2, 0.1, 0, p, p, p, p, p, p, 1 << 20, 0]
+    for i, v in ((0, 0), (1, 5), (3, 5), (5, 5), (6, 0), (7, 3), (9, 5), (10, 0), (11, 0), (13, 1.0),
+                 (14, -1.0), (15, -1.0), (16, 2), (17, 0), (20, 0), (22, 0)):
+        a = list(ok)
+        a[i] = v
+        assert f(*a) == bad, i
+    assert lib.soup_preference_loss_bwd(0, p, p, 6, 2, 6, -100, p, 0) == bad
+    assert lib.soup_policy_loss_bwd(p, p, 0, 2, 6, p, 0) == bad
+    assert lib.soup_head_logps_fwd(0, 8, p, 8, 2, p, 4, 9, 8, -100, p, p, 0, 0, p, 1 << 20, 0) == bad
+    assert lib.soup_head_logps_fwd(p, 8, p, 8, 0, p, 4, 9, 8, -100, p, p, 0, 0, p, 1 << 20, 0) == bad
+    assert lib.soup_head_logps_bwd(p, 1 << 20, p, 8, 2, 0, 8, p, p, 4, 9, 8, -100, p, 2, 0, 2, 0, p, 1 << 20,
+                                   0) == bad
+    assert lib.soup_swiglu_q8_fwd(p, 8, p, 8, p, 8, p, p, 7, p, p, 1, 4, 8, 2, 0) == bad
+    assert lib.soup_swiglu_q8_fwd(p, 65, p, 65, p, 65, p, p, 65, p, p, 1, 4, 65, 2, 0) == bad
+    assert lib.soup_swiglu_q8_bwd(p, 8, p, p, 8, p, p, 1, p, 8, p, 8, p, 7, 4, 8, 2, 0) == bad
+    assert lib.soup_q8_quantize(p, 8, p, 8, p, 1, 4, 8, 9, 0) == bad
+
+
+def test_workspace_sizes():
+    lib = _lib.lib()
+    assert lib.soup_preference_loss_workspace_bytes(0, 5) == 0
+    assert lib.soup_policy_loss_workspace_bytes(3, 4097) >= 2 * lib.soup_policy_loss_workspace_bytes(3, 4096)
+    assert lib.soup_head_logps_state_bytes(10, 0, 8) == 0
+
+
+# ---- the key tiles of a window (the kernels' index arithmetic, 128-key tiles) -------
+def _tiles(q0, window, sinks):
+    first = q0 - window + 1
+    lo = first // 128 if first > 0 else 0
+    n_sink = min(-(-sinks // 128), lo)
+    return n_sink, lo
+
+
+@pytest.mark.parametrize("S", [1, 127, 128, 129, 300, 640, 1000])
+@pytest.mark.parametrize("window", [1, 2, 64, 127, 128, 129, 130, 300, 5000])
+@pytest.mark.parametrize("sinks", [0, 1, 127, 128, 129, 400, 5000])
+def test_window_tile_lists_cover_every_visible_key(S, window, sinks):
+    window, sinks = min(window, S), min(sinks, S)
+    nq, nq64 = -(-S // 128), -(-S // 64)
+
+    def needed(qt):
+        tiles = set()
+        for q in (qt * 128, min(S, qt * 128 + 128) - 1):
+            tiles |= set(range(max(0, q - window + 1) // 128, q // 128 + 1))
+            tiles |= set(range(0, -(-min(sinks, q + 1) // 128)))
+        return tiles
+
+    for qt in range(nq):  # one query tile (dQ) and a pair of them (forward)
+        for end in {qt + 1, min(qt + 2, nq)}:
+            n_sink, lo = _tiles(qt * 128, window, sinks)
+            n = end - (lo - n_sink)
+            tiles = [j if j < n_sink else lo + j - n_sink for j in range(n)]
+            assert len(set(tiles)) == n >= 1 and all(0 <= t < end for t in tiles)
+            for t in range(qt, end):
+                assert needed(t) <= set(tiles)
+    for kt in range(nq):  # the 64-query steps of a key tile (dK / dV)
+        first, n = 2 * kt, nq64 - 2 * kt
+        if kt * 128 >= sinks:
+            n = min((kt * 128 + 127 + window - 1) // 64, nq64 - 1) - first + 1
+        assert n >= 1 and first + n <= nq64
+        for key in range(kt * 128, min(S, kt * 128 + 128)):
+            last = S - 1 if key < sinks else min(S - 1, key + window - 1)
+            assert first <= key // 64 and last // 64 < first + n
