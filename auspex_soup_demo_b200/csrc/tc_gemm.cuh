@@ -280,6 +280,21 @@ struct Sched {
   // 1: no stream-K tail, so the launch shares no scratch with others and may run
   // beside GEMMs of other streams
   int no_sk = 0;
+  // optional device count written by an earlier kernel on the stream: the launch
+  // covers that many leading rows of A instead of all (dyn_k 0: output rows, in
+  // tiles of dyn_unit; 1: the k dimension, in blocks of dyn_unit), at least one
+  // tile or block. With splits == 1 for dyn_k; not with a stream-K tail.
+  const int* dyn_rows = nullptr;
+  int dyn_k = 0;
+  int dyn_unit = 1;
+  __device__ __forceinline__ void apply_dyn() {
+    const int n = *dyn_rows;
+    const int t = n > 0 ? (n + dyn_unit - 1) / dyn_unit : 1;
+    if (dyn_k)
+      kb_total = t;
+    else
+      m_tiles = t;
+  }
   __device__ __forceinline__ uint64_t limit() const { return wait_ns ? wait_ns : kWaitNs; }
   // the instruction descriptor with the operand format of this launch
   __device__ __forceinline__ uint32_t idesc(uint32_t bf16_desc) const {
@@ -544,6 +559,10 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  if (sched.dyn_rows) {  // grid-uniform
+    pdl_wait();
+    sched.apply_dyn();
+  }
   const int n_units = sched.units();
   const uint64_t wait_ns = sched.limit();
   const uint32_t idesc = sched.idesc(kIdesc);
@@ -963,6 +982,10 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
+  if (sched.dyn_rows) {  // grid-uniform
+    pdl_wait();
+    sched.apply_dyn();
+  }
   const int n_my = sched.cluster_units(cluster, n_clusters);
   const uint64_t wait_ns = sched.limit();
   const uint32_t idesc = sched.idesc(kIdesc);

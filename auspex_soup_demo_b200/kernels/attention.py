@@ -118,15 +118,18 @@ def _kernel_layout(t: torch.Tensor):
     """(t, element strides) in a form the tensor maps can read: 16-byte aligned,
     positive strides that are multiples of 8. Dimensions of size 1 take any
     stride; anything else is copied."""
-    def strides(x):
-        full = (x.shape[1] * x.shape[2] * x.shape[3], x.shape[2] * x.shape[3], x.shape[3])
-        return [full[i] if x.shape[i] == 1 else x.stride(i) for i in range(3)]
-
-    st = strides(t)
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(v <= 0 or v % 8 for v in st):
-        t = t.clone(memory_format=torch.contiguous_format)
-        st = strides(t)
-    return t, _lib.i64_array(st)
+    b, h, s, d = t.shape
+    sb, sh, ss, sd = t.stride()
+    if b == 1:
+        sb = h * s * d
+    if h == 1:
+        sh = s * d
+    if s == 1:
+        ss = d
+    if sd != 1 or t.data_ptr() % 16 or (sb | sh | ss) % 8 or sb <= 0 or sh <= 0 or ss <= 0:
+        t = t.detach().clone(memory_format=torch.contiguous_format)
+        sb, sh, ss = h * s * d, s * d, d
+    return t, (_lib.c_i64 * 3)(sb, sh, ss)
 
 
 class WindowAttentionFunction(torch.autograd.Function):
@@ -137,24 +140,25 @@ class WindowAttentionFunction(torch.autograd.Function):
     def forward(ctx, q, k, v, scale: float, window: int, sinks: int):
         B, H, S, D = q.shape
         Hk = k.shape[1]
-        (q, qs), (k, ks), (v, vs) = (_kernel_layout(t.detach()) for t in (q, k, v))
+        (q, qs), (k, ks), (v, vs) = _kernel_layout(q), _kernel_layout(k), _kernel_layout(v)
         out = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device)
         lse = torch.empty(B, H, _s_pad(S), dtype=torch.float32, device=q.device)
         _lib.call("soup_attention_window_fwd", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
                   vs, B, H, Hk, S, D, scale, window, sinks, out.data_ptr(), lse.data_ptr(),
                   _lib.stream_of(q))
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.args = (scale, window, sinks)
+        ctx.args = (qs, ks, vs, scale, window, sinks)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        scale, window, sinks = ctx.args
+        qs, ks, vs, scale, window, sinks = ctx.args
         B, H, S, D = q.shape
         Hk = k.shape[1]
-        dout = dout.to(torch.bfloat16).contiguous()
+        if dout.dtype is not torch.bfloat16 or not dout.is_contiguous():
+            dout = dout.to(torch.bfloat16).contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
         dq = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device)
@@ -162,7 +166,6 @@ class WindowAttentionFunction(torch.autograd.Function):
         dv = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
         nbytes = _lib.lib().soup_attention_bwd_workspace_bytes(B, H, S)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        (_, qs), (_, ks), (_, vs) = (_kernel_layout(t) for t in (q, k, v))
         _lib.call("soup_attention_window_bwd", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
                   vs, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), B, H, Hk, S, D, scale, window,
                   sinks, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes,

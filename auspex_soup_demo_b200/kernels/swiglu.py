@@ -122,29 +122,36 @@ class SwiGLU8BitFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate: torch.Tensor, up: torch.Tensor):
         n = gate.shape[-1]
-        g2, u2 = _rows_8bit(gate.detach(), n), _rows_8bit(up.detach(), n)
+        g2, u2 = _rows_8bit(gate, n), _rows_8bit(up, n)
         rows = g2.shape[0]
-        out = torch.empty(rows, n, dtype=gate.dtype, device=gate.device)
-        codes = torch.empty(2, rows, n, dtype=torch.int8, device=gate.device)
-        scales = torch.empty(2, rows, -(-n // Q8_BLOCK), dtype=torch.float32, device=gate.device)
+        blocks = -(-n // Q8_BLOCK)
+        dt = _lib.dtype_code(gate.dtype)
+        out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+        # one buffer: the scales of gate, of up, the codes of gate (16-byte aligned), of up
+        c0 = -(-8 * rows * blocks // 16) * 16
+        c1 = c0 + -(-rows * n // 16) * 16
+        kept = torch.empty(c1 + rows * n, dtype=torch.int8, device=gate.device)
+        base = kept.data_ptr()
         _lib.call("soup_swiglu_q8_fwd", gate.device, g2.data_ptr(), _ld(g2), u2.data_ptr(), _ld(u2),
-                  out.data_ptr(), n, codes.data_ptr(), codes[1].data_ptr(), n, scales.data_ptr(),
-                  scales[1].data_ptr(), scales.shape[2], rows, n, _lib.dtype_code(gate.dtype),
-                  _lib.stream_of(g2))
-        ctx.save_for_backward(codes, scales)
-        ctx.dtype = gate.dtype
-        return out.view(gate.shape)
+                  out.data_ptr(), n, base + c0, base + c1, n, base, base + 4 * rows * blocks, blocks,
+                  rows, n, dt, _lib.stream_of(g2))
+        ctx.save_for_backward(kept)
+        ctx.args = (rows, n, blocks, c0, c1, dt, gate.dtype)
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy: torch.Tensor):
-        codes, scales = ctx.saved_tensors
-        _, rows, n = codes.shape
-        dy2 = _rows_8bit(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype), n)
-        dg = torch.empty(rows, n, dtype=ctx.dtype, device=dy.device)
-        du = torch.empty_like(dg)
-        swiglu_8bit_backward(dy2, codes[0], codes[1], scales[0], scales[1], dg, du)
-        return dg.view(dy.shape), du.view(dy.shape)
+        (kept,) = ctx.saved_tensors
+        rows, n, blocks, c0, c1, dt, dtype = ctx.args
+        dy2 = _rows_8bit(dy if dy.dtype is dtype else dy.to(dtype), n)
+        dg = torch.empty(dy.shape, dtype=dtype, device=dy.device)
+        du = torch.empty(dy.shape, dtype=dtype, device=dy.device)
+        base = kept.data_ptr()
+        _lib.call("soup_swiglu_q8_bwd", dy.device, dy2.data_ptr(), _ld(dy2), base + c0, base + c1, n, base,
+                  base + 4 * rows * blocks, blocks, dg.data_ptr(), n, du.data_ptr(), n, None, 0, rows, n,
+                  dt, _lib.stream_of(dy2))
+        return dg, du
 
 
 def swiglu_8bit(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:

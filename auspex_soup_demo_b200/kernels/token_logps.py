@@ -136,8 +136,8 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             _lib.call("soup_head_logps_bwd", dev, st.data_ptr(), st.numel(), _lib.ptr(hb),
                       d if hb is None else hb.stride(0), _lib.dtype_code(dt), _lib.ptr(wb),
-                      d if wb is None else wb.stride(0), t[r0:].data_ptr(), g[r0:].data_ptr(), r, v, d,
-                      ignore, None if dh is None else dh[r0:].data_ptr(),
+                      d if wb is None else wb.stride(0), g[r0:].data_ptr(), r, v, d,
+                      None if dh is None else dh[r0:].data_ptr(),
                       _lib.F32 if dh is None else _lib.dtype_code(dh.dtype), _lib.ptr(dw),
                       _lib.F32 if dw is None else _lib.dtype_code(dw.dtype), 1 if r0 else 0,
                       ws.data_ptr(), nbytes, _lib.stream_of(weight))

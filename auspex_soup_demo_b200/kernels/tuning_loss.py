@@ -16,6 +16,7 @@ One summing kernel, one joining kernel and one elementwise backward each
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -31,40 +32,49 @@ REDUCTIONS = {"token": 0, "sequence": 1}
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """(t, row stride) of a [rows, cols] tensor whose rows are contiguous and do not overlap."""
-    t = t.detach()
     n, s = t.shape
-    if (s > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < s):
-        t = t.contiguous()
-    return t, max(t.stride(0), s) if n > 1 else s
+    ld, step = t.stride()
+    if (s > 1 and step != 1) or (n > 1 and ld < s):
+        return t.detach().contiguous(), s
+    return t, ld if n > 1 else s
 
 
 def _labels(labels: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    return _rows(labels if labels.dtype == torch.int64 else labels.to(torch.int64))
+    return _rows(labels if labels.dtype is torch.int64 else labels.to(torch.int64))
+
+
+_INTEGERS = {torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8}
 
 
 def _check(fn: str, logps: torch.Tensor, labels: torch.Tensor) -> None:
-    if logps.dim() != 2 or logps.shape[0] == 0 or logps.shape[1] == 0:
-        raise ValueError(f"{fn}: logps must be [sequences, tokens], got {tuple(logps.shape)}")
-    if logps.dtype != torch.float32:
+    shape = logps.shape
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError(f"{fn}: logps must be [sequences, tokens], got {tuple(shape)}")
+    if logps.dtype is not torch.float32:
         raise TypeError(f"{fn}: logps must be float32, got {logps.dtype}")
-    if labels.shape != logps.shape:
-        raise ValueError(f"{fn}: labels {tuple(labels.shape)} for logps {tuple(logps.shape)}")
-    if labels.is_floating_point() or labels.is_complex() or labels.dtype == torch.bool:
-        raise TypeError(f"{fn}: labels must be integers")
+    if labels.shape != shape:
+        raise ValueError(f"{fn}: labels {tuple(labels.shape)} for logps {tuple(shape)}")
+    if labels.dtype not in _INTEGERS:
+        raise TypeError(f"{fn}: labels must be integers, got {labels.dtype}")
     if not logps.is_cuda or labels.device != logps.device:
         raise ValueError(f"{fn}: logps and labels must be on one CUDA device")
 
 
 def _constant(fn: str, name: str, t: torch.Tensor, shapes, device) -> None:
-    if tuple(t.shape) not in [tuple(s) for s in shapes]:
-        raise ValueError(f"{fn}: {name} has shape {tuple(t.shape)}, expected one of "
-                         f"{[tuple(s) for s in shapes]}")
-    if t.dtype != torch.float32:
+    if t.shape not in shapes:
+        raise ValueError(f"{fn}: {name} has shape {tuple(t.shape)}, expected one of {list(shapes)}")
+    if t.dtype is not torch.float32:
         raise TypeError(f"{fn}: {name} must be float32, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{fn}: {name} must be on {device}")
     if t.requires_grad:
         raise ValueError(f"{fn}: {name} is a constant of the loss; detach it")
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(fn: str, n: int, s: int) -> int:
+    """Of the entry point, rounded up to 16 (what follows it in one buffer is aligned)."""
+    return -(-getattr(_lib.lib(), fn)(n, s) // 16) * 16
 
 
 class PreferenceLossFunction(torch.autograd.Function):
@@ -82,15 +92,15 @@ class PreferenceLossFunction(torch.autograd.Function):
             mode, r = 2, ref.contiguous()
         loss = torch.empty((), dtype=torch.float32, device=dev)
         chosen, rejected = torch.empty(2, p, dtype=torch.float32, device=dev).unbind(0)
-        coef = torch.empty(n, dtype=torch.float32, device=dev)
-        nbytes = _lib.lib().soup_preference_loss_workspace_bytes(p, s)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        nbytes = _workspace_bytes("soup_preference_loss_workspace_bytes", p, s)
+        ws = torch.empty(nbytes // 4 + n, dtype=torch.float32, device=dev)  # workspace, then coef
+        coef = ws.data_ptr() + nbytes
         _lib.call("soup_preference_loss_fwd", dev, x.data_ptr(), x_ld, _lib.ptr(r), r_ld, mode,
                   lab.data_ptr(), lab_ld, p, s, ignore_index, beta, smoothing, loss_type,
-                  loss.data_ptr(), chosen.data_ptr(), coef.data_ptr(), ws.data_ptr(), nbytes,
+                  loss.data_ptr(), chosen.data_ptr(), coef, ws.data_ptr(), nbytes,
                   _lib.stream_of(logps))
-        ctx.save_for_backward(coef, lab)
-        ctx.lab_ld, ctx.ignore_index, ctx.shape = lab_ld, ignore_index, (n, s)
+        ctx.save_for_backward(ws, lab)
+        ctx.args = (nbytes, n, s, lab_ld, ignore_index)
         ctx.mark_non_differentiable(chosen, rejected)
         ctx.set_materialize_grads(False)
         return loss, chosen, rejected
@@ -100,13 +110,12 @@ class PreferenceLossFunction(torch.autograd.Function):
     def backward(ctx, grad, _c, _r):
         if grad is None:
             return (None,) * 7
-        coef, lab = ctx.saved_tensors
-        n, s = ctx.shape
-        out = torch.empty(n, s, dtype=torch.float32, device=coef.device)
+        ws, lab = ctx.saved_tensors
+        off, n, s, lab_ld, ignore_index = ctx.args
+        out = torch.empty(n, s, dtype=torch.float32, device=ws.device)
         grad = grad.to(torch.float32)
-        _lib.call("soup_preference_loss_bwd", coef.device, grad.data_ptr(), coef.data_ptr(),
-                  lab.data_ptr(), ctx.lab_ld, n // 2, s, ctx.ignore_index, out.data_ptr(),
-                  _lib.stream_of(coef))
+        _lib.call("soup_preference_loss_bwd", ws.device, grad.data_ptr(), ws.data_ptr() + off,
+                  lab.data_ptr(), lab_ld, n // 2, s, ignore_index, out.data_ptr(), _lib.stream_of(ws))
         return (out,) + (None,) * 6
 
 
@@ -143,7 +152,7 @@ def preference_loss(logps: torch.Tensor, ref_logps: Optional[torch.Tensor], labe
     if not 0.0 <= label_smoothing < 0.5 or (label_smoothing and loss_type != "sigmoid"):
         raise ValueError(f"{fn}: label_smoothing must be in [0, 0.5) and needs loss_type 'sigmoid'")
     if ref_logps is not None:
-        _constant(fn, "ref_logps", ref_logps, [(n, s), (n,)], logps.device)
+        _constant(fn, "ref_logps", ref_logps, ((n, s), (n,)), logps.device)
     return PreferenceLossFunction.apply(logps, ref_logps, labels, float(beta), float(label_smoothing),
                                         LOSS_TYPES[loss_type], int(ignore_index))
 
@@ -159,17 +168,19 @@ class PolicyLossFunction(torch.autograd.Function):
         o, o_ld = (None, 0) if old is None else _rows(old)
         r, r_ld = (None, 0) if ref is None else _rows(ref)
         a, a_ld = _rows(advantages) if advantages.dim() == 2 else (advantages.contiguous(), 0)
-        loss, kl, clipped = (torch.empty((), dtype=torch.float32, device=dev) for _ in range(3))
-        factor = torch.empty(b, dtype=torch.float32, device=dev)
-        tok = torch.empty(b, s, dtype=torch.float32, device=dev) if keep else None
-        nbytes = _lib.lib().soup_policy_loss_workspace_bytes(b, s)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        kl, clipped = torch.empty(2, dtype=torch.float32, device=dev).unbind(0)
+        nbytes = _workspace_bytes("soup_policy_loss_workspace_bytes", b, s)
+        # workspace, each sequence's weight, and (for a backward) each token's gradient
+        ws = torch.empty(nbytes // 4 + b + (b * s if keep else 0), dtype=torch.float32, device=dev)
+        factor = ws.data_ptr() + nbytes
         _lib.call("soup_policy_loss_fwd", dev, x.data_ptr(), x_ld, _lib.ptr(o), o_ld, _lib.ptr(r), r_ld,
                   a.data_ptr(), a_ld, lab.data_ptr(), lab_ld, b, s, ignore_index, lo, hi, kl_coef,
-                  reduction, loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), factor.data_ptr(),
-                  _lib.ptr(tok), ws.data_ptr(), nbytes, _lib.stream_of(logps))
+                  reduction, loss.data_ptr(), kl.data_ptr(), clipped.data_ptr(), factor,
+                  factor + 4 * b if keep else None, ws.data_ptr(), nbytes, _lib.stream_of(logps))
         if keep:
-            ctx.save_for_backward(factor, tok)
+            ctx.save_for_backward(ws)
+            ctx.args = (nbytes, b, s)
         ctx.mark_non_differentiable(kl, clipped)
         ctx.set_materialize_grads(False)
         return loss, kl, clipped
@@ -179,12 +190,13 @@ class PolicyLossFunction(torch.autograd.Function):
     def backward(ctx, grad, _k, _c):
         if grad is None:
             return (None,) * 11
-        factor, tok = ctx.saved_tensors
-        b, s = tok.shape
-        out = torch.empty_like(tok)
+        (ws,) = ctx.saved_tensors
+        off, b, s = ctx.args
+        out = torch.empty(b, s, dtype=torch.float32, device=ws.device)
         grad = grad.to(torch.float32)
-        _lib.call("soup_policy_loss_bwd", tok.device, grad.data_ptr(), factor.data_ptr(), tok.data_ptr(),
-                  b, s, out.data_ptr(), _lib.stream_of(tok))
+        factor = ws.data_ptr() + off
+        _lib.call("soup_policy_loss_bwd", ws.device, grad.data_ptr(), factor, factor + 4 * b, b, s,
+                  out.data_ptr(), _lib.stream_of(ws))
         return (out,) + (None,) * 10
 
 
@@ -219,10 +231,10 @@ def policy_loss(logps: torch.Tensor, advantages: torch.Tensor, labels: torch.Ten
         raise ValueError(f"{fn}: kl_coef must be finite and not negative")
     if kl_coef and ref_logps is None:
         raise ValueError(f"{fn}: kl_coef needs ref_logps")
-    _constant(fn, "advantages", advantages, [(b,), (b, s)], logps.device)
+    _constant(fn, "advantages", advantages, ((b,), (b, s)), logps.device)
     for name, t in (("old_logps", old_logps), ("ref_logps", ref_logps)):
         if t is not None:
-            _constant(fn, name, t, [(b, s)], logps.device)
+            _constant(fn, name, t, ((b, s),), logps.device)
     keep = torch.is_grad_enabled() and logps.requires_grad
     return PolicyLossFunction.apply(logps, advantages, labels, old_logps, ref_logps, float(clip_low),
                                     float(clip_high), float(kl_coef), REDUCTIONS[reduction],

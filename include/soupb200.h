@@ -247,13 +247,14 @@ int soup_ce_vp_backward(void* workspace, size_t workspace_bytes, const void* hid
  * No counterpart in the reference (it trains on the summed cross-entropy only).
  * logps[i] = z_i[t_i] - lse(z_i) for the logits z_i = hidden_i W^T of target
  * t_i, and the softmax entropy (entropies may be NULL); both 0 where the target
- * is ignore_index, and logps NaN where it is outside [0, vocab). Operand types and
- * row rules as for soup_ce_linear. With `state` (soup_head_logps_state_bytes)
+ * is ignore_index, and logps NaN where it is outside [0, vocab). Only rows with a
+ * target other than ignore_index take part in the matrix products, forward and
+ * backward. Operand types and row rules as for soup_ce_linear. With `state` (soup_head_logps_state_bytes)
  * the forward keeps the row-shifted exponentials that the backward multiplies;
  * without it (NULL) no [rows, vocab] buffer is written.
  * The backward takes one weight per token, dlogps[i] = dL/dlogps[i] (not read
- * where the target is ignore_index), and the state of a forward with the same
- * hidden, weight and targets; it does not change the state, so it may run more
+ * where the target was ignore_index), and the state of a forward with the same
+ * hidden and weight; it does not change the state, so it may run more
  * than once. weight_bwd: the weight itself for BF16 operands, a bf16 copy of it
  * for F16. dhidden [rows, dim] and dweight [vocab, dim] (either may be NULL) are
  * F32 or BF16; accumulate_dw != 0 adds to dweight. The calls use no scratch but
@@ -266,9 +267,8 @@ int soup_head_logps_fwd(const void* hidden, int64_t h_ld, const void* weight, in
                         void* state, size_t state_bytes, void* workspace, size_t workspace_bytes,
                         void* stream);
 int soup_head_logps_bwd(const void* state, size_t state_bytes, const void* hidden, int64_t h_ld,
-                        int in_dtype, const void* weight_bwd, int64_t wb_ld, const int64_t* targets,
-                        const float* dlogps, int64_t rows, int64_t vocab, int64_t dim,
-                        int64_t ignore_index, void* dhidden, int dh_dtype, void* dweight,
+                        int in_dtype, const void* weight_bwd, int64_t wb_ld, const float* dlogps,
+                        int64_t rows, int64_t vocab, int64_t dim, void* dhidden, int dh_dtype, void* dweight,
                         int dw_dtype, int accumulate_dw, void* workspace, size_t workspace_bytes,
                         void* stream);
 

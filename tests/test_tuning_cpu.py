@@ -138,7 +138,7 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.soup_policy_loss_bwd(p, p, 0, 2, 6, p, 0) == bad
     assert lib.soup_head_logps_fwd(0, 8, p, 8, 2, p, 4, 9, 8, -100, p, p, 0, 0, p, 1 << 20, 0) == bad
     assert lib.soup_head_logps_fwd(p, 8, p, 8, 0, p, 4, 9, 8, -100, p, p, 0, 0, p, 1 << 20, 0) == bad
-    assert lib.soup_head_logps_bwd(p, 1 << 20, p, 8, 2, 0, 8, p, p, 4, 9, 8, -100, p, 2, 0, 2, 0, p, 1 << 20,
+    assert lib.soup_head_logps_bwd(p, 1 << 20, p, 8, 2, 0, 8, p, 4, 9, 8, p, 2, 0, 2, 0, p, 1 << 20,
                                    0) == bad
     assert lib.soup_swiglu_q8_fwd(p, 8, p, 8, p, 8, p, p, 7, p, p, 1, 4, 8, 2, 0) == bad
     assert lib.soup_swiglu_q8_fwd(p, 65, p, 65, p, 65, p, p, 65, p, p, 1, 4, 65, 2, 0) == bad
