@@ -92,6 +92,7 @@ _SIGNATURES = {
                                    c_sz, c_vp]),
     "soup_attention_window_fwd": (c_int, [c_vp, P_I64, c_vp, P_I64, c_vp, P_I64, c_i64, c_i64, c_i64,
                                           c_i64, c_i64, c_f, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "soup_attention_window_bwd_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
     "soup_attention_window_bwd": (c_int, [c_vp, P_I64, c_vp, P_I64, c_vp, P_I64, c_vp, c_vp, c_vp, c_i64,
                                           c_i64, c_i64, c_i64, c_i64, c_f, c_i64, c_i64, c_vp, c_vp, c_vp,
                                           c_vp, c_sz, c_vp]),

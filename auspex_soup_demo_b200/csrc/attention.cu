@@ -36,138 +36,14 @@
 // the role records a code in the device error word, raises the CTA's abort
 // flag, the producer waits (bounded) for its copies, the MMA warp drains its
 // MMAs, and the CTA frees TMEM and returns.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-#include <cuda_bf16.h>
-#include <stdint.h>
-#include <stdio.h>
 
-#include <mutex>
-
-#include "soup_common.cuh"
-#include "tc_gemm.cuh"
+#include "attention_common.cuh"
 
 namespace soup {
 namespace attn {
 
-using bf16 = __nv_bfloat16;
-using tc::bounded_wait;
-using tc::mbar_arrive;
-using tc::mbar_arrive_expect_tx;
-using tc::mbar_init;
-using tc::mbar_try_wait;
-using tc::smem_desc_sw128;
-using tc::smem_u32;
-using tc::tc_commit;
-using tc::tc_fence_after;
-using tc::tc_fence_before;
-using tc::tc_mma_bf16;
-using tc::tmem_ld32;
-
-constexpr int kHeadDim = 128;
-constexpr int kTile = 128;             // query rows per CTA and keys per tile
-constexpr int kBox = kTile * 128;      // one [128 rows x 64 cols] bf16 box: 16 KB
-constexpr int kTileBytes = 2 * kBox;   // a 128 x 128 bf16 tile (two 64-column boxes)
 constexpr int kKStages = 2;            // forward K ring depth (a stage frees after S = Q K^T)
 constexpr int kVStages = 1;            // forward V stages (one frees after both tiles' P V)
-
-constexpr int kErrAttnProducer = 0x111;
-constexpr int kErrAttnMma = 0x112;
-constexpr int kErrAttnSoftmax = 0x113;
-constexpr int kErrAttnSmem = 0x114;  // dynamic shared memory too small after 1 KB alignment
-
-// 4-D TMA tile load (coordinates innermost first) into this CTA's shared memory.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-
-// 32 lanes x 32 consecutive fp32 columns from registers into TMEM (the
-// inverse of tmem_ld32); the caller waits with tmem_st_wait.
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
-  __syncwarp();
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
-      "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
-      "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])), "r"(__float_as_uint(v[8])),
-      "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
-      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])),
-      "r"(__float_as_uint(v[15])), "r"(__float_as_uint(v[16])), "r"(__float_as_uint(v[17])),
-      "r"(__float_as_uint(v[18])), "r"(__float_as_uint(v[19])), "r"(__float_as_uint(v[20])),
-      "r"(__float_as_uint(v[21])), "r"(__float_as_uint(v[22])), "r"(__float_as_uint(v[23])),
-      "r"(__float_as_uint(v[24])), "r"(__float_as_uint(v[25])), "r"(__float_as_uint(v[26])),
-      "r"(__float_as_uint(v[27])), "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])),
-      "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st_wait() {
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// 32 lanes x 32 fp32 columns from TMEM without waiting: several loads are
-// issued back to back and completed by one tmem_ld_wait (the registers may
-// not be read before it).
-__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, float (&v)[32]) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  __syncwarp();
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ uint32_t dynamic_smem_bytes() {
-  uint32_t v;
-  asm volatile("mov.u32 %0, %%dynamic_smem_size;" : "=r"(v));
-  return v;
-}
-// One bool from lane 0 to the warp.
-__device__ __forceinline__ bool warp_ok(bool v) { return __shfl_sync(0xffffffffu, v ? 1 : 0, 0) != 0; }
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-
-// K-major operand tile of 128 rows x 128 bf16 columns in shared memory: two
-// 16 KB boxes (columns 0-63, 64-127), rows of 128 B, 128-byte swizzle. The
-// descriptor of k-step kk (16 columns) for tcgen05.mma.
-__device__ __forceinline__ uint64_t desc_kmajor(uint32_t base, int kk) {
-  return smem_desc_sw128(base + (kk >> 2) * kBox + (kk & 3) * 32, 16, 1024);
-}
-// The same bytes read as an MN-major operand whose MN dimension is the tile's
-// 128 columns and whose K dimension is its 128 rows: k-step kk covers rows
-// [16 kk, 16 kk + 16); the two 64-column boxes are the MN atoms (LBO 16 KB).
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t base, int kk) {
-  return smem_desc_sw128(base + kk * 2048, kBox, 1024);
-}
-
-// Byte offset of the 16-byte chunk c (columns 8c..8c+7 of a 64-column box) of
-// row r in a 128-byte-swizzled box: the layout TMA writes and the descriptors read.
-__device__ __forceinline__ uint32_t swz_off(int r, int c) {
-  return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
-}
-
-// Instruction descriptors (fp32 accumulate, bf16 operands, M = N = 128).
-constexpr uint32_t kIdescKK = tc::idesc_bf16(128, false, false, 128);  // A, B K-major
-constexpr uint32_t kIdescKM = tc::idesc_bf16(128, false, true, 128);   // B MN-major
 
 struct AttnArgs {
   int B, H, Hk, S;       // batch, query heads, KV heads, sequence length
@@ -177,80 +53,7 @@ struct AttnArgs {
   float* lse;            // [B, H, S_pad] natural-log log-sum-exp of scale * q.k, rows
                          // padded to S_pad = S rounded up to 128 (padding not written)
   uint64_t wait_ns;
-  int window, sinks;     // kWin kernels only: 1 <= window <= S, 0 <= sinks <= S
 };
-
-// Sliding window with sinks (the kernels' kWin form, always causal): query q
-// sees key k iff k <= q and (q - k < window or k < sinks). The key tiles that
-// a run of queries starting at q0 needs, in the order the kernels take them:
-// the sink tiles that lie before the window's first tile, then the window's
-// tiles up to the diagonal. Tiles outside the list are never loaded, so the
-// work is (window + sinks) keys a query instead of the whole prefix.
-struct KeyTiles {
-  int n_sink, lo;  // leading sink tiles; first tile of the window
-  __device__ __forceinline__ int at(int j) const { return j < n_sink ? j : lo + (j - n_sink); }
-};
-__device__ __forceinline__ KeyTiles key_tiles(int q0, int window, int sinks) {
-  KeyTiles t;
-  const int first = q0 - window + 1;
-  t.lo = first > 0 ? first / kTile : 0;
-  const int ns = (sinks + kTile - 1) / kTile;
-  t.n_sink = ns < t.lo ? ns : t.lo;
-  return t;
-}
-// Which of 32 keys from key0 on query q sees, as bits; and which of 32 queries
-// from q0 on see key. A tile that some border crosses is masked by these words:
-// three clamped shifts a row instead of four comparisons an element (which made
-// up half of the forward's instructions: 101 us against XXX us at 4 x 2048 tokens,
-// 12 heads, window 512), and a warp whose 32 words are all empty or all full skips
-// the exponentials or the masking.
-__device__ __forceinline__ uint32_t low_bits(int n) {
-  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-}
-__device__ __forceinline__ uint32_t keys_seen(int q, int key0, int S, int window, int sinks) {
-  const int end = (q + 1 < S ? q + 1 : S) - key0;
-  return low_bits(end) & (~low_bits(q - window + 1 - key0) | low_bits(sinks - key0));
-}
-__device__ __forceinline__ uint32_t queries_seeing(int key, int q0, int S, int window, int sinks) {
-  const uint32_t in = key < sinks ? 0xffffffffu : low_bits(key + window - q0);
-  return low_bits(S - q0) & ~low_bits(key - q0) & in;
-}
-// Warp-uniform: 0 no lane's word has a bit, 1 every bit of every word, 2 otherwise.
-__device__ __forceinline__ int mask_kind(uint32_t m) {
-  if (__all_sync(0xffffffffu, m == 0u)) return 0;
-  return __all_sync(0xffffffffu, m == 0xffffffffu) ? 1 : 2;
-}
-// Some pair of the tile of keys [k0, k0 + 128) and the queries up to q_max is
-// hidden by the window.
-__device__ __forceinline__ bool win_edge(int q_max, int k0, int window, int sinks) {
-  return q_max - k0 >= window && k0 + kTile > sinks;
-}
-
-// D (TMEM) [+]= A (TMEM, M rows in lanes, two bf16 of K per 32-bit column) x B (smem descriptor).
-__device__ __forceinline__ void tc_mma_bf16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
-                                                   uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// 32 lanes x 32 consecutive 32-bit columns from registers into TMEM.
-__device__ __forceinline__ void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
-  __syncwarp();
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-      "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
 
 // ------------------------------------------------------------- forward ----
 // One CTA per (batch, query head, pair of 128-query tiles A = 2p, B = 2p + 1);
@@ -288,32 +91,6 @@ constexpr int kFwdThreads = 64 + 32 * kSoftmaxWarps;
 
 // Q, K, V maps: 4-D {D, S, heads, B} with box {64, 128, 1, 1}; coordinates
 // (d0, s0, head, b).
-// 32 lanes x 16 consecutive 32-bit columns from TMEM (waits for the load).
-__device__ __forceinline__ void tmem_ld16u(uint32_t taddr, uint32_t (&v)[16]) {
-  __syncwarp();
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
-        "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr)
-      : "memory");
-}
-
-// 32 lanes x 16 consecutive 32-bit columns from registers into TMEM.
-__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
-  __syncwarp();
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15])
-      : "memory");
-}
-
 // O row of this thread (128 fp32 TMEM columns) times alpha. A separate,
 // non-inlined function: the rescale is rare, and keeping its registers out of
 // the softmax loop avoids spills there. Warp-collective.
@@ -335,7 +112,6 @@ __device__ __noinline__ void rescale_o_row(uint32_t o_t, float alpha) {
   }
 }
 
-template <bool kWin>
 __global__ void __launch_bounds__(kFwdThreads, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                     const __grid_constant__ CUtensorMap tma_v, AttnArgs a, int* err) {
@@ -371,11 +147,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const int b = bh / a.H, h = bh % a.H;
   const int hk = h / (a.H / a.Hk);
   // key tiles each query tile attends to (B's are a superset of A's)
-  KeyTiles kt{0, 0};
-  if (kWin) kt = key_tiles(2 * pr * kTile, a.window, a.sinks);
-  const int skip = kWin ? kt.lo - kt.n_sink : 0;  // tiles of the prefix not in the list
-  const int nkv_a = (a.causal ? 2 * pr + 1 : nq) - skip;
-  const int nkv_b = (a.causal ? (2 * pr + 2 < nq ? 2 * pr + 2 : nq) : nq) - skip;
+  const int nkv_a = a.causal ? 2 * pr + 1 : nq;
+  const int nkv_b = a.causal ? (2 * pr + 2 < nq ? 2 * pr + 2 : nq) : nq;
   const uint64_t wait_ns = a.wait_ns;
 
   if (threadIdx.x == 0) {
@@ -419,22 +192,21 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       int issued_k = 0, issued_v = 0;
       for (int j = 0; j < nkv_b; ++j) {
         const int sk = j % kKStages, sv = j % kVStages;
-        const int key0 = (kWin ? kt.at(j) : j) * kTile;
         if (!bounded_wait(k_empty(sk), ((j / kKStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t kd = sbase + L::kK + sk * kTileBytes;
         mbar_arrive_expect_tx(k_full(sk), kTileBytes);
-        tma_load_4d(kd, &tma_k, k_full(sk), 0, key0, hk, b);
-        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, key0, hk, b);
+        tma_load_4d(kd, &tma_k, k_full(sk), 0, j * kTile, hk, b);
+        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, j * kTile, hk, b);
         ++issued_k;
         if (!bounded_wait(v_empty(sv), ((j / kVStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t vd = sbase + L::kV + sv * kTileBytes;
         mbar_arrive_expect_tx(v_full(sv), kTileBytes);
-        tma_load_4d(vd, &tma_v, v_full(sv), 0, key0, hk, b);
-        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, key0, hk, b);
+        tma_load_4d(vd, &tma_v, v_full(sv), 0, j * kTile, hk, b);
+        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, j * kTile, hk, b);
         ++issued_v;
       }
       // let every issued copy land before the CTA may leave (bounded)
@@ -536,12 +308,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (key >= a.S || (a.causal && key > q)) v[i] = -INFINITY;
       }
     };
-    // -inf where the word has no bit
-    auto bits32 = [&](float (&v)[32], uint32_t m) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (!(m & (1u << i))) v[i] = -INFINITY;
-    };
     auto max32 = [&](const float (&v)[32]) -> float {
       float mx[8];
 #pragma unroll
@@ -575,52 +341,29 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (lane == 0) w = bounded_wait(s_full(x), j & 1, abort_flag, err, kErrAttnSoftmax, wait_ns);
       if (!(ok = warp_ok(w))) break;
       tc_fence_after();
-      const int jt = kWin ? kt.at(j) : j;
-      const int k0 = jt * kTile;
-      const bool edge = (k0 + kTile > a.S) || (a.causal && jt == qt) ||
-                        (kWin && win_edge(qt * kTile + kTile - 1, k0, a.window, a.sinks));
-      // kWin: the four 32-key words of this row and what the warp does with each
-      uint32_t mk[4];
-      int kind[4];
-      if (kWin) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mk[c] = 0xffffffffu;
-          kind[c] = 1;
-          if (edge) {
-            mk[c] = keys_seen(q, k0 + 32 * c, a.S, a.window, a.sinks);
-            kind[c] = mask_kind(mk[c]);
-          }
-        }
-      }
-      // masked values of chunk c's 32 keys, and their maximum
-      auto mask_chunk = [&](float (&v)[32], int c) {
-        if (kWin) {
-          if (kind[c] == 2) bits32(v, mk[c]);
-        } else if (edge) {
-          mask32(v, k0 + 32 * c);
-        }
-      };
-      auto chunk_max = [&](const float (&v)[32], int c) -> float {
-        return kWin && kind[c] == 0 ? -INFINITY : max32(v);
-      };
+      const int k0 = j * kTile;
+      const bool edge = (k0 + kTile > a.S) || (a.causal && j == qt);
       // pass 1: the row maximum of the raw logits (the scale is positive): keys
       // 0-63, then keys 64-127, which stay in registers
       float s[kHalf];
-      float(&s0)[32] = *reinterpret_cast<float(*)[32]>(s);
-      float(&s1)[32] = *reinterpret_cast<float(*)[32]>(s + 32);
-      tmem_ld32_async(st_t, s0);
-      tmem_ld32_async(st_t + 32, s1);
+      tmem_ld32_async(st_t, *reinterpret_cast<float(*)[32]>(s));
+      tmem_ld32_async(st_t + 32, *reinterpret_cast<float(*)[32]>(s + 32));
       tmem_ld_wait();
-      mask_chunk(s0, 0);
-      mask_chunk(s1, 1);
-      const float m0 = fmaxf(chunk_max(s0, 0), chunk_max(s1, 1));
-      tmem_ld32_async(st_t + 64, s0);
-      tmem_ld32_async(st_t + 96, s1);
+      if (edge) {
+        mask32(*reinterpret_cast<float(*)[32]>(s), k0);
+        mask32(*reinterpret_cast<float(*)[32]>(s + 32), k0 + 32);
+      }
+      const float m0 = fmaxf(max32(*reinterpret_cast<float(*)[32]>(s)),
+                             max32(*reinterpret_cast<float(*)[32]>(s + 32)));
+      tmem_ld32_async(st_t + 64, *reinterpret_cast<float(*)[32]>(s));
+      tmem_ld32_async(st_t + 96, *reinterpret_cast<float(*)[32]>(s + 32));
       tmem_ld_wait();
-      mask_chunk(s0, 2);
-      mask_chunk(s1, 3);
-      const float m1 = fmaxf(chunk_max(s0, 2), chunk_max(s1, 3));
+      if (edge) {
+        mask32(*reinterpret_cast<float(*)[32]>(s), k0 + 64);
+        mask32(*reinterpret_cast<float(*)[32]>(s + 32), k0 + 96);
+      }
+      const float m1 = fmaxf(max32(*reinterpret_cast<float(*)[32]>(s)),
+                             max32(*reinterpret_cast<float(*)[32]>(s + 32)));
       const float mt = fmaxf(m0, m1) * a.scale_log2;
       bool rescale = false;
       float alpha = 1.f;
@@ -629,10 +372,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         m_used = mt;
         rescale = true;
       }
-      // a window may hide a row's whole first tiles: its maximum is then still
-      // -inf, and the exponent offset 0 keeps exp2(-inf + 0) = 0 (not NaN)
-      const float nm = kWin && m_used == -INFINITY ? 0.f : -m_used;
-      const uint64_t nm2 = f2_pack(nm, nm);
+      const uint64_t nm2 = f2_pack(-m_used, -m_used);
       // the previous tile's P V product has read the P buffer, and O_X is stable
       if (j > 0) {
         if (lane == 0) w = bounded_wait(pv_done(x), (j - 1) & 1, abort_flag, err, kErrAttnSoftmax,
@@ -653,27 +393,24 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           *reinterpret_cast<uint4*>(box + swz_off(r, c0 + c)) =
               make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]);
       };
-      auto exp_chunk = [&](const float (&v)[32], int c) {
-        if (kWin && kind[c] == 0) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pw[i] = 0u;
-        } else {
-          exp32(v, nm2, pw, sm2);
-        }
-        store4(pbox + (c >> 1) * kBox, 4 * (c & 1));
-      };
-      exp_chunk(s0, 2);
-      exp_chunk(s1, 3);
-      tmem_ld32_async(st_t, s0);
-      tmem_ld32_async(st_t + 32, s1);
+      exp32(*reinterpret_cast<float(*)[32]>(s), nm2, pw, sm2);
+      store4(pbox + kBox, 0);
+      exp32(*reinterpret_cast<float(*)[32]>(s + 32), nm2, pw, sm2);
+      store4(pbox + kBox, 4);
+      tmem_ld32_async(st_t, *reinterpret_cast<float(*)[32]>(s));
+      tmem_ld32_async(st_t + 32, *reinterpret_cast<float(*)[32]>(s + 32));
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free(x));
-      mask_chunk(s0, 0);
-      mask_chunk(s1, 1);
-      exp_chunk(s0, 0);
-      exp_chunk(s1, 1);
+      if (edge) {
+        mask32(*reinterpret_cast<float(*)[32]>(s), k0);
+        mask32(*reinterpret_cast<float(*)[32]>(s + 32), k0 + 32);
+      }
+      exp32(*reinterpret_cast<float(*)[32]>(s), nm2, pw, sm2);
+      store4(pbox, 0);
+      exp32(*reinterpret_cast<float(*)[32]>(s + 32), nm2, pw, sm2);
+      store4(pbox, 4);
       float sm[8];
 #pragma unroll
       for (int u = 0; u < 4; ++u) f2_unpack(sm2[u], sm[2 * u], sm[2 * u + 1]);
@@ -725,61 +462,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 }
 
 // ------------------------------------------------------------ backward ----
-// D[b, h, q] = sum_d dO[b, q, h, d] * O[b, q, h, d] (fp32) and nl2[b, h, q] =
-// -lse[b, h, q] * log2(e) (the exponent offset of P in base 2); rows padded
-// like lse ([B, H, S_pad]). dO and O are [B, S, H, D] contiguous. Sixteen lanes
-// per row (16 bytes each), rows taken in the output's (b, h, q) order so the
-// stores are contiguous, four rows per half-warp with all loads issued first.
-constexpr int kDotRows = 4;
-__global__ void __launch_bounds__(256) attn_bwd_dot_kernel(const bf16* __restrict__ dO,
-                                                           const bf16* __restrict__ O,
-                                                           const float* __restrict__ lse, int B,
-                                                           int H, int S, float* __restrict__ Dv,
-                                                           float* __restrict__ nl2) {
-  pdl_wait();
-  pdl_trigger();
-  const int64_t nrows = (int64_t)B * H * S;
-  const int sub = threadIdx.x & 15;
-  const int64_t half = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
-  const int64_t nhalves = ((int64_t)gridDim.x * blockDim.x) >> 4;
-  const int64_t s_pad = (int64_t)(S + kTile - 1) / kTile * kTile;
-  for (int64_t base = half * kDotRows; base < nrows; base += nhalves * kDotRows) {
-    uint4 a[kDotRows], c[kDotRows];
-#pragma unroll
-    for (int u = 0; u < kDotRows; ++u) {
-      const int64_t i = base + u;  // (b, h, q) row-major
-      if (i < nrows) {
-        const int q = (int)(i % S);
-        const int64_t bh = i / S;
-        const int h = (int)(bh % H), b = (int)(bh / H);
-        const int64_t row = ((int64_t)b * S + q) * H + h;
-        a[u] = *reinterpret_cast<const uint4*>(dO + row * kHeadDim + sub * 8);
-        c[u] = *reinterpret_cast<const uint4*>(O + row * kHeadDim + sub * 8);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kDotRows; ++u) {
-      const int64_t i = base + u;
-      const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&a[u]);
-      const __nv_bfloat162* cp = reinterpret_cast<const __nv_bfloat162*>(&c[u]);
-      float acc = 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 x = __bfloat1622float2(ap[e]), y = __bfloat1622float2(cp[e]);
-        acc = fmaf(x.x, y.x, fmaf(x.y, y.y, acc));
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-      if (sub == 0 && i < nrows) {
-        const int q = (int)(i % S);
-        const int64_t v = (i / S) * s_pad + q;
-        Dv[v] = acc;
-        nl2[v] = -lse[v] * kLog2e;
-      }
-    }
-  }
-}
-
 struct BwdArgs {
   int B, H, Hk, S;
   float scale;        // softmax scale (applied to dK, dQ in fp32)
@@ -792,7 +474,6 @@ struct BwdArgs {
   float* dv_part;
   bf16* dq;           // dQ kernel: [B, S, H, D]
   uint64_t wait_ns;
-  int window, sinks;  // kWin kernels only
 };
 
 // dK / dV partials of one query head for one 128-key tile, stepping through its
@@ -803,11 +484,7 @@ struct BwdArgs {
 // P^T and dS^T buffers (16 KB each: 128 keys x 64 queries, one swizzled box), so
 // this step's P / dS are computed while the tensor core runs the next step's
 // S^T / dP^T and this step's dV / dK products.
-constexpr int kQStep = 64;                 // queries per dK / dV step
 constexpr int kDkvStages = 3;
-constexpr int kStepBox = kQStep * 128;     // a [64 rows x 64 cols] bf16 box: 8 KB
-constexpr int kStepTile = 2 * kStepBox;    // a 64 x 128 bf16 tile: 16 KB
-constexpr int kPTBytes = kTile * 128;      // P^T / dS^T: 128 rows x 64 bf16 = 16 KB
 struct DkvSmem {
   static constexpr int kK = 0;
   static constexpr int kV = kK + kTileBytes;
@@ -827,33 +504,7 @@ struct DkvSmem {
 };
 static_assert(DkvSmem::kUsed + 128 <= 232448, "attention dK/dV shared memory exceeds 227 KB");
 
-// Descriptors of a 64-row step tile (two 8 KB boxes of 64 columns): as a K-major
-// operand with N = 64 rows (k-step kk: 16 columns), and as an MN-major operand
-// whose K dimension is its 64 rows (k-step kk: rows 16 kk..16 kk + 15; LBO 8 KB).
-__device__ __forceinline__ uint64_t desc_kmajor64(uint32_t base, int kk) {
-  return smem_desc_sw128(base + (kk >> 2) * kStepBox + (kk & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t desc_mnmajor64(uint32_t base, int kk) {
-  return smem_desc_sw128(base + kk * 2048, kStepBox, 1024);
-}
-// P^T / dS^T (128 rows x 64 columns, one box) as the K-major A operand.
-__device__ __forceinline__ uint64_t desc_kmajor_box(uint32_t base, int kk) {
-  return smem_desc_sw128(base + kk * 32, 16, 1024);
-}
-constexpr uint32_t kIdescKK64 = tc::idesc_bf16(64, false, false, 128);  // M 128, N 64
-
 constexpr int kBwdThreads = 64 + 32 * kSoftmaxWarps;
-
-// Untiled bulk copy global -> this CTA's shared memory (16-byte aligned
-// addresses, size a multiple of 16), completing on an mbarrier.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
-                                          uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
-      : "memory");
-}
 
 // Half a row of a packed bf16 tile (32 words = the 64 values of this thread's
 // row in one column half) into that half's 64-column swizzled box.
@@ -876,7 +527,6 @@ __device__ __forceinline__ void store_row_tile(uint8_t* tile, int r, const uint3
 // Maps: K / V over [B, Hk, S, D] (128-row boxes), Q over [B, H, S, D] and dO
 // over [B, S, H, D] viewed as [B, H, S, D] (strides S*H*D, D, H*D), both with
 // 64-row boxes.
-template <bool kWin>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tma_q,
                          const __grid_constant__ CUtensorMap tma_k,
@@ -913,13 +563,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int hk = h / (a.H / a.Hk);
   const int k0 = kt * kTile;
   const int step_first = a.causal ? kt * (kTile / kQStep) : 0;
-  // the last query that sees a key of this tile: through the window, or any when
-  // the tile holds a sink
-  int n = nq64 - step_first;
-  if (kWin && k0 >= a.sinks) {
-    const int last = (k0 + kTile - 1 + a.window - 1) / kQStep;
-    n = (last < nq64 - 1 ? last : nq64 - 1) - step_first + 1;
-  }
+  const int n = nq64 - step_first;
   const int64_t s_pad = (int64_t)nq * kTile;
   const uint64_t wait_ns = a.wait_ns;
 
@@ -1076,19 +720,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const float* vnl = reinterpret_cast<const float*>(smem + L::kVec + st * 2 * kQStep * 4) + cb;
       const float* vD = vnl + kQStep;
       const int qs = (step_first + i) * kQStep;
-      const bool edge = (qs + kQStep > a.S) || (a.causal && qs < k0 + kTile) ||
-                        (kWin && win_edge(qs + kQStep - 1, k0, a.window, a.sinks));
+      const bool edge = (qs + kQStep > a.S) || (a.causal && qs < k0 + kTile);
       uint32_t pw[16], dw[16];
-      uint32_t mk = 0xffffffffu;  // kWin: the queries of this step that see the key
-      int kind = 1;
-      if (kWin && edge) {
-        mk = queries_seeing(key, q0, a.S, a.window, a.sinks);
-        kind = mask_kind(mk);
-      }
-      if (kWin && kind == 0) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pw[e] = dw[e] = 0u;
-      } else
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const float4 nl = *reinterpret_cast<const float4*>(vnl + e);
@@ -1102,14 +735,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint64_t t1 = f2_add(f2_pack(dp[e + 2], dp[e + 3]), f2_pack(-dd.z, -dd.w));
         f2_unpack(f2_mul(f2_pack(p[0], p[1]), t0), d[0], d[1]);
         f2_unpack(f2_mul(f2_pack(p[2], p[3]), t1), d[2], d[3]);
-        // padding rows of nl2 / D may hold anything: select, do not scale
-        if (kWin) {
-          if (kind == 2) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (!(mk & (1u << (e + u)))) p[u] = d[u] = 0.f;
-          }
-        } else if (edge) {
+        if (edge) {  // padding rows of nl2 / D may hold anything: select, do not scale
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int q = q0 + e + u;
@@ -1207,7 +833,6 @@ struct DqSmem {
 };
 static_assert(DqSmem::kUsed + 128 <= 232448, "attention dQ shared memory exceeds 227 KB");
 
-template <bool kWin>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tma_q,
                        const __grid_constant__ CUtensorMap tma_k,
@@ -1242,9 +867,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const int b = bh / a.H, h = bh % a.H;
   const int hk = h / (a.H / a.Hk);
   const int q0 = qt * kTile;
-  KeyTiles kt{0, 0};
-  if (kWin) kt = key_tiles(q0, a.window, a.sinks);
-  const int n = (a.causal ? qt + 1 : nq) - (kWin ? kt.lo - kt.n_sink : 0);
+  const int n = a.causal ? qt + 1 : nq;
   const uint64_t wait_ns = a.wait_ns;
 
   if (threadIdx.x == 0) {
@@ -1285,22 +908,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int issued_k = 0, issued_v = 0;
       for (int j = 0; j < n; ++j) {
         const int sk = j % kDqKStages, sv = j % kDqVStages;
-        const int key0 = (kWin ? kt.at(j) : j) * kTile;
         if (!bounded_wait(k_empty(sk), ((j / kDqKStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t kd = sbase + L::kK + sk * kTileBytes;
         mbar_arrive_expect_tx(k_full(sk), kTileBytes);
-        tma_load_4d(kd, &tma_k, k_full(sk), 0, key0, hk, b);
-        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, key0, hk, b);
+        tma_load_4d(kd, &tma_k, k_full(sk), 0, j * kTile, hk, b);
+        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, j * kTile, hk, b);
         ++issued_k;
         if (!bounded_wait(v_empty(sv), ((j / kDqVStages) & 1) ^ 1, abort_flag, err,
                           kErrAttnProducer, wait_ns))
           break;
         const uint32_t vd = sbase + L::kV + sv * kTileBytes;
         mbar_arrive_expect_tx(v_full(sv), kTileBytes);
-        tma_load_4d(vd, &tma_v, v_full(sv), 0, key0, hk, b);
-        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, key0, hk, b);
+        tma_load_4d(vd, &tma_v, v_full(sv), 0, j * kTile, hk, b);
+        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, j * kTile, hk, b);
         ++issued_v;
       }
       uint64_t t0 = tc::globaltimer();
@@ -1400,50 +1022,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(st_empty);  // the next tile's S / dP may overwrite them
-      const int jt = kWin ? kt.at(j) : j;
-      const int k0 = jt * kTile + cb;
-      const bool edge = (jt * kTile + kTile > a.S) || (a.causal && jt == qt) ||
-                        (kWin && win_edge(q0 + kTile - 1, jt * kTile, a.window, a.sinks));
+      const int k0 = j * kTile + cb;
+      const bool edge = (j * kTile + kTile > a.S) || (a.causal && j == qt);
       uint32_t dw[kHalf / 2];
-      uint32_t mk[2];
-      int kind[2];
-      if (kWin) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          mk[c] = 0xffffffffu;
-          kind[c] = 1;
-          if (edge) {
-            mk[c] = keys_seen(q, k0 + 32 * c, a.S, a.window, a.sinks);
-            kind[c] = mask_kind(mk[c]);
-          }
+      for (int e = 0; e < kHalf; e += 2) {
+        float p0, p1, d0, d1;
+        f2_unpack(f2_fma(f2_pack(sv[e], sv[e + 1]), sl2, nl2), p0, p1);
+        p0 = fast_exp2(p0);
+        p1 = fast_exp2(p1);
+        f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0, d1);
+        if (edge) {
+          const int key = k0 + e;
+          if (key >= a.S || (a.causal && key > q)) d0 = 0.f;
+          if (key + 1 >= a.S || (a.causal && key + 1 > q)) d1 = 0.f;
         }
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        if (kWin && kind[c] == 0) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) dw[16 * c + e] = 0u;
-          continue;
-        }
-#pragma unroll
-        for (int e = 32 * c; e < 32 * c + 32; e += 2) {
-          float p0, p1, d0, d1;
-          f2_unpack(f2_fma(f2_pack(sv[e], sv[e + 1]), sl2, nl2), p0, p1);
-          p0 = fast_exp2(p0);
-          p1 = fast_exp2(p1);
-          f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0, d1);
-          if (kWin) {
-            if (kind[c] == 2) {
-              if (!(mk[c] & (1u << (e & 31)))) d0 = 0.f;
-              if (!(mk[c] & (2u << (e & 31)))) d1 = 0.f;
-            }
-          } else if (edge) {
-            const int key = k0 + e;
-            if (key >= a.S || (a.causal && key > q)) d0 = 0.f;
-            if (key + 1 >= a.S || (a.causal && key + 1 > q)) d1 = 0.f;
-          }
-          dw[e >> 1] = pack_bf16(d0, d1);
-        }
+        dw[e >> 1] = pack_bf16(d0, d1);
       }
       if (j > 0) {  // the previous tile's dQ product has read dS
         if (lane == 0) w = bounded_wait(buf_free, (j - 1) & 1, abort_flag, err, kErrAttnSoftmax,
@@ -1529,94 +1123,31 @@ __global__ void __launch_bounds__(256) attn_bwd_group_sum_kernel(const float* __
 }
 
 // ----------------------------------------------------------------- host ----
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  std::lock_guard<std::mutex> lock(cache_mutex());
-  if (!fn) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }
-  return fn;
-}
+}  // namespace attn
+}  // namespace soup
 
-// 4-D map over a bf16 [B, heads, S, D] tensor with element strides (b, h, s)
-// and a contiguous last dimension: dims {D, S, heads, B}, box {64, 128, 1, 1},
-// 128-byte swizzle, zero fill outside.
-static int make_bhsd_map(CUtensorMap* map, const void* ptr, const int64_t* strides, int64_t B,
-                         int64_t heads, int64_t S, const char* what, int box_rows = kTile) {
-  auto fn = encode_fn();
-  if (!fn) {
-    set_last_error("cuTensorMapEncodeTiled is not available from the driver");
-    return SOUP_ERR_CUDA;
-  }
-  if (int rc = bind_context()) return rc;
-  cuuint64_t dims[4] = {(cuuint64_t)kHeadDim, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
-  cuuint64_t gstr[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2,
-                        (cuuint64_t)strides[0] * 2};
-  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, gstr, box,
-                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    char msg[200];
-    snprintf(msg, sizeof(msg), "attention: cuTensorMapEncodeTiled failed (%d) for %s", (int)r, what);
-    set_last_error(msg);
-    return SOUP_ERR_UNSUPPORTED;
-  }
-  return SOUP_OK;
-}
+using namespace soup;
+using namespace soup::attn;
 
-// Strides of a [B, heads, S, 128] bf16 operand usable by TMA: 16-byte aligned
-// base, every stride a multiple of 8 elements.
-static bool bhsd_ok(const void* p, const int64_t* st) {
-  return p && aligned16(p) && st && st[0] > 0 && st[1] > 0 && st[2] > 0 && st[0] % 8 == 0 &&
-         st[1] % 8 == 0 && st[2] % 8 == 0;
-}
+extern "C" {
 
-template <typename K>
-static int set_smem(K kern, int bytes, bool* done) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return cuda_status(cudaErrorInvalidDevice);
-  std::lock_guard<std::mutex> lock(cache_mutex());
-  if (!done[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return cuda_status(e);
-    done[dev] = true;
-  }
-  return SOUP_OK;
-}
-
-static void fn_error(const char* fn, const char* text) {
-  char msg[256];
-  snprintf(msg, sizeof(msg), "%s: %s", fn, text);
-  set_last_error(msg);
-}
-
-// The forward of both forms: window 0 is the plain one. `fn` names the entry
-// point in error messages.
-static int attention_fwd(const char* fn, const void* q, const int64_t* q_strides, const void* k,
-                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                         int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
-                         int64_t head_dim, float scale, int causal, int64_t window, int64_t sinks,
-                         void* out, float* lse, void* stream) {
+int soup_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
+                       int64_t head_dim, float scale, int causal, void* out, float* lse,
+                       void* stream) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || seq <= 0 || heads % kv_heads != 0 ||
       batch * heads > (1 << 20) || seq > (1 << 24) || !out || !lse || !(scale > 0.f)) {
-    fn_error(fn, "bad arguments");
+    set_last_error("soup_attention_fwd: bad arguments");
     return SOUP_ERR_INVALID;
   }
   if (head_dim != kHeadDim) {
-    fn_error(fn, "head_dim must be 128");
+    set_last_error("soup_attention_fwd: head_dim must be 128");
     return SOUP_ERR_UNSUPPORTED;
   }
   if (!bhsd_ok(q, q_strides) || !bhsd_ok(k, k_strides) || !bhsd_ok(v, v_strides) ||
       !aligned16(out)) {
-    fn_error(fn, "q/k/v need 16-byte aligned bases and strides that are "
+    set_last_error("soup_attention_fwd: q/k/v need 16-byte aligned bases and strides that are "
                    "multiples of 8 elements (last dimension contiguous)");
     return SOUP_ERR_UNSUPPORTED;
   }
@@ -1630,45 +1161,51 @@ static int attention_fwd(const char* fn, const void* q, const int64_t* q_strides
   if ((rc = make_bhsd_map(&mq, q, q_strides, batch, heads, seq, "q"))) return rc;
   if ((rc = make_bhsd_map(&mk, k, k_strides, batch, kv_heads, seq, "k"))) return rc;
   if ((rc = make_bhsd_map(&mv, v, v_strides, batch, kv_heads, seq, "v"))) return rc;
-  static bool smem_set[2][64] = {};
-  auto kern = window ? attn_fwd_kernel<true> : attn_fwd_kernel<false>;
-  if ((rc = set_smem(kern, FwdSmem::kBytes, smem_set[window ? 1 : 0]))) return rc;
+  static bool smem_set[64] = {false};
+  if ((rc = set_smem(attn_fwd_kernel, FwdSmem::kBytes, smem_set))) return rc;
   AttnArgs a{(int)batch, (int)heads, (int)kv_heads, (int)seq, scale * 1.4426950408889634f,
-             causal ? 1 : 0, static_cast<bf16*>(out), lse, 0, (int)(window < seq ? window : seq),
-             (int)(sinks < seq ? sinks : seq)};
+             causal ? 1 : 0, static_cast<bf16*>(out), lse, 0};
   a.wait_ns = wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs;
   const int64_t npair = ((seq + kTile - 1) / kTile + 1) / 2;
-  return cuda_status(launch_pdl(kern, dim3((unsigned)(batch * heads * npair)),
+  return cuda_status(launch_pdl(attn_fwd_kernel, dim3((unsigned)(batch * heads * npair)),
                                 dim3(kFwdThreads), FwdSmem::kBytes, as_stream(stream), mq, mk, mv,
                                 a, err));
 }
 
-static int attention_bwd(const char* fn, const void* q, const int64_t* q_strides, const void* k,
-                         const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                         const void* out, const void* dout, const float* lse, int64_t batch,
-                         int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim, float scale,
-                         int causal, int64_t window, int64_t sinks, void* dq, void* dk, void* dv,
-                         void* workspace, size_t workspace_bytes, void* stream) {
+size_t soup_attention_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t seq) {
+  if (batch <= 0 || heads <= 0 || seq <= 0) return 0;
+  const size_t s_pad = (size_t)((seq + kTile - 1) / kTile * kTile);
+  const size_t dvec = (size_t)batch * heads * s_pad * 4;
+  const size_t part = (size_t)batch * heads * seq * kHeadDim * 4;
+  return 2 * ((dvec + 255) / 256 * 256) + 2 * ((part + 255) / 256 * 256);
+}
+
+int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
+                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                       const void* out, const void* dout, const float* lse, int64_t batch,
+                       int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim, float scale,
+                       int causal, void* dq, void* dk, void* dv, void* workspace,
+                       size_t workspace_bytes, void* stream) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || seq <= 0 || heads % kv_heads != 0 ||
       batch * heads > (1 << 20) || seq > (1 << 24) || !out || !dout || !lse || !dq || !dk || !dv ||
       !workspace || !(scale > 0.f)) {
-    fn_error(fn, "bad arguments");
+    set_last_error("soup_attention_bwd: bad arguments");
     return SOUP_ERR_INVALID;
   }
   if (head_dim != kHeadDim) {
-    fn_error(fn, "head_dim must be 128");
+    set_last_error("soup_attention_bwd: head_dim must be 128");
     return SOUP_ERR_UNSUPPORTED;
   }
   if (!bhsd_ok(q, q_strides) || !bhsd_ok(k, k_strides) || !bhsd_ok(v, v_strides) ||
       !aligned16(out) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
       !aligned16(lse)) {
-    fn_error(fn, "operands need 16-byte aligned bases and strides that are "
+    set_last_error("soup_attention_bwd: operands need 16-byte aligned bases and strides that are "
                    "multiples of 8 elements");
     return SOUP_ERR_UNSUPPORTED;
   }
   const size_t need = soup_attention_bwd_workspace_bytes(batch, heads, seq);
   if (workspace_bytes < need || !aligned16(workspace)) {
-    fn_error(fn, "workspace too small or misaligned");
+    set_last_error("soup_attention_bwd: workspace too small or misaligned");
     return SOUP_ERR_WORKSPACE;
   }
   int* err = device_err_ptr();
@@ -1693,11 +1230,9 @@ static int attention_bwd(const char* fn, const void* q, const int64_t* q_strides
   if ((rc = make_bhsd_map(&mdo, dout, do_strides, batch, heads, seq, "dout"))) return rc;
   if ((rc = make_bhsd_map(&mq64, q, q_strides, batch, heads, seq, "q", kQStep))) return rc;
   if ((rc = make_bhsd_map(&mdo64, dout, do_strides, batch, heads, seq, "dout", kQStep))) return rc;
-  static bool dkdv_set[2][64] = {}, dq_set[2][64] = {};
-  auto dkdv = window ? attn_bwd_dkdv_kernel<true> : attn_bwd_dkdv_kernel<false>;
-  auto dqk = window ? attn_bwd_dq_kernel<true> : attn_bwd_dq_kernel<false>;
-  if ((rc = set_smem(dkdv, DkvSmem::kBytes, dkdv_set[window ? 1 : 0]))) return rc;
-  if ((rc = set_smem(dqk, DqSmem::kBytes, dq_set[window ? 1 : 0]))) return rc;
+  static bool dkdv_set[64] = {false}, dq_set[64] = {false};
+  if ((rc = set_smem(attn_bwd_dkdv_kernel, DkvSmem::kBytes, dkdv_set))) return rc;
+  if ((rc = set_smem(attn_bwd_dq_kernel, DqSmem::kBytes, dq_set))) return rc;
   cudaStream_t st = as_stream(stream);
   const int B = (int)batch, H = (int)heads, Hk = (int)kv_heads, S = (int)seq;
   const int64_t rows = (int64_t)B * S * H;
@@ -1708,15 +1243,14 @@ static int attention_bwd(const char* fn, const void* q, const int64_t* q_strides
                                    static_cast<const bf16*>(out), lse, B, H, S, dvec, nl2))))
     return rc;
   BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, causal ? 1 : 0, lse, dvec, nl2,
-            dk_part, dv_part, static_cast<bf16*>(dq), 0, (int)(window < seq ? window : seq),
-            (int)(sinks < seq ? sinks : seq)};
+            dk_part, dv_part, static_cast<bf16*>(dq), 0};
   a.wait_ns = wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs;
   const int nt = (S + kTile - 1) / kTile;
-  if ((rc = cuda_status(launch_pdl(dkdv, dim3((unsigned)(B * H * nt)),
+  if ((rc = cuda_status(launch_pdl(attn_bwd_dkdv_kernel, dim3((unsigned)(B * H * nt)),
                                    dim3(kBwdThreads), DkvSmem::kBytes, st, mq64, mk, mv, mdo64, a,
                                    err))))
     return rc;
-  if ((rc = cuda_status(launch_pdl(dqk, dim3((unsigned)(B * H * nt)),
+  if ((rc = cuda_status(launch_pdl(attn_bwd_dq_kernel, dim3((unsigned)(B * H * nt)),
                                    dim3(kBwdThreads), DqSmem::kBytes, st, mq, mk, mv, mdo, a, err))))
     return rc;
   const int64_t n4 = (int64_t)B * S * Hk * (kHeadDim / 4);
@@ -1725,70 +1259,6 @@ static int attention_bwd(const char* fn, const void* q, const int64_t* q_strides
   return cuda_status(launch_pdl(attn_bwd_group_sum_kernel, dim3(blocks), dim3(256), 0, st,
                                 (const float*)dk_part, (const float*)dv_part, B, H, Hk, S,
                                 static_cast<bf16*>(dk), static_cast<bf16*>(dv)));
-}
-
-}  // namespace attn
-}  // namespace soup
-
-using namespace soup;
-using namespace soup::attn;
-
-extern "C" {
-
-int soup_attention_fwd(const void* q, const int64_t* q_strides, const void* k,
-                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                       int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
-                       int64_t head_dim, float scale, int causal, void* out, float* lse,
-                       void* stream) {
-  return attention_fwd("soup_attention_fwd", q, q_strides, k, k_strides, v, v_strides, batch, heads,
-                       kv_heads, seq, head_dim, scale, causal, 0, 0, out, lse, stream);
-}
-
-size_t soup_attention_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t seq) {
-  if (batch <= 0 || heads <= 0 || seq <= 0) return 0;
-  const size_t s_pad = (size_t)((seq + kTile - 1) / kTile * kTile);
-  const size_t dvec = (size_t)batch * heads * s_pad * 4;
-  const size_t part = (size_t)batch * heads * seq * kHeadDim * 4;
-  return 2 * ((dvec + 255) / 256 * 256) + 2 * ((part + 255) / 256 * 256);
-}
-
-int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
-                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                       const void* out, const void* dout, const float* lse, int64_t batch,
-                       int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim, float scale,
-                       int causal, void* dq, void* dk, void* dv, void* workspace,
-                       size_t workspace_bytes, void* stream) {
-  return attention_bwd("soup_attention_bwd", q, q_strides, k, k_strides, v, v_strides, out, dout, lse,
-                       batch, heads, kv_heads, seq, head_dim, scale, causal, 0, 0, dq, dk, dv,
-                       workspace, workspace_bytes, stream);
-}
-
-int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const void* k,
-                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
-                              int64_t head_dim, float scale, int64_t window, int64_t sinks,
-                              void* out, float* lse, void* stream) {
-  if (window <= 0 || sinks < 0) {
-    set_last_error("soup_attention_window_fwd: window must be positive and sinks not negative");
-    return SOUP_ERR_INVALID;
-  }
-  return attention_fwd("soup_attention_window_fwd", q, q_strides, k, k_strides, v, v_strides, batch,
-                       heads, kv_heads, seq, head_dim, scale, 1, window, sinks, out, lse, stream);
-}
-
-int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const void* k,
-                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                              const void* out, const void* dout, const float* lse, int64_t batch,
-                              int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim,
-                              float scale, int64_t window, int64_t sinks, void* dq, void* dk,
-                              void* dv, void* workspace, size_t workspace_bytes, void* stream) {
-  if (window <= 0 || sinks < 0) {
-    set_last_error("soup_attention_window_bwd: window must be positive and sinks not negative");
-    return SOUP_ERR_INVALID;
-  }
-  return attention_bwd("soup_attention_window_bwd", q, q_strides, k, k_strides, v, v_strides, out,
-                       dout, lse, batch, heads, kv_heads, seq, head_dim, scale, 1, window, sinks,
-                       dq, dk, dv, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,1462 @@
+// Causal grouped-query attention with a sliding window and sinks for sm_100a
+// (tcgen05.mma, accumulators in TMEM, operands staged by TMA), head dim 128,
+// bf16 in / fp32 accumulate: query q sees key k iff k <= q and (q - k < window or
+// k < sinks). No kernel in the reference; transformers masks SDPA for its
+// sliding-window layers.
+//
+// Key tiles without a visible pair are never loaded, so the products cover about
+// window + sinks keys a query. What then bounds the kernels is not the tensor pipe
+// but the chain TMEM read -> softmax -> P -> product of one tile, so each kernel
+// keeps sixteen compute warps (four a scheduler) on rows split over several
+// threads, and reads S out of TMEM once, into registers.
+//
+// Forward (one CTA per (batch, query head, pair of 128-query tiles A, B)): TMEM S_A,
+// S_B, O_A, O_B (128 columns each); P_X overwrites the first 64 columns of S_X as
+// bf16 pairs and is the A operand of O_X += P_X V read from TMEM. Two threads share
+// a query row (64 keys each) and exchange their row maxima through shared memory.
+// Backward: dK / dV per (batch, KV head, key tile): the CTA runs through the query
+// heads of its group and their queries in 64-query steps and keeps dK, dV in TMEM, so
+// no per-head partials reach memory; the far queries of the sink tiles, which every
+// later query sees, are cut into segments with fp32 partials summed in a fixed order.
+// dQ per (batch, query head, query tile). Both recompute P from the log-sum-exp; no
+// atomics, results are bitwise reproducible.
+//
+// Every mbarrier wait is bounded as in attention.cu: on expiry the role records a
+// code in the device error word, raises the CTA's abort flag, the producer waits
+// (bounded) for its copies, the MMA warp drains its MMAs, and the CTA frees TMEM and
+// returns. The forward's named barriers between the two warps of a row pair are
+// released by a leaving warp (bar.arrive), so no warp waits there for a warp that gave up.
+#include "attention_common.cuh"
+
+namespace soup {
+namespace attn {
+namespace {
+
+constexpr int kWarps = 16;  // compute warps
+constexpr int kThreads = 64 + 32 * kWarps;
+
+constexpr int kErrWinProducer = 0x121;
+constexpr int kErrWinMma = 0x122;
+constexpr int kErrWinSoftmax = 0x123;
+constexpr int kErrWinSmem = 0x124;
+
+// The key tiles that the queries from q0 on need, in the order the kernels take
+// them: the sink tiles before the window's first tile, then the window's tiles.
+struct KeyTiles {
+  int n_sink, lo;  // leading sink tiles; first tile of the window
+  __device__ __forceinline__ int at(int j) const { return j < n_sink ? j : lo + (j - n_sink); }
+};
+__device__ __forceinline__ KeyTiles key_tiles(int q0, int window, int sinks) {
+  KeyTiles t;
+  const int first = q0 - window + 1;
+  t.lo = first > 0 ? first / kTile : 0;
+  const int ns = (sinks + kTile - 1) / kTile;
+  t.n_sink = ns < t.lo ? ns : t.lo;
+  return t;
+}
+// Some pair of the tile of keys [k0, k0 + 128) and the queries up to q_max is
+// hidden by the window.
+__device__ __forceinline__ bool win_edge(int q_max, int k0, int window, int sinks) {
+  return q_max - k0 >= window && k0 + kTile > sinks;
+}
+// Which of 32 keys from key0 on query q sees, as bits; and which of 32 queries
+// from q0 on see key. A tile that some border crosses is masked by these words:
+// three clamped shifts a row instead of four comparisons an element (half of the
+// forward's instructions before: 101 against 85 us at 4 x 2048 tokens, 12 heads, window
+// 512), and a warp whose words are all empty skips the exponentials.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+__device__ __forceinline__ uint32_t keys_seen(int q, int key0, int S, int window, int sinks) {
+  const int end = (q + 1 < S ? q + 1 : S) - key0;
+  return low_bits(end) & (~low_bits(q - window + 1 - key0) | low_bits(sinks - key0));
+}
+__device__ __forceinline__ uint32_t queries_seeing(int key, int q0, int S, int window, int sinks) {
+  const uint32_t in = key < sinks ? 0xffffffffu : low_bits(key + window - q0);
+  return low_bits(S - q0) & ~low_bits(key - q0) & in;
+}
+// Warp-uniform: 0 no lane's word has a bit of `all`, 1 every one, 2 otherwise.
+__device__ __forceinline__ int mask_kind(uint32_t m, uint32_t all) {
+  if (__all_sync(0xffffffffu, (m & all) == 0u)) return 0;
+  return __all_sync(0xffffffffu, (m & all) == all) ? 1 : 2;
+}
+
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  __syncwarp();
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// ---- the MMA warp ----
+// The whole warp walks the schedule converged and one elected lane issues, so that
+// descriptors and addresses live in uniform registers. Issued from a lane == 0 branch
+// each product costs about 110 cycles of operand moves, more than a 128 x 64 x 16 product
+// takes (32), and the issuing thread bounded all three kernels: 3400 cycles per forward
+// step of two 64-key blocks of which the softmax needed 1900.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(v));
+  return v;
+}
+// Bounded wait of a converged warp; the result is warp-uniform.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                          int* err, int code, uint64_t wait_ns) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = bounded_wait(bar, parity, abort_flag, err, code, wait_ns);
+  return warp_ok(ok);
+}
+// An operand descriptor (128-byte swizzle) of which steps only change the address.
+struct Desc {
+  uint32_t lo, hi;
+  __device__ __forceinline__ Desc(uint64_t d)
+      : lo(static_cast<uint32_t>(d)), hi(static_cast<uint32_t>(d >> 32)) {}
+  __device__ __forceinline__ uint32_t at(uint32_t bytes) const { return lo + (bytes >> 4); }
+};
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t a_hi,
+                                       uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo,
+                                       uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(leader)
+      : "memory");
+}
+// Offsets in bytes of k-step kk (16 wide): of a K-major 128-column tile whose two
+// 64-column boxes are `box` bytes apart, and of an MN-major tile (16 rows of 128 B).
+__device__ __forceinline__ uint32_t kmajor_step(int kk, uint32_t box) {
+  return (kk >> 2) * box + (kk & 3) * 32;
+}
+__device__ __forceinline__ uint32_t mnmajor_step(int kk) { return kk * 2048; }
+
+__device__ __forceinline__ float max32(const float (&v)[32]) {
+  float mx[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) mx[u] = v[u];
+#pragma unroll
+  for (int i = 4; i < 32; i += 4) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) mx[u] = fmaxf(mx[u], v[i + u]);
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
+// This thread's O row (128 fp32 TMEM columns) times alpha (rare: kept out of line so
+// that its registers stay out of the softmax loop). Warp-collective.
+__device__ __noinline__ void rescale_o_row(uint32_t o_t, float alpha) {
+  const uint64_t al2 = f2_pack(alpha, alpha);
+#pragma unroll 1
+  for (int c = 0; c < kHeadDim / 16; ++c) {
+    uint32_t o[16];
+    tmem_ld16u(o_t + c * 16, o);
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      float o0, o1;
+      f2_unpack(f2_mul(f2_pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), al2), o0, o1);
+      o[i] = __float_as_uint(o0);
+      o[i + 1] = __float_as_uint(o1);
+    }
+    tmem_st16u(o_t + c * 16, o);
+    tmem_st_wait();
+  }
+}
+
+struct FwdArgs {
+  int B, H, Hk, S;
+  float scale_log2;  // softmax scale * log2(e)
+  int window, sinks;
+  bf16* out;   // [B, S, H, D] contiguous
+  float* lse;  // [B, H, S_pad]
+  uint64_t wait_ns;
+};
+
+// ------------------------------------------------------------- forward ----
+// One CTA per (batch, query head, pair of 128-query tiles A, B), keys in blocks of 64.
+// TMEM: two S buffers of 64 columns per query tile (A at 0 and 64, B at 128 and 192),
+// O_A at 256, O_B at 384; P of a block overwrites the first 32 columns of its own S
+// buffer as bf16 pairs and is the A operand of O += P V read from TMEM. With S
+// double buffered the products run a block ahead: the softmax finds its next S ready
+// and its chain holds no product. Shared memory: Q_A, Q_B (32 KB each), one ring of
+// 10 x 16 KB through which K and V blocks pass (K0 V0 K1 V1 ...), barriers.
+constexpr int kFwdWarps = 8;  // softmax warps: four per query tile, one row per thread
+constexpr int kFwdThreads = 64 + 32 * kFwdWarps;
+constexpr int kBlk = 64;      // keys per block
+constexpr int kRing = 10;
+struct WinFwdSmem {
+  static constexpr int kQ = 0;
+  static constexpr int kKV = kQ + 2 * kTileBytes;
+  static constexpr int kBar = kKV + kRing * kStepTile;
+  // q_full, full[10], empty[10], then per query tile and S buffer: s_full, p_full, pv_done
+  static constexpr int kNumBars = 1 + 2 * kRing + 12 + 1;
+  static constexpr int kMisc = kBar + kNumBars * 8;
+  static constexpr int kUsed = kMisc + 16;
+  static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
+};
+static_assert(WinFwdSmem::kUsed + 128 <= 232448, "window attention forward shared memory");
+
+__global__ void __launch_bounds__(kFwdThreads, 1)
+    win_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
+                   const __grid_constant__ CUtensorMap tma_v, FwdArgs a, int* err) {
+  using L = WinFwdSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  if ((uint32_t)(smem - smem_raw) + L::kUsed > dynamic_smem_bytes()) {  // grid-uniform
+    if (threadIdx.x == 0) atomicCAS(err, 0, kErrWinSmem);
+    return;
+  }
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + L::kBar;
+  const uint32_t q_full = bar0;
+  auto full = [&](int s) { return bar0 + 8u * (1 + s); };
+  auto empty = [&](int s) { return bar0 + 8u * (1 + kRing + s); };
+  constexpr int kB = 1 + 2 * kRing;
+  // of block i of query tile x: its S buffer is i & 1, the phase (i >> 1) & 1
+  auto s_full = [&](int x, int i) { return bar0 + 8u * (kB + 2 * x + (i & 1)); };
+  auto p_full = [&](int x, int i) { return bar0 + 8u * (kB + 4 + 2 * x + (i & 1)); };
+  auto pv_done = [&](int x, int i) { return bar0 + 8u * (kB + 8 + 2 * x + (i & 1)); };
+  const uint32_t drain_bar = bar0 + 8u * (kB + 12);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nq = (a.S + kTile - 1) / kTile;
+  const int nb = (a.S + kBlk - 1) / kBlk;
+  const int npair = (nq + 1) / 2;
+  const int bh = blockIdx.x % (a.B * a.H);
+  const int pr = npair - 1 - blockIdx.x / (a.B * a.H);  // late pairs first: early ones are short
+  const int b = bh / a.H, h = bh % a.H;
+  const int hk = h / (a.H / a.Hk);
+  // The pair's list of key blocks: the sinks' before the window, then from the first
+  // block that A's first row sees to B's diagonal (A's without a B). Query tile A
+  // takes entries 0 .. n_x[0] - 1; B, whose window may start `gap` blocks later,
+  // leaves those out: its i-th block is entry i, or i + gap past the sinks.
+  const int q_lo = 2 * pr * kTile - a.window + 1;
+  const int lo = q_lo > 0 ? q_lo / kBlk : 0;
+  const int lo_b = q_lo + kTile > 0 ? (q_lo + kTile) / kBlk : 0;
+  const int sink_blocks = (a.sinks + kBlk - 1) / kBlk;
+  const int ns = sink_blocks < lo ? sink_blocks : lo;
+  const bool has_b = 2 * pr + 1 < nq;
+  const int end_a = (2 * pr + 1) * 2 < nb ? (2 * pr + 1) * 2 : nb;  // one past A's diagonal block
+  const int end_b = (2 * pr + 2) * 2 < nb ? (2 * pr + 2) * 2 : nb;
+  const int gap = sink_blocks <= lo ? lo_b - lo : 0;
+  const int n = ns + (has_b ? end_b : end_a) - lo;  // entries
+  const int n_a = ns + end_a - lo;
+  const int n_b = has_b ? n - gap : 0;
+  auto block_of = [&](int j) { return j < ns ? j : lo + (j - ns); };
+  auto entry_of = [&](int x, int i) { return x && i >= ns ? i + gap : i; };
+  const uint64_t wait_ns = a.wait_ns;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kNumBars; ++i) {
+      const int e = i - (kB + 4);
+      // the four softmax warps of a query tile arrive once each on its p_full
+      mbar_init(bar0 + 8u * i, e >= 0 && e < 4 ? kFwdWarps / 2 : 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc::tma_prefetch_desc(&tma_q);
+    tc::tma_prefetch_desc(&tma_k);
+    tc::tma_prefetch_desc(&tma_v);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_holder)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer ----
+      const int nqt = has_b ? 2 : 1;
+      mbar_arrive_expect_tx(q_full, nqt * kTileBytes);
+      for (int x = 0; x < nqt; ++x) {
+        const uint32_t qd = sbase + L::kQ + x * kTileBytes;
+        tma_load_4d(qd, &tma_q, q_full, 0, (2 * pr + x) * kTile, h, b);
+        tma_load_4d(qd + kBox, &tma_q, q_full, 64, (2 * pr + x) * kTile, h, b);
+      }
+      int issued = 0;
+      for (int i = 0; i < 2 * n; ++i) {  // K of entry j is load 2 j, V load 2 j + 1
+        const int st = i % kRing;
+        if (!bounded_wait(empty(st), ((i / kRing) & 1) ^ 1, abort_flag, err, kErrWinProducer, wait_ns))
+          break;
+        const int key0 = block_of(i >> 1) * kBlk;
+        const CUtensorMap* map = (i & 1) ? &tma_v : &tma_k;
+        const uint32_t d = sbase + L::kKV + st * kStepTile;
+        mbar_arrive_expect_tx(full(st), kStepTile);
+        tma_load_4d(d, map, full(st), 0, key0, hk, b);
+        tma_load_4d(d + kStepBox, map, full(st), 64, key0, hk, b);
+        ++issued;
+      }
+      // let every issued copy land before the CTA may leave (bounded)
+      uint64_t t0 = tc::globaltimer();
+      while (!mbar_try_wait(q_full, 0) && tc::globaltimer() - t0 < wait_ns) {
+      }
+      for (int i = issued > kRing ? issued - kRing : 0; i < issued; ++i) {
+        t0 = tc::globaltimer();
+        while (!mbar_try_wait(full(i % kRing), (i / kRing) & 1) && tc::globaltimer() - t0 < wait_ns) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------- MMA issuer ----
+    // S of blocks 0 and 1 of both query tiles, then per block i: P V of A, S_A(i + 2)
+    // into the buffer that this product has read P from (MMAs run in issue order),
+    // and the same for B. An entry's K and V are released by its last reader: B,
+    // which comes second, unless B runs ahead of A (a gap) or does not use it.
+    const uint32_t leader = elect_one();
+    auto wait = [&](uint32_t bar, int parity) {
+      return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
+    };
+    bool ok = wait(q_full, 0);
+    bool issued = false;
+    auto last_reader = [&](int j) {
+      if (!has_b || (j >= ns && j < ns + gap)) return 0;
+      if (j >= n_a) return 1;
+      return j >= ns && gap > 0 ? 0 : 1;
+    };
+    const Desc q_desc(smem_desc_sw128(sbase + L::kQ, 16, 1024));
+    const Desc k_desc(smem_desc_sw128(sbase + L::kKV, 16, 1024));
+    const Desc v_desc(smem_desc_sw128(sbase + L::kKV, kStepBox, 1024));
+    auto issue_s = [&](int x, int i) -> bool {
+      const int j = entry_of(x, i);
+      const int st = (2 * j) % kRing;
+      if (!wait(full(st), (2 * j / kRing) & 1)) return false;
+      tc_fence_after();
+      const uint32_t d = tmem + x * 128 + (i & 1) * 64;
+#pragma unroll
+      for (int kk = 0; kk < kHeadDim / 16; ++kk)
+        mma_ss(leader, d, q_desc.at(x * kTileBytes + kmajor_step(kk, kBox)), q_desc.hi,
+               k_desc.at(st * kStepTile + kmajor_step(kk, kStepBox)), k_desc.hi, kIdescKK64,
+               kk > 0 ? 1u : 0u);
+      commit(leader, s_full(x, i));
+      if (last_reader(j) == x) commit(leader, empty(st));
+      issued = true;
+      return true;
+    };
+    auto issue_pv = [&](int x, int i) -> bool {
+      const int j = entry_of(x, i);
+      const int st = (2 * j + 1) % kRing;
+      if (!wait(full(st), ((2 * j + 1) / kRing) & 1)) return false;
+      if (!wait(p_full(x, i), (i >> 1) & 1)) return false;
+      tc_fence_after();
+      const uint32_t p = tmem + x * 128 + (i & 1) * 64;
+#pragma unroll
+      for (int kk = 0; kk < kBlk / 16; ++kk)
+        mma_ts(leader, tmem + 256 + x * 128, p + kk * 8, v_desc.at(st * kStepTile + mnmajor_step(kk)),
+               v_desc.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
+      commit(leader, pv_done(x, i));
+      if (last_reader(j) == x) commit(leader, empty(st));
+      return true;
+    };
+    for (int i = 0; i < 2 && ok; ++i) {
+      if (i < n_a) ok = issue_s(0, i);
+      if (ok && i < n_b) ok = issue_s(1, i);
+    }
+    for (int i = 0; (i < n_a || i < n_b) && ok; ++i) {
+      if (i < n_a) ok = issue_pv(0, i);
+      if (ok && i + 2 < n_a) ok = issue_s(0, i + 2);
+      if (ok && i < n_b) ok = issue_pv(1, i);
+      if (ok && i + 2 < n_b) ok = issue_s(1, i + 2);
+    }
+    if (!ok && issued) {
+      commit(leader, drain_bar);
+      uint64_t t0 = tc::globaltimer();
+      while (!mbar_try_wait(drain_bar, 0) && tc::globaltimer() - t0 < wait_ns) {
+      }
+    }
+  } else {
+    // ------------------------------------------------------- softmax ----
+    const int x = (warp - 2) >> 2;             // query tile A (0) or B (1)
+    const int quarter = warp & 3;              // TMEM lanes this warp may access
+    const int qt = 2 * pr + x;
+    const int q = qt * kTile + quarter * 32 + lane;  // query row of this thread
+    const int n_x = x ? n_b : n_a;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t s_base = tmem + x * 128 + lane_off;
+    const uint32_t o_t = tmem + 256 + x * 128 + lane_off;
+    const uint64_t sl2 = f2_pack(a.scale_log2, a.scale_log2);
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < n_x; ++i) {
+      bool w = true;
+      if (lane == 0)
+        w = bounded_wait(s_full(x, i), (i >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      if (!(ok = warp_ok(w))) break;
+      tc_fence_after();
+      const uint32_t s_t = s_base + (i & 1) * 64;
+      float s0[32], s1[32];
+      tmem_ld32_async(s_t, s0);
+      tmem_ld32_async(s_t + 32, s1);
+      const int k0 = block_of(entry_of(x, i)) * kBlk;
+      const bool edge = k0 + kBlk > a.S || k0 + kBlk > qt * kTile + 1 ||
+                        (qt * kTile + kTile - 1 - k0 >= a.window && k0 + kBlk > a.sinks);
+      int kind0 = 1, kind1 = 1;
+      uint32_t mk0 = 0xffffffffu, mk1 = 0xffffffffu;
+      if (edge) {
+        mk0 = keys_seen(q, k0, a.S, a.window, a.sinks);
+        mk1 = keys_seen(q, k0 + 32, a.S, a.window, a.sinks);
+        kind0 = mask_kind(mk0, 0xffffffffu);
+        kind1 = mask_kind(mk1, 0xffffffffu);
+      }
+      tmem_ld_wait();
+      if (kind0 == 2) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!(mk0 & (1u << e))) s0[e] = -INFINITY;
+      }
+      if (kind1 == 2) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!(mk1 & (1u << e))) s1[e] = -INFINITY;
+      }
+      const float mt = fmaxf(kind0 ? max32(s0) : -INFINITY, kind1 ? max32(s1) : -INFINITY) *
+                       a.scale_log2;
+      bool rescale = false;
+      float alpha = 1.f;
+      if (mt > m_used + 8.f) {  // also when m_used is still -inf
+        alpha = fast_exp2(m_used - mt);
+        m_used = mt;
+        rescale = true;
+      }
+      if (i > 0 && __any_sync(0xffffffffu, rescale)) {
+        // O is stable once P V (i - 1) is done (S(i) came before it; P V (i - 2) before S(i))
+        if (lane == 0)
+          w = bounded_wait(pv_done(x, i - 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax,
+                           wait_ns);
+        if (!(ok = warp_ok(w))) break;
+        tc_fence_after();
+        rescale_o_row(o_t, alpha);
+      }
+      // a row whose keys are all hidden so far: exp2(-inf - 0) = 0 instead of NaN
+      const float nm = m_used == -INFINITY ? 0.f : -m_used;
+      const uint64_t nm2 = f2_pack(nm, nm);
+      uint64_t sm2[4] = {0, 0, 0, 0};
+      uint32_t pw[32];
+      auto exps = [&](const float (&v)[32], int kind, int w0) {
+        if (kind == 0) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pw[w0 + e] = 0u;
+          return;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(v[e], v[e + 1]), sl2, nm2), x0, x1);
+          x0 = fast_exp2(x0);
+          x1 = fast_exp2(x1);
+          sm2[(e >> 1) & 3] = f2_add(sm2[(e >> 1) & 3], f2_pack(x0, x1));
+          pw[w0 + (e >> 1)] = pack_bf16(x0, x1);
+        }
+      };
+      exps(s0, kind0, 0);
+      exps(s1, kind1, 16);
+      tmem_st32u(s_t, pw);
+      float t0, t1, t2, t3;
+      f2_unpack(f2_add(sm2[0], sm2[1]), t0, t1);
+      f2_unpack(f2_add(sm2[2], sm2[3]), t2, t3);
+      const float sum = (t0 + t1) + (t2 + t3);
+      l = rescale ? l * alpha + sum : l + sum;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(x, i));
+    }
+    if (ok && n_x > 0) {
+      bool w = true;
+      if (lane == 0)
+        w = bounded_wait(pv_done(x, n_x - 1), ((n_x - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax,
+                         wait_ns);
+      ok = warp_ok(w);
+    }
+    if (ok && n_x > 0) {
+      tc_fence_after();
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      bf16* orow = a.out + ((int64_t)b * a.S + q) * (int64_t)(a.H * kHeadDim) + h * kHeadDim;
+#pragma unroll
+      for (int c = 0; c < kHeadDim / 32; ++c) {
+        float o[32];
+        tmem_ld32(o_t + c * 32, o);
+        if (q < a.S) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint4*>(orow + c * 32 + 8 * g) =
+                make_uint4(pack_bf16(o[8 * g] * inv, o[8 * g + 1] * inv),
+                           pack_bf16(o[8 * g + 2] * inv, o[8 * g + 3] * inv),
+                           pack_bf16(o[8 * g + 4] * inv, o[8 * g + 5] * inv),
+                           pack_bf16(o[8 * g + 6] * inv, o[8 * g + 7] * inv));
+        }
+      }
+      if (q < a.S)
+        a.lse[((int64_t)b * a.H + h) * ((int64_t)nq * kTile) + q] = (m_used + __log2f(l)) * kLn2;
+    }
+  }
+
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+}
+
+// ------------------------------------------------------------ backward ----
+struct BwdArgs {
+  int B, H, Hk, S;
+  float scale;       // softmax scale (applied to dK, dQ in fp32)
+  float scale_log2;  // scale * log2(e)
+  int window, sinks;
+  const float* Dv;   // [B, H, S_pad] dO . O
+  const float* nl2;  // [B, H, S_pad] -lse * log2(e)
+  bf16* dq;          // [B, S, H, D]
+  bf16* dk;          // [B, S, Hk, D]
+  bf16* dv;
+  float* part;       // fp32 partials, one slot of dK, dV [2][128][D] per entry
+  int groups;        // parts that a KV head's query heads are split into
+  int heads_per;     // query heads per part
+  int n_sink;        // sink tiles
+  int segs, seg_steps;  // segments of a sink tile's steps, and their length
+  uint64_t wait_ns;
+};
+
+// One unit of dK / dV work: a key tile, a range of 64-query steps, query heads
+// [h0, h0 + nh), and the slot its sums go to (-1: straight to dk, dv).
+struct DkvUnit {
+  int b, hk, kt, h0, nh, step0, n, slot;
+};
+__host__ __device__ __forceinline__ int dkv_sink_units(const BwdArgs& a) {
+  return a.B * a.Hk * a.n_sink * a.groups * a.segs;
+}
+__device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
+  DkvUnit u;
+  const int nq64 = (a.S + kQStep - 1) / kQStep;
+  const int n_sink_units = dkv_sink_units(a);
+  const int rep = a.H / a.Hk;
+  int g, bhk;
+  if (i < n_sink_units) {
+    u.slot = i;
+    const int seg = i % a.segs;
+    i /= a.segs;
+    g = i % a.groups;
+    i /= a.groups;
+    u.kt = i % a.n_sink;
+    bhk = i / a.n_sink;
+    const int first = u.kt * (kTile / kQStep);
+    u.step0 = first + seg * a.seg_steps;
+    const int end = u.step0 + a.seg_steps < nq64 ? u.step0 + a.seg_steps : nq64;
+    u.n = end > u.step0 ? end - u.step0 : 0;
+  } else {
+    i -= n_sink_units;
+    u.slot = a.groups > 1 ? n_sink_units + i : -1;
+    g = i % a.groups;
+    i /= a.groups;
+    bhk = i % (a.B * a.Hk);
+    u.kt = a.n_sink + i / (a.B * a.Hk);
+    u.step0 = u.kt * (kTile / kQStep);
+    // the last query that sees a key of this tile
+    const int last = (u.kt * kTile + kTile - 1 + a.window - 1) / kQStep;
+    u.n = (last < nq64 - 1 ? last : nq64 - 1) - u.step0 + 1;
+  }
+  u.b = bhk / a.Hk;
+  u.hk = bhk % a.Hk;
+  u.h0 = u.hk * rep + g * a.heads_per;
+  const int h1 = (u.hk + 1) * rep;
+  u.nh = u.h0 + a.heads_per < h1 ? a.heads_per : h1 - u.h0;
+  if (u.nh < 0) u.nh = 0;
+  return u;
+}
+
+// dK / dV of one unit. TMEM: S^T and dP^T (128 keys x 64 queries) double buffered
+// (buffer i: S^T at column 128 i, dP^T at 128 i + 64), dV at 256, dK at 384. Shared
+// memory: K, V (32 KB each, loaded once for all query heads), a ring of 3 stages of
+// 64-query (Q, dO) tiles with their nl2 / D vectors, P^T and dS^T (16 KB each). A
+// compute thread owns 16 queries of one key row of each step.
+constexpr int kDkvRing = 3;
+struct WinDkvSmem {
+  static constexpr int kK = 0;
+  static constexpr int kV = kK + kTileBytes;
+  static constexpr int kQD = kV + kTileBytes;  // stage s: Q at +0, dO at +kStepTile
+  static constexpr int kP = kQD + kDkvRing * 2 * kStepTile;
+  static constexpr int kDS = kP + kPTBytes;
+  static constexpr int kVec = kDS + kPTBytes;  // stage s: nl2, D of its 64 queries (2 x 256 B)
+  static constexpr int kBar = kVec + kDkvRing * 2 * kQStep * 4;
+  // kv_full, full[3], empty[3], st_full[2], st_empty[2], p_full, p_free, ds_full, ds_free,
+  // acc_done, drain
+  static constexpr int kNumBars = 1 + 2 * kDkvRing + 4 + 6;
+  static constexpr int kMisc = kBar + kNumBars * 8;
+  static constexpr int kUsed = kMisc + 16;
+  static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
+};
+static_assert(WinDkvSmem::kUsed + 128 <= 232448, "window attention dK/dV shared memory");
+
+__global__ void __launch_bounds__(kThreads, 1)
+    win_dkdv_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
+                    const __grid_constant__ CUtensorMap tma_v,
+                    const __grid_constant__ CUtensorMap tma_do, BwdArgs a, int* err) {
+  using L = WinDkvSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  if ((uint32_t)(smem - smem_raw) + L::kUsed > dynamic_smem_bytes()) {  // grid-uniform
+    if (threadIdx.x == 0) atomicCAS(err, 0, kErrWinSmem);
+    return;
+  }
+  const DkvUnit u = dkv_unit(a, blockIdx.x);
+  const int total = u.nh * u.n;  // steps of all this unit's query heads
+  if (total == 0) return;        // an empty segment (its slot is not read)
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + L::kBar;
+  const uint32_t kv_full = bar0;
+  auto full = [&](int st) { return bar0 + 8u * (1 + st); };
+  auto empty = [&](int st) { return bar0 + 8u * (1 + kDkvRing + st); };
+  constexpr int kB = 1 + 2 * kDkvRing;
+  auto st_full = [&](int bb) { return bar0 + 8u * (kB + bb); };
+  auto st_empty = [&](int bb) { return bar0 + 8u * (kB + 2 + bb); };
+  const uint32_t p_full = bar0 + 8u * (kB + 4), p_free = bar0 + 8u * (kB + 5);
+  const uint32_t ds_full = bar0 + 8u * (kB + 6), ds_free = bar0 + 8u * (kB + 7);
+  const uint32_t acc_done = bar0 + 8u * (kB + 8), drain_bar = bar0 + 8u * (kB + 9);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int k0 = u.kt * kTile;
+  const int64_t s_pad = ((int64_t)a.S + kTile - 1) / kTile * kTile;
+  const uint64_t wait_ns = a.wait_ns;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kNumBars; ++i) {
+      const uint32_t bar = bar0 + 8u * i;
+      const bool per_warp = bar == st_empty(0) || bar == st_empty(1) || bar == p_full || bar == ds_full;
+      mbar_init(bar, per_warp ? kWarps : 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc::tma_prefetch_desc(&tma_q);
+    tc::tma_prefetch_desc(&tma_k);
+    tc::tma_prefetch_desc(&tma_v);
+    tc::tma_prefetch_desc(&tma_do);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_holder)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer ----
+      mbar_arrive_expect_tx(kv_full, 2 * kTileBytes);
+      tma_load_4d(sbase + L::kK, &tma_k, kv_full, 0, k0, u.hk, u.b);
+      tma_load_4d(sbase + L::kK + kBox, &tma_k, kv_full, 64, k0, u.hk, u.b);
+      tma_load_4d(sbase + L::kV, &tma_v, kv_full, 0, k0, u.hk, u.b);
+      tma_load_4d(sbase + L::kV + kBox, &tma_v, kv_full, 64, k0, u.hk, u.b);
+      int issued = 0, h = u.h0, step = u.step0;
+      for (int i = 0; i < total; ++i) {
+        const int st = i % kDkvRing;
+        if (!bounded_wait(empty(st), ((i / kDkvRing) & 1) ^ 1, abort_flag, err, kErrWinProducer,
+                          wait_ns))
+          break;
+        const int q0 = step * kQStep;
+        const uint32_t qd = sbase + L::kQD + st * 2 * kStepTile;
+        const int64_t vrow = ((int64_t)u.b * a.H + h) * s_pad + q0;
+        const uint32_t vd = sbase + L::kVec + st * 2 * kQStep * 4;
+        mbar_arrive_expect_tx(full(st), 2 * kStepTile + 2 * kQStep * 4);
+        tma_load_4d(qd, &tma_q, full(st), 0, q0, h, u.b);
+        tma_load_4d(qd + kStepBox, &tma_q, full(st), 64, q0, h, u.b);
+        tma_load_4d(qd + kStepTile, &tma_do, full(st), 0, q0, h, u.b);
+        tma_load_4d(qd + kStepTile + kStepBox, &tma_do, full(st), 64, q0, h, u.b);
+        bulk_load(vd, a.nl2 + vrow, kQStep * 4, full(st));
+        bulk_load(vd + kQStep * 4, a.Dv + vrow, kQStep * 4, full(st));
+        ++issued;
+        if (++step == u.step0 + u.n) {
+          step = u.step0;
+          ++h;
+        }
+      }
+      uint64_t t0 = tc::globaltimer();
+      while (!mbar_try_wait(kv_full, 0) && tc::globaltimer() - t0 < wait_ns) {
+      }
+      for (int i = issued > kDkvRing ? issued - kDkvRing : 0; i < issued; ++i) {
+        t0 = tc::globaltimer();
+        while (!mbar_try_wait(full(i % kDkvRing), (i / kDkvRing) & 1) &&
+               tc::globaltimer() - t0 < wait_ns) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------- MMA issuer ----
+    const uint32_t leader = elect_one();
+    auto wait = [&](uint32_t bar, int parity) {
+      return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
+    };
+    bool ok = wait(kv_full, 0);
+    bool issued = false;
+    const Desc k_desc(smem_desc_sw128(sbase + L::kK, 16, 1024));
+    const Desc v_desc(smem_desc_sw128(sbase + L::kV, 16, 1024));
+    const Desc qd_desc(smem_desc_sw128(sbase + L::kQD, 16, 1024));      // as K-major operands
+    const Desc qd_mn(smem_desc_sw128(sbase + L::kQD, kStepBox, 1024));  // as MN-major operands
+    const Desc p_desc(smem_desc_sw128(sbase + L::kP, 16, 1024));
+    const Desc ds_desc(smem_desc_sw128(sbase + L::kDS, 16, 1024));
+    auto issue_sd = [&](int i) -> bool {
+      const int st = i % kDkvRing, bb = i & 1;
+      if (!wait(full(st), (i / kDkvRing) & 1)) return false;
+      if (i >= 2 && !wait(st_empty(bb), ((i >> 1) & 1) ^ 1)) return false;
+      tc_fence_after();
+      const uint32_t q_off = st * 2 * kStepTile;
+#pragma unroll
+      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // S^T = K Q^T
+        mma_ss(leader, tmem + bb * 128, k_desc.at(kmajor_step(kk, kBox)), k_desc.hi,
+               qd_desc.at(q_off + kmajor_step(kk, kStepBox)), qd_desc.hi, kIdescKK64, kk > 0 ? 1u : 0u);
+#pragma unroll
+      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // dP^T = V dO^T
+        mma_ss(leader, tmem + bb * 128 + 64, v_desc.at(kmajor_step(kk, kBox)), v_desc.hi,
+               qd_desc.at(q_off + kStepTile + kmajor_step(kk, kStepBox)), qd_desc.hi, kIdescKK64,
+               kk > 0 ? 1u : 0u);
+      commit(leader, st_full(bb));
+      issued = true;
+      return true;
+    };
+    if (ok) ok = issue_sd(0);
+    if (ok && total > 1) ok = issue_sd(1);
+    for (int i = 0; i < total && ok; ++i) {
+      const int st = i % kDkvRing;
+      const uint32_t q_off = st * 2 * kStepTile;
+      if (!(ok = wait(p_full, i & 1))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < kQStep / 16; ++kk)  // dV += P^T dO
+        mma_ss(leader, tmem + 256, p_desc.at(kk * 32), p_desc.hi,
+               qd_mn.at(q_off + kStepTile + mnmajor_step(kk)), qd_mn.hi, kIdescKM,
+               (i > 0 || kk > 0) ? 1u : 0u);
+      commit(leader, p_free);
+      if (!(ok = wait(ds_full, i & 1))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < kQStep / 16; ++kk)  // dK += dS^T Q
+        mma_ss(leader, tmem + 384, ds_desc.at(kk * 32), ds_desc.hi, qd_mn.at(q_off + mnmajor_step(kk)),
+               qd_mn.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
+      commit(leader, ds_free);
+      commit(leader, empty(st));
+      if (i + 2 < total && !(ok = issue_sd(i + 2))) break;
+    }
+    if (ok) commit(leader, acc_done);
+    if (!ok && issued) {
+      commit(leader, drain_bar);
+      uint64_t t0 = tc::globaltimer();
+      while (!mbar_try_wait(drain_bar, 0) && tc::globaltimer() - t0 < wait_ns) {
+      }
+    }
+  } else {
+    // ------------------------------------------------------- compute ----
+    const int quarter = warp & 3;
+    const int part = (warp - 2) >> 2;   // queries [16 part, 16 part + 16) of each step
+    const int cb = part * 16;
+    const int r = quarter * 32 + lane;  // key row of this thread
+    const int key = k0 + r;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    uint8_t* pbox = smem + L::kP;
+    uint8_t* dsbox = smem + L::kDS;
+    const uint64_t sl2 = f2_pack(a.scale_log2, a.scale_log2);
+    bool ok = true;
+    int step = u.step0;
+    for (int i = 0; i < total; ++i) {
+      const int st = i % kDkvRing, bb = i & 1;
+      const int qs = step * kQStep;
+      if (++step == u.step0 + u.n) step = u.step0;
+      bool w = true;
+      if (lane == 0) w = bounded_wait(st_full(bb), (i >> 1) & 1, abort_flag, err, kErrWinSoftmax,
+                                      wait_ns);
+      if (!(ok = warp_ok(w))) break;
+      tc_fence_after();
+      float sv[16], dp[16];
+      tmem_ld16_async(tmem + bb * 128 + cb + lane_off, sv);
+      tmem_ld16_async(tmem + bb * 128 + 64 + cb + lane_off, dp);
+      const bool edge = qs + kQStep > a.S || qs < k0 + kTile ||
+                        win_edge(qs + kQStep - 1, k0, a.window, a.sinks);
+      uint32_t mk = 0xffffu;
+      int kind = 1;
+      if (edge) {
+        mk = queries_seeing(key, qs + cb, a.S, a.window, a.sinks);
+        kind = mask_kind(mk, 0xffffu);
+      }
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(st_empty(bb));  // the step after next may overwrite them
+      const float* vnl = reinterpret_cast<const float*>(smem + L::kVec + st * 2 * kQStep * 4) + cb;
+      const float* vD = vnl + kQStep;
+      uint32_t pw[8], dw[8];
+      if (kind == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pw[e] = dw[e] = 0u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 nl = *reinterpret_cast<const float4*>(vnl + e);
+          const float4 dd = *reinterpret_cast<const float4*>(vD + e);
+          float p[4], d[4];
+          f2_unpack(f2_fma(f2_pack(sv[e], sv[e + 1]), sl2, f2_pack(nl.x, nl.y)), p[0], p[1]);
+          f2_unpack(f2_fma(f2_pack(sv[e + 2], sv[e + 3]), sl2, f2_pack(nl.z, nl.w)), p[2], p[3]);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) p[v] = fast_exp2(p[v]);
+          const uint64_t t0 = f2_add(f2_pack(dp[e], dp[e + 1]), f2_pack(-dd.x, -dd.y));
+          const uint64_t t1 = f2_add(f2_pack(dp[e + 2], dp[e + 3]), f2_pack(-dd.z, -dd.w));
+          f2_unpack(f2_mul(f2_pack(p[0], p[1]), t0), d[0], d[1]);
+          f2_unpack(f2_mul(f2_pack(p[2], p[3]), t1), d[2], d[3]);
+          if (kind == 2) {  // hidden and padding rows may hold anything: select, do not scale
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (!(mk & (1u << (e + v)))) p[v] = d[v] = 0.f;
+          }
+          pw[e >> 1] = pack_bf16(p[0], p[1]);
+          pw[(e >> 1) + 1] = pack_bf16(p[2], p[3]);
+          dw[e >> 1] = pack_bf16(d[0], d[1]);
+          dw[(e >> 1) + 1] = pack_bf16(d[2], d[3]);
+        }
+      }
+      if (i > 0) {  // the previous step's dV product has read P^T
+        if (lane == 0) w = bounded_wait(p_free, (i - 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+        if (!(ok = warp_ok(w))) break;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<uint4*>(pbox + swz_off(r, part * 2 + c)) =
+            make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]);
+      tc::fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+      if (i > 0) {  // the previous step's dK product has read dS^T
+        if (lane == 0) w = bounded_wait(ds_free, (i - 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+        if (!(ok = warp_ok(w))) break;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<uint4*>(dsbox + swz_off(r, part * 2 + c)) =
+            make_uint4(dw[4 * c], dw[4 * c + 1], dw[4 * c + 2], dw[4 * c + 3]);
+      tc::fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    if (ok) {
+      bool w = true;
+      if (lane == 0) w = bounded_wait(acc_done, 0, abort_flag, err, kErrWinSoftmax, wait_ns);
+      ok = warp_ok(w);
+    }
+    if (ok) {
+      tc_fence_after();
+      const int db = part * 32;  // this warp's 32 of the 128 head dims
+      float v[32], g[32];
+      tmem_ld32_async(tmem + 256 + db + lane_off, v);
+      tmem_ld32_async(tmem + 384 + db + lane_off, g);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 32; ++e) g[e] *= a.scale;
+      if (key < a.S) {
+        if (u.slot >= 0) {
+          float* pk = a.part + ((int64_t)u.slot * 2 * kTile + r) * kHeadDim + db;
+          float* pv = pk + (int64_t)kTile * kHeadDim;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            *reinterpret_cast<float4*>(pk + e) = make_float4(g[e], g[e + 1], g[e + 2], g[e + 3]);
+            *reinterpret_cast<float4*>(pv + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+        } else {
+          const int64_t o = (((int64_t)u.b * a.S + key) * a.Hk + u.hk) * kHeadDim + db;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            *reinterpret_cast<uint4*>(a.dk + o + e) =
+                make_uint4(pack_bf16(g[e], g[e + 1]), pack_bf16(g[e + 2], g[e + 3]),
+                           pack_bf16(g[e + 4], g[e + 5]), pack_bf16(g[e + 6], g[e + 7]));
+            *reinterpret_cast<uint4*>(a.dv + o + e) =
+                make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]),
+                           pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
+          }
+        }
+      }
+    }
+  }
+
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+}
+
+// dk, dv of the key tiles whose sums are in slots: the sink tiles, and with groups > 1
+// all tiles. Slots are added in a fixed order. Four elements per thread; one block
+// takes 8 key rows of one tile.
+__global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles) {
+  pdl_wait();
+  pdl_trigger();
+  const int nq64 = (a.S + kQStep - 1) / kQStep;
+  const int rows8 = blockIdx.x % (kTile / 8);
+  const int i = blockIdx.x / (kTile / 8);
+  const int kt = i % tiles, bhk = i / tiles;
+  const int r = rows8 * 8 + (threadIdx.x >> 5);
+  const int key = kt * kTile + r;
+  if (key >= a.S) return;
+  int slot0, n;
+  int segs = 1;
+  if (kt < a.n_sink) {
+    slot0 = (bhk * a.n_sink + kt) * a.groups * a.segs;
+    n = a.groups * a.segs;
+    const int steps = nq64 - kt * (kTile / kQStep);
+    segs = (steps + a.seg_steps - 1) / a.seg_steps;  // of a.segs, the others are empty
+  } else {
+    slot0 = dkv_sink_units(a) + ((kt - a.n_sink) * a.B * a.Hk + bhk) * a.groups;
+    n = a.groups;
+  }
+  const int d = (threadIdx.x & 31) * 4;
+  float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+  const int rep = a.H / a.Hk;
+  for (int s = 0; s < n; ++s) {
+    const int g = kt < a.n_sink ? s / a.segs : s;
+    if (g * a.heads_per >= rep || (kt < a.n_sink && s % a.segs >= segs)) continue;
+    const float* p = a.part + ((int64_t)(slot0 + s) * 2 * kTile + r) * kHeadDim + d;
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    const float4 y = *reinterpret_cast<const float4*>(p + kTile * kHeadDim);
+    k.x += x.x; k.y += x.y; k.z += x.z; k.w += x.w;
+    v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+  }
+  const int64_t o = (((int64_t)(bhk / a.Hk) * a.S + key) * a.Hk + bhk % a.Hk) * kHeadDim + d;
+  *reinterpret_cast<uint2*>(a.dk + o) = make_uint2(pack_bf16(k.x, k.y), pack_bf16(k.z, k.w));
+  *reinterpret_cast<uint2*>(a.dv + o) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
+// dQ of one query tile: TMEM columns S 0, dP 128, dQ 256, dS 384 (bf16, two per
+// column: the A operand of dQ += dS K read from TMEM). Shared memory: Q and dO
+// (32 KB each, loaded once), a K ring (3 x 32 KB; a stage frees after its dQ
+// product) and a V ring (2 x 32 KB; a stage frees after its dP product). A compute
+// thread owns 32 keys of one query row of each tile.
+constexpr int kDqKStages = 3;
+constexpr int kDqVStages = 2;
+struct WinDqSmem {
+  static constexpr int kQ = 0;
+  static constexpr int kDO = kQ + kTileBytes;
+  static constexpr int kK = kDO + kTileBytes;
+  static constexpr int kV = kK + kDqKStages * kTileBytes;
+  static constexpr int kBar = kV + kDqVStages * kTileBytes;
+  // qdo_full, k_full[3], k_empty[3], v_full[2], v_empty[2], st_full, st_empty, ds_full,
+  // buf_free, acc_done, drain
+  static constexpr int kNumBars = 1 + 2 * kDqKStages + 2 * kDqVStages + 6;
+  static constexpr int kMisc = kBar + kNumBars * 8;
+  static constexpr int kUsed = kMisc + 16;
+  static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
+};
+static_assert(WinDqSmem::kUsed + 128 <= 232448, "window attention dQ shared memory");
+
+__global__ void __launch_bounds__(kThreads, 1)
+    win_dq_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
+                  const __grid_constant__ CUtensorMap tma_v,
+                  const __grid_constant__ CUtensorMap tma_do, BwdArgs a, int* err) {
+  using L = WinDqSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  if ((uint32_t)(smem - smem_raw) + L::kUsed > dynamic_smem_bytes()) {  // grid-uniform
+    if (threadIdx.x == 0) atomicCAS(err, 0, kErrWinSmem);
+    return;
+  }
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + L::kBar;
+  const uint32_t qdo_full = bar0;
+  auto k_full = [&](int st) { return bar0 + 8u * (1 + st); };
+  auto k_empty = [&](int st) { return bar0 + 8u * (1 + kDqKStages + st); };
+  auto v_full = [&](int st) { return bar0 + 8u * (1 + 2 * kDqKStages + st); };
+  auto v_empty = [&](int st) { return bar0 + 8u * (1 + 2 * kDqKStages + kDqVStages + st); };
+  constexpr int kB = 1 + 2 * kDqKStages + 2 * kDqVStages;
+  const uint32_t st_full = bar0 + 8u * kB, st_empty = bar0 + 8u * (kB + 1);
+  const uint32_t ds_full = bar0 + 8u * (kB + 2), buf_free = bar0 + 8u * (kB + 3);
+  const uint32_t acc_done = bar0 + 8u * (kB + 4), drain_bar = bar0 + 8u * (kB + 5);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nq = (a.S + kTile - 1) / kTile;
+  const int bh = blockIdx.x % (a.B * a.H);
+  const int qt = nq - 1 - blockIdx.x / (a.B * a.H);  // late query tiles first
+  const int b = bh / a.H, h = bh % a.H;
+  const int hk = h / (a.H / a.Hk);
+  const int q0 = qt * kTile;
+  const KeyTiles kt = key_tiles(q0, a.window, a.sinks);
+  const int n = kt.n_sink + (qt + 1 - kt.lo);
+  const uint64_t wait_ns = a.wait_ns;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kNumBars; ++i) {
+      const uint32_t bar = bar0 + 8u * i;
+      mbar_init(bar, bar == st_empty || bar == ds_full ? kWarps : 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc::tma_prefetch_desc(&tma_q);
+    tc::tma_prefetch_desc(&tma_k);
+    tc::tma_prefetch_desc(&tma_v);
+    tc::tma_prefetch_desc(&tma_do);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_holder)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  pdl_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ------------------------------------------------ TMA producer ----
+      mbar_arrive_expect_tx(qdo_full, 2 * kTileBytes);
+      tma_load_4d(sbase + L::kQ, &tma_q, qdo_full, 0, q0, h, b);
+      tma_load_4d(sbase + L::kQ + kBox, &tma_q, qdo_full, 64, q0, h, b);
+      tma_load_4d(sbase + L::kDO, &tma_do, qdo_full, 0, q0, h, b);
+      tma_load_4d(sbase + L::kDO + kBox, &tma_do, qdo_full, 64, q0, h, b);
+      int issued_k = 0, issued_v = 0;
+      for (int j = 0; j < n; ++j) {
+        const int sk = j % kDqKStages, sv = j % kDqVStages;
+        const int key0 = kt.at(j) * kTile;
+        if (!bounded_wait(k_empty(sk), ((j / kDqKStages) & 1) ^ 1, abort_flag, err, kErrWinProducer,
+                          wait_ns))
+          break;
+        const uint32_t kd = sbase + L::kK + sk * kTileBytes;
+        mbar_arrive_expect_tx(k_full(sk), kTileBytes);
+        tma_load_4d(kd, &tma_k, k_full(sk), 0, key0, hk, b);
+        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, key0, hk, b);
+        ++issued_k;
+        if (!bounded_wait(v_empty(sv), ((j / kDqVStages) & 1) ^ 1, abort_flag, err, kErrWinProducer,
+                          wait_ns))
+          break;
+        const uint32_t vd = sbase + L::kV + sv * kTileBytes;
+        mbar_arrive_expect_tx(v_full(sv), kTileBytes);
+        tma_load_4d(vd, &tma_v, v_full(sv), 0, key0, hk, b);
+        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, key0, hk, b);
+        ++issued_v;
+      }
+      uint64_t t0 = tc::globaltimer();
+      while (!mbar_try_wait(qdo_full, 0) && tc::globaltimer() - t0 < wait_ns) {
+      }
+      for (int j = issued_k > kDqKStages ? issued_k - kDqKStages : 0; j < issued_k; ++j) {
+        t0 = tc::globaltimer();
+        while (!mbar_try_wait(k_full(j % kDqKStages), (j / kDqKStages) & 1) &&
+               tc::globaltimer() - t0 < wait_ns) {
+        }
+      }
+      for (int j = issued_v > kDqVStages ? issued_v - kDqVStages : 0; j < issued_v; ++j) {
+        t0 = tc::globaltimer();
+        while (!mbar_try_wait(v_full(j % kDqVStages), (j / kDqVStages) & 1) &&
+               tc::globaltimer() - t0 < wait_ns) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------- MMA issuer ----
+    const uint32_t leader = elect_one();
+    auto wait = [&](uint32_t bar, int parity) {
+      return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
+    };
+    bool ok = wait(qdo_full, 0);
+    bool issued = false;
+    const Desc q_desc(smem_desc_sw128(sbase + L::kQ, 16, 1024));
+    const Desc do_desc(smem_desc_sw128(sbase + L::kDO, 16, 1024));
+    const Desc k_desc(smem_desc_sw128(sbase + L::kK, 16, 1024));
+    const Desc k_mn(smem_desc_sw128(sbase + L::kK, kBox, 1024));
+    const Desc v_desc(smem_desc_sw128(sbase + L::kV, 16, 1024));
+    auto issue_sd = [&](int j) -> bool {
+      const int sk = j % kDqKStages, sv = j % kDqVStages;
+      if (!wait(k_full(sk), (j / kDqKStages) & 1)) return false;
+      if (!wait(v_full(sv), (j / kDqVStages) & 1)) return false;
+      if (j > 0 && !wait(st_empty, (j - 1) & 1)) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // S = Q K^T
+        mma_ss(leader, tmem, q_desc.at(kmajor_step(kk, kBox)), q_desc.hi,
+               k_desc.at(sk * kTileBytes + kmajor_step(kk, kBox)), k_desc.hi, kIdescKK,
+               kk > 0 ? 1u : 0u);
+#pragma unroll
+      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // dP = dO V^T
+        mma_ss(leader, tmem + 128, do_desc.at(kmajor_step(kk, kBox)), do_desc.hi,
+               v_desc.at(sv * kTileBytes + kmajor_step(kk, kBox)), v_desc.hi, kIdescKK,
+               kk > 0 ? 1u : 0u);
+      commit(leader, st_full);
+      commit(leader, v_empty(sv));
+      issued = true;
+      return true;
+    };
+    if (ok) ok = issue_sd(0);
+    for (int j = 0; j < n && ok; ++j) {
+      const int sk = j % kDqKStages;
+      if (j + 1 < n && !(ok = issue_sd(j + 1))) break;
+      if (!(ok = wait(ds_full, j & 1))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < kTile / 16; ++kk)  // dQ += dS K (dS from TMEM: 8 columns per 16 keys)
+        mma_ts(leader, tmem + 256, tmem + 384 + kk * 8, k_mn.at(sk * kTileBytes + mnmajor_step(kk)),
+               k_mn.hi, kIdescKM, (j > 0 || kk > 0) ? 1u : 0u);
+      commit(leader, buf_free);
+      commit(leader, k_empty(sk));
+    }
+    if (ok) commit(leader, acc_done);
+    if (!ok && issued) {
+      commit(leader, drain_bar);
+      uint64_t t0 = tc::globaltimer();
+      while (!mbar_try_wait(drain_bar, 0) && tc::globaltimer() - t0 < wait_ns) {
+      }
+    }
+  } else {
+    // ------------------------------------------------------- compute ----
+    const int quarter = warp & 3;
+    const int part = (warp - 2) >> 2;   // keys [32 part, 32 part + 32) of each tile
+    const int cb = part * 32;
+    const int r = quarter * 32 + lane;  // query row of this thread
+    const int q = q0 + r;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const int64_t vidx = ((int64_t)b * a.H + h) * ((int64_t)nq * kTile) + q;
+    const float nl = q < a.S ? a.nl2[vidx] : 0.f;
+    const float nd = q < a.S ? -a.Dv[vidx] : 0.f;
+    const uint64_t sl2 = f2_pack(a.scale_log2, a.scale_log2);
+    const uint64_t nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
+    const uint32_t ds_tmem = tmem + 384 + part * 16 + lane_off;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      bool w = true;
+      if (lane == 0) w = bounded_wait(st_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      if (!(ok = warp_ok(w))) break;
+      tc_fence_after();
+      float sv[32], dp[32];
+      tmem_ld32_async(tmem + cb + lane_off, sv);
+      tmem_ld32_async(tmem + 128 + cb + lane_off, dp);
+      const int jt = kt.at(j);
+      const bool edge = jt * kTile + kTile > a.S || jt == qt ||
+                        win_edge(q0 + kTile - 1, jt * kTile, a.window, a.sinks);
+      uint32_t mk = 0xffffffffu;
+      int kind = 1;
+      if (edge) {
+        mk = keys_seen(q, jt * kTile + cb, a.S, a.window, a.sinks);
+        kind = mask_kind(mk, 0xffffffffu);
+      }
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(st_empty);  // the next tile's S / dP may overwrite them
+      uint32_t dw[16];
+      if (kind == 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) dw[e] = 0u;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float p0, p1, d0, d1;
+          f2_unpack(f2_fma(f2_pack(sv[e], sv[e + 1]), sl2, nl2), p0, p1);
+          p0 = fast_exp2(p0);
+          p1 = fast_exp2(p1);
+          f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0, d1);
+          if (kind == 2) {
+            if (!(mk & (1u << e))) d0 = 0.f;
+            if (!(mk & (2u << e))) d1 = 0.f;
+          }
+          dw[e >> 1] = pack_bf16(d0, d1);
+        }
+      }
+      if (j > 0) {  // the previous tile's dQ product has read dS
+        if (lane == 0) w = bounded_wait(buf_free, (j - 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+        if (!(ok = warp_ok(w))) break;
+        tc_fence_after();
+      }
+      tmem_st16u(ds_tmem, dw);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    if (ok) {
+      bool w = true;
+      if (lane == 0) w = bounded_wait(acc_done, 0, abort_flag, err, kErrWinSoftmax, wait_ns);
+      ok = warp_ok(w);
+    }
+    if (ok) {
+      tc_fence_after();
+      bf16* orow = a.dq + ((int64_t)b * a.S + q) * (int64_t)(a.H * kHeadDim) + h * kHeadDim + cb;
+      float o[32];
+      tmem_ld32(tmem + 256 + cb + lane_off, o);
+      if (q < a.S) {
+        const float sc = a.scale;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint4*>(orow + 8 * g) =
+              make_uint4(pack_bf16(o[8 * g] * sc, o[8 * g + 1] * sc),
+                         pack_bf16(o[8 * g + 2] * sc, o[8 * g + 3] * sc),
+                         pack_bf16(o[8 * g + 4] * sc, o[8 * g + 5] * sc),
+                         pack_bf16(o[8 * g + 6] * sc, o[8 * g + 7] * sc));
+      }
+    }
+  }
+
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+}
+
+// ----------------------------------------------------------------- host ----
+void fn_error(const char* fn, const char* text) {
+  char msg[256];
+  snprintf(msg, sizeof(msg), "%s: %s", fn, text);
+  set_last_error(msg);
+}
+
+bool sizes_ok(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq) {
+  return batch > 0 && heads > 0 && kv_heads > 0 && seq > 0 && heads % kv_heads == 0 &&
+         batch * heads <= (1 << 20) && seq <= (1 << 24) &&
+         batch * heads * ((seq + kTile - 1) / kTile) <= (1 << 28);
+}
+
+// How the dK / dV work is cut: the query heads of a KV head into `groups` CTAs when
+// one CTA per key tile would leave SMs idle, the sink tiles' steps into segments as
+// long as an ordinary tile's.
+struct DkvPlan {
+  int groups, heads_per, n_sink, segs, seg_steps;
+  int64_t units, slots;
+};
+DkvPlan dkv_plan(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t window, int64_t sinks) {
+  DkvPlan p;
+  const int64_t nt = (S + kTile - 1) / kTile, nq64 = (S + kQStep - 1) / kQStep;
+  if (window > S) window = S;
+  if (sinks > S) sinks = S;
+  if (window == S) sinks = 0;  // the window alone shows every key
+  p.n_sink = (int)((sinks + kTile - 1) / kTile);
+  const int64_t steps = (kTile + window - 2) / kQStep + 1;  // of an ordinary tile
+  p.seg_steps = (int)(steps < 8 ? 8 : steps < nq64 ? steps : nq64);
+  p.segs = (int)((nq64 + p.seg_steps - 1) / p.seg_steps);
+  const int64_t rep = H / Hk;
+  const int64_t tiles = B * Hk * nt;
+  // one CTA per key tile if that fills most SMs, else the fewest head groups that do
+  int64_t g = (num_sms() * 4 / 5 + tiles - 1) / tiles;
+  if (g > rep) g = rep;
+  if (g < 1) g = 1;
+  p.heads_per = (int)((rep + g - 1) / g);
+  p.groups = (int)((rep + p.heads_per - 1) / p.heads_per);
+  const int64_t sink_units = B * Hk * p.n_sink * p.groups * p.segs;
+  const int64_t rest = B * Hk * (nt - p.n_sink) * p.groups;
+  p.units = sink_units + rest;
+  p.slots = sink_units + (p.groups > 1 ? rest : 0);
+  return p;
+}
+size_t vec_bytes(int64_t B, int64_t H, int64_t S) {
+  const size_t s_pad = (size_t)((S + kTile - 1) / kTile * kTile);
+  return ((size_t)B * H * s_pad * 4 + 255) / 256 * 256;
+}
+
+}  // namespace
+}  // namespace attn
+}  // namespace soup
+
+using namespace soup;
+using namespace soup::attn;
+
+extern "C" {
+
+int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                              int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
+                              int64_t head_dim, float scale, int64_t window, int64_t sinks,
+                              void* out, float* lse, void* stream) {
+  const char* fn = "soup_attention_window_fwd";
+  if (!sizes_ok(batch, heads, kv_heads, seq) || !out || !lse || !(scale > 0.f)) {
+    fn_error(fn, "bad arguments");
+    return SOUP_ERR_INVALID;
+  }
+  if (window <= 0 || sinks < 0) {
+    fn_error(fn, "window must be positive and sinks not negative");
+    return SOUP_ERR_INVALID;
+  }
+  if (head_dim != kHeadDim) {
+    fn_error(fn, "head_dim must be 128");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  if (!bhsd_ok(q, q_strides) || !bhsd_ok(k, k_strides) || !bhsd_ok(v, v_strides) ||
+      !aligned16(out)) {
+    fn_error(fn, "q/k/v need 16-byte aligned bases and strides that are multiples of 8 elements "
+                 "(last dimension contiguous)");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  int* err = device_err_ptr();
+  if (!err) {
+    set_last_error("device error word unavailable");
+    return SOUP_ERR_CUDA;
+  }
+  CUtensorMap mq, mk, mv;
+  int rc;
+  if ((rc = make_bhsd_map(&mq, q, q_strides, batch, heads, seq, "q"))) return rc;
+  if ((rc = make_bhsd_map(&mk, k, k_strides, batch, kv_heads, seq, "k", kBlk))) return rc;
+  if ((rc = make_bhsd_map(&mv, v, v_strides, batch, kv_heads, seq, "v", kBlk))) return rc;
+  static bool smem_set_done[64] = {false};
+  if ((rc = set_smem(win_fwd_kernel, WinFwdSmem::kBytes, smem_set_done))) return rc;
+  FwdArgs a{(int)batch, (int)heads, (int)kv_heads, (int)seq, scale * 1.4426950408889634f,
+            (int)(window < seq ? window : seq), (int)(sinks < seq ? sinks : seq),
+            static_cast<bf16*>(out), lse, wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
+  const int64_t npair = ((seq + kTile - 1) / kTile + 1) / 2;
+  return cuda_status(launch_pdl(win_fwd_kernel, dim3((unsigned)(batch * heads * npair)),
+                                dim3(kFwdThreads), WinFwdSmem::kBytes, as_stream(stream), mq, mk, mv, a,
+                                err));
+}
+
+size_t soup_attention_window_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                 int64_t seq, int64_t window, int64_t sinks) {
+  if (!sizes_ok(batch, heads, kv_heads, seq) || window <= 0 || sinks < 0) return 0;
+  const DkvPlan p = dkv_plan(batch, heads, kv_heads, seq, window, sinks);
+  return 2 * vec_bytes(batch, heads, seq) + (size_t)p.slots * 2 * kTile * kHeadDim * 4;
+}
+
+int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const void* k,
+                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                              const void* out, const void* dout, const float* lse, int64_t batch,
+                              int64_t heads, int64_t kv_heads, int64_t seq, int64_t head_dim,
+                              float scale, int64_t window, int64_t sinks, void* dq, void* dk,
+                              void* dv, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "soup_attention_window_bwd";
+  if (!sizes_ok(batch, heads, kv_heads, seq) || !out || !dout || !lse || !dq || !dk || !dv ||
+      !workspace || !(scale > 0.f)) {
+    fn_error(fn, "bad arguments");
+    return SOUP_ERR_INVALID;
+  }
+  if (window <= 0 || sinks < 0) {
+    fn_error(fn, "window must be positive and sinks not negative");
+    return SOUP_ERR_INVALID;
+  }
+  if (head_dim != kHeadDim) {
+    fn_error(fn, "head_dim must be 128");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  if (!bhsd_ok(q, q_strides) || !bhsd_ok(k, k_strides) || !bhsd_ok(v, v_strides) ||
+      !aligned16(out) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+      !aligned16(lse)) {
+    fn_error(fn, "operands need 16-byte aligned bases and strides that are multiples of 8 elements");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  const DkvPlan p = dkv_plan(batch, heads, kv_heads, seq, window, sinks);
+  const size_t vbytes = vec_bytes(batch, heads, seq);
+  if (workspace_bytes < soup_attention_window_bwd_workspace_bytes(batch, heads, kv_heads, seq, window,
+                                                                  sinks) ||
+      !aligned16(workspace)) {
+    fn_error(fn, "workspace too small or misaligned");
+    return SOUP_ERR_WORKSPACE;
+  }
+  if (p.units > 0x7fffffff) {
+    fn_error(fn, "too many key tiles");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  int* err = device_err_ptr();
+  if (!err) {
+    set_last_error("device error word unavailable");
+    return SOUP_ERR_CUDA;
+  }
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* dvec = reinterpret_cast<float*>(ws);
+  float* nl2 = reinterpret_cast<float*>(ws + vbytes);
+  float* part = reinterpret_cast<float*>(ws + 2 * vbytes);
+  CUtensorMap mq, mk, mv, mdo, mq64, mdo64;
+  int rc;
+  const int64_t do_strides[3] = {seq * heads * kHeadDim, kHeadDim, heads * kHeadDim};
+  if ((rc = make_bhsd_map(&mq, q, q_strides, batch, heads, seq, "q"))) return rc;
+  if ((rc = make_bhsd_map(&mk, k, k_strides, batch, kv_heads, seq, "k"))) return rc;
+  if ((rc = make_bhsd_map(&mv, v, v_strides, batch, kv_heads, seq, "v"))) return rc;
+  if ((rc = make_bhsd_map(&mdo, dout, do_strides, batch, heads, seq, "dout"))) return rc;
+  if ((rc = make_bhsd_map(&mq64, q, q_strides, batch, heads, seq, "q", kQStep))) return rc;
+  if ((rc = make_bhsd_map(&mdo64, dout, do_strides, batch, heads, seq, "dout", kQStep))) return rc;
+  static bool dkdv_set[64] = {false}, dq_set[64] = {false};
+  if ((rc = set_smem(win_dkdv_kernel, WinDkvSmem::kBytes, dkdv_set))) return rc;
+  if ((rc = set_smem(win_dq_kernel, WinDqSmem::kBytes, dq_set))) return rc;
+  cudaStream_t st = as_stream(stream);
+  const int B = (int)batch, H = (int)heads, Hk = (int)kv_heads, S = (int)seq;
+  const int64_t rows = (int64_t)B * S * H;
+  int64_t dot_blocks = (rows + 16 * kDotRows - 1) / (16 * kDotRows);  // 16 half-warps per block
+  if (dot_blocks > 16 * num_sms()) dot_blocks = 16 * num_sms();
+  if ((rc = cuda_status(launch_pdl(attn_bwd_dot_kernel, dim3((unsigned)dot_blocks), dim3(256), 0, st,
+                                   static_cast<const bf16*>(dout), static_cast<const bf16*>(out),
+                                   lse, B, H, S, dvec, nl2))))
+    return rc;
+  const int win = (int)(window < seq ? window : seq);
+  const int snk = win == S ? 0 : (int)(sinks < seq ? sinks : seq);
+  BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, win, snk, dvec, nl2,
+            static_cast<bf16*>(dq), static_cast<bf16*>(dk), static_cast<bf16*>(dv), part, p.groups,
+            p.heads_per, p.n_sink, p.segs, p.seg_steps,
+            wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
+  const int nt = (S + kTile - 1) / kTile;
+  if ((rc = cuda_status(launch_pdl(win_dkdv_kernel, dim3((unsigned)p.units), dim3(kThreads),
+                                   WinDkvSmem::kBytes, st, mq64, mk, mv, mdo64, a, err))))
+    return rc;
+  if ((rc = cuda_status(launch_pdl(win_dq_kernel, dim3((unsigned)(B * H * nt)), dim3(kThreads),
+                                   WinDqSmem::kBytes, st, mq, mk, mv, mdo, a, err))))
+    return rc;
+  const int tiles = p.groups > 1 ? nt : p.n_sink;  // key tiles whose sums are in slots
+  if (tiles == 0) return SOUP_OK;
+  return cuda_status(launch_pdl(win_dkdv_sum_kernel, dim3((unsigned)(B * Hk * tiles * (kTile / 8))),
+                                dim3(256), 0, st, a, tiles));
+}
+
+}  // extern "C"

@@ -164,7 +164,7 @@ class WindowAttentionFunction(torch.autograd.Function):
         dq = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device)
         dk = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
         dv = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
-        nbytes = _lib.lib().soup_attention_bwd_workspace_bytes(B, H, S)
+        nbytes = _lib.lib().soup_attention_window_bwd_workspace_bytes(B, H, Hk, S, window, sinks)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         _lib.call("soup_attention_window_bwd", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
                   vs, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), B, H, Hk, S, D, scale, window,

@@ -369,14 +369,18 @@ int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
 /* The same attention with a sliding window and sinks: query i sees key j iff
  * j <= i and (i - j < window or j < sinks), window >= 1, sinks >= 0 (either may
  * exceed seq). Only key tiles that hold a visible key are read: the cost is
- * proportional to seq (window + sinks). Buffers, layouts, strides and the
- * backward's workspace as for soup_attention_fwd / soup_attention_bwd. No kernel
- * in the reference (transformers masks SDPA for its sliding-window layers). */
+ * proportional to seq (window + sinks). Buffers, layouts and strides as for
+ * soup_attention_fwd / soup_attention_bwd; the backward's workspace is
+ * soup_attention_window_bwd_workspace_bytes (of the current device). Reproducible
+ * (no atomics). No kernel in the reference (transformers masks SDPA for its
+ * sliding-window layers). */
 int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const void* k,
                               const int64_t* k_strides, const void* v, const int64_t* v_strides,
                               int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq,
                               int64_t head_dim, float scale, int64_t window, int64_t sinks,
                               void* out, float* lse, void* stream);
+size_t soup_attention_window_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                 int64_t seq, int64_t window, int64_t sinks);
 int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const void* k,
                               const int64_t* k_strides, const void* v, const int64_t* v_strides,
                               const void* out, const void* dout, const float* lse, int64_t batch,

@@ -352,6 +352,10 @@ def _window_check(q, k, v, do, window, sinks, scale=128 ** -0.5):
     (1, 3, 1, 1000, 7, 1),       # a window far below a tile
     (1, 2, 1, 640, 640, 3),      # window = sequence: plain causal
     (1, 2, 1, 333, 5000, 9000),  # both beyond the sequence
+    (1, 8, 1, 300, 40, 2),       # eight heads of one KV head, few key tiles: heads split over CTAs
+    (1, 7, 1, 200, 70, 1),       # a head count that no split divides
+    (6, 10, 5, 900, 64, 140),    # many key tiles: one CTA for all heads; sinks in segments
+    (2, 2, 2, 2500, 130, 129),   # sink segments, two sink tiles
 ])
 def test_window_attention(B, H, Hk, S, window, sinks):
     _window_check(*_qkv(B, H, Hk, S, S + window), window, sinks)
@@ -393,7 +397,9 @@ def test_window_attention_equals_causal_when_the_window_covers_all():
         ts = [t.detach().requires_grad_(True) for t in (q, k, v)]
         out = f(*ts)
         res += [out, *torch.autograd.grad(out, ts, do)]
-    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    # two kernels that both round P, dS (2^-8 of each) and their outputs to bf16
+    for x, y in zip(a, b):
+        assert float((x.double() - y.double()).norm() / y.double().norm()) <= 2 * 2.0 ** -8
 
 
 def test_window_attention_directional_difference():
