@@ -15,7 +15,7 @@
 // bf16 pairs and is the A operand of O_X += P_X V read from TMEM. Two threads share
 // a query row (64 keys each) and exchange their row maxima through shared memory.
 // Backward: dK / dV per (batch, KV head, key tile): the CTA runs through the query
-// heads of its group and their queries in 64-query steps and keeps dK, dV in TMEM, so
+// heads of its group and their queries in 128-query steps and keeps dK, dV in TMEM, so
 // no per-head partials reach memory; the far queries of the sink tiles, which every
 // later query sees, are cut into segments with fp32 partials summed in a fixed order.
 // dQ per (batch, query head, query tile). Both recompute P from the log-sum-exp; no
@@ -79,18 +79,6 @@ __device__ __forceinline__ uint32_t queries_seeing(int key, int q0, int S, int w
 __device__ __forceinline__ int mask_kind(uint32_t m, uint32_t all) {
   if (__all_sync(0xffffffffu, (m & all) == 0u)) return 0;
   return __all_sync(0xffffffffu, (m & all) == all) ? 1 : 2;
-}
-
-__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, float (&v)[16]) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  __syncwarp();
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
 }
 
 // ---- the MMA warp ----
@@ -557,11 +545,11 @@ struct BwdArgs {
   int groups;        // parts that a KV head's query heads are split into
   int heads_per;     // query heads per part
   int n_sink;        // sink tiles
-  int segs, seg_steps;  // segments of a sink tile's steps, and their length
+  int segs, seg_steps;  // segments of a sink tile's 128-query steps, and their length
   uint64_t wait_ns;
 };
 
-// One unit of dK / dV work: a key tile, a range of 64-query steps, query heads
+// One unit of dK / dV work: a key tile, a range of 128-query steps, query heads
 // [h0, h0 + nh), and the slot its sums go to (-1: straight to dk, dv).
 struct DkvUnit {
   int b, hk, kt, h0, nh, step0, n, slot;
@@ -571,7 +559,7 @@ __host__ __device__ __forceinline__ int dkv_sink_units(const BwdArgs& a) {
 }
 __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
   DkvUnit u;
-  const int nq64 = (a.S + kQStep - 1) / kQStep;
+  const int nq = (a.S + kTile - 1) / kTile;
   const int n_sink_units = dkv_sink_units(a);
   const int rep = a.H / a.Hk;
   int g, bhk;
@@ -583,9 +571,8 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
     i /= a.groups;
     u.kt = i % a.n_sink;
     bhk = i / a.n_sink;
-    const int first = u.kt * (kTile / kQStep);
-    u.step0 = first + seg * a.seg_steps;
-    const int end = u.step0 + a.seg_steps < nq64 ? u.step0 + a.seg_steps : nq64;
+    u.step0 = u.kt + seg * a.seg_steps;
+    const int end = u.step0 + a.seg_steps < nq ? u.step0 + a.seg_steps : nq;
     u.n = end > u.step0 ? end - u.step0 : 0;
   } else {
     i -= n_sink_units;
@@ -594,10 +581,10 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
     i /= a.groups;
     bhk = i % (a.B * a.Hk);
     u.kt = a.n_sink + i / (a.B * a.Hk);
-    u.step0 = u.kt * (kTile / kQStep);
+    u.step0 = u.kt;
     // the last query that sees a key of this tile
-    const int last = (u.kt * kTile + kTile - 1 + a.window - 1) / kQStep;
-    u.n = (last < nq64 - 1 ? last : nq64 - 1) - u.step0 + 1;
+    const int last = (u.kt * kTile + kTile - 1 + a.window - 1) / kTile;
+    u.n = (last < nq - 1 ? last : nq - 1) - u.step0 + 1;
   }
   u.b = bhk / a.Hk;
   u.hk = bhk % a.Hk;
@@ -608,23 +595,26 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
   return u;
 }
 
-// dK / dV of one unit. TMEM: S^T and dP^T (128 keys x 64 queries) double buffered
-// (buffer i: S^T at column 128 i, dP^T at 128 i + 64), dV at 256, dK at 384. Shared
-// memory: K, V (32 KB each, loaded once for all query heads), a ring of 3 stages of
-// 64-query (Q, dO) tiles with their nl2 / D vectors, P^T and dS^T (16 KB each). A
-// compute thread owns 16 queries of one key row of each step.
-constexpr int kDkvRing = 3;
+// dK / dV of one unit, keys on the rows: per step of 128 queries S^T = K Q^T, dP^T = V dO^T,
+// dV += P^T dO, dK += dS^T Q. TMEM: S^T at column 0, dP^T 128, dV 256, dK 384. P^T and
+// dS^T overwrite the columns that they were computed from (bf16 pairs, the 32 queries of
+// a compute warp in the first 16 of its own 32 columns, so no warp writes what another
+// still reads) and are A operands from TMEM. The issue order
+//   dV(i), S^T(i + 1), dK(i), dP^T(i + 1), dV(i + 1), ...
+// leaves the softmax the time of two products between S^T and dV, and dS the same between
+// dP^T and dK, so the tensor pipe need not wait; products of N = 128 run at twice the rate
+// of N = 64 ones (75 cycles of issue either way). Shared memory: K, V (32 KB each, loaded
+// once for all query heads), two stages of (Q, dO) tiles with their nl2 / D vectors. A
+// compute thread owns 32 queries of one key row.
+constexpr int kDkvStages = 2;
 struct WinDkvSmem {
   static constexpr int kK = 0;
   static constexpr int kV = kK + kTileBytes;
-  static constexpr int kQD = kV + kTileBytes;  // stage s: Q at +0, dO at +kStepTile
-  static constexpr int kP = kQD + kDkvRing * 2 * kStepTile;
-  static constexpr int kDS = kP + kPTBytes;
-  static constexpr int kVec = kDS + kPTBytes;  // stage s: nl2, D of its 64 queries (2 x 256 B)
-  static constexpr int kBar = kVec + kDkvRing * 2 * kQStep * 4;
-  // kv_full, full[3], empty[3], st_full[2], st_empty[2], p_full, p_free, ds_full, ds_free,
-  // acc_done, drain
-  static constexpr int kNumBars = 1 + 2 * kDkvRing + 4 + 6;
+  static constexpr int kQD = kV + kTileBytes;  // stage s: Q at +0, dO at +kTileBytes
+  static constexpr int kVec = kQD + kDkvStages * 2 * kTileBytes;  // stage s: nl2, D (2 x 512 B)
+  static constexpr int kBar = kVec + kDkvStages * 2 * kTile * 4;
+  // kv_full, full[2], empty[2], s_full, p_full, dp_full, ds_full, acc_done, drain
+  static constexpr int kNumBars = 1 + 2 * kDkvStages + 6;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kUsed = kMisc + 16;
   static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
@@ -650,13 +640,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t bar0 = sbase + L::kBar;
   const uint32_t kv_full = bar0;
   auto full = [&](int st) { return bar0 + 8u * (1 + st); };
-  auto empty = [&](int st) { return bar0 + 8u * (1 + kDkvRing + st); };
-  constexpr int kB = 1 + 2 * kDkvRing;
-  auto st_full = [&](int bb) { return bar0 + 8u * (kB + bb); };
-  auto st_empty = [&](int bb) { return bar0 + 8u * (kB + 2 + bb); };
-  const uint32_t p_full = bar0 + 8u * (kB + 4), p_free = bar0 + 8u * (kB + 5);
-  const uint32_t ds_full = bar0 + 8u * (kB + 6), ds_free = bar0 + 8u * (kB + 7);
-  const uint32_t acc_done = bar0 + 8u * (kB + 8), drain_bar = bar0 + 8u * (kB + 9);
+  auto empty = [&](int st) { return bar0 + 8u * (1 + kDkvStages + st); };
+  constexpr int kB = 1 + 2 * kDkvStages;
+  const uint32_t s_full = bar0 + 8u * kB, p_full = bar0 + 8u * (kB + 1);
+  const uint32_t dp_full = bar0 + 8u * (kB + 2), ds_full = bar0 + 8u * (kB + 3);
+  const uint32_t acc_done = bar0 + 8u * (kB + 4), drain_bar = bar0 + 8u * (kB + 5);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
 
@@ -668,8 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kNumBars; ++i) {
       const uint32_t bar = bar0 + 8u * i;
-      const bool per_warp = bar == st_empty(0) || bar == st_empty(1) || bar == p_full || bar == ds_full;
-      mbar_init(bar, per_warp ? kWarps : 1);
+      mbar_init(bar, bar == p_full || bar == ds_full ? kWarps : 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -702,21 +689,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_load_4d(sbase + L::kV + kBox, &tma_v, kv_full, 64, k0, u.hk, u.b);
       int issued = 0, h = u.h0, step = u.step0;
       for (int i = 0; i < total; ++i) {
-        const int st = i % kDkvRing;
-        if (!bounded_wait(empty(st), ((i / kDkvRing) & 1) ^ 1, abort_flag, err, kErrWinProducer,
+        const int st = i % kDkvStages;
+        if (!bounded_wait(empty(st), ((i / kDkvStages) & 1) ^ 1, abort_flag, err, kErrWinProducer,
                           wait_ns))
           break;
-        const int q0 = step * kQStep;
-        const uint32_t qd = sbase + L::kQD + st * 2 * kStepTile;
+        const int q0 = step * kTile;
+        const uint32_t qd = sbase + L::kQD + st * 2 * kTileBytes;
         const int64_t vrow = ((int64_t)u.b * a.H + h) * s_pad + q0;
-        const uint32_t vd = sbase + L::kVec + st * 2 * kQStep * 4;
-        mbar_arrive_expect_tx(full(st), 2 * kStepTile + 2 * kQStep * 4);
+        const uint32_t vd = sbase + L::kVec + st * 2 * kTile * 4;
+        mbar_arrive_expect_tx(full(st), 2 * kTileBytes + 2 * kTile * 4);
         tma_load_4d(qd, &tma_q, full(st), 0, q0, h, u.b);
-        tma_load_4d(qd + kStepBox, &tma_q, full(st), 64, q0, h, u.b);
-        tma_load_4d(qd + kStepTile, &tma_do, full(st), 0, q0, h, u.b);
-        tma_load_4d(qd + kStepTile + kStepBox, &tma_do, full(st), 64, q0, h, u.b);
-        bulk_load(vd, a.nl2 + vrow, kQStep * 4, full(st));
-        bulk_load(vd + kQStep * 4, a.Dv + vrow, kQStep * 4, full(st));
+        tma_load_4d(qd + kBox, &tma_q, full(st), 64, q0, h, u.b);
+        tma_load_4d(qd + kTileBytes, &tma_do, full(st), 0, q0, h, u.b);
+        tma_load_4d(qd + kTileBytes + kBox, &tma_do, full(st), 64, q0, h, u.b);
+        bulk_load(vd, a.nl2 + vrow, kTile * 4, full(st));
+        bulk_load(vd + kTile * 4, a.Dv + vrow, kTile * 4, full(st));
         ++issued;
         if (++step == u.step0 + u.n) {
           step = u.step0;
@@ -726,9 +713,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint64_t t0 = tc::globaltimer();
       while (!mbar_try_wait(kv_full, 0) && tc::globaltimer() - t0 < wait_ns) {
       }
-      for (int i = issued > kDkvRing ? issued - kDkvRing : 0; i < issued; ++i) {
+      for (int i = issued > kDkvStages ? issued - kDkvStages : 0; i < issued; ++i) {
         t0 = tc::globaltimer();
-        while (!mbar_try_wait(full(i % kDkvRing), (i / kDkvRing) & 1) &&
+        while (!mbar_try_wait(full(i % kDkvStages), (i / kDkvStages) & 1) &&
                tc::globaltimer() - t0 < wait_ns) {
         }
       }
@@ -743,51 +730,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool issued = false;
     const Desc k_desc(smem_desc_sw128(sbase + L::kK, 16, 1024));
     const Desc v_desc(smem_desc_sw128(sbase + L::kV, 16, 1024));
-    const Desc qd_desc(smem_desc_sw128(sbase + L::kQD, 16, 1024));      // as K-major operands
-    const Desc qd_mn(smem_desc_sw128(sbase + L::kQD, kStepBox, 1024));  // as MN-major operands
-    const Desc p_desc(smem_desc_sw128(sbase + L::kP, 16, 1024));
-    const Desc ds_desc(smem_desc_sw128(sbase + L::kDS, 16, 1024));
-    auto issue_sd = [&](int i) -> bool {
-      const int st = i % kDkvRing, bb = i & 1;
-      if (!wait(full(st), (i / kDkvRing) & 1)) return false;
-      if (i >= 2 && !wait(st_empty(bb), ((i >> 1) & 1) ^ 1)) return false;
+    const Desc qd_desc(smem_desc_sw128(sbase + L::kQD, 16, 1024));   // as K-major operands
+    const Desc qd_mn(smem_desc_sw128(sbase + L::kQD, kBox, 1024));   // as MN-major operands
+    // S^T (dP = 0) or dP^T (1) of step i
+    auto issue_s = [&](int dP, int i) -> bool {
+      const int st = i % kDkvStages;
+      if (!wait(full(st), (i / kDkvStages) & 1)) return false;
       tc_fence_after();
-      const uint32_t q_off = st * 2 * kStepTile;
+      const uint32_t b_off = st * 2 * kTileBytes + dP * kTileBytes;
 #pragma unroll
-      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // S^T = K Q^T
-        mma_ss(leader, tmem + bb * 128, k_desc.at(kmajor_step(kk, kBox)), k_desc.hi,
-               qd_desc.at(q_off + kmajor_step(kk, kStepBox)), qd_desc.hi, kIdescKK64, kk > 0 ? 1u : 0u);
-#pragma unroll
-      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // dP^T = V dO^T
-        mma_ss(leader, tmem + bb * 128 + 64, v_desc.at(kmajor_step(kk, kBox)), v_desc.hi,
-               qd_desc.at(q_off + kStepTile + kmajor_step(kk, kStepBox)), qd_desc.hi, kIdescKK64,
-               kk > 0 ? 1u : 0u);
-      commit(leader, st_full(bb));
+      for (int kk = 0; kk < kHeadDim / 16; ++kk)
+        mma_ss(leader, tmem + dP * 128, (dP ? v_desc : k_desc).at(kmajor_step(kk, kBox)), k_desc.hi,
+               qd_desc.at(b_off + kmajor_step(kk, kBox)), qd_desc.hi, kIdescKK, kk > 0 ? 1u : 0u);
+      commit(leader, dP ? dp_full : s_full);
       issued = true;
       return true;
     };
-    if (ok) ok = issue_sd(0);
-    if (ok && total > 1) ok = issue_sd(1);
+    // dV += P^T dO (dK = 0) or dK += dS^T Q (1) of step i
+    auto issue_acc = [&](int dK, int i) -> bool {
+      const int st = i % kDkvStages;
+      if (!wait(dK ? ds_full : p_full, i & 1)) return false;
+      tc_fence_after();
+      const uint32_t b_off = st * 2 * kTileBytes + (dK ? 0 : kTileBytes);
+#pragma unroll
+      for (int kk = 0; kk < kTile / 16; ++kk)
+        mma_ts(leader, tmem + 256 + dK * 128, tmem + dK * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
+               qd_mn.at(b_off + mnmajor_step(kk)), qd_mn.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
+      return true;
+    };
+    if (ok) ok = issue_s(0, 0);
+    if (ok) ok = issue_s(1, 0);
     for (int i = 0; i < total && ok; ++i) {
-      const int st = i % kDkvRing;
-      const uint32_t q_off = st * 2 * kStepTile;
-      if (!(ok = wait(p_full, i & 1))) break;
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < kQStep / 16; ++kk)  // dV += P^T dO
-        mma_ss(leader, tmem + 256, p_desc.at(kk * 32), p_desc.hi,
-               qd_mn.at(q_off + kStepTile + mnmajor_step(kk)), qd_mn.hi, kIdescKM,
-               (i > 0 || kk > 0) ? 1u : 0u);
-      commit(leader, p_free);
-      if (!(ok = wait(ds_full, i & 1))) break;
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < kQStep / 16; ++kk)  // dK += dS^T Q
-        mma_ss(leader, tmem + 384, ds_desc.at(kk * 32), ds_desc.hi, qd_mn.at(q_off + mnmajor_step(kk)),
-               qd_mn.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
-      commit(leader, ds_free);
-      commit(leader, empty(st));
-      if (i + 2 < total && !(ok = issue_sd(i + 2))) break;
+      ok = issue_acc(0, i);
+      if (ok && i + 1 < total) ok = issue_s(0, i + 1);
+      if (ok) ok = issue_acc(1, i);
+      if (ok) commit(leader, empty(i % kDkvStages));
+      if (ok && i + 1 < total) ok = issue_s(1, i + 1);
     }
     if (ok) commit(leader, acc_done);
     if (!ok && issued) {
@@ -799,92 +777,92 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------------------------------- compute ----
     const int quarter = warp & 3;
-    const int part = (warp - 2) >> 2;   // queries [16 part, 16 part + 16) of each step
-    const int cb = part * 16;
+    const int part = (warp - 2) >> 2;   // queries [32 part, 32 part + 32) of each step
+    const int cb = part * 32;
     const int r = quarter * 32 + lane;  // key row of this thread
     const int key = k0 + r;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    uint8_t* pbox = smem + L::kP;
-    uint8_t* dsbox = smem + L::kDS;
+    const uint32_t s_t = tmem + cb + lane_off, dp_t = s_t + 128;
     const uint64_t sl2 = f2_pack(a.scale_log2, a.scale_log2);
     bool ok = true;
     int step = u.step0;
     for (int i = 0; i < total; ++i) {
-      const int st = i % kDkvRing, bb = i & 1;
-      const int qs = step * kQStep;
+      const int st = i % kDkvStages;
+      const int qs = step * kTile;
       if (++step == u.step0 + u.n) step = u.step0;
-      bool w = true;
-      if (lane == 0) w = bounded_wait(st_full(bb), (i >> 1) & 1, abort_flag, err, kErrWinSoftmax,
-                                      wait_ns);
-      if (!(ok = warp_ok(w))) break;
-      tc_fence_after();
-      float sv[16], dp[16];
-      tmem_ld16_async(tmem + bb * 128 + cb + lane_off, sv);
-      tmem_ld16_async(tmem + bb * 128 + 64 + cb + lane_off, dp);
-      const bool edge = qs + kQStep > a.S || qs < k0 + kTile ||
-                        win_edge(qs + kQStep - 1, k0, a.window, a.sinks);
-      uint32_t mk = 0xffffu;
+      const float* vnl = reinterpret_cast<const float*>(smem + L::kVec + st * 2 * kTile * 4) + cb;
+      const float* vD = vnl + kTile;
+      const bool edge = qs + kTile > a.S || qs < k0 + kTile ||
+                        win_edge(qs + kTile - 1, k0, a.window, a.sinks);
+      uint32_t mk = 0xffffffffu;
       int kind = 1;
       if (edge) {
         mk = queries_seeing(key, qs + cb, a.S, a.window, a.sinks);
-        kind = mask_kind(mk, 0xffffu);
+        kind = mask_kind(mk, 0xffffffffu);
       }
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(st_empty(bb));  // the step after next may overwrite them
-      const float* vnl = reinterpret_cast<const float*>(smem + L::kVec + st * 2 * kQStep * 4) + cb;
-      const float* vD = vnl + kQStep;
-      uint32_t pw[8], dw[8];
+      bool w = true;
+      if (lane == 0) w = bounded_wait(s_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      if (!(ok = warp_ok(w))) break;
+      tc_fence_after();
+      float p[32];
+      uint32_t words[16];
       if (kind == 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pw[e] = dw[e] = 0u;
+        for (int e = 0; e < 32; ++e) p[e] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) words[e] = 0u;
       } else {
+        tmem_ld32_async(s_t, p);
+        tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
+        for (int e = 0; e < 32; e += 4) {
           const float4 nl = *reinterpret_cast<const float4*>(vnl + e);
-          const float4 dd = *reinterpret_cast<const float4*>(vD + e);
-          float p[4], d[4];
-          f2_unpack(f2_fma(f2_pack(sv[e], sv[e + 1]), sl2, f2_pack(nl.x, nl.y)), p[0], p[1]);
-          f2_unpack(f2_fma(f2_pack(sv[e + 2], sv[e + 3]), sl2, f2_pack(nl.z, nl.w)), p[2], p[3]);
+          f2_unpack(f2_fma(f2_pack(p[e], p[e + 1]), sl2, f2_pack(nl.x, nl.y)), p[e], p[e + 1]);
+          f2_unpack(f2_fma(f2_pack(p[e + 2], p[e + 3]), sl2, f2_pack(nl.z, nl.w)), p[e + 2], p[e + 3]);
 #pragma unroll
-          for (int v = 0; v < 4; ++v) p[v] = fast_exp2(p[v]);
-          const uint64_t t0 = f2_add(f2_pack(dp[e], dp[e + 1]), f2_pack(-dd.x, -dd.y));
-          const uint64_t t1 = f2_add(f2_pack(dp[e + 2], dp[e + 3]), f2_pack(-dd.z, -dd.w));
-          f2_unpack(f2_mul(f2_pack(p[0], p[1]), t0), d[0], d[1]);
-          f2_unpack(f2_mul(f2_pack(p[2], p[3]), t1), d[2], d[3]);
-          if (kind == 2) {  // hidden and padding rows may hold anything: select, do not scale
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (!(mk & (1u << (e + v)))) p[v] = d[v] = 0.f;
-          }
-          pw[e >> 1] = pack_bf16(p[0], p[1]);
-          pw[(e >> 1) + 1] = pack_bf16(p[2], p[3]);
-          dw[e >> 1] = pack_bf16(d[0], d[1]);
-          dw[(e >> 1) + 1] = pack_bf16(d[2], d[3]);
+          for (int v = 0; v < 4; ++v) p[e + v] = fast_exp2(p[e + v]);
         }
-      }
-      if (i > 0) {  // the previous step's dV product has read P^T
-        if (lane == 0) w = bounded_wait(p_free, (i - 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-        if (!(ok = warp_ok(w))) break;
-      }
+        if (kind == 2) {  // hidden and padding rows may hold anything: select, do not scale
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<uint4*>(pbox + swz_off(r, part * 2 + c)) =
-            make_uint4(pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]);
-      tc::fence_proxy_async_smem();
+          for (int e = 0; e < 32; ++e)
+            if (!(mk & (1u << e))) p[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) words[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
+      }
+      tmem_st16u(s_t, words);
+      tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-      if (i > 0) {  // the previous step's dK product has read dS^T
-        if (lane == 0) w = bounded_wait(ds_free, (i - 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-        if (!(ok = warp_ok(w))) break;
+      if (lane == 0) {
+        mbar_arrive(p_full);
+        w = bounded_wait(dp_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
       }
+      if (!(ok = warp_ok(w))) break;
+      tc_fence_after();
+      if (kind != 0) {
+        float dp[32];
+        tmem_ld32_async(dp_t, dp);
+        tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<uint4*>(dsbox + swz_off(r, part * 2 + c)) =
-            make_uint4(dw[4 * c], dw[4 * c + 1], dw[4 * c + 2], dw[4 * c + 3]);
-      tc::fence_proxy_async_smem();
+        for (int e = 0; e < 32; e += 4) {
+          const float4 dd = *reinterpret_cast<const float4*>(vD + e);
+          float d[4];
+          f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]),
+                           f2_add(f2_pack(dp[e], dp[e + 1]), f2_pack(-dd.x, -dd.y))), d[0], d[1]);
+          f2_unpack(f2_mul(f2_pack(p[e + 2], p[e + 3]),
+                           f2_add(f2_pack(dp[e + 2], dp[e + 3]), f2_pack(-dd.z, -dd.w))), d[2], d[3]);
+          if (kind == 2) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              if (!(mk & (1u << (e + v)))) d[v] = 0.f;
+          }
+          words[e >> 1] = pack_bf16(d[0], d[1]);
+          words[(e >> 1) + 1] = pack_bf16(d[2], d[3]);
+        }
+      }
+      tmem_st16u(dp_t, words);
+      tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
@@ -944,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 __global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles) {
   pdl_wait();
   pdl_trigger();
-  const int nq64 = (a.S + kQStep - 1) / kQStep;
+  const int nq = (a.S + kTile - 1) / kTile;
   const int rows8 = blockIdx.x % (kTile / 8);
   const int i = blockIdx.x / (kTile / 8);
   const int kt = i % tiles, bhk = i / tiles;
@@ -956,8 +934,7 @@ __global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles)
   if (kt < a.n_sink) {
     slot0 = (bhk * a.n_sink + kt) * a.groups * a.segs;
     n = a.groups * a.segs;
-    const int steps = nq64 - kt * (kTile / kQStep);
-    segs = (steps + a.seg_steps - 1) / a.seg_steps;  // of a.segs, the others are empty
+    segs = (nq - kt + a.seg_steps - 1) / a.seg_steps;  // of a.segs, the others are empty
   } else {
     slot0 = dkv_sink_units(a) + ((kt - a.n_sink) * a.B * a.Hk + bhk) * a.groups;
     n = a.groups;
@@ -980,7 +957,9 @@ __global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles)
 }
 
 // dQ of one query tile: TMEM columns S 0, dP 128, dQ 256, dS 384 (bf16, two per
-// column: the A operand of dQ += dS K read from TMEM). Shared memory: Q and dO
+// column: the A operand of dQ += dS K read from TMEM). S and dP have barriers of their own:
+// S(j + 1) starts when S(j) has been read, which is during dP(j), so the tensor pipe does not
+// wait for the TMEM reads. Shared memory: Q and dO
 // (32 KB each, loaded once), a K ring (3 x 32 KB; a stage frees after its dQ
 // product) and a V ring (2 x 32 KB; a stage frees after its dP product). A compute
 // thread owns 32 keys of one query row of each tile.
@@ -992,9 +971,9 @@ struct WinDqSmem {
   static constexpr int kK = kDO + kTileBytes;
   static constexpr int kV = kK + kDqKStages * kTileBytes;
   static constexpr int kBar = kV + kDqVStages * kTileBytes;
-  // qdo_full, k_full[3], k_empty[3], v_full[2], v_empty[2], st_full, st_empty, ds_full,
-  // buf_free, acc_done, drain
-  static constexpr int kNumBars = 1 + 2 * kDqKStages + 2 * kDqVStages + 6;
+  // qdo_full, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full, s_empty, dp_full,
+  // dp_empty, ds_full, buf_free, acc_done, drain
+  static constexpr int kNumBars = 1 + 2 * kDqKStages + 2 * kDqVStages + 8;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kUsed = kMisc + 16;
   static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
@@ -1021,9 +1000,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto v_full = [&](int st) { return bar0 + 8u * (1 + 2 * kDqKStages + st); };
   auto v_empty = [&](int st) { return bar0 + 8u * (1 + 2 * kDqKStages + kDqVStages + st); };
   constexpr int kB = 1 + 2 * kDqKStages + 2 * kDqVStages;
-  const uint32_t st_full = bar0 + 8u * kB, st_empty = bar0 + 8u * (kB + 1);
-  const uint32_t ds_full = bar0 + 8u * (kB + 2), buf_free = bar0 + 8u * (kB + 3);
-  const uint32_t acc_done = bar0 + 8u * (kB + 4), drain_bar = bar0 + 8u * (kB + 5);
+  const uint32_t s_full = bar0 + 8u * kB, s_empty = bar0 + 8u * (kB + 1);
+  const uint32_t dp_full = bar0 + 8u * (kB + 2), dp_empty = bar0 + 8u * (kB + 3);
+  const uint32_t ds_full = bar0 + 8u * (kB + 4), buf_free = bar0 + 8u * (kB + 5);
+  const uint32_t acc_done = bar0 + 8u * (kB + 6), drain_bar = bar0 + 8u * (kB + 7);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
 
@@ -1041,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kNumBars; ++i) {
       const uint32_t bar = bar0 + 8u * i;
-      mbar_init(bar, bar == st_empty || bar == ds_full ? kWarps : 1);
+      mbar_init(bar, bar == s_empty || bar == dp_empty || bar == ds_full ? kWarps : 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1125,22 +1105,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto issue_sd = [&](int j) -> bool {
       const int sk = j % kDqKStages, sv = j % kDqVStages;
       if (!wait(k_full(sk), (j / kDqKStages) & 1)) return false;
-      if (!wait(v_full(sv), (j / kDqVStages) & 1)) return false;
-      if (j > 0 && !wait(st_empty, (j - 1) & 1)) return false;
+      if (j > 0 && !wait(s_empty, (j - 1) & 1)) return false;
       tc_fence_after();
 #pragma unroll
       for (int kk = 0; kk < kHeadDim / 16; ++kk)  // S = Q K^T
         mma_ss(leader, tmem, q_desc.at(kmajor_step(kk, kBox)), q_desc.hi,
                k_desc.at(sk * kTileBytes + kmajor_step(kk, kBox)), k_desc.hi, kIdescKK,
                kk > 0 ? 1u : 0u);
+      commit(leader, s_full);
+      issued = true;
+      if (!wait(v_full(sv), (j / kDqVStages) & 1)) return false;
+      if (j > 0 && !wait(dp_empty, (j - 1) & 1)) return false;
+      tc_fence_after();
 #pragma unroll
       for (int kk = 0; kk < kHeadDim / 16; ++kk)  // dP = dO V^T
         mma_ss(leader, tmem + 128, do_desc.at(kmajor_step(kk, kBox)), do_desc.hi,
                v_desc.at(sv * kTileBytes + kmajor_step(kk, kBox)), v_desc.hi, kIdescKK,
                kk > 0 ? 1u : 0u);
-      commit(leader, st_full);
+      commit(leader, dp_full);
       commit(leader, v_empty(sv));
-      issued = true;
       return true;
     };
     if (ok) ok = issue_sd(0);
@@ -1179,13 +1162,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ds_tmem = tmem + 384 + part * 16 + lane_off;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      bool w = true;
-      if (lane == 0) w = bounded_wait(st_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-      if (!(ok = warp_ok(w))) break;
-      tc_fence_after();
-      float sv[32], dp[32];
-      tmem_ld32_async(tmem + cb + lane_off, sv);
-      tmem_ld32_async(tmem + 128 + cb + lane_off, dp);
       const int jt = kt.at(j);
       const bool edge = jt * kTile + kTile > a.S || jt == qt ||
                         win_edge(q0 + kTile - 1, jt * kTile, a.window, a.sinks);
@@ -1195,10 +1171,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         mk = keys_seen(q, jt * kTile + cb, a.S, a.window, a.sinks);
         kind = mask_kind(mk, 0xffffffffu);
       }
+      bool w = true;
+      if (lane == 0) w = bounded_wait(s_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      if (!(ok = warp_ok(w))) break;
+      tc_fence_after();
+      float p[32];
+      tmem_ld32_async(tmem + cb + lane_off, p);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(st_empty);  // the next tile's S / dP may overwrite them
+      if (lane == 0) mbar_arrive(s_empty);  // the next tile's S may overwrite it
+      if (kind != 0) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          f2_unpack(f2_fma(f2_pack(p[e], p[e + 1]), sl2, nl2), p[e], p[e + 1]);
+          p[e] = fast_exp2(p[e]);
+          p[e + 1] = fast_exp2(p[e + 1]);
+        }
+      }
+      if (lane == 0) w = bounded_wait(dp_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      if (!(ok = warp_ok(w))) break;
+      tc_fence_after();
+      float dp[32];
+      tmem_ld32_async(tmem + 128 + cb + lane_off, dp);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_empty);
       uint32_t dw[16];
       if (kind == 0) {
 #pragma unroll
@@ -1206,11 +1205,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          float p0, p1, d0, d1;
-          f2_unpack(f2_fma(f2_pack(sv[e], sv[e + 1]), sl2, nl2), p0, p1);
-          p0 = fast_exp2(p0);
-          p1 = fast_exp2(p1);
-          f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0, d1);
+          float d0, d1;
+          f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0, d1);
           if (kind == 2) {
             if (!(mk & (1u << e))) d0 = 0.f;
             if (!(mk & (2u << e))) d1 = 0.f;
@@ -1284,14 +1280,14 @@ struct DkvPlan {
 };
 DkvPlan dkv_plan(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t window, int64_t sinks) {
   DkvPlan p;
-  const int64_t nt = (S + kTile - 1) / kTile, nq64 = (S + kQStep - 1) / kQStep;
+  const int64_t nt = (S + kTile - 1) / kTile;
   if (window > S) window = S;
   if (sinks > S) sinks = S;
   if (window == S) sinks = 0;  // the window alone shows every key
   p.n_sink = (int)((sinks + kTile - 1) / kTile);
-  const int64_t steps = (kTile + window - 2) / kQStep + 1;  // of an ordinary tile
-  p.seg_steps = (int)(steps < 8 ? 8 : steps < nq64 ? steps : nq64);
-  p.segs = (int)((nq64 + p.seg_steps - 1) / p.seg_steps);
+  const int64_t steps = (kTile + window - 2) / kTile + 1;  // of an ordinary tile
+  p.seg_steps = (int)(steps < 4 ? 4 : steps < nt ? steps : nt);
+  p.segs = (int)((nt + p.seg_steps - 1) / p.seg_steps);
   const int64_t rep = H / Hk;
   const int64_t tiles = B * Hk * nt;
   // one CTA per key tile if that fills most SMs, else the fewest head groups that do
@@ -1419,15 +1415,13 @@ int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const voi
   float* dvec = reinterpret_cast<float*>(ws);
   float* nl2 = reinterpret_cast<float*>(ws + vbytes);
   float* part = reinterpret_cast<float*>(ws + 2 * vbytes);
-  CUtensorMap mq, mk, mv, mdo, mq64, mdo64;
+  CUtensorMap mq, mk, mv, mdo;
   int rc;
   const int64_t do_strides[3] = {seq * heads * kHeadDim, kHeadDim, heads * kHeadDim};
   if ((rc = make_bhsd_map(&mq, q, q_strides, batch, heads, seq, "q"))) return rc;
   if ((rc = make_bhsd_map(&mk, k, k_strides, batch, kv_heads, seq, "k"))) return rc;
   if ((rc = make_bhsd_map(&mv, v, v_strides, batch, kv_heads, seq, "v"))) return rc;
   if ((rc = make_bhsd_map(&mdo, dout, do_strides, batch, heads, seq, "dout"))) return rc;
-  if ((rc = make_bhsd_map(&mq64, q, q_strides, batch, heads, seq, "q", kQStep))) return rc;
-  if ((rc = make_bhsd_map(&mdo64, dout, do_strides, batch, heads, seq, "dout", kQStep))) return rc;
   static bool dkdv_set[64] = {false}, dq_set[64] = {false};
   if ((rc = set_smem(win_dkdv_kernel, WinDkvSmem::kBytes, dkdv_set))) return rc;
   if ((rc = set_smem(win_dq_kernel, WinDqSmem::kBytes, dq_set))) return rc;
@@ -1448,7 +1442,7 @@ int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const voi
             wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
   const int nt = (S + kTile - 1) / kTile;
   if ((rc = cuda_status(launch_pdl(win_dkdv_kernel, dim3((unsigned)p.units), dim3(kThreads),
-                                   WinDkvSmem::kBytes, st, mq64, mk, mv, mdo64, a, err))))
+                                   WinDkvSmem::kBytes, st, mq, mk, mv, mdo, a, err))))
     return rc;
   if ((rc = cuda_status(launch_pdl(win_dq_kernel, dim3((unsigned)(B * H * nt)), dim3(kThreads),
                                    WinDqSmem::kBytes, st, mq, mk, mv, mdo, a, err))))
