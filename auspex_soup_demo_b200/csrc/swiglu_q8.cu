@@ -4,7 +4,7 @@
 // fp32 scale per block of 64 consecutive columns of a row (the last block of a
 // row may be shorter),
 //   scale = absmax / 127,  code = rint(x * (127 / absmax)),  value = code * scale,
-// each fp32 operation rounded to nearest (IEEE divisions), so the codes are the
+// each fp32 operation rounded to nearest (the divisions too), so the codes are the
 // same on every path. A block whose absmax is below 2^-100 is all zeros (there
 // 127 / absmax would overflow); one that holds an infinity or a NaN stands for
 // NaN throughout, so a diverged forward stays visible in the gradient.
@@ -30,25 +30,106 @@ __device__ __forceinline__ float q8_sigmoid<float>(float g) {
   return 1.f / (1.f + expf(-g));
 }
 
+// silu(g) u of two elements; 16-bit types on packed pairs, with the hardware exponential
+// and reciprocal (2^-22 each, far below the types' rounding). For g -> -inf the divisor
+// overflows and the result is the limit 0.
+template <typename T>
+__device__ __forceinline__ void q8_swiglu2(float g0, float g1, float u0, float u1, float& o0, float& o1) {
+  const uint64_t g = f2_pack(g0, g1);
+  float e0, e1;
+  f2_unpack(f2_mul(g, f2_pack(-kLog2e, -kLog2e)), e0, e1);
+  f2_unpack(f2_add(f2_pack(fast_exp2(e0), fast_exp2(e1)), f2_pack(1.f, 1.f)), e0, e1);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e0));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(e1));
+  f2_unpack(f2_mul(f2_mul(g, f2_pack(e0, e1)), f2_pack(u0, u1)), o0, o1);
+}
+template <>
+__device__ __forceinline__ void q8_swiglu2<float>(float g0, float g1, float u0, float u1, float& o0,
+                                                  float& o1) {
+  o0 = (g0 * q8_sigmoid<float>(g0)) * u0;
+  o1 = (g1 * q8_sigmoid<float>(g1)) * u1;
+}
+
 // |x| as ordered bits: NaN above infinity above every number, so an integer
 // maximum over a block also finds a NaN.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-__device__ __forceinline__ void q8_scale(uint32_t top_bits, float& inv, float& scale) {
-  const float top = __uint_as_float(top_bits);
-  inv = top < 7.8886090522101181e-31f ? 0.f : __fdiv_rn(127.f, top);  // 2^-100
-  scale = __fdiv_rn(top, 127.f);
+// inv = 127 / absmax and scale = absmax / 127, both correctly rounded. The second
+// divides by a constant: a product with the rounded reciprocal and one residual step
+// (Markstein's theorem) instead of a division.
+__device__ __forceinline__ void q8_scale(float top, float& inv, float& scale) {
+  constexpr float kR = 1.f / 127.f;
+  const bool tiny = top < 7.8886090522101181e-31f;  // 2^-100: the block stands for zeros
+  inv = tiny ? 0.f : __fdiv_rn(127.f, top);
+  const float q = __fmul_rn(top, kR);
+  scale = tiny ? 0.f : __fmaf_rn(__fmaf_rn(-127.f, q, top), kR, q);
 }
-__device__ __forceinline__ int q8_code(float x, float inv) { return __float2int_rn(__fmul_rn(x, inv)); }
+// rint(x * inv) for |x * inv| <= 127 as the low byte of the result: adding 1.5 * 2^23
+// rounds to an integer, to even on ties, without the conversion unit, whose rate (that of
+// the exponential) would bound the kernel. The product is rounded by itself: a fused
+// multiply-add, or packed pairs, which the compiler fuses, give other codes on ties.
+constexpr float kMagic = 12582912.f;
+__device__ __forceinline__ uint32_t q8_code(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), kMagic));
+}
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// Byte j of a word of codes as a float (exact): the code + 128 as the low bits of 2^23.
+__device__ __forceinline__ float code_float(uint32_t biased, int j) {
+  return __uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7550 | j)) - 8388736.f;
+}
 
-template <int L>  // maximum over groups of L neighbouring lanes
-__device__ __forceinline__ uint32_t group_max(uint32_t v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    const uint32_t w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = v > w ? v : w;
+// i / d for 0 <= i < 2^31 by a product (Granlund and Montgomery): d >= 1.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(uint32_t div) : d(div) {
+    shift = 0;
+    while ((1ull << shift) < div) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - div)) / div + 1);
   }
-  return v;
+  __device__ __forceinline__ uint32_t div(uint32_t i) const {
+    return (uint32_t)(((uint64_t)__umulhi(i, mul) + i) >> shift);
+  }
+};
+
+// Maxima of |g| and |u| over groups of L neighbouring lanes (a block of 64 columns), from
+// this lane's vectors. 16-bit types: as pairs of 16-bit integers, both tensors in one word
+// for the exchange between lanes.
+template <typename T, int L>
+__device__ __forceinline__ void block_tops(const Vec16<T>& g, const Vec16<T>& u, float& gt, float& ut) {
+  if (sizeof(T) == 2) {
+    const uint4 a = g.u, b = u.u;
+    constexpr uint32_t kAbs = 0x7fff7fffu;
+    const uint32_t x = __vmaxu2(__vmaxu2(a.x & kAbs, a.y & kAbs), __vmaxu2(a.z & kAbs, a.w & kAbs));
+    const uint32_t y = __vmaxu2(__vmaxu2(b.x & kAbs, b.y & kAbs), __vmaxu2(b.z & kAbs, b.w & kAbs));
+    // low halves of x and y in one word, high halves in another
+    uint32_t m = __vmaxu2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    union {
+      uint16_t s;
+      T t;
+    } c;
+    c.s = (uint16_t)(m & 0xffffu);
+    gt = Cvt<T>::to_f(c.t);
+    c.s = (uint16_t)(m >> 16);
+    ut = Cvt<T>::to_f(c.t);
+  } else {
+    uint32_t x = 0, y = 0;
+#pragma unroll
+    for (int j = 0; j < Vec16<T>::N; ++j) {
+      x = max(x, abs_bits(Cvt<T>::to_f(g.v[j])));
+      y = max(y, abs_bits(Cvt<T>::to_f(u.v[j])));
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+      y = max(y, __shfl_xor_sync(0xffffffffu, y, o));
+    }
+    gt = __uint_as_float(x);
+    ut = __uint_as_float(y);
+  }
 }
 
 struct FwdArgs {
@@ -79,54 +160,51 @@ struct BwdArgs {
   int64_t rows, cols;
 };
 
-// 8 / NE x 16-byte codes pieces: NE codes as one store.
+// The codes of one vector of NE floats in one store.
 template <int NE>
-__device__ __forceinline__ void st_codes(int8_t* p, const int (&q)[NE]) {
-  if (NE == 8) {
-    uint2 w;
-    w.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)q[3] << 24;
-    w.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | (uint32_t)q[7] << 24;
-    *reinterpret_cast<uint2*>(p) = w;
-  } else {
-    *reinterpret_cast<uint32_t*>(p) =
-        (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)q[3] << 24;
-  }
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[NE], float inv) {
+  uint32_t w[NE / 4];
+#pragma unroll
+  for (int j = 0; j < NE; j += 4)
+    w[j / 4] = low_bytes(q8_code(v[j], inv), q8_code(v[j + 1], inv), q8_code(v[j + 2], inv),
+                         q8_code(v[j + 3], inv));
+  if (NE == 8)
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[NE / 4 - 1]));
+  else
+    __stcs(reinterpret_cast<uint32_t*>(p), w[0]);
 }
 template <int NE>
-__device__ __forceinline__ void ld_codes(const int8_t* p, float (&v)[NE], float scale) {
-  uint32_t w[2];
+__device__ __forceinline__ void load_codes(const int8_t* p, uint32_t (&w)[NE / 4]) {
   if (NE == 8) {
     const uint2 t = __ldcs(reinterpret_cast<const uint2*>(p));
     w[0] = t.x;
-    w[1] = t.y;
+    w[NE / 4 - 1] = t.y;
   } else {
     w[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
-    w[1] = 0;
   }
-#pragma unroll
-  for (int j = 0; j < NE; ++j)
-    v[j] = (float)(int)(int8_t)(w[j >> 2] >> (8 * (j & 3))) * scale;
 }
 
 // Vector path: every row start 16-byte aligned (codes: 8 or 4 bytes), cols a
 // multiple of the vector. 64 / NE neighbouring lanes share a block.
 // kHasAct: SwiGLU forward (gate and up); otherwise quantise `gate` alone.
+// Bound by HBM: 8192 x 8960 bf16 (596 MB) in XXXF us. Before the conversions left the
+// special-function unit and the row index its 64-bit division, issue slots bounded it (150 us).
 template <typename T, bool kHasAct>
-__global__ void __launch_bounds__(256) q8_fwd_vec_kernel(FwdArgs a, int64_t vpr) {
+__global__ void __launch_bounds__(256) q8_fwd_vec_kernel(FwdArgs a, FastDiv vpr, uint32_t total) {
   constexpr int NE = Vec16<T>::N;
   constexpr int L = kBlk / NE;
   pdl_wait();
   pdl_trigger();
-  const int64_t total = a.rows * vpr;  // vpr: vectors per row, padded to whole blocks
   const int lane = threadIdx.x & 31;
   const T* gate = static_cast<const T*>(a.gate);
   const T* up = static_cast<const T*>(a.up);
   T* out = static_cast<T*>(a.out);
-  for (int64_t base = blockIdx.x * (int64_t)blockDim.x + (threadIdx.x & ~31); base < total;
-       base += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t i = base + lane;
-    const int64_t r = i / vpr;
-    const int64_t c = (i - r * vpr) * NE;
+  // total: vectors, rows padded to whole blocks (vpr vectors a row); below 2^31
+  for (uint32_t base = blockIdx.x * blockDim.x + (threadIdx.x & ~31u); base < total;
+       base += gridDim.x * blockDim.x) {
+    const uint32_t i = base + lane;
+    const uint32_t r = vpr.div(i);
+    const uint32_t c = (i - r * vpr.d) * NE;
     const bool in = i < total && c < a.cols;
     Vec16<T> g, u;
     g.u = u.u = make_uint4(0, 0, 0, 0);
@@ -134,37 +212,37 @@ __global__ void __launch_bounds__(256) q8_fwd_vec_kernel(FwdArgs a, int64_t vpr)
       g = ld16_stream(gate + r * a.gate_ld + c);
       if (kHasAct) u = ld16_stream(up + r * a.up_ld + c);
     }
+    float gt, ut;
+    block_tops<T, L>(g, u, gt, ut);
+    // half of a block's lanes divide for gate, the other half for up
+    const bool second = kHasAct && (lane & (L / 2));
+    float inv, sc;
+    q8_scale(second ? ut : gt, inv, sc);
+    const float inv_x = kHasAct ? __shfl_xor_sync(0xffffffffu, inv, L / 2) : 0.f;
+    if ((lane & (L / 2 - 1)) == 0 && i < total && c - (lane & (L - 1)) * NE < a.cols) {
+      if (second)
+        a.us[r * a.s_ld + c / kBlk] = sc;
+      else if (kHasAct || (lane & (L - 1)) == 0)
+        a.gs[r * a.s_ld + c / kBlk] = sc;
+    }
+    if (!in) continue;
     float gf[NE], uf[NE];
-    uint32_t gm = 0, um = 0;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
       gf[j] = Cvt<T>::to_f(g.v[j]);
-      gm = max(gm, abs_bits(gf[j]));
-      if (kHasAct) {
-        uf[j] = Cvt<T>::to_f(u.v[j]);
-        um = max(um, abs_bits(uf[j]));
-      }
+      uf[j] = Cvt<T>::to_f(u.v[j]);
     }
-    gm = group_max<L>(gm);
-    if (kHasAct) um = group_max<L>(um);
-    if (!in) continue;
-    float inv, sc;
-    int q[NE];
-    q8_scale(gm, inv, sc);
-#pragma unroll
-    for (int j = 0; j < NE; ++j) q[j] = q8_code(gf[j], inv);
-    st_codes<NE>(a.gq + r * a.q_ld + c, q);
-    if ((lane & (L - 1)) == 0) a.gs[r * a.s_ld + c / kBlk] = sc;
+    store_codes<NE>(a.gq + r * a.q_ld + c, gf, second ? inv_x : inv);
     if (kHasAct) {
-      q8_scale(um, inv, sc);
-#pragma unroll
-      for (int j = 0; j < NE; ++j) q[j] = q8_code(uf[j], inv);
-      st_codes<NE>(a.uq + r * a.q_ld + c, q);
-      if ((lane & (L - 1)) == 0) a.us[r * a.s_ld + c / kBlk] = sc;
+      store_codes<NE>(a.uq + r * a.q_ld + c, uf, second ? inv : inv_x);
       Vec16<T> o;
 #pragma unroll
-      for (int j = 0; j < NE; ++j)
-        o.v[j] = Cvt<T>::from_f((gf[j] * q8_sigmoid<T>(gf[j])) * uf[j]);
+      for (int j = 0; j < NE; j += 2) {
+        float x0, x1;
+        q8_swiglu2<T>(gf[j], gf[j + 1], uf[j], uf[j + 1], x0, x1);
+        o.v[j] = Cvt<T>::from_f(x0);
+        o.v[j + 1] = Cvt<T>::from_f(x1);
+      }
       st16_stream(out + r * a.out_ld + c, o);
     }
   }
@@ -194,11 +272,14 @@ __global__ void __launch_bounds__(256) q8_fwd_scalar_kernel(FwdArgs a, int64_t b
       gm = max(gm, abs_bits(g[e]));
       um = max(um, abs_bits(u[e]));
     }
-    gm = group_max<32>(gm);
-    um = group_max<32>(um);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      gm = max(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+      um = max(um, __shfl_xor_sync(0xffffffffu, um, o));
+    }
     float ginv, gsc, uinv = 0.f, usc = 0.f;
-    q8_scale(gm, ginv, gsc);
-    if (kHasAct) q8_scale(um, uinv, usc);
+    q8_scale(__uint_as_float(gm), ginv, gsc);
+    if (kHasAct) q8_scale(__uint_as_float(um), uinv, usc);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int64_t c = b * kBlk + lane + 32 * e;
@@ -225,25 +306,26 @@ __device__ __forceinline__ void q8_bwd_f(float d, float g, float u, float& dg, f
   h = si * u;
 }
 
+// 8192 x 8960 bf16 (596 MB) in XXXB us (108 with conversion instructions and 64-bit divisions).
 template <typename T, bool kHasH>
-__global__ void __launch_bounds__(256) q8_bwd_vec_kernel(BwdArgs a, int64_t vpr) {
+__global__ void __launch_bounds__(256) q8_bwd_vec_kernel(BwdArgs a, FastDiv vpr, uint32_t total) {
   constexpr int NE = Vec16<T>::N;
   pdl_wait();
   pdl_trigger();
-  const int64_t total = a.rows * vpr;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / vpr;
-    const int64_t c = (i - r * vpr) * NE;
+  for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < total; i += gridDim.x * blockDim.x) {
+    const uint32_t r = vpr.div(i);
+    const uint32_t c = (i - r * vpr.d) * NE;
     const Vec16<T> d = ld16_stream(static_cast<const T*>(a.dy) + r * a.dy_ld + c);
-    float g[NE], u[NE];
-    ld_codes<NE>(a.gq + r * a.q_ld + c, g, a.gs[r * a.s_ld + c / kBlk]);
-    ld_codes<NE>(a.uq + r * a.q_ld + c, u, a.us[r * a.s_ld + c / kBlk]);
+    uint32_t gw[NE / 4], uw[NE / 4];
+    load_codes<NE>(a.gq + r * a.q_ld + c, gw);
+    load_codes<NE>(a.uq + r * a.q_ld + c, uw);
+    const float gs = a.gs[r * a.s_ld + c / kBlk], us = a.us[r * a.s_ld + c / kBlk];
     Vec16<T> dg, du, h;
 #pragma unroll
     for (int j = 0; j < NE; ++j) {
       float x, y, z;
-      q8_bwd_f<T>(Cvt<T>::to_f(d.v[j]), g[j], u[j], x, y, z);
+      q8_bwd_f<T>(Cvt<T>::to_f(d.v[j]), code_float(gw[j / 4] ^ 0x80808080u, j & 3) * gs,
+                  code_float(uw[j / 4] ^ 0x80808080u, j & 3) * us, x, y, z);
       dg.v[j] = Cvt<T>::from_f(x);
       du.v[j] = Cvt<T>::from_f(y);
       if (kHasH) h.v[j] = Cvt<T>::from_f(z);
@@ -279,6 +361,10 @@ int grid_for(int64_t threads) {
   return blocks < 1 ? 1 : (int)blocks;
 }
 
+// The vector kernels index vectors in 31 bits and step past the end by up to one grid
+// (8 x 256 threads on each SM); larger tensors take the scalar kernels' 64-bit indices.
+constexpr int64_t kMaxVecs = (int64_t(1) << 31) - (int64_t(1) << 20);
+
 template <typename T>
 bool vec_ok(const void* p, int64_t ld) {
   return aligned16(p) && (ld * (int64_t)sizeof(T)) % 16 == 0;
@@ -295,11 +381,10 @@ int run_fwd(const FwdArgs& a, cudaStream_t st) {
   const bool vec = a.cols % NE == 0 && vec_ok<T>(a.gate, a.gate_ld) && codes_ok<NE>(a.gq, a.q_ld) &&
                    (!kHasAct || (vec_ok<T>(a.up, a.up_ld) && vec_ok<T>(a.out, a.out_ld) &&
                                  codes_ok<NE>(a.uq, a.q_ld)));
-  if (vec) {
-    const int64_t vpr = bpr * (kBlk / NE);
-    return cuda_status(launch_pdl(q8_fwd_vec_kernel<T, kHasAct>, dim3(grid_for(a.rows * vpr)),
-                                  dim3(256), 0, st, a, vpr));
-  }
+  const int64_t vpr = bpr * (kBlk / NE), total = a.rows * vpr;
+  if (vec && total < kMaxVecs)
+    return cuda_status(launch_pdl(q8_fwd_vec_kernel<T, kHasAct>, dim3(grid_for(total)), dim3(256), 0,
+                                  st, a, FastDiv((uint32_t)vpr), (uint32_t)total));
   return cuda_status(launch_pdl(q8_fwd_scalar_kernel<T, kHasAct>, dim3(grid_for(a.rows * bpr * 32)),
                                 dim3(256), 0, st, a, bpr));
 }
@@ -310,11 +395,10 @@ int run_bwd_h(const BwdArgs& a, cudaStream_t st) {
   const bool vec = a.cols % NE == 0 && vec_ok<T>(a.dy, a.dy_ld) && vec_ok<T>(a.dg, a.dg_ld) &&
                    vec_ok<T>(a.du, a.du_ld) && codes_ok<NE>(a.gq, a.q_ld) &&
                    codes_ok<NE>(a.uq, a.q_ld) && (!kHasH || vec_ok<T>(a.h, a.h_ld));
-  if (vec) {
-    const int64_t vpr = a.cols / NE;
-    return cuda_status(launch_pdl(q8_bwd_vec_kernel<T, kHasH>, dim3(grid_for(a.rows * vpr)),
-                                  dim3(256), 0, st, a, vpr));
-  }
+  const int64_t vpr = a.cols / NE, total = a.rows * vpr;
+  if (vec && total < kMaxVecs)
+    return cuda_status(launch_pdl(q8_bwd_vec_kernel<T, kHasH>, dim3(grid_for(total)), dim3(256), 0,
+                                  st, a, FastDiv((uint32_t)vpr), (uint32_t)total));
   return cuda_status(launch_pdl(q8_bwd_scalar_kernel<T, kHasH>, dim3(grid_for(a.rows * a.cols)),
                                 dim3(256), 0, st, a));
 }
