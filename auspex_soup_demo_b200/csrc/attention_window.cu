@@ -5,15 +5,9 @@
 // sliding-window layers.
 //
 // Key tiles without a visible pair are never loaded, so the products cover about
-// window + sinks keys a query. What then bounds the kernels is not the tensor pipe
-// but the chain TMEM read -> softmax -> P -> product of one tile, so each kernel
-// keeps sixteen compute warps (four a scheduler) on rows split over several
-// threads, and reads S out of TMEM once, into registers.
-//
-// Forward (one CTA per (batch, query head, pair of 128-query tiles A, B)): TMEM S_A,
-// S_B, O_A, O_B (128 columns each); P_X overwrites the first 64 columns of S_X as
-// bf16 pairs and is the A operand of O_X += P_X V read from TMEM. Two threads share
-// a query row (64 keys each) and exchange their row maxima through shared memory.
+// window + sinks keys a query.
+// Forward: one CTA per (batch, query head, pair of 128-query tiles), keys in blocks of 64,
+// one thread per query row.
 // Backward: dK / dV per (batch, KV head, key tile): the CTA runs through the query
 // heads of its group and their queries in 128-query steps and keeps dK, dV in TMEM, so
 // no per-head partials reach memory; the far queries of the sink tiles, which every
@@ -24,8 +18,7 @@
 // Every mbarrier wait is bounded as in attention.cu: on expiry the role records a
 // code in the device error word, raises the CTA's abort flag, the producer waits
 // (bounded) for its copies, the MMA warp drains its MMAs, and the CTA frees TMEM and
-// returns. The forward's named barriers between the two warps of a row pair are
-// released by a leaving warp (bar.arrive), so no warp waits there for a warp that gave up.
+// returns. Launches are plain ones: for kernels of 15 us and more an early start gains nothing.
 #include "attention_common.cuh"
 
 namespace soup {
@@ -79,6 +72,19 @@ __device__ __forceinline__ uint32_t queries_seeing(int key, int q0, int S, int w
 __device__ __forceinline__ int mask_kind(uint32_t m, uint32_t all) {
   if (__all_sync(0xffffffffu, (m & all) == 0u)) return 0;
   return __all_sync(0xffffffffu, (m & all) == all) ? 1 : 2;
+}
+
+// 32 lanes x 16 fp32 columns from TMEM without waiting (see tmem_ld32_async).
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  __syncwarp();
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 
 // ---- the MMA warp ----
@@ -291,7 +297,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  pdl_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -520,7 +525,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     }
   }
 
-  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -677,7 +681,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  pdl_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -906,7 +909,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -920,8 +922,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 // all tiles. Slots are added in a fixed order. Four elements per thread; one block
 // takes 8 key rows of one tile.
 __global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles) {
-  pdl_wait();
-  pdl_trigger();
   const int nq = (a.S + kTile - 1) / kTile;
   const int rows8 = blockIdx.x % (kTile / 8);
   const int i = blockIdx.x / (kTile / 8);
@@ -1042,7 +1042,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
-  pdl_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -1192,26 +1191,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) w = bounded_wait(dp_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
       if (!(ok = warp_ok(w))) break;
       tc_fence_after();
-      float dp[32];
-      tmem_ld32_async(tmem + 128 + cb + lane_off, dp);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(dp_empty);
       uint32_t dw[16];
-      if (kind == 0) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) dw[e] = 0u;
-      } else {
+      for (int c = 0; c < 32; c += 16) {  // in two pieces: no register spills
+        float dp[16];
+        tmem_ld16_async(tmem + 128 + cb + c + lane_off, dp);
+        tmem_ld_wait();
+        if (c == 16) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(dp_empty);
+        }
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
+        for (int e = 0; e < 16; e += 2) {
           float d0, d1;
-          f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0, d1);
+          f2_unpack(f2_mul(f2_pack(p[c + e], p[c + e + 1]), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0,
+                    d1);
           if (kind == 2) {
-            if (!(mk & (1u << e))) d0 = 0.f;
-            if (!(mk & (2u << e))) d1 = 0.f;
+            if (!(mk & (1u << (c + e)))) d0 = 0.f;
+            if (!(mk & (2u << (c + e)))) d1 = 0.f;
           }
-          dw[e >> 1] = pack_bf16(d0, d1);
+          dw[(c + e) >> 1] = kind == 0 ? 0u : pack_bf16(d0, d1);
         }
       }
       if (j > 0) {  // the previous tile's dQ product has read dS
@@ -1248,7 +1248,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
-  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -1356,9 +1355,9 @@ int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const voi
             (int)(window < seq ? window : seq), (int)(sinks < seq ? sinks : seq),
             static_cast<bf16*>(out), lse, wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
   const int64_t npair = ((seq + kTile - 1) / kTile + 1) / 2;
-  return cuda_status(launch_pdl(win_fwd_kernel, dim3((unsigned)(batch * heads * npair)),
-                                dim3(kFwdThreads), WinFwdSmem::kBytes, as_stream(stream), mq, mk, mv, a,
-                                err));
+  win_fwd_kernel<<<(unsigned)(batch * heads * npair), kFwdThreads, WinFwdSmem::kBytes,
+                   as_stream(stream)>>>(mq, mk, mv, a, err);
+  return launch_status();
 }
 
 size_t soup_attention_window_bwd_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
@@ -1430,10 +1429,9 @@ int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const voi
   const int64_t rows = (int64_t)B * S * H;
   int64_t dot_blocks = (rows + 16 * kDotRows - 1) / (16 * kDotRows);  // 16 half-warps per block
   if (dot_blocks > 16 * num_sms()) dot_blocks = 16 * num_sms();
-  if ((rc = cuda_status(launch_pdl(attn_bwd_dot_kernel, dim3((unsigned)dot_blocks), dim3(256), 0, st,
-                                   static_cast<const bf16*>(dout), static_cast<const bf16*>(out),
-                                   lse, B, H, S, dvec, nl2))))
-    return rc;
+  attn_bwd_dot_kernel<<<(unsigned)dot_blocks, 256, 0, st>>>(
+      static_cast<const bf16*>(dout), static_cast<const bf16*>(out), lse, B, H, S, dvec, nl2);
+  if ((rc = launch_status())) return rc;
   const int win = (int)(window < seq ? window : seq);
   const int snk = win == S ? 0 : (int)(sinks < seq ? sinks : seq);
   BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, win, snk, dvec, nl2,
@@ -1441,16 +1439,14 @@ int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const voi
             p.heads_per, p.n_sink, p.segs, p.seg_steps,
             wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
   const int nt = (S + kTile - 1) / kTile;
-  if ((rc = cuda_status(launch_pdl(win_dkdv_kernel, dim3((unsigned)p.units), dim3(kThreads),
-                                   WinDkvSmem::kBytes, st, mq, mk, mv, mdo, a, err))))
-    return rc;
-  if ((rc = cuda_status(launch_pdl(win_dq_kernel, dim3((unsigned)(B * H * nt)), dim3(kThreads),
-                                   WinDqSmem::kBytes, st, mq, mk, mv, mdo, a, err))))
-    return rc;
+  win_dkdv_kernel<<<(unsigned)p.units, kThreads, WinDkvSmem::kBytes, st>>>(mq, mk, mv, mdo, a, err);
+  if ((rc = launch_status())) return rc;
+  win_dq_kernel<<<(unsigned)(B * H * nt), kThreads, WinDqSmem::kBytes, st>>>(mq, mk, mv, mdo, a, err);
+  if ((rc = launch_status())) return rc;
   const int tiles = p.groups > 1 ? nt : p.n_sink;  // key tiles whose sums are in slots
   if (tiles == 0) return SOUP_OK;
-  return cuda_status(launch_pdl(win_dkdv_sum_kernel, dim3((unsigned)(B * Hk * tiles * (kTile / 8))),
-                                dim3(256), 0, st, a, tiles));
+  win_dkdv_sum_kernel<<<(unsigned)(B * Hk * tiles * (kTile / 8)), 256, 0, st>>>(a, tiles);
+  return launch_status();
 }
 
 }  // extern "C"
