@@ -74,24 +74,10 @@ __device__ __forceinline__ int mask_kind(uint32_t m, uint32_t all) {
   return __all_sync(0xffffffffu, (m & all) == all) ? 1 : 2;
 }
 
-// 32 lanes x 16 fp32 columns from TMEM without waiting (see tmem_ld32_async).
-__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, float (&v)[16]) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  __syncwarp();
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
 // ---- the MMA warp ----
 // The whole warp walks the schedule converged and one elected lane issues, so that
 // descriptors and addresses live in uniform registers. Issued from a lane == 0 branch
-// each product costs about 110 cycles of operand moves, more than a 128 x 64 x 16 product
-// takes (32), and the issuing thread bounded all three kernels: 3400 cycles per forward
+// each product took about 110 cycles, more than a 128 x 64 x 16 product does (75), and the issuing thread bounded all three kernels: 3400 cycles per forward
 // step of two 64-key blocks of which the softmax needed 1900.
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t v;
@@ -204,6 +190,10 @@ struct FwdArgs {
 // double buffered the products run a block ahead: the softmax finds its next S ready
 // and its chain holds no product. Shared memory: Q_A, Q_B (32 KB each), one ring of
 // 10 x 16 KB through which K and V blocks pass (K0 V0 K1 V1 ...), barriers.
+// At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 158 us, 612 TFLOP/s of the
+// visible pairs' products; bound by the softmax warps (TMEM reads and exponentials of a
+// block). Measured slower there: 16 softmax warps, two per row (166 us), and 128-key
+// blocks with P over S.
 constexpr int kFwdWarps = 8;  // softmax warps: four per query tile, one row per thread
 constexpr int kFwdThreads = 64 + 32 * kFwdWarps;
 constexpr int kBlk = 64;      // keys per block
@@ -610,6 +600,10 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
 // of N = 64 ones (75 cycles of issue either way). Shared memory: K, V (32 KB each, loaded
 // once for all query heads), two stages of (Q, dO) tiles with their nl2 / D vectors. A
 // compute thread owns 32 queries of one key row.
+// At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 238 us. Bound by the chain
+// TMEM read, exponentials, TMEM write of the compute warps, whose TMEM reads take 600 to
+// 1000 cycles while products run; exponentials by polynomial, eight compute warps and
+// P through shared memory measured no faster.
 constexpr int kDkvStages = 2;
 struct WinDkvSmem {
   static constexpr int kK = 0;
@@ -956,13 +950,14 @@ __global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles)
   *reinterpret_cast<uint2*>(a.dv + o) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
-// dQ of one query tile: TMEM columns S 0, dP 128, dQ 256, dS 384 (bf16, two per
-// column: the A operand of dQ += dS K read from TMEM). S and dP have barriers of their own:
+// dQ of one query tile: TMEM columns S 0, dP 128, dQ 256, two dS buffers 384 and 448 (bf16, two
+// per column: the A operand of dQ += dS K read from TMEM). S and dP have barriers of their own:
 // S(j + 1) starts when S(j) has been read, which is during dP(j), so the tensor pipe does not
-// wait for the TMEM reads. Shared memory: Q and dO
-// (32 KB each, loaded once), a K ring (3 x 32 KB; a stage frees after its dQ
-// product) and a V ring (2 x 32 KB; a stage frees after its dP product). A compute
-// thread owns 32 keys of one query row of each tile.
+// wait for the TMEM reads, and with two dS buffers the next dS is written while the product
+// of the last one runs (187 us with two against 216 with one, at 1 x 16001 tokens, 12 heads
+// over 2, window 1000, 16 sinks). Shared memory: Q and dO (32 KB each, loaded once), a K
+// ring (3 x 32 KB; a stage frees after its dQ product) and a V ring (2 x 32 KB; a stage
+// frees after its dP product). A compute thread owns 32 keys of one query row of each tile.
 constexpr int kDqKStages = 3;
 constexpr int kDqVStages = 2;
 struct WinDqSmem {
@@ -972,8 +967,8 @@ struct WinDqSmem {
   static constexpr int kV = kK + kDqKStages * kTileBytes;
   static constexpr int kBar = kV + kDqVStages * kTileBytes;
   // qdo_full, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full, s_empty, dp_full,
-  // dp_empty, ds_full, buf_free, acc_done, drain
-  static constexpr int kNumBars = 1 + 2 * kDqKStages + 2 * kDqVStages + 8;
+  // dp_empty, ds_full[2], ds_free[2], acc_done, drain
+  static constexpr int kNumBars = 1 + 2 * kDqKStages + 2 * kDqVStages + 10;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kUsed = kMisc + 16;
   static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
@@ -1002,8 +997,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kB = 1 + 2 * kDqKStages + 2 * kDqVStages;
   const uint32_t s_full = bar0 + 8u * kB, s_empty = bar0 + 8u * (kB + 1);
   const uint32_t dp_full = bar0 + 8u * (kB + 2), dp_empty = bar0 + 8u * (kB + 3);
-  const uint32_t ds_full = bar0 + 8u * (kB + 4), buf_free = bar0 + 8u * (kB + 5);
-  const uint32_t acc_done = bar0 + 8u * (kB + 6), drain_bar = bar0 + 8u * (kB + 7);
+  // of tile j: its dS buffer is j & 1, the phase (j >> 1) & 1
+  auto ds_full = [&](int j) { return bar0 + 8u * (kB + 4 + (j & 1)); };
+  auto ds_free = [&](int j) { return bar0 + 8u * (kB + 6 + (j & 1)); };
+  const uint32_t acc_done = bar0 + 8u * (kB + 8), drain_bar = bar0 + 8u * (kB + 9);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
 
@@ -1021,7 +1018,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kNumBars; ++i) {
       const uint32_t bar = bar0 + 8u * i;
-      mbar_init(bar, bar == s_empty || bar == dp_empty || bar == ds_full ? kWarps : 1);
+      mbar_init(bar, bar == s_empty || bar == dp_empty || bar == ds_full(0) || bar == ds_full(1)
+                         ? kWarps
+                         : 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1129,13 +1128,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int j = 0; j < n && ok; ++j) {
       const int sk = j % kDqKStages;
       if (j + 1 < n && !(ok = issue_sd(j + 1))) break;
-      if (!(ok = wait(ds_full, j & 1))) break;
+      if (!(ok = wait(ds_full(j), (j >> 1) & 1))) break;
       tc_fence_after();
 #pragma unroll
       for (int kk = 0; kk < kTile / 16; ++kk)  // dQ += dS K (dS from TMEM: 8 columns per 16 keys)
-        mma_ts(leader, tmem + 256, tmem + 384 + kk * 8, k_mn.at(sk * kTileBytes + mnmajor_step(kk)),
+        mma_ts(leader, tmem + 256, tmem + 384 + (j & 1) * 64 + kk * 8, k_mn.at(sk * kTileBytes + mnmajor_step(kk)),
                k_mn.hi, kIdescKM, (j > 0 || kk > 0) ? 1u : 0u);
-      commit(leader, buf_free);
+      commit(leader, ds_free(j));
       commit(leader, k_empty(sk));
     }
     if (ok) commit(leader, acc_done);
@@ -1191,39 +1190,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) w = bounded_wait(dp_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
       if (!(ok = warp_ok(w))) break;
       tc_fence_after();
+      float dp[32];
+      tmem_ld32_async(tmem + 128 + cb + lane_off, dp);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_empty);
+#pragma unroll
+      for (int e = 0; e < 32; e += 2)
+        f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), p[e], p[e + 1]);
+      if (kind != 1) {  // hidden keys may hold anything: select, do not scale
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!(mk & (1u << e))) p[e] = 0.f;
+      }
       uint32_t dw[16];
 #pragma unroll
-      for (int c = 0; c < 32; c += 16) {  // in two pieces: no register spills
-        float dp[16];
-        tmem_ld16_async(tmem + 128 + cb + c + lane_off, dp);
-        tmem_ld_wait();
-        if (c == 16) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(dp_empty);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          float d0, d1;
-          f2_unpack(f2_mul(f2_pack(p[c + e], p[c + e + 1]), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), d0,
-                    d1);
-          if (kind == 2) {
-            if (!(mk & (1u << (c + e)))) d0 = 0.f;
-            if (!(mk & (2u << (c + e)))) d1 = 0.f;
-          }
-          dw[(c + e) >> 1] = kind == 0 ? 0u : pack_bf16(d0, d1);
-        }
-      }
-      if (j > 0) {  // the previous tile's dQ product has read dS
-        if (lane == 0) w = bounded_wait(buf_free, (j - 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      for (int e = 0; e < 16; ++e) dw[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
+      if (j > 1) {  // the dQ product of the tile before the previous one has read this buffer
+        if (lane == 0)
+          w = bounded_wait(ds_free(j), ((j - 2) >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
         if (!(ok = warp_ok(w))) break;
         tc_fence_after();
       }
-      tmem_st16u(ds_tmem, dw);
+      tmem_st16u(ds_tmem + (j & 1) * 64, dw);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) mbar_arrive(ds_full(j));
     }
     if (ok) {
       bool w = true;
