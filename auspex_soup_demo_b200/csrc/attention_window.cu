@@ -1132,8 +1132,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
 #pragma unroll
       for (int kk = 0; kk < kTile / 16; ++kk)  // dQ += dS K (dS from TMEM: 8 columns per 16 keys)
-        mma_ts(leader, tmem + 256, tmem + 384 + (j & 1) * 64 + kk * 8, k_mn.at(sk * kTileBytes + mnmajor_step(kk)),
-               k_mn.hi, kIdescKM, (j > 0 || kk > 0) ? 1u : 0u);
+        mma_ts(leader, tmem + 256, tmem + 384 + (j & 1) * 64 + kk * 8,
+               k_mn.at(sk * kTileBytes + mnmajor_step(kk)), k_mn.hi, kIdescKM, (j > 0 || kk > 0) ? 1u : 0u);
       commit(leader, ds_free(j));
       commit(leader, k_empty(sk));
     }

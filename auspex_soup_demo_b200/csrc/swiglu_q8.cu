@@ -377,7 +377,9 @@ int grid_for(int64_t threads) {
 }
 
 // The vector kernels index vectors in 31 bits and step past the end by up to two grids
-// (2 x 8 x 256 threads on each SM); larger tensors take the scalar kernels' 64-bit indices.
+// (2 x 8 x 256 threads on each SM), and columns in 32; larger tensors take the scalar kernels'
+// 64-bit indices.
+constexpr int64_t kMaxCols = int64_t(1) << 31;
 constexpr int64_t kMaxVecs = (int64_t(1) << 31) - (int64_t(1) << 20);
 
 template <typename T>
@@ -397,7 +399,7 @@ int run_fwd(const FwdArgs& a, cudaStream_t st) {
                    (!kHasAct || (vec_ok<T>(a.up, a.up_ld) && vec_ok<T>(a.out, a.out_ld) &&
                                  codes_ok<NE>(a.uq, a.q_ld)));
   const int64_t vpr = bpr * (kBlk / NE), total = a.rows * vpr;
-  if (vec && total < kMaxVecs)
+  if (vec && total < kMaxVecs && a.cols < kMaxCols)
     return cuda_status(launch_pdl(q8_fwd_vec_kernel<T, kHasAct>, dim3(grid_for(total)), dim3(256), 0,
                                   st, a, FastDiv((uint32_t)vpr), (uint32_t)total));
   return cuda_status(launch_pdl(q8_fwd_scalar_kernel<T, kHasAct>, dim3(grid_for(a.rows * bpr * 32)),
@@ -411,7 +413,7 @@ int run_bwd_h(const BwdArgs& a, cudaStream_t st) {
                    vec_ok<T>(a.du, a.du_ld) && codes_ok<NE>(a.gq, a.q_ld) &&
                    codes_ok<NE>(a.uq, a.q_ld) && (!kHasH || vec_ok<T>(a.h, a.h_ld));
   const int64_t vpr = a.cols / NE, total = a.rows * vpr;
-  if (vec && total < kMaxVecs)
+  if (vec && total < kMaxVecs && a.cols < kMaxCols)
     return cuda_status(launch_pdl(q8_bwd_vec_kernel<T, kHasH>, dim3(grid_for(total)), dim3(256), 0,
                                   st, a, FastDiv((uint32_t)vpr), (uint32_t)total));
   return cuda_status(launch_pdl(q8_bwd_scalar_kernel<T, kHasH>, dim3(grid_for(a.rows * a.cols)),

@@ -210,25 +210,33 @@ def soup_attention(module, query, key, value, attention_mask, dropout: float = 0
                    scaling=None, is_causal=None, **kwargs):
     """transformers ``AttentionInterface`` function: (attn_output [B, S, H, D], None).
 
-    A ``sliding_window`` (transformers passes the layer's) limits each query to its
-    last ``sliding_window`` keys, plus the first ``attention_sink_tokens`` of the
-    sequence when the module's config sets that. Causal when the module is (and the query is longer than one token), as
+    Causal when the module is (and the query is longer than one token), as
     transformers' SDPA path decides (``integrations/sdpa_attention.py``). Calls
-    outside the kernels' form go to transformers' SDPA function."""
+    outside the kernels' form go to transformers' SDPA function.
+
+    A ``sliding_window`` (transformers passes the layer's) limits each query of a
+    causal module to its last ``sliding_window`` keys, plus the first
+    ``attention_sink_tokens`` of the sequence when the module's config sets that. With
+    a cache the queries are the last tokens of the keys; sinks need the whole sequence
+    in one call, since a sliding layer's cache drops the first tokens."""
     window = kwargs.get("sliding_window")
-    if window is not None and query.shape[2] == key.shape[2]:
+    n_q, n_k = query.shape[2], key.shape[2]
+    if (window is not None and attention_mask is None and n_q <= n_k
+            and (is_causal if is_causal is not None else getattr(module, "is_causal", True))):
         # transformers builds no mask for an attention function of its own registry
         # entry, so the window is this function's to apply
-        causal = is_causal if is_causal is not None else getattr(module, "is_causal", True)
         sinks = int(getattr(getattr(module, "config", None), "attention_sink_tokens", 0) or 0)
-        if causal and attention_mask is None and window < query.shape[2]:
-            scale = scaling if scaling is not None else query.shape[-1] ** -0.5
-            if (not dropout and query.is_cuda and query.shape[-1] == HEAD_DIM
+        if sinks and n_q < n_k and window <= n_k:
+            raise ValueError("soup_attention: attention_sink_tokens with a cache longer than the sliding "
+                             "window; run the whole sequence in one call (use_cache=False)")
+        if window < n_k:
+            if (n_q == n_k and not dropout and query.is_cuda and query.shape[-1] == HEAD_DIM
                     and query.dtype == key.dtype == value.dtype == torch.bfloat16):
+                scale = scaling if scaling is not None else query.shape[-1] ** -0.5
                 return window_attention(query, key, value, float(scale), window, sinks), None
-            i = torch.arange(query.shape[2], device=query.device)
-            dist = i[:, None] - i[None, :]
-            attention_mask = ((dist >= 0) & ((dist < window) | (i[None, :] < sinks)))[None, None]
+            k_pos = torch.arange(n_k, device=query.device)
+            dist = (k_pos[:, None] - k_pos[None, :])[n_k - n_q:]
+            attention_mask = ((dist >= 0) & ((dist < window) | (k_pos[None, :] < sinks)))[None, None]
     if not _supported(module, query, key, value, attention_mask, dropout):
         from transformers.integrations.sdpa_attention import sdpa_attention_forward
 

@@ -705,3 +705,21 @@ def test_model_with_sliding_window_layers():
     with torch.no_grad():
         x = a(ids).logits.double()
     assert float((x - z).norm() / z.norm()) <= 0.02
+
+
+def test_model_with_sliding_window_layers_and_a_cache():
+    kw = dict(use_sliding_window=True, sliding_window=20, max_window_layers=1)
+    ids = torch.randint(0, 1000, (2, 70), generator=_gen(8), device=DEV)
+    a = _model(2, "soup", **kw)
+    with torch.no_grad():
+        whole = a(ids).logits.double()
+        first = a(ids[:, :60], use_cache=True)
+        rest = [first.logits]
+        cache = first.past_key_values
+        for i in range(60, 70):
+            step = a(ids[:, i:i + 1], past_key_values=cache, use_cache=True)
+            cache = step.past_key_values
+            rest.append(step.logits)
+    rest = torch.cat(rest, 1).double()
+    # the same model by two bf16 attention kernels through two layers
+    assert float((whole - rest).norm() / whole.norm()) <= 0.02

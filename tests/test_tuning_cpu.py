@@ -191,3 +191,43 @@ def test_window_tile_lists_cover_every_visible_key(S, window, sinks):
         for key in range(kt * 128, min(S, kt * 128 + 128)):
             last = S - 1 if key < sinks else min(S - 1, key + window - 1)
             assert first <= key // 64 and last // 64 < first + n
+
+
+class _Layer(torch.nn.Module):
+    """What soup_attention reads of a transformers attention layer."""
+
+    def __init__(self, groups, sinks=0):
+        super().__init__()
+        self.is_causal, self.num_key_value_groups = True, groups
+        self.config = type("Config", (), {"attention_sink_tokens": sinks})()
+
+
+@pytest.mark.parametrize("n_q,n_k,window,sinks", [
+    (13, 13, 4, 0), (13, 13, 4, 2), (13, 13, 1, 0), (13, 13, 40, 3), (3, 13, 4, 0), (1, 13, 4, 0),
+    (1, 4, 4, 0), (5, 8, 4, 0), (1, 1, 1, 0),
+])
+def test_sliding_layer_off_the_kernels(n_q, n_k, window, sinks):
+    """Prefill, chunks and single tokens against a cache; fp64, so only the sums' order differs."""
+    from auspex_soup_demo_b200.kernels.attention import soup_attention
+
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(2, h, n, 16, generator=g, dtype=torch.float64)
+               for h, n in ((4, n_q), (2, n_k), (2, n_k)))
+    out, _ = soup_attention(_Layer(2, sinks), q, k, v, None, scaling=0.3, sliding_window=window)
+    ref = torch.empty(2, n_q, 4, 16, dtype=torch.float64)
+    for h in range(4):
+        for i in range(n_q):
+            pos = n_k - n_q + i
+            see = [j for j in range(pos + 1) if pos - j < window or j < sinks]
+            p = torch.softmax(0.3 * (k[:, h // 2, see] @ q[:, h, i, :, None])[..., 0], -1)
+            ref[:, i, h] = (p[:, None] @ v[:, h // 2, see])[:, 0]
+    assert (out - ref).abs().max() <= 1e-13 * v.abs().max()
+
+
+@pytest.mark.parametrize("n_q,n_k", [(1, 4), (1, 13), (5, 8)])
+def test_sliding_layer_refuses_sinks_beyond_a_cache(n_q, n_k):
+    from auspex_soup_demo_b200.kernels.attention import soup_attention
+
+    q, k = torch.zeros(1, 2, n_q, 16), torch.zeros(1, 2, n_k, 16)
+    with pytest.raises(ValueError, match="attention_sink_tokens"):
+        soup_attention(_Layer(1, 2), q, k, k, None, sliding_window=4)
