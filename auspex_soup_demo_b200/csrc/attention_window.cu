@@ -15,6 +15,8 @@
 // dQ per (batch, query head, query tile). Both recompute P from the log-sum-exp; no
 // atomics, results are bitwise reproducible.
 //
+// A CTA leaves only after every asynchronous arrival on its barriers has landed: the
+// producer waits for its copies, the MMA warp for its commits.
 // Every mbarrier wait is bounded as in attention.cu: on expiry the role records a
 // code in the device error word, raises the CTA's abort flag, the producer waits
 // (bounded) for its copies, the MMA warp drains its MMAs, and the CTA frees TMEM and
@@ -382,6 +384,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (ok && i < n_b) ok = issue_pv(1, i);
       if (ok && i + 2 < n_b) ok = issue_s(1, i + 2);
     }
+    // the ring's last arrivals (nothing else waits for them)
+    for (int i = 2 * n > kRing ? 2 * n - kRing : 0; i < 2 * n && ok; ++i)
+      ok = wait(empty(i % kRing), (i / kRing) & 1);
     if (!ok && issued) {
       commit(leader, drain_bar);
       uint64_t t0 = tc::globaltimer();
@@ -765,6 +770,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && i + 1 < total) ok = issue_s(1, i + 1);
     }
     if (ok) commit(leader, acc_done);
+    for (int i = total > kDkvStages ? total - kDkvStages : 0; i < total && ok; ++i)
+      ok = wait(empty(i % kDkvStages), (i / kDkvStages) & 1);
     if (!ok && issued) {
       commit(leader, drain_bar);
       uint64_t t0 = tc::globaltimer();
@@ -1138,6 +1145,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       commit(leader, k_empty(sk));
     }
     if (ok) commit(leader, acc_done);
+    for (int j = n > kDqKStages ? n - kDqKStages : 0; j < n && ok; ++j) {
+      ok = wait(k_empty(j % kDqKStages), (j / kDqKStages) & 1);
+      if (ok && j >= n - kDqVStages) ok = wait(v_empty(j % kDqVStages), (j / kDqVStages) & 1);
+      if (ok && j >= n - 2) ok = wait(ds_free(j), (j >> 1) & 1);
+    }
     if (!ok && issued) {
       commit(leader, drain_bar);
       uint64_t t0 = tc::globaltimer();
