@@ -194,6 +194,17 @@ def stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
+def once_differentiable(backward):
+    """``torch.autograd.function.once_differentiable`` whose checks (3 us a call) run only
+    when a graph of the backward itself is asked for (create_graph)."""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
 def call(fn: str, device: torch.device, *args) -> None:
     """Invoke entry point `fn` with `device` current; raise on failure."""
     f = getattr(lib(), fn)

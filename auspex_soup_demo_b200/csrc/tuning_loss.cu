@@ -6,8 +6,8 @@
 // kernel sums each sequence (one block per sequence and chunk of tokens) into
 // one record per block, a second, one block, joins the records in a fixed
 // order (no atomics: the same inputs give the same bits) and writes the loss,
-// the metrics and one gradient factor per sequence; the backward is one
-// elementwise pass. Labels equal to ignore_index mark masked tokens: their
+// the metrics and one gradient factor per sequence; when the blocks fit a
+// cluster, one launch does both. The backward is one elementwise pass. Labels equal to ignore_index mark masked tokens: their
 // values are selected away, never multiplied, so infinities and NaN there do
 // not reach a sum. Sums over tokens run in 64 bits: thousands of terms of
 // either sign leave a difference that 32 bits would round away, and the adds
@@ -18,18 +18,56 @@ namespace soup {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = 4096;  // tokens per block of the summing kernels
+// Tokens per block of the summing kernels: forward of the policy loss over 2 x 16384 tokens
+// 8.5 us (4096: 11.1, 1024: 7.1), over 2048 x 2048 25.3 us (4096: 25.9, 1024: 31.8).
+constexpr int kChunk = 2048;
 constexpr int kUnroll = 4;    // tokens per thread whose loads are in flight together
 
-__device__ __forceinline__ double block_sum(double v, double* sh) {
+// v[i] = its sum over the block, in every thread; sh: N doubles a warp. At most 32 warps.
+template <int N>
+__device__ __forceinline__ void block_sums(double (&v)[N], double* sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (lane == 0) sh[warp * N + i] = v[i];
+  }
   __syncthreads();
-  double t = 0.0;
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += sh[i];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = lane < warps ? sh[lane * N + i] : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
   __syncthreads();
-  return t;
+}
+
+// Few blocks (the usual step: a handful of sequences) sum and join in one launch: the
+// blocks form one cluster, whose first block joins the records after a cluster barrier.
+// 4 x 512 tokens, in a graph: preference 3.3 us against 3.7 with two launches, policy 3.9
+// against 7.5; eager calls save the launch (3 us of host time).
+constexpr int kClusterBlocks = 8;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned blocks, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = blocks;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
 // ------------------------------------------------------------ preference ----
@@ -48,11 +86,8 @@ struct PrefArgs {
 };
 
 // records[n][c] = (sum of log ratios, labelled tokens) of sequence n, chunk c
-__global__ void __launch_bounds__(kThreads) pref_sum_kernel(PrefArgs a, int chunks,
-                                                            double2* __restrict__ records) {
-  __shared__ double sh[kThreads / 32];
-  pdl_wait();
-  pdl_trigger();
+__device__ __forceinline__ void pref_sum(const PrefArgs& a, int chunks, double2* records) {
+  __shared__ double sh[2 * kThreads / 32];
   const int64_t n = blockIdx.x / chunks;
   const int c = blockIdx.x % chunks;
   const int64_t s0 = (int64_t)c * kChunk;
@@ -81,9 +116,9 @@ __global__ void __launch_bounds__(kThreads) pref_sum_kernel(PrefArgs a, int chun
       }
     }
   }
-  sum = block_sum(sum, sh);
-  const double n_lab = block_sum((double)cnt, sh);
-  if (threadIdx.x == 0) records[blockIdx.x] = make_double2(sum, n_lab);
+  double v[2] = {sum, (double)cnt};
+  block_sums(v, sh);
+  if (threadIdx.x == 0) records[blockIdx.x] = make_double2(v[0], v[1]);
 }
 
 // Per pair p: h = score(chosen) - score(rejected), the loss and dL/dh; then the
@@ -93,14 +128,9 @@ __global__ void __launch_bounds__(kThreads) pref_sum_kernel(PrefArgs a, int chun
 // pair, so the wider arithmetic hides behind the launch.
 __device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
 
-__global__ void __launch_bounds__(kThreads) pref_join_kernel(PrefArgs a, int chunks,
-                                                             const double2* __restrict__ records,
-                                                             float* __restrict__ loss,
-                                                             float* __restrict__ rewards,
-                                                             float* __restrict__ coef) {
+__device__ __forceinline__ void pref_join(const PrefArgs& a, int chunks, const double2* records,
+                                          float* loss, float* rewards, float* coef) {
   __shared__ double sh[kThreads / 32];
-  pdl_wait();
-  pdl_trigger();
   double total = 0.0;
   for (int64_t p = threadIdx.x; p < a.pairs; p += kThreads) {
     double d[2], per[2];
@@ -109,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) pref_join_kernel(PrefArgs a, int chu
       const int64_t n = p + w * a.pairs;
       double sum = 0.0, cnt = 0.0;
       for (int c = 0; c < chunks; ++c) {
-        const double2 r = records[n * chunks + c];
+        const double2 r = __ldcg(records + n * chunks + c);  // another block's writes
         sum += r.x;
         cnt += r.y;
       }
@@ -141,8 +171,30 @@ __global__ void __launch_bounds__(kThreads) pref_join_kernel(PrefArgs a, int chu
     coef[p] = (float)(ipo ? g * per[0] : g);
     coef[p + a.pairs] = (float)(ipo ? -g * per[1] : -g);
   }
-  total = block_sum(total, sh);
-  if (threadIdx.x == 0) loss[0] = (float)(total / (double)a.pairs);
+  double v[1] = {total};
+  block_sums(v, sh);
+  if (threadIdx.x == 0) loss[0] = (float)(v[0] / (double)a.pairs);
+}
+
+__global__ void __launch_bounds__(kThreads) pref_sum_kernel(PrefArgs a, int chunks, double2* records) {
+  pdl_wait();
+  pdl_trigger();
+  pref_sum(a, chunks, records);
+}
+__global__ void __launch_bounds__(kThreads) pref_join_kernel(PrefArgs a, int chunks,
+                                                             const double2* records, float* loss,
+                                                             float* rewards, float* coef) {
+  pdl_wait();
+  pdl_trigger();
+  pref_join(a, chunks, records, loss, rewards, coef);
+}
+__global__ void __launch_bounds__(kThreads) pref_cluster_kernel(PrefArgs a, int chunks, double2* records,
+                                                                float* loss, float* rewards, float* coef) {
+  pdl_wait();
+  pdl_trigger();
+  pref_sum(a, chunks, records);
+  cluster_sync();
+  if (blockIdx.x == 0) pref_join(a, chunks, records, loss, rewards, coef);
 }
 
 // dlogps[n, s] = labelled ? grad_loss * factor[n] * (per_token ? tok[n, s] : 1) : 0
@@ -202,22 +254,15 @@ struct PolicyArgs {
   int reduction;
 };
 
-struct PolicyRecord {
-  double loss, kl;
-  double clipped, count;
-};
-
+// Records of two double2 per (sequence, chunk): loss and KL sums, clipped and labelled tokens.
 // Per token: r = exp(x - old), L = -min(r A, clip(r) A) + c (e^d - d - 1) with
 // d = ref - x, and dL/dx = -A r (0 where the clipped branch is the smaller one)
 // + c (1 - e^d), stored for the backward. Which side of a clip border a ratio
 // lies on is decided on x - old in 64 bits (exact there) against the border's
 // logarithm, so the gradient's jump does not depend on exp's rounding.
-__global__ void __launch_bounds__(kThreads) policy_sum_kernel(PolicyArgs a, int chunks,
-                                                              PolicyRecord* __restrict__ records,
-                                                              float* __restrict__ tok_grad) {
-  __shared__ double sh[kThreads / 32];
-  pdl_wait();
-  pdl_trigger();
+__device__ __forceinline__ void policy_sum(const PolicyArgs& a, int chunks, double2* records,
+                                           float* __restrict__ tok_grad) {
+  __shared__ double sh[4 * kThreads / 32];
   const int64_t n = blockIdx.x / chunks;
   const int64_t s0 = (int64_t)(blockIdx.x % chunks) * kChunk;
   const int64_t s1 = s0 + kChunk < a.seq ? s0 + kChunk : a.seq;
@@ -269,34 +314,32 @@ __global__ void __launch_bounds__(kThreads) policy_sum_kernel(PolicyArgs a, int 
       if (tok_grad) tok_grad[n * a.seq + j] = g;
     }
   }
-  loss = block_sum(loss, sh);
-  kl = block_sum(kl, sh);
-  const double nc = block_sum((double)clipped, sh);
-  const double nl = block_sum((double)cnt, sh);
-  if (threadIdx.x == 0) records[blockIdx.x] = PolicyRecord{loss, kl, nc, nl};
+  double v[4] = {loss, kl, (double)clipped, (double)cnt};
+  block_sums(v, sh);
+  if (threadIdx.x == 0) {
+    records[2 * blockIdx.x] = make_double2(v[0], v[1]);
+    records[2 * blockIdx.x + 1] = make_double2(v[2], v[3]);
+  }
 }
 
 // out[0] = loss, out[1] = mean KL, out[2] = clipped share; factor[n] = weight of
 // a labelled token of sequence n in the loss.
-__global__ void __launch_bounds__(1024) policy_join_kernel(PolicyArgs a, int chunks,
-                                                           const PolicyRecord* __restrict__ records,
-                                                           float* __restrict__ out_loss,
-                                                           float* __restrict__ out_kl,
-                                                           float* __restrict__ out_clipped,
-                                                           float* __restrict__ factor) {
-  __shared__ double sh[32];
-  pdl_wait();
-  pdl_trigger();
+template <int kWarps>
+__device__ __forceinline__ void policy_join(const PolicyArgs& a, int chunks, const double2* records,
+                                            float* out_loss, float* out_kl, float* out_clipped,
+                                            float* factor) {
+  __shared__ double sh[4 * kWarps];
   double loss = 0.0, kl = 0.0, clipped = 0.0, count = 0.0;
   const bool by_seq = a.reduction == SOUP_POLICY_SEQUENCE;
   for (int64_t n = threadIdx.x; n < a.batch; n += blockDim.x) {
     double l = 0.0, c = 0.0;
     for (int i = 0; i < chunks; ++i) {
-      const PolicyRecord r = records[n * chunks + i];
-      l += r.loss;
-      c += r.count;
-      kl += r.kl;
-      clipped += r.clipped;
+      const double2 x = __ldcg(records + 2 * (n * chunks + i));  // another block's writes
+      const double2 y = __ldcg(records + 2 * (n * chunks + i) + 1);
+      l += x.x;
+      kl += x.y;
+      clipped += y.x;
+      c += y.y;
     }
     count += c;
     if (by_seq) {
@@ -307,18 +350,41 @@ __global__ void __launch_bounds__(1024) policy_join_kernel(PolicyArgs a, int chu
       loss += l;
     }
   }
-  loss = block_sum(loss, sh);
-  kl = block_sum(kl, sh);
-  clipped = block_sum(clipped, sh);
-  count = block_sum(count, sh);
-  const double inv = 1.0 / (count > 1.0 ? count : 1.0);
+  double v[4] = {loss, kl, clipped, count};
+  block_sums(v, sh);
+  const double inv = 1.0 / (v[3] > 1.0 ? v[3] : 1.0);
   if (!by_seq)
     for (int64_t n = threadIdx.x; n < a.batch; n += blockDim.x) factor[n] = (float)inv;
   if (threadIdx.x == 0) {
-    out_loss[0] = (float)(by_seq ? loss : loss * inv);
-    out_kl[0] = (float)(kl * inv);
-    out_clipped[0] = (float)(clipped * inv);
+    out_loss[0] = (float)(by_seq ? v[0] : v[0] * inv);
+    out_kl[0] = (float)(v[1] * inv);
+    out_clipped[0] = (float)(v[2] * inv);
   }
+}
+
+__global__ void __launch_bounds__(kThreads) policy_sum_kernel(PolicyArgs a, int chunks, double2* records,
+                                                              float* tok_grad) {
+  pdl_wait();
+  pdl_trigger();
+  policy_sum(a, chunks, records, tok_grad);
+}
+__global__ void __launch_bounds__(1024) policy_join_kernel(PolicyArgs a, int chunks,
+                                                           const double2* records, float* loss,
+                                                           float* kl, float* clipped, float* factor) {
+  pdl_wait();
+  pdl_trigger();
+  policy_join<32>(a, chunks, records, loss, kl, clipped, factor);
+}
+__global__ void __launch_bounds__(kThreads) policy_cluster_kernel(PolicyArgs a, int chunks,
+                                                                  double2* records, float* tok_grad,
+                                                                  float* loss, float* kl,
+                                                                  float* clipped, float* factor) {
+  pdl_wait();
+  pdl_trigger();
+  policy_sum(a, chunks, records, tok_grad);
+  cluster_sync();
+  if (blockIdx.x == 0)
+    policy_join<kThreads / 32>(a, chunks, records, loss, kl, clipped, factor);
 }
 
 int64_t chunks_of(int64_t seq) { return (seq + kChunk - 1) / kChunk; }
@@ -367,6 +433,9 @@ int soup_preference_loss_fwd(const float* logps, int64_t lp_ld, const float* ref
              label_smoothing, loss_type};
   double2* rec = static_cast<double2*>(workspace);
   cudaStream_t st = as_stream(stream);
+  if (2 * pairs * chunks <= kClusterBlocks)
+    return cuda_status(launch_cluster(pref_cluster_kernel, (unsigned)(2 * pairs * chunks), st, a, chunks,
+                                      rec, loss, rewards, coef));
   int rc = cuda_status(launch_pdl(pref_sum_kernel, dim3((unsigned)(2 * pairs * chunks)),
                                   dim3(kThreads), 0, st, a, chunks, rec));
   if (rc) return rc;
@@ -390,7 +459,7 @@ int soup_preference_loss_bwd(const float* grad_loss, const float* coef, const in
 
 size_t soup_policy_loss_workspace_bytes(int64_t batch, int64_t seq) {
   if (!sizes_ok(batch, seq)) return 0;
-  return (size_t)(batch * chunks_of(seq)) * sizeof(PolicyRecord);
+  return (size_t)(batch * chunks_of(seq)) * 2 * sizeof(double2);
 }
 
 int soup_policy_loss_fwd(const float* logps, int64_t lp_ld, const float* old_logps, int64_t old_ld,
@@ -421,13 +490,16 @@ int soup_policy_loss_fwd(const float* logps, int64_t lp_ld, const float* old_log
   PolicyArgs a{logps, lp_ld, old_logps, old_ld, ref_logps, ref_ld, advantages, adv_ld, labels,
                lab_ld, batch, seq, ignore_index, log(1.0 - clip_low), log(1.0 + clip_high),
                (float)(1.0 - clip_low), (float)(1.0 + clip_high), kl_coef, reduction};
-  PolicyRecord* rec = static_cast<PolicyRecord*>(workspace);
+  double2* rec = static_cast<double2*>(workspace);
   cudaStream_t st = as_stream(stream);
+  if (batch * chunks <= kClusterBlocks)
+    return cuda_status(launch_cluster(policy_cluster_kernel, (unsigned)(batch * chunks), st, a, chunks,
+                                      rec, tok_grad, loss, kl, clipped, factor));
   int rc = cuda_status(launch_pdl(policy_sum_kernel, dim3((unsigned)(batch * chunks)),
                                   dim3(kThreads), 0, st, a, chunks, rec, tok_grad));
   if (rc) return rc;
   return cuda_status(launch_pdl(policy_join_kernel, dim3(1), dim3(1024), 0, st, a, chunks,
-                                (const PolicyRecord*)rec, loss, kl, clipped, factor));
+                                (const double2*)rec, loss, kl, clipped, factor));
 }
 
 int soup_policy_loss_bwd(const float* grad_loss, const float* factor, const float* tok_grad,

@@ -22,10 +22,10 @@ the QLoRA step:
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -132,6 +132,11 @@ def _kernel_layout(t: torch.Tensor):
     return t, (_lib.c_i64 * 3)(sb, sh, ss)
 
 
+@functools.lru_cache(maxsize=256)
+def _window_workspace_bytes(*sizes: int) -> int:
+    return _lib.lib().soup_attention_window_bwd_workspace_bytes(*sizes)
+
+
 class WindowAttentionFunction(torch.autograd.Function):
     """out [B, S, H, D] of :func:`window_attention`; backward recomputes P from the
     saved log-sum-exp."""
@@ -151,7 +156,7 @@ class WindowAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         qs, ks, vs, scale, window, sinks = ctx.args
@@ -164,7 +169,7 @@ class WindowAttentionFunction(torch.autograd.Function):
         dq = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device)
         dk = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
         dv = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
-        nbytes = _lib.lib().soup_attention_window_bwd_workspace_bytes(B, H, Hk, S, window, sinks)
+        nbytes = _window_workspace_bytes(B, H, Hk, S, window, sinks)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
         _lib.call("soup_attention_window_bwd", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
                   vs, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), B, H, Hk, S, D, scale, window,

@@ -13,7 +13,6 @@ from __future__ import annotations
 
 import torch
 import torch.utils.checkpoint
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from ._shim import LaunchShim
@@ -84,7 +83,7 @@ Q8_BLOCK = 64  # consecutive columns that share one fp32 scale
 
 
 def _rows_8bit(t: torch.Tensor, n: int) -> torch.Tensor:
-    t2 = _rows(t, n)
+    t2 = t if t.dim() == 2 and t.stride(1) == 1 else _rows(t, n)
     return t2 if t2.shape[0] < 2 or t2.stride(0) >= n else t2.contiguous()
 
 
@@ -126,7 +125,7 @@ class SwiGLU8BitFunction(torch.autograd.Function):
         rows = g2.shape[0]
         blocks = -(-n // Q8_BLOCK)
         dt = _lib.dtype_code(gate.dtype)
-        out = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+        out = torch.empty(*gate.shape, dtype=gate.dtype, device=gate.device)
         # one buffer: the scales of gate, of up, the codes of gate (16-byte aligned), of up
         c0 = -(-8 * rows * blocks // 16) * 16
         c1 = c0 + -(-rows * n // 16) * 16
@@ -140,13 +139,13 @@ class SwiGLU8BitFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dy: torch.Tensor):
         (kept,) = ctx.saved_tensors
         rows, n, blocks, c0, c1, dt, dtype = ctx.args
         dy2 = _rows_8bit(dy if dy.dtype is dtype else dy.to(dtype), n)
-        dg = torch.empty(dy.shape, dtype=dtype, device=dy.device)
-        du = torch.empty(dy.shape, dtype=dtype, device=dy.device)
+        dg = torch.empty(*dy.shape, dtype=dtype, device=dy.device)
+        du = torch.empty(*dy.shape, dtype=dtype, device=dy.device)
         base = kept.data_ptr()
         _lib.call("soup_swiglu_q8_bwd", dy.device, dy2.data_ptr(), _ld(dy2), base + c0, base + c1, n, base,
                   base + 4 * rows * blocks, blocks, dg.data_ptr(), n, du.data_ptr(), n, None, 0, rows, n,

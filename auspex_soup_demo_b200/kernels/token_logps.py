@@ -20,7 +20,6 @@ from __future__ import annotations
 from typing import Any, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import chunked_ce
@@ -102,7 +101,7 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
         return logps, ents
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, dlogps, _dents):
         if dlogps is None:
             return None, None, None, None, None

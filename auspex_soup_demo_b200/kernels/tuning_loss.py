@@ -21,7 +21,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .chunked_ce import IGNORE_INDEX
@@ -106,7 +105,7 @@ class PreferenceLossFunction(torch.autograd.Function):
         return loss, chosen, rejected
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, grad, _c, _r):
         if grad is None:
             return (None,) * 7
@@ -186,7 +185,7 @@ class PolicyLossFunction(torch.autograd.Function):
         return loss, kl, clipped
 
     @staticmethod
-    @once_differentiable
+    @_lib.once_differentiable
     def backward(ctx, grad, _k, _c):
         if grad is None:
             return (None,) * 11

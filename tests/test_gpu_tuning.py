@@ -185,7 +185,7 @@ def test_head_token_logps_directional_difference():
 
 
 # ----------------------------------------------------------------- preference -----
-@pytest.mark.parametrize("pairs,s", [(1, 1), (1, 7), (2, 512), (3, 4096), (5, 4097), (300, 33), (2, 20001)])
+@pytest.mark.parametrize("pairs,s", [(1, 1), (1, 7), (2, 512), (3, 4096), (5, 4097), (300, 33), (2, 20001), (1, 8192), (1, 2049)])
 @pytest.mark.parametrize("kind,eps", [("sigmoid", 0.0), ("sigmoid", 0.1), ("hinge", 0.0), ("ipo", 0.0)])
 def test_preference_loss(pairs, s, kind, eps):
     g = _gen(pairs * 31 + s)
@@ -241,7 +241,7 @@ def test_preference_loss_extreme_margins():
 
 
 # --------------------------------------------------------------------- policy -----
-@pytest.mark.parametrize("b,s", [(1, 1), (3, 7), (8, 512), (2, 4097), (1500, 33)])
+@pytest.mark.parametrize("b,s", [(1, 1), (3, 7), (8, 512), (2, 4097), (1500, 33), (2, 8192), (4, 2049)])
 @pytest.mark.parametrize("reduction", ["token", "sequence"])
 @pytest.mark.parametrize("case", ["full", "no_old", "no_ref", "plain"])
 def test_policy_loss(b, s, reduction, case):
