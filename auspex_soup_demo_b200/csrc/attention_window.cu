@@ -105,35 +105,25 @@ struct Desc {
       : lo(static_cast<uint32_t>(d)), hi(static_cast<uint32_t>(d >> 32)) {}
   __device__ __forceinline__ uint32_t at(uint32_t bytes) const { return lo + (bytes >> 4); }
 };
-__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t a_hi,
-                                       uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "setp.ne.b32 q, %7, 0;\n\t"
-      "mov.b64 da, {%1, %2};\n\t"
-      "mov.b64 db, {%3, %4};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo,
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo,
                                        uint32_t b_hi, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "setp.ne.b32 q, %6, 0;\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc), "r"(leader)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "mov.b64 da, {%1, %2};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t leader, uint32_t bar) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred q;\n\t"
-      "setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
-      "r"(leader)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
       : "memory");
 }
 // Offsets in bytes of k-step kk (16 wide): of a K-major 128-column tile whose two
@@ -329,7 +319,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     // into the buffer that this product has read P from (MMAs run in issue order),
     // and the same for B. An entry's K and V are released by its last reader: B,
     // which comes second, unless B runs ahead of A (a gap) or does not use it.
-    const uint32_t leader = elect_one();
     auto wait = [&](uint32_t bar, int parity) {
       return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
     };
@@ -349,13 +338,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (!wait(full(st), (2 * j / kRing) & 1)) return false;
       tc_fence_after();
       const uint32_t d = tmem + x * 128 + (i & 1) * 64;
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kHeadDim / 16; ++kk)
-        mma_ss(leader, d, q_desc.at(x * kTileBytes + kmajor_step(kk, kBox)), q_desc.hi,
-               k_desc.at(st * kStepTile + kmajor_step(kk, kStepBox)), k_desc.hi, kIdescKK64,
-               kk > 0 ? 1u : 0u);
-      commit(leader, s_full(x, i));
-      if (last_reader(j) == x) commit(leader, empty(st));
+        for (int kk = 0; kk < kHeadDim / 16; ++kk)
+          mma_ss(d, q_desc.at(x * kTileBytes + kmajor_step(kk, kBox)), q_desc.hi,
+                 k_desc.at(st * kStepTile + kmajor_step(kk, kStepBox)), k_desc.hi, kIdescKK64,
+                 kk > 0 ? 1u : 0u);
+        tc_commit(s_full(x, i));
+        if (last_reader(j) == x) tc_commit(empty(st));
+      }
+      __syncwarp();
       issued = true;
       return true;
     };
@@ -366,12 +358,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (!wait(p_full(x, i), (i >> 1) & 1)) return false;
       tc_fence_after();
       const uint32_t p = tmem + x * 128 + (i & 1) * 64;
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kBlk / 16; ++kk)
-        mma_ts(leader, tmem + 256 + x * 128, p + kk * 8, v_desc.at(st * kStepTile + mnmajor_step(kk)),
-               v_desc.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
-      commit(leader, pv_done(x, i));
-      if (last_reader(j) == x) commit(leader, empty(st));
+        for (int kk = 0; kk < kBlk / 16; ++kk)
+          mma_ts(tmem + 256 + x * 128, p + kk * 8, v_desc.at(st * kStepTile + mnmajor_step(kk)),
+                 v_desc.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
+        tc_commit(pv_done(x, i));
+        if (last_reader(j) == x) tc_commit(empty(st));
+      }
+      __syncwarp();
       return true;
     };
     for (int i = 0; i < 2 && ok; ++i) {
@@ -388,7 +383,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     for (int i = 2 * n > kRing ? 2 * n - kRing : 0; i < 2 * n && ok; ++i)
       ok = wait(empty(i % kRing), (i / kRing) & 1);
     if (!ok && issued) {
-      commit(leader, drain_bar);
+      if (elect_one()) tc_commit(drain_bar);
+      __syncwarp();
       uint64_t t0 = tc::globaltimer();
       while (!mbar_try_wait(drain_bar, 0) && tc::globaltimer() - t0 < wait_ns) {
       }
@@ -724,7 +720,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // --------------------------------------------------- MMA issuer ----
-    const uint32_t leader = elect_one();
     auto wait = [&](uint32_t bar, int parity) {
       return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
     };
@@ -740,11 +735,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!wait(full(st), (i / kDkvStages) & 1)) return false;
       tc_fence_after();
       const uint32_t b_off = st * 2 * kTileBytes + dP * kTileBytes;
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kHeadDim / 16; ++kk)
-        mma_ss(leader, tmem + dP * 128, (dP ? v_desc : k_desc).at(kmajor_step(kk, kBox)), k_desc.hi,
-               qd_desc.at(b_off + kmajor_step(kk, kBox)), qd_desc.hi, kIdescKK, kk > 0 ? 1u : 0u);
-      commit(leader, dP ? dp_full : s_full);
+        for (int kk = 0; kk < kHeadDim / 16; ++kk)
+          mma_ss(tmem + dP * 128, (dP ? v_desc : k_desc).at(kmajor_step(kk, kBox)), k_desc.hi,
+                 qd_desc.at(b_off + kmajor_step(kk, kBox)), qd_desc.hi, kIdescKK, kk > 0 ? 1u : 0u);
+        tc_commit(dP ? dp_full : s_full);
+      }
+      __syncwarp();
       issued = true;
       return true;
     };
@@ -754,10 +752,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!wait(dK ? ds_full : p_full, i & 1)) return false;
       tc_fence_after();
       const uint32_t b_off = st * 2 * kTileBytes + (dK ? 0 : kTileBytes);
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk)
-        mma_ts(leader, tmem + 256 + dK * 128, tmem + dK * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
-               qd_mn.at(b_off + mnmajor_step(kk)), qd_mn.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
+        for (int kk = 0; kk < kTile / 16; ++kk)
+          mma_ts(tmem + 256 + dK * 128, tmem + dK * 128 + (kk >> 1) * 32 + (kk & 1) * 8,
+                 qd_mn.at(b_off + mnmajor_step(kk)), qd_mn.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
+      }
+      __syncwarp();
       return true;
     };
     if (ok) ok = issue_s(0, 0);
@@ -766,14 +767,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = issue_acc(0, i);
       if (ok && i + 1 < total) ok = issue_s(0, i + 1);
       if (ok) ok = issue_acc(1, i);
-      if (ok) commit(leader, empty(i % kDkvStages));
+      if (ok && elect_one()) tc_commit(empty(i % kDkvStages));
+      __syncwarp();
       if (ok && i + 1 < total) ok = issue_s(1, i + 1);
     }
-    if (ok) commit(leader, acc_done);
+    if (ok && elect_one()) tc_commit(acc_done);
+    __syncwarp();
     for (int i = total > kDkvStages ? total - kDkvStages : 0; i < total && ok; ++i)
       ok = wait(empty(i % kDkvStages), (i / kDkvStages) & 1);
     if (!ok && issued) {
-      commit(leader, drain_bar);
+      if (elect_one()) tc_commit(drain_bar);
+      __syncwarp();
       uint64_t t0 = tc::globaltimer();
       while (!mbar_try_wait(drain_bar, 0) && tc::globaltimer() - t0 < wait_ns) {
       }
@@ -1096,7 +1100,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // --------------------------------------------------- MMA issuer ----
-    const uint32_t leader = elect_one();
     auto wait = [&](uint32_t bar, int parity) {
       return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
     };
@@ -1112,23 +1115,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!wait(k_full(sk), (j / kDqKStages) & 1)) return false;
       if (j > 0 && !wait(s_empty, (j - 1) & 1)) return false;
       tc_fence_after();
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // S = Q K^T
-        mma_ss(leader, tmem, q_desc.at(kmajor_step(kk, kBox)), q_desc.hi,
-               k_desc.at(sk * kTileBytes + kmajor_step(kk, kBox)), k_desc.hi, kIdescKK,
-               kk > 0 ? 1u : 0u);
-      commit(leader, s_full);
+        for (int kk = 0; kk < kHeadDim / 16; ++kk)  // S = Q K^T
+          mma_ss(tmem, q_desc.at(kmajor_step(kk, kBox)), q_desc.hi,
+                 k_desc.at(sk * kTileBytes + kmajor_step(kk, kBox)), k_desc.hi, kIdescKK,
+                 kk > 0 ? 1u : 0u);
+        tc_commit(s_full);
+      }
+      __syncwarp();
       issued = true;
       if (!wait(v_full(sv), (j / kDqVStages) & 1)) return false;
       if (j > 0 && !wait(dp_empty, (j - 1) & 1)) return false;
       tc_fence_after();
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kHeadDim / 16; ++kk)  // dP = dO V^T
-        mma_ss(leader, tmem + 128, do_desc.at(kmajor_step(kk, kBox)), do_desc.hi,
-               v_desc.at(sv * kTileBytes + kmajor_step(kk, kBox)), v_desc.hi, kIdescKK,
-               kk > 0 ? 1u : 0u);
-      commit(leader, dp_full);
-      commit(leader, v_empty(sv));
+        for (int kk = 0; kk < kHeadDim / 16; ++kk)  // dP = dO V^T
+          mma_ss(tmem + 128, do_desc.at(kmajor_step(kk, kBox)), do_desc.hi,
+                 v_desc.at(sv * kTileBytes + kmajor_step(kk, kBox)), v_desc.hi, kIdescKK,
+                 kk > 0 ? 1u : 0u);
+        tc_commit(dp_full);
+        tc_commit(v_empty(sv));
+      }
+      __syncwarp();
       return true;
     };
     if (ok) ok = issue_sd(0);
@@ -1137,21 +1146,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (j + 1 < n && !(ok = issue_sd(j + 1))) break;
       if (!(ok = wait(ds_full(j), (j >> 1) & 1))) break;
       tc_fence_after();
+      if (elect_one()) {
 #pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk)  // dQ += dS K (dS from TMEM: 8 columns per 16 keys)
-        mma_ts(leader, tmem + 256, tmem + 384 + (j & 1) * 64 + kk * 8,
-               k_mn.at(sk * kTileBytes + mnmajor_step(kk)), k_mn.hi, kIdescKM, (j > 0 || kk > 0) ? 1u : 0u);
-      commit(leader, ds_free(j));
-      commit(leader, k_empty(sk));
+        for (int kk = 0; kk < kTile / 16; ++kk)  // dQ += dS K (dS from TMEM: 8 columns per 16 keys)
+          mma_ts(tmem + 256, tmem + 384 + (j & 1) * 64 + kk * 8,
+                 k_mn.at(sk * kTileBytes + mnmajor_step(kk)), k_mn.hi, kIdescKM, (j > 0 || kk > 0) ? 1u : 0u);
+        tc_commit(ds_free(j));
+        tc_commit(k_empty(sk));
+      }
+      __syncwarp();
     }
-    if (ok) commit(leader, acc_done);
+    if (ok && elect_one()) tc_commit(acc_done);
+    __syncwarp();
     for (int j = n > kDqKStages ? n - kDqKStages : 0; j < n && ok; ++j) {
       ok = wait(k_empty(j % kDqKStages), (j / kDqKStages) & 1);
       if (ok && j >= n - kDqVStages) ok = wait(v_empty(j % kDqVStages), (j / kDqVStages) & 1);
       if (ok && j >= n - 2) ok = wait(ds_free(j), (j >> 1) & 1);
     }
     if (!ok && issued) {
-      commit(leader, drain_bar);
+      if (elect_one()) tc_commit(drain_bar);
+      __syncwarp();
       uint64_t t0 = tc::globaltimer();
       while (!mbar_try_wait(drain_bar, 0) && tc::globaltimer() - t0 < wait_ns) {
       }
