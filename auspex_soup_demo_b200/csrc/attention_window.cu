@@ -6,8 +6,8 @@
 //
 // Key tiles without a visible pair are never loaded, so the products cover about
 // window + sinks keys a query.
-// Forward: one CTA per (batch, query head, pair of 128-query tiles), keys in blocks of 64,
-// one thread per query row.
+// Forward: one CTA per (batch, query head, 128-query tile), keys in blocks of 64, one
+// thread per query row.
 // Backward: dK / dV per (batch, KV head, key tile): the CTA runs through the query
 // heads of its group and their queries in 128-query steps and keeps dK, dV in TMEM, so
 // no per-head partials reach memory; the far queries of the sink tiles, which every
@@ -30,10 +30,10 @@ namespace {
 constexpr int kWarps = 16;  // compute warps
 constexpr int kThreads = 64 + 32 * kWarps;
 
-constexpr int kErrWinProducer = 0x121;
-constexpr int kErrWinMma = 0x122;
-constexpr int kErrWinSoftmax = 0x123;
-constexpr int kErrWinSmem = 0x124;
+constexpr int kErrWinProducer = 0x131;
+constexpr int kErrWinMma = 0x132;
+constexpr int kErrWinSoftmax = 0x133;
+constexpr int kErrWinSmem = 0x134;
 
 // The key tiles that the queries from q0 on need, in the order the kernels take
 // them: the sink tiles before the window's first tile, then the window's tiles.
@@ -77,10 +77,13 @@ __device__ __forceinline__ int mask_kind(uint32_t m, uint32_t all) {
 }
 
 // ---- the MMA warp ----
-// The whole warp walks the schedule converged and one elected lane issues, so that
-// descriptors and addresses live in uniform registers. Issued from a lane == 0 branch
-// each product took about 110 cycles, more than a 128 x 64 x 16 product does (75), and the issuing thread bounded all three kernels: 3400 cycles per forward
-// step of two 64-key blocks of which the softmax needed 1900.
+// The whole warp walks the schedule converged, so that waits are one instruction and
+// descriptors and addresses are uniform; each group of products and its commits runs in the
+// branch of an elected thread. From a lane == 0 branch around the whole schedule each product
+// took about 110 cycles, more than a 128 x 64 x 16 product does (75), and the issuing thread
+// bounded all three kernels. Do not issue them from the converged warp under a predicate
+// that only one thread has set instead of a branch: that is 2 % faster, but commits then
+// go astray now and then (a wait that expires, or an illegal address).
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t v;
   asm volatile(
@@ -175,34 +178,34 @@ struct FwdArgs {
 };
 
 // ------------------------------------------------------------- forward ----
-// One CTA per (batch, query head, pair of 128-query tiles A, B), keys in blocks of 64.
-// TMEM: two S buffers of 64 columns per query tile (A at 0 and 64, B at 128 and 192),
-// O_A at 256, O_B at 384; P of a block overwrites the first 32 columns of its own S
-// buffer as bf16 pairs and is the A operand of O += P V read from TMEM. With S
-// double buffered the products run a block ahead: the softmax finds its next S ready
-// and its chain holds no product. Shared memory: Q_A, Q_B (32 KB each), one ring of
-// 10 x 16 KB through which K and V blocks pass (K0 V0 K1 V1 ...), barriers.
-// At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 158 us, 612 TFLOP/s of the
-// visible pairs' products; bound by the softmax warps (TMEM reads and exponentials of a
-// block). Measured slower there: 16 softmax warps, two per row (166 us), and 128-key
-// blocks with P over S.
-constexpr int kFwdWarps = 8;  // softmax warps: four per query tile, one row per thread
+// One CTA per (batch, query head, 128-query tile), keys in blocks of 64, two CTAs an SM.
+// TMEM (256 columns): two S buffers of 64 columns, O at 128; P of a block overwrites the
+// first 32 columns of its own S buffer as bf16 pairs and is the A operand of O += P V
+// read from TMEM. With S double buffered the products run a block ahead: the softmax
+// finds its next S ready and its chain holds no product; the other CTA's products fill the
+// time in which this one starts and ends. Shared memory: Q (32 KB), one
+// ring of 5 x 16 KB through which K and V blocks pass (K0 V0 K1 V1 ...), barriers.
+// At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 134 us, 722 TFLOP/s of the
+// visible pairs' products; 168 us with one CTA an SM for a pair of query tiles that shares
+// the K and V blocks. Bound by the products (N = 64 ones take as long as N = 128 ones) and
+// the softmax warps' TMEM reads beside them.
+constexpr int kFwdWarps = 4;  // softmax warps, one row per thread
 constexpr int kFwdThreads = 64 + 32 * kFwdWarps;
 constexpr int kBlk = 64;      // keys per block
-constexpr int kRing = 10;
+constexpr int kRing = 5;
 struct WinFwdSmem {
   static constexpr int kQ = 0;
-  static constexpr int kKV = kQ + 2 * kTileBytes;
+  static constexpr int kKV = kQ + kTileBytes;
   static constexpr int kBar = kKV + kRing * kStepTile;
-  // q_full, full[10], empty[10], then per query tile and S buffer: s_full, p_full, pv_done
-  static constexpr int kNumBars = 1 + 2 * kRing + 12 + 1;
+  // q_full, full[5], empty[5], then per S buffer: s_full, p_full, pv_done; drain
+  static constexpr int kNumBars = 1 + 2 * kRing + 6 + 1;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kUsed = kMisc + 16;
-  static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
+  static constexpr int kBytes = 115712;  // half of an SM's 228 KB less 1 KB a CTA
 };
-static_assert(WinFwdSmem::kUsed + 128 <= 232448, "window attention forward shared memory");
+static_assert(WinFwdSmem::kUsed + 512 <= WinFwdSmem::kBytes, "window attention forward shared memory");
 
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(kFwdThreads, 2)
     win_fwd_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                    const __grid_constant__ CUtensorMap tma_v, FwdArgs a, int* err) {
   using L = WinFwdSmem;
@@ -219,47 +222,36 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   auto full = [&](int s) { return bar0 + 8u * (1 + s); };
   auto empty = [&](int s) { return bar0 + 8u * (1 + kRing + s); };
   constexpr int kB = 1 + 2 * kRing;
-  // of block i of query tile x: its S buffer is i & 1, the phase (i >> 1) & 1
-  auto s_full = [&](int x, int i) { return bar0 + 8u * (kB + 2 * x + (i & 1)); };
-  auto p_full = [&](int x, int i) { return bar0 + 8u * (kB + 4 + 2 * x + (i & 1)); };
-  auto pv_done = [&](int x, int i) { return bar0 + 8u * (kB + 8 + 2 * x + (i & 1)); };
-  const uint32_t drain_bar = bar0 + 8u * (kB + 12);
+  // of block i: its S buffer is i & 1, the phase (i >> 1) & 1
+  auto s_full = [&](int i) { return bar0 + 8u * (kB + (i & 1)); };
+  auto p_full = [&](int i) { return bar0 + 8u * (kB + 2 + (i & 1)); };
+  auto pv_done = [&](int i) { return bar0 + 8u * (kB + 4 + (i & 1)); };
+  const uint32_t drain_bar = bar0 + 8u * (kB + 6);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nq = (a.S + kTile - 1) / kTile;
   const int nb = (a.S + kBlk - 1) / kBlk;
-  const int npair = (nq + 1) / 2;
   const int bh = blockIdx.x % (a.B * a.H);
-  const int pr = npair - 1 - blockIdx.x / (a.B * a.H);  // late pairs first: early ones are short
+  const int qt = nq - 1 - blockIdx.x / (a.B * a.H);  // late tiles first: early ones are short
   const int b = bh / a.H, h = bh % a.H;
   const int hk = h / (a.H / a.Hk);
-  // The pair's list of key blocks: the sinks' before the window, then from the first
-  // block that A's first row sees to B's diagonal (A's without a B). Query tile A
-  // takes entries 0 .. n_x[0] - 1; B, whose window may start `gap` blocks later,
-  // leaves those out: its i-th block is entry i, or i + gap past the sinks.
-  const int q_lo = 2 * pr * kTile - a.window + 1;
+  // The tile's list of key blocks: the sinks' before the window, then from the first
+  // block that its first row sees to the diagonal.
+  const int q_lo = qt * kTile - a.window + 1;
   const int lo = q_lo > 0 ? q_lo / kBlk : 0;
-  const int lo_b = q_lo + kTile > 0 ? (q_lo + kTile) / kBlk : 0;
   const int sink_blocks = (a.sinks + kBlk - 1) / kBlk;
   const int ns = sink_blocks < lo ? sink_blocks : lo;
-  const bool has_b = 2 * pr + 1 < nq;
-  const int end_a = (2 * pr + 1) * 2 < nb ? (2 * pr + 1) * 2 : nb;  // one past A's diagonal block
-  const int end_b = (2 * pr + 2) * 2 < nb ? (2 * pr + 2) * 2 : nb;
-  const int gap = sink_blocks <= lo ? lo_b - lo : 0;
-  const int n = ns + (has_b ? end_b : end_a) - lo;  // entries
-  const int n_a = ns + end_a - lo;
-  const int n_b = has_b ? n - gap : 0;
-  auto block_of = [&](int j) { return j < ns ? j : lo + (j - ns); };
-  auto entry_of = [&](int x, int i) { return x && i >= ns ? i + gap : i; };
+  const int end = 2 * qt + 2 < nb ? 2 * qt + 2 : nb;  // one past the diagonal block
+  const int n = ns + end - lo;
+  auto block_of = [&](int i) { return i < ns ? i : lo + (i - ns); };
   const uint64_t wait_ns = a.wait_ns;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kNumBars; ++i) {
-      const int e = i - (kB + 4);
-      // the four softmax warps of a query tile arrive once each on its p_full
-      mbar_init(bar0 + 8u * i, e >= 0 && e < 4 ? kFwdWarps / 2 : 1);
+      const uint32_t bar = bar0 + 8u * i;
+      mbar_init(bar, bar == p_full(0) || bar == p_full(1) ? kFwdWarps : 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -271,7 +263,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_holder)),
-                 "r"(512)
+                 "r"(256)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -283,15 +275,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       // ------------------------------------------------ TMA producer ----
-      const int nqt = has_b ? 2 : 1;
-      mbar_arrive_expect_tx(q_full, nqt * kTileBytes);
-      for (int x = 0; x < nqt; ++x) {
-        const uint32_t qd = sbase + L::kQ + x * kTileBytes;
-        tma_load_4d(qd, &tma_q, q_full, 0, (2 * pr + x) * kTile, h, b);
-        tma_load_4d(qd + kBox, &tma_q, q_full, 64, (2 * pr + x) * kTile, h, b);
-      }
+      mbar_arrive_expect_tx(q_full, kTileBytes);
+      tma_load_4d(sbase + L::kQ, &tma_q, q_full, 0, qt * kTile, h, b);
+      tma_load_4d(sbase + L::kQ + kBox, &tma_q, q_full, 64, qt * kTile, h, b);
       int issued = 0;
-      for (int i = 0; i < 2 * n; ++i) {  // K of entry j is load 2 j, V load 2 j + 1
+      for (int i = 0; i < 2 * n; ++i) {  // K of block j is load 2 j, V load 2 j + 1
         const int st = i % kRing;
         if (!bounded_wait(empty(st), ((i / kRing) & 1) ^ 1, abort_flag, err, kErrWinProducer, wait_ns))
           break;
@@ -315,69 +303,56 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     }
   } else if (warp == 1) {
     // --------------------------------------------------- MMA issuer ----
-    // S of blocks 0 and 1 of both query tiles, then per block i: P V of A, S_A(i + 2)
-    // into the buffer that this product has read P from (MMAs run in issue order),
-    // and the same for B. An entry's K and V are released by its last reader: B,
-    // which comes second, unless B runs ahead of A (a gap) or does not use it.
+    // S of blocks 0 and 1, then per block i: P V (i), S(i + 2) into the buffer that this
+    // product has read P from (MMAs run in issue order).
     auto wait = [&](uint32_t bar, int parity) {
       return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
     };
     bool ok = wait(q_full, 0);
     bool issued = false;
-    auto last_reader = [&](int j) {
-      if (!has_b || (j >= ns && j < ns + gap)) return 0;
-      if (j >= n_a) return 1;
-      return j >= ns && gap > 0 ? 0 : 1;
-    };
     const Desc q_desc(smem_desc_sw128(sbase + L::kQ, 16, 1024));
     const Desc k_desc(smem_desc_sw128(sbase + L::kKV, 16, 1024));
     const Desc v_desc(smem_desc_sw128(sbase + L::kKV, kStepBox, 1024));
-    auto issue_s = [&](int x, int i) -> bool {
-      const int j = entry_of(x, i);
-      const int st = (2 * j) % kRing;
-      if (!wait(full(st), (2 * j / kRing) & 1)) return false;
+    auto issue_s = [&](int i) -> bool {
+      const int st = (2 * i) % kRing;
+      if (!wait(full(st), (2 * i / kRing) & 1)) return false;
       tc_fence_after();
-      const uint32_t d = tmem + x * 128 + (i & 1) * 64;
+      const uint32_t d = tmem + (i & 1) * 64;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kHeadDim / 16; ++kk)
-          mma_ss(d, q_desc.at(x * kTileBytes + kmajor_step(kk, kBox)), q_desc.hi,
+          mma_ss(d, q_desc.at(kmajor_step(kk, kBox)), q_desc.hi,
                  k_desc.at(st * kStepTile + kmajor_step(kk, kStepBox)), k_desc.hi, kIdescKK64,
                  kk > 0 ? 1u : 0u);
-        tc_commit(s_full(x, i));
-        if (last_reader(j) == x) tc_commit(empty(st));
+        tc_commit(s_full(i));
+        tc_commit(empty(st));
       }
       __syncwarp();
       issued = true;
       return true;
     };
-    auto issue_pv = [&](int x, int i) -> bool {
-      const int j = entry_of(x, i);
-      const int st = (2 * j + 1) % kRing;
-      if (!wait(full(st), ((2 * j + 1) / kRing) & 1)) return false;
-      if (!wait(p_full(x, i), (i >> 1) & 1)) return false;
+    auto issue_pv = [&](int i) -> bool {
+      const int st = (2 * i + 1) % kRing;
+      if (!wait(full(st), ((2 * i + 1) / kRing) & 1)) return false;
+      if (!wait(p_full(i), (i >> 1) & 1)) return false;
       tc_fence_after();
-      const uint32_t p = tmem + x * 128 + (i & 1) * 64;
+      const uint32_t p = tmem + (i & 1) * 64;
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kBlk / 16; ++kk)
-          mma_ts(tmem + 256 + x * 128, p + kk * 8, v_desc.at(st * kStepTile + mnmajor_step(kk)),
-                 v_desc.hi, kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
-        tc_commit(pv_done(x, i));
-        if (last_reader(j) == x) tc_commit(empty(st));
+          mma_ts(tmem + 128, p + kk * 8, v_desc.at(st * kStepTile + mnmajor_step(kk)), v_desc.hi,
+                 kIdescKM, (i > 0 || kk > 0) ? 1u : 0u);
+        tc_commit(pv_done(i));
+        tc_commit(empty(st));
       }
       __syncwarp();
       return true;
     };
-    for (int i = 0; i < 2 && ok; ++i) {
-      if (i < n_a) ok = issue_s(0, i);
-      if (ok && i < n_b) ok = issue_s(1, i);
-    }
-    for (int i = 0; (i < n_a || i < n_b) && ok; ++i) {
-      if (i < n_a) ok = issue_pv(0, i);
-      if (ok && i + 2 < n_a) ok = issue_s(0, i + 2);
-      if (ok && i < n_b) ok = issue_pv(1, i);
-      if (ok && i + 2 < n_b) ok = issue_s(1, i + 2);
+    if (ok) ok = issue_s(0);
+    if (ok && n > 1) ok = issue_s(1);
+    for (int i = 0; i < n && ok; ++i) {
+      ok = issue_pv(i);
+      if (ok && i + 2 < n) ok = issue_s(i + 2);
     }
     // the ring's last arrivals (nothing else waits for them)
     for (int i = 2 * n > kRing ? 2 * n - kRing : 0; i < 2 * n && ok; ++i)
@@ -391,28 +366,25 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     }
   } else {
     // ------------------------------------------------------- softmax ----
-    const int x = (warp - 2) >> 2;             // query tile A (0) or B (1)
-    const int quarter = warp & 3;              // TMEM lanes this warp may access
-    const int qt = 2 * pr + x;
+    const int quarter = warp & 3;                    // TMEM lanes this warp may access
     const int q = qt * kTile + quarter * 32 + lane;  // query row of this thread
-    const int n_x = x ? n_b : n_a;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t s_base = tmem + x * 128 + lane_off;
-    const uint32_t o_t = tmem + 256 + x * 128 + lane_off;
+    const uint32_t s_base = tmem + lane_off;
+    const uint32_t o_t = tmem + 128 + lane_off;
     const uint64_t sl2 = f2_pack(a.scale_log2, a.scale_log2);
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int i = 0; i < n_x; ++i) {
+    for (int i = 0; i < n; ++i) {
       bool w = true;
       if (lane == 0)
-        w = bounded_wait(s_full(x, i), (i >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+        w = bounded_wait(s_full(i), (i >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
       if (!(ok = warp_ok(w))) break;
       tc_fence_after();
       const uint32_t s_t = s_base + (i & 1) * 64;
       float s0[32], s1[32];
       tmem_ld32_async(s_t, s0);
       tmem_ld32_async(s_t + 32, s1);
-      const int k0 = block_of(entry_of(x, i)) * kBlk;
+      const int k0 = block_of(i) * kBlk;
       const bool edge = k0 + kBlk > a.S || k0 + kBlk > qt * kTile + 1 ||
                         (qt * kTile + kTile - 1 - k0 >= a.window && k0 + kBlk > a.sinks);
       int kind0 = 1, kind1 = 1;
@@ -446,8 +418,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       if (i > 0 && __any_sync(0xffffffffu, rescale)) {
         // O is stable once P V (i - 1) is done (S(i) came before it; P V (i - 2) before S(i))
         if (lane == 0)
-          w = bounded_wait(pv_done(x, i - 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax,
-                           wait_ns);
+          w = bounded_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
         if (!(ok = warp_ok(w))) break;
         tc_fence_after();
         rescale_o_row(o_t, alpha);
@@ -484,16 +455,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(x, i));
+      if (lane == 0) mbar_arrive(p_full(i));
     }
-    if (ok && n_x > 0) {
+    if (ok) {
       bool w = true;
       if (lane == 0)
-        w = bounded_wait(pv_done(x, n_x - 1), ((n_x - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax,
-                         wait_ns);
+        w = bounded_wait(pv_done(n - 1), ((n - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
       ok = warp_ok(w);
     }
-    if (ok && n_x > 0) {
+    if (ok) {
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : 0.f;
       bf16* orow = a.out + ((int64_t)b * a.S + q) * (int64_t)(a.H * kHeadDim) + h * kHeadDim;
@@ -520,7 +490,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256)
                  : "memory");
   }
 }
@@ -1374,8 +1344,8 @@ int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const voi
   FwdArgs a{(int)batch, (int)heads, (int)kv_heads, (int)seq, scale * 1.4426950408889634f,
             (int)(window < seq ? window : seq), (int)(sinks < seq ? sinks : seq),
             static_cast<bf16*>(out), lse, wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
-  const int64_t npair = ((seq + kTile - 1) / kTile + 1) / 2;
-  win_fwd_kernel<<<(unsigned)(batch * heads * npair), kFwdThreads, WinFwdSmem::kBytes,
+  const int64_t nq = (seq + kTile - 1) / kTile;
+  win_fwd_kernel<<<(unsigned)(batch * heads * nq), kFwdThreads, WinFwdSmem::kBytes,
                    as_stream(stream)>>>(mq, mk, mv, a, err);
   return launch_status();
 }
