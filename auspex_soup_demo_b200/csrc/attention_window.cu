@@ -35,19 +35,26 @@ constexpr int kErrWinMma = 0x132;
 constexpr int kErrWinSoftmax = 0x133;
 constexpr int kErrWinSmem = 0x134;
 
-// The key tiles that the queries from q0 on need, in the order the kernels take
-// them: the sink tiles before the window's first tile, then the window's tiles.
-struct KeyTiles {
-  int n_sink, lo;  // leading sink tiles; first tile of the window
-  __device__ __forceinline__ int at(int j) const { return j < n_sink ? j : lo + (j - n_sink); }
+constexpr int kBlk = 64;  // keys per block of the forward and of dQ
+// The key blocks that query tile qt needs, in the order the kernels take them: the sinks'
+// before the window, then from the first block that the tile's first row sees to the diagonal.
+struct KeyBlocks {
+  int n_sink, lo, n;  // leading sink blocks; first block of the window; blocks
+  __device__ __forceinline__ int at(int i) const { return i < n_sink ? i : lo + (i - n_sink); }
 };
-__device__ __forceinline__ KeyTiles key_tiles(int q0, int window, int sinks) {
-  KeyTiles t;
-  const int first = q0 - window + 1;
-  t.lo = first > 0 ? first / kTile : 0;
-  const int ns = (sinks + kTile - 1) / kTile;
-  t.n_sink = ns < t.lo ? ns : t.lo;
-  return t;
+__device__ __forceinline__ KeyBlocks key_blocks(int qt, int S, int window, int sinks) {
+  KeyBlocks k;
+  const int first = qt * kTile - window + 1;
+  k.lo = first > 0 ? first / kBlk : 0;
+  const int ns = (sinks + kBlk - 1) / kBlk;
+  k.n_sink = ns < k.lo ? ns : k.lo;
+  const int nb = (S + kBlk - 1) / kBlk;
+  k.n = k.n_sink + (2 * qt + 2 < nb ? 2 * qt + 2 : nb) - k.lo;
+  return k;
+}
+// Some pair of the block of keys from k0 and the query tile from q0 is hidden.
+__device__ __forceinline__ bool block_edge(int k0, int q0, int S, int window, int sinks) {
+  return k0 + kBlk > S || k0 + kBlk > q0 + 1 || (q0 + kTile - 1 - k0 >= window && k0 + kBlk > sinks);
 }
 // Some pair of the tile of keys [k0, k0 + 128) and the queries up to q_max is
 // hidden by the window.
@@ -191,7 +198,6 @@ struct FwdArgs {
 // the softmax warps' TMEM reads beside them.
 constexpr int kFwdWarps = 4;  // softmax warps, one row per thread
 constexpr int kFwdThreads = 64 + 32 * kFwdWarps;
-constexpr int kBlk = 64;      // keys per block
 constexpr int kRing = 5;
 struct WinFwdSmem {
   static constexpr int kQ = 0;
@@ -232,20 +238,12 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nq = (a.S + kTile - 1) / kTile;
-  const int nb = (a.S + kBlk - 1) / kBlk;
   const int bh = blockIdx.x % (a.B * a.H);
   const int qt = nq - 1 - blockIdx.x / (a.B * a.H);  // late tiles first: early ones are short
   const int b = bh / a.H, h = bh % a.H;
   const int hk = h / (a.H / a.Hk);
-  // The tile's list of key blocks: the sinks' before the window, then from the first
-  // block that its first row sees to the diagonal.
-  const int q_lo = qt * kTile - a.window + 1;
-  const int lo = q_lo > 0 ? q_lo / kBlk : 0;
-  const int sink_blocks = (a.sinks + kBlk - 1) / kBlk;
-  const int ns = sink_blocks < lo ? sink_blocks : lo;
-  const int end = 2 * qt + 2 < nb ? 2 * qt + 2 : nb;  // one past the diagonal block
-  const int n = ns + end - lo;
-  auto block_of = [&](int i) { return i < ns ? i : lo + (i - ns); };
+  const KeyBlocks kb = key_blocks(qt, a.S, a.window, a.sinks);
+  const int n = kb.n;
   const uint64_t wait_ns = a.wait_ns;
 
   if (threadIdx.x == 0) {
@@ -283,7 +281,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
         const int st = i % kRing;
         if (!bounded_wait(empty(st), ((i / kRing) & 1) ^ 1, abort_flag, err, kErrWinProducer, wait_ns))
           break;
-        const int key0 = block_of(i >> 1) * kBlk;
+        const int key0 = kb.at(i >> 1) * kBlk;
         const CUtensorMap* map = (i & 1) ? &tma_v : &tma_k;
         const uint32_t d = sbase + L::kKV + st * kStepTile;
         mbar_arrive_expect_tx(full(st), kStepTile);
@@ -384,12 +382,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       float s0[32], s1[32];
       tmem_ld32_async(s_t, s0);
       tmem_ld32_async(s_t + 32, s1);
-      const int k0 = block_of(i) * kBlk;
-      const bool edge = k0 + kBlk > a.S || k0 + kBlk > qt * kTile + 1 ||
-                        (qt * kTile + kTile - 1 - k0 >= a.window && k0 + kBlk > a.sinks);
+      const int k0 = kb.at(i) * kBlk;
       int kind0 = 1, kind1 = 1;
       uint32_t mk0 = 0xffffffffu, mk1 = 0xffffffffu;
-      if (edge) {
+      if (block_edge(k0, qt * kTile, a.S, a.window, a.sinks)) {
         mk0 = keys_seen(q, k0, a.S, a.window, a.sinks);
         mk1 = keys_seen(q, k0 + 32, a.S, a.window, a.sinks);
         kind0 = mask_kind(mk0, 0xffffffffu);
@@ -501,8 +497,11 @@ struct BwdArgs {
   float scale;       // softmax scale (applied to dK, dQ in fp32)
   float scale_log2;  // scale * log2(e)
   int window, sinks;
-  const float* Dv;   // [B, H, S_pad] dO . O
-  const float* nl2;  // [B, H, S_pad] -lse * log2(e)
+  float* Dv;         // [B, H, S_pad] dO . O: written by the dQ kernel, read by dK / dV's
+  float* nl2;        // [B, H, S_pad] -lse * log2(e), the same
+  const bf16* out;   // [B, S, H, D]
+  const bf16* dout;
+  const float* lse;  // [B, H, S_pad]
   bf16* dq;          // [B, S, H, D]
   bf16* dk;          // [B, S, Hk, D]
   bf16* dv;
@@ -931,32 +930,39 @@ __global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles)
   *reinterpret_cast<uint2*>(a.dv + o) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
 }
 
-// dQ of one query tile: TMEM columns S 0, dP 128, dQ 256, two dS buffers 384 and 448 (bf16, two
-// per column: the A operand of dQ += dS K read from TMEM). S and dP have barriers of their own:
-// S(j + 1) starts when S(j) has been read, which is during dP(j), so the tensor pipe does not
-// wait for the TMEM reads, and with two dS buffers the next dS is written while the product
-// of the last one runs (187 us with two against 216 with one, at 1 x 16001 tokens, 12 heads
-// over 2, window 1000, 16 sinks). Shared memory: Q and dO (32 KB each, loaded once), a K
-// ring (3 x 32 KB; a stage frees after its dQ product) and a V ring (2 x 32 KB; a stage
-// frees after its dP product). A compute thread owns 32 keys of one query row of each tile.
-constexpr int kDqKStages = 3;
-constexpr int kDqVStages = 2;
+// dQ of one query tile, keys in blocks of 64, two CTAs an SM (one fills the tensor pipe while
+// the other's compute warps work, starts or ends): 204 us with D at 1 x 16001 tokens, 12 heads
+// over 2, window 1000, 16 sinks, against 206 + 31 us of one CTA an SM with 128-key tiles and a
+// kernel for D; 76 against 76 + 20 us at 4 x 2048 tokens, window 512. A persistent CTA that
+// loads the next tile's operands early measured 212 and 85 us. Bound by the products: N = 64
+// ones take as long as N = 128 ones.
+// TMEM (256 columns): S 0, dP 64, dQ 128. dS overwrites the dP columns that it was computed
+// from (bf16 pairs, the 32 keys of a compute warp in the first 16 of its own 32 columns) and
+// is the A operand of dQ += dS K read from TMEM. Issue order
+//   S(i + 1), dQ(i), dP(i + 1), S(i + 2), ...
+// Shared memory: Q and dO (32 KB each), two K blocks and a V block of 16 KB. A compute thread
+// owns 32 keys of one query row of each block.
+// The compute warps first form D = dO . O of the tile's rows, and store it with
+// -lse log2(e) for the dK / dV kernel, which follows: no kernel of its own reads out and dout.
+constexpr int kDqWarps = 8;
+constexpr int kDqThreads = 64 + 32 * kDqWarps;
 struct WinDqSmem {
   static constexpr int kQ = 0;
   static constexpr int kDO = kQ + kTileBytes;
   static constexpr int kK = kDO + kTileBytes;
-  static constexpr int kV = kK + kDqKStages * kTileBytes;
-  static constexpr int kBar = kV + kDqVStages * kTileBytes;
-  // qdo_full, k_full[3], k_empty[3], v_full[2], v_empty[2], s_full, s_empty, dp_full,
-  // dp_empty, ds_full[2], ds_free[2], acc_done, drain
-  static constexpr int kNumBars = 1 + 2 * kDqKStages + 2 * kDqVStages + 10;
+  static constexpr int kV = kK + 2 * kStepTile;
+  static constexpr int kBar = kV + kStepTile;
+  // qdo_full, k_full[2], k_empty[2], v_full, v_empty, s_full, s_empty, dp_full, ds_full, d_full,
+  // acc_done, drain
+  static constexpr int kNumBars = 14;
   static constexpr int kMisc = kBar + kNumBars * 8;
-  static constexpr int kUsed = kMisc + 16;
-  static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
+  static constexpr int kD = kMisc + 16;  // D of the rows
+  static constexpr int kUsed = kD + kTile * 4;
+  static constexpr int kBytes = 115712;  // half of an SM's 228 KB less 1 KB a CTA
 };
-static_assert(WinDqSmem::kUsed + 128 <= 232448, "window attention dQ shared memory");
+static_assert(WinDqSmem::kUsed + 256 <= WinDqSmem::kBytes, "window attention dQ shared memory");
 
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kDqThreads, 2)
     win_dq_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_k,
                   const __grid_constant__ CUtensorMap tma_v,
                   const __grid_constant__ CUtensorMap tma_do, BwdArgs a, int* err) {
@@ -971,17 +977,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sbase = smem_u32(smem);
   const uint32_t bar0 = sbase + L::kBar;
   const uint32_t qdo_full = bar0;
-  auto k_full = [&](int st) { return bar0 + 8u * (1 + st); };
-  auto k_empty = [&](int st) { return bar0 + 8u * (1 + kDqKStages + st); };
-  auto v_full = [&](int st) { return bar0 + 8u * (1 + 2 * kDqKStages + st); };
-  auto v_empty = [&](int st) { return bar0 + 8u * (1 + 2 * kDqKStages + kDqVStages + st); };
-  constexpr int kB = 1 + 2 * kDqKStages + 2 * kDqVStages;
-  const uint32_t s_full = bar0 + 8u * kB, s_empty = bar0 + 8u * (kB + 1);
-  const uint32_t dp_full = bar0 + 8u * (kB + 2), dp_empty = bar0 + 8u * (kB + 3);
-  // of tile j: its dS buffer is j & 1, the phase (j >> 1) & 1
-  auto ds_full = [&](int j) { return bar0 + 8u * (kB + 4 + (j & 1)); };
-  auto ds_free = [&](int j) { return bar0 + 8u * (kB + 6 + (j & 1)); };
-  const uint32_t acc_done = bar0 + 8u * (kB + 8), drain_bar = bar0 + 8u * (kB + 9);
+  auto k_full = [&](int i) { return bar0 + 8u * (1 + (i & 1)); };
+  auto k_empty = [&](int i) { return bar0 + 8u * (3 + (i & 1)); };
+  const uint32_t v_full = bar0 + 8u * 5, v_empty = bar0 + 8u * 6;
+  const uint32_t s_full = bar0 + 8u * 7, s_empty = bar0 + 8u * 8;
+  const uint32_t dp_full = bar0 + 8u * 9, ds_full = bar0 + 8u * 10, d_full = bar0 + 8u * 11;
+  const uint32_t acc_done = bar0 + 8u * 12, drain_bar = bar0 + 8u * 13;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
 
@@ -992,16 +993,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int b = bh / a.H, h = bh % a.H;
   const int hk = h / (a.H / a.Hk);
   const int q0 = qt * kTile;
-  const KeyTiles kt = key_tiles(q0, a.window, a.sinks);
-  const int n = kt.n_sink + (qt + 1 - kt.lo);
+  const KeyBlocks kb = key_blocks(qt, a.S, a.window, a.sinks);
+  const int n = kb.n;
   const uint64_t wait_ns = a.wait_ns;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kNumBars; ++i) {
       const uint32_t bar = bar0 + 8u * i;
-      mbar_init(bar, bar == s_empty || bar == dp_empty || bar == ds_full(0) || bar == ds_full(1)
-                         ? kWarps
-                         : 1);
+      mbar_init(bar, bar == s_empty || bar == ds_full || bar == d_full ? kDqWarps : 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -1014,7 +1013,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_holder)),
-                 "r"(512)
+                 "r"(256)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -1032,40 +1031,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_load_4d(sbase + L::kDO, &tma_do, qdo_full, 0, q0, h, b);
       tma_load_4d(sbase + L::kDO + kBox, &tma_do, qdo_full, 64, q0, h, b);
       int issued_k = 0, issued_v = 0;
-      for (int j = 0; j < n; ++j) {
-        const int sk = j % kDqKStages, sv = j % kDqVStages;
-        const int key0 = kt.at(j) * kTile;
-        if (!bounded_wait(k_empty(sk), ((j / kDqKStages) & 1) ^ 1, abort_flag, err, kErrWinProducer,
-                          wait_ns))
+      for (int i = 0; i < n; ++i) {
+        const int key0 = kb.at(i) * kBlk;
+        if (!bounded_wait(k_empty(i), ((i >> 1) & 1) ^ 1, abort_flag, err, kErrWinProducer, wait_ns))
           break;
-        const uint32_t kd = sbase + L::kK + sk * kTileBytes;
-        mbar_arrive_expect_tx(k_full(sk), kTileBytes);
-        tma_load_4d(kd, &tma_k, k_full(sk), 0, key0, hk, b);
-        tma_load_4d(kd + kBox, &tma_k, k_full(sk), 64, key0, hk, b);
+        const uint32_t kd = sbase + L::kK + (i & 1) * kStepTile;
+        mbar_arrive_expect_tx(k_full(i), kStepTile);
+        tma_load_4d(kd, &tma_k, k_full(i), 0, key0, hk, b);
+        tma_load_4d(kd + kStepBox, &tma_k, k_full(i), 64, key0, hk, b);
         ++issued_k;
-        if (!bounded_wait(v_empty(sv), ((j / kDqVStages) & 1) ^ 1, abort_flag, err, kErrWinProducer,
-                          wait_ns))
-          break;
-        const uint32_t vd = sbase + L::kV + sv * kTileBytes;
-        mbar_arrive_expect_tx(v_full(sv), kTileBytes);
-        tma_load_4d(vd, &tma_v, v_full(sv), 0, key0, hk, b);
-        tma_load_4d(vd + kBox, &tma_v, v_full(sv), 64, key0, hk, b);
+        if (!bounded_wait(v_empty, (i & 1) ^ 1, abort_flag, err, kErrWinProducer, wait_ns)) break;
+        mbar_arrive_expect_tx(v_full, kStepTile);
+        tma_load_4d(sbase + L::kV, &tma_v, v_full, 0, key0, hk, b);
+        tma_load_4d(sbase + L::kV + kStepBox, &tma_v, v_full, 64, key0, hk, b);
         ++issued_v;
       }
       uint64_t t0 = tc::globaltimer();
       while (!mbar_try_wait(qdo_full, 0) && tc::globaltimer() - t0 < wait_ns) {
       }
-      for (int j = issued_k > kDqKStages ? issued_k - kDqKStages : 0; j < issued_k; ++j) {
+      for (int i = issued_k > 2 ? issued_k - 2 : 0; i < issued_k; ++i) {
         t0 = tc::globaltimer();
-        while (!mbar_try_wait(k_full(j % kDqKStages), (j / kDqKStages) & 1) &&
-               tc::globaltimer() - t0 < wait_ns) {
+        while (!mbar_try_wait(k_full(i), (i >> 1) & 1) && tc::globaltimer() - t0 < wait_ns) {
         }
       }
-      for (int j = issued_v > kDqVStages ? issued_v - kDqVStages : 0; j < issued_v; ++j) {
-        t0 = tc::globaltimer();
-        while (!mbar_try_wait(v_full(j % kDqVStages), (j / kDqVStages) & 1) &&
-               tc::globaltimer() - t0 < wait_ns) {
-        }
+      t0 = tc::globaltimer();
+      while (issued_v > 0 && !mbar_try_wait(v_full, (issued_v - 1) & 1) &&
+             tc::globaltimer() - t0 < wait_ns) {
       }
     }
   } else if (warp == 1) {
@@ -1078,61 +1069,59 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Desc q_desc(smem_desc_sw128(sbase + L::kQ, 16, 1024));
     const Desc do_desc(smem_desc_sw128(sbase + L::kDO, 16, 1024));
     const Desc k_desc(smem_desc_sw128(sbase + L::kK, 16, 1024));
-    const Desc k_mn(smem_desc_sw128(sbase + L::kK, kBox, 1024));
+    const Desc k_mn(smem_desc_sw128(sbase + L::kK, kStepBox, 1024));
     const Desc v_desc(smem_desc_sw128(sbase + L::kV, 16, 1024));
-    auto issue_sd = [&](int j) -> bool {
-      const int sk = j % kDqKStages, sv = j % kDqVStages;
-      if (!wait(k_full(sk), (j / kDqKStages) & 1)) return false;
-      if (j > 0 && !wait(s_empty, (j - 1) & 1)) return false;
+    auto issue_s = [&](int i) -> bool {  // S = Q K^T
+      if (!wait(k_full(i), (i >> 1) & 1)) return false;
+      if (i > 0 && !wait(s_empty, (i - 1) & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kHeadDim / 16; ++kk)  // S = Q K^T
+        for (int kk = 0; kk < kHeadDim / 16; ++kk)
           mma_ss(tmem, q_desc.at(kmajor_step(kk, kBox)), q_desc.hi,
-                 k_desc.at(sk * kTileBytes + kmajor_step(kk, kBox)), k_desc.hi, kIdescKK,
+                 k_desc.at((i & 1) * kStepTile + kmajor_step(kk, kStepBox)), k_desc.hi, kIdescKK64,
                  kk > 0 ? 1u : 0u);
         tc_commit(s_full);
       }
       __syncwarp();
       issued = true;
-      if (!wait(v_full(sv), (j / kDqVStages) & 1)) return false;
-      if (j > 0 && !wait(dp_empty, (j - 1) & 1)) return false;
+      return true;
+    };
+    auto issue_dp = [&](int i) -> bool {  // dP = dO V^T
+      if (!wait(v_full, i & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kHeadDim / 16; ++kk)  // dP = dO V^T
-          mma_ss(tmem + 128, do_desc.at(kmajor_step(kk, kBox)), do_desc.hi,
-                 v_desc.at(sv * kTileBytes + kmajor_step(kk, kBox)), v_desc.hi, kIdescKK,
-                 kk > 0 ? 1u : 0u);
+        for (int kk = 0; kk < kHeadDim / 16; ++kk)
+          mma_ss(tmem + 64, do_desc.at(kmajor_step(kk, kBox)), do_desc.hi,
+                 v_desc.at(kmajor_step(kk, kStepBox)), v_desc.hi, kIdescKK64, kk > 0 ? 1u : 0u);
         tc_commit(dp_full);
-        tc_commit(v_empty(sv));
+        tc_commit(v_empty);
       }
       __syncwarp();
       return true;
     };
-    if (ok) ok = issue_sd(0);
-    for (int j = 0; j < n && ok; ++j) {
-      const int sk = j % kDqKStages;
-      if (j + 1 < n && !(ok = issue_sd(j + 1))) break;
-      if (!(ok = wait(ds_full(j), (j >> 1) & 1))) break;
+    if (ok) ok = issue_s(0);
+    if (ok) ok = issue_dp(0);
+    for (int i = 0; i < n && ok; ++i) {
+      if (i + 1 < n && !(ok = issue_s(i + 1))) break;
+      if (!(ok = wait(ds_full, i & 1))) break;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kTile / 16; ++kk)  // dQ += dS K (dS from TMEM: 8 columns per 16 keys)
-          mma_ts(tmem + 256, tmem + 384 + (j & 1) * 64 + kk * 8,
-                 k_mn.at(sk * kTileBytes + mnmajor_step(kk)), k_mn.hi, kIdescKM, (j > 0 || kk > 0) ? 1u : 0u);
-        tc_commit(ds_free(j));
-        tc_commit(k_empty(sk));
+        for (int kk = 0; kk < kBlk / 16; ++kk)  // dQ += dS K
+          mma_ts(tmem + 128, tmem + 64 + (kk >> 1) * 32 + (kk & 1) * 8,
+                 k_mn.at((i & 1) * kStepTile + mnmajor_step(kk)), k_mn.hi, kIdescKM,
+                 (i > 0 || kk > 0) ? 1u : 0u);
+        tc_commit(k_empty(i));
+        if (i + 1 == n) tc_commit(acc_done);
       }
       __syncwarp();
+      if (i + 1 < n) ok = issue_dp(i + 1);
     }
-    if (ok && elect_one()) tc_commit(acc_done);
-    __syncwarp();
-    for (int j = n > kDqKStages ? n - kDqKStages : 0; j < n && ok; ++j) {
-      ok = wait(k_empty(j % kDqKStages), (j / kDqKStages) & 1);
-      if (ok && j >= n - kDqVStages) ok = wait(v_empty(j % kDqVStages), (j / kDqVStages) & 1);
-      if (ok && j >= n - 2) ok = wait(ds_free(j), (j >> 1) & 1);
-    }
+    // the last arrivals of the rings
+    for (int i = n > 2 ? n - 2 : 0; i < n && ok; ++i) ok = wait(k_empty(i), (i >> 1) & 1);
+    if (ok) ok = wait(v_empty, (n - 1) & 1);
     if (!ok && issued) {
       if (elect_one()) tc_commit(drain_bar);
       __syncwarp();
@@ -1143,38 +1132,76 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------------------------------- compute ----
     const int quarter = warp & 3;
-    const int part = (warp - 2) >> 2;   // keys [32 part, 32 part + 32) of each tile
-    const int cb = part * 32;
+    const int part = (warp - 2) >> 2;   // keys [32 part, 32 part + 32) of each block
     const int r = quarter * 32 + lane;  // query row of this thread
     const int q = q0 + r;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const int64_t vidx = ((int64_t)b * a.H + h) * ((int64_t)nq * kTile) + q;
-    const float nl = q < a.S ? a.nl2[vidx] : 0.f;
-    const float nd = q < a.S ? -a.Dv[vidx] : 0.f;
     const uint64_t sl2 = f2_pack(a.scale_log2, a.scale_log2);
+    const uint32_t s_t = tmem + part * 32 + lane_off, dp_t = s_t + 64;
+    const int64_t vrow = ((int64_t)b * a.H + h) * ((int64_t)nq * kTile);
+    float* d_rows = reinterpret_cast<float*>(smem + L::kD);
+    bool ok = true, w = true;
+    const float nl = q < a.S ? -a.lse[vrow + q] * kLog2e : 0.f;
+    {  // D: 16 lanes a row (16 bytes each), four rows of a half-warp in flight
+      const int sub = lane & 15;
+#pragma unroll 1
+      for (int r0 = ((warp - 2) * 2 + (lane >> 4)) * 4; r0 < kTile; r0 += 8 * kDqWarps) {
+        uint4 x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = y[e] = make_uint4(0, 0, 0, 0);
+          if (q0 + r0 + e < a.S) {
+            const int64_t o = (((int64_t)b * a.S + q0 + r0 + e) * a.H + h) * kHeadDim + sub * 8;
+            x[e] = *reinterpret_cast<const uint4*>(a.dout + o);
+            y[e] = *reinterpret_cast<const uint4*>(a.out + o);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const __nv_bfloat162* xp = reinterpret_cast<const __nv_bfloat162*>(&x[e]);
+          const __nv_bfloat162* yp = reinterpret_cast<const __nv_bfloat162*>(&y[e]);
+          float acc = 0.f;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float2 f = __bfloat1622float2(xp[v]), g = __bfloat1622float2(yp[v]);
+            acc = fmaf(f.x, g.x, fmaf(f.y, g.y, acc));
+          }
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+          if (sub == 0) d_rows[r0 + e] = acc;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(d_full);
+        w = bounded_wait(d_full, 0, abort_flag, err, kErrWinSoftmax, wait_ns);
+      }
+      ok = warp_ok(w);
+      __syncwarp();
+    }
+    const float nd = ok ? -d_rows[r] : 0.f;
+    if (ok && part == 0 && q < a.S) {
+      a.Dv[vrow + q] = -nd;
+      a.nl2[vrow + q] = nl;
+    }
     const uint64_t nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
-    const uint32_t ds_tmem = tmem + 384 + part * 16 + lane_off;
-    bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      const int jt = kt.at(j);
-      const bool edge = jt * kTile + kTile > a.S || jt == qt ||
-                        win_edge(q0 + kTile - 1, jt * kTile, a.window, a.sinks);
+    for (int i = 0; i < n && ok; ++i) {
+      const int k0 = kb.at(i) * kBlk;
       uint32_t mk = 0xffffffffu;
       int kind = 1;
-      if (edge) {
-        mk = keys_seen(q, jt * kTile + cb, a.S, a.window, a.sinks);
+      if (block_edge(k0, q0, a.S, a.window, a.sinks)) {
+        mk = keys_seen(q, k0 + part * 32, a.S, a.window, a.sinks);
         kind = mask_kind(mk, 0xffffffffu);
       }
-      bool w = true;
-      if (lane == 0) w = bounded_wait(s_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      if (lane == 0) w = bounded_wait(s_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
       if (!(ok = warp_ok(w))) break;
       tc_fence_after();
       float p[32];
-      tmem_ld32_async(tmem + cb + lane_off, p);
+      tmem_ld32_async(s_t, p);
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(s_empty);  // the next tile's S may overwrite it
+      if (lane == 0) mbar_arrive(s_empty);  // the next block's S may overwrite it
       if (kind != 0) {
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
@@ -1183,18 +1210,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           p[e + 1] = fast_exp2(p[e + 1]);
         }
       }
-      if (lane == 0) w = bounded_wait(dp_full, j & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
+      if (lane == 0) w = bounded_wait(dp_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
       if (!(ok = warp_ok(w))) break;
       tc_fence_after();
       float dp[32];
-      tmem_ld32_async(tmem + 128 + cb + lane_off, dp);
+      tmem_ld32_async(dp_t, dp);
       tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(dp_empty);
 #pragma unroll
       for (int e = 0; e < 32; e += 2)
-        f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), p[e], p[e + 1]);
+        f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]), f2_add(f2_pack(dp[e], dp[e + 1]), nd2)), p[e],
+                  p[e + 1]);
       if (kind != 1) {  // hidden keys may hold anything: select, do not scale
 #pragma unroll
         for (int e = 0; e < 32; ++e)
@@ -1203,37 +1228,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t dw[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) dw[e] = pack_bf16(p[2 * e], p[2 * e + 1]);
-      if (j > 1) {  // the dQ product of the tile before the previous one has read this buffer
-        if (lane == 0)
-          w = bounded_wait(ds_free(j), ((j - 2) >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-        if (!(ok = warp_ok(w))) break;
-        tc_fence_after();
-      }
-      tmem_st16u(ds_tmem + (j & 1) * 64, dw);
+      tmem_st16u(dp_t, dw);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full(j));
+      if (lane == 0) mbar_arrive(ds_full);
     }
     if (ok) {
-      bool w = true;
       if (lane == 0) w = bounded_wait(acc_done, 0, abort_flag, err, kErrWinSoftmax, wait_ns);
       ok = warp_ok(w);
     }
     if (ok) {
       tc_fence_after();
-      bf16* orow = a.dq + ((int64_t)b * a.S + q) * (int64_t)(a.H * kHeadDim) + h * kHeadDim + cb;
-      float o[32];
-      tmem_ld32(tmem + 256 + cb + lane_off, o);
-      if (q < a.S) {
-        const float sc = a.scale;
+      bf16* orow = a.dq + (((int64_t)b * a.S + q) * a.H + h) * kHeadDim + part * 64;
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint4*>(orow + 8 * g) =
-              make_uint4(pack_bf16(o[8 * g] * sc, o[8 * g + 1] * sc),
-                         pack_bf16(o[8 * g + 2] * sc, o[8 * g + 3] * sc),
-                         pack_bf16(o[8 * g + 4] * sc, o[8 * g + 5] * sc),
-                         pack_bf16(o[8 * g + 6] * sc, o[8 * g + 7] * sc));
+      for (int c = 0; c < 2; ++c) {
+        float o[32];
+        tmem_ld32(tmem + 128 + part * 64 + c * 32 + lane_off, o);
+        if (q < a.S) {
+          const float sc = a.scale;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint4*>(orow + c * 32 + 8 * g) =
+                make_uint4(pack_bf16(o[8 * g] * sc, o[8 * g + 1] * sc),
+                           pack_bf16(o[8 * g + 2] * sc, o[8 * g + 3] * sc),
+                           pack_bf16(o[8 * g + 4] * sc, o[8 * g + 5] * sc),
+                           pack_bf16(o[8 * g + 6] * sc, o[8 * g + 7] * sc));
+        }
       }
     }
   }
@@ -1242,7 +1263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256)
                  : "memory");
   }
 }
@@ -1404,34 +1425,32 @@ int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const voi
   float* dvec = reinterpret_cast<float*>(ws);
   float* nl2 = reinterpret_cast<float*>(ws + vbytes);
   float* part = reinterpret_cast<float*>(ws + 2 * vbytes);
-  CUtensorMap mq, mk, mv, mdo;
+  CUtensorMap mq, mk, mv, mkb, mvb, mdo;  // tiles of 128 keys (dK, dV) and blocks of 64 (dQ)
   int rc;
   const int64_t do_strides[3] = {seq * heads * kHeadDim, kHeadDim, heads * kHeadDim};
   if ((rc = make_bhsd_map(&mq, q, q_strides, batch, heads, seq, "q"))) return rc;
   if ((rc = make_bhsd_map(&mk, k, k_strides, batch, kv_heads, seq, "k"))) return rc;
   if ((rc = make_bhsd_map(&mv, v, v_strides, batch, kv_heads, seq, "v"))) return rc;
+  if ((rc = make_bhsd_map(&mkb, k, k_strides, batch, kv_heads, seq, "k", kBlk))) return rc;
+  if ((rc = make_bhsd_map(&mvb, v, v_strides, batch, kv_heads, seq, "v", kBlk))) return rc;
   if ((rc = make_bhsd_map(&mdo, dout, do_strides, batch, heads, seq, "dout"))) return rc;
   static bool dkdv_set[64] = {false}, dq_set[64] = {false};
   if ((rc = set_smem(win_dkdv_kernel, WinDkvSmem::kBytes, dkdv_set))) return rc;
   if ((rc = set_smem(win_dq_kernel, WinDqSmem::kBytes, dq_set))) return rc;
   cudaStream_t st = as_stream(stream);
   const int B = (int)batch, H = (int)heads, Hk = (int)kv_heads, S = (int)seq;
-  const int64_t rows = (int64_t)B * S * H;
-  int64_t dot_blocks = (rows + 16 * kDotRows - 1) / (16 * kDotRows);  // 16 half-warps per block
-  if (dot_blocks > 16 * num_sms()) dot_blocks = 16 * num_sms();
-  attn_bwd_dot_kernel<<<(unsigned)dot_blocks, 256, 0, st>>>(
-      static_cast<const bf16*>(dout), static_cast<const bf16*>(out), lse, B, H, S, dvec, nl2);
-  if ((rc = launch_status())) return rc;
   const int win = (int)(window < seq ? window : seq);
   const int snk = win == S ? 0 : (int)(sinks < seq ? sinks : seq);
   BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, win, snk, dvec, nl2,
+            static_cast<const bf16*>(out), static_cast<const bf16*>(dout), lse,
             static_cast<bf16*>(dq), static_cast<bf16*>(dk), static_cast<bf16*>(dv), part, p.groups,
             p.heads_per, p.n_sink, p.segs, p.seg_steps,
             wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
   const int nt = (S + kTile - 1) / kTile;
-  win_dkdv_kernel<<<(unsigned)p.units, kThreads, WinDkvSmem::kBytes, st>>>(mq, mk, mv, mdo, a, err);
+  win_dq_kernel<<<(unsigned)(B * H * nt), kDqThreads, WinDqSmem::kBytes, st>>>(mq, mkb, mvb, mdo, a,
+                                                                              err);
   if ((rc = launch_status())) return rc;
-  win_dq_kernel<<<(unsigned)(B * H * nt), kThreads, WinDqSmem::kBytes, st>>>(mq, mk, mv, mdo, a, err);
+  win_dkdv_kernel<<<(unsigned)p.units, kThreads, WinDkvSmem::kBytes, st>>>(mq, mk, mv, mdo, a, err);
   if ((rc = launch_status())) return rc;
   const int tiles = p.groups > 1 ? nt : p.n_sink;  // key tiles whose sums are in slots
   if (tiles == 0) return SOUP_OK;
