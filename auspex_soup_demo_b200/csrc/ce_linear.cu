@@ -1353,11 +1353,25 @@ __global__ void __launch_bounds__(256) logps_gather_kernel(
   const T* h = H + (int64_t)row * h_ld;
   const T* w = W + (t >= 0 && t < vocab ? t : 0) * w_ld;
   float acc = 0.f;
-  for (int k = lane * 8; k < dim; k += 256) {
-    const Vec16<T> a = ld16(h + k), b = ld16(w + k);
-    st16(out + k, a);
+  constexpr int kBatch = 4;  // vectors in flight
+  for (int k0 = lane * 8; k0 < dim; k0 += 256 * kBatch) {
+    Vec16<T> a[kBatch], b[kBatch];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc = fmaf(Cvt<T>::to_f(a.v[i]), Cvt<T>::to_f(b.v[i]), acc);
+    for (int u = 0; u < kBatch; ++u) {
+      const int k = k0 + 256 * u;
+      a[u].u = b[u].u = make_uint4(0, 0, 0, 0);
+      if (k < dim) {
+        a[u] = ld16(h + k);
+        b[u] = ld16(w + k);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int k = k0 + 256 * u;
+      if (k < dim) st16(out + k, a[u]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc = fmaf(Cvt<T>::to_f(a[u].v[i]), Cvt<T>::to_f(b[u].v[i]), acc);
+    }
   }
   acc = warp_sum(acc);
   if (lane == 0) {

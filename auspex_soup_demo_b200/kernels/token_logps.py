@@ -17,6 +17,7 @@ model's log-probabilities) nothing of size [tokens, vocab] is written.
 
 from __future__ import annotations
 
+import functools
 from typing import Any, Tuple
 
 import torch
@@ -42,12 +43,20 @@ def _operand_dtype(hidden: torch.Tensor, weight: torch.Tensor) -> torch.dtype:
     return torch.bfloat16 if both else torch.float16
 
 
+@functools.lru_cache(maxsize=256)
+def _state_bytes(n: int, vocab: int, dim: int) -> int:
+    return _lib.lib().soup_head_logps_state_bytes(n, vocab, dim)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(n: int, vocab: int, dim: int, backward: int) -> int:
+    return _lib.lib().soup_head_logps_workspace_bytes(n, vocab, dim, backward)
+
+
 def _block_rows(n: int, vocab: int, dim: int) -> int:
     """Rows per launch sequence: what CE_WORKSPACE_BYTES holds (0: all)."""
     budget = chunked_ce.CE_WORKSPACE_BYTES
-    lib = _lib.lib()
-    full = (lib.soup_head_logps_state_bytes(n, vocab, dim)
-            + lib.soup_head_logps_workspace_bytes(n, vocab, dim, 0))
+    full = _state_bytes(n, vocab, dim) + _workspace_bytes(n, vocab, dim, 0)
     if budget <= 0 or full <= budget:
         return n
     return min(n, max(256, int(budget // (full / n)) // 256 * 256))
@@ -56,7 +65,7 @@ def _block_rows(n: int, vocab: int, dim: int) -> int:
 def _forward(h, w, labels, ignore_index, logps, ents, state) -> None:
     n, d = h.shape
     v = w.shape[0]
-    nbytes = _lib.lib().soup_head_logps_workspace_bytes(n, v, d, 0)
+    nbytes = _workspace_bytes(n, v, d, 0)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
     _lib.call("soup_head_logps_fwd", h.device, h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
               _lib.dtype_code(h.dtype), labels.data_ptr(), n, v, d, ignore_index, logps.data_ptr(),
@@ -65,7 +74,7 @@ def _forward(h, w, labels, ignore_index, logps, ents, state) -> None:
 
 
 def _new_state(n, v, d, device) -> torch.Tensor:
-    return torch.empty(_lib.lib().soup_head_logps_state_bytes(n, v, d), dtype=torch.uint8, device=device)
+    return torch.empty(_state_bytes(n, v, d), dtype=torch.uint8, device=device)
 
 
 class HeadTokenLogpsFunction(torch.autograd.Function):
@@ -119,7 +128,6 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
         if need_w:
             one = ctx.block == n and weight.dtype in (torch.bfloat16, torch.float32)
             dw = torch.empty(v, d, dtype=weight.dtype if one else torch.float32, device=dev)
-        lib = _lib.lib()
         for r0 in range(0, n, ctx.block):
             r = min(n, r0 + ctx.block) - r0
             hb = None if h is None else h[r0:r0 + r]
@@ -131,7 +139,7 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
                     lp = torch.empty(min(n, ctx.block), dtype=torch.float32, device=dev)
                 st = st_buf
                 _forward(hb, w, t[r0:r0 + r], ignore, lp, None, st)
-            nbytes = lib.soup_head_logps_workspace_bytes(r, v, d, 1)
+            nbytes = _workspace_bytes(r, v, d, 1)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             _lib.call("soup_head_logps_bwd", dev, st.data_ptr(), st.numel(), _lib.ptr(hb),
                       d if hb is None else hb.stride(0), _lib.dtype_code(dt), _lib.ptr(wb),

@@ -149,48 +149,45 @@ def test_entry_points_refuse_bad_arguments():
 def test_workspace_sizes():
     lib = _lib.lib()
     assert lib.soup_preference_loss_workspace_bytes(0, 5) == 0
-    assert lib.soup_policy_loss_workspace_bytes(3, 4097) >= 2 * lib.soup_policy_loss_workspace_bytes(3, 4096)
+    assert lib.soup_policy_loss_workspace_bytes(3, 4097) > lib.soup_policy_loss_workspace_bytes(3, 4096)
     assert lib.soup_head_logps_state_bytes(10, 0, 8) == 0
 
 
-# ---- the key tiles of a window (the kernels' index arithmetic, 128-key tiles) -------
-def _tiles(q0, window, sinks):
-    first = q0 - window + 1
-    lo = first // 128 if first > 0 else 0
-    n_sink = min(-(-sinks // 128), lo)
-    return n_sink, lo
+# ---- the key blocks of a window (the kernels' index arithmetic, 64-key blocks) -------
+def _blocks(qt, S, window, sinks):
+    first = qt * 128 - window + 1
+    lo = first // 64 if first > 0 else 0
+    n_sink = min(-(-sinks // 64), lo)
+    return n_sink, lo, n_sink + min(2 * qt + 2, -(-S // 64)) - lo
 
 
 @pytest.mark.parametrize("S", [1, 127, 128, 129, 300, 640, 1000])
 @pytest.mark.parametrize("window", [1, 2, 64, 127, 128, 129, 130, 300, 5000])
 @pytest.mark.parametrize("sinks", [0, 1, 127, 128, 129, 400, 5000])
-def test_window_tile_lists_cover_every_visible_key(S, window, sinks):
+def test_window_block_lists_cover_every_visible_key(S, window, sinks):
     window, sinks = min(window, S), min(sinks, S)
     nq, nq64 = -(-S // 128), -(-S // 64)
 
     def needed(qt):
-        tiles = set()
-        for q in (qt * 128, min(S, qt * 128 + 128) - 1):
-            tiles |= set(range(max(0, q - window + 1) // 128, q // 128 + 1))
-            tiles |= set(range(0, -(-min(sinks, q + 1) // 128)))
-        return tiles
+        blocks = set()
+        for q in range(qt * 128, min(S, qt * 128 + 128)):
+            blocks |= set(range(max(0, q - window + 1) // 64, q // 64 + 1))
+            blocks |= set(range(0, -(-min(sinks, q + 1) // 64)))
+        return blocks
 
-    for qt in range(nq):  # one query tile (dQ) and a pair of them (forward)
-        for end in {qt + 1, min(qt + 2, nq)}:
-            n_sink, lo = _tiles(qt * 128, window, sinks)
-            n = end - (lo - n_sink)
-            tiles = [j if j < n_sink else lo + j - n_sink for j in range(n)]
-            assert len(set(tiles)) == n >= 1 and all(0 <= t < end for t in tiles)
-            for t in range(qt, end):
-                assert needed(t) <= set(tiles)
-    for kt in range(nq):  # the 64-query steps of a key tile (dK / dV)
-        first, n = 2 * kt, nq64 - 2 * kt
+    for qt in range(nq):  # one query tile (forward and dQ)
+        n_sink, lo, n = _blocks(qt, S, window, sinks)
+        blocks = [i if i < n_sink else lo + i - n_sink for i in range(n)]
+        assert len(set(blocks)) == n >= 1 and all(0 <= i < nq64 for i in blocks)
+        assert needed(qt) <= set(blocks)
+    for kt in range(nq):  # the 128-query steps of a key tile (dK / dV)
+        first, n = kt, nq - kt
         if kt * 128 >= sinks:
-            n = min((kt * 128 + 127 + window - 1) // 64, nq64 - 1) - first + 1
-        assert n >= 1 and first + n <= nq64
+            n = min((kt * 128 + 127 + window - 1) // 128, nq - 1) - first + 1
+        assert n >= 1 and first + n <= nq
         for key in range(kt * 128, min(S, kt * 128 + 128)):
             last = S - 1 if key < sinks else min(S - 1, key + window - 1)
-            assert first <= key // 64 and last // 64 < first + n
+            assert first <= key // 128 and last // 128 < first + n
 
 
 class _Layer(torch.nn.Module):
