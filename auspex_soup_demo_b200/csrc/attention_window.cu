@@ -14,6 +14,12 @@
 // later query sees, are cut into segments with fp32 partials summed in a fixed order.
 // dQ per (batch, query head, query tile). Both recompute P from the log-sum-exp; no
 // atomics, results are bitwise reproducible.
+// Maxima, sums, log-sum-exps, D and all accumulators are fp32. P and dS are rounded to bf16,
+// as operands of products that run at the bf16 rate: at most 2^-8 of each entry, of either
+// sign, so it averages out in a sum over many keys and adds about the result's own bf16
+// rounding where a few keys dominate. D takes the bf16 output, the one that the caller holds. Hidden keys of a block that is read have weight 0
+// by selection, but 0 x NaN in a product is NaN: V must be finite there, as for any masked
+// softmax attention.
 //
 // A CTA leaves only after every asynchronous arrival on its barriers has landed: the
 // producer waits for its copies, the MMA warp for its commits.

@@ -43,7 +43,8 @@ const char* soup_last_error(void);
  * meanwhile by a kernel on another stream stays for the next read), then
  * synchronises the given stream. Codes: 0x101 producer, 0x102 MMA issuer,
  * 0x103 epilogue wait expired, 0x104 a stream-K partial never became
- * ready. No counterpart in the reference (its Triton kernels have no
+ * ready; 0x131-0x133 the producer, MMA issuer and compute warps of the window
+ * attention, 0x134 its shared memory too small. No counterpart in the reference (its Triton kernels have no
  * device-side waits). */
 int soup_device_error(void* stream, int* out_code);
 
@@ -249,9 +250,10 @@ int soup_ce_vp_backward(void* workspace, size_t workspace_bytes, const void* hid
  * t_i, and the softmax entropy (entropies may be NULL); both 0 where the target
  * is ignore_index, and logps NaN where it is outside [0, vocab). Only rows with a
  * target other than ignore_index take part in the matrix products, forward and
- * backward. Operand types and row rules as for soup_ce_linear. With `state` (soup_head_logps_state_bytes)
- * the forward keeps the row-shifted exponentials that the backward multiplies;
- * without it (NULL) no [rows, vocab] buffer is written.
+ * backward. Operand types and row rules as for soup_ce_linear. With `state`
+ * (soup_head_logps_state_bytes) the forward keeps the row-shifted exponentials
+ * that the backward multiplies; without it (NULL) no [rows, vocab] buffer is
+ * written.
  * The backward takes one weight per token, dlogps[i] = dL/dlogps[i] (not read
  * where the target was ignore_index), and the state of a forward with the same
  * hidden and weight; it does not change the state, so it may run more
