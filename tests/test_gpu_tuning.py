@@ -587,6 +587,33 @@ def test_window_and_swiglu8_in_graphs():
         assert all(torch.equal(a, b) for a, b in zip(res, want))
 
 
+def test_window_on_two_streams_at_once():
+    """More CTAs than SMs on each stream, with the head's products between them."""
+    st = _chain_inputs(41)
+    st["h"].requires_grad_(True)
+    st["w"].requires_grad_(True)
+    ins = [[t.detach().requires_grad_(True) for t in qkv] + [do]
+           for *qkv, do in (_qkv(2, 12, 2, 1300, 32), _qkv(3, 8, 4, 1111, 33))]
+
+    def run(i):
+        *qkv, do = ins[i]
+        o = kernels.window_attention(*qkv, 0.09, 300 - 100 * i, 70)
+        return [o.detach()] + list(torch.autograd.grad(o, qkv, do)) + [t.detach() for t in _chain(st)]
+
+    want = [run(0), run(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ins]
+    outs = [None, None]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i] = run(i)
+    torch.cuda.synchronize()
+    for a, b in zip(outs, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert _lib.device_error(torch.device(DEV)) == 0
+
+
 # ------------------------------------------------------------------- the model ----
 def _model(layers=2, attention="sdpa", **over):
     from auspex_soup_demo_b200 import apply, qlora
@@ -723,3 +750,28 @@ def test_model_with_sliding_window_layers_and_a_cache():
     rest = torch.cat(rest, 1).double()
     # the same model by two bf16 attention kernels through two layers
     assert float((whole - rest).norm() / whole.norm()) <= 0.02
+
+
+def test_second_derivatives_are_refused():
+    lab = torch.tensor([[1, -100, 2], [3, 4, -100]], device=DEV)
+    x = torch.randn(2, 3, device=DEV, generator=_gen(51)).requires_grad_(True)
+    h = torch.randn(2, 3, 64, device=DEV, generator=_gen(52)).bfloat16().requires_grad_(True)
+    w = torch.randn(40, 64, device=DEV, generator=_gen(53)).bfloat16()
+    q = torch.randn(1, 2, 9, 128, device=DEV, generator=_gen(54)).bfloat16().requires_grad_(True)
+    calls = [(lambda: kernels.preference_loss(x, None, lab)[0], x),
+             (lambda: kernels.policy_loss(x, torch.ones(2, device=DEV), lab)[0], x),
+             (lambda: kernels.head_token_logps(h, w, lab)[0].sum(), h),
+             (lambda: kernels.window_attention(q, q, q, 0.1, 4).float().sum(), q),
+             (lambda: kernels.swiglu_8bit(h, h).float().sum(), h)]
+    for f, leaf in calls:
+        plain = torch.autograd.grad(f(), [leaf])[0]
+        (g,) = torch.autograd.grad(f(), [leaf], create_graph=True)
+        assert torch.equal(g.detach(), plain)
+        # torch: a backward whose incoming gradient is a constant gives a constant
+        with pytest.raises(RuntimeError, match="does not require grad"):
+            torch.autograd.grad(g.float().square().sum(), [leaf])
+        factor = torch.ones((), device=DEV, requires_grad=True)
+        (g,) = torch.autograd.grad(f() * factor, [leaf], create_graph=True)
+        assert torch.equal(g.detach(), plain)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.float().square().sum().backward()
