@@ -200,8 +200,9 @@ struct FwdArgs {
 // ring of 5 x 16 KB through which K and V blocks pass (K0 V0 K1 V1 ...), barriers.
 // At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 134 us, 722 TFLOP/s of the
 // visible pairs' products; 168 us with one CTA an SM for a pair of query tiles that shares
-// the K and V blocks. Bound by the products (N = 64 ones take as long as N = 128 ones) and
-// the softmax warps' TMEM reads beside them.
+// the K and V blocks. A block takes a CTA 2080 cycles, of which the products of both CTAs
+// on the SM are 1800 (N = 64 ones take as long as N = 128 ones). Two threads a row (154 us)
+// or maxima only where a block's sum grows (137 us) are no faster.
 constexpr int kFwdWarps = 4;  // softmax warps, one row per thread
 constexpr int kFwdThreads = 64 + 32 * kFwdWarps;
 constexpr int kRing = 5;
@@ -576,10 +577,12 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
 // of N = 64 ones (75 cycles of issue either way). Shared memory: K, V (32 KB each, loaded
 // once for all query heads), two stages of (Q, dO) tiles with their nl2 / D vectors. A
 // compute thread owns 32 queries of one key row.
-// At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 238 us. Bound by the chain
-// TMEM read, exponentials, TMEM write of the compute warps, whose TMEM reads take 600 to
-// 1000 cycles while products run; exponentials by polynomial, eight compute warps and
-// P through shared memory measured no faster.
+// At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 238 us. Bound by the loop
+// dV(i), S^T(i + 1), P(i + 1): 3840 cycles a step, of which the two products take 1200, the
+// TMEM read up to 800 (beside products), the exponentials 1000 (the special-function rate
+// of 128 x 128) and handoffs the rest; dP and dS run beside it. Exponentials by polynomial,
+// eight compute warps, P through shared memory and two groups of warps on 64-query steps
+// (S^T double buffered, but products of N = 64) measured no faster.
 constexpr int kDkvStages = 2;
 struct WinDkvSmem {
   static constexpr int kK = 0;
