@@ -380,10 +380,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      bool w = true;
-      if (lane == 0)
-        w = bounded_wait(s_full(i), (i >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-      if (!(ok = warp_ok(w))) break;
+      if (!(ok = warp_wait(s_full(i), (i >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns))) break;
       tc_fence_after();
       const uint32_t s_t = s_base + (i & 1) * 64;
       float s0[32], s1[32];
@@ -420,9 +417,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
       }
       if (i > 0 && __any_sync(0xffffffffu, rescale)) {
         // O is stable once P V (i - 1) is done (S(i) came before it; P V (i - 2) before S(i))
-        if (lane == 0)
-          w = bounded_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-        if (!(ok = warp_ok(w))) break;
+        if (!(ok = warp_wait(pv_done(i - 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWinSoftmax, wait_ns))) break;
         tc_fence_after();
         rescale_o_row(o_t, alpha);
       }
@@ -786,9 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mk = queries_seeing(key, qs + cb, a.S, a.window, a.sinks);
         kind = mask_kind(mk, 0xffffffffu);
       }
-      bool w = true;
-      if (lane == 0) w = bounded_wait(s_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-      if (!(ok = warp_ok(w))) break;
+      if (!(ok = warp_wait(s_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns))) break;
       tc_fence_after();
       float p[32];
       uint32_t words[16];
@@ -820,11 +813,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(p_full);
-        w = bounded_wait(dp_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-      }
-      if (!(ok = warp_ok(w))) break;
+      if (lane == 0) mbar_arrive(p_full);
+      if (!(ok = warp_wait(dp_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns))) break;
       tc_fence_after();
       if (kind != 0) {
         float dp[32];
@@ -1202,8 +1192,7 @@ __global__ void __launch_bounds__(kDqThreads, 2)
         mk = keys_seen(q, k0 + part * 32, a.S, a.window, a.sinks);
         kind = mask_kind(mk, 0xffffffffu);
       }
-      if (lane == 0) w = bounded_wait(s_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-      if (!(ok = warp_ok(w))) break;
+      if (!(ok = warp_wait(s_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns))) break;
       tc_fence_after();
       float p[32];
       tmem_ld32_async(s_t, p);
@@ -1219,8 +1208,7 @@ __global__ void __launch_bounds__(kDqThreads, 2)
           p[e + 1] = fast_exp2(p[e + 1]);
         }
       }
-      if (lane == 0) w = bounded_wait(dp_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns);
-      if (!(ok = warp_ok(w))) break;
+      if (!(ok = warp_wait(dp_full, i & 1, abort_flag, err, kErrWinSoftmax, wait_ns))) break;
       tc_fence_after();
       float dp[32];
       tmem_ld32_async(dp_t, dp);
