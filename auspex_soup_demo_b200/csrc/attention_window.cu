@@ -89,6 +89,26 @@ __device__ __forceinline__ int mask_kind(uint32_t m, uint32_t all) {
   return __all_sync(0xffffffffu, (m & all) == all) ? 1 : 2;
 }
 
+// 2^x of a pair on the FMA pipe, for x <= 127: x = n + f with n whole and |f| <= 1/2, a cubic
+// for 2^f (relative error 7.5e-5, a fiftieth of P's rounding to bf16) and n into the exponent.
+// NaN stays NaN; below -126 the result is 2^-126.
+__device__ __forceinline__ void exp2_fma(float& x0, float& x1) {
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x0));  // -126
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x1));
+  constexpr float kMagic = 12582912.f + 127.f;  // 1.5 * 2^23: the sum's low bits are n + 127
+  const uint64_t x = f2_pack(x0, x1);
+  const uint64_t t = f2_add(x, f2_pack(kMagic, kMagic));
+  const uint64_t f = f2_fma(f2_add(t, f2_pack(-kMagic, -kMagic)), f2_pack(-1.f, -1.f), x);
+  uint64_t y = f2_fma(f, f2_pack(0.0551716648f, 0.0551716648f), f2_pack(0.242611125f, 0.242611125f));
+  y = f2_fma(f, y, f2_pack(0.693260968f, 0.693260968f));
+  y = f2_fma(f, y, f2_pack(0.999928057f, 0.999928057f));
+  float t0, t1;
+  f2_unpack(t, t0, t1);
+  const float s0 = __uint_as_float(__float_as_uint(t0) << 23);
+  const float s1 = __uint_as_float(__float_as_uint(t1) << 23);
+  f2_unpack(f2_mul(y, f2_pack(s0, s1)), x0, x1);
+}
+
 // ---- the MMA warp ----
 // The whole warp walks the schedule converged, so that waits are one instruction and
 // descriptors and addresses are uniform; each group of products and its commits runs in the
@@ -572,12 +592,13 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
 // of N = 64 ones (75 cycles of issue either way). Shared memory: K, V (32 KB each, loaded
 // once for all query heads), two stages of (Q, dO) tiles with their nl2 / D vectors. A
 // compute thread owns 32 queries of one key row.
-// At 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks: 238 us. Bound by the loop
-// dV(i), S^T(i + 1), P(i + 1): 3840 cycles a step, of which the two products take 1200, the
-// TMEM read up to 800 (beside products), the exponentials 1000 (the special-function rate
-// of 128 x 128) and handoffs the rest; dP and dS run beside it. Exponentials by polynomial,
-// eight compute warps, P through shared memory and two groups of warps on 64-query steps
-// (S^T double buffered, but products of N = 64) measured no faster.
+// Bound by the loop dV(i), S^T(i + 1), P(i + 1): about 3400 cycles a step, of which the two
+// products take 1200, the TMEM read up to 800 (beside products), the exponentials 800-1000
+// (at the special-function rate 1024 for 128 x 128) and handoffs the rest; dP and dS run
+// beside it. A quarter of the exponentials goes to the FMA pipe: forward and backward of
+// 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks take 526 us against 540 with none
+// and 532 with half. Eight compute warps, P through shared memory and two groups of warps on
+// 64-query steps (S^T double buffered, but products of N = 64) measured no faster.
 constexpr int kDkvStages = 2;
 struct WinDkvSmem {
   static constexpr int kK = 0;
@@ -798,8 +819,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float4 nl = *reinterpret_cast<const float4*>(vnl + e);
           f2_unpack(f2_fma(f2_pack(p[e], p[e + 1]), sl2, f2_pack(nl.x, nl.y)), p[e], p[e + 1]);
           f2_unpack(f2_fma(f2_pack(p[e + 2], p[e + 3]), sl2, f2_pack(nl.z, nl.w)), p[e + 2], p[e + 3]);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) p[e + v] = fast_exp2(p[e + v]);
+          if (e % 8 == 0) {
+            exp2_fma(p[e], p[e + 1]);
+          } else {
+            p[e] = fast_exp2(p[e]);
+            p[e + 1] = fast_exp2(p[e + 1]);
+          }
+          p[e + 2] = fast_exp2(p[e + 2]);
+          p[e + 3] = fast_exp2(p[e + 3]);
         }
         if (kind == 2) {  // hidden and padding rows may hold anything: select, do not scale
 #pragma unroll
