@@ -30,7 +30,7 @@ from .chunked_ce import IGNORE_INDEX, _extract_head_weight, _tma_rows_ok
 def _rows_as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """t as [rows, dim] operand rows of ``dtype`` that TMA can read."""
     t = t.detach()
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         t = t.to(dtype)
     return t if _tma_rows_ok(t) and t.stride(0) >= t.shape[1] else t.clone(
         memory_format=torch.contiguous_format)
@@ -62,15 +62,15 @@ def _block_rows(n: int, vocab: int, dim: int) -> int:
     return min(n, max(256, int(budget // (full / n)) // 256 * 256))
 
 
-def _forward(h, w, labels, ignore_index, logps, ents, state) -> None:
-    n, d = h.shape
-    v = w.shape[0]
+def _forward(h, w, labels, r0, n, ignore_index, logps, ents, state) -> None:
+    """Rows [r0, r0 + n); logps and ents: addresses of the first row's results."""
+    v, d = w.shape
     nbytes = _workspace_bytes(n, v, d, 0)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
-    _lib.call("soup_head_logps_fwd", h.device, h.data_ptr(), h.stride(0), w.data_ptr(), w.stride(0),
-              _lib.dtype_code(h.dtype), labels.data_ptr(), n, v, d, ignore_index, logps.data_ptr(),
-              _lib.ptr(ents), _lib.ptr(state), 0 if state is None else state.numel(), ws.data_ptr(),
-              nbytes, _lib.stream_of(h))
+    _lib.call("soup_head_logps_fwd", h.device, h.data_ptr() + r0 * h.stride(0) * 2, h.stride(0),
+              w.data_ptr(), w.stride(0), _lib.dtype_code(h.dtype), labels.data_ptr() + r0 * 8, n, v, d,
+              ignore_index, logps, ents, _lib.ptr(state), 0 if state is None else state.numel(),
+              ws.data_ptr(), nbytes, _lib.stream_of(h))
 
 
 def _new_state(n, v, d, device) -> torch.Tensor:
@@ -87,24 +87,23 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
         dt = _operand_dtype(hidden, weight)
         h = _rows_as(hidden.reshape(-1, d), dt)
         w = _rows_as(weight, dt)
-        t = labels.reshape(-1).to(torch.int64).contiguous()
+        t = labels if labels.dtype is torch.int64 else labels.to(torch.int64)
+        t = t.detach().contiguous()
         n = h.shape[0]
         dev = hidden.device
-        logps = torch.empty(n, dtype=torch.float32, device=dev)
-        ents = torch.empty(n, dtype=torch.float32, device=dev)
+        logps = torch.empty(*labels.shape, dtype=torch.float32, device=dev)
+        ents = torch.empty(*labels.shape, dtype=torch.float32, device=dev)
         rb = _block_rows(n, v, d)
         state = _new_state(n, v, d, dev) if keep and rb == n else None
         for r0 in range(0, n, rb):
-            r1 = min(n, r0 + rb)
-            _forward(h[r0:r1], w, t[r0:r1], ignore_index, logps[r0:r1], ents[r0:r1], state)
+            _forward(h, w, t, r0, min(rb, n - r0), ignore_index, logps.data_ptr() + 4 * r0,
+                     ents.data_ptr() + 4 * r0, state)
         if keep:
             # h is needed for the head's gradient and to run blocks again
             need_h = ctx.needs_input_grad[1] or state is None
             ctx.save_for_backward(weight, t, state, h if need_h else None)
             ctx.hidden_shape, ctx.hidden_dtype = hidden.shape, hidden.dtype
             ctx.operand_dtype, ctx.ignore_index, ctx.block = dt, ignore_index, rb
-        shape = hidden.shape[:-1]
-        logps, ents = logps.view(shape), ents.view(shape)
         ctx.mark_non_differentiable(ents)
         ctx.set_materialize_grads(False)
         return logps, ents
@@ -118,19 +117,18 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
         need_h, need_w = ctx.needs_input_grad[:2]
         dt, ignore = ctx.operand_dtype, ctx.ignore_index
         n, (v, d), dev = t.numel(), weight.shape, weight.device
-        g = dlogps.reshape(-1).to(torch.float32).contiguous()
+        g = dlogps.to(torch.float32).contiguous()
         wb = _rows_as(weight, torch.bfloat16) if need_h else None
         w = None
         dh = dw = None
         if need_h:
             out_dt = torch.bfloat16 if ctx.hidden_dtype == torch.bfloat16 else torch.float32
-            dh = torch.empty(n, d, dtype=out_dt, device=dev)
+            dh = torch.empty(*ctx.hidden_shape, dtype=out_dt, device=dev)
         if need_w:
             one = ctx.block == n and weight.dtype in (torch.bfloat16, torch.float32)
             dw = torch.empty(v, d, dtype=weight.dtype if one else torch.float32, device=dev)
         for r0 in range(0, n, ctx.block):
             r = min(n, r0 + ctx.block) - r0
-            hb = None if h is None else h[r0:r0 + r]
             st = state
             if st is None:  # more rows than the budget holds: this block's exponentials again
                 if w is None:
@@ -138,18 +136,19 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
                     st_buf = _new_state(min(n, ctx.block), v, d, dev)
                     lp = torch.empty(min(n, ctx.block), dtype=torch.float32, device=dev)
                 st = st_buf
-                _forward(hb, w, t[r0:r0 + r], ignore, lp, None, st)
+                _forward(h, w, t, r0, r, ignore, lp.data_ptr(), None, st)
             nbytes = _workspace_bytes(r, v, d, 1)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            _lib.call("soup_head_logps_bwd", dev, st.data_ptr(), st.numel(), _lib.ptr(hb),
-                      d if hb is None else hb.stride(0), _lib.dtype_code(dt), _lib.ptr(wb),
-                      d if wb is None else wb.stride(0), g[r0:].data_ptr(), r, v, d,
-                      None if dh is None else dh[r0:].data_ptr(),
+            _lib.call("soup_head_logps_bwd", dev, st.data_ptr(), st.numel(),
+                      None if h is None else h.data_ptr() + r0 * h.stride(0) * 2,
+                      d if h is None else h.stride(0), _lib.dtype_code(dt), _lib.ptr(wb),
+                      d if wb is None else wb.stride(0), g.data_ptr() + 4 * r0, r, v, d,
+                      None if dh is None else dh.data_ptr() + r0 * d * dh.element_size(),
                       _lib.F32 if dh is None else _lib.dtype_code(dh.dtype), _lib.ptr(dw),
                       _lib.F32 if dw is None else _lib.dtype_code(dw.dtype), 1 if r0 else 0,
                       ws.data_ptr(), nbytes, _lib.stream_of(weight))
         if dh is not None:
-            dh = dh.to(ctx.hidden_dtype).view(ctx.hidden_shape)
+            dh = dh.to(ctx.hidden_dtype)
         if dw is not None:
             dw = dw.to(weight.dtype)
         return dh, dw, None, None, None
