@@ -226,7 +226,7 @@ def soup_attention(module, query, key, value, attention_mask, dropout: float = 0
     in one call, since a sliding layer's cache drops the first tokens."""
     window = kwargs.get("sliding_window")
     n_q, n_k = query.shape[2], key.shape[2]
-    if (window is not None and attention_mask is None and n_q <= n_k
+    if (window and attention_mask is None and n_q <= n_k
             and (is_causal if is_causal is not None else getattr(module, "is_causal", True))):
         # transformers builds no mask for an attention function of its own registry
         # entry, so the window is this function's to apply
