@@ -42,6 +42,76 @@
 namespace soup {
 namespace attn {
 
+constexpr int kErrAttnProducer = 0x111;
+constexpr int kErrAttnMma = 0x112;
+constexpr int kErrAttnSoftmax = 0x113;
+constexpr int kErrAttnSmem = 0x114;  // dynamic shared memory too small after 1 KB alignment
+
+// 32 lanes x 32 consecutive fp32 columns from registers into TMEM (the
+// inverse of tmem_ld32); the caller waits with tmem_st_wait.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+  __syncwarp();
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+      "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+      "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])), "r"(__float_as_uint(v[8])),
+      "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
+      "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])),
+      "r"(__float_as_uint(v[15])), "r"(__float_as_uint(v[16])), "r"(__float_as_uint(v[17])),
+      "r"(__float_as_uint(v[18])), "r"(__float_as_uint(v[19])), "r"(__float_as_uint(v[20])),
+      "r"(__float_as_uint(v[21])), "r"(__float_as_uint(v[22])), "r"(__float_as_uint(v[23])),
+      "r"(__float_as_uint(v[24])), "r"(__float_as_uint(v[25])), "r"(__float_as_uint(v[26])),
+      "r"(__float_as_uint(v[27])), "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])),
+      "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
+      : "memory");
+}
+// K-major operand tile of 128 rows x 128 bf16 columns in shared memory: two
+// 16 KB boxes (columns 0-63, 64-127), rows of 128 B, 128-byte swizzle. The
+// descriptor of k-step kk (16 columns) for tcgen05.mma.
+__device__ __forceinline__ uint64_t desc_kmajor(uint32_t base, int kk) {
+  return smem_desc_sw128(base + (kk >> 2) * kBox + (kk & 3) * 32, 16, 1024);
+}
+// The same bytes read as an MN-major operand whose MN dimension is the tile's
+// 128 columns and whose K dimension is its 128 rows: k-step kk covers rows
+// [16 kk, 16 kk + 16); the two 64-column boxes are the MN atoms (LBO 16 KB).
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t base, int kk) {
+  return smem_desc_sw128(base + kk * 2048, kBox, 1024);
+}
+
+// Byte offset of the 16-byte chunk c (columns 8c..8c+7 of a 64-column box) of
+// row r in a 128-byte-swizzled box: the layout TMA writes and the descriptors read.
+__device__ __forceinline__ uint32_t swz_off(int r, int c) {
+  return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
+}
+
+// D (TMEM) [+]= A (TMEM, M rows in lanes, two bf16 of K per 32-bit column) x B (smem descriptor).
+__device__ __forceinline__ void tc_mma_bf16_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
+                                                   uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Descriptors of a 64-row step tile (two 8 KB boxes of 64 columns): as a K-major
+// operand with N = 64 rows (k-step kk: 16 columns), and as an MN-major operand
+// whose K dimension is its 64 rows (k-step kk: rows 16 kk..16 kk + 15; LBO 8 KB).
+__device__ __forceinline__ uint64_t desc_kmajor64(uint32_t base, int kk) {
+  return smem_desc_sw128(base + (kk >> 2) * kStepBox + (kk & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t desc_mnmajor64(uint32_t base, int kk) {
+  return smem_desc_sw128(base + kk * 2048, kStepBox, 1024);
+}
+// P^T / dS^T (128 rows x 64 columns, one box) as the K-major A operand.
+__device__ __forceinline__ uint64_t desc_kmajor_box(uint32_t base, int kk) {
+  return smem_desc_sw128(base + kk * 32, 16, 1024);
+}
+
 constexpr int kKStages = 2;            // forward K ring depth (a stage frees after S = Q K^T)
 constexpr int kVStages = 1;            // forward V stages (one frees after both tiles' P V)
 
@@ -462,6 +532,64 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 }
 
 // ------------------------------------------------------------ backward ----
+constexpr int kQStep = 64;                 // queries per dK / dV step
+constexpr int kPTBytes = kTile * 128;      // P^T / dS^T: 128 rows x 64 bf16 = 16 KB
+
+// D[b, h, q] = sum_d dO[b, q, h, d] * O[b, q, h, d] (fp32) and nl2[b, h, q] =
+// -lse[b, h, q] * log2(e) (the exponent offset of P in base 2); rows padded
+// like lse ([B, H, S_pad]). dO and O are [B, S, H, D] contiguous. Sixteen lanes
+// per row (16 bytes each), rows taken in the output's (b, h, q) order so the
+// stores are contiguous, four rows per half-warp with all loads issued first.
+constexpr int kDotRows = 4;
+__global__ void __launch_bounds__(256) attn_bwd_dot_kernel(const bf16* __restrict__ dO,
+                                                           const bf16* __restrict__ O,
+                                                           const float* __restrict__ lse, int B,
+                                                           int H, int S, float* __restrict__ Dv,
+                                                           float* __restrict__ nl2) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t nrows = (int64_t)B * H * S;
+  const int sub = threadIdx.x & 15;
+  const int64_t half = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+  const int64_t nhalves = ((int64_t)gridDim.x * blockDim.x) >> 4;
+  const int64_t s_pad = (int64_t)(S + kTile - 1) / kTile * kTile;
+  for (int64_t base = half * kDotRows; base < nrows; base += nhalves * kDotRows) {
+    uint4 a[kDotRows], c[kDotRows];
+#pragma unroll
+    for (int u = 0; u < kDotRows; ++u) {
+      const int64_t i = base + u;  // (b, h, q) row-major
+      if (i < nrows) {
+        const int q = (int)(i % S);
+        const int64_t bh = i / S;
+        const int h = (int)(bh % H), b = (int)(bh / H);
+        const int64_t row = ((int64_t)b * S + q) * H + h;
+        a[u] = *reinterpret_cast<const uint4*>(dO + row * kHeadDim + sub * 8);
+        c[u] = *reinterpret_cast<const uint4*>(O + row * kHeadDim + sub * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kDotRows; ++u) {
+      const int64_t i = base + u;
+      const __nv_bfloat162* ap = reinterpret_cast<const __nv_bfloat162*>(&a[u]);
+      const __nv_bfloat162* cp = reinterpret_cast<const __nv_bfloat162*>(&c[u]);
+      float acc = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = __bfloat1622float2(ap[e]), y = __bfloat1622float2(cp[e]);
+        acc = fmaf(x.x, y.x, fmaf(x.y, y.y, acc));
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+      if (sub == 0 && i < nrows) {
+        const int q = (int)(i % S);
+        const int64_t v = (i / S) * s_pad + q;
+        Dv[v] = acc;
+        nl2[v] = -lse[v] * kLog2e;
+      }
+    }
+  }
+}
+
 struct BwdArgs {
   int B, H, Hk, S;
   float scale;        // softmax scale (applied to dK, dQ in fp32)
