@@ -38,17 +38,19 @@ def _strides(t: torch.Tensor):
 
 
 def _check(q, k, v, any_stride: bool = False):
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
         raise ValueError("attention: q, k, v must be [B, heads, S, D]")
-    B, H, S, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[2] != S or k.shape[3] != D:
-        raise ValueError(f"attention: shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
-    if k.shape[1] == 0 or H % k.shape[1]:
+    B, H, S, D = qs
+    Hk = ks[1]
+    if ks != vs or ks[0] != B or ks[2] != S or ks[3] != D:
+        raise ValueError(f"attention: shapes q {tuple(qs)} k {tuple(ks)} v {tuple(vs)}")
+    if Hk == 0 or H % Hk:
         raise ValueError("attention: query heads must be a multiple of the KV heads")
     for t in (q, k, v):
-        if t.dtype != torch.bfloat16 or not t.is_cuda or (t.stride(-1) != 1 and not any_stride):
+        if t.dtype is not torch.bfloat16 or not t.is_cuda or not (any_stride or t.stride(-1) == 1):
             raise ValueError("attention: q, k, v must be bf16 CUDA tensors with a contiguous last dim")
-    return B, H, k.shape[1], S, D
+    return B, H, Hk, S, D
 
 
 def _s_pad(S: int) -> int:
@@ -166,16 +168,19 @@ class WindowAttentionFunction(torch.autograd.Function):
             dout = dout.to(torch.bfloat16).contiguous()
         if dout.data_ptr() % 16:
             dout = dout.clone()
-        dq = torch.empty(B, S, H, D, dtype=torch.bfloat16, device=q.device)
-        dk = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
-        dv = torch.empty(B, S, Hk, D, dtype=torch.bfloat16, device=q.device)
+        dev = q.device
+        # [B, heads, S, D] over [B, S, heads, D] memory
+        dq = torch.empty_strided((B, H, S, D), (S * H * D, D, H * D, 1), dtype=torch.bfloat16, device=dev)
+        kv = (S * Hk * D, D, Hk * D, 1)
+        dk = torch.empty_strided((B, Hk, S, D), kv, dtype=torch.bfloat16, device=dev)
+        dv = torch.empty_strided((B, Hk, S, D), kv, dtype=torch.bfloat16, device=dev)
         nbytes = _window_workspace_bytes(B, H, Hk, S, window, sinks)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _lib.call("soup_attention_window_bwd", q.device, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        _lib.call("soup_attention_window_bwd", dev, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(),
                   vs, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), B, H, Hk, S, D, scale, window,
                   sinks, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes,
                   _lib.stream_of(q))
-        return dq.transpose(1, 2), dk.transpose(1, 2), dv.transpose(1, 2), None, None, None
+        return dq, dk, dv, None, None, None
 
 
 def window_attention(q, k, v, scale: float, window: int, sinks: int = 0) -> torch.Tensor:
@@ -190,9 +195,9 @@ def window_attention(q, k, v, scale: float, window: int, sinks: int = 0) -> torc
     B, H, Hk, S, D = _check(q, k, v, any_stride=True)
     if D != HEAD_DIM:
         raise ValueError(f"window_attention: head dim must be {HEAD_DIM}, got {D}")
-    if k.device != q.device or v.device != q.device:
+    if not q.get_device() == k.get_device() == v.get_device():
         raise ValueError("window_attention: q, k and v must be on one device")
-    if min(B, H, Hk, S) == 0:
+    if B == 0 or H == 0 or S == 0:
         raise ValueError(f"window_attention: empty input, q {tuple(q.shape)} k {tuple(k.shape)}")
     window, sinks = int(window), int(sinks)
     if window < 1 or sinks < 0:
