@@ -190,7 +190,11 @@ def check(fn: str, status: int) -> None:
 
 def stream_of(t: torch.Tensor) -> int:
     """The raw handle of the stream torch considers current for t's device (without
-    the Stream object of torch.cuda.current_stream, which costs 3 us a call)."""
+    the Stream object of torch.cuda.current_stream, which costs 3 us a call). A tensor
+    that is not on a CUDA device is refused here: its raw handle would be the current
+    device's, and the kernel would read host memory."""
+    if not t.is_cuda:
+        raise ValueError(f"expected a CUDA tensor, got one on {t.device}")
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
