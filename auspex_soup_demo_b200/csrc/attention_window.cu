@@ -21,6 +21,9 @@
 // by selection, but 0 x NaN in a product is NaN: V must be finite there, as for any masked
 // softmax attention.
 //
+// A product that overwrites TMEM columns which an earlier product reads waits for that one's
+// commit: PTX keeps only products of one accumulator and shape in issue order. The waits cost
+// 2 % (forward and backward of 16001 tokens 540 us against 526, of 4 x 2048 190 against 186).
 // A CTA leaves only after every asynchronous arrival on its barriers has landed: the
 // producer waits for its copies, the MMA warp for its commits.
 // Every mbarrier wait is bounded as in attention.cu: on expiry the role records a
@@ -328,8 +331,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     }
   } else if (warp == 1) {
     // --------------------------------------------------- MMA issuer ----
-    // S of blocks 0 and 1, then per block i: P V (i), S(i + 2) into the buffer that this
-    // product has read P from (MMAs run in issue order).
+    // S of blocks 0 and 1, then per block i: P V (i) and, once it is done, S(i + 2) into the
+    // buffer that it has read P from.
     auto wait = [&](uint32_t bar, int parity) {
       return warp_wait(bar, parity, abort_flag, err, kErrWinMma, wait_ns);
     };
@@ -377,7 +380,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2)
     if (ok && n > 1) ok = issue_s(1);
     for (int i = 0; i < n && ok; ++i) {
       ok = issue_pv(i);
-      if (ok && i + 2 < n) ok = issue_s(i + 2);
+      if (ok && i + 2 < n) ok = wait(pv_done(i), (i >> 1) & 1) && issue_s(i + 2);
     }
     // the ring's last arrivals (nothing else waits for them)
     for (int i = 2 * n > kRing ? 2 * n - kRing : 0; i < 2 * n && ok; ++i)
@@ -597,7 +600,7 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
 // (at the special-function rate 1024 for 128 x 128) and handoffs the rest; dP and dS run
 // beside it. A quarter of the exponentials goes to the FMA pipe: forward and backward of
 // 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks take 526 us against 540 with none
-// and 532 with half. Eight compute warps, P through shared memory and two groups of warps on
+// and 532 with half (540 with the waits between products, which came later). Eight compute warps, P through shared memory and two groups of warps on
 // 64-query steps (S^T double buffered, but products of N = 64) measured no faster.
 constexpr int kDkvStages = 2;
 struct WinDkvSmem {
@@ -606,8 +609,8 @@ struct WinDkvSmem {
   static constexpr int kQD = kV + kTileBytes;  // stage s: Q at +0, dO at +kTileBytes
   static constexpr int kVec = kQD + kDkvStages * 2 * kTileBytes;  // stage s: nl2, D (2 x 512 B)
   static constexpr int kBar = kVec + kDkvStages * 2 * kTile * 4;
-  // kv_full, full[2], empty[2], s_full, p_full, dp_full, ds_full, acc_done, drain
-  static constexpr int kNumBars = 1 + 2 * kDkvStages + 6;
+  // kv_full, full[2], empty[2], s_full, p_full, dp_full, ds_full, acc_done, dv_done, drain
+  static constexpr int kNumBars = 1 + 2 * kDkvStages + 7;
   static constexpr int kMisc = kBar + kNumBars * 8;
   static constexpr int kUsed = kMisc + 16;
   static constexpr int kBytes = kUsed + 1024 <= 232448 ? kUsed + 1024 : 232448;
@@ -637,7 +640,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kB = 1 + 2 * kDkvStages;
   const uint32_t s_full = bar0 + 8u * kB, p_full = bar0 + 8u * (kB + 1);
   const uint32_t dp_full = bar0 + 8u * (kB + 2), ds_full = bar0 + 8u * (kB + 3);
-  const uint32_t acc_done = bar0 + 8u * (kB + 4), drain_bar = bar0 + 8u * (kB + 5);
+  const uint32_t acc_done = bar0 + 8u * (kB + 4), dv_done = bar0 + 8u * (kB + 5);
+  const uint32_t drain_bar = bar0 + 8u * (kB + 6);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
 
@@ -757,13 +761,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     if (ok) ok = issue_s(0, 0);
     if (ok) ok = issue_s(1, 0);
+    // S^T and dP^T of a step overwrite the P^T and dS^T that dV and dK of the step before
+    // read: each follows its commit
     for (int i = 0; i < total && ok; ++i) {
+      const bool more = i + 1 < total;
       ok = issue_acc(0, i);
-      if (ok && i + 1 < total) ok = issue_s(0, i + 1);
+      if (ok && more) {
+        if (elect_one()) tc_commit(dv_done);
+        __syncwarp();
+        ok = wait(dv_done, i & 1) && issue_s(0, i + 1);
+      }
       if (ok) ok = issue_acc(1, i);
       if (ok && elect_one()) tc_commit(empty(i % kDkvStages));
       __syncwarp();
-      if (ok && i + 1 < total) ok = issue_s(1, i + 1);
+      if (ok && more) ok = wait(empty(i % kDkvStages), (i / kDkvStages) & 1) && issue_s(1, i + 1);
     }
     if (ok && elect_one()) tc_commit(acc_done);
     __syncwarp();
@@ -1143,7 +1154,8 @@ __global__ void __launch_bounds__(kDqThreads, 2)
         if (i + 1 == n) tc_commit(acc_done);
       }
       __syncwarp();
-      if (i + 1 < n) ok = issue_dp(i + 1);
+      // dP(i + 1) overwrites the dS that dQ has read
+      if (i + 1 < n) ok = wait(k_empty(i), (i >> 1) & 1) && issue_dp(i + 1);
     }
     // the last arrivals of the rings
     for (int i = n > 2 ? n - 2 : 0; i < n && ok; ++i) ok = wait(k_empty(i), (i >> 1) & 1);
