@@ -280,6 +280,15 @@ def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and 16-byte aligned, copied only if it is not. For tensors that a
+    forward saved in that form: a saved-tensor hook (activation offloading) may hand
+    back the same values in another layout."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return t.detach().clone(memory_format=torch.contiguous_format)
+
+
 def i64_array(values):
     return (ctypes.c_int64 * len(values))(*values)
 

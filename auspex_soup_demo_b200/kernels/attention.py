@@ -134,6 +134,13 @@ def _kernel_layout(t: torch.Tensor):
     return t, (_lib.c_i64 * 3)(sb, sh, ss)
 
 
+def _restored(t: torch.Tensor, saved):
+    """:func:`_kernel_layout` of a saved tensor. ``saved`` holds its (strides, kernel
+    strides) in the forward: a saved-tensor hook may hand it back in another layout."""
+    stride, kernel = saved
+    return (t, kernel) if t.stride() == stride and t.data_ptr() % 16 == 0 else _kernel_layout(t)
+
+
 @functools.lru_cache(maxsize=256)
 def _window_workspace_bytes(*sizes: int) -> int:
     return _lib.lib().soup_attention_window_bwd_workspace_bytes(*sizes)
@@ -154,16 +161,18 @@ class WindowAttentionFunction(torch.autograd.Function):
                   vs, B, H, Hk, S, D, scale, window, sinks, out.data_ptr(), lse.data_ptr(),
                   _lib.stream_of(q))
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.args = (qs, ks, vs, scale, window, sinks)
+        ctx.args = ((q.stride(), qs), (k.stride(), ks), (v.stride(), vs), scale, window, sinks)
         return out
 
     @staticmethod
     @_lib.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        qs, ks, vs, scale, window, sinks = ctx.args
+        ql, kl, vl, scale, window, sinks = ctx.args
         B, H, S, D = q.shape
         Hk = k.shape[1]
+        (q, qs), (k, ks), (v, vs) = _restored(q, ql), _restored(k, kl), _restored(v, vl)
+        out, lse = _lib.dense(out), _lib.dense(lse)
         if dout.dtype is not torch.bfloat16 or not dout.is_contiguous():
             dout = dout.to(torch.bfloat16).contiguous()
         if dout.data_ptr() % 16:

@@ -1,0 +1,57 @@
+"""The preference / policy tuning operators in calls that a training program makes around
+them: offloaded activations, far references, caches, short batches.
+
+Where two calls have to agree bit for bit, the kernels sum in a fixed order and the
+inputs are the same; other tolerances are derived at their test.
+"""
+
+import pytest
+import torch
+
+from auspex_soup_demo_b200 import _lib, kernels
+
+pytestmark = pytest.mark.gpu
+
+IGNORE = -100
+DEV = "cuda"
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+# ----------------------------------------------------------- saved-tensor hooks ----
+def _offload(pin):
+    return torch.autograd.graph.save_on_cpu(pin_memory=pin)
+
+
+def _same_under_offload(call, leaves):
+    """Outputs and gradients of ``call`` under save_on_cpu equal those without."""
+    def run():
+        out = call()
+        out = out if isinstance(out, tuple) else (out,)
+        dout = torch.randn(out[0].shape, generator=_gen(99), device=DEV).to(out[0].dtype)
+        return [t.detach().clone() for t in out], dout, out[0]
+
+    want, dout, first = run()
+    want += torch.autograd.grad(first, leaves, dout)
+    for pin in (True, False):
+        with _offload(pin):
+            got, dout, first = run()
+            got += torch.autograd.grad(first, leaves, dout)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), pin
+    assert _lib.device_error(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("source", ["transposed", "fused projection"])
+def test_window_attention_under_offload(source):
+    B, H, Hk, S, D = 2, 4, 2, 200, 128
+    if source == "transposed":
+        q, k, v = (torch.randn(B, S, h, D, generator=_gen(h), device=DEV).bfloat16().transpose(1, 2)
+                   for h in (H, Hk, Hk))
+    else:
+        big = torch.randn(B, S, (H + 2 * Hk) * D, generator=_gen(1), device=DEV).bfloat16()
+        q, k, v = (big[..., a * D:(a + h) * D].view(B, S, h, D).transpose(1, 2)
+                   for a, h in ((0, H), (H, Hk), (H + Hk, Hk)))
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    _same_under_offload(lambda: kernels.window_attention(q, k, v, 0.1, 50, 4), [q, k, v])

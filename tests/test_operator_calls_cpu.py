@@ -16,3 +16,69 @@ from auspex_soup_demo_b200 import _lib, kernels
 def test_host_tensors_are_refused_before_a_launch(call):
     with pytest.raises(ValueError, match="expected a CUDA tensor"):
         call(torch.zeros(4, 8))
+
+
+# ------------------------------------------------- saved tensors in other layouts ----
+def _relaid(t, layout):
+    """The values of t as a saved-tensor hook may hand them back."""
+    if layout == "contiguous":  # torch.autograd.graph.save_on_cpu
+        return t.detach().clone(memory_format=torch.contiguous_format)
+    if layout == "gaps":
+        wide = t.new_empty(*t.shape[:-1], t.shape[-1] + 64)
+        wide[..., :t.shape[-1]] = t.detach()
+        return wide[..., :t.shape[-1]]
+    flat = t.new_empty(t.numel() + 1)  # one element off
+    flat[1:] = t.detach().reshape(-1)
+    return flat[1:].view(t.shape)
+
+
+class _Calls:
+    """Records the library calls of host tensors instead of making them, and hands saved
+    tensors back in another layout."""
+
+    def __init__(self, monkeypatch, layout):
+        self.calls, self.back, self.layout = {}, [], layout
+        monkeypatch.setattr(_lib, "call", lambda fn, dev, *args: self.calls.__setitem__(fn, args))
+        monkeypatch.setattr(_lib, "stream_of", lambda t: 0)
+
+    def hooks(self):
+        def unpack(t):
+            self.back.append(_relaid(t, self.layout))
+            return self.back[-1]
+
+        return torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack)
+
+
+LAYOUTS = ["contiguous", "gaps", "odd"]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("source", ["transposed", "fused projection"])
+def test_window_backward_reads_what_came_back(monkeypatch, layout, source):
+    from auspex_soup_demo_b200.kernels import attention
+
+    rec = _Calls(monkeypatch, layout)
+    monkeypatch.setattr(attention, "_window_workspace_bytes", lambda *sizes: 256)
+    B, H, Hk, S, D = 2, 4, 2, 200, 128
+    if source == "transposed":
+        q, k, v = (torch.randn(B, S, h, D).bfloat16().transpose(1, 2) for h in (H, Hk, Hk))
+    else:
+        big = torch.randn(B, S, (H + 2 * Hk) * D).bfloat16()
+        q, k, v = (big[..., a * D:(a + h) * D].view(B, S, h, D).transpose(1, 2)
+                   for a, h in ((0, H), (H, Hk), (H + Hk, Hk)))
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    with rec.hooks():
+        out = attention.WindowAttentionFunction.apply(q, k, v, 0.1, 50, 4)
+    out.backward(torch.zeros_like(out))
+    fwd, bwd = rec.calls["soup_attention_window_fwd"], rec.calls["soup_attention_window_bwd"]
+    for i, t in enumerate((q, k, v)):
+        assert fwd[2 * i] == t.data_ptr() and list(fwd[2 * i + 1]) == list(t.stride()[:3])
+        got = rec.back[i]
+        strides = list(bwd[2 * i + 1])
+        if layout == "odd":  # not readable in place
+            assert bwd[2 * i] != got.data_ptr() and bwd[2 * i] % 16 == 0
+            assert strides == [t.shape[1] * S * D, S * D, D]
+        else:
+            assert bwd[2 * i] == got.data_ptr() and strides == list(got.stride()[:3])
+    for i, got in ((6, rec.back[3]), (8, rec.back[4])):  # out, log-sum-exp: contiguous
+        assert bwd[i] % 16 == 0 and (bwd[i] == got.data_ptr()) == (layout == "contiguous")
