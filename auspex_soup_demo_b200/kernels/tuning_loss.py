@@ -99,7 +99,7 @@ class PreferenceLossFunction(torch.autograd.Function):
                   loss.data_ptr(), chosen.data_ptr(), coef, ws.data_ptr(), nbytes,
                   _lib.stream_of(logps))
         ctx.save_for_backward(ws, lab)
-        ctx.args = (nbytes, n, s, lab_ld, ignore_index)
+        ctx.args = (nbytes, n, s, ignore_index)
         ctx.mark_non_differentiable(chosen, rejected)
         ctx.set_materialize_grads(False)
         return loss, chosen, rejected
@@ -110,7 +110,9 @@ class PreferenceLossFunction(torch.autograd.Function):
         if grad is None:
             return (None,) * 7
         ws, lab = ctx.saved_tensors
-        off, n, s, lab_ld, ignore_index = ctx.args
+        off, n, s, ignore_index = ctx.args
+        # a saved-tensor hook may hand both back in another layout
+        ws, (lab, lab_ld) = _lib.dense(ws), _rows(lab)
         out = torch.empty(n, s, dtype=torch.float32, device=ws.device)
         grad = grad.to(torch.float32)
         _lib.call("soup_preference_loss_bwd", ws.device, grad.data_ptr(), ws.data_ptr() + off,
@@ -189,7 +191,7 @@ class PolicyLossFunction(torch.autograd.Function):
     def backward(ctx, grad, _k, _c):
         if grad is None:
             return (None,) * 11
-        (ws,) = ctx.saved_tensors
+        ws = _lib.dense(ctx.saved_tensors[0])
         off, b, s = ctx.args
         out = torch.empty(b, s, dtype=torch.float32, device=ws.device)
         grad = grad.to(torch.float32)

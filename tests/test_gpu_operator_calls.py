@@ -55,3 +55,26 @@ def test_window_attention_under_offload(source):
                    for a, h in ((0, H), (H, Hk), (H + Hk, Hk)))
     q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
     _same_under_offload(lambda: kernels.window_attention(q, k, v, 0.1, 50, 4), [q, k, v])
+
+
+def _logp_batch(n, s, seed):
+    """logps [n, s], and labels as a slice of a wider tensor."""
+    g = _gen(seed)
+    ids = torch.randint(0, 1000, (n, s + 1), generator=g, device=DEV)
+    ids = torch.where(torch.rand(n, s + 1, generator=g, device=DEV) < 0.6, ids, torch.full_like(ids, IGNORE))
+    x = -torch.rand(n, s, generator=g, device=DEV) * 3
+    return x.requires_grad_(True), ids[:, 1:], g
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "ipo"])
+def test_preference_loss_under_offload(kind):
+    x, lab, g = _logp_batch(6, 33, 2)
+    ref = x.detach() + 0.1
+    _same_under_offload(lambda: kernels.preference_loss(x, ref, lab, loss_type=kind), [x])
+
+
+def test_policy_loss_under_offload():
+    x, lab, g = _logp_batch(5, 33, 3)
+    adv = torch.randn(5, 66, generator=g, device=DEV)[:, ::2]
+    old = x.detach() + 0.1
+    _same_under_offload(lambda: kernels.policy_loss(x, adv, lab, old, old, kl_coef=0.1), [x])

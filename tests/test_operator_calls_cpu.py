@@ -23,6 +23,9 @@ def _relaid(t, layout):
     """The values of t as a saved-tensor hook may hand them back."""
     if layout == "contiguous":  # torch.autograd.graph.save_on_cpu
         return t.detach().clone(memory_format=torch.contiguous_format)
+    if layout == "gaps" and t.dim() == 1:
+        wide = t.new_empty(2 * t.numel())[::2]
+        return wide.copy_(t.detach())
     if layout == "gaps":
         wide = t.new_empty(*t.shape[:-1], t.shape[-1] + 64)
         wide[..., :t.shape[-1]] = t.detach()
@@ -82,3 +85,34 @@ def test_window_backward_reads_what_came_back(monkeypatch, layout, source):
             assert bwd[2 * i] == got.data_ptr() and strides == list(got.stride()[:3])
     for i, got in ((6, rec.back[3]), (8, rec.back[4])):  # out, log-sum-exp: contiguous
         assert bwd[i] % 16 == 0 and (bwd[i] == got.data_ptr()) == (layout == "contiguous")
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_preference_backward_reads_what_came_back(monkeypatch, layout):
+    rec = _Calls(monkeypatch, layout)
+    x = torch.randn(4, 8).requires_grad_(True)
+    labels = torch.arange(36).view(4, 9)[:, 1:]
+    with rec.hooks():
+        loss, _, _ = kernels.tuning_loss.PreferenceLossFunction.apply(x, None, labels, 0.1, 0.0, 0, -100)
+    loss.backward(torch.ones(()))
+    fwd, bwd = rec.calls["soup_preference_loss_fwd"], rec.calls["soup_preference_loss_bwd"]
+    assert (fwd[5], fwd[6]) == (labels.data_ptr(), 9)
+    ws, lab = rec.back
+    # rows are read where they are (an int64 pointer is aligned to its element)
+    assert (bwd[2], bwd[3]) == (lab.data_ptr(), {"contiguous": 8, "gaps": 8 + 64, "odd": 8}[layout])
+    off = fwd[15] - fwd[16]  # the coefficients, behind the workspace
+    assert (bwd[1] - off) % 16 == 0 and (bwd[1] == ws.data_ptr() + off) == (layout == "contiguous")
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_policy_backward_reads_what_came_back(monkeypatch, layout):
+    rec = _Calls(monkeypatch, layout)
+    x = torch.randn(4, 8).requires_grad_(True)
+    with rec.hooks():
+        loss, _, _ = kernels.tuning_loss.PolicyLossFunction.apply(
+            x, torch.randn(4), torch.arange(36).view(4, 9)[:, 1:], None, None, 0.2, 0.2, 0.0, 0, -100, True)
+    loss.backward(torch.ones(()))
+    fwd, bwd = rec.calls["soup_policy_loss_fwd"], rec.calls["soup_policy_loss_bwd"]
+    (ws,), off = rec.back, fwd[20] - fwd[22]
+    assert bwd[2] - bwd[1] == fwd[21] - fwd[20] == 16
+    assert (bwd[1] - off) % 16 == 0 and (bwd[1] == ws.data_ptr() + off) == (layout == "contiguous")
