@@ -141,7 +141,8 @@ class SwiGLU8BitFunction(torch.autograd.Function):
     @staticmethod
     @_lib.once_differentiable
     def backward(ctx, dy: torch.Tensor):
-        (kept,) = ctx.saved_tensors
+        # scales and codes are read by address: as they were, whatever a saved-tensor hook returns
+        kept = _lib.dense(ctx.saved_tensors[0])
         rows, n, blocks, c0, c1, dt, dtype = ctx.args
         dy2 = _rows_8bit(dy if dy.dtype is dtype else dy.to(dtype), n)
         dg = torch.empty(*dy.shape, dtype=dtype, device=dy.device)

@@ -116,6 +116,10 @@ class HeadTokenLogpsFunction(torch.autograd.Function):
         weight, t, state, h = ctx.saved_tensors
         need_h, need_w = ctx.needs_input_grad[:2]
         dt, ignore = ctx.operand_dtype, ctx.ignore_index
+        # a saved-tensor hook may hand them back in another layout (the weight's rows: below)
+        t = _lib.dense(t)
+        state = None if state is None else _lib.dense(state)
+        h = None if h is None else _rows_as(h, dt)
         n, (v, d), dev = t.numel(), weight.shape, weight.device
         g = dlogps.to(torch.float32).contiguous()
         wb = _rows_as(weight, torch.bfloat16) if need_h else None

@@ -965,7 +965,7 @@ class _LoRAMLPFn(torch.autograd.Function):
         else:
             dxa_d, dxa_dT = d2 @ b16_d, None
         if ctx.keep8:
-            codes, scales = y, h  # of [g | u] as [rows * blocks, 2 * IL_BLOCK]
+            codes, scales = _lib.dense(y), _lib.dense(h)  # of [g | u] as [rows * blocks, 2 * IL_BLOCK]
             m, inter = d2.shape[0], group.outs[0]
             dh = torch.empty(m, inter, device=d2.device, dtype=d2.dtype)
             if _fused_ok(d2.shape[1], d2, w_d, dxa_d, as16_d, n=inter):

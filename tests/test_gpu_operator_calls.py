@@ -78,3 +78,49 @@ def test_policy_loss_under_offload():
     adv = torch.randn(5, 66, generator=g, device=DEV)[:, ::2]
     old = x.detach() + 0.1
     _same_under_offload(lambda: kernels.policy_loss(x, adv, lab, old, old, kl_coef=0.1), [x])
+
+
+@pytest.mark.parametrize("budget", [None, 1 << 20], ids=["one block", "blocks"])
+def test_head_token_logps_under_offload(monkeypatch, budget):
+    from auspex_soup_demo_b200.kernels import chunked_ce
+
+    if budget:
+        monkeypatch.setattr(chunked_ce, "CE_WORKSPACE_BYTES", budget)
+    g = _gen(4)
+    h = torch.randn(10, 70, 128, generator=g, device=DEV).bfloat16()[..., :64].requires_grad_(True)
+    w = (torch.randn(900, 64, generator=g, device=DEV) * 0.1).bfloat16().requires_grad_(True)
+    lab = torch.randint(0, 900, (10, 71), generator=g, device=DEV)[:, 1:]
+    _same_under_offload(lambda: kernels.head_token_logps(h, w, lab), [h, w])
+
+
+def test_swiglu_8bit_under_offload():
+    both = torch.randn(40, 400, generator=_gen(5), device=DEV).bfloat16()
+    gate, up = (both[:, i * 200:(i + 1) * 200].requires_grad_(True) for i in (0, 1))
+    _same_under_offload(lambda: kernels.swiglu_8bit(gate, up), [gate, up])
+
+
+def test_mlp_kept_in_8_bits_under_offload():
+    """The QLoRA step's MLP: the codes and scales of [gate | up] come back from the host."""
+    from auspex_soup_demo_b200 import apply, qlora
+    from auspex_soup_demo_b200.kernels import swiglu
+
+    apply()
+    cfg = qlora.qwen2_1p5b_config(1, hidden_size=256, intermediate_size=512, num_attention_heads=2,
+                                  num_key_value_heads=1, vocab_size=500)
+    tr = qlora.QLoRATrainer(qlora.build_qwen2_qlora(cfg, seed=1), lr=0.0)
+    with torch.no_grad():
+        for n, p in tr.model.named_parameters():
+            if "lora_B" in n:
+                p.copy_(torch.randn(p.shape, generator=_gen(6), device=DEV) * 0.05)
+    ids = torch.randint(0, 500, (2, 128), generator=_gen(7), device=DEV)
+    lab = qlora.causal_labels(ids)
+    old = swiglu.CHECKPOINT_8BIT
+    try:
+        swiglu.CHECKPOINT_8BIT = True
+        tr.step(ids, lab, 254.0)
+        want = tr.flat_grad.clone()
+        with _offload(True):
+            tr.step(ids, lab, 254.0)
+    finally:
+        swiglu.CHECKPOINT_8BIT = old
+    assert float(want.abs().max()) > 0 and torch.equal(tr.flat_grad, want)

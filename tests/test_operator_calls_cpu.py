@@ -116,3 +116,52 @@ def test_policy_backward_reads_what_came_back(monkeypatch, layout):
     (ws,), off = rec.back, fwd[20] - fwd[22]
     assert bwd[2] - bwd[1] == fwd[21] - fwd[20] == 16
     assert (bwd[1] - off) % 16 == 0 and (bwd[1] == ws.data_ptr() + off) == (layout == "contiguous")
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_swiglu_8bit_backward_reads_what_came_back(monkeypatch, layout):
+    from auspex_soup_demo_b200.kernels import swiglu
+
+    rec = _Calls(monkeypatch, layout)
+    g, u = (torch.randn(3, 70).requires_grad_(True) for _ in range(2))
+    with rec.hooks():
+        h = swiglu.SwiGLU8BitFunction.apply(g, u)
+    h.backward(torch.zeros_like(h))
+    fwd, bwd = rec.calls["soup_swiglu_q8_fwd"], rec.calls["soup_swiglu_q8_bwd"]
+    codes, scales = (bwd[2], bwd[3]), (bwd[5], bwd[6])
+    base = scales[0]
+    assert base % 16 == 0 and (base == rec.back[0].data_ptr()) == (layout == "contiguous")
+    assert [p - base for p in codes + scales] == [p - fwd[9] for p in fwd[6:8] + fwd[9:11]]
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("blocks", [False, True])
+def test_token_logps_backward_reads_what_came_back(monkeypatch, layout, blocks):
+    from auspex_soup_demo_b200.kernels import chunked_ce, token_logps
+
+    rec = _Calls(monkeypatch, layout)
+    monkeypatch.setattr(token_logps, "_state_bytes", lambda n, v, d: 512 * n)
+    monkeypatch.setattr(token_logps, "_workspace_bytes", lambda n, v, d, b: 512 * n)
+    if blocks:
+        monkeypatch.setattr(chunked_ce, "CE_WORKSPACE_BYTES", 1)
+    hidden = torch.randn(300, 64).bfloat16().requires_grad_(True)
+    weight = torch.randn(70, 64).bfloat16().requires_grad_(True)
+    labels = torch.randint(0, 70, (300,))
+    with rec.hooks():
+        logps, _ = token_logps.HeadTokenLogpsFunction.apply(hidden, weight, labels, -100, True)
+    rec.calls.clear()
+    logps.backward(torch.zeros_like(logps))
+    bwd = rec.calls["soup_head_logps_bwd"]
+    back_w, back_t, *back = rec.back
+    state, h = (None, back[0]) if blocks else back
+    same = layout == "contiguous"
+    inplace = layout != "odd"  # rows with gaps are read where they are
+    last = 256 * 64 * 2 if blocks else 0  # the last block starts at row 256
+    gap = 128 if layout == "gaps" else 64
+    assert (bwd[2] - (last * gap // 64) == h.data_ptr()) == inplace and bwd[2] % 16 == 0
+    assert bwd[3] == gap and bwd[6] == gap and (bwd[5] == back_w.data_ptr()) == inplace
+    if blocks:
+        again = rec.calls["soup_head_logps_fwd"]
+        assert again[1] == again[3] == gap and (again[5] - 256 * 8 == back_t.data_ptr()) == same
+    else:
+        assert bwd[0] % 16 == 0 and (bwd[0] == state.data_ptr()) == same
