@@ -304,8 +304,10 @@ __device__ __forceinline__ void policy_sum(const PolicyArgs& a, int chunks, doub
           const float em = expm1f(d);
           const float k = em - d;
           kl += (double)k;
-          l += a.kl_coef * k;
-          g -= a.kl_coef * em;
+          if (a.kl_coef != 0.f) {  // without a coefficient the term is the metric's alone: 0 x inf is NaN
+            l += a.kl_coef * k;
+            g -= a.kl_coef * em;
+          }
         }
         loss += (double)l;
         clipped += cut ? 1 : 0;

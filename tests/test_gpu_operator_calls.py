@@ -124,3 +124,22 @@ def test_mlp_kept_in_8_bits_under_offload():
     finally:
         swiglu.CHECKPOINT_8BIT = old
     assert float(want.abs().max()) > 0 and torch.equal(tr.flat_grad, want)
+
+
+# ------------------------------------------------------------------ policy loss ----
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_policy_loss_reference_for_the_metric_alone(reduction):
+    """kl_coef = 0: the reference enters mean_kl and nothing else, however far it is."""
+    x, lab, g = _logp_batch(6, 300, 8)
+    adv = torch.randn(6, generator=g, device=DEV)
+    old = x.detach() + 0.1
+
+    def run(ref):
+        loss, kl, cut = kernels.policy_loss(x, adv, lab, old, ref, kl_coef=0.0, reduction=reduction)
+        return loss.detach(), kl, cut, torch.autograd.grad(loss, [x])[0]
+
+    loss, _, cut, dx = run(None)
+    for shift, finite in ((100.0, False), (-100.0, True), (0.5, True), (float("nan"), False)):
+        got = run(x.detach() + shift)
+        assert torch.equal(got[0], loss) and torch.equal(got[2], cut) and torch.equal(got[3], dx), shift
+        assert bool(torch.isfinite(got[1])) == finite
