@@ -294,8 +294,9 @@ __device__ __forceinline__ void policy_sum(const PolicyArgs& a, int chunks, doub
       float g = 0.f;
       if (t[u] != a.ignore) {
         const float A = ad[u];
-        const double delta = od ? (double)x[u] - (double)o[u] : 0.0;
-        const float ratio = od ? expf((float)delta) : 1.f;
+        // without old_logps x - x: 0, or NaN for a log-probability that is none
+        const double delta = (double)x[u] - (double)o[u];
+        const float ratio = od ? expf((float)delta) : 1.f + (float)delta;
         const bool cut = (A > 0.f && delta > a.log_hi) || (A < 0.f && delta < a.log_lo);
         float l = cut ? -(A > 0.f ? a.hi : a.lo) * A : -ratio * A;
         g = cut ? 0.f : -A * ratio;

@@ -219,7 +219,8 @@ def policy_loss(logps: torch.Tensor, advantages: torch.Tensor, labels: torch.Ten
     (no KL term without ref_logps). ``reduction="token"`` is the mean over all
     labelled tokens, ``"sequence"`` the mean over the batch of each sequence's
     mean (0 for a sequence without labelled tokens). mean_kl (of e^d - d - 1) and
-    clipped_share are detached means over the labelled tokens.
+    clipped_share are detached means over the labelled tokens. A labelled token's NaN
+    log-probability (a label outside the vocabulary has one) makes the loss NaN.
     """
     fn = "policy_loss"
     _check(fn, logps, labels)

@@ -143,3 +143,36 @@ def test_policy_loss_reference_for_the_metric_alone(reduction):
         got = run(x.detach() + shift)
         assert torch.equal(got[0], loss) and torch.equal(got[2], cut) and torch.equal(got[3], dx), shift
         assert bool(torch.isfinite(got[1])) == finite
+
+
+@pytest.mark.parametrize("ref", [False, True])
+@pytest.mark.parametrize("bad,old", [
+    ("nan", False), ("nan", True), ("inf", False), ("-inf", False),  # with old_logps a ratio of inf or 0
+])
+def test_policy_loss_keeps_a_broken_log_probability_visible(bad, old, ref):
+    x, lab, g = _logp_batch(4, 70, 9)
+    o = x.detach() - 0.05 if old else None
+    r = x.detach() + 0.05 if ref else None
+    lab = lab.clone()
+    lab[2, 5], lab[1, 3] = 7, IGNORE
+    with torch.no_grad():
+        x[2, 5] = float(bad)
+        x[1, 3] = float("nan")  # unlabelled: not used
+    for adv in (torch.ones(4, device=DEV), -torch.ones(4, device=DEV)):
+        loss, _, _ = kernels.policy_loss(x, adv, lab, o, r, kl_coef=0.1 if ref else 0.0)
+        (dx,) = torch.autograd.grad(loss, [x])
+        assert torch.isnan(loss)
+        nan = torch.isnan(dx)
+        assert bool(nan[2, 5]) and int(nan.sum()) == 1
+
+
+def test_policy_loss_of_a_label_outside_the_vocabulary():
+    g = _gen(10)
+    h = torch.randn(2, 30, 64, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    w = (torch.randn(200, 64, generator=g, device=DEV) * 0.1).bfloat16()
+    lab = torch.randint(0, 200, (2, 30), generator=g, device=DEV)
+    lab[1, 4] = 200
+    logps, _ = kernels.head_token_logps(h, w, lab)
+    loss, _, _ = kernels.policy_loss(logps, torch.ones(2, device=DEV), lab)
+    (dh,) = torch.autograd.grad(loss, [h])
+    assert torch.isnan(loss) and torch.isnan(dh[1, 4]).all() and int(torch.isnan(dh).any(-1).sum()) == 1
