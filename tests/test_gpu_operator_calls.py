@@ -176,3 +176,25 @@ def test_policy_loss_of_a_label_outside_the_vocabulary():
     loss, _, _ = kernels.policy_loss(logps, torch.ones(2, device=DEV), lab)
     (dh,) = torch.autograd.grad(loss, [h])
     assert torch.isnan(loss) and torch.isnan(dh[1, 4]).all() and int(torch.isnan(dh).any(-1).sum()) == 1
+
+
+@pytest.mark.parametrize("size", [1e-5, 1e-4, 1e-3, 1e-2, 0.1, 0.45, 0.55, 1.0, 3.0])
+@pytest.mark.parametrize("n", [(1, 1), (7, 100)])
+def test_policy_loss_kl_near_the_reference(size, n):
+    """The KL estimate keeps its digits for a policy that has hardly left its reference.
+
+    d = ref - logps is rounded to fp32 (2^-24, twice that in d^2), the estimate takes a
+    few more roundings; from |d| = 0.5 on expm1(d) - d loses a factor of up to 5 of
+    expm1's 2^-23, below that nothing cancels. Every term is positive, so the bound of a
+    term, 2^-20 of it, is that of the mean."""
+    g = _gen(11)
+    x = -1 - torch.rand(*n, generator=g, device=DEV)
+    d = size * (0.9 + 0.2 * torch.rand(*n, generator=g, device=DEV))
+    ref = x + torch.where(torch.rand(*n, generator=g, device=DEV) < 0.5, d, -d)
+    lab = torch.zeros(*n, dtype=torch.int64, device=DEV)
+    _, kl, _ = kernels.policy_loss(x, torch.ones(n[0], device=DEV), lab, None, ref, kl_coef=0.1)
+    d = ref.double() - x.double()
+    # in 64 bits the first terms of the series, whose cancellation expm1 would leave at small d
+    small = d * d * (0.5 + d * (1 / 6 + d * (1 / 24 + d * (1 / 120 + d / 720))))
+    want = torch.where(d.abs() < 0.02, small, torch.expm1(d) - d).mean()
+    assert abs(float(kl) - float(want)) <= 2.0 ** -20 * float(want)
