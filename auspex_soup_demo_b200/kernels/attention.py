@@ -240,22 +240,26 @@ def soup_attention(module, query, key, value, attention_mask, dropout: float = 0
     in one call, since a sliding layer's cache drops the first tokens."""
     window = kwargs.get("sliding_window")
     n_q, n_k = query.shape[2], key.shape[2]
-    if (window and attention_mask is None and n_q <= n_k
+    if (attention_mask is None and n_q <= n_k
             and (is_causal if is_causal is not None else getattr(module, "is_causal", True))):
-        # transformers builds no mask for an attention function of its own registry
-        # entry, so the window is this function's to apply
-        sinks = int(getattr(getattr(module, "config", None), "attention_sink_tokens", 0) or 0)
+        # no mask came with the call, so causality and the window are this function's to apply
+        sinks = int(getattr(getattr(module, "config", None), "attention_sink_tokens", 0) or 0) if window else 0
         if sinks and n_q < n_k and window <= n_k:
             raise ValueError("soup_attention: attention_sink_tokens with a cache longer than the sliding "
                              "window; run the whole sequence in one call (use_cache=False)")
-        if window < n_k:
-            if (n_q == n_k and not dropout and query.is_cuda and query.shape[-1] == HEAD_DIM
-                    and query.dtype == key.dtype == value.dtype == torch.bfloat16):
-                scale = scaling if scaling is not None else query.shape[-1] ** -0.5
-                return window_attention(query, key, value, float(scale), window, sinks), None
+        hides = bool(window) and window < n_k
+        if hides and (n_q == n_k and not dropout and query.is_cuda and query.shape[-1] == HEAD_DIM
+                      and query.dtype == key.dtype == value.dtype == torch.bfloat16):
+            scale = scaling if scaling is not None else query.shape[-1] ** -0.5
+            return window_attention(query, key, value, float(scale), window, sinks), None
+        if hides or 1 < n_q < n_k:  # SDPA's own causal mask takes the queries for the first tokens
             k_pos = torch.arange(n_k, device=query.device)
             dist = (k_pos[:, None] - k_pos[None, :])[n_k - n_q:]
-            attention_mask = ((dist >= 0) & ((dist < window) | (k_pos[None, :] < sinks)))[None, None]
+            attention_mask = dist >= 0
+            if hides:
+                attention_mask &= (dist < window) | (k_pos[None, :] < sinks)
+            attention_mask = attention_mask[None, None]
+            is_causal = False  # in the mask
     if not _supported(module, query, key, value, attention_mask, dropout):
         from transformers.integrations.sdpa_attention import sdpa_attention_forward
 

@@ -165,3 +165,67 @@ def test_token_logps_backward_reads_what_came_back(monkeypatch, layout, blocks):
         assert again[1] == again[3] == gap and (again[5] - 256 * 8 == back_t.data_ptr()) == same
     else:
         assert bwd[0] % 16 == 0 and (bwd[0] == state.data_ptr()) == same
+
+
+# ------------------------------------------------------- attention against a cache ----
+class _Layer(torch.nn.Module):
+    """What soup_attention reads of a transformers attention layer."""
+
+    def __init__(self, groups, sinks=0):
+        super().__init__()
+        self.is_causal, self.num_key_value_groups = True, groups
+        self.config = type("Config", (), {"attention_sink_tokens": sinks})()
+
+
+@pytest.mark.parametrize("n_q,n_k,window,sinks", [
+    (4, 12, 12, 0), (4, 12, 64, 0), (4, 12, None, 0), (2, 3, None, 0), (11, 12, 12, 0), (4, 12, 13, 3),
+    (4, 12, 11, 0), (1, 12, None, 0), (12, 12, None, 2), (12, 12, 12, 2),
+])
+@pytest.mark.parametrize("explicit", [False, True])
+def test_chunk_against_a_cache(n_q, n_k, window, sinks, explicit):
+    """The queries are the last tokens of the keys; fp64, so only the sums' order differs."""
+    from auspex_soup_demo_b200.kernels.attention import soup_attention
+
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(2, h, n, 16, generator=g, dtype=torch.float64)
+               for h, n in ((4, n_q), (2, n_k), (2, n_k)))
+    kw = {"is_causal": True} if explicit and n_q > 1 else {}
+    out, _ = soup_attention(_Layer(2, sinks), q, k, v, None, scaling=0.3, sliding_window=window, **kw)
+    for h in range(4):
+        for i in range(n_q):
+            pos = n_k - n_q + i
+            see = [j for j in range(pos + 1) if window is None or pos - j < window or j < sinks]
+            p = torch.softmax(0.3 * (k[:, h // 2, see] @ q[:, h, i, :, None])[..., 0], -1)
+            want = (p[:, None] @ v[:, h // 2, see])[:, 0]
+            assert (out[:, i, h] - want).abs().max() <= 1e-13 * v.abs().max()
+
+
+def _tiny_model(impl, **over):
+    from transformers import Qwen2Config, Qwen2ForCausalLM
+
+    from auspex_soup_demo_b200.kernels import attention
+
+    attention.register()
+    torch.manual_seed(0)
+    cfg = Qwen2Config(vocab_size=50, hidden_size=32, intermediate_size=64, num_hidden_layers=2,
+                      num_attention_heads=4, num_key_value_heads=2, attn_implementation=impl, **over)
+    return Qwen2ForCausalLM(cfg).eval()
+
+
+SLIDING = dict(use_sliding_window=True, sliding_window=4, max_window_layers=1)
+
+
+@pytest.mark.parametrize("over", [{}, SLIDING, dict(SLIDING, sliding_window=30)],
+                         ids=["full", "sliding", "wide window"])
+def test_model_continues_a_cache_with_a_chunk(over):
+    a = _tiny_model("soup_b200", **over)
+    ids = torch.randint(0, 50, (2, 14), generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        whole = a(ids).logits
+        cache, parts = None, []
+        for lo, hi in ((0, 5), (5, 11), (11, 12), (12, 14)):
+            r = a(ids[:, lo:hi], past_key_values=cache, use_cache=True)
+            cache = r.past_key_values
+            parts.append(r.logits)
+    # the same fp32 sums in another order; logits are below 1
+    assert (torch.cat(parts, 1) - whole).abs().max() <= 1e-5
