@@ -254,10 +254,10 @@ def soup_attention(module, query, key, value, attention_mask, dropout: float = 0
             return window_attention(query, key, value, float(scale), window, sinks), None
         if hides or 1 < n_q < n_k:  # SDPA's own causal mask takes the queries for the first tokens
             k_pos = torch.arange(n_k, device=query.device)
-            dist = (k_pos[:, None] - k_pos[None, :])[n_k - n_q:]
+            dist = k_pos[n_k - n_q:, None] - k_pos  # of the queries alone: [n_q, n_k]
             attention_mask = dist >= 0
             if hides:
-                attention_mask &= (dist < window) | (k_pos[None, :] < sinks)
+                attention_mask &= (dist < window) | (k_pos < sinks)
             attention_mask = attention_mask[None, None]
             is_causal = False  # in the mask
     if not _supported(module, query, key, value, attention_mask, dropout):

@@ -229,3 +229,26 @@ def test_model_continues_a_cache_with_a_chunk(over):
             parts.append(r.logits)
     # the same fp32 sums in another order; logits are below 1
     assert (torch.cat(parts, 1) - whole).abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("n_q,n_k,window", [(1, 8192, 100), (3, 8192, None)])
+def test_cached_attention_takes_memory_of_the_queries_alone(n_q, n_k, window):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from auspex_soup_demo_b200.kernels.attention import soup_attention
+
+    class Largest(TorchDispatchMode):
+        numel = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            for t in out if isinstance(out, (tuple, list)) else (out,):
+                if isinstance(t, torch.Tensor):
+                    self.numel = max(self.numel, t.untyped_storage().nbytes())
+            return out
+
+    q, k, v = (torch.randn(1, 2, n, 16) for n in (n_q, n_k, n_k))
+    with Largest() as seen:
+        out, _ = soup_attention(_Layer(1), q, k, v, None, sliding_window=window)
+    assert out.shape == (1, n_q, 2, 16)
+    assert 0 < seen.numel <= 4 * k.numel() * k.element_size()  # [n_k, n_k] would be 64 times that and more
