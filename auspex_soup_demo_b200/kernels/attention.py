@@ -16,7 +16,8 @@ the QLoRA step:
   ``AttentionInterface`` signature, registered under the name ``"soup_b200"``
   by :func:`register`. Calls the kernels have no form for (an attention mask,
   dropout, a head dim other than 128, non-bf16 or CPU tensors) go to
-  transformers' SDPA function unchanged. Layers with a ``sliding_window`` (and,
+  transformers' SDPA function unchanged; :func:`soup_mask` decides which calls of a
+  model need a mask. Layers with a ``sliding_window`` (and,
   optionally, ``config.attention_sink_tokens``) take :func:`window_attention`.
 """
 
@@ -271,9 +272,49 @@ def soup_attention(module, query, key, value, attention_mask, dropout: float = 0
     return flash_attention(query, key, value, float(scale), causal), None
 
 
+def _kernels_mask_it(q_length, kv_length, q_offset, kv_offset, attention_mask, local_size, config) -> bool:
+    """Whether :func:`soup_attention` without a mask computes this layer type's causal
+    attention: the whole sequence in one call, the window (if any) the layer's own, and
+    padding, if any, only behind the tokens of each row, where no token looks."""
+    if q_length != kv_length or not isinstance(q_offset, int) or q_offset or kv_offset:
+        return False
+    if local_size is not None and local_size != getattr(config, "sliding_window", None):
+        return False  # attention in chunks
+    if attention_mask is None:
+        return True
+    if attention_mask.dim() != 2 or attention_mask.shape[1] != kv_length or (
+            attention_mask.is_cuda and torch.cuda.is_current_stream_capturing()):
+        return False  # (a capture cannot look at the values)
+    kept = attention_mask != 0
+    return not bool((kept[:, 1:] & ~kept[:, :-1]).any())
+
+
+def soup_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, attention_mask=None, local_size=None,
+              allow_is_causal_skip: bool = True, config=None, **kwargs):
+    """transformers ``AttentionMaskInterface`` function of ``INTERFACE_NAME``: no mask for
+    the calls that :func:`soup_attention` masks itself, else transformers' SDPA mask
+    (padding before or between tokens, caches, packed sequences), which takes the call
+    to SDPA."""
+    from transformers.masking_utils import sdpa_mask
+
+    if allow_is_causal_skip and _kernels_mask_it(q_length, kv_length, q_offset, kv_offset, attention_mask,
+                                                 local_size, config):
+        return None
+    if local_size is not None and getattr(config, "attention_sink_tokens", 0):
+        if not (isinstance(q_offset, int) and attention_mask is None and q_offset + q_length <= local_size):
+            raise ValueError("soup_attention: attention_sink_tokens need the whole sequence in one call "
+                             "(use_cache=False), with no padding before its tokens")
+    if attention_mask is not None and attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
+        allow_is_causal_skip = False
+    return sdpa_mask(batch_size=batch_size, q_length=q_length, kv_length=kv_length, q_offset=q_offset,
+                     kv_offset=kv_offset, attention_mask=attention_mask, local_size=local_size,
+                     allow_is_causal_skip=allow_is_causal_skip, config=config, **kwargs)
+
+
 def register() -> str:
-    """Register :func:`soup_attention` with transformers under ``INTERFACE_NAME``."""
-    from transformers import AttentionInterface
+    """Register :func:`soup_attention` and its masks with transformers under ``INTERFACE_NAME``."""
+    from transformers import AttentionInterface, AttentionMaskInterface
 
     AttentionInterface.register(INTERFACE_NAME, soup_attention)
+    AttentionMaskInterface.register(INTERFACE_NAME, soup_mask)
     return INTERFACE_NAME

@@ -198,3 +198,72 @@ def test_policy_loss_kl_near_the_reference(size, n):
     small = d * d * (0.5 + d * (1 / 6 + d * (1 / 24 + d * (1 / 120 + d / 720))))
     want = torch.where(d.abs() < 0.02, small, torch.expm1(d) - d).mean()
     assert abs(float(kl) - float(want)) <= 2.0 ** -20 * float(want)
+
+
+# ---------------------------------------------------------------- sliding layers ----
+def _model(attention, **over):
+    from auspex_soup_demo_b200 import apply, qlora
+
+    apply()
+    cfg = qlora.qwen2_1p5b_config(2, attention, hidden_size=256, intermediate_size=512, num_attention_heads=2,
+                                  num_key_value_heads=1, vocab_size=1000, use_sliding_window=True,
+                                  sliding_window=20, max_window_layers=1, **over)
+    return qlora.build_qwen2_qlora(cfg, seed=1).eval()
+
+
+def test_token_against_a_long_cache_takes_little_memory():
+    from auspex_soup_demo_b200.kernels.attention import soup_attention
+
+    class Layer(torch.nn.Module):
+        is_causal, num_key_value_groups = True, 6
+
+    q, k, v = (torch.randn(1, h, n, 128, generator=_gen(n + h), device=DEV).bfloat16()
+               for h, n in ((12, 1), (2, 32768), (2, 32768)))
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    out, _ = soup_attention(Layer(), q, k, v, None, sliding_window=4096)
+    # keys and values once for every query head (6 groups each), not 32768^2 distances
+    assert torch.cuda.max_memory_allocated() - base <= 16 * (k.nbytes + v.nbytes)
+    see = slice(32768 - 4096, None)
+    kk, vv = (t[:, :, see].double().repeat_interleave(6, 1) for t in (k, v))
+    want = torch.softmax(q.double() @ kk.transpose(2, 3) * 128 ** -0.5, -1) @ vv
+    # P and the output rounded to bf16 (2^-8 each, P's averaging out over 4096 keys)
+    err = (out.transpose(1, 2).double() - want).abs()
+    assert bool((err <= 2.0 ** -8 * 1.03 * want.abs() + 2.0 ** -8 * float(want.abs().max())).all())
+
+
+def test_padded_batches_of_a_model_with_sliding_layers(monkeypatch):
+    a, b = _model("soup"), _model("sdpa")
+    ids = torch.randint(0, 1000, (3, 150), generator=_gen(20), device=DEV)
+    calls = []
+    call = _lib.call
+    monkeypatch.setattr(_lib, "call", lambda fn, *args: (calls.append(fn), call(fn, *args))[1])
+    for kind in ("none", "right", "left"):
+        mask = torch.ones(3, 150, dtype=torch.long, device=DEV)
+        if kind == "right":
+            mask[0, 90:] = 0
+        if kind == "left":
+            mask[1, :40] = 0
+        calls.clear()
+        with torch.no_grad():
+            x = a(ids, attention_mask=mask).logits[mask.bool()].double()
+            on_kernels = {"soup_attention_window_fwd", "soup_attention_fwd"} <= set(calls)
+            y = b(ids, attention_mask=mask).logits[mask.bool()].double()
+        # two bf16 attention kernels through two layers
+        assert float((x - y).norm() / y.norm()) <= 0.02, kind
+        assert on_kernels == (kind != "left")
+
+
+def test_chunks_against_a_cache_of_a_model_with_sliding_layers():
+    a = _model("soup")
+    ids = torch.randint(0, 1000, (2, 70), generator=_gen(21), device=DEV)
+    with torch.no_grad():
+        whole = a(ids).logits.double()
+        cache, parts = None, []
+        for lo, hi in ((0, 15), (15, 30), (30, 31), (31, 70)):
+            r = a(ids[:, lo:hi], past_key_values=cache, use_cache=True)
+            cache = r.past_key_values
+            parts.append(r.logits)
+    rest = torch.cat(parts, 1).double()
+    assert float((whole - rest).norm() / whole.norm()) <= 0.02  # as above

@@ -252,3 +252,71 @@ def test_cached_attention_takes_memory_of_the_queries_alone(n_q, n_k, window):
         out, _ = soup_attention(_Layer(1), q, k, v, None, sliding_window=window)
     assert out.shape == (1, n_q, 2, 16)
     assert 0 < seen.numel <= 4 * k.numel() * k.element_size()  # [n_k, n_k] would be 64 times that and more
+
+
+# ------------------------------------------------------------- masks of a model ----
+def _padded(kind):
+    m = torch.ones(2, 12, dtype=torch.long)
+    if kind == "left":
+        m[0, :3] = 0
+    elif kind == "right":
+        m[0, 9:] = 0
+    elif kind == "hole":
+        m[1, 5:7] = 0
+    return m
+
+
+@pytest.mark.parametrize("kind", ["none", "left", "right", "hole"])
+@pytest.mark.parametrize("over", [{}, SLIDING], ids=["full", "sliding"])
+def test_padded_batch_as_with_sdpa(kind, over):
+    ids = torch.randint(0, 50, (2, 12), generator=torch.Generator().manual_seed(2))
+    mask = _padded(kind)
+    a, b = (_tiny_model(impl, **over) for impl in ("soup_b200", "sdpa"))
+    with torch.no_grad():
+        x, y = (m(ids, attention_mask=mask).logits[mask.bool()] for m in (a, b))
+    assert (x - y).abs().max() <= 1e-6  # the same fp32 sums, perhaps in another order
+
+
+@pytest.mark.parametrize("over", [{}, SLIDING], ids=["full", "sliding"])
+@pytest.mark.parametrize("static", [False, True])
+def test_generation_from_a_padded_batch_as_with_sdpa(over, static):
+    ids = torch.randint(0, 50, (2, 12), generator=torch.Generator().manual_seed(3))
+    kw = dict(cache_implementation="static") if static else {}
+    a, b = (_tiny_model(impl, **over).generate(ids, attention_mask=_padded("left"), max_new_tokens=5,
+                                               do_sample=False, pad_token_id=0, output_scores=True,
+                                               return_dict_in_generate=True, **kw)
+            for impl in ("soup_b200", "sdpa"))
+    assert torch.equal(a.sequences, b.sequences)
+    assert max((x - y).abs().max() for x, y in zip(a.scores, b.scores)) <= 1e-5
+
+
+def _mask(kind=None, q=12, k=12, offset=0, local=None, sinks=0, **kw):
+    from auspex_soup_demo_b200.kernels.attention import soup_mask
+    from transformers.masking_utils import causal_mask_function
+
+    config = type("Config", (), {"sliding_window": 4, "attention_sink_tokens": sinks})()
+    return soup_mask(batch_size=2, q_length=q, kv_length=k, q_offset=offset, kv_offset=0,
+                     mask_function=causal_mask_function, attention_mask=kind and _padded(kind).bool(),
+                     local_size=local, config=config, **kw)
+
+
+@pytest.mark.parametrize("local", [None, 4])
+def test_masks_that_the_kernels_need_not(local):
+    """Whole sequences, also with padding behind them, stay on the kernels."""
+    for kind in (None, "none", "right"):
+        assert _mask(kind, local=local, sinks=3) is None
+    for kind in ("left", "hole"):
+        assert _mask(kind, local=local).shape == (2, 1, 12, 12)
+    assert _mask(None, local=local, allow_is_causal_skip=False).shape[-2:] == (12, 12)
+    assert _mask(None, 3, 12, 9, local=local).shape[-2:] == (3, 12)
+    assert _mask(None, local=5).shape[-2:] == (12, 12)  # not this layer type's window: chunks
+
+
+@pytest.mark.parametrize("call", [
+    lambda: _mask("left", local=4, sinks=2),
+    lambda: _mask(None, 1, 4, 11, local=4, sinks=2),
+    lambda: _mask(None, 3, 12, torch.tensor(9), local=4, sinks=2, allow_is_causal_skip=False),
+])
+def test_sinks_refuse_masks_they_are_not_in(call):
+    with pytest.raises(ValueError, match="attention_sink_tokens"):
+        call()
