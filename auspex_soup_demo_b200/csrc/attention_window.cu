@@ -1317,6 +1317,18 @@ bool sizes_ok(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq) {
          batch * heads * ((seq + kTile - 1) / kTile) <= (1 << 28);
 }
 
+// The visible keys in the form that the kernels run fastest: a window and sinks that
+// together reach every key (window + sinks >= seq) are the plain causal case.
+struct Visible {
+  int window, sinks;
+};
+Visible visible(int64_t seq, int64_t window, int64_t sinks) {
+  if (window > seq) window = seq;
+  if (sinks > seq) sinks = seq;
+  if (window + sinks >= seq) return {(int)seq, 0};
+  return {(int)window, (int)sinks};
+}
+
 // How the dK / dV work is cut: the query heads of a KV head into `groups` CTAs when
 // one CTA per key tile would leave SMs idle, the sink tiles' steps into segments as
 // long as an ordinary tile's.
@@ -1327,11 +1339,9 @@ struct DkvPlan {
 DkvPlan dkv_plan(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t window, int64_t sinks) {
   DkvPlan p;
   const int64_t nt = (S + kTile - 1) / kTile;
-  if (window > S) window = S;
-  if (sinks > S) sinks = S;
-  if (window == S) sinks = 0;  // the window alone shows every key
-  p.n_sink = (int)((sinks + kTile - 1) / kTile);
-  const int64_t steps = (kTile + window - 2) / kTile + 1;  // of an ordinary tile
+  const Visible vis = visible(S, window, sinks);
+  p.n_sink = (vis.sinks + kTile - 1) / kTile;
+  const int64_t steps = (kTile + vis.window - 2) / kTile + 1;  // of an ordinary tile
   p.seg_steps = (int)(steps < 4 ? 4 : steps < nt ? steps : nt);
   p.segs = (int)((nt + p.seg_steps - 1) / p.seg_steps);
   const int64_t rep = H / Hk;
@@ -1398,9 +1408,9 @@ int soup_attention_window_fwd(const void* q, const int64_t* q_strides, const voi
   if ((rc = make_bhsd_map(&mv, v, v_strides, batch, kv_heads, seq, "v", kBlk))) return rc;
   static bool smem_set_done[64] = {false};
   if ((rc = set_smem(win_fwd_kernel, WinFwdSmem::kBytes, smem_set_done))) return rc;
-  FwdArgs a{(int)batch, (int)heads, (int)kv_heads, (int)seq, scale * 1.4426950408889634f,
-            (int)(window < seq ? window : seq), (int)(sinks < seq ? sinks : seq),
-            static_cast<bf16*>(out), lse, wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
+  const Visible vis = visible(seq, window, sinks);
+  FwdArgs a{(int)batch, (int)heads, (int)kv_heads, (int)seq, scale * 1.4426950408889634f, vis.window,
+            vis.sinks, static_cast<bf16*>(out), lse, wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
   const int64_t nq = (seq + kTile - 1) / kTile;
   win_fwd_kernel<<<(unsigned)(batch * heads * nq), kFwdThreads, WinFwdSmem::kBytes,
                    as_stream(stream)>>>(mq, mk, mv, a, err);
@@ -1475,9 +1485,8 @@ int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const voi
   if ((rc = set_smem(win_dq_kernel, WinDqSmem::kBytes, dq_set))) return rc;
   cudaStream_t st = as_stream(stream);
   const int B = (int)batch, H = (int)heads, Hk = (int)kv_heads, S = (int)seq;
-  const int win = (int)(window < seq ? window : seq);
-  const int snk = win == S ? 0 : (int)(sinks < seq ? sinks : seq);
-  BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, win, snk, dvec, nl2,
+  const Visible vis = visible(seq, window, sinks);
+  BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, vis.window, vis.sinks, dvec, nl2,
             static_cast<const bf16*>(out), static_cast<const bf16*>(dout), lse,
             static_cast<bf16*>(dq), static_cast<bf16*>(dk), static_cast<bf16*>(dv), part, p.groups,
             p.heads_per, p.n_sink, p.segs, p.seg_steps,

@@ -267,3 +267,20 @@ def test_chunks_against_a_cache_of_a_model_with_sliding_layers():
             parts.append(r.logits)
     rest = torch.cat(parts, 1).double()
     assert float((whole - rest).norm() / whole.norm()) <= 0.02  # as above
+
+
+# ------------------------------------------------------- window attention's key ranges ----
+@pytest.mark.parametrize("S,window,sinks", [(500, 7, 493), (500, 7, 500), (300, 1, 299), (640, 320, 320),
+                                            (129, 128, 1), (1, 1, 0)])
+def test_window_and_sinks_that_hide_nothing(S, window, sinks):
+    """Bit for bit the causal case, in which no key is hidden either."""
+    q, k, v = (torch.randn(2, S, h, 128, generator=_gen(S + h), device=DEV).bfloat16().transpose(1, 2)
+               .requires_grad_(True) for h in (4, 2, 2))
+    do = torch.randn(2, S, 4, 128, generator=_gen(S), device=DEV).bfloat16()
+
+    def run(*span):
+        out = kernels.window_attention(q, k, v, 0.09, *span)
+        return [out.detach()] + list(torch.autograd.grad(out, [q, k, v], do))
+
+    assert all(torch.equal(a, b) for a, b in zip(run(window, sinks), run(S, 0)))
+    assert _lib.device_error(torch.device(DEV)) == 0

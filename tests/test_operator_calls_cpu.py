@@ -320,3 +320,11 @@ def test_masks_that_the_kernels_need_not(local):
 def test_sinks_refuse_masks_they_are_not_in(call):
     with pytest.raises(ValueError, match="attention_sink_tokens"):
         call()
+
+
+# -------------------------------------------------- workspace of the window backward ----
+@pytest.mark.parametrize("S,window,sinks", [(16384, 128, 16384), (16384, 128, 16256), (5000, 1, 5000),
+                                            (5000, 2500, 2500), (700, 699, 1)])
+def test_window_and_sinks_that_hide_nothing_take_no_more_than_the_causal_case(S, window, sinks):
+    size = _lib.lib().soup_attention_window_bwd_workspace_bytes
+    assert size(1, 32, 8, S, window, sinks) == size(1, 32, 8, S, S, 0) > 0
