@@ -534,7 +534,8 @@ struct BwdArgs {
   int groups;        // parts that a KV head's query heads are split into
   int heads_per;     // query heads per part
   int n_sink;        // sink tiles
-  int segs, seg_steps;  // segments of a sink tile's 128-query steps, and their length
+  int segs, seg_steps;  // most segments of a sink tile's 128-query steps, and their length
+  int sink_slots;       // segments that the sink tiles of one KV head have, together
   uint64_t wait_ns;
 };
 
@@ -546,6 +547,17 @@ struct DkvUnit {
 __host__ __device__ __forceinline__ int dkv_sink_units(const BwdArgs& a) {
   return a.B * a.Hk * a.n_sink * a.groups * a.segs;
 }
+// Sink tile kt has ceil((nq - kt) / seg_steps) segments; those of the tiles before it:
+__host__ __device__ __forceinline__ int64_t segments_of_last(int64_t tiles, int64_t seg_steps) {
+  const int64_t n = tiles / seg_steps, r = tiles % seg_steps;  // sum of ceil(m / seg_steps), m = 1..tiles
+  return seg_steps * (n * (n + 1) / 2) + r * (n + 1);
+}
+__host__ __device__ __forceinline__ int segments_before(int kt, int nq, int seg_steps) {
+  return static_cast<int>(segments_of_last(nq, seg_steps) - segments_of_last(nq - kt, seg_steps));
+}
+__host__ __device__ __forceinline__ int segments_of(int kt, int nq, int seg_steps) {
+  return (nq - kt + seg_steps - 1) / seg_steps;
+}
 __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
   DkvUnit u;
   const int nq = (a.S + kTile - 1) / kTile;
@@ -553,19 +565,20 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
   const int rep = a.H / a.Hk;
   int g, bhk;
   if (i < n_sink_units) {
-    u.slot = i;
     const int seg = i % a.segs;
     i /= a.segs;
     g = i % a.groups;
     i /= a.groups;
     u.kt = i % a.n_sink;
     bhk = i / a.n_sink;
+    u.slot = (bhk * a.sink_slots + segments_before(u.kt, nq, a.seg_steps)) * a.groups +
+             g * segments_of(u.kt, nq, a.seg_steps) + seg;
     u.step0 = u.kt + seg * a.seg_steps;
     const int end = u.step0 + a.seg_steps < nq ? u.step0 + a.seg_steps : nq;
     u.n = end > u.step0 ? end - u.step0 : 0;
   } else {
     i -= n_sink_units;
-    u.slot = a.groups > 1 ? n_sink_units + i : -1;
+    u.slot = a.groups > 1 ? a.B * a.Hk * a.sink_slots * a.groups + i : -1;
     g = i % a.groups;
     i /= a.groups;
     bhk = i % (a.B * a.Hk);
@@ -631,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   const DkvUnit u = dkv_unit(a, blockIdx.x);
   const int total = u.nh * u.n;  // steps of all this unit's query heads
-  if (total == 0) return;        // an empty segment (its slot is not read)
+  if (total == 0) return;        // an empty segment: later tiles have fewer (it has no slot)
   const uint32_t sbase = smem_u32(smem);
   const uint32_t bar0 = sbase + L::kBar;
   const uint32_t kv_full = bar0;
@@ -941,21 +954,16 @@ __global__ void __launch_bounds__(256) win_dkdv_sum_kernel(BwdArgs a, int tiles)
   const int key = kt * kTile + r;
   if (key >= a.S) return;
   int slot0, n;
-  int segs = 1;
   if (kt < a.n_sink) {
-    slot0 = (bhk * a.n_sink + kt) * a.groups * a.segs;
-    n = a.groups * a.segs;
-    segs = (nq - kt + a.seg_steps - 1) / a.seg_steps;  // of a.segs, the others are empty
+    slot0 = (bhk * a.sink_slots + segments_before(kt, nq, a.seg_steps)) * a.groups;
+    n = a.groups * segments_of(kt, nq, a.seg_steps);
   } else {
-    slot0 = dkv_sink_units(a) + ((kt - a.n_sink) * a.B * a.Hk + bhk) * a.groups;
+    slot0 = (a.B * a.Hk * a.sink_slots + (kt - a.n_sink) * a.B * a.Hk + bhk) * a.groups;
     n = a.groups;
   }
   const int d = (threadIdx.x & 31) * 4;
   float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-  const int rep = a.H / a.Hk;
   for (int s = 0; s < n; ++s) {
-    const int g = kt < a.n_sink ? s / a.segs : s;
-    if (g * a.heads_per >= rep || (kt < a.n_sink && s % a.segs >= segs)) continue;
     const float* p = a.part + ((int64_t)(slot0 + s) * 2 * kTile + r) * kHeadDim + d;
     const float4 x = *reinterpret_cast<const float4*>(p);
     const float4 y = *reinterpret_cast<const float4*>(p + kTile * kHeadDim);
@@ -1331,9 +1339,10 @@ Visible visible(int64_t seq, int64_t window, int64_t sinks) {
 
 // How the dK / dV work is cut: the query heads of a KV head into `groups` CTAs when
 // one CTA per key tile would leave SMs idle, the sink tiles' steps into segments as
-// long as an ordinary tile's.
+// long as an ordinary tile's, or, with many sinks, a quarter of an SM's share of all steps
+// (each segment costs 128 KB of partials, and shorter ones no longer even out the SMs).
 struct DkvPlan {
-  int groups, heads_per, n_sink, segs, seg_steps;
+  int groups, heads_per, n_sink, segs, seg_steps, sink_slots;
   int64_t units, slots;
 };
 DkvPlan dkv_plan(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t window, int64_t sinks) {
@@ -1342,8 +1351,6 @@ DkvPlan dkv_plan(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t window, in
   const Visible vis = visible(S, window, sinks);
   p.n_sink = (vis.sinks + kTile - 1) / kTile;
   const int64_t steps = (kTile + vis.window - 2) / kTile + 1;  // of an ordinary tile
-  p.seg_steps = (int)(steps < 4 ? 4 : steps < nt ? steps : nt);
-  p.segs = (int)((nt + p.seg_steps - 1) / p.seg_steps);
   const int64_t rep = H / Hk;
   const int64_t tiles = B * Hk * nt;
   // one CTA per key tile if that fills most SMs, else the fewest head groups that do
@@ -1352,10 +1359,18 @@ DkvPlan dkv_plan(int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t window, in
   if (g < 1) g = 1;
   p.heads_per = (int)((rep + g - 1) / g);
   p.groups = (int)((rep + p.heads_per - 1) / p.heads_per);
+  const int64_t ns = p.n_sink, tile_steps = steps < nt ? steps : nt;
+  const int64_t all = B * Hk * p.groups * (ns * nt - ns * (ns - 1) / 2 + (nt - ns) * tile_steps);
+  const int64_t share = (all + 4 * num_sms() - 1) / (4 * num_sms());
+  int64_t seg = share > tile_steps ? share : tile_steps;
+  if (seg > nt) seg = nt;
+  p.seg_steps = (int)(seg < 4 ? 4 : seg);
+  p.segs = (int)((nt + p.seg_steps - 1) / p.seg_steps);
+  p.sink_slots = segments_before(p.n_sink, (int)nt, p.seg_steps);
   const int64_t sink_units = B * Hk * p.n_sink * p.groups * p.segs;
   const int64_t rest = B * Hk * (nt - p.n_sink) * p.groups;
   p.units = sink_units + rest;
-  p.slots = sink_units + (p.groups > 1 ? rest : 0);
+  p.slots = B * Hk * p.sink_slots * p.groups + (p.groups > 1 ? rest : 0);
   return p;
 }
 size_t vec_bytes(int64_t B, int64_t H, int64_t S) {
@@ -1489,7 +1504,7 @@ int soup_attention_window_bwd(const void* q, const int64_t* q_strides, const voi
   BwdArgs a{B, H, Hk, S, scale, scale * 1.4426950408889634f, vis.window, vis.sinks, dvec, nl2,
             static_cast<const bf16*>(out), static_cast<const bf16*>(dout), lse,
             static_cast<bf16*>(dq), static_cast<bf16*>(dk), static_cast<bf16*>(dv), part, p.groups,
-            p.heads_per, p.n_sink, p.segs, p.seg_steps,
+            p.heads_per, p.n_sink, p.segs, p.seg_steps, p.sink_slots,
             wait_limit_ns() ? wait_limit_ns() : tc::kWaitNs};
   const int nt = (S + kTile - 1) / kTile;
   win_dq_kernel<<<(unsigned)(B * H * nt), kDqThreads, WinDqSmem::kBytes, st>>>(mq, mkb, mvb, mdo, a,

@@ -81,3 +81,13 @@ def test_long_window(B, H, Hk, S, window, sinks):
         assert all(torch.equal(a, b) for a, b in zip(run(), got))
     torch.cuda.synchronize()
     assert _lib.device_error(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("B,H,Hk,S,window,sinks", [
+    (1, 4, 2, 6000, 128, 3000),  # sink tiles in long segments
+    (1, 2, 1, 5000, 1, 4990),    # nearly all keys are sinks
+    (3, 6, 3, 2100, 70, 1000),
+    (1, 8, 1, 3000, 200, 900),   # heads split over CTAs beside the segments
+])
+def test_many_sinks(B, H, Hk, S, window, sinks):
+    test_long_window(B, H, Hk, S, window, sinks)

@@ -328,3 +328,66 @@ def test_sinks_refuse_masks_they_are_not_in(call):
 def test_window_and_sinks_that_hide_nothing_take_no_more_than_the_causal_case(S, window, sinks):
     size = _lib.lib().soup_attention_window_bwd_workspace_bytes
     assert size(1, 32, 8, S, window, sinks) == size(1, 32, 8, S, S, 0) > 0
+
+
+def _dkv_plan(B, H, Hk, S, window, sinks, sms=148):
+    """The host's cut of the dK / dV work, restated."""
+    nt, rep = -(-S // 128), H // Hk
+    window, sinks = min(window, S), min(sinks, S)
+    if window + sinks >= S:
+        window, sinks = S, 0
+    ns = -(-sinks // 128)
+    tile_steps = min((128 + window - 2) // 128 + 1, nt)
+    g = max(1, min(rep, -(-(sms * 4 // 5) // (B * Hk * nt))))
+    heads_per = -(-rep // g)
+    groups = -(-rep // heads_per)
+    work = B * Hk * groups * (ns * nt - ns * (ns - 1) // 2 + (nt - ns) * tile_steps)
+    seg_steps = max(4, min(nt, max(tile_steps, -(-work // (4 * sms)))))
+    return nt, ns, groups, heads_per, seg_steps
+
+
+# batch, heads, KV heads, length, window, sinks
+CUTS = [(1, 32, 8, 16384, 128, 8192), (1, 12, 2, 16001, 1000, 16), (4, 12, 2, 2048, 512, 4),
+        (2, 6, 3, 5000, 1, 4998), (1, 8, 1, 131072, 128, 65536), (1, 7, 1, 1000, 70, 129), (1, 1, 1, 1, 1, 0),
+        (3, 4, 4, 4097, 700, 0), (2, 8, 2, 1300, 1300, 5)]
+
+
+@pytest.mark.parametrize("sizes", CUTS)
+def test_partial_slots_of_the_window_backward(sizes):
+    """Every partial has a slot of its own inside the workspace; the sink tiles' segments cover
+    their steps."""
+    B, H, Hk, S, _, _ = sizes
+    nt, ns, groups, heads_per, seg_steps = _dkv_plan(*sizes)
+    before, used = 0, set()
+    starts = []
+    for kt in range(ns):
+        n = nt - kt
+        q, r = divmod(nt - kt, seg_steps)
+        q0, r0 = divmod(nt, seg_steps)
+        closed = (seg_steps * q0 * (q0 + 1) // 2 + r0 * (q0 + 1)) - (seg_steps * q * (q + 1) // 2 + r * (q + 1))
+        assert closed == before  # the kernels' closed form of the segments of earlier tiles
+        starts.append((before, -(-n // seg_steps)))
+        before += -(-n // seg_steps)
+    for bhk in range(B * Hk):
+        for first, count in starts:
+            for g in range(groups):
+                for seg in range(count):
+                    slot = (bhk * before + first) * groups + g * count + seg
+                    assert slot not in used
+                    used.add(slot)
+    rest = B * Hk * (nt - ns) * groups if groups > 1 else 0
+    assert used == set(range(B * Hk * before * groups))
+    assert (groups - 1) * heads_per < H // Hk <= groups * heads_per
+    vectors = 2 * (-(-B * H * nt * 128 * 4 // 256) * 256)
+    got = _lib.lib().soup_attention_window_bwd_workspace_bytes(*sizes)
+    assert got == vectors + (len(used) + rest) * 2 * 128 * 128 * 4
+
+
+@pytest.mark.parametrize("sizes", CUTS)
+def test_partials_stay_linear_in_the_sink_tiles(sizes):
+    B, H, Hk, S, _, _ = sizes
+    nt, ns, groups, _, _ = _dkv_plan(*sizes)
+    partials = (_lib.lib().soup_attention_window_bwd_workspace_bytes(*sizes)
+                - 2 * (-(-B * H * nt * 128 * 4 // 256) * 256)) // (2 * 128 * 128 * 4)
+    # one slot a sink tile (and a tile, when few tiles split their heads), and four an SM
+    assert partials <= B * Hk * groups * (nt if groups > 1 else ns) + 4 * 148
