@@ -93,12 +93,19 @@ def _ld(t: torch.Tensor) -> int:
 
 def quantize_8bit(x2: torch.Tensor):
     """(codes int8 [rows, n], scales fp32 [rows, ceil(n / 64)]) of a CUDA tensor
-    [rows, n]: per 64 consecutive columns scale = absmax / 127 and
+    [..., n]: per 64 consecutive columns scale = absmax / 127 and
     code = round(x * (127 / absmax)); the kept value is code * scale."""
+    if x2.dim() == 0 or x2.shape[-1] == 0:
+        raise ValueError(f"quantize_8bit: needs rows of columns, got {tuple(x2.shape)}")
+    _lib.dtype_code(x2.dtype)
+    if not x2.is_cuda:
+        raise ValueError("quantize_8bit: the tensor must be on a CUDA device")
     x2 = _rows_8bit(x2.detach(), x2.shape[-1])
     rows, n = x2.shape
     codes = torch.empty(rows, n, dtype=torch.int8, device=x2.device)
     scales = torch.empty(rows, -(-n // Q8_BLOCK), dtype=torch.float32, device=x2.device)
+    if rows == 0:
+        return codes, scales
     _lib.call("soup_q8_quantize", x2.device, x2.data_ptr(), _ld(x2), codes.data_ptr(), n,
               scales.data_ptr(), scales.shape[1], rows, n, _lib.dtype_code(x2.dtype), _lib.stream_of(x2))
     return codes, scales

@@ -284,3 +284,13 @@ def test_window_and_sinks_that_hide_nothing(S, window, sinks):
 
     assert all(torch.equal(a, b) for a, b in zip(run(window, sinks), run(S, 0)))
     assert _lib.device_error(torch.device(DEV)) == 0
+
+
+# ------------------------------------------------------------------ 8-bit codes ----
+def test_quantize_8bit_shapes():
+    codes, scales = kernels.quantize_8bit(torch.empty(0, 70, device=DEV))
+    assert codes.shape == (0, 70) and scales.shape == (0, 2)
+    x = torch.randn(3, 4, 70, generator=_gen(30), device=DEV)
+    want = kernels.quantize_8bit(x.view(12, 70))
+    for t in (x, x.transpose(0, 1).contiguous().transpose(0, 1)):
+        assert all(torch.equal(a, b) for a, b in zip(kernels.quantize_8bit(t), want))

@@ -18,6 +18,15 @@ def test_host_tensors_are_refused_before_a_launch(call):
         call(torch.zeros(4, 8))
 
 
+@pytest.mark.parametrize("x,error", [
+    (torch.zeros(4, 8), ValueError), (torch.zeros(()), ValueError), (torch.zeros(4, 0), ValueError),
+    (torch.zeros(4, 8, dtype=torch.int32), TypeError), (torch.zeros(4, 8, dtype=torch.float64), TypeError),
+])
+def test_quantize_8bit_refusals(x, error):
+    with pytest.raises(error, match="quantize_8bit|unsupported dtype"):
+        kernels.quantize_8bit(x)
+
+
 # ------------------------------------------------- saved tensors in other layouts ----
 def _relaid(t, layout):
     """The values of t as a saved-tensor hook may hand them back."""
