@@ -189,7 +189,8 @@ def head_token_logps(hidden: torch.Tensor, head: Any, labels: torch.Tensor,
     if weight.shape[0] == 0 or weight.shape[1] == 0 or weight.shape[1] % 8:
         raise ValueError("head_token_logps: the head needs rows, and a width that is a multiple of 8")
     if labels.numel() == 0:
-        z = hidden.sum(-1, dtype=torch.float32) * 0.0  # empty, connected to hidden
+        # empty, connected to the states and the head
+        z = hidden.sum(-1, dtype=torch.float32) + weight[:0].sum(dtype=torch.float32)
         return z, z.detach().clone()
     keep = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
     return HeadTokenLogpsFunction.apply(hidden, weight, labels, int(ignore_index), keep)

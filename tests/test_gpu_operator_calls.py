@@ -294,3 +294,16 @@ def test_quantize_8bit_shapes():
     want = kernels.quantize_8bit(x.view(12, 70))
     for t in (x, x.transpose(0, 1).contiguous().transpose(0, 1)):
         assert all(torch.equal(a, b) for a, b in zip(kernels.quantize_8bit(t), want))
+
+
+# ---------------------------------------------------------------------- no tokens ----
+@pytest.mark.parametrize("shape", [(0,), (2, 0)])
+@pytest.mark.parametrize("trained", ["states", "head", "both"])
+def test_head_token_logps_of_no_tokens(shape, trained):
+    h = torch.empty(*shape, 64, device=DEV, dtype=torch.bfloat16).requires_grad_(trained != "head")
+    w = torch.randn(100, 64, device=DEV).bfloat16().requires_grad_(trained != "states")
+    lp, ent = kernels.head_token_logps(h, w, torch.empty(*shape, dtype=torch.int64, device=DEV))
+    assert lp.shape == ent.shape == shape and lp.dtype == torch.float32 and not ent.requires_grad
+    leaves = [t for t in (h, w) if t.requires_grad]
+    for t, g in zip(leaves, torch.autograd.grad(lp.sum(), leaves)):
+        assert g.shape == t.shape and not g.any()
