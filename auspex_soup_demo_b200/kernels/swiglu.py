@@ -185,6 +185,8 @@ def swiglu_8bit(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 #: Keep the MLP's gate and up in 8 bits from forward to backward instead of
 #: recomputing them (takes precedence over RECOMPUTE in training): 2.1 bytes per
 #: token and intermediate column, no second gate/up GEMM.
+#: The QLoRA step's grouped MLPs do so where they run as one Function
+#: (``qlora.FUSE_MLP_BACKWARD``, bf16); others recompute, with a warning.
 CHECKPOINT_8BIT = False
 
 #: Recompute gate/up + SwiGLU in backward (the reference's selective recompute,

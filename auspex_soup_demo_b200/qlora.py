@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import warnings
 from typing import Iterable, Optional
 
 import numpy as np
@@ -622,11 +623,15 @@ class LoRAProjectionGroup:
         SwiGLU backward fused into down's input-gradient GEMM (FUSE_MLP_BACKWARD)
         when the activations are kept, bf16, and down is an ungrouped LoRA linear.
         ``keep8`` keeps [g | u] of that form in 8 bits (and h not at all); a form the
-        one Function does not take then recomputes instead."""
+        one Function does not take recomputes instead, with a warning."""
         if (FUSE_MLP_BACKWARD and not recompute and self.interleaved
                 and isinstance(down, _LoRABase) and down.lora_group is None
                 and x.dtype == torch.bfloat16 and down.in_features == self.outs[0]):
             return _LoRAMLPFn.apply(x, self, down, keep8, down.lora_A, down.lora_B, *self.params())
+        if keep8:
+            warnings.warn("swiglu.CHECKPOINT_8BIT keeps nothing in 8 bits here: this MLP is not run as one "
+                          "Function (FUSE_MLP_BACKWARD, interleaved gate/up rows, bf16 states and an ungrouped "
+                          "LoRA down projection), so its activations are recomputed", stacklevel=2)
         return down(self.swiglu(x, recompute or keep8))
 
 

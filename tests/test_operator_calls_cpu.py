@@ -400,3 +400,25 @@ def test_partials_stay_linear_in_the_sink_tiles(sizes):
                 - 2 * (-(-B * H * nt * 128 * 4 // 256) * 256)) // (2 * 128 * 128 * 4)
     # one slot a sink tile (and a tile, when few tiles split their heads), and four an SM
     assert partials <= B * Hk * groups * (nt if groups > 1 else ns) + 4 * 148
+
+
+# -------------------------------------------------------------- 8-bit checkpoints ----
+@pytest.mark.parametrize("keep8", [False, True])
+def test_mlp_that_cannot_keep_8_bits_says_so(keep8):
+    """A grouped MLP off the one-Function form (here: fp16 states) recomputes."""
+    import warnings
+
+    from auspex_soup_demo_b200 import qlora
+
+    class Group:
+        interleaved, outs = True, [8]
+
+        def swiglu(self, x, recompute):
+            return x * (2.0 if recompute else 3.0)
+
+    x = torch.ones(2, 8, dtype=torch.float16)
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        y = qlora.LoRAProjectionGroup.mlp(Group(), x, lambda h: h, False, keep8)
+    assert y[0, 0] == (2.0 if keep8 else 3.0)
+    assert [w for w in seen if "CHECKPOINT_8BIT" in str(w.message)] != [] if keep8 else not seen
