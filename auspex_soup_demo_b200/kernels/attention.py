@@ -79,6 +79,7 @@ def attention_backward(q, k, v, out, lse, dout, scale: float, causal: bool = Tru
     if dout.shape != (B, S, H, D):
         raise ValueError(f"attention: dout must be [B, S, H, D], got {tuple(dout.shape)}")
     dout = dout.to(torch.bfloat16).contiguous()
+    out = _lib.dense(out)
     base = lse._base if lse._base is not None else lse
     if base.shape != (B, H, _s_pad(S)) or base.dtype != torch.float32 or not base.is_contiguous():
         raise ValueError("attention: lse must come from attention_forward")
@@ -101,7 +102,8 @@ class FlashAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale: float, causal: bool):
         out, lse = attention_forward(q, k, v, scale, causal)
-        ctx.save_for_backward(q, k, v, out, lse)
+        # the padded buffer itself: a saved-tensor hook hands a view back without its base
+        ctx.save_for_backward(q, k, v, out, lse._base)
         ctx.scale = scale
         ctx.causal = causal
         return out
@@ -109,7 +111,7 @@ class FlashAttentionFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        dq, dk, dv = attention_backward(q, k, v, out, lse, dout, ctx.scale, ctx.causal)
+        dq, dk, dv = attention_backward(q, k, v, out, _lib.dense(lse), dout, ctx.scale, ctx.causal)
         return dq, dk, dv, None, None
 
 

@@ -57,6 +57,15 @@ def test_window_attention_under_offload(source):
     _same_under_offload(lambda: kernels.window_attention(q, k, v, 0.1, 50, 4), [q, k, v])
 
 
+@pytest.mark.parametrize("S", [200, 256])
+def test_causal_attention_under_offload(S):
+    from auspex_soup_demo_b200.kernels.attention import flash_attention
+
+    q, k, v = (torch.randn(2, S, h, 128, generator=_gen(h), device=DEV).bfloat16().transpose(1, 2)
+               .requires_grad_(True) for h in (4, 2, 2))
+    _same_under_offload(lambda: flash_attention(q, k, v, 0.1), [q, k, v])
+
+
 def _logp_batch(n, s, seed):
     """logps [n, s], and labels as a slice of a wider tensor."""
     g = _gen(seed)

@@ -96,6 +96,25 @@ def test_window_backward_reads_what_came_back(monkeypatch, layout, source):
         assert bwd[i] % 16 == 0 and (bwd[i] == got.data_ptr()) == (layout == "contiguous")
 
 
+@pytest.mark.parametrize("S", [128, 200])
+def test_causal_backward_under_hooks(monkeypatch, S):
+    """The log-sum-exp's padded buffer comes back, whatever the length."""
+    from auspex_soup_demo_b200.kernels import attention
+
+    rec = _Calls(monkeypatch, "contiguous")
+    monkeypatch.setattr(_lib, "scratch", lambda dev, n: torch.empty(max(n, 16), dtype=torch.uint8))
+    monkeypatch.setattr(attention, "_check", lambda q, k, v: (*q.shape[:2], k.shape[1], *q.shape[2:]))
+    q, k, v = (torch.randn(2, S, h, 128).bfloat16().transpose(1, 2).requires_grad_(True) for h in (4, 2, 2))
+    with rec.hooks():
+        out = attention.flash_attention(q, k, v, 0.1)
+    out.backward(torch.zeros_like(out))
+    bwd = rec.calls["soup_attention_bwd"]
+    assert rec.back[4].shape == (2, 4, -(-S // 128) * 128) and bwd[8] == rec.back[4].data_ptr()
+    for i in range(3):
+        assert bwd[2 * i] == rec.back[i].data_ptr()
+        assert list(bwd[2 * i + 1]) == list(rec.back[i].stride()[:3])
+
+
 @pytest.mark.parametrize("layout", LAYOUTS)
 def test_preference_backward_reads_what_came_back(monkeypatch, layout):
     rec = _Calls(monkeypatch, layout)
