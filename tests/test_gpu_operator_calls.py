@@ -316,3 +316,55 @@ def test_head_token_logps_of_no_tokens(shape, trained):
     leaves = [t for t in (h, w) if t.requires_grad]
     for t, g in zip(leaves, torch.autograd.grad(lp.sum(), leaves)):
         assert g.shape == t.shape and not g.any()
+
+
+# ------------------------------------------------------------------- large vocabulary ----
+def test_head_token_logps_at_offsets_past_32_bits():
+    """15000 tokens x 151936: the kept exponentials pass 2^31 elements. Rows at both ends
+    against 64 bits; tolerances as in the tests of small sizes: fp32 accumulation of 64
+    products, lse in fp32, dz's factor and the result rounded to bf16 (2^-8 each)."""
+    n, d, v = 15000, 64, 151936
+    g = _gen(40)
+    w = (torch.randn(v, d, generator=g, device=DEV) * 0.05).bfloat16()
+    lab = torch.randint(0, v, (n,), generator=g, device=DEV)
+    lab[5::97] = IGNORE
+    h = torch.randn(n, d, generator=g, device=DEV).bfloat16().requires_grad_(True)
+    up = torch.randn(n, generator=g, device=DEV)
+    lp, ent = kernels.head_token_logps(h, w, lab)
+    (dh,) = torch.autograd.grad(lp, [h], up)
+    assert _lib.device_error(torch.device(DEV)) == 0
+    rows = torch.cat([torch.arange(20, device=DEV), torch.arange(n - 300, n, device=DEV)])
+    z = h.detach()[rows].double() @ w.double().t()
+    lsm = torch.log_softmax(z, 1)
+    keep = lab[rows] != IGNORE
+    idx = lab[rows].clamp(min=0)[:, None]
+    want = torch.where(keep, lsm.gather(1, idx)[:, 0], torch.zeros_like(lsm[:, 0]))
+    mag = float((h.detach()[rows].double().abs() @ w.double().abs().t()).max())
+    tol = 4 * 8 * 2.0 ** -24 * mag + 2.0 ** -20 * (1 + want.abs())
+    assert bool(((lp[rows].double() - want).abs() <= tol).all())
+    p = lsm.exp()
+    we = torch.where(keep, -(p * lsm).sum(1), torch.zeros_like(want))
+    assert bool(((ent[rows].double() - we).abs() <= 16 * tol).all())
+    gk = torch.where(keep, up[rows].double(), torch.zeros_like(want))
+    p.scatter_add_(1, idx, -torch.ones_like(idx, dtype=torch.float64))  # -dz / gk
+    wd = -(p @ w.double()) * gk[:, None]
+    u = 2.0 ** -8 * 1.02
+    bound = u * (p.abs() @ w.double().abs()) * gk.abs()[:, None] + 2.0 ** -8 * wd.abs() + 1e-7
+    assert bool(((dh[rows].double() - wd).abs() <= bound).all())
+
+
+def test_padded_batch_in_a_graph():
+    """Under capture no value of the padding mask is looked at: it is applied by SDPA."""
+    a = _model("soup")
+    ids = torch.randint(0, 1000, (2, 150), generator=_gen(41), device=DEV)
+    mask = torch.ones(2, 150, dtype=torch.long, device=DEV)
+    mask[0, :30] = 0
+    with torch.no_grad():
+        want = a(ids, attention_mask=mask).logits[mask.bool()].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = a(ids, attention_mask=mask).logits
+        graph.replay()
+        torch.cuda.synchronize()
+    assert torch.equal(out[mask.bool()], want)

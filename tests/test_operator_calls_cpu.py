@@ -441,3 +441,39 @@ def test_mlp_that_cannot_keep_8_bits_says_so(keep8):
         y = qlora.LoRAProjectionGroup.mlp(Group(), x, lambda h: h, False, keep8)
     assert y[0, 0] == (2.0 if keep8 else 3.0)
     assert [w for w in seen if "CHECKPOINT_8BIT" in str(w.message)] != [] if keep8 else not seen
+
+
+# ------------------------------------------------------- the exponential on the FMA pipe ----
+def test_cubic_exponential_over_its_range():
+    """The window backward's 2^x on the FMA pipe, restated in numpy with the source's
+    constants: 7.5e-5 of the value for -126 <= x <= 127, never below 2^-126."""
+    import os
+    import re
+
+    import numpy as np
+
+    src = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", "attention_window.cu")).read()
+    body = src[src.index("void exp2_fma("):]
+    body = body[:body.index("\n}")]
+    c3, c2, c1, c0 = (float(x) for x in dict.fromkeys(re.findall(r"f2_pack\((0\.\d+)f", body)))
+    f32 = np.float32
+    x = np.concatenate([np.linspace(-126, 127, 400001), np.arange(-126, 128), np.arange(-126, 127) + 0.5,
+                        [-1e30, -200.0, -126.5]]).astype(f32)
+    lo = np.maximum(x, f32(-126))
+    magic = f32(12582912 + 127)
+    t = (lo + magic).astype(f32)
+    f = (lo.astype(np.float64) - (t - magic).astype(f32)).astype(f32)  # exact: n is near x
+
+    def fma(a, b, c):  # one rounding: the product of two fp32 values is exact in 64 bits
+        return (a.astype(np.float64) * b.astype(np.float64) + np.float64(f32(c))).astype(f32)
+
+    y = fma(f, np.full_like(f, c3), c2)
+    y = fma(f, y, c1)
+    y = fma(f, y, c0)
+    scale = (t.view(np.uint32) << np.uint32(23)).view(f32)
+    with np.errstate(over="ignore"):
+        got = (y * scale).astype(np.float64)
+    want = np.exp2(lo.astype(np.float64))
+    assert np.abs(f).max() <= 0.5
+    assert (np.abs(got / want - 1) <= 7.6e-5).all()
+    assert (got >= 2.0 ** -126 * (1 - 7.6e-5)).all()
