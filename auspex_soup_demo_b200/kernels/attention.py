@@ -257,10 +257,10 @@ def soup_attention(module, query, key, value, attention_mask, dropout: float = 0
             return window_attention(query, key, value, float(scale), window, sinks), None
         if hides or 1 < n_q < n_k:  # SDPA's own causal mask takes the queries for the first tokens
             k_pos = torch.arange(n_k, device=query.device)
-            dist = k_pos[n_k - n_q:, None] - k_pos  # of the queries alone: [n_q, n_k]
-            attention_mask = dist >= 0
+            q_pos = k_pos[n_k - n_q:, None]
+            attention_mask = k_pos <= q_pos  # [n_q, n_k], one byte a pair
             if hides:
-                attention_mask &= (dist < window) | (k_pos < sinks)
+                attention_mask &= (k_pos > q_pos - window) | (k_pos < sinks)
             attention_mask = attention_mask[None, None]
             is_causal = False  # in the mask
     if not _supported(module, query, key, value, attention_mask, dropout):

@@ -477,3 +477,25 @@ def test_cubic_exponential_over_its_range():
     assert np.abs(f).max() <= 0.5
     assert (np.abs(got / want - 1) <= 7.6e-5).all()
     assert (got >= 2.0 ** -126 * (1 - 7.6e-5)).all()
+
+
+def test_window_mask_takes_a_byte_a_pair():
+    """A whole sequence off the kernels: no [n, n] tensor of distances beside the mask."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from auspex_soup_demo_b200.kernels.attention import soup_attention
+
+    wide = []
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            for t in out if isinstance(out, (tuple, list)) else (out,):
+                if isinstance(t, torch.Tensor) and not t.is_floating_point() and t.numel() >= 500 * 500:
+                    wide.append(t.element_size())
+            return out
+
+    q = torch.randn(1, 1, 500, 16)
+    with Seen():
+        soup_attention(_Layer(1), q, q, q, None, sliding_window=30)
+    assert wide and max(wide) == 1
