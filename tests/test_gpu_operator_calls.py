@@ -368,3 +368,40 @@ def test_padded_batch_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
     assert torch.equal(out[mask.bool()], want)
+
+
+# ------------------------------------------------------------------------ small sizes ----
+@pytest.mark.parametrize("n,d,v", [(1, 8, 1), (3, 8, 2), (2, 16, 9), (257, 8, 3), (1, 8, 70000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("trained", ["states", "head", "both"])
+def test_head_token_logps_smallest_sizes(n, d, v, dtype, trained):
+    """fp32 accumulation of 8 or 16 products and an lse in fp32; gradients through factors
+    rounded to bf16 (2^-8; twice for the head and for fp16's bf16 copy of it)."""
+    g = _gen(n + v)
+    h = torch.randn(n, d, generator=g, device=DEV).to(dtype).requires_grad_(trained != "head")
+    w = torch.randn(v, d, generator=g, device=DEV).to(dtype).requires_grad_(trained != "states")
+    lab = torch.randint(0, v, (n,), generator=g, device=DEV)
+    up = torch.randn(n, generator=g, device=DEV)
+    lp, ent = kernels.head_token_logps(h, w, lab)
+    leaves = [t for t in (h, w) if t.requires_grad]
+    grads = dict(zip(map(id, leaves), torch.autograd.grad(lp, leaves, up)))
+    h6, w6 = h.detach().double(), w.detach().double()
+    z = h6 @ w6.t()
+    lsm = torch.log_softmax(z, 1)
+    p = lsm.exp()
+    want = lsm.gather(1, lab[:, None])[:, 0]
+    mag = float((h6.abs() @ w6.abs().t()).max())
+    tol = 16 * 2.0 ** -24 * mag + 2.0 ** -20 * (1 + want.abs())
+    assert bool(((lp.double() - want).abs() <= tol).all())
+    assert bool(((ent.double() + (p * lsm).sum(1)).abs() <= 40 * tol.max()).all())  # |z - lse| below 40
+    dz = -p
+    dz.scatter_add_(1, lab[:, None], torch.ones_like(want)[:, None])
+    dz = dz * up.double()[:, None]
+    u = 2 * 2.0 ** -8 * 1.02
+    # dz itself is off by the logits' error: p (1 - p) of it
+    slack = (p * up.double().abs()[:, None] + dz.abs()) * 4 * tol.max()
+    for t, a, size in ((h, dz @ w6, (dz.abs() * u + slack) @ w6.abs()),
+                       (w, dz.t() @ h6, (dz.abs() * u + slack).t() @ h6.abs())):
+        if id(t) in grads:
+            got = grads[id(t)].double()
+            assert bool(((got - a).abs() <= size + 2.0 ** -8 * a.abs() + 1e-7).all())
