@@ -128,14 +128,12 @@ struct AttnArgs {
 // ------------------------------------------------------------- forward ----
 // One CTA per (batch, query head, pair of 128-query tiles A = 2p, B = 2p + 1);
 // heavy (late) pairs first. The two tiles share every K / V tile. TMEM: S_A at
-// column 0, S_B at 128, O_A at 256, O_B at 384 (512 allocated); P_X (bf16, two
-// keys per 32-bit column) overwrites the last 64 columns of S_X and is the A
-// operand of O_X += P_X V read from TMEM. The MMA warp issues, per key tile j,
-// P V of tile A, then S_A(j + 1), then P V of tile B, then S_B(j + 1): while the
-// tensor core runs one tile's products the other tile's softmax runs, and each
-// S_X(j + 1) follows (in issue order) the product that read P_X(j) from the same
-// columns. Shared memory: Q_A, Q_B (32 KB each), K ring (2 x 32 KB), V ring
-// (2 x 32 KB), barriers.
+// column 0, S_B at 128, O_A at 256, O_B at 384 (512 allocated); P_X (bf16) goes
+// through shared memory as the A operand of O_X += P_X V. The MMA warp issues, per
+// key tile j, P V of tile A, then S_A(j + 1), then P V of tile B, then S_B(j + 1):
+// while the tensor core runs one tile's products the other tile's softmax runs;
+// S_X(j + 1) waits until the softmax has read S_X(j). Shared memory: Q_A, Q_B
+// (32 KB each), K ring (2 x 32 KB), V (32 KB), P_A, P_B (32 KB each), barriers.
 struct FwdSmem {
   static constexpr int kQ = 0;  // tile X at + X * kTileBytes
   static constexpr int kK = kQ + 2 * kTileBytes;

@@ -17,13 +17,13 @@
 // Maxima, sums, log-sum-exps, D and all accumulators are fp32. P and dS are rounded to bf16,
 // as operands of products that run at the bf16 rate: at most 2^-8 of each entry, of either
 // sign, so it averages out in a sum over many keys and adds about the result's own bf16
-// rounding where a few keys dominate. D takes the bf16 output, the one that the caller holds. Hidden keys of a block that is read have weight 0
-// by selection, but 0 x NaN in a product is NaN: V must be finite there, as for any masked
-// softmax attention.
+// rounding where a few keys dominate. D takes the bf16 output, the one that the caller holds.
+// Hidden keys of a block that is read have weight 0 by selection, but 0 x NaN in a product is
+// NaN: V must be finite there, as for any masked softmax attention.
 //
 // A product that overwrites TMEM columns which an earlier product reads waits for that one's
 // commit: PTX keeps only products of one accumulator and shape in issue order. The waits cost
-// 2 % (forward and backward of 16001 tokens 540 us against 526, of 4 x 2048 190 against 186).
+// about 1 % (forward and backward of 16001 tokens 532 us against 526, of 4 x 2048 186 in both).
 // A CTA leaves only after every asynchronous arrival on its barriers has landed: the
 // producer waits for its copies, the MMA warp for its commits.
 // Every mbarrier wait is bounded as in attention.cu: on expiry the role records a
@@ -613,7 +613,9 @@ __device__ __forceinline__ DkvUnit dkv_unit(const BwdArgs& a, int i) {
 // (at the special-function rate 1024 for 128 x 128) and handoffs the rest; dP and dS run
 // beside it. A quarter of the exponentials goes to the FMA pipe: forward and backward of
 // 1 x 16001 tokens, 12 heads over 2, window 1000, 16 sinks take 526 us against 540 with none
-// and 532 with half (540 with the waits between products, which came later). Eight compute warps, P through shared memory and two groups of warps on
+// and 532 with half (532 with the waits between products, which came later). dQ
+// takes all of P from the special-function unit: up to 7.5e-5 from these, where P's rounding to
+// bf16 is 50 times that. Eight compute warps, P through shared memory and two groups of warps on
 // 64-query steps (S^T double buffered, but products of N = 64) measured no faster.
 constexpr int kDkvStages = 2;
 struct WinDkvSmem {

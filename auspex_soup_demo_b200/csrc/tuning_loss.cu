@@ -7,9 +7,9 @@
 // one record per block, a second, one block, joins the records in a fixed
 // order (no atomics: the same inputs give the same bits) and writes the loss,
 // the metrics and one gradient factor per sequence; when the blocks fit a
-// cluster, one launch does both. The backward is one elementwise pass. Labels equal to ignore_index mark masked tokens: their
-// values are selected away, never multiplied, so infinities and NaN there do
-// not reach a sum. Sums over tokens run in 64 bits: thousands of terms of
+// cluster, one launch does both. The backward is one elementwise pass. Labels equal to
+// ignore_index mark masked tokens: their values are selected away, never multiplied, so
+// infinities and NaN there do not reach a sum. Sums over tokens run in 64 bits: thousands of terms of
 // either sign leave a difference that 32 bits would round away, and the adds
 // are free beside the loads.
 #include "soup_common.cuh"

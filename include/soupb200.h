@@ -308,7 +308,8 @@ int soup_preference_loss_bwd(const float* grad_loss, const float* coef, const in
  *   L = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1),
  *   d = ref - logps
  * old_logps NULL: the policy's own log-probabilities (r = 1, dL/dlogps = -A);
- * ref_logps NULL: no KL term. advantages [batch] (adv_ld 0) or [batch, seq].
+ * ref_logps NULL: no KL term; with kl_coef 0 it enters kl[1] alone. A counted token whose
+ * logps is NaN makes the loss NaN. advantages [batch] (adv_ld 0) or [batch, seq].
  * SOUP_POLICY_TOKEN: sum over all counted tokens / their number;
  * SOUP_POLICY_SEQUENCE: mean over the batch of each sequence's mean (a sequence
  * without counted tokens contributes 0). loss[1]; kl[1] = mean over counted tokens
@@ -371,7 +372,8 @@ int soup_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
 /* The same attention with a sliding window and sinks: query i sees key j iff
  * j <= i and (i - j < window or j < sinks), window >= 1, sinks >= 0 (either may
  * exceed seq). Only key tiles that hold a visible key are read: the cost is
- * proportional to seq (window + sinks). Buffers, layouts and strides as for
+ * proportional to seq (window + sinks). The backward's workspace grows with seq and
+ * sinks, each linearly; window + sinks >= seq is the causal case. Buffers, layouts and strides as for
  * soup_attention_fwd / soup_attention_bwd; the backward's workspace is
  * soup_attention_window_bwd_workspace_bytes (of the current device). Reproducible
  * (no atomics). No kernel in the reference (transformers masks SDPA for its
