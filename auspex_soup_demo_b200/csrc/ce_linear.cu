@@ -28,6 +28,7 @@
 
 #include <atomic>
 
+#include "multi_lora.cuh"
 #include "soup_common.cuh"
 #include "tc_gemm.cuh"
 
@@ -1861,7 +1862,72 @@ static int check_in_dtype(const char* fn, int in_dtype, const void* weight_bwd, 
   return SOUP_OK;
 }
 
+static int gemm_bf16_run(const void* a, int64_t lda, int a_mn_major, const void* b, int64_t ldb,
+                         int b_mn_major, const void* a2, int64_t lda2, const void* b2, int64_t ldb2,
+                         int64_t r, const uint64_t* k2_mask, const void* bias, void* c, int64_t ldc,
+                         int c_dtype, int64_t m, int64_t n, int64_t k, float alpha, int accumulate,
+                         cudaStream_t stream) {
+  if (!a || !b || !c || m <= 0 || n <= 0 || k <= 0 || m > (1 << 30) || n > (1 << 30) ||
+      k > (1 << 30) || r < 0 || r > 4096 || (r > 0 && (!a2 || !b2))) {
+    set_last_error("soup_gemm_bf16: bad arguments");
+    return SOUP_ERR_INVALID;
+  }
+  if (c_dtype != SOUP_F32 && c_dtype != SOUP_BF16) {
+    set_last_error("soup_gemm_bf16: C dtype must be F32 or BF16");
+    return SOUP_ERR_INVALID;
+  }
+  if ((a_mn_major ? lda < m : lda < k) || (b_mn_major ? ldb < n : ldb < k) || ldc < n ||
+      (r > 0 && ((a_mn_major ? lda2 < m : lda2 < r) || (b_mn_major ? ldb2 < n : ldb2 < r)))) {
+    set_last_error("soup_gemm_bf16: leading dimension too small");
+    return SOUP_ERR_INVALID;
+  }
+  if (!tma_ok(a, lda) || !tma_ok(b, ldb) || (r > 0 && (!tma_ok(a2, lda2) || !tma_ok(b2, ldb2)))) {
+    set_last_error("soup_gemm_bf16: operands need 16-byte aligned rows");
+    return SOUP_ERR_UNSUPPORTED;
+  }
+  CUtensorMap ma, mb, ma2, mb2;
+  int rc;
+  if ((rc = make_operand_map(&ma, a, a_mn_major != 0, m, k, lda, BM))) return rc;
+  if ((rc = make_operand_map(&mb, b, b_mn_major != 0, n, k, ldb, b_box_rows()))) return rc;
+  if (r > 0) {
+    // the rank-r segment: boxes are 64 deep along K; TMA fills the columns
+    // (K-major) or rows (MN-major) beyond r with zeros
+    if ((rc = make_operand_map(&ma2, a2, a_mn_major != 0, m, r, lda2, BM))) return rc;
+    if ((rc = make_operand_map(&mb2, b2, b_mn_major != 0, n, r, ldb2, b_box_rows()))) return rc;
+  } else {
+    ma2 = ma;
+    mb2 = mb;
+  }
+  const int es = c_dtype == SOUP_BF16 ? 2 : 4;
+  const int vec = (aligned16(c) && (ldc * es) % 16 == 0) ? 1 : 0;
+  CUtensorMap mc = ma;
+  const int tma = (c_dtype == SOUP_BF16 && !accumulate && vec &&
+                   make_store_map(&mc, c, n, m, ldc) == SOUP_OK) ? 1 : 0;
+  EpiStore<kBN>::Params ep{c, ldc, 0, nullptr, alpha, c_dtype == SOUP_BF16 ? 1 : 0, accumulate ? 1 : 0,
+                           vec, (int)m, (int)n, static_cast<const bf16*>(bias), tma};
+  const int mt = m_tiles(m), nt = (int)((n + kBN - 1) / kBN);
+  const int kb1 = (int)((k + BK - 1) / BK), kb2 = (int)((r + BK - 1) / BK);
+  Sched sc{mt, nt, 1, kb1 + kb2, nt > mt ? 0 : 1, kb2};
+  if (k2_mask) {
+    sc.k2_mask = k2_mask;
+    sc.no_sk = 1;
+  }
+  using E = EpiStore<kBN>;
+  if (!a_mn_major && !b_mn_major) return launch_gemm<false, false, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
+  if (!a_mn_major && b_mn_major) return launch_gemm<false, true, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
+  if (a_mn_major && !b_mn_major) return launch_gemm<true, false, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
+  return launch_gemm<true, true, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
+}
+
 }  // namespace tc
+
+int gemm_bf16_masked_k2(const void* a, int64_t lda, const void* b, int64_t ldb, bool b_mn, const void* a2,
+                        int64_t lda2, const void* b2, int64_t ldb2, int64_t r, const uint64_t* k2_mask,
+                        const void* bias, void* out, int64_t ldo, int64_t m, int64_t n, int64_t k,
+                        cudaStream_t stream) {
+  return tc::gemm_bf16_run(a, lda, 0, b, ldb, b_mn ? 1 : 0, a2, lda2, b2, ldb2, r, k2_mask, bias, out, ldo, SOUP_BF16,
+                           m, n, k, 1.0f, 0, stream);
+}
 }  // namespace soup
 
 using namespace soup;
@@ -2416,54 +2482,9 @@ int soup_gemm_bf16(const void* a, int64_t lda, int a_mn_major, const void* b, in
 int soup_gemm_bf16_lora(const void* a, int64_t lda, int a_mn_major, const void* b, int64_t ldb,
                         int b_mn_major, const void* a2, int64_t lda2, const void* b2, int64_t ldb2,
                         int64_t r, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t m,
-                        int64_t n, int64_t k, float alpha, int accumulate, void* stream_) {
-  if (!a || !b || !c || m <= 0 || n <= 0 || k <= 0 || m > (1 << 30) || n > (1 << 30) ||
-      k > (1 << 30) || r < 0 || r > 4096 || (r > 0 && (!a2 || !b2))) {
-    set_last_error("soup_gemm_bf16: bad arguments");
-    return SOUP_ERR_INVALID;
-  }
-  if (c_dtype != SOUP_F32 && c_dtype != SOUP_BF16) {
-    set_last_error("soup_gemm_bf16: C dtype must be F32 or BF16");
-    return SOUP_ERR_INVALID;
-  }
-  if ((a_mn_major ? lda < m : lda < k) || (b_mn_major ? ldb < n : ldb < k) || ldc < n ||
-      (r > 0 && ((a_mn_major ? lda2 < m : lda2 < r) || (b_mn_major ? ldb2 < n : ldb2 < r)))) {
-    set_last_error("soup_gemm_bf16: leading dimension too small");
-    return SOUP_ERR_INVALID;
-  }
-  if (!tma_ok(a, lda) || !tma_ok(b, ldb) || (r > 0 && (!tma_ok(a2, lda2) || !tma_ok(b2, ldb2)))) {
-    set_last_error("soup_gemm_bf16: operands need 16-byte aligned rows");
-    return SOUP_ERR_UNSUPPORTED;
-  }
-  CUtensorMap ma, mb, ma2, mb2;
-  int rc;
-  if ((rc = make_operand_map(&ma, a, a_mn_major != 0, m, k, lda, BM))) return rc;
-  if ((rc = make_operand_map(&mb, b, b_mn_major != 0, n, k, ldb, b_box_rows()))) return rc;
-  if (r > 0) {
-    // the rank-r segment: boxes are 64 deep along K; TMA fills the columns
-    // (K-major) or rows (MN-major) beyond r with zeros
-    if ((rc = make_operand_map(&ma2, a2, a_mn_major != 0, m, r, lda2, BM))) return rc;
-    if ((rc = make_operand_map(&mb2, b2, b_mn_major != 0, n, r, ldb2, b_box_rows()))) return rc;
-  } else {
-    ma2 = ma;
-    mb2 = mb;
-  }
-  const int es = c_dtype == SOUP_BF16 ? 2 : 4;
-  const int vec = (aligned16(c) && (ldc * es) % 16 == 0) ? 1 : 0;
-  CUtensorMap mc = ma;
-  const int tma = (c_dtype == SOUP_BF16 && !accumulate && vec &&
-                   make_store_map(&mc, c, n, m, ldc) == SOUP_OK) ? 1 : 0;
-  EpiStore<kBN>::Params ep{c, ldc, 0, nullptr, alpha, c_dtype == SOUP_BF16 ? 1 : 0, accumulate ? 1 : 0,
-                           vec, (int)m, (int)n, static_cast<const bf16*>(bias), tma};
-  const int mt = m_tiles(m), nt = (int)((n + kBN - 1) / kBN);
-  const int kb1 = (int)((k + BK - 1) / BK), kb2 = (int)((r + BK - 1) / BK);
-  Sched sc{mt, nt, 1, kb1 + kb2, nt > mt ? 0 : 1, kb2};
-  cudaStream_t stream = as_stream(stream_);
-  using E = EpiStore<kBN>;
-  if (!a_mn_major && !b_mn_major) return launch_gemm<false, false, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
-  if (!a_mn_major && b_mn_major) return launch_gemm<false, true, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
-  if (a_mn_major && !b_mn_major) return launch_gemm<true, false, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
-  return launch_gemm<true, true, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
+                        int64_t n, int64_t k, float alpha, int accumulate, void* stream) {
+  return soup::tc::gemm_bf16_run(a, lda, a_mn_major, b, ldb, b_mn_major, a2, lda2, b2, ldb2, r, nullptr, bias, c, ldc,
+                             c_dtype, m, n, k, alpha, accumulate, as_stream(stream));
 }
 
 int soup_gemm_bf16_lora_dswiglu(const void* a, int64_t lda, const void* b, int64_t ldb,

@@ -287,6 +287,22 @@ struct Sched {
   const int* dyn_rows = nullptr;
   int dyn_k = 0;
   int dyn_unit = 1;
+  // optional words of 256-row tiles of A (written by an earlier kernel on the
+  // stream): a tile's second segment then is the blocks of its set bits, in
+  // ascending order, instead of all kb2 (at most 64). With splits == 1 and no
+  // stream-K tail.
+  const uint64_t* k2_mask = nullptr;
+  __device__ __forceinline__ uint64_t k2_word(int mt256) const { return k2_mask ? k2_mask[mt256] : 0; }
+  __device__ __forceinline__ int k_end(int kb1, uint64_t word) const {
+    return k2_mask ? kb_total - kb2 + __popcll(word) : kb1;
+  }
+  // k offset of block kb of a tile; `word` holds the tile's rank blocks still to come
+  __device__ __forceinline__ int k_elem_of(int kb, uint64_t& word) const {
+    if (!k2_mask || !second(kb)) return k_elem(kb);
+    const int b = __ffsll(static_cast<long long>(word)) - 1;
+    word &= word - 1;
+    return b * BK;
+  }
   __device__ __forceinline__ void apply_dyn() {
     const int n = *dyn_rows;
     const int t = n > 0 ? (n + dyn_unit - 1) / dyn_unit : 1;
@@ -577,6 +593,8 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
         int mt, nt, ks, kb0, kb1;
         sched.decode(u, mt, nt, ks);
         sched.k_range(ks, kb0, kb1);
+        uint64_t word = sched.k2_word(mt >> 1);
+        kb1 = sched.k_end(kb1, word);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1u;
@@ -588,7 +606,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
           const uint32_t a_dst = sbase + s * L::kStageBytes;
           const uint32_t b_dst = a_dst + L::kABytes;
           mbar_arrive_expect_tx(full_bar(s), L::kStageBytes);
-          const int k0 = sched.k_elem(kb);
+          const int k0 = sched.k_elem_of(kb, word);
           const bool seg2 = sched.second(kb);
           const CUtensorMap* ma = seg2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mb = seg2 ? &tma_b2 : &tma_b;
@@ -630,6 +648,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
         int mt, nt, ks, kb0, kb1;
         sched.decode(u, mt, nt, ks);
         sched.k_range(ks, kb0, kb1);
+        kb1 = sched.k_end(kb1, sched.k2_word(mt >> 1));
         const uint32_t acc = lt & 1u;
         const uint32_t acc_ph = (lt >> 1) & 1u;
         if (!bounded_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag, err, kErrWaitMma, wait_ns)) {
@@ -1003,7 +1022,9 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
         const Unit w = sched_unit(sched, cluster, n_clusters, i);
         const int a_row = w.mt * 2 * BM + static_cast<int>(rank) * BM;
         const int b_row = w.nt * BN + static_cast<int>(rank) * BNH;
-        for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+        uint64_t word = sched.k2_word(w.mt);
+        const int kb1 = sched.k_end(w.kb1, word);
+        for (int kb = w.kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1u;
           if (!bounded_wait(empty_bar(s), ph ^ 1u, abort_flag, err, kErrWaitProducer, wait_ns)) {
@@ -1015,7 +1036,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
           const uint32_t b_dst = a_dst + L::kABytes;
           const uint32_t fb = cluster_addr(full_bar(s), 0);
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), kPairBytes);
-          const int k0 = sched.k_elem(kb);
+          const int k0 = sched.k_elem_of(kb, word);
           const bool seg2 = sched.second(kb);
           const CUtensorMap* ma = seg2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mb = seg2 ? &tma_b2 : &tma_b;
@@ -1056,7 +1077,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
       bool issued = false;
       for (int i = 0; i < n_my && ok; ++i, ++lt) {
         const Unit w = sched_unit(sched, cluster, n_clusters, i);
-        const int kb0 = w.kb0, kb1 = w.kb1;
+        const int kb0 = w.kb0, kb1 = sched.k_end(w.kb1, sched.k2_word(w.mt));
         const uint32_t acc = lt & 1u;
         const uint32_t acc_ph = (lt >> 1) & 1u;
         if (!bounded_wait<true>(tempty_bar(acc), acc_ph ^ 1u, abort_flag, err, kErrWaitMma, wait_ns)) {

@@ -1,7 +1,9 @@
 """sm_100a fused ops behind the reference's kernel-package names.
 
 Mirrors the export list of the reference's ``solution/kernels/__init__.py:3-51``,
-and adds the operators of preference and policy tuning (no counterpart there).
+and adds (no counterpart there) the operators of preference and policy tuning,
+norms of queries and keys with their rotation, positions of several axes, and
+projections with several adapters.
 """
 
 from .attention import window_attention
@@ -13,6 +15,8 @@ from .chunked_ce import (
     patch_soup_chunked_loss,
     fused_linear_cross_entropy,
 )
+from .multi_lora import multi_lora_linear
+from .qk_norm_rope import apply_multi_axis_rope, apply_qk_norm_rope, rope_axes
 from .rmsnorm import (
     _rms_norm_fwd_kernel,
     _rms_norm_bwd_dx_kernel,
@@ -70,4 +74,8 @@ __all__ = [
     "window_attention",
     "swiglu_8bit",
     "quantize_8bit",
+    "apply_qk_norm_rope",
+    "apply_multi_axis_rope",
+    "rope_axes",
+    "multi_lora_linear",
 ]

@@ -44,7 +44,8 @@ const char* soup_last_error(void);
  * synchronises the given stream. Codes: 0x101 producer, 0x102 MMA issuer,
  * 0x103 epilogue wait expired, 0x104 a stream-K partial never became
  * ready; 0x131-0x133 the producer, MMA issuer and compute warps of the window
- * attention, 0x134 its shared memory too small. No counterpart in the reference (its Triton kernels have no
+ * attention, 0x134 its shared memory too small; 0x141-0x143 the producer, MMA issuer
+ * and epilogue of the adapters' rank products, 0x144 their shared memory. No counterpart in the reference (its Triton kernels have no
  * device-side waits). */
 int soup_device_error(void* stream, int* out_code);
 
@@ -149,6 +150,83 @@ int soup_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_
               const int64_t* k_out_strides, int64_t hk, const void* cos, const void* sin,
               int64_t cos_sb, int64_t cos_ss, int64_t batch, int64_t seq, int64_t head_dim,
               int dtype, int cos_dtype, int inverse, void* stream);
+
+/* ---- Norms of queries and keys with their rotation ---------------------------
+ * No counterpart in the reference (its RoPE takes rows as they are). One launch
+ * normalises every head's row of q and k (n = x * w / sqrt(mean(x^2) + eps); both
+ * weights [head_dim], or both NULL for a rotation alone) and rotates its halves.
+ * Angles come from cos / sin tables (table_dtype; first head_dim / 2 entries at
+ * [b * table_sb + s * table_ss]), or, with cos and sin NULL, from positions:
+ * positions[axes[i] * pos_sa + b * pos_sb + s * pos_ss] * inv_freq[i], int32 or
+ * (positions_64) int64, reduced in 64 bits; axes [head_dim / 2] is host memory.
+ * inverse != 0 rotates back (without weights: the backward of a rotation alone).
+ * head_dim even, at most 512; strides {b, h, s} in elements, last dim contiguous.
+ * soup_qk_norm_rope_bwd: gradients of q, k and, where not NULL, of the weights
+ * (w_dtype), summed over tokens and heads in 32 bits in a fixed order through the
+ * workspace; workspace may be NULL without weight gradients. */
+int soup_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int64_t hq,
+                      const void* k, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
+                      int64_t hk, const void* q_weight, const void* k_weight, float eps, const void* cos,
+                      const void* sin, int64_t table_sb, int64_t table_ss, int table_dtype, const void* positions,
+                      int positions_64, int64_t pos_sa, int64_t pos_sb, int64_t pos_ss, const float* inv_freq,
+                      const uint8_t* axes, int64_t batch, int64_t seq, int64_t head_dim, int dtype, int w_dtype,
+                      int inverse, void* stream);
+size_t soup_qk_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t hq, int64_t hk,
+                                             int64_t head_dim);
+int soup_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_out_strides, const void* q, const int64_t* q_strides,
+                          void* dq, const int64_t* dq_strides, int64_t hq, const void* dk_out,
+                          const int64_t* dk_out_strides, const void* k, const int64_t* k_strides, void* dk,
+                          const int64_t* dk_strides, int64_t hk, const void* q_weight, const void* k_weight,
+                          float eps, void* dq_weight, void* dk_weight, const void* cos, const void* sin,
+                          int64_t table_sb, int64_t table_ss, int table_dtype, const void* positions,
+                          int positions_64, int64_t pos_sa, int64_t pos_sb, int64_t pos_ss, const float* inv_freq,
+                          const uint8_t* axes, int64_t batch, int64_t seq, int64_t head_dim, int dtype, int w_dtype,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- A projection with several adapters ----------------------------------------
+ * No counterpart in the reference (one adapter, peft). y_t = W x_t + bias + s_a B_a A_a
+ * x_t, a = ids[t / tokens_per_id] (int32, or int64 with ids_64; an id outside
+ * [0, adapters) means none). bf16: x [tokens, k], weight [n, k], bias [n] or NULL,
+ * lora_a [adapters, rank, k], lora_b [n, adapters, rank], y [tokens, n]; scales fp32
+ * [adapters]; fp32 accumulation, the rank products rounded to bf16 between. n, k and
+ * adapters * rank are multiples of 8, adapters * rank <= 4096, tokens <= 2^21. The
+ * state (soup_multi_lora_state_bytes, the caller's) holds the rank products and is what
+ * the backward needs of the forward.
+ * soup_multi_lora_bwd: dx [tokens, k] bf16, da and db (fp32 or bf16, laid out as lora_a
+ * and lora_b; rows of adapters without tokens are 0), each where not NULL; x is read
+ * for da alone. workspace for dx or da. Bitwise reproducible. */
+size_t soup_multi_lora_state_bytes(int64_t tokens, int64_t adapters, int64_t rank);
+int soup_multi_lora_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias,
+                        const void* lora_a, const void* lora_b, const float* scales, const void* ids, int ids_64,
+                        int64_t tokens_per_id, int64_t tokens, int64_t n, int64_t k, int64_t adapters, int64_t rank,
+                        void* y, int64_t ldy, void* state, size_t state_bytes, void* stream);
+size_t soup_multi_lora_bwd_workspace_bytes(int64_t tokens, int64_t adapters, int64_t rank);
+int soup_multi_lora_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                        const void* lora_a, const void* lora_b, const float* scales, const void* ids, int ids_64,
+                        int64_t tokens_per_id, int64_t tokens, int64_t n, int64_t k, int64_t adapters, int64_t rank,
+                        const void* state, size_t state_bytes, void* dx, int64_t lddx, void* da, int da_dtype,
+                        void* db, int db_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- AdamW over many tensors ---------------------------------------------------
+ * No counterpart in the reference (the HF Trainer's optimiser). The tensors' tables
+ * (addresses, sizes, first state block of each) are host arrays, passed on as launch
+ * arguments; all tensors of a call have one dtype. State block b holds elements
+ * [256 b, 256 b + 256) of exp_avg and exp_avg_sq; a tensor starts at a block of its
+ * own. state_bits 32: fp32 moments. state_bits 8: e4m3 exp_avg and e4m3 square roots
+ * of exp_avg_sq, each block with an fp32 scale (its largest value / 448).
+ * soup_grad_square appends its partial sums of squares (64 bits) at *partials of the
+ * workspace and raises *partials; with partials > 0 the step scales gradients by
+ * min(1, max_norm / (sqrt(sum) + 1e-6)) and writes the norm to norm_out (may be NULL).
+ * step (device fp32) counts completed steps and is raised by the call with last != 0;
+ * ticket is a device int, 0 at first, of the optimiser's own. */
+size_t soup_grad_square_workspace_bytes(int64_t tensors);
+int soup_grad_square(const void* const* grads, const int64_t* sizes, int count, int dtype, void* workspace,
+                     size_t workspace_bytes, int* partials, void* stream);
+int soup_adamw_multi(void* const* params, const void* const* grads, const int64_t* sizes, const int32_t* blocks,
+                     int count, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                     float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps, double weight_decay,
+                     double max_norm, const void* grad_squares, int partials, float* norm_out, float* step,
+                     int* ticket, int last, void* stream);
 
 /* ---- Cross-entropy on a logits buffer ------------------------------------
  * Replaces solution/kernels/chunked_ce.py:32-128
