@@ -19,12 +19,14 @@
 // common growth and decay goes into the scales, so values do not stall where a single
 // step's change is below half a step of the format.
 //
-// A warp takes a block: 8 elements a lane in two 16-byte loads (one for 16-bit
-// tensors), the maxima by shuffles. A CTA takes 2048 elements at a time and a
-// contiguous run of such chunks over all tensors, whose table (pointers and sizes)
+// A warp takes blocks of 256: 8 elements a lane in two 16-byte loads (one for 16-bit
+// tensors), the maxima by one integer reduction each, the arithmetic on packed pairs.
+// A CTA takes 4096 elements at a time and a contiguous run of such chunks over all tensors, whose table (pointers and sizes)
 // comes as a kernel argument, so that a launch needs no copy and can be captured.
 #include <cuda_fp8.h>
 #include <stdio.h>
+
+#include <type_traits>
 
 #include "soup_common.cuh"
 
@@ -33,10 +35,10 @@ namespace {
 
 constexpr int kBlock = 256;              // elements that share a scale
 constexpr int kWarps = 8;
-constexpr int kChunk = kBlock * kWarps;  // elements of a CTA's turn
+constexpr int kBlocksPerWarp = 2;
+constexpr int kChunk = kBlock * kWarps * kBlocksPerWarp;  // elements of a CTA's turn
 constexpr int kThreads = 32 * kWarps;
 constexpr float kE4m3Max = 448.f;
-constexpr float kE4m3Least = 0.001953125f;  // 2^-9
 
 struct Tensor {
   void* p;
@@ -51,6 +53,9 @@ struct Table {
   int count, chunks;
   Tensor t[N];
 };
+
+// resident CTAs of the step's kernel on an SM (85 or 51 registers a thread)
+__host__ __device__ constexpr int ctas_per_sm(bool eight) { return eight ? 3 : 5; }
 
 struct Hyper {
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, lr, decay;  // decay: 1 - lr wd
@@ -82,76 +87,146 @@ __device__ __forceinline__ void chunk_run(int chunks, int& c0, int& c1) {
   c1 = (int)((int64_t)chunks * (blockIdx.x + 1) / gridDim.x);
 }
 
-// 8 consecutive elements as floats; `left` of them exist, the others read 0.
+// Pairs of elements in packed 32-bit arithmetic: one instruction for two.
+__device__ __forceinline__ uint64_t f2_same(float x) { return f2_pack(x, x); }
+
+// Eight consecutive elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int left, bool vec, float (&f)[8]) {
-  constexpr int NE = Vec16<T>::N;
-  if (left >= 8 && vec) {
+struct Raw8 {
+  static constexpr int kWords = 2 * (int)sizeof(T);
+  uint32_t u[kWords];
+  __device__ __forceinline__ void load(const T* p, int left, bool vec) {
+    if (left >= 8 && vec) {
 #pragma unroll
-    for (int i = 0; i < 8; i += NE) {
-      const Vec16<T> q = ld16_stream(p + i);
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p) + i / 4);
+        u[i] = q.x;
+        u[i + 1] = q.y;
+        u[i + 2] = q.z;
+        u[i + 3] = q.w;
+      }
+    } else {
+      union {
+        T t[8];
+        uint32_t w[kWords];
+      } r;
 #pragma unroll
-      for (int e = 0; e < NE; ++e) f[i + e] = Cvt<T>::to_f(q.v[e]);
+      for (int i = 0; i < 8; ++i) r.t[i] = i < left ? p[i] : Cvt<T>::from_f(0.f);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) u[i] = r.w[i];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < left ? Cvt<T>::to_f(p[i]) : 0.f;
   }
+  __device__ __forceinline__ uint64_t pair(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return f2_pack(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      return f2_pack(f.x, f.y);
+    }
+  }
+  __device__ __forceinline__ void set(int i, uint64_t v) {
+    float x, y;
+    f2_unpack(v, x, y);
+    if constexpr (sizeof(T) == 4) {
+      u[2 * i] = __float_as_uint(x);
+      u[2 * i + 1] = __float_as_uint(y);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+      u[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      const __half2 h = __floats2half2_rn(x, y);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, int left, bool vec) const {
+    if (left >= 8 && vec) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4)
+        __stcs(reinterpret_cast<uint4*>(p) + i / 4, make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]));
+    } else {
+      union {
+        T t[8];
+        uint32_t w[kWords];
+      } r;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) r.w[i] = u[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) p[i] = r.t[i];
+    }
+  }
+};
+
+__device__ __forceinline__ uint64_t pair_of_codes(uint2 c, int i) {
+  const uint32_t w = i < 2 ? c.x : c.y;
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * (i & 1))), __NV_E4M3);
+  const float2 v = __half22float2(__half2(h));
+  return f2_pack(v.x, v.y);
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int left, bool vec, const float (&f)[8]) {
-  constexpr int NE = Vec16<T>::N;
-  if (left >= 8 && vec) {
-#pragma unroll
-    for (int i = 0; i < 8; i += NE) {
-      Vec16<T> q;
-#pragma unroll
-      for (int e = 0; e < NE; ++e) q.v[e] = Cvt<T>::from_f(f[i + e]);
-      st16_stream(p + i, q);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) p[i] = Cvt<T>::from_f(f[i]);
-  }
+// Root and reciprocal to 2^-22, subnormals as 0: the IEEE forms cost more instructions
+// than all the rest.
+__device__ __forceinline__ float root_approx(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-
-__device__ __forceinline__ void from_codes(uint2 c, float scale, float (&f)[8]) {
-  const uint32_t w[2] = {c.x, c.y};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
-    const float2 v = __half22float2(__half2(h));
-    f[2 * i] = v.x * scale;
-    f[2 * i + 1] = v.y * scale;
-  }
+__device__ __forceinline__ float recip_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Scale of the warp's block and its codes. Values that are not finite are left out of
-// the maximum: they must not wipe out the other 255.
+// the maximum (they must not wipe out the other 255): fmaxf passes NaN over, and a
+// maximum that is infinite, which no sound step has, is taken again without them. The
+// bits of numbers of 0 or more order as the numbers do, so one integer reduction of the
+// warp gives the maximum.
 template <bool ROOT>
-__device__ __forceinline__ uint2 to_codes(const float (&f)[8], float& scale) {
-  float top = 0.f;
+__device__ __forceinline__ uint2 to_codes(const uint64_t (&f)[4], float& scale) {
+  float v[8], top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(f[i]);
-    top = a <= 3.4028235e38f ? fmaxf(top, a) : top;
+  for (int i = 0; i < 4; ++i) {
+    f2_unpack(f[i], v[2 * i], v[2 * i + 1]);
+    top = fmaxf(top, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
   }
-  top = warp_max(top);
-  scale = top / kE4m3Max;
-  // a subnormal scale has no finite reciprocal: such a block is divided
-  const float inv = scale >= 1.17549435e-38f ? 1.f / scale : 0.f;
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+  if (top > 3.4028235e38f) {  // warp-uniform
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]) <= 3.4028235e38f ? fabsf(v[i]) : 0.f);
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+  }
+  scale = top * (1.f / kE4m3Max);
+  uint64_t y[4];
+  if (scale >= 1.17549435e-38f) {  // warp-uniform
+    const uint64_t inv = f2_same(recip_approx(scale));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = f2_mul(f[i], inv);
+  } else {
+    // no finite reciprocal: scaled up by 2^64 first (a block of zeros stays 0)
+    const float inv = scale > 0.f ? 1.f / (scale * 1.8446744e19f) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = f2_pack(v[2 * i] * 1.8446744e19f * inv, v[2 * i + 1] * 1.8446744e19f * inv);
+  }
   uint32_t w[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 y = make_float2(f[2 * i] * inv, f[2 * i + 1] * inv);
-    if (inv == 0.f && scale > 0.f) y = make_float2(f[2 * i] / scale, f[2 * i + 1] / scale);
-    if constexpr (ROOT) {
-      if (f[2 * i] > 0.f) y.x = fmaxf(y.x, kE4m3Least);
-      if (f[2 * i + 1] > 0.f) y.y = fmaxf(y.y, kE4m3Least);
-    }
-    w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
+    float lo, hi;
+    f2_unpack(y[i], lo, hi);
+    w[i >> 1] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3) << (16 * (i & 1));
+  }
+  if constexpr (ROOT) {
+    // roots that are not 0 and were rounded to it (rare: a code of 0 is looked for first)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if ((w[j] - 0x01010101u) & ~w[j] & 0x80808080u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (((w[j] >> (8 * i)) & 0xffu) == 0 && v[4 * j + i] > 0.f) w[j] |= 1u << (8 * i);
+      }
   }
   return make_uint2(w[0], w[1]);
 }
@@ -167,8 +242,8 @@ __device__ __forceinline__ double block_sum(double v, double* share) {
   return s;
 }
 
-// Sum of squares of the gradients: one partial a CTA, in 64 bits (the clip coefficient
-// scales every element, so its error would be in all of them).
+// Sum of squares of the gradients: eight squares in 32 bits, then one partial a CTA in
+// 64 bits (the clip coefficient scales every element, so its error is in all of them).
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_constant__ Table<N> tab,
                                                                double* __restrict__ partial) {
@@ -182,13 +257,32 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
   for (int c = c0; c < c1; ++c) {
     while (ti + 1 < tab.count && tab.t[ti + 1].chunk0 <= c) ++ti;
     const Tensor& t = tab.t[ti];
-    const int64_t e = (int64_t)(c - t.chunk0) * kChunk + threadIdx.x * 8;
-    if (e >= t.n) continue;
-    const int64_t rest = t.n - e;
-    float g[8];
-    load8(static_cast<const T*>(t.g) + e, rest < 8 ? (int)rest : 8, (reinterpret_cast<uintptr_t>(t.g) & 15) == 0, g);
+    const bool vec = (reinterpret_cast<uintptr_t>(t.g) & 15) == 0;
+    Raw8<T> g[kBlocksPerWarp];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fma((double)g[i], (double)g[i], sum);
+    for (int u = 0; u < kBlocksPerWarp; ++u) {
+      const int64_t e = (int64_t)(c - t.chunk0) * kChunk + (u * kThreads + threadIdx.x) * 8;
+      const int64_t rest = t.n - e;
+      g[u].load(static_cast<const T*>(t.g) + e, rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest, vec);
+    }
+#pragma unroll
+    for (int u = 0; u < kBlocksPerWarp; ++u) {
+      uint64_t sq = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sq = f2_fma(g[u].pair(i), g[u].pair(i), sq);
+      float lo, hi;
+      f2_unpack(sq, lo, hi);
+      lo += hi;
+      if (lo > 3.4028235e38f) {  // squares past 32 bits
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f2_unpack(g[u].pair(i), lo, hi);
+          sum += (double)lo * lo + (double)hi * hi;
+        }
+      } else {
+        sum += lo;
+      }
+    }
   }
   sum = block_sum(sum, share);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
@@ -198,7 +292,7 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
 // `step` counts the steps done; `ticket` is 0 between launches. The last CTA of the
 // step's last launch (bump) raises the count after every CTA has read it.
 template <typename T, bool EIGHT, int N>
-__global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_constant__ Table<N> tab, States st,
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(EIGHT)) adamw_multi_kernel(const __grid_constant__ Table<N> tab, States st,
                                                                Hyper h, const double* __restrict__ partial,
                                                                int partials, float* __restrict__ norm_out,
                                                                float* __restrict__ step, int* __restrict__ ticket,
@@ -227,66 +321,113 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
     coefs[2] = clip;
   }
   __syncthreads();
-  const float step_size = coefs[0], root_scale = coefs[1], clip = coefs[2];
-  int c0, c1;
-  chunk_run(tab.chunks, c0, c1);
-  const int lane8 = threadIdx.x * 8;
-  int ti = c0 < c1 ? find_tensor(tab, c0) : 0;
-  for (int c = c0; c < c1; ++c) {
+  const uint64_t step_size = f2_same(-coefs[0]), root_scale = f2_same(coefs[1]), clip = f2_same(coefs[2]);
+  const uint64_t c1 = f2_same(h.one_minus_beta1), c2 = f2_same(h.one_minus_beta2), b2 = f2_same(h.beta2);
+  const uint64_t eps = f2_same(h.eps), decay = f2_same(h.decay), minus = f2_same(-1.f);
+  int first, end;
+  chunk_run(tab.chunks, first, end);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int ti = first < end ? find_tensor(tab, first) : 0;
+  for (int c = first; c < end; ++c) {
     while (ti + 1 < tab.count && tab.t[ti + 1].chunk0 <= c) ++ti;
     const Tensor& t = tab.t[ti];
-    const int64_t e = (int64_t)(c - t.chunk0) * kChunk + lane8;
-    const int64_t rest = t.n - e;
-    // a warp's block is there as a whole or in part, or not at all
-    if (t.n <= e - (threadIdx.x & 31) * 8) continue;
-    const int left = rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest;
     const bool vp = (reinterpret_cast<uintptr_t>(t.p) & 15) == 0, vg = (reinterpret_cast<uintptr_t>(t.g) & 15) == 0;
-    const int64_t blk = t.block0 + (e >> 8);
-    const int64_t at = blk * kBlock + (threadIdx.x & 31) * 8;
-    float p[8], g[8], m[8], v[8];
-    load8(static_cast<const T*>(t.g) + e, left, vg, g);
-    load8(static_cast<const T*>(t.p) + e, left, vp, p);
-    if constexpr (EIGHT) {
-      const uint2 mc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.m) + at));
-      const uint2 vc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.v) + at));
-      from_codes(mc, st.m_scale[blk], m);
-      from_codes(vc, st.v_scale[blk], v);
+    // the warp's kUnroll blocks of the chunk, all loads first
+    constexpr int U = EIGHT ? 2 : 1;
+    constexpr int kTurns = kBlocksPerWarp / U;
+#pragma unroll 1
+    for (int turn = 0; turn < kTurns; ++turn) {
+      Raw8<T> p[U], g[U];
+      Raw8<float> m32[EIGHT ? 1 : U], v32[EIGHT ? 1 : U];
+      uint2 mc[U], vc[U];
+      float ms[U], vs[U];
+      int left[U];
+      int64_t e[U], at[U];
+      int64_t blk[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= v[i];
-    } else {
-      load8(static_cast<const float*>(st.m) + at, 8, true, m);
-      load8(static_cast<const float*>(st.v) + at, 8, true, v);
-    }
-    float root[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float gi = g[i] * clip;
-      m[i] = fmaf(h.one_minus_beta1, gi - m[i], m[i]);
-      v[i] = fmaf(h.one_minus_beta2 * gi, gi, v[i] * h.beta2);
-      root[i] = sqrtf(v[i]);
-      p[i] = fmaf(p[i], h.decay, -(step_size * m[i] / fmaf(root[i], root_scale, h.eps)));
-    }
-    store8(static_cast<T*>(t.p) + e, left, vp, p);
-    if constexpr (EIGHT) {
-      // what lies behind a tensor's end stays 0
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i >= left) m[i] = root[i] = 0.f;
-      float ms, vs;
-      const uint2 mc = to_codes<false>(m, ms);
-      const uint2 vc = to_codes<true>(root, vs);
-      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m) + at), mc);
-      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v) + at), vc);
-      if ((threadIdx.x & 31) == 0) {
-        st.m_scale[blk] = ms;
-        st.v_scale[blk] = vs;
+      for (int u = 0; u < U; ++u) {
+        const int64_t w0 = (int64_t)(c - t.chunk0) * kChunk + ((turn * U + u) * kWarps + warp) * kBlock;
+        e[u] = w0 + lane * 8;
+        const int64_t rest = t.n - e[u];
+        left[u] = rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest;
+        blk[u] = t.block0 + (w0 >> 8);
+        at[u] = blk[u] * kBlock + lane * 8;
+        if (w0 >= t.n) {  // no such block: warp-uniform
+          blk[u] = -1;
+          continue;
+        }
+        g[u].load(static_cast<const T*>(t.g) + e[u], left[u], vg);
+        p[u].load(static_cast<const T*>(t.p) + e[u], left[u], vp);
+        if constexpr (EIGHT) {
+          mc[u] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.m) + at[u]));
+          vc[u] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.v) + at[u]));
+          ms[u] = st.m_scale[blk[u]];
+          vs[u] = st.v_scale[blk[u]];
+        } else {
+          m32[u].load(static_cast<const float*>(st.m) + at[u], 8, true);
+          v32[u].load(static_cast<const float*>(st.v) + at[u], 8, true);
+        }
       }
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i >= left) m[i] = v[i] = 0.f;
-      store8(static_cast<float*>(st.m) + at, 8, true, m);
-      store8(static_cast<float*>(st.v) + at, 8, true, v);
+      for (int u = 0; u < U; ++u) {
+        if (blk[u] < 0) continue;
+        uint64_t m[4], v[4], root[4];
+        const uint64_t msc = EIGHT ? f2_same(ms[u]) : 0, vsc = EIGHT ? f2_same(vs[u]) : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (EIGHT) {
+            m[i] = f2_mul(pair_of_codes(mc[u], i), msc);
+            v[i] = f2_mul(pair_of_codes(vc[u], i), vsc);
+            v[i] = f2_mul(v[i], v[i]);
+          } else {
+            m[i] = m32[u].pair(i);
+            v[i] = v32[u].pair(i);
+          }
+          const uint64_t gi = f2_mul(g[u].pair(i), clip);
+          m[i] = f2_fma(c1, f2_fma(m[i], minus, gi), m[i]);
+          v[i] = f2_fma(f2_mul(c2, gi), gi, f2_mul(v[i], b2));
+          float lo, hi;
+          f2_unpack(v[i], lo, hi);
+          root[i] = f2_pack(root_approx(lo), root_approx(hi));
+          f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
+          const uint64_t inv = f2_pack(recip_approx(lo), recip_approx(hi));
+          p[u].set(i, f2_fma(f2_mul(m[i], step_size), inv, f2_mul(p[u].pair(i), decay)));
+        }
+        p[u].store(static_cast<T*>(t.p) + e[u], left[u], vp);
+        if (left[u] < 8) {
+          // what lies behind a tensor's end stays 0
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool a = 2 * i < left[u], b = 2 * i + 1 < left[u];
+            float x, y;
+            f2_unpack(m[i], x, y);
+            m[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
+            f2_unpack(v[i], x, y);
+            v[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
+            f2_unpack(root[i], x, y);
+            root[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
+          }
+        }
+        if constexpr (EIGHT) {
+          float sm, sv;
+          const uint2 cm = to_codes<false>(m, sm);
+          const uint2 cv = to_codes<true>(root, sv);
+          __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m) + at[u]), cm);
+          __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v) + at[u]), cv);
+          if (lane == 0) {
+            st.m_scale[blk[u]] = sm;
+            st.v_scale[blk[u]] = sv;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            m32[u].set(i, m[i]);
+            v32[u].set(i, v[i]);
+          }
+          m32[u].store(static_cast<float*>(st.m) + at[u], 8, true);
+          v32[u].store(static_cast<float*>(st.v) + at[u], 8, true);
+        }
+      }
     }
   }
   if (bump && threadIdx.x == 0) {
@@ -299,12 +440,13 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
   }
 }
 
+constexpr int kSquareCtas = 6;              // of grad_square_kernel on an SM, each with a partial sum
 constexpr int kSmall = 64, kLarge = 960;  // tensors of a launch: arguments of 2 and 30 KB
 
 inline int chunks_of(int64_t n) { return (int)((n + kChunk - 1) / kChunk); }
 
-inline int grid_of(int chunks) {
-  const int cap = num_sms() * 4;
+inline int grid_of(int chunks, int per_sm) {
+  const int cap = num_sms() * per_sm;
   return chunks < cap ? (chunks < 1 ? 1 : chunks) : cap;
 }
 
@@ -361,7 +503,7 @@ template <typename T, int N>
 int square_launch(const Args& a, int i0, int i1, double* partial, int* used, cudaStream_t st) {
   Table<N> tab;
   fill_table(tab, a, i0, i1);
-  const int grid = grid_of(tab.chunks) < num_sms() * 2 ? grid_of(tab.chunks) : num_sms() * 2;
+  const int grid = grid_of(tab.chunks, kSquareCtas);
   *used += grid;
   return launch_table(grad_square_kernel<T, N>, grid, st, tab, partial);
 }
@@ -371,7 +513,7 @@ int step_launch(const Args& a, int i0, int i1, const States& s, const Hyper& h, 
                 float* norm_out, float* step, int* ticket, int bump, cudaStream_t st) {
   Table<N> tab;
   fill_table(tab, a, i0, i1);
-  return launch_table(adamw_multi_kernel<T, EIGHT, N>, grid_of(tab.chunks), st, tab, s, h, partial, partials, norm_out,
+  return launch_table(adamw_multi_kernel<T, EIGHT, N>, grid_of(tab.chunks, ctas_per_sm(EIGHT)), st, tab, s, h, partial, partials, norm_out,
                       step, ticket, bump);
 }
 
@@ -392,7 +534,7 @@ int square_run(const Args& a, double* partial, int cap, int* used, cudaStream_t 
   const int most = a.count <= kSmall ? kSmall : kLarge;
   for (int i0 = 0; i0 < a.count;) {
     const int i1 = launch_end(a, i0, most);
-    if (*used + num_sms() * 2 > cap) {
+    if (*used + num_sms() * kSquareCtas > cap) {
       set_last_error("soup_grad_square: workspace too small");
       return SOUP_ERR_WORKSPACE;
     }
@@ -430,8 +572,7 @@ extern "C" {
 
 size_t soup_grad_square_workspace_bytes(int64_t tensors) {
   if (tensors <= 0) return 0;
-  // two partials an SM for each launch
-  return sizeof(double) * 2 * (size_t)num_sms() * (size_t)((tensors + kLarge - 1) / kLarge);
+  return sizeof(double) * kSquareCtas * (size_t)num_sms() * (size_t)((tensors + kLarge - 1) / kLarge);
 }
 
 int soup_grad_square(const void* const* grads, const int64_t* sizes, int count, int dtype, void* workspace,

@@ -4,7 +4,7 @@
 //   y1 = n1 c - n2 s,  y2 = n1 s + n2 c                      (halves of the head dim)
 // backward:
 //   dn1 = g1 c + g2 s, dn2 = g2 c - g1 s
-//   dx  = rstd (dn w - x rstd^2 mean(dn w x)),  dw = sum over tokens and heads of dn x rstd
+//   dx  = rstd (dn w - x rstd * rstd mean(dn w x)),  dw = sum over tokens and heads of dn x rstd
 // c and s of frequency i come from cos / sin tables, or from the token's position
 // on that frequency's axis: theta = pos[axis(i)] * inv_freq[i], reduced to a
 // fraction of a turn in 64 bits (a position of 100000 leaves 3e-3 of an angle in
@@ -14,12 +14,15 @@
 // written; rstd is formed again from x, which is read anyway). Everything between
 // is in 32 bits; the one rounding is the output's.
 //
-// A row (token, head) is `lanes` threads of one warp, each with a 16-byte vector
-// of the first half and the matching vector of the second, so a rotation needs no
-// exchange and a norm needs log2(lanes) shuffles. A CTA takes P tokens at a time:
-// their rows' loads are in flight while the CTA forms the P tables in shared
-// memory, which all heads then read. Head dims whose half is not a multiple of a
-// vector, or rows that are not 16-byte aligned, take a warp per row instead.
+// A row (token, head) is `lanes` threads of one warp, each with NE elements of the
+// first half and the matching NE of the second, so a rotation needs no exchange and a
+// norm needs log2(lanes) shuffles. A thread keeps its (head, elements) slot for P
+// tokens, whose loads are in flight together. cos and sin come by vector loads beside
+// them, or, from positions, through a table that the CTA forms in shared memory. Head
+// dims whose half is not a multiple of a vector, or rows that are not 16-byte aligned,
+// take a warp per row instead.
+#include <type_traits>
+
 #include "soup_common.cuh"
 
 namespace soup {
@@ -27,7 +30,7 @@ namespace {
 
 constexpr int kMaxDim = 512;        // head dim
 constexpr int kMaxHalf = kMaxDim / 2;
-constexpr int kMaxThreads = 512;
+constexpr int kMaxThreads = 256;
 
 struct HeadRows {
   const void* x;       // q or k
@@ -52,12 +55,33 @@ struct Angles {
   uint8_t axis[kMaxHalf];
 };
 
+// Division of an index below 2^31 by d as a product: with l = ceil(log2 d) and
+// m = ceil(2^(31 + l) / d), n m >> (31 + l) is n / d (Granlund and Montgomery's division
+// by an invariant).
+struct Div {
+  uint32_t m;
+  int shift;
+  uint32_t d;
+  __device__ __forceinline__ void split(uint32_t n, int64_t& q, int64_t& r) const {
+    const uint32_t t = (uint32_t)(((uint64_t)n * m) >> shift);
+    q = t;
+    r = n - t * d;
+  }
+};
+
+inline Div make_div(int64_t d) {
+  int l = 0;
+  while ((int64_t(1) << l) < d) ++l;
+  return Div{(uint32_t)((((uint64_t)1 << (31 + l)) + (uint64_t)d - 1) / (uint64_t)d), 31 + l, (uint32_t)d};
+}
+
 struct Shape {
-  int64_t tokens;      // batch * seq
-  int64_t seq;
+  int batch, seq;
+  Div tiles;           // of a sequence: of P tokens (qk_rope_any_kernel: of one)
   int half;
   int lanes;           // threads of a row (a power of two)
-  float eps;
+  int group_heads;     // heads of a CTA
+  float eps, inv_d;    // inv_d: 1 / D
   int w_dtype;
   float sign;          // -1: the inverse rotation
 };
@@ -68,277 +92,421 @@ __device__ __forceinline__ float load_as_f(const void* p, int64_t i, int dtype) 
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
-// cos and sin of frequency i for the token at (b, s)
+// cos and sin of a position on frequency i
+__device__ __forceinline__ void turn(const Angles& a, int64_t b, int64_t s, int i, float& c, float& sn) {
+  const int64_t at = a.axis[i] * a.pa + b * a.pb + s * a.ps;
+  const double pos = a.pos64 ? (double)static_cast<const long long*>(a.pos)[at]
+                             : (double)static_cast<const int*>(a.pos)[at];
+  const double turns = pos * ((double)a.inv_freq[i] * 0.15915494309189533577);  // 1 / (2 pi)
+  sincospif((float)(2.0 * (turns - rint(turns))), &sn, &c);
+}
 __device__ __forceinline__ void angle_of(const Angles& a, int64_t b, int64_t s, int i, float& c, float& sn) {
   if (a.cos) {
     const int64_t at = b * a.tb + s * a.ts + i;
     c = load_as_f(a.cos, at, a.dtype);
     sn = load_as_f(a.sin, at, a.dtype);
   } else {
-    const int64_t at = a.axis[i] * a.pa + b * a.pb + s * a.ps;
-    const double pos = a.pos64 ? (double)static_cast<const long long*>(a.pos)[at]
-                               : (double)static_cast<const int*>(a.pos)[at];
-    const double turns = pos * ((double)a.inv_freq[i] * 0.15915494309189533577);  // 1 / (2 pi)
-    sincospif((float)(2.0 * (turns - rint(turns))), &sn, &c);
+    turn(a, b, s, i, c, sn);
   }
 }
 
-// The tables of tokens [n0, n0 + P) into shared memory (cos, then sin, half each).
-template <int P>
-__device__ __forceinline__ void fill_tables(const Angles& a, const Shape& sh, int64_t n0, float* tab) {
-  for (int e = threadIdx.x; e < P * sh.half; e += blockDim.x) {
-    const int p = e / sh.half, i = e - p * sh.half;
-    const int64_t n = n0 + p;
-    if (n >= sh.tokens) break;
-    const int64_t b = n / sh.seq;
-    float c, s;
-    angle_of(a, b, n - b * sh.seq, i, c, s);
-    tab[p * 2 * sh.half + i] = c;
-    tab[(p * 2 + 1) * sh.half + i] = sh.sign * s;
-  }
-}
-
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-template <int NE>
-__device__ __forceinline__ void load_table(const float* t, float (&v)[NE]) {
+// NE consecutive elements of type T in loads of up to 16 bytes, read and written as
+// packed pairs of 32-bit numbers.
+template <typename T, int NE>
+struct Pack {
+  static constexpr int kBytes = NE * (int)sizeof(T);
+  static constexpr int kWords = kBytes / 4;
+  uint32_t u[kWords];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int e = 0; e < NE; e += 4) {
-    const float4 q = *reinterpret_cast<const float4*>(t + e);
-    v[e] = q.x;
-    v[e + 1] = q.y;
-    v[e + 2] = q.z;
-    v[e + 3] = q.w;
+    for (int i = 0; i < kWords; ++i) u[i] = 0;
+  }
+  template <bool STREAM>
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4* q = reinterpret_cast<const uint4*>(p) + i / 4;
+        const uint4 r = STREAM ? __ldcs(q) : *q;
+        u[i] = r.x;
+        u[i + 1] = r.y;
+        u[i + 2] = r.z;
+        u[i + 3] = r.w;
+      }
+    } else {
+      static_assert(kBytes == 8, "8 or a multiple of 16 bytes");
+      const uint2* q = reinterpret_cast<const uint2*>(p);
+      const uint2 r = STREAM ? __ldcs(q) : *q;
+      u[0] = r.x;
+      u[1] = r.y;
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kBytes % 16 == 0) {
+#pragma unroll
+      for (int i = 0; i < kWords; i += 4)
+        __stcs(reinterpret_cast<uint4*>(p) + i / 4, make_uint4(u[i], u[i + 1], u[i + 2], u[i + 3]));
+    } else {
+      __stcs(reinterpret_cast<uint2*>(p), make_uint2(u[0], u[1]));
+    }
+  }
+  __device__ __forceinline__ uint64_t pair(int i) const {
+    if constexpr (sizeof(T) == 4) {
+      return f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return f2_pack(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      return f2_pack(f.x, f.y);
+    }
+  }
+  __device__ __forceinline__ void set(int i, uint64_t v) {
+    float x, y;
+    f2_unpack(v, x, y);
+    if constexpr (sizeof(T) == 4) {
+      u[2 * i] = __float_as_uint(x);
+      u[2 * i + 1] = __float_as_uint(y);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+      u[i] = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      const __half2 h = __floats2half2_rn(x, y);
+      u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+};
+
+__device__ __forceinline__ uint64_t f2_same(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ float f2_sum(uint64_t p) {
+  float x, y;
+  f2_unpack(p, x, y);
+  return x + y;
+}
+// a c - b s
+__device__ __forceinline__ uint64_t f2_cross(uint64_t a, uint64_t c, uint64_t b, uint64_t s) {
+  return f2_fma(f2_mul(b, s), f2_same(-1.f), f2_mul(a, c));
+}
+
+// Where cos and sin come from.
+constexpr int kTableT = 0;    // tables of the rows' type
+constexpr int kTableF = 1;    // fp32 tables
+constexpr int kPositions = 2;
+
+template <typename T, int SRC>
+struct TableType {
+  using type = typename std::conditional<SRC == kTableT, T, float>::type;
+};
+
+template <typename T, int NE>
+__device__ __forceinline__ void load_weights(const void* w, int at, int dtype, uint64_t (&f)[NE / 2]) {
+  if (dtype == SOUP_F32) {
+    Pack<float, NE> p;
+    p.template load<false>(static_cast<const float*>(w) + at);
+#pragma unroll
+    for (int e = 0; e < NE / 2; ++e) f[e] = p.pair(e);
+  } else {
+    Pack<T, NE> p;
+    p.template load<false>(static_cast<const T*>(w) + at);
+#pragma unroll
+    for (int e = 0; e < NE / 2; ++e) f[e] = p.pair(e);
   }
 }
+
+// The tables of tokens [s0, s0 + P) of sequence b into shared memory (cos, then sin).
+template <int P>
+__device__ __forceinline__ void fill_tables(const Angles& a, const Shape& sh, int64_t b, int64_t s0, float* tab) {
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    if (s0 + p >= sh.seq) break;
+    for (int i = threadIdx.x; i < sh.half; i += blockDim.x) {
+      float c, sn;
+      turn(a, b, s0 + p, i, c, sn);
+      tab[p * 2 * sh.half + i] = c;
+      tab[(p * 2 + 1) * sh.half + i] = sn;
+    }
+  }
+}
+
+// A thread's slot: its rows and its place in them.
+struct Slot {
+  bool on, isq;
+  int64_t hh;
+  int d;
+  __device__ __forceinline__ Slot(const HeadRows& q, const HeadRows& k, const Shape& sh, int ne) {
+    const int shift = __ffs(sh.lanes) - 1;
+    const int local = threadIdx.x >> shift;
+    const int h = blockIdx.y * sh.group_heads + local;
+    d = (threadIdx.x & (sh.lanes - 1)) * ne;
+    on = local < sh.group_heads && h < q.heads + k.heads && d < sh.half;
+    isq = h < q.heads;
+    hh = isq ? h : h - q.heads;
+    if (!on) d = 0;
+  }
+};
+
+// cos and sin of a thread's elements for a token, p-th of the CTA's.
+template <typename T, int NE, int SRC>
+struct Turn {
+  using TT = typename TableType<T, SRC>::type;
+  Pack<TT, NE> c, s;
+  __device__ __forceinline__ void load(const TT* cos, const TT* sin) {
+    c.template load<false>(cos);
+    s.template load<false>(sin);
+  }
+  __device__ __forceinline__ void take(const float* tab, int p, int half, int d) {
+    if constexpr (SRC == kPositions) {
+      c.template load<false>(tab + p * 2 * half + d);
+      s.template load<false>(tab + (p * 2 + 1) * half + d);
+    }
+  }
+};
 
 // Forward (and, without weights and with sign -1, the backward of a rotation alone).
-template <typename T, int P, bool NORM>
-__global__ void __launch_bounds__(kMaxThreads) qk_rope_fwd_kernel(HeadRows q, HeadRows k,
-                                                                  const __grid_constant__ Angles ang,
-                                                                  Shape sh) {
-  constexpr int NE = Vec16<T>::N;
-  __shared__ __align__(16) float tab[P * 2 * kMaxHalf];
+// CTA (x, y): P tokens of a sequence, heads [y group_heads, ...).
+template <typename T, int NE, int P, bool NORM, int SRC>
+__global__ void __launch_bounds__(kMaxThreads, NE == 8 ? 2 : P == 4 ? 3 : 4) qk_rope_fwd_kernel(
+    HeadRows q, HeadRows k, const __grid_constant__ Angles ang, Shape sh) {
+  using Tr = Turn<T, NE, SRC>;
+  __shared__ __align__(16) float tab[SRC == kPositions ? P * 2 * kMaxHalf : 4];
   pdl_wait();
   pdl_trigger();
-  const int half = sh.half, chunks = half / NE;
-  const int shift = __ffs(sh.lanes) - 1;
-  const int slots = (q.heads + k.heads) << shift;
-  const int64_t n0 = (int64_t)blockIdx.x * P;
-  bool ready = false;
-  for (int base = 0; base < slots; base += blockDim.x) {
-    const int i = base + threadIdx.x;
-    const int h = i >> shift, d = (i & (sh.lanes - 1)) * NE;
-    const bool on = i < slots && d < chunks * NE;
-    const bool isq = h < q.heads;
-    const HeadRows& t = isq ? q : k;
-    const int64_t hh = isq ? h : h - q.heads;
-    Vec16<T> x1[P], x2[P];
+  const int half = sh.half;
+  int64_t b, s0;
+  sh.tiles.split(blockIdx.x, b, s0);
+  s0 *= P;
+  const int n = min((int)(sh.seq - s0), P);
+  const Slot slot(q, k, sh, NE);
+  const HeadRows& t = slot.isq ? q : k;
+  const T* xp = static_cast<const T*>(t.x) + slot.hh * t.xh + slot.d + b * t.xb + s0 * t.xs;
+  T* op = static_cast<T*>(t.out) + slot.hh * t.oh + slot.d + b * t.ob + s0 * t.os;
+  const typename Tr::TT *cp = nullptr, *sp = nullptr;
+  if constexpr (SRC != kPositions) {
+    const int64_t at = b * ang.tb + s0 * ang.ts + slot.d;
+    cp = static_cast<const typename Tr::TT*>(ang.cos) + at;
+    sp = static_cast<const typename Tr::TT*>(ang.sin) + at;
+  }
+  Pack<T, NE> x1[P], x2[P];
+  Tr tr[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    x1[p].zero();
+    x2[p].zero();
+    if (slot.on && p < n) {
+      x1[p].template load<true>(xp);
+      x2[p].template load<true>(xp + half);
+      if constexpr (SRC != kPositions) {
+        tr[p].load(cp, sp);
+        cp += ang.ts;
+        sp += ang.ts;
+      }
+      xp += t.xs;
+    }
+  }
+  if constexpr (SRC == kPositions) {
+    fill_tables<P>(ang, sh, b, s0, tab);
+    __syncthreads();
+  }
+  float rstd[P];
+  uint64_t w1[NE / 2], w2[NE / 2];
+  if constexpr (NORM) {
+    load_weights<T, NE>(t.w, slot.d, sh.w_dtype, w1);
+    load_weights<T, NE>(t.w, half + slot.d, sh.w_dtype, w2);
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      x1[p].u = make_uint4(0, 0, 0, 0);
-      x2[p].u = make_uint4(0, 0, 0, 0);
-      const int64_t n = n0 + p;
-      if (on && n < sh.tokens) {
-        const int64_t b = n / sh.seq, s = n - b * sh.seq;
-        const T* xp = static_cast<const T*>(t.x) + b * t.xb + hh * t.xh + s * t.xs + d;
-        x1[p] = ld16_stream(xp);
-        x2[p] = ld16_stream(xp + half);
-      }
-    }
-    float w1[NE], w2[NE];
-    if constexpr (NORM) {
+      uint64_t ss = 0;
 #pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        w1[e] = on ? load_as_f(t.w, d + e, sh.w_dtype) : 0.f;
-        w2[e] = on ? load_as_f(t.w, half + d + e, sh.w_dtype) : 0.f;
+      for (int e = 0; e < NE / 2; ++e) {
+        const uint64_t a = x1[p].pair(e), c = x2[p].pair(e);
+        ss = f2_fma(a, a, f2_fma(c, c, ss));
       }
+      rstd[p] = f2_sum(ss);
     }
-    if (!ready) {  // block-uniform
-      fill_tables<P>(ang, sh, n0, tab);
-      __syncthreads();
-      ready = true;
+    for (int o = sh.lanes >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) rstd[p] += __shfl_xor_sync(0xffffffffu, rstd[p], o);
     }
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int64_t n = n0 + p;
-      if (n >= sh.tokens) break;  // block-uniform
-      float a[NE], bb[NE];
+    for (int p = 0; p < P; ++p) rstd[p] = rsqrtf(fmaf(rstd[p], sh.inv_d, sh.eps));
+  }
+  const uint64_t sign = f2_same(sh.sign);
 #pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        a[e] = Cvt<T>::to_f(x1[p].v[e]);
-        bb[e] = Cvt<T>::to_f(x2[p].v[e]);
-      }
+  for (int p = 0; p < P; ++p) {
+    if (!slot.on || p >= n) break;
+    tr[p].take(tab, p, half, slot.d);
+    Pack<T, NE> y1, y2;
+#pragma unroll
+    for (int e = 0; e < NE / 2; ++e) {
+      uint64_t a = x1[p].pair(e), c = x2[p].pair(e);
+      uint64_t cs = tr[p].c.pair(e), sn = tr[p].s.pair(e);
       if constexpr (NORM) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) ss = fmaf(a[e], a[e], fmaf(bb[e], bb[e], ss));
-        ss = lanes_sum(ss, sh.lanes);
-        const float rstd = 1.f / sqrtf(ss / (float)(2 * half) + sh.eps);
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          a[e] = a[e] * rstd * w1[e];
-          bb[e] = bb[e] * rstd * w2[e];
-        }
+        const uint64_t r = f2_same(rstd[p]);
+        a = f2_mul(f2_mul(a, r), w1[e]);
+        c = f2_mul(f2_mul(c, r), w2[e]);
+      } else {
+        sn = f2_mul(sn, sign);
       }
-      if (on) {
-        float c[NE], s[NE];
-        load_table<NE>(tab + p * 2 * half + d, c);
-        load_table<NE>(tab + (p * 2 + 1) * half + d, s);
-        const int64_t b = n / sh.seq, sp = n - b * sh.seq;
-        T* op = static_cast<T*>(t.out) + b * t.ob + hh * t.oh + sp * t.os + d;
-        Vec16<T> y1, y2;
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          y1.v[e] = Cvt<T>::from_f(a[e] * c[e] - bb[e] * s[e]);
-          y2.v[e] = Cvt<T>::from_f(a[e] * s[e] + bb[e] * c[e]);
-        }
-        st16_stream(op, y1);
-        st16_stream(op + half, y2);
-      }
+      y1.set(e, f2_cross(a, cs, c, sn));
+      y2.set(e, f2_fma(a, sn, f2_mul(c, cs)));
     }
+    y1.store(op);
+    y2.store(op + half);
+    op += t.os;
   }
 }
 
-// Backward with norms. One (head, vector) slot a thread for all of the CTA's
-// tokens, so a thread's share of dw stays in its registers; blockIdx.y takes the
-// next blockDim.x slots. The CTA joins its rows of dw in the order of the heads and
-// leaves one partial row [2][D] (q, k), which dw_join_kernel sums in block order.
-template <typename T, int P>
-__global__ void __launch_bounds__(kMaxThreads) qk_norm_rope_bwd_kernel(HeadRows q, HeadRows k,
-                                                                       const __grid_constant__ Angles ang,
-                                                                       Shape sh, float* __restrict__ dw_part) {
-  constexpr int NE = Vec16<T>::N;
+// Backward with norms. A thread keeps its slot for all of the CTA's tokens, so that its
+// share of dw stays in its registers. The CTA joins its rows of dw in the order of the
+// heads and leaves one partial row [2][D] (q, k), which dw_join_kernel sums in block
+// order.
+template <typename T, int NE, int P, int SRC>
+__global__ void __launch_bounds__(kMaxThreads, NE == 4 ? 3 : 1) qk_norm_rope_bwd_kernel(
+    HeadRows q, HeadRows k, const __grid_constant__ Angles ang, Shape sh, float* __restrict__ dw_part) {
+  using Tr = Turn<T, NE, SRC>;
   extern __shared__ __align__(16) float smem[];  // tables [P][2][half], later dw [blockDim][2 NE]
   pdl_wait();
+  const int half = sh.half;
+  const Slot slot(q, k, sh, NE);
+  const HeadRows& t = slot.isq ? q : k;
+  const T* xp = static_cast<const T*>(t.x) + slot.hh * t.xh + slot.d;
+  const T* gp = static_cast<const T*>(t.g) + slot.hh * t.gh + slot.d;
+  T* op = static_cast<T*>(t.out) + slot.hh * t.oh + slot.d;
+  uint64_t w1[NE / 2], w2[NE / 2], dw1[NE / 2], dw2[NE / 2];
+  load_weights<T, NE>(t.w, slot.d, sh.w_dtype, w1);
+  load_weights<T, NE>(t.w, half + slot.d, sh.w_dtype, w2);
+#pragma unroll
+  for (int e = 0; e < NE / 2; ++e) dw1[e] = dw2[e] = 0;
+  const int tiles = (int)sh.tiles.d * sh.batch;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    int64_t b, s0;
+    sh.tiles.split(tile, b, s0);
+    s0 *= P;
+    const int n = min((int)(sh.seq - s0), P);
+    const T* xr = xp + b * t.xb + s0 * t.xs;
+    const T* gr = gp + b * t.gb + s0 * t.gs;
+    T* out = op + b * t.ob + s0 * t.os;
+    Pack<T, NE> x1[P], x2[P], g1[P], g2[P];
+    Tr tr[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      x1[p].zero();
+      x2[p].zero();
+      g1[p].zero();
+      g2[p].zero();
+      tr[p].c.zero();
+      tr[p].s.zero();
+      if (slot.on && p < n) {
+        x1[p].template load<true>(xr + p * t.xs);
+        x2[p].template load<true>(xr + p * t.xs + half);
+        g1[p].template load<true>(gr + p * t.gs);
+        g2[p].template load<true>(gr + p * t.gs + half);
+        if constexpr (SRC != kPositions) {
+          const int64_t at = b * ang.tb + (s0 + p) * ang.ts + slot.d;
+          tr[p].load(static_cast<const typename Tr::TT*>(ang.cos) + at,
+                     static_cast<const typename Tr::TT*>(ang.sin) + at);
+        }
+      }
+    }
+    if constexpr (SRC == kPositions) {
+      __syncthreads();  // the tables of the tile before are read
+      fill_tables<P>(ang, sh, b, s0, smem);
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (slot.on && p < n) tr[p].take(smem, p, half, slot.d);
+    }
+    float ss[P], dot[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      uint64_t sq = 0, dt = 0;
+#pragma unroll
+      for (int e = 0; e < NE / 2; ++e) {
+        const uint64_t a = x1[p].pair(e), c = x2[p].pair(e), cs = tr[p].c.pair(e), sn = tr[p].s.pair(e);
+        const uint64_t ga = g1[p].pair(e), gb = g2[p].pair(e);
+        sq = f2_fma(a, a, f2_fma(c, c, sq));
+        dt = f2_fma(f2_mul(f2_fma(ga, cs, f2_mul(gb, sn)), w1[e]), a, dt);
+        dt = f2_fma(f2_mul(f2_cross(gb, cs, ga, sn), w2[e]), c, dt);
+      }
+      ss[p] = f2_sum(sq);
+      dot[p] = f2_sum(dt);
+    }
+    for (int o = sh.lanes >> 1; o > 0; o >>= 1) {
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        ss[p] += __shfl_xor_sync(0xffffffffu, ss[p], o);
+        dot[p] += __shfl_xor_sync(0xffffffffu, dot[p], o);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const float rstd = rsqrtf(fmaf(ss[p], sh.inv_d, sh.eps));
+      const uint64_t r = f2_same(rstd);
+      const uint64_t back = f2_same(-dot[p] * sh.inv_d * rstd);
+      Pack<T, NE> y1, y2;
+#pragma unroll
+      for (int e = 0; e < NE / 2; ++e) {
+        const uint64_t a = x1[p].pair(e), c = x2[p].pair(e), cs = tr[p].c.pair(e), sn = tr[p].s.pair(e);
+        const uint64_t ga = g1[p].pair(e), gb = g2[p].pair(e);
+        const uint64_t d1 = f2_fma(ga, cs, f2_mul(gb, sn)), d2 = f2_cross(gb, cs, ga, sn);
+        const uint64_t h1 = f2_mul(a, r), h2 = f2_mul(c, r);
+        dw1[e] = f2_fma(d1, h1, dw1[e]);
+        dw2[e] = f2_fma(d2, h2, dw2[e]);
+        y1.set(e, f2_mul(r, f2_fma(h1, back, f2_mul(d1, w1[e]))));
+        y2.set(e, f2_mul(r, f2_fma(h2, back, f2_mul(d2, w2[e]))));
+      }
+      if (slot.on && p < n) {
+        y1.store(out + p * t.os);
+        y2.store(out + p * t.os + half);
+      }
+    }
+  }
   pdl_trigger();
-  const int half = sh.half, chunks = half / NE;
-  const int shift = __ffs(sh.lanes) - 1;
-  const int slots = (q.heads + k.heads) << shift;
-  const int i = blockIdx.y * blockDim.x + threadIdx.x;
-  const int h = i >> shift, d = (i & (sh.lanes - 1)) * NE;
-  const bool on = i < slots && d < chunks * NE;
-  const bool isq = h < q.heads;
-  const HeadRows& t = isq ? q : k;
-  const int64_t hh = isq ? h : h - q.heads;
-  float w1[NE], w2[NE], dw1[NE], dw2[NE];
-#pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    w1[e] = on ? load_as_f(t.w, d + e, sh.w_dtype) : 0.f;
-    w2[e] = on ? load_as_f(t.w, half + d + e, sh.w_dtype) : 0.f;
-    dw1[e] = dw2[e] = 0.f;
-  }
-  const int64_t tiles = (sh.tokens + P - 1) / P;
-  const float inv_d = 1.f / (float)(2 * half);
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t n0 = tile * P;
-    Vec16<T> x1[P], x2[P], g1[P], g2[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      x1[p].u = x2[p].u = g1[p].u = g2[p].u = make_uint4(0, 0, 0, 0);
-      const int64_t n = n0 + p;
-      if (on && n < sh.tokens) {
-        const int64_t b = n / sh.seq, s = n - b * sh.seq;
-        const T* xp = static_cast<const T*>(t.x) + b * t.xb + hh * t.xh + s * t.xs + d;
-        const T* gp = static_cast<const T*>(t.g) + b * t.gb + hh * t.gh + s * t.gs + d;
-        x1[p] = ld16_stream(xp);
-        x2[p] = ld16_stream(xp + half);
-        g1[p] = ld16_stream(gp);
-        g2[p] = ld16_stream(gp + half);
-      }
-    }
-    __syncthreads();  // the tables of the tile before are read
-    fill_tables<P>(ang, sh, n0, smem);
-    __syncthreads();
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int64_t n = n0 + p;
-      if (n >= sh.tokens) break;  // block-uniform
-      float c[NE], s[NE], dn1[NE], dn2[NE];
-      const int dt = on ? d : 0;
-      load_table<NE>(smem + p * 2 * half + dt, c);
-      load_table<NE>(smem + (p * 2 + 1) * half + dt, s);
-      float ss = 0.f, dot = 0.f;
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const float a = Cvt<T>::to_f(x1[p].v[e]), bb = Cvt<T>::to_f(x2[p].v[e]);
-        const float ga = Cvt<T>::to_f(g1[p].v[e]), gb = Cvt<T>::to_f(g2[p].v[e]);
-        dn1[e] = ga * c[e] + gb * s[e];
-        dn2[e] = gb * c[e] - ga * s[e];
-        ss = fmaf(a, a, fmaf(bb, bb, ss));
-        dot = fmaf(dn1[e] * w1[e], a, fmaf(dn2[e] * w2[e], bb, dot));
-      }
-      for (int o = sh.lanes >> 1; o > 0; o >>= 1) {
-        ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      }
-      const float rstd = 1.f / sqrtf(ss * inv_d + sh.eps);
-      const float back = dot * inv_d * rstd * rstd;
-      Vec16<T> y1, y2;
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        const float a = Cvt<T>::to_f(x1[p].v[e]), bb = Cvt<T>::to_f(x2[p].v[e]);
-        dw1[e] = fmaf(dn1[e], a * rstd, dw1[e]);
-        dw2[e] = fmaf(dn2[e], bb * rstd, dw2[e]);
-        y1.v[e] = Cvt<T>::from_f(rstd * (dn1[e] * w1[e] - a * back));
-        y2.v[e] = Cvt<T>::from_f(rstd * (dn2[e] * w2[e] - bb * back));
-      }
-      if (on) {
-        const int64_t b = n / sh.seq, sp = n - b * sh.seq;
-        T* op = static_cast<T*>(t.out) + b * t.ob + hh * t.oh + sp * t.os + d;
-        st16_stream(op, y1);
-        st16_stream(op + half, y2);
-      }
-    }
-  }
   if (!dw_part) return;
   __syncthreads();
   float* mine = smem + threadIdx.x * 2 * NE;
 #pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    mine[e] = dw1[e];
-    mine[NE + e] = dw2[e];
+  for (int e = 0; e < NE / 2; ++e) {
+    f2_unpack(dw1[e], mine[2 * e], mine[2 * e + 1]);
+    f2_unpack(dw2[e], mine[NE + 2 * e], mine[NE + 2 * e + 1]);
   }
   __syncthreads();
-  // this block's heads, in order; a block's slots start at a head's first
+  // this block's heads, in order
   const int dim = 2 * half;
-  const int h0 = (blockIdx.y * blockDim.x) >> shift;
-  const int h1 = min((int)((blockIdx.y + 1) * blockDim.x) >> shift, q.heads + k.heads);
+  const int h0 = blockIdx.y * sh.group_heads;
+  const int h1 = min(h0 + sh.group_heads, q.heads + k.heads);
   float* row = dw_part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * dim;
   for (int e = threadIdx.x; e < 2 * dim; e += blockDim.x) {
     const int which = e / dim, col = e - which * dim;
     const int second = col >= half ? 1 : 0, c = col - second * half;
     const int lo = which ? max(h0, q.heads) : h0, hi = which ? h1 : min(h1, q.heads);
     float sum = 0.f;
-    for (int hd = lo; hd < hi; ++hd) {
-      const int th = (hd << shift) + c / NE - blockIdx.y * blockDim.x;
-      sum += smem[th * 2 * NE + second * NE + c % NE];
-    }
+    for (int hd = lo; hd < hi; ++hd)
+      sum += smem[((hd - h0) * sh.lanes + c / NE) * 2 * NE + second * NE + c % NE];
     row[e] = sum;
   }
 }
 
-// dw [2][D] = sum of the partial rows in block order: a warp-wide group of 32
-// threads a column group, 32 rows apart, joined in shared memory.
-__global__ void __launch_bounds__(1024) dw_join_kernel(const float* __restrict__ part, int rows, int dim,
-                                                       void* __restrict__ dwq, void* __restrict__ dwk,
-                                                       int w_dtype) {
-  __shared__ float acc[32][33];
+// dw [2][D] = sum of the partial rows in block order: eight columns a CTA, 64 threads a
+// column, 64 rows apart, joined in shared memory.
+constexpr int kJoinCols = 8, kJoinRows = 64;
+__global__ void __launch_bounds__(kJoinCols * kJoinRows) dw_join_kernel(const float* __restrict__ part, int rows,
+                                                                        int dim, void* __restrict__ dwq,
+                                                                        void* __restrict__ dwk, int w_dtype) {
+  __shared__ float acc[kJoinRows][kJoinCols + 1];
   pdl_wait();
   pdl_trigger();
-  const int col = blockIdx.x * 32 + threadIdx.x;
+  const int lane = threadIdx.x % kJoinCols, r0 = threadIdx.x / kJoinCols;
+  const int col = blockIdx.x * kJoinCols + lane;
   float s = 0.f;
-  if (col < 2 * dim)
-    for (int r = threadIdx.y; r < rows; r += 32) s += part[(int64_t)r * 2 * dim + col];
-  acc[threadIdx.y][threadIdx.x] = s;
+  if (col < 2 * dim) {
+#pragma unroll 8
+    for (int r = r0; r < rows; r += kJoinRows) s += part[(int64_t)r * 2 * dim + col];
+  }
+  acc[r0][lane] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && col < 2 * dim) {
+  if (threadIdx.x < kJoinCols && col < 2 * dim) {
     float t = 0.f;
 #pragma unroll
-    for (int r = 0; r < 32; ++r) t += acc[r][threadIdx.x];
+    for (int r = 0; r < kJoinRows; ++r) t += acc[r][lane];
     void* dst = col < dim ? dwq : dwk;
     const int c = col < dim ? col : col - dim;
     if (!dst) return;
@@ -364,13 +532,14 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_rope_any_kernel(HeadRows q,
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const HeadRows& t = blockIdx.y ? k : q;
   const int half = sh.half;
-  const int64_t rows = sh.tokens * t.heads;
+  const int64_t rows = (int64_t)sh.batch * sh.seq * t.heads;
   float dw1[kAnyPairs], dw2[kAnyPairs];
 #pragma unroll
   for (int j = 0; j < kAnyPairs; ++j) dw1[j] = dw2[j] = 0.f;
   for (int64_t r = (int64_t)blockIdx.x * kAnyWarps + warp; r < rows; r += (int64_t)gridDim.x * kAnyWarps) {
     const int64_t n = r / t.heads, hh = r - n * t.heads;
-    const int64_t b = n / sh.seq, s = n - b * sh.seq;
+    int64_t b, s;
+    sh.tiles.split((uint32_t)n, b, s);
     const T* xp = static_cast<const T*>(t.x) + b * t.xb + hh * t.xh + s * t.xs;
     const T* gp = BWD && NORM ? static_cast<const T*>(t.g) + b * t.gb + hh * t.gh + s * t.gs : nullptr;
     T* op = static_cast<T*>(t.out) + b * t.ob + hh * t.oh + s * t.os;
@@ -436,32 +605,39 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_rope_any_kernel(HeadRows q,
   }
 }
 
-// Threads of a CTA and rows of dw partials of the backward, from sizes alone (the
-// caller's workspace is sized by them).
-struct BwdPlan {
-  int threads, groups, blocks;  // groups: CTAs that share a token tile
+// Threads, groups of heads and blocks of a launch, from sizes alone (the caller's
+// workspace is sized by them).
+struct Plan {
+  int lanes, group_heads, groups, threads;
 };
+
+Plan plan_of(int heads, int half, int ne) {
+  Plan p;
+  p.lanes = 1;
+  while (p.lanes < half / ne) p.lanes <<= 1;
+  const int64_t slots = (int64_t)heads * p.lanes;
+  p.groups = (int)((slots + kMaxThreads - 1) / kMaxThreads);
+  p.group_heads = (heads + p.groups - 1) / p.groups;
+  p.groups = (heads + p.group_heads - 1) / p.group_heads;
+  p.threads = (p.group_heads * p.lanes + 31) / 32 * 32;
+  return p;
+}
 
 constexpr int kBwdTokens = 2;
 
-inline int row_lanes(int chunks) {
-  int l = 1;
-  while (l < chunks) l <<= 1;
-  return l;
+int64_t tiles_of(int64_t batch, int64_t seq, int tokens) { return batch * ((seq + tokens - 1) / tokens); }
+
+// CTAs along the tokens of a backward: three CTAs of 256 threads an SM in all.
+int bwd_blocks(int64_t batch, int64_t seq, const Plan& p) {
+  int64_t cap = (int64_t)num_sms() * (3 * kMaxThreads / p.threads) / p.groups;
+  if (cap < 1) cap = 1;
+  const int64_t tiles = tiles_of(batch, seq, kBwdTokens);
+  return (int)(tiles < cap ? tiles : cap);
 }
 
-BwdPlan bwd_plan(int64_t tokens, int64_t heads, int lanes) {
-  BwdPlan p;
-  const int64_t slots = heads * lanes;
-  p.threads = slots >= kMaxThreads ? kMaxThreads : (int)((slots + 31) / 32 * 32);
-  // whole heads in a block: lanes divides 32, so also the thread count
-  p.groups = (int)((slots + p.threads - 1) / p.threads);
-  int64_t cap = (int64_t)num_sms() * (p.threads <= 128 ? 6 : p.threads <= 256 ? 4 : 2) / p.groups;
-  if (cap < 1) cap = 1;
-  const int64_t tiles = (tokens + kBwdTokens - 1) / kBwdTokens;
-  p.blocks = (int)(tiles < cap ? tiles : cap);
-  return p;
-}
+// Elements of a half that a thread holds; 0: no vector form. Four also for 16-bit rows:
+// weights, shares of dw and four tokens' rows then fit 64 registers.
+int row_ne(int half) { return half % 4 == 0 && half / 4 <= 32 ? 4 : half % 8 == 0 && half / 8 <= 32 ? 8 : 0; }
 
 constexpr int kAnyBlocks = 592;  // of each tensor, at most
 
@@ -470,43 +646,65 @@ int any_blocks(int64_t tokens, int64_t heads) {
   return (int)(b < kAnyBlocks ? (b < 1 ? 1 : b) : kAnyBlocks);
 }
 
+// 16-byte aligned rows, tables and weights.
 bool rows_ok(const HeadRows& t, bool grads, int64_t es) {
-  if (t.heads == 0) return true;
   auto ok = [&](const void* p, int64_t b, int64_t h, int64_t s) {
     return aligned16(p) && (b * es) % 16 == 0 && (h * es) % 16 == 0 && (s * es) % 16 == 0;
   };
-  return ok(t.x, t.xb, t.xh, t.xs) && ok(t.out, t.ob, t.oh, t.os) && (!grads || ok(t.g, t.gb, t.gh, t.gs));
+  return ok(t.x, t.xb, t.xh, t.xs) && ok(t.out, t.ob, t.oh, t.os) && (!grads || ok(t.g, t.gb, t.gh, t.gs)) &&
+         (!t.w || aligned16(t.w));
 }
 
 template <typename T>
-bool vector_path(const HeadRows& q, const HeadRows& k, int half, bool grads) {
-  constexpr int NE = Vec16<T>::N;
-  return half % NE == 0 && half / NE <= 32 && rows_ok(q, grads, sizeof(T)) && rows_ok(k, grads, sizeof(T));
+bool vectors_ok(const HeadRows& q, const HeadRows& k, const Angles& a, int dtype, int half, int ne, bool grads) {
+  if (ne == 0 || half % ne || half / ne > 32 || (half * sizeof(T)) % 16 || !rows_ok(q, grads, sizeof(T)) ||
+      !rows_ok(k, grads, sizeof(T)))
+    return false;
+  if (!a.cos) return true;
+  const int64_t es = a.dtype == SOUP_F32 ? 4 : 2;
+  return (a.dtype == dtype || a.dtype == SOUP_F32) && aligned16(a.cos) && aligned16(a.sin) && (a.tb * es) % 16 == 0 &&
+         (a.ts * es) % 16 == 0;
+}
+
+template <typename T, int NE, int P, bool NORM>
+cudaError_t fwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, int src, dim3 grid,
+                       int threads, cudaStream_t st) {
+  switch (src) {
+    case kTableT: return launch_pdl(qk_rope_fwd_kernel<T, NE, P, NORM, kTableT>, grid, dim3(threads), 0, st, q, k, a, sh);
+    case kTableF: return launch_pdl(qk_rope_fwd_kernel<T, NE, P, NORM, kTableF>, grid, dim3(threads), 0, st, q, k, a, sh);
+    default: return launch_pdl(qk_rope_fwd_kernel<T, NE, P, NORM, kPositions>, grid, dim3(threads), 0, st, q, k, a, sh);
+  }
+}
+
+int source_of(const Angles& a, int dtype) {
+  return !a.cos ? kPositions : a.dtype == dtype && dtype != SOUP_F32 ? kTableT : kTableF;
 }
 
 template <typename T>
-int run_fwd(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, bool norm, cudaStream_t st) {
-  constexpr int NE = Vec16<T>::N;
-  const int heads = q.heads + k.heads;
+int run_fwd(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, bool norm, int dtype, cudaStream_t st) {
   cudaError_t e;
-  if (vector_path<T>(q, k, sh.half, false)) {
-    sh.lanes = row_lanes(sh.half / NE);
-    const int64_t slots = (int64_t)heads * sh.lanes;
-    int threads = slots >= 256 ? 256 : (int)((slots + 31) / 32 * 32);
-    // four tokens a CTA keep 128 bytes a thread in flight; with few tokens one a
-    // CTA, so that more SMs share them
-    if (sh.tokens >= 4 * (int64_t)num_sms()) {
-      const dim3 grid((unsigned)((sh.tokens + 3) / 4));
-      e = norm ? launch_pdl(qk_rope_fwd_kernel<T, 4, true>, grid, dim3(threads), 0, st, q, k, a, sh)
-               : launch_pdl(qk_rope_fwd_kernel<T, 4, false>, grid, dim3(threads), 0, st, q, k, a, sh);
-    } else {
-      const dim3 grid((unsigned)sh.tokens);
-      e = norm ? launch_pdl(qk_rope_fwd_kernel<T, 1, true>, grid, dim3(threads), 0, st, q, k, a, sh)
-               : launch_pdl(qk_rope_fwd_kernel<T, 1, false>, grid, dim3(threads), 0, st, q, k, a, sh);
-    }
+  const int ne = row_ne(sh.half);
+  if (vectors_ok<T>(q, k, a, dtype, sh.half, ne, false)) {
+    const Plan p = plan_of(q.heads + k.heads, sh.half, ne);
+    sh.lanes = p.lanes;
+    sh.group_heads = p.group_heads;
+    const int src = source_of(a, dtype);
+    // four tokens a thread in flight; with few tokens one, so that more SMs share them
+    const bool few = tiles_of(sh.batch, sh.seq, 4) < num_sms() || sh.seq < 4 || ne == 8;
+    const dim3 grid((unsigned)tiles_of(sh.batch, sh.seq, few ? 1 : 4), p.groups);
+    sh.tiles = make_div(few ? sh.seq : (sh.seq + 3) / 4);
+    if (ne == 8)
+      e = norm ? fwd_launch<T, 8, 1, true>(q, k, a, sh, src, grid, p.threads, st)
+               : fwd_launch<T, 8, 1, false>(q, k, a, sh, src, grid, p.threads, st);
+    else if (few)
+      e = norm ? fwd_launch<T, 4, 1, true>(q, k, a, sh, src, grid, p.threads, st)
+               : fwd_launch<T, 4, 1, false>(q, k, a, sh, src, grid, p.threads, st);
+    else
+      e = norm ? fwd_launch<T, 4, 4, true>(q, k, a, sh, src, grid, p.threads, st)
+               : fwd_launch<T, 4, 4, false>(q, k, a, sh, src, grid, p.threads, st);
   } else {
     const int most = q.heads > k.heads ? q.heads : k.heads;
-    const dim3 grid(any_blocks(sh.tokens, most), k.heads ? 2 : 1);
+    const dim3 grid(any_blocks((int64_t)sh.batch * sh.seq, most), 2);
     float* none = nullptr;
     e = norm ? launch_pdl(qk_rope_any_kernel<T, true, false>, grid, dim3(32 * kAnyWarps), 0, st, q, k, a, sh, none)
              : launch_pdl(qk_rope_any_kernel<T, false, false>, grid, dim3(32 * kAnyWarps), 0, st, q, k, a, sh, none);
@@ -514,32 +712,53 @@ int run_fwd(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, boo
   return cuda_status(e);
 }
 
+template <typename T, int NE>
+cudaError_t bwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, int src, bool dw, float* part,
+                       int* rows, cudaStream_t st) {
+  const Plan p = plan_of(q.heads + k.heads, sh.half, NE);
+  sh.lanes = p.lanes;
+  sh.group_heads = p.group_heads;
+  const int blocks = bwd_blocks(sh.batch, sh.seq, p);
+  sh.tiles = make_div((sh.seq + kBwdTokens - 1) / kBwdTokens);
+  *rows = blocks * p.groups;
+  size_t smem = sizeof(float) * (size_t)kBwdTokens * 2 * sh.half;
+  const size_t join = sizeof(float) * (size_t)p.threads * 2 * NE;
+  if (join > smem) smem = join;
+  const dim3 grid(blocks, p.groups), block(p.threads);
+  if (!dw) part = nullptr;
+  switch (src) {
+    case kTableT:
+      return launch_pdl(qk_norm_rope_bwd_kernel<T, NE, kBwdTokens, kTableT>, grid, block, smem, st, q, k, a, sh, part);
+    case kTableF:
+      return launch_pdl(qk_norm_rope_bwd_kernel<T, NE, kBwdTokens, kTableF>, grid, block, smem, st, q, k, a, sh, part);
+    default:
+      return launch_pdl(qk_norm_rope_bwd_kernel<T, NE, kBwdTokens, kPositions>, grid, block, smem, st, q, k, a, sh,
+                        part);
+  }
+}
+
 template <typename T>
 int run_bwd(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, void* dwq, void* dwk, float* part,
-            cudaStream_t st) {
-  constexpr int NE = Vec16<T>::N;
-  const int heads = q.heads + k.heads, dim = 2 * sh.half;
+            int dtype, cudaStream_t st) {
+  const int dim = 2 * sh.half;
   const bool dw = dwq || dwk;
   int rows;
   cudaError_t e;
-  if (vector_path<T>(q, k, sh.half, true)) {
-    sh.lanes = row_lanes(sh.half / NE);
-    const BwdPlan p = bwd_plan(sh.tokens, heads, sh.lanes);
-    size_t smem = sizeof(float) * (size_t)kBwdTokens * dim;
-    const size_t join = sizeof(float) * (size_t)p.threads * 2 * NE;
-    if (dw && join > smem) smem = join;
-    rows = p.blocks * p.groups;
-    e = launch_pdl(qk_norm_rope_bwd_kernel<T, kBwdTokens>, dim3(p.blocks, p.groups), dim3(p.threads), smem, st, q,
-                   k, a, sh, dw ? part : nullptr);
+  const int ne = row_ne(sh.half);
+  if (vectors_ok<T>(q, k, a, dtype, sh.half, ne, true)) {
+    const int src = source_of(a, dtype);
+    e = ne == 4 ? bwd_launch<T, 4>(q, k, a, sh, src, dw, part, &rows, st)
+                : bwd_launch<T, 8>(q, k, a, sh, src, dw, part, &rows, st);
   } else {
     const int most = q.heads > k.heads ? q.heads : k.heads;
-    rows = any_blocks(sh.tokens, most);
+    rows = any_blocks((int64_t)sh.batch * sh.seq, most);
     e = launch_pdl(qk_rope_any_kernel<T, true, true>, dim3(rows, 2), dim3(32 * kAnyWarps), 0, st, q, k, a, sh,
                    dw ? part : nullptr);
   }
   if (e != cudaSuccess || !dw) return cuda_status(e);
-  return cuda_status(launch_pdl(dw_join_kernel, dim3((2 * dim + 31) / 32), dim3(32, 32), 0, st,
-                                static_cast<const float*>(part), rows, dim, dwq, dwk, sh.w_dtype));
+  return cuda_status(launch_pdl(dw_join_kernel, dim3((2 * dim + kJoinCols - 1) / kJoinCols),
+                                dim3(kJoinCols * kJoinRows), 0, st, static_cast<const float*>(part), rows, dim, dwq,
+                                dwk, sh.w_dtype));
 }
 
 bool fill_angles(Angles& a, const void* cos, const void* sin, int64_t tb, int64_t ts, int dtype, const void* pos,
@@ -575,13 +794,13 @@ extern "C" {
 size_t soup_qk_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t hq, int64_t hk,
                                              int64_t head_dim) {
   if (batch <= 0 || seq <= 0 || hq <= 0 || hk <= 0 || head_dim <= 0) return 0;
-  // the most partial rows any dtype and alignment gives
+  // the more partial rows of the two forms
   const int64_t tokens = batch * seq;
   int64_t rows = any_blocks(tokens, hq > hk ? hq : hk);
-  for (int ne = 4; ne <= 8; ne += 4) {
-    if ((head_dim / 2) % ne || head_dim / 2 / ne > 32) continue;
-    const BwdPlan p = bwd_plan(tokens, hq + hk, row_lanes((int)(head_dim / 2 / ne)));
-    if ((int64_t)p.blocks * p.groups > rows) rows = (int64_t)p.blocks * p.groups;
+  if (const int ne = row_ne((int)(head_dim / 2))) {
+    const Plan p = plan_of((int)(hq + hk), (int)(head_dim / 2), ne);
+    const int64_t r = (int64_t)bwd_blocks(batch, seq, p) * p.groups;
+    if (r > rows) rows = r;
   }
   return sizeof(float) * (size_t)(rows * 2 * head_dim);
 }
@@ -596,7 +815,7 @@ int soup_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, cons
   const bool norm = q_weight || k_weight;
   if (!q || !q_strides || !q_out || !q_out_strides || hq <= 0 || !k || !k_strides || !k_out || !k_out_strides ||
       hk <= 0 || batch <= 0 || seq <= 0 || head_dim <= 0 || head_dim % 2 || head_dim > kMaxDim || hq > 4096 ||
-      hk > 4096 || batch > (int64_t(1) << 31) / seq || (norm && (!q_weight || !k_weight || inverse))) {
+      hk > 4096 || batch >= (int64_t(1) << 31) / seq || (norm && (!q_weight || !k_weight || inverse))) {
     set_last_error("soup_qk_norm_rope: bad arguments");
     return SOUP_ERR_INVALID;
   }
@@ -610,11 +829,11 @@ int soup_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, cons
               q_out_strides[0], q_out_strides[1], q_out_strides[2], q_weight, (int)hq};
   HeadRows tk{k, nullptr, k_out, k_strides[0], k_strides[1], k_strides[2], 0, 0, 0,
               k_out_strides[0], k_out_strides[1], k_out_strides[2], k_weight, (int)hk};
-  Shape sh{batch * seq, seq, (int)(head_dim / 2), 32, eps, w_dtype, inverse ? -1.f : 1.f};
+  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, eps, 1.f / (float)head_dim, w_dtype, inverse ? -1.f : 1.f};
   cudaStream_t st = as_stream(stream);
-  if (dtype == SOUP_BF16) return run_fwd<__nv_bfloat16>(tq, tk, a, sh, norm, st);
-  if (dtype == SOUP_F16) return run_fwd<__half>(tq, tk, a, sh, norm, st);
-  if (dtype == SOUP_F32) return run_fwd<float>(tq, tk, a, sh, norm, st);
+  if (dtype == SOUP_BF16) return run_fwd<__nv_bfloat16>(tq, tk, a, sh, norm, dtype, st);
+  if (dtype == SOUP_F16) return run_fwd<__half>(tq, tk, a, sh, norm, dtype, st);
+  if (dtype == SOUP_F32) return run_fwd<float>(tq, tk, a, sh, norm, dtype, st);
   set_last_error("soup_qk_norm_rope: unsupported dtype");
   return SOUP_ERR_INVALID;
 }
@@ -631,7 +850,7 @@ int soup_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_out_strides, con
   if (!dq_out || !dq_out_strides || !q || !q_strides || !dq || !dq_strides || hq <= 0 || !dk_out ||
       !dk_out_strides || !k || !k_strides || !dk || !dk_strides || hk <= 0 || !q_weight || !k_weight || batch <= 0 ||
       seq <= 0 || head_dim <= 0 || head_dim % 2 || head_dim > kMaxDim || hq > 4096 || hk > 4096 ||
-      batch > (int64_t(1) << 31) / seq) {
+      batch >= (int64_t(1) << 31) / seq) {
     set_last_error("soup_qk_norm_rope_bwd: bad arguments");
     return SOUP_ERR_INVALID;
   }
@@ -653,12 +872,12 @@ int soup_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_out_strides, con
   HeadRows tk{k, dk_out, dk, k_strides[0], k_strides[1], k_strides[2],
               dk_out_strides[0], dk_out_strides[1], dk_out_strides[2],
               dk_strides[0], dk_strides[1], dk_strides[2], k_weight, (int)hk};
-  Shape sh{batch * seq, seq, (int)(head_dim / 2), 32, eps, w_dtype, 1.f};
+  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, eps, 1.f / (float)head_dim, w_dtype, 1.f};
   float* part = static_cast<float*>(workspace);
   cudaStream_t st = as_stream(stream);
-  if (dtype == SOUP_BF16) return run_bwd<__nv_bfloat16>(tq, tk, a, sh, dq_weight, dk_weight, part, st);
-  if (dtype == SOUP_F16) return run_bwd<__half>(tq, tk, a, sh, dq_weight, dk_weight, part, st);
-  if (dtype == SOUP_F32) return run_bwd<float>(tq, tk, a, sh, dq_weight, dk_weight, part, st);
+  if (dtype == SOUP_BF16) return run_bwd<__nv_bfloat16>(tq, tk, a, sh, dq_weight, dk_weight, part, dtype, st);
+  if (dtype == SOUP_F16) return run_bwd<__half>(tq, tk, a, sh, dq_weight, dk_weight, part, dtype, st);
+  if (dtype == SOUP_F32) return run_bwd<float>(tq, tk, a, sh, dq_weight, dk_weight, part, dtype, st);
   set_last_error("soup_qk_norm_rope_bwd: unsupported dtype");
   return SOUP_ERR_INVALID;
 }

@@ -189,8 +189,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         params, ptrs = held.params, held.ptrs
         for code, idx, sizes, blocks in held.by_dtype:
             grads = [params[i].grad for i in idx]
-            if None in grads:
-                keep = [(i, g) for i, g in zip(idx, grads) if g is not None]
+            keep = [(i, g) for i, g in zip(idx, grads) if g is not None]
+            if len(keep) < len(idx):
                 if not keep:
                     continue
                 idx = [i for i, _ in keep]
