@@ -21,7 +21,8 @@
 //
 // A warp takes blocks of 256: 8 elements a lane in two 16-byte loads (one for 16-bit
 // tensors), the maxima by one integer reduction each, the arithmetic on packed pairs.
-// A CTA takes 4096 elements at a time and a contiguous run of such chunks over all tensors, whose table (pointers and sizes)
+// A CTA takes a contiguous run of blocks over all tensors, its warps in turns with the
+// next block's loads in flight; the tensors' table (pointers and sizes)
 // comes as a kernel argument, so that a launch needs no copy and can be captured.
 #include <cuda_fp8.h>
 #include <stdio.h>
@@ -35,8 +36,6 @@ namespace {
 
 constexpr int kBlock = 256;              // elements that share a scale
 constexpr int kWarps = 8;
-constexpr int kBlocksPerWarp = 2;
-constexpr int kChunk = kBlock * kWarps * kBlocksPerWarp;  // elements of a CTA's turn
 constexpr int kThreads = 32 * kWarps;
 constexpr float kE4m3Max = 448.f;
 
@@ -45,17 +44,17 @@ struct Tensor {
   const void* g;
   int64_t n;
   int block0;   // first state block
-  int chunk0;   // chunks of the tensors before it in this launch
+  int first;    // blocks of the tensors before it in this launch
 };
 
 template <int N>
 struct Table {
-  int count, chunks;
+  int count, blocks;
   Tensor t[N];
 };
 
-// resident CTAs of the step's kernel on an SM (85 or 51 registers a thread)
-__host__ __device__ constexpr int ctas_per_sm(bool eight) { return eight ? 3 : 5; }
+// resident CTAs of the step's kernel on an SM (80 registers a thread)
+constexpr int kStepCtas = 3;
 
 struct Hyper {
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, lr, decay;  // decay: 1 - lr wd
@@ -70,21 +69,22 @@ struct States {
   float* v_scale;
 };
 
-// The tensor that holds chunk c.
+// The tensor that holds block c of the launch.
 template <int N>
 __device__ __forceinline__ int find_tensor(const Table<N>& tab, int c) {
   int lo = 0, hi = tab.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (tab.t[mid].chunk0 <= c) lo = mid;
+    if (tab.t[mid].first <= c) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
 
-__device__ __forceinline__ void chunk_run(int chunks, int& c0, int& c1) {
-  c0 = (int)((int64_t)chunks * blockIdx.x / gridDim.x);
-  c1 = (int)((int64_t)chunks * (blockIdx.x + 1) / gridDim.x);
+// The CTA's run of blocks, a contiguous one; its warps take turns in it.
+__device__ __forceinline__ void block_run(int blocks, int& c0, int& c1) {
+  c0 = (int)((int64_t)blocks * blockIdx.x / gridDim.x);
+  c1 = (int)((int64_t)blocks * (blockIdx.x + 1) / gridDim.x);
 }
 
 // Pairs of elements in packed 32-bit arithmetic: one instruction for two.
@@ -251,22 +251,32 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
   pdl_wait();
   pdl_trigger();
   int c0, c1;
-  chunk_run(tab.chunks, c0, c1);
+  block_run(tab.blocks, c0, c1);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum = 0.0;
-  int ti = c0 < c1 ? find_tensor(tab, c0) : 0;
-  for (int c = c0; c < c1; ++c) {
-    while (ti + 1 < tab.count && tab.t[ti + 1].chunk0 <= c) ++ti;
-    const Tensor& t = tab.t[ti];
-    const bool vec = (reinterpret_cast<uintptr_t>(t.g) & 15) == 0;
-    Raw8<T> g[kBlocksPerWarp];
+  int ti = c0 < c1 ? find_tensor(tab, min(c0 + warp, c1 - 1)) : 0;
+  constexpr int U = 4;  // blocks of a warp in flight
+  for (int c = c0 + warp; c < c1; c += U * kWarps) {
+    Raw8<T> g[U];
 #pragma unroll
-    for (int u = 0; u < kBlocksPerWarp; ++u) {
-      const int64_t e = (int64_t)(c - t.chunk0) * kChunk + (u * kThreads + threadIdx.x) * 8;
-      const int64_t rest = t.n - e;
-      g[u].load(static_cast<const T*>(t.g) + e, rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest, vec);
+    for (int u = 0; u < U; ++u) {
+      const int blk = c + u * kWarps;
+      int left = 0;
+      const T* at = nullptr;
+      bool vec = false;
+      if (blk < c1) {
+        while (ti + 1 < tab.count && tab.t[ti + 1].first <= blk) ++ti;
+        const Tensor& t = tab.t[ti];
+        const int64_t e = (int64_t)(blk - t.first) * kBlock + lane * 8;
+        const int64_t rest = t.n - e;
+        left = rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest;
+        at = static_cast<const T*>(t.g) + e;
+        vec = (reinterpret_cast<uintptr_t>(t.g) & 15) == 0;
+      }
+      g[u].load(at, left, vec);
     }
 #pragma unroll
-    for (int u = 0; u < kBlocksPerWarp; ++u) {
+    for (int u = 0; u < U; ++u) {
       uint64_t sq = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) sq = f2_fma(g[u].pair(i), g[u].pair(i), sq);
@@ -292,7 +302,7 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
 // `step` counts the steps done; `ticket` is 0 between launches. The last CTA of the
 // step's last launch (bump) raises the count after every CTA has read it.
 template <typename T, bool EIGHT, int N>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(EIGHT)) adamw_multi_kernel(const __grid_constant__ Table<N> tab, States st,
+__global__ void __launch_bounds__(kThreads, kStepCtas) adamw_multi_kernel(const __grid_constant__ Table<N> tab, States st,
                                                                Hyper h, const double* __restrict__ partial,
                                                                int partials, float* __restrict__ norm_out,
                                                                float* __restrict__ step, int* __restrict__ ticket,
@@ -324,111 +334,115 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(EIGHT)) adamw_multi_kern
   const uint64_t step_size = f2_same(-coefs[0]), root_scale = f2_same(coefs[1]), clip = f2_same(coefs[2]);
   const uint64_t c1 = f2_same(h.one_minus_beta1), c2 = f2_same(h.one_minus_beta2), b2 = f2_same(h.beta2);
   const uint64_t eps = f2_same(h.eps), decay = f2_same(h.decay), minus = f2_same(-1.f);
-  int first, end;
-  chunk_run(tab.chunks, first, end);
+  int begin, end;
+  block_run(tab.blocks, begin, end);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int ti = first < end ? find_tensor(tab, first) : 0;
-  for (int c = first; c < end; ++c) {
-    while (ti + 1 < tab.count && tab.t[ti + 1].chunk0 <= c) ++ti;
+  int ti = begin < end ? find_tensor(tab, min(begin + warp, end - 1)) : 0;
+
+  // what a lane holds of a block; the next block's is in flight while one is computed
+  struct Held {
+    Raw8<T> p, g;
+    Raw8<float> m, v;  // 32 bits
+    uint2 mc, vc;      // 8 bits
+    float ms, vs;
+    T* out;
+    int left;
+    bool vec;
+    int64_t blk;
+  };
+  auto load = [&](int c, Held& d) {
+    while (ti + 1 < tab.count && tab.t[ti + 1].first <= c) ++ti;
     const Tensor& t = tab.t[ti];
-    const bool vp = (reinterpret_cast<uintptr_t>(t.p) & 15) == 0, vg = (reinterpret_cast<uintptr_t>(t.g) & 15) == 0;
-    // the warp's kUnroll blocks of the chunk, all loads first
-    constexpr int U = EIGHT ? 2 : 1;
-    constexpr int kTurns = kBlocksPerWarp / U;
-#pragma unroll 1
-    for (int turn = 0; turn < kTurns; ++turn) {
-      Raw8<T> p[U], g[U];
-      Raw8<float> m32[EIGHT ? 1 : U], v32[EIGHT ? 1 : U];
-      uint2 mc[U], vc[U];
-      float ms[U], vs[U];
-      int left[U];
-      int64_t e[U], at[U];
-      int64_t blk[U];
+    const int64_t e = (int64_t)(c - t.first) * kBlock + lane * 8;
+    const int64_t rest = t.n - e;
+    d.left = rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest;
+    d.blk = t.block0 + (c - t.first);
+    d.vec = (reinterpret_cast<uintptr_t>(t.p) & 15) == 0;
+    d.out = static_cast<T*>(t.p) + e;
+    d.g.load(static_cast<const T*>(t.g) + e, d.left, (reinterpret_cast<uintptr_t>(t.g) & 15) == 0);
+    d.p.load(d.out, d.left, d.vec);
+    const int64_t at = d.blk * kBlock + lane * 8;
+    if constexpr (EIGHT) {
+      d.mc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.m) + at));
+      d.vc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.v) + at));
+      d.ms = st.m_scale[d.blk];
+      d.vs = st.v_scale[d.blk];
+    } else {
+      d.m.load(static_cast<const float*>(st.m) + at, 8, true);
+      d.v.load(static_cast<const float*>(st.v) + at, 8, true);
+    }
+  };
+  auto update = [&](Held& d) {
+    uint64_t m[4], v[4], root[4];
+    const uint64_t msc = EIGHT ? f2_same(d.ms) : 0, vsc = EIGHT ? f2_same(d.vs) : 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t w0 = (int64_t)(c - t.chunk0) * kChunk + ((turn * U + u) * kWarps + warp) * kBlock;
-        e[u] = w0 + lane * 8;
-        const int64_t rest = t.n - e[u];
-        left[u] = rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest;
-        blk[u] = t.block0 + (w0 >> 8);
-        at[u] = blk[u] * kBlock + lane * 8;
-        if (w0 >= t.n) {  // no such block: warp-uniform
-          blk[u] = -1;
-          continue;
-        }
-        g[u].load(static_cast<const T*>(t.g) + e[u], left[u], vg);
-        p[u].load(static_cast<const T*>(t.p) + e[u], left[u], vp);
-        if constexpr (EIGHT) {
-          mc[u] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.m) + at[u]));
-          vc[u] = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.v) + at[u]));
-          ms[u] = st.m_scale[blk[u]];
-          vs[u] = st.v_scale[blk[u]];
-        } else {
-          m32[u].load(static_cast<const float*>(st.m) + at[u], 8, true);
-          v32[u].load(static_cast<const float*>(st.v) + at[u], 8, true);
-        }
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (EIGHT) {
+        m[i] = f2_mul(pair_of_codes(d.mc, i), msc);
+        v[i] = f2_mul(pair_of_codes(d.vc, i), vsc);
+        v[i] = f2_mul(v[i], v[i]);
+      } else {
+        m[i] = d.m.pair(i);
+        v[i] = d.v.pair(i);
       }
+      const uint64_t gi = f2_mul(d.g.pair(i), clip);
+      m[i] = f2_fma(c1, f2_fma(m[i], minus, gi), m[i]);
+      v[i] = f2_fma(f2_mul(c2, gi), gi, f2_mul(v[i], b2));
+      float lo, hi;
+      f2_unpack(v[i], lo, hi);
+      root[i] = f2_pack(root_approx(lo), root_approx(hi));
+      f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
+      const uint64_t inv = f2_pack(recip_approx(lo), recip_approx(hi));
+      d.p.set(i, f2_fma(f2_mul(m[i], step_size), inv, f2_mul(d.p.pair(i), decay)));
+    }
+    d.p.store(d.out, d.left, d.vec);
+    if (d.left < 8) {
+      // what lies behind a tensor's end stays 0
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (blk[u] < 0) continue;
-        uint64_t m[4], v[4], root[4];
-        const uint64_t msc = EIGHT ? f2_same(ms[u]) : 0, vsc = EIGHT ? f2_same(vs[u]) : 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (EIGHT) {
-            m[i] = f2_mul(pair_of_codes(mc[u], i), msc);
-            v[i] = f2_mul(pair_of_codes(vc[u], i), vsc);
-            v[i] = f2_mul(v[i], v[i]);
-          } else {
-            m[i] = m32[u].pair(i);
-            v[i] = v32[u].pair(i);
-          }
-          const uint64_t gi = f2_mul(g[u].pair(i), clip);
-          m[i] = f2_fma(c1, f2_fma(m[i], minus, gi), m[i]);
-          v[i] = f2_fma(f2_mul(c2, gi), gi, f2_mul(v[i], b2));
-          float lo, hi;
-          f2_unpack(v[i], lo, hi);
-          root[i] = f2_pack(root_approx(lo), root_approx(hi));
-          f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
-          const uint64_t inv = f2_pack(recip_approx(lo), recip_approx(hi));
-          p[u].set(i, f2_fma(f2_mul(m[i], step_size), inv, f2_mul(p[u].pair(i), decay)));
-        }
-        p[u].store(static_cast<T*>(t.p) + e[u], left[u], vp);
-        if (left[u] < 8) {
-          // what lies behind a tensor's end stays 0
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool a = 2 * i < left[u], b = 2 * i + 1 < left[u];
-            float x, y;
-            f2_unpack(m[i], x, y);
-            m[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
-            f2_unpack(v[i], x, y);
-            v[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
-            f2_unpack(root[i], x, y);
-            root[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
-          }
-        }
-        if constexpr (EIGHT) {
-          float sm, sv;
-          const uint2 cm = to_codes<false>(m, sm);
-          const uint2 cv = to_codes<true>(root, sv);
-          __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m) + at[u]), cm);
-          __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v) + at[u]), cv);
-          if (lane == 0) {
-            st.m_scale[blk[u]] = sm;
-            st.v_scale[blk[u]] = sv;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            m32[u].set(i, m[i]);
-            v32[u].set(i, v[i]);
-          }
-          m32[u].store(static_cast<float*>(st.m) + at[u], 8, true);
-          v32[u].store(static_cast<float*>(st.v) + at[u], 8, true);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const bool a = 2 * i < d.left, b = 2 * i + 1 < d.left;
+        float x, y;
+        f2_unpack(m[i], x, y);
+        m[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
+        f2_unpack(v[i], x, y);
+        v[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
+        f2_unpack(root[i], x, y);
+        root[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
       }
     }
+    const int64_t at = d.blk * kBlock + lane * 8;
+    if constexpr (EIGHT) {
+      float sm, sv;
+      const uint2 cm = to_codes<false>(m, sm);
+      const uint2 cv = to_codes<true>(root, sv);
+      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m) + at), cm);
+      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v) + at), cv);
+      if (lane == 0) {
+        st.m_scale[d.blk] = sm;
+        st.v_scale[d.blk] = sv;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        d.m.set(i, m[i]);
+        d.v.set(i, v[i]);
+      }
+      d.m.store(static_cast<float*>(st.m) + at, 8, true);
+      d.v.store(static_cast<float*>(st.v) + at, 8, true);
+    }
+  };
+  // two blocks in turn: one in flight, one computed
+  Held a, b;
+  int c = begin + warp;
+  if (c < end) load(c, a);
+  while (c < end) {
+    c += kWarps;
+    if (c < end) load(c, b);
+    update(a);
+    if (c >= end) break;
+    c += kWarps;
+    if (c < end) load(c, a);
+    update(b);
   }
   if (bump && threadIdx.x == 0) {
     // every CTA has read the count before its ticket
@@ -443,11 +457,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(EIGHT)) adamw_multi_kern
 constexpr int kSquareCtas = 6;              // of grad_square_kernel on an SM, each with a partial sum
 constexpr int kSmall = 64, kLarge = 960;  // tensors of a launch: arguments of 2 and 30 KB
 
-inline int chunks_of(int64_t n) { return (int)((n + kChunk - 1) / kChunk); }
+inline int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
-inline int grid_of(int chunks, int per_sm) {
-  const int cap = num_sms() * per_sm;
-  return chunks < cap ? (chunks < 1 ? 1 : chunks) : cap;
+// CTAs of a launch: a block for every warp, as far as they are resident together
+inline int grid_of(int blocks, int per_sm) {
+  const int cap = num_sms() * per_sm, want = (blocks + kWarps - 1) / kWarps;
+  return want < cap ? want : cap;
 }
 
 struct Args {
@@ -458,26 +473,26 @@ struct Args {
   int count;
 };
 
-// Tensors [i0, i1) into a table; returns the chunks.
+// Tensors [i0, i1) into a table.
 template <int N>
 void fill_table(Table<N>& tab, const Args& a, int i0, int i1) {
-  int chunks = 0;
+  int blocks = 0;
   for (int i = i0; i < i1; ++i) {
-    tab.t[i - i0] = Tensor{a.params ? a.params[i] : nullptr, a.grads[i], a.sizes[i], a.blocks ? a.blocks[i] : 0, chunks};
-    chunks += chunks_of(a.sizes[i]);
+    tab.t[i - i0] = Tensor{a.params ? a.params[i] : nullptr, a.grads[i], a.sizes[i], a.blocks ? a.blocks[i] : 0, blocks};
+    blocks += (int)blocks_of(a.sizes[i]);
   }
   tab.count = i1 - i0;
-  tab.chunks = chunks;
+  tab.blocks = blocks;
 }
 
-// The end of the launch that starts with tensor i0: at most `most` tensors and 2^30 chunks.
+// The end of the launch that starts with tensor i0: at most `most` tensors and 2^30 blocks
+// (a tensor has at most as many).
 int launch_end(const Args& a, int i0, int most) {
-  int64_t chunks = 0;
+  int64_t blocks = 0;
   int i = i0;
   while (i < a.count && i - i0 < most) {
-    const int64_t c = chunks_of(a.sizes[i]);
-    if (i > i0 && chunks + c > (1 << 30)) break;
-    chunks += c;
+    blocks += blocks_of(a.sizes[i]);
+    if (i > i0 && blocks > (1 << 30)) break;
     ++i;
   }
   return i;
@@ -503,7 +518,7 @@ template <typename T, int N>
 int square_launch(const Args& a, int i0, int i1, double* partial, int* used, cudaStream_t st) {
   Table<N> tab;
   fill_table(tab, a, i0, i1);
-  const int grid = grid_of(tab.chunks, kSquareCtas);
+  const int grid = grid_of(tab.blocks, kSquareCtas);
   *used += grid;
   return launch_table(grad_square_kernel<T, N>, grid, st, tab, partial);
 }
@@ -513,7 +528,7 @@ int step_launch(const Args& a, int i0, int i1, const States& s, const Hyper& h, 
                 float* norm_out, float* step, int* ticket, int bump, cudaStream_t st) {
   Table<N> tab;
   fill_table(tab, a, i0, i1);
-  return launch_table(adamw_multi_kernel<T, EIGHT, N>, grid_of(tab.chunks, ctas_per_sm(EIGHT)), st, tab, s, h, partial, partials, norm_out,
+  return launch_table(adamw_multi_kernel<T, EIGHT, N>, grid_of(tab.blocks, kStepCtas), st, tab, s, h, partial, partials, norm_out,
                       step, ticket, bump);
 }
 

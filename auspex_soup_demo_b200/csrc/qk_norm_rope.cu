@@ -16,11 +16,13 @@
 //
 // A row (token, head) is `lanes` threads of one warp, each with NE elements of the
 // first half and the matching NE of the second, so a rotation needs no exchange and a
-// norm needs log2(lanes) shuffles. A thread keeps its (head, elements) slot for P
-// tokens, whose loads are in flight together. cos and sin come by vector loads beside
-// them, or, from positions, through a table that the CTA forms in shared memory. Head
-// dims whose half is not a multiple of a vector, or rows that are not 16-byte aligned,
-// take a warp per row instead.
+// norm needs log2(lanes) shuffles. A CTA walks a run of tokens; a thread keeps its
+// (head, elements) slot for all of them. Its rows arrive by cp.async in a ring of
+// shared memory of its own (nobody else reads them, so no barrier), several tokens
+// ahead, which keeps enough bytes in flight without the registers for them. Head dims
+// whose half is not a multiple of a vector, or rows that are not 16-byte aligned, take
+// a warp per row instead.
+#include <mutex>
 #include <type_traits>
 
 #include "soup_common.cuh"
@@ -31,6 +33,11 @@ namespace {
 constexpr int kMaxDim = 512;        // head dim
 constexpr int kMaxHalf = kMaxDim / 2;
 constexpr int kMaxThreads = 256;
+// Stages of a thread's ring, and resident CTAs of 256 threads on an SM by the bytes of a
+// half that a thread holds: the rings take 128 to 196 KB of an SM's shared memory.
+constexpr int kFwdStages = 4, kBwdStages = 4;
+__host__ __device__ constexpr int fwd_ctas(int bytes) { return bytes == 16 ? 3 : 2; }
+__host__ __device__ constexpr int bwd_ctas(int bytes) { return bytes == 16 ? 2 : 1; }
 
 struct HeadRows {
   const void* x;       // q or k
@@ -77,7 +84,7 @@ inline Div make_div(int64_t d) {
 
 struct Shape {
   int batch, seq;
-  Div tiles;           // of a sequence: of P tokens (qk_rope_any_kernel: of one)
+  Div tokens;          // of a sequence
   int half;
   int lanes;           // threads of a row (a power of two)
   int group_heads;     // heads of a CTA
@@ -212,21 +219,6 @@ __device__ __forceinline__ void load_weights(const void* w, int at, int dtype, u
   }
 }
 
-// The tables of tokens [s0, s0 + P) of sequence b into shared memory (cos, then sin).
-template <int P>
-__device__ __forceinline__ void fill_tables(const Angles& a, const Shape& sh, int64_t b, int64_t s0, float* tab) {
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    if (s0 + p >= sh.seq) break;
-    for (int i = threadIdx.x; i < sh.half; i += blockDim.x) {
-      float c, sn;
-      turn(a, b, s0 + p, i, c, sn);
-      tab[p * 2 * sh.half + i] = c;
-      tab[(p * 2 + 1) * sh.half + i] = sn;
-    }
-  }
-}
-
 // A thread's slot: its rows and its place in them.
 struct Slot {
   bool on, isq;
@@ -244,7 +236,7 @@ struct Slot {
   }
 };
 
-// cos and sin of a thread's elements for a token, p-th of the CTA's.
+// cos and sin of a thread's elements for a token.
 template <typename T, int NE, int SRC>
 struct Turn {
   using TT = typename TableType<T, SRC>::type;
@@ -253,216 +245,297 @@ struct Turn {
     c.template load<false>(cos);
     s.template load<false>(sin);
   }
-  __device__ __forceinline__ void take(const float* tab, int p, int half, int d) {
-    if constexpr (SRC == kPositions) {
-      c.template load<false>(tab + p * 2 * half + d);
-      s.template load<false>(tab + (p * 2 + 1) * half + d);
-    }
+};
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A place in a run of tokens: their sequence and position, and the offset of the
+// thread's elements in one strided tensor (or of the tables' row).
+struct Cursor {
+  int64_t at, step, wrap;  // wrap: from the last token of a sequence to the next one's first
+  int s;
+  __device__ __forceinline__ Cursor(int64_t b, int64_t s0, int64_t sb, int64_t ss, int seq)
+      : at(b * sb + s0 * ss), step(ss), wrap(sb - (int64_t)(seq - 1) * ss), s((int)s0) {}
+  __device__ __forceinline__ void next(int seq) {
+    const bool last = ++s == seq;
+    at += last ? wrap : step;
+    if (last) s = 0;
   }
 };
 
+constexpr int kGroup = 4;  // tokens whose tables a CTA forms together (kPositions)
+
+// The tables of tokens [n0, n0 + kGroup) of the run's end n1 into shared memory.
+__device__ __forceinline__ void fill_tables(const Angles& a, const Shape& sh, int n0, int n1, float* tab) {
+  for (int e = threadIdx.x; e < kGroup * sh.half; e += blockDim.x) {
+    const int p = e / sh.half, i = e - p * sh.half;
+    if (n0 + p >= n1) break;
+    int64_t b, s;
+    sh.tokens.split(n0 + p, b, s);
+    float c, sn;
+    turn(a, b, s, i, c, sn);
+    tab[p * 2 * sh.half + i] = c;
+    tab[(p * 2 + 1) * sh.half + i] = sn;
+  }
+}
+
+// The CTA's run of tokens.
+__device__ __forceinline__ void token_run(const Shape& sh, int& n0, int& n1) {
+  const int64_t total = (int64_t)sh.batch * sh.seq;
+  n0 = (int)(total * blockIdx.x / gridDim.x);
+  n1 = (int)(total * (blockIdx.x + 1) / gridDim.x);
+}
+
+// Walks the run: ring of S stages of PIECES 16-byte pieces a thread, filled by
+// issue(token's stage address), tables from `src`, then work(stage address, tables).
+template <int S, int SRC, class Issue, class Work>
+__device__ __forceinline__ void walk_tokens(const Angles& ang, const Shape& sh, float* tab, uint32_t ring,
+                                            uint32_t stage_bytes, Issue&& issue, Work&& work) {
+  int n0, n1;
+  token_run(sh, n0, n1);
+  int put = 0;
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i) {
+    if (n0 + i < n1) issue(ring + put * stage_bytes);
+    copy_commit();
+    put = put + 1 == S ? 0 : put + 1;
+  }
+  int get = 0;
+  for (int n = n0; n < n1; ++n) {
+    if (n + S - 1 < n1) issue(ring + put * stage_bytes);
+    copy_commit();
+    put = put + 1 == S ? 0 : put + 1;
+    const float* table = tab;
+    if constexpr (SRC == kPositions) {
+      // two groups' tables in turn: what a group overwrites was read before the last barrier
+      const int g = n - n0;
+      float* mine = tab + (g / kGroup & 1) * kGroup * 2 * sh.half;
+      if (g % kGroup == 0) {
+        fill_tables(ang, sh, n, n1, mine);
+        __syncthreads();
+      }
+      table = mine + g % kGroup * 2 * sh.half;
+    }
+    copy_wait<S - 1>();
+    work(ring + get * stage_bytes, table);
+    get = get + 1 == S ? 0 : get + 1;
+  }
+}
+
+// A piece is NE elements of every thread: 16-byte parts, `pitch` (16 x threads) apart.
+template <typename T, int NE>
+__device__ __forceinline__ void take(Pack<T, NE>& p, uint32_t at, uint32_t pitch) {
+#pragma unroll
+  for (int i = 0; i < Pack<T, NE>::kWords; i += 4)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(p.u[i]), "=r"(p.u[i + 1]), "=r"(p.u[i + 2]), "=r"(p.u[i + 3])
+                 : "r"(at + i / 4 * pitch)
+                 : "memory");
+}
+template <typename T, int NE>
+__device__ __forceinline__ void give(uint32_t at, const T* src, uint32_t pitch) {
+#pragma unroll
+  for (int i = 0; i < Pack<T, NE>::kWords; i += 4) copy16(at + i / 4 * pitch, src + i * 4 / sizeof(T));
+}
+
 // Forward (and, without weights and with sign -1, the backward of a rotation alone).
-// CTA (x, y): P tokens of a sequence, heads [y group_heads, ...).
-template <typename T, int NE, int P, bool NORM, int SRC>
-__global__ void __launch_bounds__(kMaxThreads, NE == 8 ? 2 : P == 4 ? 3 : 4) qk_rope_fwd_kernel(
+template <typename T, int NE, bool NORM, int SRC>
+__global__ void __launch_bounds__(kMaxThreads, fwd_ctas(NE * (int)sizeof(T))) qk_rope_fwd_kernel(
     HeadRows q, HeadRows k, const __grid_constant__ Angles ang, Shape sh) {
   using Tr = Turn<T, NE, SRC>;
-  __shared__ __align__(16) float tab[SRC == kPositions ? P * 2 * kMaxHalf : 4];
+  using TT = typename Tr::TT;
+  extern __shared__ __align__(16) uint8_t smem[];  // ring, then (kPositions) two groups' tables
   pdl_wait();
-  pdl_trigger();
   const int half = sh.half;
-  int64_t b, s0;
-  sh.tiles.split(blockIdx.x, b, s0);
-  s0 *= P;
-  const int n = min((int)(sh.seq - s0), P);
   const Slot slot(q, k, sh, NE);
   const HeadRows& t = slot.isq ? q : k;
-  const T* xp = static_cast<const T*>(t.x) + slot.hh * t.xh + slot.d + b * t.xb + s0 * t.xs;
-  T* op = static_cast<T*>(t.out) + slot.hh * t.oh + slot.d + b * t.ob + s0 * t.os;
-  const typename Tr::TT *cp = nullptr, *sp = nullptr;
-  if constexpr (SRC != kPositions) {
-    const int64_t at = b * ang.tb + s0 * ang.ts + slot.d;
-    cp = static_cast<const typename Tr::TT*>(ang.cos) + at;
-    sp = static_cast<const typename Tr::TT*>(ang.sin) + at;
-  }
-  Pack<T, NE> x1[P], x2[P];
-  Tr tr[P];
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    x1[p].zero();
-    x2[p].zero();
-    if (slot.on && p < n) {
-      x1[p].template load<true>(xp);
-      x2[p].template load<true>(xp + half);
-      if constexpr (SRC != kPositions) {
-        tr[p].load(cp, sp);
-        cp += ang.ts;
-        sp += ang.ts;
-      }
-      xp += t.xs;
-    }
-  }
-  if constexpr (SRC == kPositions) {
-    fill_tables<P>(ang, sh, b, s0, tab);
-    __syncthreads();
-  }
-  float rstd[P];
+  const T* x = static_cast<const T*>(t.x) + slot.hh * t.xh + slot.d;
+  T* out = static_cast<T*>(t.out) + slot.hh * t.oh + slot.d;
   uint64_t w1[NE / 2], w2[NE / 2];
   if constexpr (NORM) {
     load_weights<T, NE>(t.w, slot.d, sh.w_dtype, w1);
     load_weights<T, NE>(t.w, half + slot.d, sh.w_dtype, w2);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      uint64_t ss = 0;
-#pragma unroll
-      for (int e = 0; e < NE / 2; ++e) {
-        const uint64_t a = x1[p].pair(e), c = x2[p].pair(e);
-        ss = f2_fma(a, a, f2_fma(c, c, ss));
-      }
-      rstd[p] = f2_sum(ss);
-    }
-    for (int o = sh.lanes >> 1; o > 0; o >>= 1) {
-#pragma unroll
-      for (int p = 0; p < P; ++p) rstd[p] += __shfl_xor_sync(0xffffffffu, rstd[p], o);
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p) rstd[p] = rsqrtf(fmaf(rstd[p], sh.inv_d, sh.eps));
   }
   const uint64_t sign = f2_same(sh.sign);
+  const uint32_t pitch = 16 * blockDim.x, piece = NE * sizeof(T) / 16 * pitch;
+  constexpr int S = kFwdStages;
+  float* tab = reinterpret_cast<float*>(smem + S * 2 * piece);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+  int n0, n1;
+  token_run(sh, n0, n1);
+  int64_t b, s0;
+  sh.tokens.split(n0, b, s0);
+  Cursor in(b, s0, t.xb, t.xs, sh.seq), to(b, s0, t.ob, t.os, sh.seq), row(b, s0, ang.tb, ang.ts, sh.seq);
+  walk_tokens<S, SRC>(
+      ang, sh, tab, ring, 2 * piece,
+      [&](uint32_t at) {
+        if (slot.on) {
+          give<T, NE>(at, x + in.at, pitch);
+          give<T, NE>(at + piece, x + in.at + half, pitch);
+        }
+        in.next(sh.seq);
+      },
+      [&](uint32_t at, const float* table) {
+        Tr tr;
+        if constexpr (SRC == kPositions) {
+          tr.load(table + slot.d, table + half + slot.d);
+        } else {
+          tr.load(static_cast<const TT*>(ang.cos) + row.at + slot.d, static_cast<const TT*>(ang.sin) + row.at + slot.d);
+          row.next(sh.seq);
+        }
+        Pack<T, NE> x1, x2;
+        if (slot.on) {
+          take(x1, at, pitch);
+          take(x2, at + piece, pitch);
+        } else {
+          x1.zero();
+          x2.zero();
+        }
+        uint64_t r = 0;
+        if constexpr (NORM) {
+          uint64_t ss = 0;
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    if (!slot.on || p >= n) break;
-    tr[p].take(tab, p, half, slot.d);
-    Pack<T, NE> y1, y2;
+          for (int e = 0; e < NE / 2; ++e) {
+            const uint64_t u = x1.pair(e), v = x2.pair(e);
+            ss = f2_fma(u, u, f2_fma(v, v, ss));
+          }
+          float sum = f2_sum(ss);
+          for (int o = sh.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          r = f2_same(rsqrtf(fmaf(sum, sh.inv_d, sh.eps)));
+        }
+        Pack<T, NE> y1, y2;
 #pragma unroll
-    for (int e = 0; e < NE / 2; ++e) {
-      uint64_t a = x1[p].pair(e), c = x2[p].pair(e);
-      uint64_t cs = tr[p].c.pair(e), sn = tr[p].s.pair(e);
-      if constexpr (NORM) {
-        const uint64_t r = f2_same(rstd[p]);
-        a = f2_mul(f2_mul(a, r), w1[e]);
-        c = f2_mul(f2_mul(c, r), w2[e]);
-      } else {
-        sn = f2_mul(sn, sign);
-      }
-      y1.set(e, f2_cross(a, cs, c, sn));
-      y2.set(e, f2_fma(a, sn, f2_mul(c, cs)));
-    }
-    y1.store(op);
-    y2.store(op + half);
-    op += t.os;
-  }
+        for (int e = 0; e < NE / 2; ++e) {
+          uint64_t u = x1.pair(e), v = x2.pair(e);
+          uint64_t cs = tr.c.pair(e), sn = tr.s.pair(e);
+          if constexpr (NORM) {
+            u = f2_mul(f2_mul(u, r), w1[e]);
+            v = f2_mul(f2_mul(v, r), w2[e]);
+          } else {
+            sn = f2_mul(sn, sign);
+          }
+          y1.set(e, f2_cross(u, cs, v, sn));
+          y2.set(e, f2_fma(u, sn, f2_mul(v, cs)));
+        }
+        if (slot.on) {
+          y1.store(out + to.at);
+          y2.store(out + to.at + half);
+        }
+        to.next(sh.seq);
+      });
+  pdl_trigger();
 }
 
-// Backward with norms. A thread keeps its slot for all of the CTA's tokens, so that its
-// share of dw stays in its registers. The CTA joins its rows of dw in the order of the
-// heads and leaves one partial row [2][D] (q, k), which dw_join_kernel sums in block
-// order.
-template <typename T, int NE, int P, int SRC>
-__global__ void __launch_bounds__(kMaxThreads, NE == 4 ? 3 : 1) qk_norm_rope_bwd_kernel(
+// Backward with norms. The thread's share of dw stays in its registers. The CTA joins
+// its rows of dw in the order of the heads and leaves one partial row [2][D] (q, k),
+// which dw_join_kernel sums in block order.
+template <typename T, int NE, int SRC>
+__global__ void __launch_bounds__(kMaxThreads, bwd_ctas(NE * (int)sizeof(T))) qk_norm_rope_bwd_kernel(
     HeadRows q, HeadRows k, const __grid_constant__ Angles ang, Shape sh, float* __restrict__ dw_part) {
   using Tr = Turn<T, NE, SRC>;
-  extern __shared__ __align__(16) float smem[];  // tables [P][2][half], later dw [blockDim][2 NE]
+  using TT = typename Tr::TT;
+  extern __shared__ __align__(16) uint8_t smem[];  // ring, tables; later dw [blockDim][2 NE]
   pdl_wait();
   const int half = sh.half;
   const Slot slot(q, k, sh, NE);
   const HeadRows& t = slot.isq ? q : k;
-  const T* xp = static_cast<const T*>(t.x) + slot.hh * t.xh + slot.d;
-  const T* gp = static_cast<const T*>(t.g) + slot.hh * t.gh + slot.d;
-  T* op = static_cast<T*>(t.out) + slot.hh * t.oh + slot.d;
+  const T* x = static_cast<const T*>(t.x) + slot.hh * t.xh + slot.d;
+  const T* g = static_cast<const T*>(t.g) + slot.hh * t.gh + slot.d;
+  T* out = static_cast<T*>(t.out) + slot.hh * t.oh + slot.d;
   uint64_t w1[NE / 2], w2[NE / 2], dw1[NE / 2], dw2[NE / 2];
   load_weights<T, NE>(t.w, slot.d, sh.w_dtype, w1);
   load_weights<T, NE>(t.w, half + slot.d, sh.w_dtype, w2);
 #pragma unroll
   for (int e = 0; e < NE / 2; ++e) dw1[e] = dw2[e] = 0;
-  const int tiles = (int)sh.tiles.d * sh.batch;
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    int64_t b, s0;
-    sh.tiles.split(tile, b, s0);
-    s0 *= P;
-    const int n = min((int)(sh.seq - s0), P);
-    const T* xr = xp + b * t.xb + s0 * t.xs;
-    const T* gr = gp + b * t.gb + s0 * t.gs;
-    T* out = op + b * t.ob + s0 * t.os;
-    Pack<T, NE> x1[P], x2[P], g1[P], g2[P];
-    Tr tr[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      x1[p].zero();
-      x2[p].zero();
-      g1[p].zero();
-      g2[p].zero();
-      tr[p].c.zero();
-      tr[p].s.zero();
-      if (slot.on && p < n) {
-        x1[p].template load<true>(xr + p * t.xs);
-        x2[p].template load<true>(xr + p * t.xs + half);
-        g1[p].template load<true>(gr + p * t.gs);
-        g2[p].template load<true>(gr + p * t.gs + half);
-        if constexpr (SRC != kPositions) {
-          const int64_t at = b * ang.tb + (s0 + p) * ang.ts + slot.d;
-          tr[p].load(static_cast<const typename Tr::TT*>(ang.cos) + at,
-                     static_cast<const typename Tr::TT*>(ang.sin) + at);
+  const uint32_t pitch = 16 * blockDim.x, piece = NE * sizeof(T) / 16 * pitch;
+  constexpr int S = kBwdStages;
+  float* tab = reinterpret_cast<float*>(smem + S * 4 * piece);
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
+  int n0, n1;
+  token_run(sh, n0, n1);
+  int64_t b, s0;
+  sh.tokens.split(n0, b, s0);
+  Cursor in(b, s0, t.xb, t.xs, sh.seq), gin(b, s0, t.gb, t.gs, sh.seq), to(b, s0, t.ob, t.os, sh.seq),
+      row(b, s0, ang.tb, ang.ts, sh.seq);
+  walk_tokens<S, SRC>(
+      ang, sh, tab, ring, 4 * piece,
+      [&](uint32_t at) {
+        if (slot.on) {
+          give<T, NE>(at, x + in.at, pitch);
+          give<T, NE>(at + piece, x + in.at + half, pitch);
+          give<T, NE>(at + 2 * piece, g + gin.at, pitch);
+          give<T, NE>(at + 3 * piece, g + gin.at + half, pitch);
         }
-      }
-    }
-    if constexpr (SRC == kPositions) {
-      __syncthreads();  // the tables of the tile before are read
-      fill_tables<P>(ang, sh, b, s0, smem);
-      __syncthreads();
+        in.next(sh.seq);
+        gin.next(sh.seq);
+      },
+      [&](uint32_t at, const float* table) {
+        Tr tr;
+        if constexpr (SRC == kPositions) {
+          tr.load(table + slot.d, table + half + slot.d);
+        } else {
+          tr.load(static_cast<const TT*>(ang.cos) + row.at + slot.d, static_cast<const TT*>(ang.sin) + row.at + slot.d);
+          row.next(sh.seq);
+        }
+        Pack<T, NE> x1, x2, g1, g2;
+        if (slot.on) {
+          take(x1, at, pitch);
+          take(x2, at + piece, pitch);
+          take(g1, at + 2 * piece, pitch);
+          take(g2, at + 3 * piece, pitch);
+        } else {
+          x1.zero();
+          x2.zero();
+          g1.zero();
+          g2.zero();
+        }
+        uint64_t sq = 0, dt = 0;
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-        if (slot.on && p < n) tr[p].take(smem, p, half, slot.d);
-    }
-    float ss[P], dot[P];
+        for (int e = 0; e < NE / 2; ++e) {
+          const uint64_t u = x1.pair(e), v = x2.pair(e), cs = tr.c.pair(e), sn = tr.s.pair(e);
+          const uint64_t ga = g1.pair(e), gb = g2.pair(e);
+          sq = f2_fma(u, u, f2_fma(v, v, sq));
+          dt = f2_fma(f2_mul(f2_fma(ga, cs, f2_mul(gb, sn)), w1[e]), u, dt);
+          dt = f2_fma(f2_mul(f2_cross(gb, cs, ga, sn), w2[e]), v, dt);
+        }
+        float ss = f2_sum(sq), dot = f2_sum(dt);
+        for (int o = sh.lanes >> 1; o > 0; o >>= 1) {
+          ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        }
+        const float rstd = rsqrtf(fmaf(ss, sh.inv_d, sh.eps));
+        const uint64_t r = f2_same(rstd);
+        const uint64_t mean = f2_same(-dot * sh.inv_d * rstd);
+        Pack<T, NE> y1, y2;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      uint64_t sq = 0, dt = 0;
-#pragma unroll
-      for (int e = 0; e < NE / 2; ++e) {
-        const uint64_t a = x1[p].pair(e), c = x2[p].pair(e), cs = tr[p].c.pair(e), sn = tr[p].s.pair(e);
-        const uint64_t ga = g1[p].pair(e), gb = g2[p].pair(e);
-        sq = f2_fma(a, a, f2_fma(c, c, sq));
-        dt = f2_fma(f2_mul(f2_fma(ga, cs, f2_mul(gb, sn)), w1[e]), a, dt);
-        dt = f2_fma(f2_mul(f2_cross(gb, cs, ga, sn), w2[e]), c, dt);
-      }
-      ss[p] = f2_sum(sq);
-      dot[p] = f2_sum(dt);
-    }
-    for (int o = sh.lanes >> 1; o > 0; o >>= 1) {
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        ss[p] += __shfl_xor_sync(0xffffffffu, ss[p], o);
-        dot[p] += __shfl_xor_sync(0xffffffffu, dot[p], o);
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const float rstd = rsqrtf(fmaf(ss[p], sh.inv_d, sh.eps));
-      const uint64_t r = f2_same(rstd);
-      const uint64_t back = f2_same(-dot[p] * sh.inv_d * rstd);
-      Pack<T, NE> y1, y2;
-#pragma unroll
-      for (int e = 0; e < NE / 2; ++e) {
-        const uint64_t a = x1[p].pair(e), c = x2[p].pair(e), cs = tr[p].c.pair(e), sn = tr[p].s.pair(e);
-        const uint64_t ga = g1[p].pair(e), gb = g2[p].pair(e);
-        const uint64_t d1 = f2_fma(ga, cs, f2_mul(gb, sn)), d2 = f2_cross(gb, cs, ga, sn);
-        const uint64_t h1 = f2_mul(a, r), h2 = f2_mul(c, r);
-        dw1[e] = f2_fma(d1, h1, dw1[e]);
-        dw2[e] = f2_fma(d2, h2, dw2[e]);
-        y1.set(e, f2_mul(r, f2_fma(h1, back, f2_mul(d1, w1[e]))));
-        y2.set(e, f2_mul(r, f2_fma(h2, back, f2_mul(d2, w2[e]))));
-      }
-      if (slot.on && p < n) {
-        y1.store(out + p * t.os);
-        y2.store(out + p * t.os + half);
-      }
-    }
-  }
+        for (int e = 0; e < NE / 2; ++e) {
+          const uint64_t cs = tr.c.pair(e), sn = tr.s.pair(e);
+          const uint64_t ga = g1.pair(e), gb = g2.pair(e);
+          const uint64_t d1 = f2_fma(ga, cs, f2_mul(gb, sn)), d2 = f2_cross(gb, cs, ga, sn);
+          const uint64_t h1 = f2_mul(x1.pair(e), r), h2 = f2_mul(x2.pair(e), r);
+          dw1[e] = f2_fma(d1, h1, dw1[e]);
+          dw2[e] = f2_fma(d2, h2, dw2[e]);
+          y1.set(e, f2_mul(r, f2_fma(h1, mean, f2_mul(d1, w1[e]))));
+          y2.set(e, f2_mul(r, f2_fma(h2, mean, f2_mul(d2, w2[e]))));
+        }
+        if (slot.on) {
+          y1.store(out + to.at);
+          y2.store(out + to.at + half);
+        }
+        to.next(sh.seq);
+      });
   pdl_trigger();
   if (!dw_part) return;
   __syncthreads();
-  float* mine = smem + threadIdx.x * 2 * NE;
+  float* join = reinterpret_cast<float*>(smem);
+  float* mine = join + threadIdx.x * 2 * NE;
 #pragma unroll
   for (int e = 0; e < NE / 2; ++e) {
     f2_unpack(dw1[e], mine[2 * e], mine[2 * e + 1]);
@@ -473,15 +546,15 @@ __global__ void __launch_bounds__(kMaxThreads, NE == 4 ? 3 : 1) qk_norm_rope_bwd
   const int dim = 2 * half;
   const int h0 = blockIdx.y * sh.group_heads;
   const int h1 = min(h0 + sh.group_heads, q.heads + k.heads);
-  float* row = dw_part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * dim;
+  float* part = dw_part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * dim;
   for (int e = threadIdx.x; e < 2 * dim; e += blockDim.x) {
     const int which = e / dim, col = e - which * dim;
     const int second = col >= half ? 1 : 0, c = col - second * half;
     const int lo = which ? max(h0, q.heads) : h0, hi = which ? h1 : min(h1, q.heads);
     float sum = 0.f;
     for (int hd = lo; hd < hi; ++hd)
-      sum += smem[((hd - h0) * sh.lanes + c / NE) * 2 * NE + second * NE + c % NE];
-    row[e] = sum;
+      sum += join[((hd - h0) * sh.lanes + c / NE) * 2 * NE + second * NE + c % NE];
+    part[e] = sum;
   }
 }
 
@@ -539,7 +612,7 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_rope_any_kernel(HeadRows q,
   for (int64_t r = (int64_t)blockIdx.x * kAnyWarps + warp; r < rows; r += (int64_t)gridDim.x * kAnyWarps) {
     const int64_t n = r / t.heads, hh = r - n * t.heads;
     int64_t b, s;
-    sh.tiles.split((uint32_t)n, b, s);
+    sh.tokens.split((uint32_t)n, b, s);
     const T* xp = static_cast<const T*>(t.x) + b * t.xb + hh * t.xh + s * t.xs;
     const T* gp = BWD && NORM ? static_cast<const T*>(t.g) + b * t.gb + hh * t.gh + s * t.gs : nullptr;
     T* op = static_cast<T*>(t.out) + b * t.ob + hh * t.oh + s * t.os;
@@ -623,21 +696,19 @@ Plan plan_of(int heads, int half, int ne) {
   return p;
 }
 
-constexpr int kBwdTokens = 2;
-
-int64_t tiles_of(int64_t batch, int64_t seq, int tokens) { return batch * ((seq + tokens - 1) / tokens); }
-
-// CTAs along the tokens of a backward: three CTAs of 256 threads an SM in all.
-int bwd_blocks(int64_t batch, int64_t seq, const Plan& p) {
-  int64_t cap = (int64_t)num_sms() * (3 * kMaxThreads / p.threads) / p.groups;
+// CTAs along the tokens: as many as are resident together.
+int blocks_of(int64_t tokens, int ctas, const Plan& p) {
+  int64_t cap = (int64_t)num_sms() * (ctas * kMaxThreads / p.threads) / p.groups;
   if (cap < 1) cap = 1;
-  const int64_t tiles = tiles_of(batch, seq, kBwdTokens);
-  return (int)(tiles < cap ? tiles : cap);
+  return (int)(tokens < cap ? tokens : cap);
 }
 
-// Elements of a half that a thread holds; 0: no vector form. Four also for 16-bit rows:
-// weights, shares of dw and four tokens' rows then fit 64 registers.
-int row_ne(int half) { return half % 4 == 0 && half / 4 <= 32 ? 4 : half % 8 == 0 && half / 8 <= 32 ? 8 : 0; }
+// Elements of a half that a thread holds: 16 bytes, or 32 where 32 threads would not
+// hold the half (fp32 beyond a head dim of 256); 0: no vector form.
+int row_ne(int half, int es) {
+  const int ne = 16 / es;
+  return half % ne == 0 && half / ne <= 32 ? ne : half % (2 * ne) == 0 && half / (2 * ne) <= 32 ? 2 * ne : 0;
+}
 
 constexpr int kAnyBlocks = 592;  // of each tensor, at most
 
@@ -657,7 +728,7 @@ bool rows_ok(const HeadRows& t, bool grads, int64_t es) {
 
 template <typename T>
 bool vectors_ok(const HeadRows& q, const HeadRows& k, const Angles& a, int dtype, int half, int ne, bool grads) {
-  if (ne == 0 || half % ne || half / ne > 32 || (half * sizeof(T)) % 16 || !rows_ok(q, grads, sizeof(T)) ||
+  if (ne == 0 || half % ne || half / ne > 32 || !rows_ok(q, grads, sizeof(T)) ||
       !rows_ok(k, grads, sizeof(T)))
     return false;
   if (!a.cos) return true;
@@ -666,14 +737,71 @@ bool vectors_ok(const HeadRows& q, const HeadRows& k, const Angles& a, int dtype
          (a.ts * es) % 16 == 0;
 }
 
-template <typename T, int NE, int P, bool NORM>
-cudaError_t fwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, int src, dim3 grid,
-                       int threads, cudaStream_t st) {
-  switch (src) {
-    case kTableT: return launch_pdl(qk_rope_fwd_kernel<T, NE, P, NORM, kTableT>, grid, dim3(threads), 0, st, q, k, a, sh);
-    case kTableF: return launch_pdl(qk_rope_fwd_kernel<T, NE, P, NORM, kTableF>, grid, dim3(threads), 0, st, q, k, a, sh);
-    default: return launch_pdl(qk_rope_fwd_kernel<T, NE, P, NORM, kPositions>, grid, dim3(threads), 0, st, q, k, a, sh);
+// Shared memory of a launch: the rings, and with positions two groups' tables.
+inline size_t ring_bytes(int stages, int pieces, int bytes, int threads, int src, int half) {
+  return (size_t)stages * pieces * bytes * threads +
+         (src == kPositions ? sizeof(float) * 2 * kGroup * 2 * half : 0);
+}
+
+// A launch of a kernel with more than 48 KB of shared memory, allowed once a device.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_ring(void (*kernel)(KArgs...), bool (&ready)[64], dim3 grid, int threads, size_t smem,
+                        cudaStream_t st, Args... args) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  {
+    std::lock_guard<std::mutex> lock(cache_mutex());
+    if (!ready[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+      if (e != cudaSuccess) return e;
+      ready[dev] = true;
+    }
   }
+  return launch_pdl(kernel, grid, dim3(threads), smem, st, args...);
+}
+
+template <typename T, int NE, bool NORM, int SRC>
+cudaError_t fwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, cudaStream_t st) {
+  static bool ready[64] = {false};
+  const Plan p = plan_of(q.heads + k.heads, sh.half, NE);
+  sh.lanes = p.lanes;
+  sh.group_heads = p.group_heads;
+  const dim3 grid(blocks_of((int64_t)sh.batch * sh.seq, fwd_ctas(NE * sizeof(T)), p), p.groups);
+  return launch_ring(qk_rope_fwd_kernel<T, NE, NORM, SRC>, ready, grid, p.threads,
+                     ring_bytes(kFwdStages, 2, NE * sizeof(T), p.threads, SRC, sh.half), st, q, k, a, sh);
+}
+
+template <typename T, int NE>
+cudaError_t fwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, bool norm, int src,
+                       cudaStream_t st) {
+  if (norm && src == kTableT) return fwd_launch<T, NE, true, kTableT>(q, k, a, sh, st);
+  if (norm && src == kTableF) return fwd_launch<T, NE, true, kTableF>(q, k, a, sh, st);
+  if (norm) return fwd_launch<T, NE, true, kPositions>(q, k, a, sh, st);
+  if (src == kTableT) return fwd_launch<T, NE, false, kTableT>(q, k, a, sh, st);
+  if (src == kTableF) return fwd_launch<T, NE, false, kTableF>(q, k, a, sh, st);
+  return fwd_launch<T, NE, false, kPositions>(q, k, a, sh, st);
+}
+
+template <typename T, int NE, int SRC>
+cudaError_t bwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, float* part, int* rows,
+                       cudaStream_t st) {
+  static bool ready[64] = {false};
+  const Plan p = plan_of(q.heads + k.heads, sh.half, NE);
+  sh.lanes = p.lanes;
+  sh.group_heads = p.group_heads;
+  const dim3 grid(blocks_of((int64_t)sh.batch * sh.seq, bwd_ctas(NE * sizeof(T)), p), p.groups);
+  *rows = (int)(grid.x * grid.y);
+  return launch_ring(qk_norm_rope_bwd_kernel<T, NE, SRC>, ready, grid, p.threads,
+                     ring_bytes(kBwdStages, 4, NE * sizeof(T), p.threads, SRC, sh.half), st, q, k, a, sh, part);
+}
+
+template <typename T, int NE>
+cudaError_t bwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, int src, float* part,
+                       int* rows, cudaStream_t st) {
+  if (src == kTableT) return bwd_launch<T, NE, kTableT>(q, k, a, sh, part, rows, st);
+  if (src == kTableF) return bwd_launch<T, NE, kTableF>(q, k, a, sh, part, rows, st);
+  return bwd_launch<T, NE, kPositions>(q, k, a, sh, part, rows, st);
 }
 
 int source_of(const Angles& a, int dtype) {
@@ -681,79 +809,40 @@ int source_of(const Angles& a, int dtype) {
 }
 
 template <typename T>
-int run_fwd(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, bool norm, int dtype, cudaStream_t st) {
-  cudaError_t e;
-  const int ne = row_ne(sh.half);
+int run_fwd(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, bool norm, int dtype,
+            cudaStream_t st) {
+  constexpr int NE = 16 / (int)sizeof(T);
+  const int ne = row_ne(sh.half, sizeof(T));
   if (vectors_ok<T>(q, k, a, dtype, sh.half, ne, false)) {
-    const Plan p = plan_of(q.heads + k.heads, sh.half, ne);
-    sh.lanes = p.lanes;
-    sh.group_heads = p.group_heads;
     const int src = source_of(a, dtype);
-    // four tokens a thread in flight; with few tokens one, so that more SMs share them
-    const bool few = tiles_of(sh.batch, sh.seq, 4) < num_sms() || sh.seq < 4 || ne == 8;
-    const dim3 grid((unsigned)tiles_of(sh.batch, sh.seq, few ? 1 : 4), p.groups);
-    sh.tiles = make_div(few ? sh.seq : (sh.seq + 3) / 4);
-    if (ne == 8)
-      e = norm ? fwd_launch<T, 8, 1, true>(q, k, a, sh, src, grid, p.threads, st)
-               : fwd_launch<T, 8, 1, false>(q, k, a, sh, src, grid, p.threads, st);
-    else if (few)
-      e = norm ? fwd_launch<T, 4, 1, true>(q, k, a, sh, src, grid, p.threads, st)
-               : fwd_launch<T, 4, 1, false>(q, k, a, sh, src, grid, p.threads, st);
-    else
-      e = norm ? fwd_launch<T, 4, 4, true>(q, k, a, sh, src, grid, p.threads, st)
-               : fwd_launch<T, 4, 4, false>(q, k, a, sh, src, grid, p.threads, st);
-  } else {
-    const int most = q.heads > k.heads ? q.heads : k.heads;
-    const dim3 grid(any_blocks((int64_t)sh.batch * sh.seq, most), 2);
-    float* none = nullptr;
-    e = norm ? launch_pdl(qk_rope_any_kernel<T, true, false>, grid, dim3(32 * kAnyWarps), 0, st, q, k, a, sh, none)
-             : launch_pdl(qk_rope_any_kernel<T, false, false>, grid, dim3(32 * kAnyWarps), 0, st, q, k, a, sh, none);
+    return cuda_status(ne == NE ? fwd_launch<T, NE>(q, k, a, sh, norm, src, st)
+                                : fwd_launch<T, 2 * NE>(q, k, a, sh, norm, src, st));
   }
-  return cuda_status(e);
-}
-
-template <typename T, int NE>
-cudaError_t bwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, int src, bool dw, float* part,
-                       int* rows, cudaStream_t st) {
-  const Plan p = plan_of(q.heads + k.heads, sh.half, NE);
-  sh.lanes = p.lanes;
-  sh.group_heads = p.group_heads;
-  const int blocks = bwd_blocks(sh.batch, sh.seq, p);
-  sh.tiles = make_div((sh.seq + kBwdTokens - 1) / kBwdTokens);
-  *rows = blocks * p.groups;
-  size_t smem = sizeof(float) * (size_t)kBwdTokens * 2 * sh.half;
-  const size_t join = sizeof(float) * (size_t)p.threads * 2 * NE;
-  if (join > smem) smem = join;
-  const dim3 grid(blocks, p.groups), block(p.threads);
-  if (!dw) part = nullptr;
-  switch (src) {
-    case kTableT:
-      return launch_pdl(qk_norm_rope_bwd_kernel<T, NE, kBwdTokens, kTableT>, grid, block, smem, st, q, k, a, sh, part);
-    case kTableF:
-      return launch_pdl(qk_norm_rope_bwd_kernel<T, NE, kBwdTokens, kTableF>, grid, block, smem, st, q, k, a, sh, part);
-    default:
-      return launch_pdl(qk_norm_rope_bwd_kernel<T, NE, kBwdTokens, kPositions>, grid, block, smem, st, q, k, a, sh,
-                        part);
-  }
+  const int most = q.heads > k.heads ? q.heads : k.heads;
+  const dim3 grid(any_blocks((int64_t)sh.batch * sh.seq, most), 2), block(32 * kAnyWarps);
+  float* none = nullptr;
+  return cuda_status(norm ? launch_pdl(qk_rope_any_kernel<T, true, false>, grid, block, 0, st, q, k, a, sh, none)
+                          : launch_pdl(qk_rope_any_kernel<T, false, false>, grid, block, 0, st, q, k, a, sh, none));
 }
 
 template <typename T>
-int run_bwd(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, void* dwq, void* dwk, float* part,
+int run_bwd(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, void* dwq, void* dwk, float* part,
             int dtype, cudaStream_t st) {
+  constexpr int NE = 16 / (int)sizeof(T);
   const int dim = 2 * sh.half;
   const bool dw = dwq || dwk;
+  if (!dw) part = nullptr;
   int rows;
   cudaError_t e;
-  const int ne = row_ne(sh.half);
+  const int ne = row_ne(sh.half, sizeof(T));
   if (vectors_ok<T>(q, k, a, dtype, sh.half, ne, true)) {
     const int src = source_of(a, dtype);
-    e = ne == 4 ? bwd_launch<T, 4>(q, k, a, sh, src, dw, part, &rows, st)
-                : bwd_launch<T, 8>(q, k, a, sh, src, dw, part, &rows, st);
+    e = ne == NE ? bwd_launch<T, NE>(q, k, a, sh, src, part, &rows, st)
+                 : bwd_launch<T, 2 * NE>(q, k, a, sh, src, part, &rows, st);
   } else {
     const int most = q.heads > k.heads ? q.heads : k.heads;
     rows = any_blocks((int64_t)sh.batch * sh.seq, most);
-    e = launch_pdl(qk_rope_any_kernel<T, true, true>, dim3(rows, 2), dim3(32 * kAnyWarps), 0, st, q, k, a, sh,
-                   dw ? part : nullptr);
+    e = launch_pdl(qk_rope_any_kernel<T, true, true>, dim3(rows, 2), dim3(32 * kAnyWarps), 0, st, q, k, a, sh, part);
   }
   if (e != cudaSuccess || !dw) return cuda_status(e);
   return cuda_status(launch_pdl(dw_join_kernel, dim3((2 * dim + kJoinCols - 1) / kJoinCols),
@@ -794,12 +883,14 @@ extern "C" {
 size_t soup_qk_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t hq, int64_t hk,
                                              int64_t head_dim) {
   if (batch <= 0 || seq <= 0 || hq <= 0 || hk <= 0 || head_dim <= 0) return 0;
-  // the more partial rows of the two forms
+  // the most partial rows of the forms
   const int64_t tokens = batch * seq;
   int64_t rows = any_blocks(tokens, hq > hk ? hq : hk);
-  if (const int ne = row_ne((int)(head_dim / 2))) {
+  for (int es = 2; es <= 4; es += 2) {
+    const int ne = row_ne((int)(head_dim / 2), es);
+    if (!ne) continue;
     const Plan p = plan_of((int)(hq + hk), (int)(head_dim / 2), ne);
-    const int64_t r = (int64_t)bwd_blocks(batch, seq, p) * p.groups;
+    const int64_t r = (int64_t)blocks_of(tokens, bwd_ctas(ne * es), p) * p.groups;
     if (r > rows) rows = r;
   }
   return sizeof(float) * (size_t)(rows * 2 * head_dim);
