@@ -78,7 +78,7 @@ _SIGNATURES = {
     "soup_grad_square_workspace_bytes": (c_sz, [c_i64]),
     "soup_grad_square": (c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_sz, ctypes.POINTER(c_int), c_vp]),
     "soup_adamw_multi": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_d, c_d,
-                                 c_d, c_d, c_d, c_d, c_vp, c_int, c_vp, c_vp, c_vp, c_int, c_vp]),
+                                 c_d, c_d, c_d, c_d, c_vp, c_int, c_vp, c_vp, c_int, c_vp, c_vp]),
     "soup_multi_lora_state_bytes": (c_sz, [c_i64, c_i64, c_i64]),
     "soup_multi_lora_fwd": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_i64, c_i64,
                                     c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_sz, c_vp]),

@@ -20,13 +20,13 @@
 // step's change is below half a step of the format.
 //
 // A warp takes blocks of 256: 8 elements a lane in two 16-byte loads (one for 16-bit
-// tensors), the maxima by one integer reduction each, the arithmetic on packed pairs.
-// A CTA takes a contiguous run of blocks over all tensors, its warps in turns with the
-// next block's loads in flight; the tensors' table (pointers and sizes)
-// comes as a kernel argument, so that a launch needs no copy and can be captured.
+// tensors), the maxima by one integer reduction each, the arithmetic on packed pairs. The
+// tensors' table (pointers and sizes) comes as a kernel argument, so that a launch needs
+// no copy and can be captured.
 #include <cuda_fp8.h>
 #include <stdio.h>
 
+#include <mutex>
 #include <type_traits>
 
 #include "soup_common.cuh"
@@ -53,13 +53,20 @@ struct Table {
   Tensor t[N];
 };
 
-// resident CTAs of the step's kernel on an SM (80 registers a thread)
-constexpr int kStepCtas = 3;
+// CTAs of the step's kernel on an SM (40 to 48 registers a thread). Each warp takes one
+// block and is done: CTAs then come in the order of memory. A grid of resident CTAs that
+// stride over the tensors, or walk a run of them each, drifts apart, and DRAM serves many
+// pages at a time: 8-bit states of 233 M bf16 elements take 407 us this way, 464 to 619
+// us with resident CTAs of every depth tried, with or without a ring of cp.async copies.
+__host__ __device__ constexpr int step_ctas(int es) { return es == 4 ? 5 : 6; }
 
 struct Hyper {
-  float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, lr, decay;  // decay: 1 - lr wd
-  double log_beta1, log_beta2;
-  float max_norm;
+  float one_minus_beta1, beta2, one_minus_beta2, eps, decay;  // decay: 1 - lr wd
+};
+
+// What a step's elements share, left by adamw_coef_kernel.
+struct Coefs {
+  float step_size, root_scale, clip, pad;  // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
 };
 
 struct States {
@@ -79,12 +86,6 @@ __device__ __forceinline__ int find_tensor(const Table<N>& tab, int c) {
     else hi = mid - 1;
   }
   return lo;
-}
-
-// The CTA's run of blocks, a contiguous one; its warps take turns in it.
-__device__ __forceinline__ void block_run(int blocks, int& c0, int& c1) {
-  c0 = (int)((int64_t)blocks * blockIdx.x / gridDim.x);
-  c1 = (int)((int64_t)blocks * (blockIdx.x + 1) / gridDim.x);
 }
 
 // Pairs of elements in packed 32-bit arithmetic: one instruction for two.
@@ -250,13 +251,11 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
   __shared__ double share[kWarps];
   pdl_wait();
   pdl_trigger();
-  int c0, c1;
-  block_run(tab.blocks, c0, c1);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum = 0.0;
-  int ti = c0 < c1 ? find_tensor(tab, min(c0 + warp, c1 - 1)) : 0;
+  int ti = 0;
   constexpr int U = 4;  // blocks of a warp in flight
-  for (int c = c0 + warp; c < c1; c += U * kWarps) {
+  for (int c = blockIdx.x * U * kWarps + warp; c < tab.blocks; c += gridDim.x * U * kWarps) {
     Raw8<T> g[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -264,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
       int left = 0;
       const T* at = nullptr;
       bool vec = false;
-      if (blk < c1) {
+      if (blk < tab.blocks) {
         while (ti + 1 < tab.count && tab.t[ti + 1].first <= blk) ++ti;
         const Tensor& t = tab.t[ti];
         const int64_t e = (int64_t)(blk - t.first) * kBlock + lane * 8;
@@ -298,159 +297,127 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// The step. `partial`: the sums of squares of all of the step's tensors, or null.
-// `step` counts the steps done; `ticket` is 0 between launches. The last CTA of the
-// step's last launch (bump) raises the count after every CTA has read it.
-template <typename T, bool EIGHT, int N>
-__global__ void __launch_bounds__(kThreads, kStepCtas) adamw_multi_kernel(const __grid_constant__ Table<N> tab, States st,
-                                                               Hyper h, const double* __restrict__ partial,
-                                                               int partials, float* __restrict__ norm_out,
-                                                               float* __restrict__ step, int* __restrict__ ticket,
-                                                               int bump) {
+// The coefficients of step t = *step + 1 and, from the sums of squares, the clip
+// coefficient and the norm. `raise`: the step's last call, after which the count is t.
+__global__ void __launch_bounds__(kThreads) adamw_coef_kernel(double lr, double log_beta1, double log_beta2,
+                                                              double max_norm, const double* __restrict__ partial,
+                                                              int partials, float* __restrict__ norm_out,
+                                                              float* __restrict__ step, int raise,
+                                                              Coefs* __restrict__ out) {
   __shared__ double share[kWarps];
-  __shared__ float coefs[3];
   pdl_wait();
   pdl_trigger();
   double sum = 0.0;
-  if (partial) {
-    for (int i = threadIdx.x; i < partials; i += kThreads) sum += partial[i];
-    sum = block_sum(sum, share);
+  for (int i = threadIdx.x; i < partials; i += kThreads) sum += partial[i];
+  sum = block_sum(sum, share);
+  if (threadIdx.x != 0) return;
+  const double t = (double)*step + 1.0;
+  Coefs c;
+  // 1 - b^t = -expm1(t log b): exact also in the first steps
+  c.step_size = (float)(lr / -expm1(t * log_beta1));
+  c.root_scale = (float)(1.0 / sqrt(-expm1(t * log_beta2)));
+  c.clip = 1.f;
+  c.pad = 0.f;
+  if (partials > 0) {
+    const double norm = sqrt(sum), k = max_norm / (norm + 1e-6);
+    c.clip = k > 1.0 ? 1.f : (float)k;  // a norm that is not a number stays visible in every element
+    if (norm_out) *norm_out = (float)norm;
   }
-  if (threadIdx.x == 0) {
-    const double t = (double)*step + 1.0;
-    // 1 - b^t = -expm1(t log b): exact also in the first steps
-    coefs[0] = (float)((double)h.lr / -expm1(t * h.log_beta1));
-    coefs[1] = (float)(1.0 / sqrt(-expm1(t * h.log_beta2)));
-    float clip = 1.f;
-    if (partial) {
-      const double norm = sqrt(sum);
-      const double c = (double)h.max_norm / (norm + 1e-6);
-      clip = c > 1.0 ? 1.f : (float)c;  // a norm that is not a number stays visible in every element
-      if (blockIdx.x == 0 && norm_out) *norm_out = (float)norm;
-    }
-    coefs[2] = clip;
-  }
-  __syncthreads();
-  const uint64_t step_size = f2_same(-coefs[0]), root_scale = f2_same(coefs[1]), clip = f2_same(coefs[2]);
+  *out = c;
+  if (raise) *step = (float)t;
+}
+
+// The step: a warp a block.
+template <typename T, bool EIGHT, int N>
+__global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_kernel(const __grid_constant__ Table<N> tab,
+                                                                                 States st, Hyper h,
+                                                                                 const Coefs* __restrict__ coefs) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * kWarps + warp;
+  const int ti = find_tensor(tab, min(c, tab.blocks - 1));
+  pdl_wait();
+  pdl_trigger();
+  if (c >= tab.blocks) return;  // warp-uniform; no barrier follows
+  const float4 co = *reinterpret_cast<const float4*>(coefs);
+  const uint64_t step_size = f2_same(-co.x), root_scale = f2_same(co.y), clip = f2_same(co.z);
   const uint64_t c1 = f2_same(h.one_minus_beta1), c2 = f2_same(h.one_minus_beta2), b2 = f2_same(h.beta2);
   const uint64_t eps = f2_same(h.eps), decay = f2_same(h.decay), minus = f2_same(-1.f);
-  int begin, end;
-  block_run(tab.blocks, begin, end);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int ti = begin < end ? find_tensor(tab, min(begin + warp, end - 1)) : 0;
-
-  // what a lane holds of a block; the next block's is in flight while one is computed
-  struct Held {
-    Raw8<T> p, g;
-    Raw8<float> m, v;  // 32 bits
-    uint2 mc, vc;      // 8 bits
-    float ms, vs;
-    T* out;
-    int left;
-    bool vec;
-    int64_t blk;
-  };
-  auto load = [&](int c, Held& d) {
-    while (ti + 1 < tab.count && tab.t[ti + 1].first <= c) ++ti;
-    const Tensor& t = tab.t[ti];
-    const int64_t e = (int64_t)(c - t.first) * kBlock + lane * 8;
-    const int64_t rest = t.n - e;
-    d.left = rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest;
-    d.blk = t.block0 + (c - t.first);
-    d.vec = (reinterpret_cast<uintptr_t>(t.p) & 15) == 0;
-    d.out = static_cast<T*>(t.p) + e;
-    d.g.load(static_cast<const T*>(t.g) + e, d.left, (reinterpret_cast<uintptr_t>(t.g) & 15) == 0);
-    d.p.load(d.out, d.left, d.vec);
-    const int64_t at = d.blk * kBlock + lane * 8;
+  const Tensor& t = tab.t[ti];
+  const int64_t e = (int64_t)(c - t.first) * kBlock + lane * 8;
+  const int64_t rest = t.n - e;
+  const int left = rest >= 8 ? 8 : rest < 0 ? 0 : (int)rest;
+  const int64_t blk = t.block0 + (c - t.first), at = blk * kBlock + lane * 8;
+  const bool vg = (reinterpret_cast<uintptr_t>(t.g) & 15) == 0, vp = (reinterpret_cast<uintptr_t>(t.p) & 15) == 0;
+  Raw8<T> p, g;
+  Raw8<float> m32, v32;
+  uint2 mc, vc;
+  float ms = 0.f, vs = 0.f;
+  g.load(static_cast<const T*>(t.g) + e, left, vg);
+  p.load(static_cast<const T*>(t.p) + e, left, vp);
+  if constexpr (EIGHT) {
+    mc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.m) + at));
+    vc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.v) + at));
+    ms = st.m_scale[blk];
+    vs = st.v_scale[blk];
+  } else {
+    m32.load(static_cast<const float*>(st.m) + at, 8, true);
+    v32.load(static_cast<const float*>(st.v) + at, 8, true);
+  }
+  uint64_t m[4], v[4], root[4];
+  const uint64_t msc = f2_same(ms), vsc = f2_same(vs);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     if constexpr (EIGHT) {
-      d.mc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.m) + at));
-      d.vc = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(st.v) + at));
-      d.ms = st.m_scale[d.blk];
-      d.vs = st.v_scale[d.blk];
+      m[i] = f2_mul(pair_of_codes(mc, i), msc);
+      v[i] = f2_mul(pair_of_codes(vc, i), vsc);
+      v[i] = f2_mul(v[i], v[i]);
     } else {
-      d.m.load(static_cast<const float*>(st.m) + at, 8, true);
-      d.v.load(static_cast<const float*>(st.v) + at, 8, true);
+      m[i] = m32.pair(i);
+      v[i] = v32.pair(i);
     }
-  };
-  auto update = [&](Held& d) {
-    uint64_t m[4], v[4], root[4];
-    const uint64_t msc = EIGHT ? f2_same(d.ms) : 0, vsc = EIGHT ? f2_same(d.vs) : 0;
+    const uint64_t gi = f2_mul(g.pair(i), clip);
+    m[i] = f2_fma(c1, f2_fma(m[i], minus, gi), m[i]);
+    v[i] = f2_fma(f2_mul(c2, gi), gi, f2_mul(v[i], b2));
+    float lo, hi;
+    f2_unpack(v[i], lo, hi);
+    root[i] = f2_pack(root_approx(lo), root_approx(hi));
+    f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
+    const uint64_t inv = f2_pack(recip_approx(lo), recip_approx(hi));
+    p.set(i, f2_fma(f2_mul(m[i], step_size), inv, f2_mul(p.pair(i), decay)));
+  }
+  p.store(static_cast<T*>(t.p) + e, left, vp);
+  if (left < 8) {
+    // what lies behind a tensor's end stays 0
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if constexpr (EIGHT) {
-        m[i] = f2_mul(pair_of_codes(d.mc, i), msc);
-        v[i] = f2_mul(pair_of_codes(d.vc, i), vsc);
-        v[i] = f2_mul(v[i], v[i]);
-      } else {
-        m[i] = d.m.pair(i);
-        v[i] = d.v.pair(i);
-      }
-      const uint64_t gi = f2_mul(d.g.pair(i), clip);
-      m[i] = f2_fma(c1, f2_fma(m[i], minus, gi), m[i]);
-      v[i] = f2_fma(f2_mul(c2, gi), gi, f2_mul(v[i], b2));
-      float lo, hi;
-      f2_unpack(v[i], lo, hi);
-      root[i] = f2_pack(root_approx(lo), root_approx(hi));
-      f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
-      const uint64_t inv = f2_pack(recip_approx(lo), recip_approx(hi));
-      d.p.set(i, f2_fma(f2_mul(m[i], step_size), inv, f2_mul(d.p.pair(i), decay)));
+      const bool a = 2 * i < left, b = 2 * i + 1 < left;
+      float x, y;
+      f2_unpack(m[i], x, y);
+      m[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
+      f2_unpack(v[i], x, y);
+      v[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
+      f2_unpack(root[i], x, y);
+      root[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
     }
-    d.p.store(d.out, d.left, d.vec);
-    if (d.left < 8) {
-      // what lies behind a tensor's end stays 0
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool a = 2 * i < d.left, b = 2 * i + 1 < d.left;
-        float x, y;
-        f2_unpack(m[i], x, y);
-        m[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
-        f2_unpack(v[i], x, y);
-        v[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
-        f2_unpack(root[i], x, y);
-        root[i] = f2_pack(a ? x : 0.f, b ? y : 0.f);
-      }
-    }
-    const int64_t at = d.blk * kBlock + lane * 8;
-    if constexpr (EIGHT) {
-      float sm, sv;
-      const uint2 cm = to_codes<false>(m, sm);
-      const uint2 cv = to_codes<true>(root, sv);
-      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m) + at), cm);
-      __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v) + at), cv);
-      if (lane == 0) {
-        st.m_scale[d.blk] = sm;
-        st.v_scale[d.blk] = sv;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        d.m.set(i, m[i]);
-        d.v.set(i, v[i]);
-      }
-      d.m.store(static_cast<float*>(st.m) + at, 8, true);
-      d.v.store(static_cast<float*>(st.v) + at, 8, true);
-    }
-  };
-  // two blocks in turn: one in flight, one computed
-  Held a, b;
-  int c = begin + warp;
-  if (c < end) load(c, a);
-  while (c < end) {
-    c += kWarps;
-    if (c < end) load(c, b);
-    update(a);
-    if (c >= end) break;
-    c += kWarps;
-    if (c < end) load(c, a);
-    update(b);
   }
-  if (bump && threadIdx.x == 0) {
-    // every CTA has read the count before its ticket
-    __threadfence();
-    if (atomicAdd(ticket, 1) == (int)gridDim.x - 1) {
-      *ticket = 0;
-      *step += 1.f;
+  if constexpr (EIGHT) {
+    float sm, sv;
+    const uint2 cm = to_codes<false>(m, sm);
+    const uint2 cv = to_codes<true>(root, sv);
+    __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m) + at), cm);
+    __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v) + at), cv);
+    if (lane == 0) {
+      st.m_scale[blk] = sm;
+      st.v_scale[blk] = sv;
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m32.set(i, m[i]);
+      v32.set(i, v[i]);
+    }
+    m32.store(static_cast<float*>(st.m) + at, 8, true);
+    v32.store(static_cast<float*>(st.v) + at, 8, true);
   }
 }
 
@@ -524,12 +491,11 @@ int square_launch(const Args& a, int i0, int i1, double* partial, int* used, cud
 }
 
 template <typename T, bool EIGHT, int N>
-int step_launch(const Args& a, int i0, int i1, const States& s, const Hyper& h, const double* partial, int partials,
-                float* norm_out, float* step, int* ticket, int bump, cudaStream_t st) {
+int step_launch(const Args& a, int i0, int i1, const States& s, const Hyper& h, const Coefs* coefs, cudaStream_t st) {
   Table<N> tab;
   fill_table(tab, a, i0, i1);
-  return launch_table(adamw_multi_kernel<T, EIGHT, N>, grid_of(tab.blocks, kStepCtas), st, tab, s, h, partial, partials, norm_out,
-                      step, ticket, bump);
+  const int grid = (tab.blocks + kWarps - 1) / kWarps;
+  return launch_table(adamw_multi_kernel<T, EIGHT, N>, grid, st, tab, s, h, coefs);
 }
 
 int check_tensors(const char* fn, const Args& a, bool step) {
@@ -563,15 +529,12 @@ int square_run(const Args& a, double* partial, int cap, int* used, cudaStream_t 
 }
 
 template <typename T, bool EIGHT>
-int step_run(const Args& a, const States& s, const Hyper& h, const double* partial, int partials, float* norm_out,
-             float* step, int* ticket, int bump, cudaStream_t st) {
+int step_run(const Args& a, const States& s, const Hyper& h, const Coefs* coefs, cudaStream_t st) {
   const int most = a.count <= kSmall ? kSmall : kLarge;
   for (int i0 = 0; i0 < a.count;) {
     const int i1 = launch_end(a, i0, most);
-    const int b = bump && i1 == a.count ? 1 : 0;
-    const int rc = most == kSmall
-                       ? step_launch<T, EIGHT, kSmall>(a, i0, i1, s, h, partial, partials, norm_out, step, ticket, b, st)
-                       : step_launch<T, EIGHT, kLarge>(a, i0, i1, s, h, partial, partials, norm_out, step, ticket, b, st);
+    const int rc = most == kSmall ? step_launch<T, EIGHT, kSmall>(a, i0, i1, s, h, coefs, st)
+                                  : step_launch<T, EIGHT, kLarge>(a, i0, i1, s, h, coefs, st);
     if (rc) return rc;
     i0 = i1;
   }
@@ -611,31 +574,31 @@ int soup_grad_square(const void* const* grads, const int64_t* sizes, int count, 
 int soup_adamw_multi(void* const* params, const void* const* grads, const int64_t* sizes, const int32_t* blocks,
                      int count, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
                      float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps, double weight_decay,
-                     double max_norm, const void* grad_squares, int partials, float* norm_out, float* step,
-                     int* ticket, int last, void* stream) {
+                     double max_norm, const void* grad_squares, int partials, float* norm_out, float* step, int last,
+                     float* coefs, void* stream) {
   const Args a{params, grads, sizes, blocks, count};
   if (int rc = check_tensors("soup_adamw_multi", a, true)) return rc;
-  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps > 0.0) || !exp_avg || !exp_avg_sq ||
-      !step || !ticket || (state_bits != 8 && state_bits != 32) ||
+  if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 1e-30) || !exp_avg || !exp_avg_sq ||
+      !step || !coefs || (state_bits != 8 && state_bits != 32) ||
       (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)) || partials < 0 || (partials > 0 && !grad_squares) ||
-      !aligned16(exp_avg) || !aligned16(exp_avg_sq)) {
+      !aligned16(exp_avg) || !aligned16(exp_avg_sq) || !aligned16(coefs) ||
+      (dtype != SOUP_F32 && dtype != SOUP_BF16 && dtype != SOUP_F16)) {
     set_last_error("soup_adamw_multi: bad arguments");
     return SOUP_ERR_INVALID;
   }
   const States s{exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale};
-  const Hyper h{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)lr,
-                (float)(1.0 - lr * weight_decay), log(beta1), log(beta2), (float)max_norm};
-  const double* sq = partials > 0 ? static_cast<const double*>(grad_squares) : nullptr;
+  const Hyper h{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay)};
   cudaStream_t st = as_stream(stream);
-#define RUN(T)                                                                                                  \
-  return state_bits == 8 ? step_run<T, true>(a, s, h, sq, partials, norm_out, step, ticket, last, st)           \
-                         : step_run<T, false>(a, s, h, sq, partials, norm_out, step, ticket, last, st)
+  Coefs* co = reinterpret_cast<Coefs*>(coefs);
+  if (int rc = cuda_status(launch_pdl(adamw_coef_kernel, dim3(1), dim3(kThreads), 0, st, lr, log(beta1), log(beta2),
+                                      max_norm, static_cast<const double*>(grad_squares), partials, norm_out, step,
+                                      last, co)))
+    return rc;
+#define RUN(T) return state_bits == 8 ? step_run<T, true>(a, s, h, co, st) : step_run<T, false>(a, s, h, co, st)
   if (dtype == SOUP_F32) RUN(float);
   if (dtype == SOUP_BF16) RUN(__nv_bfloat16);
-  if (dtype == SOUP_F16) RUN(__half);
+  RUN(__half);
 #undef RUN
-  set_last_error("soup_adamw_multi: unsupported dtype");
-  return SOUP_ERR_INVALID;
 }
 
 }  // extern "C"

@@ -91,8 +91,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             raise ValueError(f"lr must be a number of 0 or more, not {group['lr']!r}")
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"betas must be in [0, 1), got {group['betas']}")
-        if not group["eps"] > 0.0:
-            raise ValueError(f"eps must be positive, not {group['eps']!r}")
+        if not 1e-30 <= group["eps"] < math.inf:
+            raise ValueError(f"eps must be at least 1e-30, not {group['eps']!r}")
         if not group["weight_decay"] >= 0.0:
             raise ValueError(f"weight_decay must be 0 or more, not {group['weight_decay']!r}")
 
@@ -128,7 +128,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         held.v_scale = torch.zeros(total, dtype=torch.float32, device=dev) if eight else None
         if self._step is None:
             self._step = torch.zeros((), dtype=torch.float32, device=dev)
-            self._ticket = torch.zeros((), dtype=torch.int32, device=dev)
+            self._coefs = torch.zeros(4, dtype=torch.float32, device=dev)
         if self.max_grad_norm is not None:
             launches = sum(len(h.by_dtype) for h in itertools.chain(self._held, [held]))
             tensors = sum(len(h.params) for h in itertools.chain(self._held, [held]))
@@ -239,5 +239,5 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                           code, self.state_bits, held.m.data_ptr(), held.v.data_ptr(), _lib.ptr(held.m_scale),
                           _lib.ptr(held.v_scale), group["lr"], b1, b2, group["eps"], group["weight_decay"],
                           self.max_grad_norm or 0.0, squares, partials.value, _lib.ptr(self.grad_norm),
-                          self._step.data_ptr(), self._ticket.data_ptr(), 1 if done == launches else 0, stream)
+                          self._step.data_ptr(), 1 if done == launches else 0, self._coefs.data_ptr(), stream)
         return loss

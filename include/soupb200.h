@@ -218,15 +218,15 @@ int soup_multi_lora_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx
  * workspace and raises *partials; with partials > 0 the step scales gradients by
  * min(1, max_norm / (sqrt(sum) + 1e-6)) and writes the norm to norm_out (may be NULL).
  * step (device fp32) counts completed steps and is raised by the call with last != 0;
- * ticket is a device int, 0 at first, of the optimiser's own. */
+ * coefs: four device floats, 16-byte aligned, of the optimiser's own. eps >= 1e-30. */
 size_t soup_grad_square_workspace_bytes(int64_t tensors);
 int soup_grad_square(const void* const* grads, const int64_t* sizes, int count, int dtype, void* workspace,
                      size_t workspace_bytes, int* partials, void* stream);
 int soup_adamw_multi(void* const* params, const void* const* grads, const int64_t* sizes, const int32_t* blocks,
                      int count, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
                      float* exp_avg_sq_scale, double lr, double beta1, double beta2, double eps, double weight_decay,
-                     double max_norm, const void* grad_squares, int partials, float* norm_out, float* step,
-                     int* ticket, int last, void* stream);
+                     double max_norm, const void* grad_squares, int partials, float* norm_out, float* step, int last,
+                     float* coefs, void* stream);
 
 /* ---- Cross-entropy on a logits buffer ------------------------------------
  * Replaces solution/kernels/chunked_ce.py:32-128
