@@ -35,8 +35,9 @@ constexpr int kMaxHalf = kMaxDim / 2;
 constexpr int kMaxThreads = 256;
 // Stages of a thread's ring, and resident CTAs of 256 threads on an SM by the bytes of a
 // half that a thread holds: the rings take 128 to 196 KB of an SM's shared memory.
-constexpr int kFwdStages = 4, kBwdStages = 4;
-__host__ __device__ constexpr int fwd_ctas(int bytes) { return bytes == 16 ? 3 : 2; }
+constexpr int kBwdStages = 4;
+constexpr int kFwdTokens = 2;
+__host__ __device__ constexpr int fwd_ctas(int bytes) { return bytes == 16 ? 4 : 2; }
 __host__ __device__ constexpr int bwd_ctas(int bytes) { return bytes == 16 ? 2 : 1; }
 
 struct HeadRows {
@@ -88,6 +89,7 @@ struct Shape {
   int half;
   int lanes;           // threads of a row (a power of two)
   int group_heads;     // heads of a CTA
+  int side;            // tokens that it takes side by side
   float eps, inv_d;    // inv_d: 1 / D
   int w_dtype;
   float sign;          // -1: the inverse rotation
@@ -223,13 +225,14 @@ __device__ __forceinline__ void load_weights(const void* w, int at, int dtype, u
 struct Slot {
   bool on, isq;
   int64_t hh;
-  int d;
+  int d, token;  // token: among those that the CTA takes side by side
   __device__ __forceinline__ Slot(const HeadRows& q, const HeadRows& k, const Shape& sh, int ne) {
     const int shift = __ffs(sh.lanes) - 1;
-    const int local = threadIdx.x >> shift;
-    const int h = blockIdx.y * sh.group_heads + local;
+    const int row = threadIdx.x >> shift;
+    token = threadIdx.y;
+    const int h = blockIdx.y * sh.group_heads + row;
     d = (threadIdx.x & (sh.lanes - 1)) * ne;
-    on = local < sh.group_heads && h < q.heads + k.heads && d < sh.half;
+    on = row < sh.group_heads && h < q.heads + k.heads && d < sh.half;
     isq = h < q.heads;
     hh = isq ? h : h - q.heads;
     if (!on) d = 0;
@@ -272,9 +275,10 @@ struct Cursor {
 
 constexpr int kGroup = 4;  // tokens whose tables a CTA forms together (kPositions)
 
-// The tables of tokens [n0, n0 + kGroup) of the run's end n1 into shared memory.
-__device__ __forceinline__ void fill_tables(const Angles& a, const Shape& sh, int n0, int n1, float* tab) {
-  for (int e = threadIdx.x; e < kGroup * sh.half; e += blockDim.x) {
+// The tables of `count` tokens from n0 on, as far as n1, into shared memory.
+__device__ __forceinline__ void fill_tables(const Angles& a, const Shape& sh, int n0, int n1, int count, float* tab) {
+  const int threads = blockDim.x * blockDim.y;
+  for (int e = threadIdx.y * blockDim.x + threadIdx.x; e < count * sh.half; e += threads) {
     const int p = e / sh.half, i = e - p * sh.half;
     if (n0 + p >= n1) break;
     int64_t b, s;
@@ -318,7 +322,7 @@ __device__ __forceinline__ void walk_tokens(const Angles& ang, const Shape& sh, 
       const int g = n - n0;
       float* mine = tab + (g / kGroup & 1) * kGroup * 2 * sh.half;
       if (g % kGroup == 0) {
-        fill_tables(ang, sh, n, n1, mine);
+        fill_tables(ang, sh, n, n1, kGroup, mine);
         __syncthreads();
       }
       table = mine + g % kGroup * 2 * sh.half;
@@ -345,92 +349,92 @@ __device__ __forceinline__ void give(uint32_t at, const T* src, uint32_t pitch) 
   for (int i = 0; i < Pack<T, NE>::kWords; i += 4) copy16(at + i / 4 * pitch, src + i * 4 / sizeof(T));
 }
 
-// Forward (and, without weights and with sign -1, the backward of a rotation alone).
-template <typename T, int NE, bool NORM, int SRC>
+// Forward (and, without weights and with sign -1, the backward of a rotation alone). A
+// thread takes one row's elements of P tokens; CTA (x, y) the tokens [x C P, ...) of all
+// its heads, C of them side by side. CTAs come in the order of memory.
+template <typename T, int NE, int P, bool NORM, int SRC>
 __global__ void __launch_bounds__(kMaxThreads, fwd_ctas(NE * (int)sizeof(T))) qk_rope_fwd_kernel(
     HeadRows q, HeadRows k, const __grid_constant__ Angles ang, Shape sh) {
   using Tr = Turn<T, NE, SRC>;
   using TT = typename Tr::TT;
-  extern __shared__ __align__(16) uint8_t smem[];  // ring, then (kPositions) two groups' tables
+  extern __shared__ __align__(16) float tab[];  // (kPositions) tables of the CTA's tokens
   pdl_wait();
-  const int half = sh.half;
+  pdl_trigger();
+  const int half = sh.half, total = sh.batch * sh.seq;
+  const int base = blockIdx.x * sh.side * P;
   const Slot slot(q, k, sh, NE);
   const HeadRows& t = slot.isq ? q : k;
   const T* x = static_cast<const T*>(t.x) + slot.hh * t.xh + slot.d;
   T* out = static_cast<T*>(t.out) + slot.hh * t.oh + slot.d;
+  Pack<T, NE> x1[P], x2[P];
+  Tr tr[P];
+  int64_t to[P];
+  bool on[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int n = base + p * sh.side + slot.token;
+    on[p] = slot.on && n < total;
+    x1[p].zero();
+    x2[p].zero();
+    if (on[p]) {
+      int64_t b, s;
+      sh.tokens.split(n, b, s);
+      const T* r = x + b * t.xb + s * t.xs;
+      to[p] = b * t.ob + s * t.os;
+      x1[p].template load<true>(r);
+      x2[p].template load<true>(r + half);
+      if constexpr (SRC != kPositions) {
+        const int64_t at = b * ang.tb + s * ang.ts + slot.d;
+        tr[p].load(static_cast<const TT*>(ang.cos) + at, static_cast<const TT*>(ang.sin) + at);
+      }
+    }
+  }
   uint64_t w1[NE / 2], w2[NE / 2];
   if constexpr (NORM) {
     load_weights<T, NE>(t.w, slot.d, sh.w_dtype, w1);
     load_weights<T, NE>(t.w, half + slot.d, sh.w_dtype, w2);
   }
-  const uint64_t sign = f2_same(sh.sign);
-  const uint32_t pitch = 16 * blockDim.x, piece = NE * sizeof(T) / 16 * pitch;
-  constexpr int S = kFwdStages;
-  float* tab = reinterpret_cast<float*>(smem + S * 2 * piece);
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16;
-  int n0, n1;
-  token_run(sh, n0, n1);
-  int64_t b, s0;
-  sh.tokens.split(n0, b, s0);
-  Cursor in(b, s0, t.xb, t.xs, sh.seq), to(b, s0, t.ob, t.os, sh.seq), row(b, s0, ang.tb, ang.ts, sh.seq);
-  walk_tokens<S, SRC>(
-      ang, sh, tab, ring, 2 * piece,
-      [&](uint32_t at) {
-        if (slot.on) {
-          give<T, NE>(at, x + in.at, pitch);
-          give<T, NE>(at + piece, x + in.at + half, pitch);
-        }
-        in.next(sh.seq);
-      },
-      [&](uint32_t at, const float* table) {
-        Tr tr;
-        if constexpr (SRC == kPositions) {
-          tr.load(table + slot.d, table + half + slot.d);
-        } else {
-          tr.load(static_cast<const TT*>(ang.cos) + row.at + slot.d, static_cast<const TT*>(ang.sin) + row.at + slot.d);
-          row.next(sh.seq);
-        }
-        Pack<T, NE> x1, x2;
-        if (slot.on) {
-          take(x1, at, pitch);
-          take(x2, at + piece, pitch);
-        } else {
-          x1.zero();
-          x2.zero();
-        }
-        uint64_t r = 0;
-        if constexpr (NORM) {
-          uint64_t ss = 0;
+  if constexpr (SRC == kPositions) {
+    fill_tables(ang, sh, base, min(base + P * sh.side, total), P * sh.side, tab);
+    __syncthreads();
+  }
 #pragma unroll
-          for (int e = 0; e < NE / 2; ++e) {
-            const uint64_t u = x1.pair(e), v = x2.pair(e);
-            ss = f2_fma(u, u, f2_fma(v, v, ss));
-          }
-          float sum = f2_sum(ss);
-          for (int o = sh.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          r = f2_same(rsqrtf(fmaf(sum, sh.inv_d, sh.eps)));
-        }
-        Pack<T, NE> y1, y2;
+  for (int p = 0; p < P; ++p) {
+    uint64_t r = 0;
+    if constexpr (NORM) {
+      uint64_t ss = 0;
 #pragma unroll
-        for (int e = 0; e < NE / 2; ++e) {
-          uint64_t u = x1.pair(e), v = x2.pair(e);
-          uint64_t cs = tr.c.pair(e), sn = tr.s.pair(e);
-          if constexpr (NORM) {
-            u = f2_mul(f2_mul(u, r), w1[e]);
-            v = f2_mul(f2_mul(v, r), w2[e]);
-          } else {
-            sn = f2_mul(sn, sign);
-          }
-          y1.set(e, f2_cross(u, cs, v, sn));
-          y2.set(e, f2_fma(u, sn, f2_mul(v, cs)));
-        }
-        if (slot.on) {
-          y1.store(out + to.at);
-          y2.store(out + to.at + half);
-        }
-        to.next(sh.seq);
-      });
-  pdl_trigger();
+      for (int e = 0; e < NE / 2; ++e) {
+        const uint64_t u = x1[p].pair(e), v = x2[p].pair(e);
+        ss = f2_fma(u, u, f2_fma(v, v, ss));
+      }
+      float sum = f2_sum(ss);
+      for (int o = sh.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      r = f2_same(rsqrtf(fmaf(sum, sh.inv_d, sh.eps)));
+    }
+    if (!on[p]) continue;
+    if constexpr (SRC == kPositions) {
+      const float* mine = tab + (p * sh.side + slot.token) * 2 * half + slot.d;
+      tr[p].load(mine, mine + half);
+    }
+    const uint64_t sign = f2_same(sh.sign);
+    Pack<T, NE> y1, y2;
+#pragma unroll
+    for (int e = 0; e < NE / 2; ++e) {
+      uint64_t u = x1[p].pair(e), v = x2[p].pair(e);
+      uint64_t cs = tr[p].c.pair(e), sn = tr[p].s.pair(e);
+      if constexpr (NORM) {
+        u = f2_mul(f2_mul(u, r), w1[e]);
+        v = f2_mul(f2_mul(v, r), w2[e]);
+      } else {
+        sn = f2_mul(sn, sign);
+      }
+      y1.set(e, f2_cross(u, cs, v, sn));
+      y2.set(e, f2_fma(u, sn, f2_mul(v, cs)));
+    }
+    y1.store(out + to[p]);
+    y2.store(out + to[p] + half);
+  }
 }
 
 // Backward with norms. The thread's share of dw stays in its registers. The CTA joins
@@ -679,12 +683,12 @@ __global__ void __launch_bounds__(32 * kAnyWarps) qk_rope_any_kernel(HeadRows q,
 }
 
 // Threads, groups of heads and blocks of a launch, from sizes alone (the caller's
-// workspace is sized by them).
+// workspace is sized by them). many: tokens side by side fill the CTA's threads.
 struct Plan {
-  int lanes, group_heads, groups, threads;
+  int lanes, group_heads, groups, threads, side;
 };
 
-Plan plan_of(int heads, int half, int ne) {
+Plan plan_of(int heads, int half, int ne, bool many) {
   Plan p;
   p.lanes = 1;
   while (p.lanes < half / ne) p.lanes <<= 1;
@@ -692,7 +696,9 @@ Plan plan_of(int heads, int half, int ne) {
   p.groups = (int)((slots + kMaxThreads - 1) / kMaxThreads);
   p.group_heads = (heads + p.groups - 1) / p.groups;
   p.groups = (heads + p.group_heads - 1) / p.group_heads;
-  p.threads = (p.group_heads * p.lanes + 31) / 32 * 32;
+  p.threads = p.group_heads * p.lanes;
+  p.side = many ? kMaxThreads / p.threads : 1;
+  if (p.side == 1) p.threads = (p.threads + 31) / 32 * 32;
   return p;
 }
 
@@ -763,13 +769,16 @@ cudaError_t launch_ring(void (*kernel)(KArgs...), bool (&ready)[64], dim3 grid, 
 
 template <typename T, int NE, bool NORM, int SRC>
 cudaError_t fwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, cudaStream_t st) {
-  static bool ready[64] = {false};
-  const Plan p = plan_of(q.heads + k.heads, sh.half, NE);
+  const int64_t tokens = (int64_t)sh.batch * sh.seq;
+  // few tokens: one a CTA, so that more SMs share them
+  const Plan p = plan_of(q.heads + k.heads, sh.half, NE, tokens >= 4 * num_sms());
   sh.lanes = p.lanes;
   sh.group_heads = p.group_heads;
-  const dim3 grid(blocks_of((int64_t)sh.batch * sh.seq, fwd_ctas(NE * sizeof(T)), p), p.groups);
-  return launch_ring(qk_rope_fwd_kernel<T, NE, NORM, SRC>, ready, grid, p.threads,
-                     ring_bytes(kFwdStages, 2, NE * sizeof(T), p.threads, SRC, sh.half), st, q, k, a, sh);
+  sh.side = p.side;
+  constexpr int P = kFwdTokens;
+  const size_t smem = SRC == kPositions ? sizeof(float) * P * p.side * 2 * sh.half : 0;
+  const dim3 grid((unsigned)((tokens + P * p.side - 1) / (P * p.side)), p.groups);
+  return launch_pdl(qk_rope_fwd_kernel<T, NE, P, NORM, SRC>, grid, dim3(p.threads, p.side), smem, st, q, k, a, sh);
 }
 
 template <typename T, int NE>
@@ -787,9 +796,10 @@ template <typename T, int NE, int SRC>
 cudaError_t bwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Shape sh, float* part, int* rows,
                        cudaStream_t st) {
   static bool ready[64] = {false};
-  const Plan p = plan_of(q.heads + k.heads, sh.half, NE);
+  const Plan p = plan_of(q.heads + k.heads, sh.half, NE, false);
   sh.lanes = p.lanes;
   sh.group_heads = p.group_heads;
+  sh.side = 1;
   const dim3 grid(blocks_of((int64_t)sh.batch * sh.seq, bwd_ctas(NE * sizeof(T)), p), p.groups);
   *rows = (int)(grid.x * grid.y);
   return launch_ring(qk_norm_rope_bwd_kernel<T, NE, SRC>, ready, grid, p.threads,
@@ -889,7 +899,7 @@ size_t soup_qk_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t
   for (int es = 2; es <= 4; es += 2) {
     const int ne = row_ne((int)(head_dim / 2), es);
     if (!ne) continue;
-    const Plan p = plan_of((int)(hq + hk), (int)(head_dim / 2), ne);
+    const Plan p = plan_of((int)(hq + hk), (int)(head_dim / 2), ne, false);
     const int64_t r = (int64_t)blocks_of(tokens, bwd_ctas(ne * es), p) * p.groups;
     if (r > rows) rows = r;
   }
@@ -920,7 +930,7 @@ int soup_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, cons
               q_out_strides[0], q_out_strides[1], q_out_strides[2], q_weight, (int)hq};
   HeadRows tk{k, nullptr, k_out, k_strides[0], k_strides[1], k_strides[2], 0, 0, 0,
               k_out_strides[0], k_out_strides[1], k_out_strides[2], k_weight, (int)hk};
-  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, eps, 1.f / (float)head_dim, w_dtype, inverse ? -1.f : 1.f};
+  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, 1, eps, 1.f / (float)head_dim, w_dtype, inverse ? -1.f : 1.f};
   cudaStream_t st = as_stream(stream);
   if (dtype == SOUP_BF16) return run_fwd<__nv_bfloat16>(tq, tk, a, sh, norm, dtype, st);
   if (dtype == SOUP_F16) return run_fwd<__half>(tq, tk, a, sh, norm, dtype, st);
@@ -963,7 +973,7 @@ int soup_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_out_strides, con
   HeadRows tk{k, dk_out, dk, k_strides[0], k_strides[1], k_strides[2],
               dk_out_strides[0], dk_out_strides[1], dk_out_strides[2],
               dk_strides[0], dk_strides[1], dk_strides[2], k_weight, (int)hk};
-  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, eps, 1.f / (float)head_dim, w_dtype, 1.f};
+  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, 1, eps, 1.f / (float)head_dim, w_dtype, 1.f};
   float* part = static_cast<float*>(workspace);
   cudaStream_t st = as_stream(stream);
   if (dtype == SOUP_BF16) return run_bwd<__nv_bfloat16>(tq, tk, a, sh, dq_weight, dk_weight, part, dtype, st);
