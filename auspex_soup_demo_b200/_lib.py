@@ -67,14 +67,10 @@ _SIGNATURES = {
                                 c_i64, c_i64, c_int, c_vp]),
     "soup_rope": (c_int, [c_vp, P_I64, c_vp, P_I64, c_i64, c_vp, P_I64, c_vp, P_I64, c_i64, c_vp,
                           c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_int, c_int, c_vp]),
-    "soup_qk_norm_rope": (c_int, [c_vp, P_I64, c_vp, P_I64, c_i64, c_vp, P_I64, c_vp, P_I64, c_i64, c_vp, c_vp,
-                                  c_f, c_vp, c_vp, c_i64, c_i64, c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_vp,
-                                  c_vp, c_i64, c_i64, c_i64, c_int, c_int, c_int, c_vp]),
+    "soup_qk_norm_rope": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "soup_qk_norm_rope_bwd_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64, c_i64]),
-    "soup_qk_norm_rope_bwd": (c_int, [c_vp, P_I64, c_vp, P_I64, c_vp, P_I64, c_i64, c_vp, P_I64, c_vp, P_I64,
-                                      c_vp, P_I64, c_i64, c_vp, c_vp, c_f, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64,
-                                      c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
-                                      c_int, c_int, c_vp, c_sz, c_vp]),
+    "soup_qk_norm_rope_bwd": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                      c_vp, c_vp, c_sz, c_vp]),
     "soup_grad_square_workspace_bytes": (c_sz, [c_i64]),
     "soup_grad_square": (c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_sz, ctypes.POINTER(c_int), c_vp]),
     "soup_adamw_multi": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_d, c_d,

@@ -22,6 +22,8 @@
 // ahead, which keeps enough bytes in flight without the registers for them. Head dims
 // whose half is not a multiple of a vector, or rows that are not 16-byte aligned, take
 // a warp per row instead.
+#include <stdio.h>
+
 #include <mutex>
 #include <type_traits>
 
@@ -860,27 +862,48 @@ int run_bwd(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& 
                                 dwk, sh.w_dtype));
 }
 
-bool fill_angles(Angles& a, const void* cos, const void* sin, int64_t tb, int64_t ts, int dtype, const void* pos,
-                 int pos64, int64_t pa, int64_t pb, int64_t ps, const float* inv_freq, const uint8_t* axis,
-                 int64_t half) {
+bool fill_angles(Angles& a, const soup_qk_rope& d, const void* table, const void* second, const uint8_t* axes) {
   a = Angles{};
-  if (cos && sin) {
-    a.cos = cos;
-    a.sin = sin;
-    a.tb = tb;
-    a.ts = ts;
-    a.dtype = dtype;
-    return dtype == SOUP_F32 || dtype == SOUP_BF16 || dtype == SOUP_F16;
+  if (!table || !second) return false;
+  if (d.source == SOUP_ROPE_TABLES) {
+    a.cos = table;
+    a.sin = second;
+    a.tb = d.table[1];
+    a.ts = d.table[2];
+    a.dtype = (int)d.table_dtype;
+    return a.dtype == SOUP_F32 || a.dtype == SOUP_BF16 || a.dtype == SOUP_F16;
   }
-  if (cos || sin || !pos || !inv_freq || !axis) return false;
-  a.pos = pos;
-  a.pos64 = pos64;
-  a.pa = pa;
-  a.pb = pb;
-  a.ps = ps;
-  a.inv_freq = inv_freq;
-  for (int64_t i = 0; i < half; ++i) a.axis[i] = axis[i];
+  if (!axes || (d.source != SOUP_ROPE_INT32 && d.source != SOUP_ROPE_INT64)) return false;
+  a.pos = table;
+  a.pos64 = d.source == SOUP_ROPE_INT64;
+  a.pa = d.table[0];
+  a.pb = d.table[1];
+  a.ps = d.table[2];
+  a.inv_freq = static_cast<const float*>(second);
+  for (int64_t i = 0; i < d.head_dim / 2; ++i) a.axis[i] = axes[i];
   return true;
+}
+
+int check_desc(const char* fn, const soup_qk_rope* d) {
+  if (d && d->batch > 0 && d->seq > 0 && d->head_dim > 0 && d->head_dim % 2 == 0 && d->head_dim <= kMaxDim &&
+      d->hq > 0 && d->hk > 0 && d->hq <= 4096 && d->hk <= 4096 && d->batch < (int64_t(1) << 31) / d->seq &&
+      d->q[3] == 1 && d->q_out[3] == 1 && d->k[3] == 1 && d->k_out[3] == 1 && d->eps >= 0.0 &&
+      (d->w_dtype == d->dtype || d->w_dtype == SOUP_F32))
+    return SOUP_OK;
+  char msg[96];
+  snprintf(msg, sizeof(msg), "%s: bad sizes, strides or types", fn);
+  set_last_error(msg);
+  return SOUP_ERR_INVALID;
+}
+
+HeadRows rows_of(const void* x, const void* g, void* out, const int64_t* xs, const int64_t* gs, const int64_t* os,
+                 const void* w, int64_t heads) {
+  return HeadRows{x, g, out, xs[0], xs[1], xs[2], gs[0], gs[1], gs[2], os[0], os[1], os[2], w, (int)heads};
+}
+
+Shape shape_of(const soup_qk_rope& d) {
+  return Shape{(int)d.batch, (int)d.seq, make_div(d.seq), (int)(d.head_dim / 2), 32, 0, 1, (float)d.eps,
+               1.f / (float)d.head_dim, (int)d.w_dtype, d.inverse ? -1.f : 1.f};
 }
 
 }  // namespace
@@ -906,31 +929,22 @@ size_t soup_qk_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t
   return sizeof(float) * (size_t)(rows * 2 * head_dim);
 }
 
-int soup_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int64_t hq,
-                      const void* k, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
-                      int64_t hk, const void* q_weight, const void* k_weight, float eps, const void* cos,
-                      const void* sin, int64_t table_sb, int64_t table_ss, int table_dtype, const void* positions,
-                      int positions_64, int64_t pos_sa, int64_t pos_sb, int64_t pos_ss, const float* inv_freq,
-                      const uint8_t* axes, int64_t batch, int64_t seq, int64_t head_dim, int dtype, int w_dtype,
-                      int inverse, void* stream) {
+int soup_qk_norm_rope(const void* q, void* q_out, const void* k, void* k_out, const void* q_weight,
+                      const void* k_weight, const void* table, const void* second, const uint8_t* axes,
+                      const soup_qk_rope* desc, void* stream) {
+  if (int rc = check_desc("soup_qk_norm_rope", desc)) return rc;
   const bool norm = q_weight || k_weight;
-  if (!q || !q_strides || !q_out || !q_out_strides || hq <= 0 || !k || !k_strides || !k_out || !k_out_strides ||
-      hk <= 0 || batch <= 0 || seq <= 0 || head_dim <= 0 || head_dim % 2 || head_dim > kMaxDim || hq > 4096 ||
-      hk > 4096 || batch >= (int64_t(1) << 31) / seq || (norm && (!q_weight || !k_weight || inverse))) {
+  Angles a;
+  if (!q || !q_out || !k || !k_out || (norm && (!q_weight || !k_weight || desc->inverse)) ||
+      !fill_angles(a, *desc, table, second, axes)) {
     set_last_error("soup_qk_norm_rope: bad arguments");
     return SOUP_ERR_INVALID;
   }
-  Angles a;
-  if (!fill_angles(a, cos, sin, table_sb, table_ss, table_dtype, positions, positions_64, pos_sa, pos_sb, pos_ss,
-                   inv_freq, axes, head_dim / 2)) {
-    set_last_error("soup_qk_norm_rope: cos and sin tables, or positions with inv_freq and axes");
-    return SOUP_ERR_INVALID;
-  }
-  HeadRows tq{q, nullptr, q_out, q_strides[0], q_strides[1], q_strides[2], 0, 0, 0,
-              q_out_strides[0], q_out_strides[1], q_out_strides[2], q_weight, (int)hq};
-  HeadRows tk{k, nullptr, k_out, k_strides[0], k_strides[1], k_strides[2], 0, 0, 0,
-              k_out_strides[0], k_out_strides[1], k_out_strides[2], k_weight, (int)hk};
-  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, 1, eps, 1.f / (float)head_dim, w_dtype, inverse ? -1.f : 1.f};
+  const soup_qk_rope& d = *desc;
+  const HeadRows tq = rows_of(q, nullptr, q_out, d.q, d.q, d.q_out, q_weight, d.hq);
+  const HeadRows tk = rows_of(k, nullptr, k_out, d.k, d.k, d.k_out, k_weight, d.hk);
+  const Shape sh = shape_of(d);
+  const int dtype = (int)d.dtype;
   cudaStream_t st = as_stream(stream);
   if (dtype == SOUP_BF16) return run_fwd<__nv_bfloat16>(tq, tk, a, sh, norm, dtype, st);
   if (dtype == SOUP_F16) return run_fwd<__half>(tq, tk, a, sh, norm, dtype, st);
@@ -939,41 +953,28 @@ int soup_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, cons
   return SOUP_ERR_INVALID;
 }
 
-int soup_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_out_strides, const void* q, const int64_t* q_strides,
-                          void* dq, const int64_t* dq_strides, int64_t hq, const void* dk_out,
-                          const int64_t* dk_out_strides, const void* k, const int64_t* k_strides, void* dk,
-                          const int64_t* dk_strides, int64_t hk, const void* q_weight, const void* k_weight,
-                          float eps, void* dq_weight, void* dk_weight, const void* cos, const void* sin,
-                          int64_t table_sb, int64_t table_ss, int table_dtype, const void* positions,
-                          int positions_64, int64_t pos_sa, int64_t pos_sb, int64_t pos_ss, const float* inv_freq,
-                          const uint8_t* axes, int64_t batch, int64_t seq, int64_t head_dim, int dtype, int w_dtype,
+int soup_qk_norm_rope_bwd(const void* dq_out, const void* q, void* dq, const void* dk_out, const void* k, void* dk,
+                          const void* q_weight, const void* k_weight, void* dq_weight, void* dk_weight,
+                          const void* table, const void* second, const uint8_t* axes, const soup_qk_rope* desc,
                           void* workspace, size_t workspace_bytes, void* stream) {
-  if (!dq_out || !dq_out_strides || !q || !q_strides || !dq || !dq_strides || hq <= 0 || !dk_out ||
-      !dk_out_strides || !k || !k_strides || !dk || !dk_strides || hk <= 0 || !q_weight || !k_weight || batch <= 0 ||
-      seq <= 0 || head_dim <= 0 || head_dim % 2 || head_dim > kMaxDim || hq > 4096 || hk > 4096 ||
-      batch >= (int64_t(1) << 31) / seq) {
-    set_last_error("soup_qk_norm_rope_bwd: bad arguments");
-    return SOUP_ERR_INVALID;
-  }
+  if (int rc = check_desc("soup_qk_norm_rope_bwd", desc)) return rc;
+  const soup_qk_rope& d = *desc;
   Angles a;
-  if (!fill_angles(a, cos, sin, table_sb, table_ss, table_dtype, positions, positions_64, pos_sa, pos_sb, pos_ss,
-                   inv_freq, axes, head_dim / 2)) {
-    set_last_error("soup_qk_norm_rope_bwd: cos and sin tables, or positions with inv_freq and axes");
+  if (!dq_out || !q || !dq || !dk_out || !k || !dk || !q_weight || !k_weight || d.inverse || d.q_grad[3] != 1 ||
+      d.k_grad[3] != 1 || !fill_angles(a, d, table, second, axes)) {
+    set_last_error("soup_qk_norm_rope_bwd: bad arguments");
     return SOUP_ERR_INVALID;
   }
   if ((dq_weight || dk_weight) &&
       (!workspace || !aligned16(workspace) ||
-       workspace_bytes < soup_qk_norm_rope_bwd_workspace_bytes(batch, seq, hq, hk, head_dim))) {
+       workspace_bytes < soup_qk_norm_rope_bwd_workspace_bytes(d.batch, d.seq, d.hq, d.hk, d.head_dim))) {
     set_last_error("soup_qk_norm_rope_bwd: workspace missing, unaligned or too small");
     return SOUP_ERR_WORKSPACE;
   }
-  HeadRows tq{q, dq_out, dq, q_strides[0], q_strides[1], q_strides[2],
-              dq_out_strides[0], dq_out_strides[1], dq_out_strides[2],
-              dq_strides[0], dq_strides[1], dq_strides[2], q_weight, (int)hq};
-  HeadRows tk{k, dk_out, dk, k_strides[0], k_strides[1], k_strides[2],
-              dk_out_strides[0], dk_out_strides[1], dk_out_strides[2],
-              dk_strides[0], dk_strides[1], dk_strides[2], k_weight, (int)hk};
-  Shape sh{(int)batch, (int)seq, make_div(seq), (int)(head_dim / 2), 32, 0, 1, eps, 1.f / (float)head_dim, w_dtype, 1.f};
+  const HeadRows tq = rows_of(q, dq_out, dq, d.q, d.q_grad, d.q_out, q_weight, d.hq);
+  const HeadRows tk = rows_of(k, dk_out, dk, d.k, d.k_grad, d.k_out, k_weight, d.hk);
+  const Shape sh = shape_of(d);
+  const int dtype = (int)d.dtype;
   float* part = static_cast<float*>(workspace);
   cudaStream_t st = as_stream(stream);
   if (dtype == SOUP_BF16) return run_bwd<__nv_bfloat16>(tq, tk, a, sh, dq_weight, dk_weight, part, dtype, st);

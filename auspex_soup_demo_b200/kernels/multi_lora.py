@@ -9,6 +9,7 @@ once: csrc/multi_lora.cu.
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Union
 
 import torch
@@ -20,17 +21,46 @@ MAX_RANK_COLUMNS = 4096
 MAX_TOKENS = 1 << 21
 
 
+@functools.lru_cache(maxsize=256)
+def _state_bytes(tokens: int, adapters: int, rank: int) -> int:
+    return _lib.lib().soup_multi_lora_state_bytes(tokens, adapters, rank)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(tokens: int, adapters: int, rank: int) -> int:
+    return _lib.lib().soup_multi_lora_bwd_workspace_bytes(tokens, adapters, rank)
+
+
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """t as [rows, width] operand rows that TMA can read (copied only if they are not)."""
-    t = t.reshape(-1, width)
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < width or t.data_ptr() % 16:
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    ld, step = t.stride()
+    if step != 1 or ld % 8 or ld < width or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
 def _factor(t: torch.Tensor) -> torch.Tensor:
     """A stack of factors as dense bf16."""
-    return _lib.dense(t.detach().to(torch.bfloat16))
+    return _lib.dense(t if t.dtype is torch.bfloat16 else t.detach().to(torch.bfloat16))
+
+
+def _forward(x, weight, lora_a, lora_b, ids, scaling, bias, per: int):
+    """(y, x rows, weight rows, bf16 factors, state)"""
+    n, k = weight.shape
+    x2, w = _rows(x, k), _rows(weight, k)
+    a16, b16 = _factor(lora_a), _factor(lora_b)
+    na, r = lora_a.shape[0], lora_a.shape[1]
+    t = x2.shape[0]
+    y = x.new_empty((*x.shape[:-1], n))
+    nbytes = _state_bytes(t, na, r)
+    state = x.new_empty(nbytes, dtype=torch.uint8)
+    _lib.call("soup_multi_lora_fwd", x.device, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _lib.ptr(bias),
+              a16.data_ptr(), b16.data_ptr(), scaling.data_ptr(), ids.data_ptr(),
+              1 if ids.dtype is torch.int64 else 0, per, t, n, k, na, r, y.data_ptr(), n, state.data_ptr(),
+              nbytes, _lib.stream_of(x))
+    return y, x2, w, a16, b16, state
 
 
 class MultiLoRAFunction(torch.autograd.Function):
@@ -38,25 +68,10 @@ class MultiLoRAFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, lora_a, lora_b, ids, scaling, bias, per: int):
-        k, n = x.shape[-1], weight.shape[0]
-        x2, w = _rows(x, k), _rows(weight, k)
-        a16, b16 = _factor(lora_a), _factor(lora_b)
-        na, r = lora_a.shape[:2]
-        t = x2.shape[0]
-        dev = x.device
-        y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=dev)
-        nbytes = _lib.lib().soup_multi_lora_state_bytes(t, na, r)
-        state = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("soup_multi_lora_fwd", dev, x2.data_ptr(), x2.stride(0), w.data_ptr(), w.stride(0), _lib.ptr(bias),
-                  a16.data_ptr(), b16.data_ptr(), scaling.data_ptr(), ids.data_ptr(),
-                  1 if ids.dtype is torch.int64 else 0, per, t, n, k, na, r, y.data_ptr(), n, state.data_ptr(),
-                  nbytes, _lib.stream_of(x))
-        need = ctx.needs_input_grad
-        if need[0] or need[2] or need[3]:
-            # x is needed for lora_a's gradient alone
-            ctx.save_for_backward(x2 if need[2] else None, w, a16, b16, ids, scaling, state)
-            ctx.per, ctx.shape = per, x.shape
-            ctx.dtypes = lora_a.dtype, lora_b.dtype
+        y, x2, w, a16, b16, state = _forward(x, weight, lora_a, lora_b, ids, scaling, bias, per)
+        # x is needed for lora_a's gradient alone
+        ctx.save_for_backward(x2 if ctx.needs_input_grad[2] else None, w, a16, b16, ids, scaling, state)
+        ctx.meta = per, x.shape, lora_a.dtype, lora_b.dtype
         return y
 
     @staticmethod
@@ -66,37 +81,37 @@ class MultiLoRAFunction(torch.autograd.Function):
         x2, w, a16, b16, ids, scaling, state = ctx.saved_tensors
         a16, b16, state = _lib.dense(a16), _lib.dense(b16), _lib.dense(state)
         ids, scaling = ids.contiguous(), scaling.contiguous()
+        per, shape, a_dtype, b_dtype = ctx.meta
         n, k = w.shape
         w = _rows(w, k)
-        na, r = a16.shape[:2]
+        na, r = a16.shape[0], a16.shape[1]
         need_x, _, need_a, need_b = ctx.needs_input_grad[:4]
         dy2 = _rows(dy, n)
         t = dy2.shape[0]
         dev = dy2.device
         x2 = _rows(x2, k) if need_a else None
-        dx = torch.empty(ctx.shape, dtype=dy2.dtype, device=dev) if need_x else None
+        dx = dy2.new_empty(shape) if need_x else None
 
         def grad(need, like, dtype):
             if not need:
                 return None
-            return torch.empty(like.shape, dtype=torch.bfloat16 if dtype is torch.bfloat16 else torch.float32,
-                               device=dev)
+            return torch.empty_like(like) if dtype is torch.bfloat16 else torch.empty_like(like, dtype=torch.float32)
 
-        da, db = grad(need_a, a16, ctx.dtypes[0]), grad(need_b, b16, ctx.dtypes[1])
+        da, db = grad(need_a, a16, a_dtype), grad(need_b, b16, b_dtype)
         nbytes, ws = 0, None
         if need_x or need_a:
-            nbytes = _lib.lib().soup_multi_lora_bwd_workspace_bytes(t, na, r)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            nbytes = _workspace_bytes(t, na, r)
+            ws = dy2.new_empty(nbytes, dtype=torch.uint8)
         _lib.call("soup_multi_lora_bwd", dev, dy2.data_ptr(), dy2.stride(0), _lib.ptr(x2),
                   k if x2 is None else x2.stride(0), w.data_ptr(), w.stride(0), a16.data_ptr(), b16.data_ptr(),
-                  scaling.data_ptr(), ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, ctx.per, t, n, k, na, r,
+                  scaling.data_ptr(), ids.data_ptr(), 1 if ids.dtype is torch.int64 else 0, per, t, n, k, na, r,
                   state.data_ptr(), state.numel(), _lib.ptr(dx), k, _lib.ptr(da),
                   _lib.F32 if da is None else _lib.dtype_code(da.dtype), _lib.ptr(db),
                   _lib.F32 if db is None else _lib.dtype_code(db.dtype), _lib.ptr(ws), nbytes, _lib.stream_of(dy2))
-        if da is not None:
-            da = da.to(ctx.dtypes[0])
-        if db is not None:
-            db = db.to(ctx.dtypes[1])
+        if da is not None and da.dtype is not a_dtype:
+            da = da.to(a_dtype)
+        if db is not None and db.dtype is not b_dtype:
+            db = db.to(b_dtype)
         return dx, None, da, db, None, None, None, None
 
 
@@ -123,44 +138,46 @@ def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tenso
     that streams the weight once through all SMs.
     """
     fn = "multi_lora_linear"
-    if x.dim() < 1 or weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
+    xs, ws, sa, sb = x.shape, weight.shape, lora_a.shape, lora_b.shape
+    if len(xs) < 1 or len(ws) != 2 or len(sa) != 3 or len(sb) != 3:
         raise ValueError(f"{fn}: x [..., K], weight [N, K], lora_a [adapters, rank, K], lora_b [N, adapters, rank]; got "
-                         f"{tuple(x.shape)}, {tuple(weight.shape)}, {tuple(lora_a.shape)}, {tuple(lora_b.shape)}")
-    n, k = weight.shape
-    na, r, ka = lora_a.shape
-    if x.shape[-1] != k or ka != k or tuple(lora_b.shape) != (n, na, r):
-        raise ValueError(f"{fn}: x {tuple(x.shape)}, weight {tuple(weight.shape)}, lora_a {tuple(lora_a.shape)} and "
-                         f"lora_b {tuple(lora_b.shape)} do not fit together")
-    if 0 in (n, k, na, r) or n % 8 or k % 8 or na * r % 8 or na * r > MAX_RANK_COLUMNS:
+                         f"{tuple(xs)}, {tuple(ws)}, {tuple(sa)}, {tuple(sb)}")
+    n, k = ws
+    na, r, ka = sa
+    if xs[-1] != k or ka != k or sb != (n, na, r):
+        raise ValueError(f"{fn}: x {tuple(xs)}, weight {tuple(ws)}, lora_a {tuple(sa)} and lora_b {tuple(sb)} do not "
+                         "fit together")
+    if n == 0 or k == 0 or na * r == 0 or n % 8 or k % 8 or na * r % 8 or na * r > MAX_RANK_COLUMNS:
         raise ValueError(f"{fn}: N, K and adapters * rank must be multiples of 8, adapters * rank at most "
                          f"{MAX_RANK_COLUMNS}; got N {n}, K {k}, {na} adapters of rank {r}")
     if x.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16:
         raise TypeError(f"{fn}: x and weight must be bfloat16, got {x.dtype} and {weight.dtype}")
-    for t in (lora_a, lora_b):
-        _lib.dtype_code(t.dtype)
+    _lib.dtype_code(lora_a.dtype)
+    _lib.dtype_code(lora_b.dtype)
     dev = x.device
-    if not x.is_cuda or any(t.device != dev for t in (weight, lora_a, lora_b, adapter_ids)):
+    if not x.is_cuda or weight.device != dev or lora_a.device != dev or lora_b.device != dev or \
+            adapter_ids.device != dev:
         raise ValueError(f"{fn}: all tensors must be on one CUDA device")
     if weight.requires_grad:
         raise ValueError(f"{fn}: the weight is frozen; detach it")
-    if adapter_ids.dtype not in (torch.int64, torch.int32):
+    if adapter_ids.dtype is not torch.int64 and adapter_ids.dtype is not torch.int32:
         raise TypeError(f"{fn}: adapter_ids must be int64 or int32, got {adapter_ids.dtype}")
-    ishape, lead = tuple(adapter_ids.shape), tuple(x.shape[:-1])
-    if ishape == lead:
+    ishape = adapter_ids.shape
+    if ishape == xs[:-1]:
         per = 1
-    elif len(lead) == 2 and ishape == lead[:1]:
-        per = max(1, lead[1])
+    elif len(xs) == 3 and ishape == xs[:1]:
+        per = max(1, xs[1])
     else:
-        raise ValueError(f"{fn}: adapter_ids {ishape} for x {tuple(x.shape)}: one for each token, or for each sequence "
+        raise ValueError(f"{fn}: adapter_ids {tuple(ishape)} for x {tuple(xs)}: one for each token, or for each sequence "
                          "of x [B, S, K]")
     if bias is not None:
-        if tuple(bias.shape) != (n,) or bias.dtype is not torch.bfloat16 or bias.device != dev:
+        if bias.shape != (n,) or bias.dtype is not torch.bfloat16 or bias.device != dev:
             raise ValueError(f"{fn}: bias must be bfloat16 [{n}] on {dev}")
         if bias.requires_grad:
             raise ValueError(f"{fn}: the bias is frozen; detach it")
         bias = bias.contiguous()
     if isinstance(scaling, torch.Tensor):
-        if tuple(scaling.shape) != (na,) or scaling.dtype is not torch.float32 or scaling.device != dev:
+        if scaling.shape != (na,) or scaling.dtype is not torch.float32 or scaling.device != dev:
             raise ValueError(f"{fn}: scaling must be a number, or float32 [{na}] on {dev}")
         if scaling.requires_grad:
             raise ValueError(f"{fn}: scaling is a constant; detach it")
@@ -172,5 +189,8 @@ def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tenso
         raise ValueError(f"{fn}: at most {MAX_TOKENS} tokens, got {t}")
     if t == 0:
         # empty, connected to the states and the factors
-        return x.new_zeros(*lead, n) + (x.sum() + lora_a[:, :0].sum() + lora_b[:0].sum()).to(x.dtype)
-    return MultiLoRAFunction.apply(x, weight, lora_a, lora_b, adapter_ids.contiguous(), scaling, bias, per)
+        return x.new_zeros(*xs[:-1], n) + (x.sum() + lora_a[:, :0].sum() + lora_b[:0].sum()).to(x.dtype)
+    ids = adapter_ids.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad):
+        return MultiLoRAFunction.apply(x, weight, lora_a, lora_b, ids, scaling, bias, per)
+    return _forward(x, weight, lora_a, lora_b, ids, scaling, bias, per)[0]

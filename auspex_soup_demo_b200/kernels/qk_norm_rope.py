@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -25,6 +26,11 @@ import torch
 from .. import _lib
 
 MAX_HEAD_DIM = 512
+
+# soup_qk_rope: sizes, types, table strides, six tensors' strides, eps
+_DESC = struct.Struct("=5q5q3q24qd")
+_NONE = (0, 0, 0, 0)
+_TABLES, _INT32, _INT64 = 0, 1, 2
 
 
 @functools.lru_cache(maxsize=64)
@@ -63,47 +69,28 @@ def _head_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _strides(t: torch.Tensor):
-    s = t.stride()
-    return _lib.i64_array(s[:3])
-
-
-class _Angles:
-    """Arguments of both C calls that say where the angles come from."""
-
-    __slots__ = ("args", "keep")
-
-    @staticmethod
-    def tables(cos, sin, shape):
-        b, _, s, d = shape
-        a = _Angles()
+def _source(a: torch.Tensor, c: torch.Tensor, axes):
+    """(table dtype code, source, its three strides, axes) for the C calls: a and c are
+    tables [B | 1, S, D] or [S, D], or positions [axes, B | 1, S] or [axes, S] and frequencies."""
+    st = a.stride()
+    wide = len(st) == 3
+    if axes is None:
         # only the first half of a table's row is read
-        sb = cos.stride(0) if cos.dim() > 2 and cos.shape[0] > 1 else 0
-        a.keep = (cos, sin)
-        a.args = (cos.data_ptr(), sin.data_ptr(), sb, cos.stride(-2), _lib.dtype_code(cos.dtype), 0, 0, 0, 0, 0, 0,
-                  None)
-        return a
-
-    @staticmethod
-    def positions(pos, inv_freq, axes):
-        a = _Angles()
-        st = pos.stride()
-        a.keep = (pos, inv_freq)
-        # [axes, B | 1, S] or [axes, S]
-        sb = st[1] if pos.dim() == 3 and pos.shape[1] > 1 else 0
-        a.args = (0, 0, 0, 0, 0, pos.data_ptr(), 1 if pos.dtype is torch.int64 else 0, st[0], sb, st[-1],
-                  inv_freq.data_ptr(), _axes_bytes(axes))
-        return a
+        return _lib.dtype_code(a.dtype), _TABLES, (0, st[0] if wide and a.shape[0] > 1 else 0, st[-2]), None
+    return (0, _INT64 if a.dtype is torch.int64 else _INT32,
+            (st[0], st[1] if wide and a.shape[1] > 1 else 0, st[-1]), _axes_bytes(axes))
 
 
-def _forward(q, k, qw, kw, eps, angles, inverse=0):
-    b, hq, s, d = q.shape
-    hk = k.shape[1]
+def _forward(q, k, qw, kw, eps, a, c, axes, inverse=0):
     qo, ko = torch.empty_like(q), torch.empty_like(k)
-    _lib.call("soup_qk_norm_rope", q.device, q.data_ptr(), _strides(q), qo.data_ptr(), _strides(qo), hq,
-              k.data_ptr(), _strides(k), ko.data_ptr(), _strides(ko), hk, _lib.ptr(qw), _lib.ptr(kw), eps,
-              *angles.args, b, s, d, _lib.dtype_code(q.dtype), 0 if qw is None else _lib.dtype_code(qw.dtype),
-              inverse, _lib.stream_of(q))
+    b, hq, s, d = q.shape
+    code = _lib.dtype_code(q.dtype)
+    tcode, src, ts, ax = _source(a, c, axes)
+    desc = _DESC.pack(b, s, d, hq, k.shape[1], code, code if qw is None else _lib.dtype_code(qw.dtype), tcode, src,
+                      inverse, *ts, *q.stride(), *qo.stride(), *k.stride(), *ko.stride(), *_NONE, *_NONE, eps)
+    _lib.call("soup_qk_norm_rope", q.device, q.data_ptr(), qo.data_ptr(), k.data_ptr(), ko.data_ptr(),
+              0 if qw is None else qw.data_ptr(), 0 if kw is None else kw.data_ptr(), a.data_ptr(), c.data_ptr(), ax,
+              desc, _lib.stream_of(q))
     return qo, ko
 
 
@@ -113,14 +100,12 @@ class QKNormRoPEFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, qw, kw, eps: float, a, c, axes):
-        make = _Angles.tables(a, c, q.shape) if axes is None else _Angles.positions(a, c, axes)
-        out = _forward(q, k, qw, kw, eps, make)
+        out = _forward(q, k, qw, kw, eps, a, c, axes)
         if qw is None:
             ctx.save_for_backward(a, c)
         else:
             ctx.save_for_backward(a, c, q, k, qw, kw)
-        ctx.eps, ctx.axes = eps, axes
-        ctx.meta = (q.shape, k.shape, q.dtype)
+        ctx.meta = eps, axes, q.shape, k.shape, q.dtype
         ctx.set_materialize_grads(False)
         return out
 
@@ -129,38 +114,40 @@ class QKNormRoPEFunction(torch.autograd.Function):
     def backward(ctx, gq, gk):
         if gq is None and gk is None:
             return (None,) * 8
-        qs, ks, dt = ctx.meta
+        eps, axes, qs, ks, dt = ctx.meta
         saved = ctx.saved_tensors
-        a, c = saved[:2]
+        a, c = saved[0], saved[1]
+        # a saved-tensor hook may hand them back in another layout
+        if axes is None:
+            if a.stride(-1) != 1 or c.stride() != a.stride():
+                a, c = a.contiguous(), c.contiguous()
+        elif not c.is_contiguous():
+            c = c.contiguous()
         dev = a.device
-        # a saved-tensor hook may hand tables and positions back in another layout
-        if ctx.axes is None:
-            a, c = _table_rows(a, c)
-            make = _Angles.tables(a, c, qs)
-        else:
-            make = _Angles.positions(a, c.contiguous(), ctx.axes)
         gq = torch.zeros(qs, dtype=dt, device=dev) if gq is None else _head_rows(gq)
         gk = torch.zeros(ks, dtype=dt, device=dev) if gk is None else _head_rows(gk)
         if len(saved) == 2:
-            dq, dk = _forward(gq, gk, None, None, ctx.eps, make, 1)
+            dq, dk = _forward(gq, gk, None, None, eps, a, c, axes, 1)
             return dq, dk, None, None, None, None, None, None
         q, k = _head_rows(saved[2]), _head_rows(saved[3])
-        qw, kw = saved[4].contiguous(), saved[5].contiguous()
-        need_q, need_k = ctx.needs_input_grad[2:4]
+        qw, kw = _lib.dense(saved[4]), _lib.dense(saved[5])
+        _, _, need_q, need_k = ctx.needs_input_grad[:4]
         b, hq, s, d = qs
         hk = ks[1]
         dq, dk = torch.empty_like(q), torch.empty_like(k)
-        dqw = torch.empty(d, dtype=qw.dtype, device=dev) if need_q else None
-        dkw = torch.empty(d, dtype=qw.dtype, device=dev) if need_k else None
-        nbytes, ws = 0, None
+        dqw = torch.empty_like(qw) if need_q else None
+        dkw = torch.empty_like(kw) if need_k else None
+        nbytes, ws = 0, 0
         if need_q or need_k:
             nbytes = _workspace_bytes(b, s, hq, hk, d)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("soup_qk_norm_rope_bwd", dev, gq.data_ptr(), _strides(gq), q.data_ptr(), _strides(q),
-                  dq.data_ptr(), _strides(dq), hq, gk.data_ptr(), _strides(gk), k.data_ptr(), _strides(k),
-                  dk.data_ptr(), _strides(dk), hk, qw.data_ptr(), kw.data_ptr(), ctx.eps, _lib.ptr(dqw),
-                  _lib.ptr(dkw), *make.args, b, s, d, _lib.dtype_code(dt), _lib.dtype_code(qw.dtype), _lib.ptr(ws),
-                  nbytes, _lib.stream_of(q))
+            buf = a.new_empty(nbytes, dtype=torch.uint8)
+            ws = buf.data_ptr()
+        tcode, src, ts, ax = _source(a, c, axes)
+        desc = _DESC.pack(b, s, d, hq, hk, _lib.dtype_code(dt), _lib.dtype_code(qw.dtype), tcode, src, 0, *ts,
+                          *q.stride(), *dq.stride(), *k.stride(), *dk.stride(), *gq.stride(), *gk.stride(), eps)
+        _lib.call("soup_qk_norm_rope_bwd", dev, gq.data_ptr(), q.data_ptr(), dq.data_ptr(), gk.data_ptr(),
+                  k.data_ptr(), dk.data_ptr(), qw.data_ptr(), kw.data_ptr(), _lib.ptr(dqw), _lib.ptr(dkw),
+                  a.data_ptr(), c.data_ptr(), ax, desc, ws, nbytes, _lib.stream_of(q))
         return dq, dk, dqw, dkw, None, None, None, None
 
 
@@ -191,12 +178,6 @@ def _check(fn: str, q, k, qw, kw, eps):
             raise ValueError(f"{fn}: eps must be 0 or more, not {eps}")
 
 
-def _table_rows(cos, sin):
-    if cos.stride(-1) != 1 or sin.stride() != cos.stride():
-        cos, sin = cos.contiguous(), sin.contiguous()
-    return cos, sin
-
-
 def _apply(q, k, qw, kw, eps, a, c, axes):
     if 0 in q.shape or 0 in k.shape:
         # no rows: empty results, connected to what they are made of
@@ -205,10 +186,10 @@ def _apply(q, k, qw, kw, eps, a, c, axes):
     q, k = _head_rows(q), _head_rows(k)
     if qw is not None:
         qw, kw = qw.contiguous(), kw.contiguous()
-    if not torch.is_grad_enabled():
-        make = _Angles.tables(a, c, q.shape) if axes is None else _Angles.positions(a, c, axes)
-        return _forward(q, k, qw, kw, eps, make)
-    return QKNormRoPEFunction.apply(q, k, qw, kw, eps, a, c, axes)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
+                                    (qw is not None and (qw.requires_grad or kw.requires_grad))):
+        return QKNormRoPEFunction.apply(q, k, qw, kw, eps, a, c, axes)
+    return _forward(q, k, qw, kw, eps, a, c, axes)
 
 
 def apply_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -227,23 +208,24 @@ def apply_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     _check("apply_qk_norm_rope", q, k, q_weight, k_weight, eps)
     if q_weight is None:
         raise ValueError("apply_qk_norm_rope: norm weights are needed; apply_fast_rope_qk rotates alone")
-    b, _, s, d = q.shape
     if cos.dim() == 4 and cos.shape[1] == 1:
         cos = cos[:, 0]
     if sin.dim() == 4 and sin.shape[1] == 1:
         sin = sin[:, 0]
-    for t in (cos, sin):
-        if t.dim() not in (2, 3) or tuple(t.shape[-2:]) != (s, d) or (t.dim() == 3 and t.shape[0] not in (1, b)):
-            raise ValueError(f"apply_qk_norm_rope: cos and sin must be [B | 1, 1, S, D], [B | 1, S, D] or [S, D], got "
-                             f"{tuple(t.shape)}")
-        if t.device != q.device:
-            raise ValueError(f"apply_qk_norm_rope: cos and sin must be on {q.device}")
-        _lib.dtype_code(t.dtype)
-        if t.requires_grad:
-            raise ValueError("apply_qk_norm_rope: cos and sin are constants; detach them")
-    if cos.shape != sin.shape or cos.dtype != sin.dtype:
-        raise ValueError("apply_qk_norm_rope: cos and sin must share shape and dtype")
-    cos, sin = _table_rows(cos, sin)
+    shape = cos.shape
+    if sin.shape != shape or len(shape) not in (2, 3) or shape[-2:] != (q.shape[2], q.shape[3]) or \
+            (len(shape) == 3 and shape[0] not in (1, q.shape[0])):
+        raise ValueError(f"apply_qk_norm_rope: cos and sin must be [B | 1, 1, S, D], [B | 1, S, D] or [S, D], got "
+                         f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+    if cos.device != q.device or sin.device != q.device:
+        raise ValueError(f"apply_qk_norm_rope: cos and sin must be on {q.device}")
+    if cos.dtype != sin.dtype:
+        raise TypeError(f"apply_qk_norm_rope: cos and sin must share their type, got {cos.dtype} and {sin.dtype}")
+    _lib.dtype_code(cos.dtype)
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("apply_qk_norm_rope: cos and sin are constants; detach them")
+    if cos.stride(-1) != 1 or sin.stride() != cos.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
     return _apply(q, k, q_weight, k_weight, float(eps), cos, sin, None)
 
 

@@ -118,7 +118,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         for i, p in enumerate(params):
             if p.numel():
                 by.setdefault(p.dtype, []).append(i)
-        held.by_dtype = [(_lib.dtype_code(d), idx, array.array("q", [held.sizes[i] for i in idx]),
+        held.by_dtype = [(_lib.dtype_code(d), d, idx, array.array("q", [held.sizes[i] for i in idx]),
                           array.array("i", [blocks[i] for i in idx])) for d, idx in by.items()]
         eight = self.state_bits == 8
         dt = torch.float8_e4m3fn if eight else torch.float32
@@ -187,30 +187,26 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         type's parameters that have a gradient; the gradients are kept until the launch."""
         out = []
         params, ptrs = held.params, held.ptrs
-        for code, idx, sizes, blocks in held.by_dtype:
+        for code, dtype, idx, sizes, blocks in held.by_dtype:
             grads = [params[i].grad for i in idx]
-            keep = [(i, g) for i, g in zip(idx, grads) if g is not None]
+            keep = [i for i, g in zip(idx, grads) if g is not None]
             if len(keep) < len(idx):
                 if not keep:
                     continue
-                idx = [i for i, _ in keep]
-                grads = [g for _, g in keep]
+                idx = keep
+                grads = [g for g in grads if g is not None]
                 sizes = array.array("q", [held.sizes[i] for i in idx])
                 blocks = array.array("i", [held.blocks[i] for i in idx])
-            for j, g in enumerate(grads):
-                if not g.is_contiguous():
-                    if g.layout is not torch.strided:
-                        raise ValueError("MultiTensorAdamW: gradients must be dense")
-                    grads[j] = g.contiguous()
-            for t in {(g.dtype, g.device) for g in grads}:
-                if _lib.dtype_code(t[0]) != code or t[1] != device:
-                    raise ValueError(f"MultiTensorAdamW: a gradient of type {t[0]} on {t[1]} for parameters of another "
-                                     "type or device")
+            if not all([g.is_contiguous() for g in grads]):
+                if any(g.layout is not torch.strided for g in grads):
+                    raise ValueError("MultiTensorAdamW: gradients must be dense")
+                grads = [g.detach().contiguous() for g in grads]
+            if {g.dtype for g in grads} != {dtype} or grads[0].device != device:
+                raise ValueError(f"MultiTensorAdamW: gradients must be {dtype} on {device}, as their parameters")
             out.append((code, array.array("Q", [ptrs[i]() for i in idx]),
                         array.array("Q", [g.data_ptr() for g in grads]), sizes, blocks, grads))
         return out
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One step over all parameters that have a gradient."""
         loss = None

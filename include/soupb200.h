@@ -155,32 +155,36 @@ int soup_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_
  * No counterpart in the reference (its RoPE takes rows as they are). One launch
  * normalises every head's row of q and k (n = x * w / sqrt(mean(x^2) + eps); both
  * weights [head_dim], or both NULL for a rotation alone) and rotates its halves.
- * Angles come from cos / sin tables (table_dtype; first head_dim / 2 entries at
- * [b * table_sb + s * table_ss]), or, with cos and sin NULL, from positions:
- * positions[axes[i] * pos_sa + b * pos_sb + s * pos_ss] * inv_freq[i], int32 or
- * (positions_64) int64, reduced in 64 bits; axes [head_dim / 2] is host memory.
- * inverse != 0 rotates back (without weights: the backward of a rotation alone).
- * head_dim even, at most 512; strides {b, h, s} in elements, last dim contiguous.
- * soup_qk_norm_rope_bwd: gradients of q, k and, where not NULL, of the weights
- * (w_dtype), summed over tokens and heads in 32 bits in a fixed order through the
- * workspace; workspace may be NULL without weight gradients. */
-int soup_qk_norm_rope(const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int64_t hq,
-                      const void* k, const int64_t* k_strides, void* k_out, const int64_t* k_out_strides,
-                      int64_t hk, const void* q_weight, const void* k_weight, float eps, const void* cos,
-                      const void* sin, int64_t table_sb, int64_t table_ss, int table_dtype, const void* positions,
-                      int positions_64, int64_t pos_sa, int64_t pos_sb, int64_t pos_ss, const float* inv_freq,
-                      const uint8_t* axes, int64_t batch, int64_t seq, int64_t head_dim, int dtype, int w_dtype,
-                      int inverse, void* stream);
+ * Angles, by `source`: cos and sin tables (table, second; table_dtype; the first
+ * head_dim / 2 entries at [b * table[1] + s * table[2]]), or positions (table, int32 or
+ * int64) and fp32 frequencies (second [head_dim / 2]): frequency i turns by
+ * table[axes[i] * table[0] + b * table[1] + s * table[2]] * second[i], reduced in 64 bits;
+ * axes [head_dim / 2] is host memory. inverse != 0 rotates back (without weights: the
+ * backward of a rotation alone). head_dim even, at most 512; strides {b, h, s, 1} in
+ * elements.
+ * soup_qk_norm_rope_bwd: gradients of q, k (strides q_out, k_out) from those of the
+ * rotated rows (q_grad, k_grad), and, where not NULL, of the weights (w_dtype), summed
+ * over tokens and heads in 32 bits in a fixed order through the workspace, which may be
+ * NULL without weight gradients. */
+#define SOUP_ROPE_TABLES 0
+#define SOUP_ROPE_INT32 1
+#define SOUP_ROPE_INT64 2
+typedef struct {
+  int64_t batch, seq, head_dim, hq, hk;
+  int64_t dtype, w_dtype, table_dtype, source, inverse;
+  int64_t table[3];
+  int64_t q[4], q_out[4], k[4], k_out[4];
+  int64_t q_grad[4], k_grad[4]; /* backward */
+  double eps;
+} soup_qk_rope;
+int soup_qk_norm_rope(const void* q, void* q_out, const void* k, void* k_out, const void* q_weight,
+                      const void* k_weight, const void* table, const void* second, const uint8_t* axes,
+                      const soup_qk_rope* desc, void* stream);
 size_t soup_qk_norm_rope_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t hq, int64_t hk,
                                              int64_t head_dim);
-int soup_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_out_strides, const void* q, const int64_t* q_strides,
-                          void* dq, const int64_t* dq_strides, int64_t hq, const void* dk_out,
-                          const int64_t* dk_out_strides, const void* k, const int64_t* k_strides, void* dk,
-                          const int64_t* dk_strides, int64_t hk, const void* q_weight, const void* k_weight,
-                          float eps, void* dq_weight, void* dk_weight, const void* cos, const void* sin,
-                          int64_t table_sb, int64_t table_ss, int table_dtype, const void* positions,
-                          int positions_64, int64_t pos_sa, int64_t pos_sb, int64_t pos_ss, const float* inv_freq,
-                          const uint8_t* axes, int64_t batch, int64_t seq, int64_t head_dim, int dtype, int w_dtype,
+int soup_qk_norm_rope_bwd(const void* dq_out, const void* q, void* dq, const void* dk_out, const void* k, void* dk,
+                          const void* q_weight, const void* k_weight, void* dq_weight, void* dk_weight,
+                          const void* table, const void* second, const uint8_t* axes, const soup_qk_rope* desc,
                           void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- A projection with several adapters ----------------------------------------
