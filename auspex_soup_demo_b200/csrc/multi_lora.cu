@@ -24,7 +24,8 @@
 //
 // Few tokens (T <= 64: next tokens of many requests): the base product is W's bytes.
 // The same kernel then streams W as the 128-row operand against all tokens at once
-// (N = T rounded up), so that every SM takes part, with U and B's blocks behind.
+// (N = T rounded up), so that every SM takes part, with U and B's blocks behind; it starts
+// beside the kernel that forms U and waits for that one only before its rank blocks.
 //
 // u and v are rounded to bf16 between the two products, as x, dy and the factors are.
 //
@@ -155,12 +156,15 @@ __device__ __forceinline__ uint64_t warp_or64(uint64_t v) {
   return ((uint64_t)hi << 32) | lo;
 }
 
-// The k blocks of a CTA: a run of blocks, then (kModeFew) the rank blocks of a word; or
-// (kModeGrad) the set bits [lo, hi) of a bit list. Producer and MMA issuer walk the same.
+// The k blocks of a CTA: a run of blocks and (kModeFew) behind it its share of the rank
+// blocks of the tokens' word; or (kModeGrad) the set bits [lo, hi) of a bit list.
+// Producer and MMA issuer walk the same.
 struct KWalk {
-  int kb, end;          // run
-  uint64_t word;        // rank blocks behind it
-  const uint32_t* bits; // or: bit list
+  int kb, end;             // run
+  const uint64_t* pending; // the word, not read yet
+  int rank, ks;
+  uint64_t word;           // rank blocks still to come
+  const uint32_t* bits;    // or: bit list
   int skip, left;
   int w;
   uint32_t cur;
@@ -192,6 +196,19 @@ struct KWalk {
     if (kb < end) {
       k_block = kb++;
       return true;
+    }
+    if (pending) {
+      // the word and U are of the kernel before, whose end is waited for only here: the
+      // run's operands were complete before that kernel let this one start
+      pdl_wait();
+      uint64_t all = *pending;
+      pending = nullptr;
+      const int n = __popcll(all);
+      const int lo = n * rank / ks, hi = n * (rank + 1) / ks;
+      for (int i = 0; i < hi; ++i) {
+        if (i >= lo) word |= all & (~all + 1);
+        all &= all - 1;
+      }
     }
     if (word) {
       k_block = __ffsll((long long)word) - 1;
@@ -243,8 +260,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int rb = blockIdx.y;
   const uint64_t wait_ns = a.wait_ns ? a.wait_ns : kWaitNs;
 
-  pdl_wait();
-  pdl_trigger();
+  if constexpr (MODE != kModeFew) {
+    pdl_wait();
+    pdl_trigger();
+  }
   bool mine = true;  // kModeRank: this tile's 128 tokens have the rank block
   if constexpr (MODE == kModeRank) {
     // words of the 256 tokens around this tile, from the ids; cluster-uniform
@@ -303,21 +322,13 @@ __global__ void __launch_bounds__(kThreads, 2)
       k.left = (int)((int64_t)count * (rank + 1) / ks) - k.skip;
       k.w = -1;
     } else {
-      // kModeFew: the rank blocks are shared out behind the run, to the last CTA of the cluster
       k.kb = (int)((int64_t)a.kb_total * rank / ks);
       k.end = (int)((int64_t)a.kb_total * (rank + 1) / ks);
       if (MODE == kModeRank && !mine) k.end = k.kb;
       if (MODE == kModeFew) {
-        uint64_t w = a.mask256[0];
-        const int n = __popcll(w);
-        const int lo = (int)((int64_t)n * rank / ks), hi = (int)((int64_t)n * (rank + 1) / ks);
-        for (int i = 0; i < lo; ++i) w &= w - 1;
-        uint64_t part_word = 0;
-        for (int i = lo; i < hi; ++i) {
-          part_word |= w & (~w + 1);
-          w &= w - 1;
-        }
-        k.word = part_word;
+        k.pending = a.mask256;
+        k.rank = rank;
+        k.ks = ks;
       }
     }
     return k;
@@ -398,10 +409,16 @@ __global__ void __launch_bounds__(kThreads, 2)
     // ------------------------------------------------------ epilogue ----
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
-    KWalk k = walk();
-    int kb;
-    bool second;
-    any = k.next(kb, second);
+    if constexpr (MODE == kModeFew) {
+      any = true;  // the run is at least four blocks
+      pdl_wait();  // y may be memory that the kernels before this one still used
+      pdl_trigger();
+    } else {
+      KWalk k = walk();
+      int kb;
+      bool second;
+      any = k.next(kb, second);
+    }
     bool ok = true;
     if (lane == 0) ok = bounded_wait(acc_bar, 0, abort_flag, err, kErrEpilogue, wait_ns);
     ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -504,6 +521,51 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
+  }
+}
+
+// U of few tokens: a warp a (token, rank column), 16 bytes of x and of A's row a lane and
+// step. Bound by the latency of ids -> A -> sum, a third of the tile kernel's.
+constexpr int kFewWarps = 8;
+__global__ void __launch_bounds__(32 * kFewWarps) few_rank_kernel(const bf16* __restrict__ x, int64_t ldx,
+                                                                  const bf16* __restrict__ lora_a, const Args a) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x, j = blockIdx.y * kFewWarps + warp;
+  const int id = adapter_of(a, t);
+  if (id >= 0 && j < a.rank) {
+    const uint4* row = reinterpret_cast<const uint4*>(lora_a + ((int64_t)id * a.rank + j) * a.k);
+    const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)t * ldx);
+    uint64_t sum = 0;
+    const int parts = a.k / 8;
+#pragma unroll 4
+    for (int i = lane; i < parts; i += 32) {
+      const uint4 u = xr[i], v = row[i];
+      const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        sum = f2_fma(f2_pack(__uint_as_float(us[q] << 16), __uint_as_float(us[q] & 0xffff0000u)),
+                     f2_pack(__uint_as_float(vs[q] << 16), __uint_as_float(vs[q] & 0xffff0000u)), sum);
+    }
+    float lo, hi;
+    f2_unpack(sum, lo, hi);
+    const float dot = warp_sum(lo + hi);
+    if (lane == 0)
+      a.u[(int64_t)t * a.rank_cols + id * a.rank + j] = __float2bfloat16_rn(dot * a.scales[id]);
+  }
+  if (blockIdx.y != 0 || warp != 0) return;
+  // the word of all tokens, and 0 in its blocks' columns of other adapters
+  const uint64_t word =
+      warp_or64(adapter_bits(a, adapter_of(a, lane)) | adapter_bits(a, adapter_of(a, 32 + lane)));
+  if (t == 0 && lane == 0) a.mask64[0] = a.mask256[0] = word;
+  const int own0 = id * a.rank, own1 = id < 0 ? own0 : own0 + a.rank;
+  bf16* u = a.u + (int64_t)t * a.rank_cols;
+  for (uint64_t w = word; w; w &= w - 1) {
+    const int c0 = (__ffsll((long long)w) - 1) * kRankBlock;
+#pragma unroll
+    for (int c = c0 + lane; c < c0 + kRankBlock; c += 32)
+      if (c < a.rank_cols && (c < own0 || c >= own1)) u[c] = __float2bfloat16_rn(0.f);
   }
 }
 
@@ -757,8 +819,13 @@ int soup_multi_lora_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
   Args a = base_args(ids, ids_64, tokens_per_id, scales, tokens, adapters, rank, s, l);
   bf16* u = reinterpret_cast<bf16*>(s + l.u);
   cudaStream_t st = as_stream(stream);
-  if (int rc = rank_product(x, ldx, k, lora_a, false, a, u, true, st)) return rc;
   if (tokens <= kFewTokens) {
+    a.k = (int)k;
+    a.u = u;
+    if (int rc = cuda_status(launch_pdl(few_rank_kernel, dim3((unsigned)tokens, (a.rank + kFewWarps - 1) / kFewWarps),
+                                        dim3(32 * kFewWarps), 0, st, static_cast<const bf16*>(x), ldx,
+                                        static_cast<const bf16*>(lora_a), a)))
+      return rc;
     a.y = static_cast<bf16*>(y);
     a.ldy = ldy;
     a.bias = static_cast<const bf16*>(bias);
@@ -766,6 +833,7 @@ int soup_multi_lora_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
     if (tokens <= 32) return few_product<32>(x, ldx, weight, ldw, lora_b, n, k, u, a, st);
     return few_product<64>(x, ldx, weight, ldw, lora_b, n, k, u, a, st);
   }
+  if (int rc = rank_product(x, ldx, k, lora_a, false, a, u, true, st)) return rc;
   return gemm_bf16_masked_k2(x, ldx, weight, ldw, false, u, a.rank_cols, lora_b, a.rank_cols, a.rank_cols, a.mask256,
                              bias, y, ldy, tokens, n, k, st);
 }
