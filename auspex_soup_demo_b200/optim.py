@@ -15,6 +15,7 @@ import array
 import ctypes
 import itertools
 import math
+import operator
 from typing import Iterable, Optional
 
 import torch
@@ -25,6 +26,10 @@ from . import _lib
 STATE_BLOCK = 256
 
 
+_grad, _dtype = operator.attrgetter("grad"), operator.attrgetter("dtype")
+_data_ptr, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+
+
 def _address(a: array.array) -> int:
     return a.buffer_info()[0]
 
@@ -32,7 +37,7 @@ def _address(a: array.array) -> int:
 class _Held:
     """States and launch tables of one parameter group."""
 
-    __slots__ = ("params", "ptrs", "sizes", "blocks", "by_dtype", "m", "v", "m_scale", "v_scale")
+    __slots__ = ("params", "sizes", "by_dtype", "m", "v", "m_scale", "v_scale")
 
 
 class MultiTensorAdamW(torch.optim.Optimizer):
@@ -111,15 +116,14 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if total >= 1 << 31:
             raise ValueError("MultiTensorAdamW: a parameter group has at most 2^39 elements")
         held.params = list(params)
-        held.ptrs = [p.data_ptr for p in params]
         held.sizes = [p.numel() for p in params]
-        held.blocks = blocks
         by = {}
         for i, p in enumerate(params):
             if p.numel():
                 by.setdefault(p.dtype, []).append(i)
-        held.by_dtype = [(_lib.dtype_code(d), d, idx, array.array("q", [held.sizes[i] for i in idx]),
-                          array.array("i", [blocks[i] for i in idx])) for d, idx in by.items()]
+        held.by_dtype = [(_lib.dtype_code(d), d, [held.params[i] for i in idx],
+                          array.array("q", [held.sizes[i] for i in idx]), array.array("i", [blocks[i] for i in idx]))
+                         for d, idx in by.items()]
         eight = self.state_bits == 8
         dt = torch.float8_e4m3fn if eight else torch.float32
         held.m = torch.zeros(total, STATE_BLOCK, dtype=torch.uint8 if eight else dt, device=dev).view(dt)
@@ -186,25 +190,26 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         """(dtype code, parameter addresses, gradient addresses, sizes, blocks, gradients) of each
         type's parameters that have a gradient; the gradients are kept until the launch."""
         out = []
-        params, ptrs = held.params, held.ptrs
-        for code, dtype, idx, sizes, blocks in held.by_dtype:
-            grads = [params[i].grad for i in idx]
-            keep = [i for i, g in zip(idx, grads) if g is not None]
-            if len(keep) < len(idx):
+        for code, dtype, params, sizes, blocks in held.by_dtype:
+            # map over C methods: a step of hundreds of tensors is bound by these loops
+            grads = list(map(_grad, params))
+            try:
+                grad_ptrs = array.array("Q", map(_data_ptr, grads))
+            except TypeError:  # parameters without a gradient
+                keep = [i for i, g in enumerate(grads) if g is not None]
                 if not keep:
                     continue
-                idx = keep
-                grads = [g for g in grads if g is not None]
-                sizes = array.array("q", [held.sizes[i] for i in idx])
-                blocks = array.array("i", [held.blocks[i] for i in idx])
-            if not all([g.is_contiguous() for g in grads]):
+                params, grads = [params[i] for i in keep], [grads[i] for i in keep]
+                sizes, blocks = (array.array(t.typecode, [t[i] for i in keep]) for t in (sizes, blocks))
+                grad_ptrs = array.array("Q", map(_data_ptr, grads))
+            if not all(map(_is_contiguous, grads)):
                 if any(g.layout is not torch.strided for g in grads):
                     raise ValueError("MultiTensorAdamW: gradients must be dense")
                 grads = [g.detach().contiguous() for g in grads]
-            if {g.dtype for g in grads} != {dtype} or grads[0].device != device:
+                grad_ptrs = array.array("Q", map(_data_ptr, grads))
+            if set(map(_dtype, grads)) != {dtype} or grads[0].device != device:
                 raise ValueError(f"MultiTensorAdamW: gradients must be {dtype} on {device}, as their parameters")
-            out.append((code, array.array("Q", [ptrs[i]() for i in idx]),
-                        array.array("Q", [g.data_ptr() for g in grads]), sizes, blocks, grads))
+            out.append((code, array.array("Q", map(_data_ptr, params)), grad_ptrs, sizes, blocks, grads))
         return out
 
     def step(self, closure=None):
