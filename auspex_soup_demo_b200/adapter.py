@@ -47,25 +47,46 @@ def lora_modules(model) -> Dict[str, torch.nn.Module]:
     return out
 
 
-def adapter_state_dict(model) -> Dict[str, torch.Tensor]:
-    """PEFT-named LoRA tensors (CPU, contiguous, the parameters' dtype)."""
+def _factors(mod, index: Optional[int]):
+    """(A [r, in], B [out, r]) of a module; of adapter ``index`` where it holds several."""
+    if mod.lora_A.dim() == 2:
+        if index not in (None, 0):
+            raise IndexError(f"adapter {index} of a model with one adapter")
+        return mod.lora_A.detach(), mod.lora_B.detach()
+    n = mod.lora_A.shape[0]
+    if index is None:
+        raise ValueError(f"the model holds {n} adapters: say which (index)")
+    if not 0 <= index < n:
+        raise IndexError(f"adapter {index} of {n}")
+    return mod.lora_A.detach()[index], mod.lora_B.detach()[:, index]
+
+
+def _scaling(mod, index: Optional[int]) -> float:
+    return mod.alphas[index] / mod.lora_A.shape[1] if mod.lora_A.dim() == 3 else mod.scaling
+
+
+def adapter_state_dict(model, index: Optional[int] = None) -> Dict[str, torch.Tensor]:
+    """PEFT-named LoRA tensors (CPU, contiguous, the parameters' dtype); ``index``: which
+    adapter of a model with several."""
     sd = {}
     for path, mod in lora_modules(model).items():
-        sd[f"{_PREFIX}{path}.lora_A.weight"] = mod.lora_A.detach().to("cpu").contiguous()
-        sd[f"{_PREFIX}{path}.lora_B.weight"] = mod.lora_B.detach().to("cpu").contiguous()
+        a, b = _factors(mod, index)
+        sd[f"{_PREFIX}{path}.lora_A.weight"] = a.to("cpu").contiguous()
+        sd[f"{_PREFIX}{path}.lora_B.weight"] = b.to("cpu").contiguous()
     return sd
 
 
 def adapter_config(model, base_model_name_or_path: str, r: Optional[int] = None,
-                   lora_alpha: Optional[float] = None, lora_dropout: float = 0.0) -> dict:
+                   lora_alpha: Optional[float] = None, lora_dropout: float = 0.0,
+                   index: Optional[int] = None) -> dict:
     """The LoraConfig dictionary PEFT stores beside the weights."""
     mods = lora_modules(model)
     if not mods:
         raise ValueError("model has no LoRA-wrapped modules")
     first = next(iter(mods.values()))
-    r = int(r if r is not None else first.lora_A.shape[0])
+    r = int(r if r is not None else _factors(first, index)[0].shape[0])
     if lora_alpha is None:
-        lora_alpha = first.scaling * r
+        lora_alpha = _scaling(first, index) * r
     alpha = float(lora_alpha)
     if alpha.is_integer():
         alpha = int(alpha)
@@ -94,13 +115,14 @@ def adapter_config(model, base_model_name_or_path: str, r: Optional[int] = None,
 
 
 def save_adapter(model, directory: str, base_model_name_or_path: str = "Qwen/Qwen2.5-1.5B-Instruct",
-                 lora_dropout: float = 0.0) -> str:
-    """Write ``adapter_model.safetensors`` + ``adapter_config.json``; returns the directory."""
+                 lora_dropout: float = 0.0, index: Optional[int] = None) -> str:
+    """Write ``adapter_model.safetensors`` + ``adapter_config.json`` (of adapter ``index``
+    of a model with several); returns the directory."""
     from safetensors.torch import save_file
 
     os.makedirs(directory, exist_ok=True)
-    sd = adapter_state_dict(model)
-    cfg = adapter_config(model, base_model_name_or_path, lora_dropout=lora_dropout)
+    sd = adapter_state_dict(model, index)
+    cfg = adapter_config(model, base_model_name_or_path, lora_dropout=lora_dropout, index=index)
     save_file(sd, os.path.join(directory, ADAPTER_WEIGHTS), metadata={"format": "pt"})
     with open(os.path.join(directory, ADAPTER_CONFIG), "w", encoding="utf-8") as fh:
         json.dump(cfg, fh, indent=2, sort_keys=True)
@@ -108,8 +130,9 @@ def save_adapter(model, directory: str, base_model_name_or_path: str = "Qwen/Qwe
     return directory
 
 
-def load_adapter(model, directory: str, strict: bool = True) -> dict:
-    """Copy a PEFT LoRA adapter into the model's LoRA factors; returns its config.
+def load_adapter(model, directory: str, strict: bool = True, index: Optional[int] = None) -> dict:
+    """Copy a PEFT LoRA adapter into the model's LoRA factors (those of adapter ``index``
+    of a model with several); returns its config.
 
     Checks that r and lora_alpha match the wrapped modules (the scale is baked
     into each module) and, with ``strict``, that the file and the model hold
@@ -138,23 +161,23 @@ def load_adapter(model, directory: str, strict: bool = True) -> dict:
             if strict:
                 raise KeyError(f"adapter tensor for a module the model does not wrap: {key}")
             continue
-        param = mod.lora_A if which == "A" else mod.lora_B
+        param = _factors(mod, index)[0 if which == "A" else 1]
         if tuple(param.shape) != tuple(value.shape):
             raise ValueError(f"{key}: shape {tuple(value.shape)} vs model {tuple(param.shape)}")
-        with torch.no_grad():
-            param.copy_(value.to(device=param.device, dtype=param.dtype))
+        param.copy_(value.to(device=param.device, dtype=param.dtype))
         seen.add((path, which))
     if strict:
         missing = [f"{p}.lora_{w}" for p in mods for w in "AB" if (p, w) not in seen]
         if missing:
             raise KeyError(f"adapter lacks {len(missing)} LoRA tensors, e.g. {missing[:3]}")
     for path, mod in mods.items():
-        r = mod.lora_A.shape[0]
+        r = _factors(mod, index)[0].shape[0]
         if int(cfg.get("r", r)) != r:
             raise ValueError(f"adapter r={cfg.get('r')} but {path} has rank {r}")
-        alpha = float(cfg.get("lora_alpha", mod.scaling * r))
-        if abs(alpha / r - mod.scaling) > 1e-12 * max(1.0, abs(mod.scaling)):
-            raise ValueError(f"adapter scale {alpha}/{r} differs from {path}'s {mod.scaling}")
+        scaling = _scaling(mod, index)
+        alpha = float(cfg.get("lora_alpha", scaling * r))
+        if abs(alpha / r - scaling) > 1e-12 * max(1.0, abs(scaling)):
+            raise ValueError(f"adapter scale {alpha}/{r} differs from {path}'s {scaling}")
     return cfg
 
 

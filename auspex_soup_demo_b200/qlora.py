@@ -1051,12 +1051,20 @@ def qwen2_1p5b_config(num_layers: int = 28, attention: str = "sdpa", **overrides
 
 def build_qwen2_qlora(config=None, device="cuda", seed: int = 0, r: int = 16, alpha: int = 32,
                       targets: Iterable[str] = LORA_TARGETS, quantize: bool = True,
-                      dtype: torch.dtype = torch.bfloat16, group: bool = True):
+                      dtype: torch.dtype = torch.bfloat16, group: bool = True,
+                      adapters: Optional[int] = None, qk_norm: bool = False, train_norms: bool = False,
+                      rope_sections=None, rope_interleaved: bool = False):
     """Randomly initialised Qwen2 model with (NF4 +) LoRA on the target linears.
 
     quantize=False keeps dense frozen base weights (CPU runs and tests).
     group=True computes each layer's q/k/v and gate/up projections as one GEMM
     each on CUDA (LoRAProjectionGroup); parameters and names are unchanged.
+
+    adapters=n holds n adapters in every target linear (``multi_adapter``; alpha a
+    number or one for each); the batch's ids are set through ``model.adapter_ids`` or
+    the trainer's ``adapter_ids``. qk_norm, train_norms, rope_sections and
+    rope_interleaved: norms of queries and keys for each head and positions of several
+    axes (:func:`.heads.install_heads`). CUDA, bf16.
     """
     from transformers import Qwen2ForCausalLM
 
@@ -1066,6 +1074,16 @@ def build_qwen2_qlora(config=None, device="cuda", seed: int = 0, r: int = 16, al
         model = Qwen2ForCausalLM(cfg)
     model.to(dtype)
     wrap = LoRANF4Linear if quantize else LoRADenseLinear
+    if adapters is not None:
+        from .multi_adapter import AdapterIds, MultiLoRADenseLinear, MultiLoRANF4Linear
+
+        if adapters < 1:
+            raise ValueError(f"adapters must be at least 1, not {adapters}")
+        ids = model.adapter_ids = AdapterIds(adapters)
+        several = MultiLoRANF4Linear if quantize else MultiLoRADenseLinear
+
+        def wrap(lin, r, alpha):
+            return several(lin, ids, r, alpha)
     # LoRA factors get their own seed point, independent of how much of the
     # global RNG the model construction consumed; every rank starts from the
     # same adapters.
@@ -1079,7 +1097,11 @@ def build_qwen2_qlora(config=None, device="cuda", seed: int = 0, r: int = 16, al
                 lin = getattr(parent, name, None)
                 if isinstance(lin, torch.nn.Linear):
                     setattr(parent, name, wrap(lin, r, alpha))
-    if group:
+    if qk_norm or rope_sections is not None:
+        from .heads import install_heads
+
+        install_heads(model, qk_norm, rope_sections, rope_interleaved, train_norms)
+    if group and adapters is None:
         group_projections(model)
     if torch.cuda.is_available():
         torch.cuda.empty_cache()
@@ -1113,7 +1135,7 @@ class QLoRATrainer:
 
     def __init__(self, model, lr: float = 2e-4, chunk: int = 64, ddp: bool = False,
                  loss_fn=None, fused_adamw: Optional[bool] = None, weight_decay: float = 0.0,
-                 optimizer: str = "auto"):
+                 optimizer: str = "auto", max_grad_norm: Optional[float] = None):
         from .kernels import make_triton_chunked_loss_function
 
         self.model = model
@@ -1173,11 +1195,22 @@ class QLoRATrainer:
         on_cuda = self.params[0].is_cuda
         # AdamW (HF Trainer defaults: betas 0.9 / 0.999, eps 1e-8, weight decay 0).
         # "soup": one soup_adamw_flat launch over the flat buffers that also
-        # writes the 16-bit copies; "torch": torch.optim.AdamW; "auto": soup on CUDA.
-        if optimizer not in ("auto", "soup", "torch"):
-            raise ValueError(f"optimizer must be auto, soup or torch, not {optimizer!r}")
+        # writes the 16-bit copies; "soup8": optim.MultiTensorAdamW with 8-bit
+        # moments (2 bytes a parameter instead of 8); "torch": torch.optim.AdamW;
+        # "auto": soup on CUDA, soup8 when max_grad_norm is given.
+        if optimizer not in ("auto", "soup", "soup8", "torch"):
+            raise ValueError(f"optimizer must be auto, soup, soup8 or torch, not {optimizer!r}")
+        if optimizer == "auto" and on_cuda and max_grad_norm is not None:
+            optimizer = "soup8"
+        if max_grad_norm is not None and optimizer != "soup8":
+            raise ValueError("max_grad_norm needs optimizer='soup8' (on CUDA)")
         self.lr, self.betas, self.eps, self.weight_decay = lr, (0.9, 0.999), 1e-8, weight_decay
-        if optimizer == "soup" or (optimizer == "auto" and on_cuda):
+        if optimizer == "soup8":
+            from .optim import MultiTensorAdamW
+
+            self.opt = MultiTensorAdamW(self.params, lr=lr, betas=self.betas, eps=self.eps,
+                                        weight_decay=weight_decay, state_bits=8, max_grad_norm=max_grad_norm)
+        elif optimizer == "soup" or (optimizer == "auto" and on_cuda):
             if not on_cuda:
                 raise ValueError("optimizer='soup' needs CUDA parameters")
             self.exp_avg = torch.zeros_like(self.flat_param)
@@ -1206,7 +1239,14 @@ class QLoRATrainer:
             dist.all_reduce(self.flat_grad, op=dist.ReduceOp.SUM)
             self.flat_grad.mul_(1.0 / self.world)
 
-    def _hidden(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def _hidden(self, input_ids: torch.Tensor, adapter_ids=None, position_ids=None) -> torch.Tensor:
+        if adapter_ids is not None:
+            holder = getattr(self.model, "adapter_ids", None)
+            if holder is None:
+                raise ValueError("adapter_ids for a model without several adapters")
+            holder.set(adapter_ids)
+        if position_ids is not None and position_ids.dim() == 3 and self._no_mask is None:
+            raise ValueError("positions of several axes need layers of full attention")
         # Batches here are unpadded single sequences, so the attention mask is
         # exactly the causal pattern. Handing transformers a prepared "no mask"
         # keeps SDPA on is_causal with grouped K/V heads also while a CUDA graph
@@ -1214,22 +1254,27 @@ class QLoRATrainer:
         # stream capture and then materialises a [B, 1, S, S] mask, which makes
         # SDPA expand K/V to every query head and use a masked kernel (about 3x
         # slower on B200 at S=2048).
-        out = self.body(input_ids=input_ids, attention_mask=self._no_mask)
+        out = self.body(input_ids=input_ids, attention_mask=self._no_mask, position_ids=position_ids)
         return out.last_hidden_state if hasattr(out, "last_hidden_state") else out[0]
 
     def _begin_step(self):
         self.flat_grad.zero_()
         self._refresh_param16()  # the factors may have been changed outside the trainer
 
-    def step(self, input_ids: torch.Tensor, labels: torch.Tensor, denominator: float):
+    def step(self, input_ids: torch.Tensor, labels: torch.Tensor, denominator: float, adapter_ids=None,
+             position_ids=None):
+        """One step. adapter_ids [B] or [B, S]: the adapter of each sequence or token, for a
+        model with several; position_ids [B, S] or [axes, B, S] where positions are not
+        0, 1, 2, ... (these two also in the other steps)."""
         self._begin_step()
-        hidden = self._hidden(input_ids)
+        hidden = self._hidden(input_ids, adapter_ids, position_ids)
         loss, entropy, token_loss, correct = self.loss_fn.apply(
             hidden, self.model.lm_head, labels, self.chunk, denominator, -100, True)
         self._end_step(loss)
         return loss.detach(), correct
 
-    def token_logps(self, input_ids: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+    def token_logps(self, input_ids: torch.Tensor, labels: torch.Tensor, adapter_ids=None,
+                    position_ids=None) -> torch.Tensor:
         """Log-probabilities [B, S] of the labels (:func:`causal_labels` of the ids,
         unscored positions set to -100) without a gradient. Before the first step
         they are the base model's (LoRA's B starts at 0): the reference of
@@ -1238,28 +1283,30 @@ class QLoRATrainer:
 
         with torch.no_grad():
             self._refresh_param16()
-            return head_token_logps(self._hidden(input_ids), self.model.lm_head, labels)[0]
+            return head_token_logps(self._hidden(input_ids, adapter_ids, position_ids), self.model.lm_head,
+                                    labels)[0]
 
-    def preference_step(self, input_ids: torch.Tensor, labels: torch.Tensor, ref_logps, **options):
+    def preference_step(self, input_ids: torch.Tensor, labels: torch.Tensor, ref_logps, adapter_ids=None,
+                        position_ids=None, **options):
         """One step on P preference pairs: ids and labels [2P, S], chosen answers
         first; options as in :func:`kernels.preference_loss`. Returns (loss, chosen
         rewards, rejected rewards)."""
         from .kernels import head_token_logps, preference_loss
 
         self._begin_step()
-        logps, _ = head_token_logps(self._hidden(input_ids), self.model.lm_head, labels)
+        logps, _ = head_token_logps(self._hidden(input_ids, adapter_ids, position_ids), self.model.lm_head, labels)
         loss, chosen, rejected = preference_loss(logps, ref_logps, labels, **options)
         self._end_step(loss)
         return loss.detach(), chosen, rejected
 
     def policy_step(self, input_ids: torch.Tensor, labels: torch.Tensor, advantages: torch.Tensor,
-                    **options):
+                    adapter_ids=None, position_ids=None, **options):
         """One step on sampled answers with advantages [B] or [B, S]; options as in
         :func:`kernels.policy_loss`. Returns (loss, mean KL, clipped share)."""
         from .kernels import head_token_logps, policy_loss
 
         self._begin_step()
-        logps, _ = head_token_logps(self._hidden(input_ids), self.model.lm_head, labels)
+        logps, _ = head_token_logps(self._hidden(input_ids, adapter_ids, position_ids), self.model.lm_head, labels)
         loss, kl, clipped = policy_loss(logps, advantages, labels, **options)
         self._end_step(loss)
         return loss.detach(), kl, clipped
@@ -1388,36 +1435,41 @@ class QLoRATrainer:
                 dst.copy_(src)
 
     def capture(self, input_ids: torch.Tensor, labels: torch.Tensor, denominator: float,
-                warmup: int = 3):
+                warmup: int = 3, adapter_ids=None, position_ids=None):
         """Record one step on static `input_ids`/`labels` buffers as a CUDA graph.
 
-        Later batches are copied into the same buffers before :meth:`replay`.
+        Later batches are copied into the same buffers (adapter and position ids too)
+        before :meth:`replay`.
         `denominator` is baked into the graph (the count of non-ignored labels
         is the same for every batch of fixed shape without padding).
         """
         self.static_ids = input_ids
         self.static_labels = labels
+        self.static_adapter_ids, self.static_position_ids = adapter_ids, position_ids
         side = torch.cuda.Stream(input_ids.device)
         side.wait_stream(torch.cuda.current_stream(input_ids.device))
         with torch.cuda.stream(side):
             for _ in range(warmup):
-                self.step(input_ids, labels, denominator)
+                self.step(input_ids, labels, denominator, adapter_ids, position_ids)
         torch.cuda.current_stream(input_ids.device).wait_stream(side)
         torch.cuda.synchronize(input_ids.device)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
-            self.static_loss, self.static_correct = self.step(input_ids, labels, denominator)
+            self.static_loss, self.static_correct = self.step(input_ids, labels, denominator, adapter_ids,
+                                                              position_ids)
         return self.static_loss
 
     def replay(self):
         self.graph.replay()
         return self.static_loss, self.static_correct
 
-    def save_adapter(self, directory: str, base_model_name_or_path: str = "Qwen/Qwen2.5-1.5B-Instruct"):
-        """Write the LoRA factors as a PEFT adapter directory (see ``adapter.save_adapter``)."""
+    def save_adapter(self, directory: str, base_model_name_or_path: str = "Qwen/Qwen2.5-1.5B-Instruct",
+                     index: Optional[int] = None):
+        """Write the LoRA factors as a PEFT adapter directory (see ``adapter.save_adapter``;
+        index: which adapter of a model with several)."""
         from .adapter import save_adapter
 
-        return save_adapter(self.model, directory, base_model_name_or_path)
+        return save_adapter(self.model, directory, base_model_name_or_path, index=index)
 
     def release_graph(self):
         """Drop the captured graph (do this before destroying the process group)."""
