@@ -816,12 +816,12 @@ static int m_tiles(int64_t m) { return static_cast<int>((m + tile_m() - 1) / til
 
 constexpr int kPairStages = 6;
 
-template <bool A_MN, bool B_MN, class Epi>
+template <bool A_MN, bool B_MN, class Epi, bool K2MASK = false>
 static int launch_gemm_single(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& ma2,
                               const CUtensorMap& mb2, const CUtensorMap& mc, Sched sched,
                               const typename Epi::Params& ep, cudaStream_t stream, int* err) {
   using L = SmemLayout<kBN, kStages, kEpiWarps>;
-  auto kern = gemm_kernel<kBN, kStages, A_MN, B_MN, Epi, kEpiWarps>;
+  auto kern = gemm_kernel<kBN, kStages, A_MN, B_MN, Epi, kEpiWarps, K2MASK>;
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -901,13 +901,13 @@ static int plan_stream_k(Sched& sched, int max_cl, int dev) {
   return tiles > max_cl ? max_cl : (int)skc;
 }
 
-template <bool A_MN, bool B_MN, class Epi>
+template <bool A_MN, bool B_MN, class Epi, bool K2MASK = false>
 static int launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& ma2,
                             const CUtensorMap& mb2, const CUtensorMap& mc, Sched sched,
                             const typename Epi::Params& ep, cudaStream_t stream, int* err) {
   using L = SmemLayout<kBN / 2, kPairStages, kEpiWarps>;
   static_assert(L::kBytes <= 232448, "pair GEMM shared memory exceeds 227 KB");
-  auto kern = gemm_pair_kernel<kBN, kPairStages, A_MN, B_MN, Epi, kEpiWarps>;
+  auto kern = gemm_pair_kernel<kBN, kPairStages, A_MN, B_MN, Epi, kEpiWarps, K2MASK>;
   static int max_clusters[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -958,7 +958,7 @@ static int launch_gemm_pair(const CUtensorMap& ma, const CUtensorMap& mb, const 
 // sched.m_tiles counts tile_m() rows. ma2 / mb2 are read for the last
 // sched.kb2 k-blocks (the second K segment); mc is the output map of an
 // epilogue that stores through TMA (any valid map otherwise).
-template <bool A_MN, bool B_MN, class Epi>
+template <bool A_MN, bool B_MN, class Epi, bool K2MASK = false>
 static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& ma2,
                        const CUtensorMap& mb2, const CUtensorMap& mc, Sched sched,
                        const typename Epi::Params& ep, cudaStream_t stream) {
@@ -971,8 +971,8 @@ static int launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const CUten
   }
   if (sched.wait_ns == 0) sched.wait_ns = wait_limit_ns();
   if (use_pairs())
-    return launch_gemm_pair<A_MN, B_MN, Epi>(ma, mb, ma2, mb2, mc, sched, ep, stream, err);
-  return launch_gemm_single<A_MN, B_MN, Epi>(ma, mb, ma2, mb2, mc, sched, ep, stream, err);
+    return launch_gemm_pair<A_MN, B_MN, Epi, K2MASK>(ma, mb, ma2, mb2, mc, sched, ep, stream, err);
+  return launch_gemm_single<A_MN, B_MN, Epi, K2MASK>(ma, mb, ma2, mb2, mc, sched, ep, stream, err);
 }
 
 // One K segment (sched.kb2 must be 0).
@@ -1908,11 +1908,13 @@ static int gemm_bf16_run(const void* a, int64_t lda, int a_mn_major, const void*
   const int mt = m_tiles(m), nt = (int)((n + kBN - 1) / kBN);
   const int kb1 = (int)((k + BK - 1) / BK), kb2 = (int)((r + BK - 1) / BK);
   Sched sc{mt, nt, 1, kb1 + kb2, nt > mt ? 0 : 1, kb2};
-  if (k2_mask) {
+  using E = EpiStore<kBN>;
+  if (k2_mask) {  // a is K-major
     sc.k2_mask = k2_mask;
     sc.no_sk = 1;
+    return b_mn_major ? launch_gemm<false, true, E, true>(ma, mb, ma2, mb2, mc, sc, ep, stream)
+                      : launch_gemm<false, false, E, true>(ma, mb, ma2, mb2, mc, sc, ep, stream);
   }
-  using E = EpiStore<kBN>;
   if (!a_mn_major && !b_mn_major) return launch_gemm<false, false, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
   if (!a_mn_major && b_mn_major) return launch_gemm<false, true, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);
   if (a_mn_major && !b_mn_major) return launch_gemm<true, false, E>(ma, mb, ma2, mb2, mc, sc, ep, stream);

@@ -287,18 +287,15 @@ struct Sched {
   const int* dyn_rows = nullptr;
   int dyn_k = 0;
   int dyn_unit = 1;
-  // optional words of 256-row tiles of A (written by an earlier kernel on the
-  // stream): a tile's second segment then is the blocks of its set bits, in
-  // ascending order, instead of all kb2 (at most 64). With splits == 1 and no
-  // stream-K tail.
+  // kernels with K2MASK alone: words of 256-row tiles of A (written by an earlier kernel
+  // on the stream); a tile's second segment then is the blocks of its set bits, in
+  // ascending order, instead of all kb2 (at most 64). With splits == 1 and no stream-K
+  // tail. A template parameter, since the branches cost the other GEMMs 4 % of their time.
   const uint64_t* k2_mask = nullptr;
-  __device__ __forceinline__ uint64_t k2_word(int mt256) const { return k2_mask ? k2_mask[mt256] : 0; }
-  __device__ __forceinline__ int k_end(int kb1, uint64_t word) const {
-    return k2_mask ? kb_total - kb2 + __popcll(word) : kb1;
-  }
-  // k offset of block kb of a tile; `word` holds the tile's rank blocks still to come
-  __device__ __forceinline__ int k_elem_of(int kb, uint64_t& word) const {
-    if (!k2_mask || !second(kb)) return k_elem(kb);
+  __device__ __forceinline__ int k2_end(uint64_t word) const { return kb_total - kb2 + __popcll(word); }
+  // k offset of block kb of a tile; `word` holds the tile's blocks still to come
+  __device__ __forceinline__ int k2_elem(int kb, uint64_t& word) const {
+    if (!second(kb)) return k_elem(kb);
     const int b = __ffsll(static_cast<long long>(word)) - 1;
     word &= word - 1;
     return b * BK;
@@ -510,7 +507,7 @@ __device__ __forceinline__ bool bounded_wait(uint32_t bar, uint32_t parity,
 //                               int lane, uint32_t tmem_acc /* lane base applied */,
 //                               uint8_t* stage /* this warp's kEpiWarpBytes of smem */,
 //                               int group, int ngroups /* column part of the tile */);
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS, bool K2MASK = false>
 __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
                 const __grid_constant__ CUtensorMap tma_a2,
@@ -593,8 +590,11 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
         int mt, nt, ks, kb0, kb1;
         sched.decode(u, mt, nt, ks);
         sched.k_range(ks, kb0, kb1);
-        uint64_t word = sched.k2_word(mt >> 1);
-        kb1 = sched.k_end(kb1, word);
+        uint64_t word = 0;
+        if constexpr (K2MASK) {
+          word = sched.k2_mask[mt >> 1];
+          kb1 = sched.k2_end(word);
+        }
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1u;
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
           const uint32_t a_dst = sbase + s * L::kStageBytes;
           const uint32_t b_dst = a_dst + L::kABytes;
           mbar_arrive_expect_tx(full_bar(s), L::kStageBytes);
-          const int k0 = sched.k_elem_of(kb, word);
+          const int k0 = K2MASK ? sched.k2_elem(kb, word) : sched.k_elem(kb);
           const bool seg2 = sched.second(kb);
           const CUtensorMap* ma = seg2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mb = seg2 ? &tma_b2 : &tma_b;
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
         int mt, nt, ks, kb0, kb1;
         sched.decode(u, mt, nt, ks);
         sched.k_range(ks, kb0, kb1);
-        kb1 = sched.k_end(kb1, sched.k2_word(mt >> 1));
+        if constexpr (K2MASK) kb1 = sched.k2_end(sched.k2_mask[mt >> 1]);
         const uint32_t acc = lt & 1u;
         const uint32_t acc_ph = (lt >> 1) & 1u;
         if (!bounded_wait(tempty_bar(acc), acc_ph ^ 1u, abort_flag, err, kErrWaitMma, wait_ns)) {
@@ -930,7 +930,7 @@ __device__ __forceinline__ bool sk_fix(const Sched& s, const Unit& w, uint32_t r
 // Sched for this kernel counts m tiles of 2 x BM rows; the grid is
 // 2 x (number of clusters) with cluster dimension (2, 1, 1). With
 // sched.sk_tiles > 0 the tail tiles run as stream-K parts (see Sched).
-template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS>
+template <int BN, int STAGES, bool A_MN, bool B_MN, class Epi, int EPI_WARPS, bool K2MASK = false>
 __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tma_a,
                      const __grid_constant__ CUtensorMap tma_b,
@@ -1022,8 +1022,12 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
         const Unit w = sched_unit(sched, cluster, n_clusters, i);
         const int a_row = w.mt * 2 * BM + static_cast<int>(rank) * BM;
         const int b_row = w.nt * BN + static_cast<int>(rank) * BNH;
-        uint64_t word = sched.k2_word(w.mt);
-        const int kb1 = sched.k_end(w.kb1, word);
+        uint64_t word = 0;
+        int kb1 = w.kb1;
+        if constexpr (K2MASK) {
+          word = sched.k2_mask[w.mt];
+          kb1 = sched.k2_end(word);
+        }
         for (int kb = w.kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1u;
@@ -1036,7 +1040,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
           const uint32_t b_dst = a_dst + L::kABytes;
           const uint32_t fb = cluster_addr(full_bar(s), 0);
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), kPairBytes);
-          const int k0 = sched.k_elem_of(kb, word);
+          const int k0 = K2MASK ? sched.k2_elem(kb, word) : sched.k_elem(kb);
           const bool seg2 = sched.second(kb);
           const CUtensorMap* ma = seg2 ? &tma_a2 : &tma_a;
           const CUtensorMap* mb = seg2 ? &tma_b2 : &tma_b;
@@ -1077,7 +1081,9 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS), 1)
       bool issued = false;
       for (int i = 0; i < n_my && ok; ++i, ++lt) {
         const Unit w = sched_unit(sched, cluster, n_clusters, i);
-        const int kb0 = w.kb0, kb1 = sched.k_end(w.kb1, sched.k2_word(w.mt));
+        const int kb0 = w.kb0;
+        int kb1 = w.kb1;
+        if constexpr (K2MASK) kb1 = sched.k2_end(sched.k2_mask[w.mt]);
         const uint32_t acc = lt & 1u;
         const uint32_t acc_ph = (lt >> 1) & 1u;
         if (!bounded_wait<true>(tempty_bar(acc), acc_ph ^ 1u, abort_flag, err, kErrWaitMma, wait_ns)) {
