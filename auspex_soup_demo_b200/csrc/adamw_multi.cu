@@ -253,9 +253,9 @@ __global__ void __launch_bounds__(kThreads) grad_square_kernel(const __grid_cons
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double sum = 0.0;
-  int ti = 0;
   constexpr int U = 4;  // blocks of a warp in flight
   for (int c = blockIdx.x * U * kWarps + warp; c < tab.blocks; c += gridDim.x * U * kWarps) {
+    int ti = find_tensor(tab, c);  // (a turn may pass over hundreds of small tensors)
     Raw8<T> g[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {

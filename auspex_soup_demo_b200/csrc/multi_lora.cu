@@ -22,9 +22,9 @@
 // (M 128, N 64), the k range split over a cluster whose CTAs add their partial tiles
 // in rank order through distributed shared memory (bitwise reproducible).
 //
-// Few tokens (T <= 64: next tokens of many requests): the base product is W's bytes.
+// Few tokens (next tokens of many requests): the base product is W's bytes.
 // The same kernel then streams W as the 128-row operand against all tokens at once
-// (N = T rounded up), so that every SM takes part, with U and B's blocks behind; it starts
+// (N = T rounded up, at most 128 a CTA), so that every SM takes part, with U and B's blocks behind; it starts
 // beside the kernel that forms U and waits for that one only before its rank blocks.
 //
 // u and v are rounded to bf16 between the two products, as x, dy and the factors are.
@@ -54,11 +54,11 @@ namespace {
 using bf16 = __nv_bfloat16;
 using namespace tc;
 
-constexpr int kStages = 4;
 constexpr int kThreads = 192;
 constexpr int kRankBlock = 64;     // rank columns of a block
 constexpr int kMaxRank = 4096;     // adapters x rank: one bit per block in 64 bits
-constexpr int kFewTokens = 64;
+constexpr int kFewTokens = 256;    // at most, of kModeFew: one word of rank blocks
+constexpr int kFewTile = 128;      // of them in a CTA's columns
 constexpr int kMaxTokens = 1 << 21;
 constexpr int kErrProducer = 0x141;
 constexpr int kErrMma = 0x142;
@@ -72,11 +72,15 @@ constexpr int kModeFew = 2;   // y of few tokens: rows are features, columns tok
 
 template <int NP>
 struct Smem {
+  // two CTAs an SM
+  static constexpr int kStages = NP > 64 ? 3 : 4;
   static constexpr int kABytes = 128 * 64 * 2;
   static constexpr int kBBytes = NP * 64 * 2;
   static constexpr int kStage = kABytes + kBBytes;
-  static constexpr int kPartStride = NP + 4;
-  static_assert(128 * kPartStride * 4 <= kStages * kStage, "the partial tile reuses the stages");
+  static constexpr int kPartStride = NP + 4;  // [row][column]
+  static constexpr int kPartStrideT = 132;    // [column][row]
+  static_assert(128 * kPartStride * 4 <= kStages * kStage && NP * kPartStrideT * 4 <= kStages * kStage,
+                "the partial tile reuses the stages");
   static constexpr int kBar = kStages * kStage;
   static constexpr int kNumBars = 2 * kStages + 1;  // full[S], empty[S], acc_full
   static constexpr int kMisc = kBar + kNumBars * 8;  // tmem, abort, words[8]
@@ -118,8 +122,7 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
   return v;
 }
 // 32 lanes x 16 consecutive fp32 columns (no wait; tcgen05.wait::ld follows).
@@ -134,6 +137,15 @@ __device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, float* v) {
       : "r"(taddr));
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ uint2 pack_bf16x4(float4 f) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(f.x, f.y), hi = __floats2bfloat162_rn(f.z, f.w);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+__device__ __forceinline__ void store_grad(const Args& a, int64_t at, float4 f) {
+  if (a.grad_f32) *reinterpret_cast<float4*>(static_cast<float*>(a.grad) + at) = f;
+  else *reinterpret_cast<uint2*>(static_cast<bf16*>(a.grad) + at) = pack_bf16x4(f);
 }
 
 // Adapter of token t: -1 for none, for an id outside [0, adapters) and behind the last token.
@@ -220,7 +232,8 @@ struct KWalk {
   }
 };
 
-// Grid: (tiles of 128 rows) x ks, rank blocks (kModeRank, kModeGrad) or 1; clusters of ks.
+// Grid: (tiles of 128 rows) x ks, rank blocks (kModeRank, kModeGrad) or token tiles
+// (kModeFew); clusters of ks.
 // A K-major: map {k, rows}, box {64, 128}; MN-major (kModeGrad): map {rows, k}, box {64, 64}.
 // B K-major: map {k, columns}, box {64, NP}; MN-major: map {columns, k}, box {64, 64}.
 template <int MODE, bool B_MN, int NP>
@@ -230,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                      const Args a, int* err) {
   using L = Smem<NP>;
   constexpr bool A_MN = MODE == kModeGrad;
-  constexpr uint32_t kCols = NP <= 32 ? 32 : 64;
+  constexpr uint32_t kCols = NP <= 32 ? 32 : NP;
   constexpr uint32_t kIdesc = idesc_bf16(NP, A_MN, B_MN, 128);
   static_assert(!B_MN || NP == 64, "an MN-major factor is read 64 columns at a time");
   extern __shared__ uint8_t smem_raw[];
@@ -245,8 +258,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t sbase = smem_u32(smem);
   const uint32_t bar0 = sbase + L::kBar;
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
-  auto empty_bar = [&](int s) { return bar0 + 8u * (kStages + s); };
-  const uint32_t acc_bar = bar0 + 8u * (2 * kStages);
+  auto empty_bar = [&](int s) { return bar0 + 8u * (L::kStages + s); };
+  const uint32_t acc_bar = bar0 + 8u * (2 * L::kStages);
   float* part = reinterpret_cast<float*>(smem);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
@@ -334,6 +347,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     return k;
   };
 
+  // The result's rows follow one another in memory (else its columns do): the partial tile
+  // is kept in that order too, for whole sectors between peers and wide stores. With lanes
+  // a row apart a cluster of 6 took 9 us to add up 128 x 128, a third of it now.
+  const bool by_column = MODE == kModeFew || (MODE == kModeGrad && a.grad_trans);
   bool any = false;  // epilogue: this CTA has a partial tile
   if (warp == 0) {
     if (lane == 0) {
@@ -342,8 +359,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       int it = 0, kb;
       bool second;
       while (k.next(kb, second)) {
-        const int s = it % kStages;
-        const uint32_t ph = (it / kStages) & 1u;
+        const int s = it % L::kStages;
+        const uint32_t ph = (it / L::kStages) & 1u;
         if (!bounded_wait(empty_bar(s), ph ^ 1u, abort_flag, err, kErrProducer, wait_ns)) break;
         const uint32_t a_dst = sbase + s * L::kStage;
         const uint32_t b_dst = a_dst + L::kABytes;
@@ -356,17 +373,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         } else {
           tma_load_2d(a_dst, ma, full_bar(s), kb * 64, mt * 128);
         }
-        const int col0 = MODE == kModeFew ? 0 : rb * kRankBlock;
+        const int col0 = rb * (MODE == kModeFew ? kFewTile : kRankBlock);
         if (B_MN) tma_load_2d(b_dst, mb, full_bar(s), col0, kb * 64);
         else tma_load_2d(b_dst, mb, full_bar(s), kb * 64, col0);
         ++it;
       }
       // let the copies still in flight land before the CTA may leave (bounded)
-      const int n_wait = it < kStages ? it : kStages;
+      const int n_wait = it < L::kStages ? it : L::kStages;
       for (int i = 1; i <= n_wait; ++i) {
         const int j = it - i;
         const uint64_t t0 = globaltimer();
-        while (!mbar_try_wait(full_bar(j % kStages), (j / kStages) & 1u) && globaltimer() - t0 < wait_ns) {
+        while (!mbar_try_wait(full_bar(j % L::kStages), (j / L::kStages) & 1u) && globaltimer() - t0 < wait_ns) {
         }
       }
     }
@@ -377,8 +394,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       int it = 0, kb;
       bool second;
       while (k.next(kb, second)) {
-        const int s = it % kStages;
-        const uint32_t ph = (it / kStages) & 1u;
+        const int s = it % L::kStages;
+        const uint32_t ph = (it / L::kStages) & 1u;
         if (!bounded_wait(full_bar(s), ph, abort_flag, err, kErrMma, wait_ns)) break;
         tc_fence_after();
         const uint32_t a_addr = sbase + s * L::kStage;
@@ -434,10 +451,15 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int c = 0; c < NP; ++c) v[c] = 0.f;
     }
-    float* prow = part + row * L::kPartStride;
+    if (by_column) {
 #pragma unroll
-    for (int c = 0; c < NP; c += 4)
-      *reinterpret_cast<float4*>(prow + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+      for (int c = 0; c < NP; ++c) part[c * L::kPartStrideT + row] = v[c];
+    } else {
+      float* prow = part + row * L::kPartStride;
+#pragma unroll
+      for (int c = 0; c < NP; c += 4)
+        *reinterpret_cast<float4*>(prow + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+    }
   }
 
   // every thread of every CTA of the cluster: the partial tiles are complete
@@ -445,71 +467,84 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (ks > 1) cluster_sync_all();
   else __syncthreads();
 
-  if (warp >= 2 && !*abort_flag) {
-    const int t = threadIdx.x - 64;
-    const int r0 = 128 * rank / ks, rs = 128 * (rank + 1) / ks - r0;  // rows this CTA reduces and writes
-    const int items = rs * (NP / 4);
+  if (!*abort_flag) {
     const uint32_t part_addr = smem_u32(part);
-    for (int item = t; item < items; item += 128) {
-      // consecutive threads: rows of one column group where columns are far apart in
-      // memory (kModeFew, transposed gradients), else column groups of one row
-      const bool by_row = MODE == kModeFew || (MODE == kModeGrad && a.grad_trans);
-      const int rl = by_row ? item % rs : item / (NP / 4);
-      const int cg = by_row ? item / rs : item % (NP / 4);
-      const int r = r0 + rl, col = cg * 4;
-      const uint32_t off = static_cast<uint32_t>((r * L::kPartStride + col) * 4);
+    uint32_t peer[16];
+    if (ks > 1) {
+#pragma unroll
+      for (int p = 0; p < 16; ++p) peer[p] = p < ks ? cluster_addr(part_addr, p) : 0u;
+    }
+    // partials in rank order, eight of them in flight
+    auto reduce = [&](int off) {
+      if (ks == 1) return *reinterpret_cast<const float4*>(part + off);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int p0 = 0; p0 < ks; p0 += 8) {
+#pragma unroll
+      for (int p = 0; p < 16; p += 8) {
+        if (p >= ks) break;
         float4 q[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int p = p0 + u;
-          q[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (p < ks)
-            q[u] = (p == rank) ? *reinterpret_cast<const float4*>(part + r * L::kPartStride + col)
-                               : ld_cluster_f4(cluster_addr(part_addr + off, p));
-        }
+        for (int u = 0; u < 8; ++u)
+          if (p + u < ks) q[u] = ld_cluster_f4(peer[p + u] + off * 4);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (p0 + u < ks) {
+        for (int u = 0; u < 8; ++u)
+          if (p + u < ks) {
             sum.x += q[u].x;
             sum.y += q[u].y;
             sum.z += q[u].z;
             sum.w += q[u].w;
           }
-        }
       }
-      const int row = mt * 128 + r;
-      if (row >= a.rows) continue;
-      const float f[4] = {sum.x, sum.y, sum.z, sum.w};
-      if constexpr (MODE == kModeRank) {
-        const int c0 = rb * kRankBlock + col;
-        if (c0 >= a.rank_cols) continue;  // rank_cols is a multiple of 8
-        const int id = adapter_of(a, row);
-        const float sc = id < 0 ? 0.f : a.scales[id];
-        const int lo = id * a.rank, hi = lo + a.rank;
-        float g[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) g[j] = id >= 0 && c0 + j >= lo && c0 + j < hi ? f[j] * sc : 0.f;
-        const __nv_bfloat162 p01 = __floats2bfloat162_rn(g[0], g[1]), p23 = __floats2bfloat162_rn(g[2], g[3]);
-        uint2 o;
-        o.x = *reinterpret_cast<const uint32_t*>(&p01);
-        o.y = *reinterpret_cast<const uint32_t*>(&p23);
-        *reinterpret_cast<uint2*>(a.u + (int64_t)row * a.rank_cols + c0) = o;
-      } else if constexpr (MODE == kModeGrad) {
-        const int c0 = rb * kRankBlock + col;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (c0 + j >= a.rank_cols) break;
-          const int64_t at = a.grad_trans ? (int64_t)(c0 + j) * a.rows + row : (int64_t)row * a.rank_cols + c0 + j;
-          if (a.grad_f32) static_cast<float*>(a.grad)[at] = f[j];
-          else static_cast<bf16*>(a.grad)[at] = __float2bfloat16_rn(f[j]);
+      return sum;
+    };
+    if (by_column) {
+      // this CTA adds up and writes its share of the columns, a warp one at a time, a lane
+      // four rows (rows are a multiple of 8)
+      const int r = lane * 4, row = mt * 128 + r;
+      const int col0 = rb * (MODE == kModeFew ? kFewTile : kRankBlock);
+      const int cols = min(NP, (MODE == kModeFew ? a.tokens : a.rank_cols) - col0);
+      const int end = row < a.rows ? cols * (rank + 1) / ks : 0;
+      int col = cols * rank / ks + warp;
+      if constexpr (MODE == kModeFew) {
+        float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (a.bias && col < end)
+          b = make_float4(__bfloat162float(a.bias[row]), __bfloat162float(a.bias[row + 1]),
+                          __bfloat162float(a.bias[row + 2]), __bfloat162float(a.bias[row + 3]));
+#pragma unroll 2
+        for (; col < end; col += kThreads / 32) {
+          const float4 f = reduce(col * L::kPartStrideT + r);
+          *reinterpret_cast<uint2*>(a.y + (int64_t)(col0 + col) * a.ldy + row) =
+              pack_bf16x4(make_float4(f.x + b.x, f.y + b.y, f.z + b.z, f.w + b.w));
         }
       } else {
-        const float b = a.bias ? __bfloat162float(a.bias[row]) : 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < a.tokens) a.y[(int64_t)(col + j) * a.ldy + row] = __float2bfloat16_rn(f[j] + b);
+#pragma unroll 2
+        for (; col < end; col += kThreads / 32)
+          store_grad(a, (int64_t)(col0 + col) * a.rows + row, reduce(col * L::kPartStrideT + r));
+      }
+    } else {
+      // its share of the rows, a thread four columns of every (kThreads / G)-th
+      // (rank_cols is a multiple of 8)
+      const int r0 = 128 * rank / ks, rs = 128 * (rank + 1) / ks - r0;
+      constexpr int G = NP / 4;
+      const int col = (int)threadIdx.x % G * 4, c0 = rb * kRankBlock + col;
+      const int rows = c0 < a.rank_cols ? min(rs, a.rows - mt * 128 - r0) : 0;
+#pragma unroll 2
+      for (int i = (int)threadIdx.x / G; i < rows; i += kThreads / G) {
+        const int r = r0 + i, row = mt * 128 + r;
+        float4 f = reduce(r * L::kPartStride + col);
+        const int64_t at = (int64_t)row * a.rank_cols + c0;
+        if constexpr (MODE == kModeRank) {
+          // 0 outside the token's adapter, whatever the product of the others' columns is
+          const int id = adapter_of(a, row);
+          const float sc = id < 0 ? 0.f : a.scales[id];
+          const int lo = id * a.rank, hi = id < 0 ? lo : lo + a.rank;
+          f.x = c0 >= lo && c0 < hi ? f.x * sc : 0.f;
+          f.y = c0 + 1 >= lo && c0 + 1 < hi ? f.y * sc : 0.f;
+          f.z = c0 + 2 >= lo && c0 + 2 < hi ? f.z * sc : 0.f;
+          f.w = c0 + 3 >= lo && c0 + 3 < hi ? f.w * sc : 0.f;
+          *reinterpret_cast<uint2*>(a.u + at) = pack_bf16x4(f);
+        } else {
+          store_grad(a, at, f);
+        }
       }
     }
   }
@@ -556,9 +591,14 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rank_kernel(const bf16* __
   }
   if (blockIdx.y != 0 || warp != 0) return;
   // the word of all tokens, and 0 in its blocks' columns of other adapters
-  const uint64_t word =
-      warp_or64(adapter_bits(a, adapter_of(a, lane)) | adapter_bits(a, adapter_of(a, 32 + lane)));
-  if (t == 0 && lane == 0) a.mask64[0] = a.mask256[0] = word;
+  uint64_t word = 0;
+  for (int b = 0; b * 64 < a.tokens; ++b) {
+    const uint64_t w = warp_or64(adapter_bits(a, adapter_of(a, b * 64 + lane)) |
+                                 adapter_bits(a, adapter_of(a, b * 64 + 32 + lane)));
+    if (t == 0 && lane == 0) a.mask64[b] = w;
+    word |= w;
+  }
+  if (t == 0 && lane == 0) a.mask256[0] = word;
   const int own0 = id * a.rank, own1 = id < 0 ? own0 : own0 + a.rank;
   bf16* u = a.u + (int64_t)t * a.rank_cols;
   for (uint64_t w = word; w; w &= w - 1) {
@@ -763,7 +803,9 @@ int few_product(const void* x, int64_t ldx, const void* w, int64_t ldw, const vo
   if ((rc = map2d(&mb, x, k, a.tokens, ldx, NP))) return rc;
   if ((rc = map2d(&ma2, lora_b, a.rank_cols, n, a.rank_cols, 128))) return rc;
   if ((rc = map2d(&mb2, u, a.rank_cols, a.tokens, a.rank_cols, NP))) return rc;
-  return launch<kModeFew, false, NP>(ma, mb, ma2, mb2, a, a.kb_total, 1, (a.rows + 127) / 128, st);
+  const int token_tiles = (a.tokens + kFewTile - 1) / kFewTile;
+  return launch<kModeFew, false, NP>(ma, mb, ma2, mb2, a, a.kb_total, token_tiles, (a.rows + 127) / 128 * token_tiles,
+                                     st);
 }
 
 Args base_args(const void* ids, int ids_64, int64_t per, const float* scales, int64_t tokens, int64_t adapters,
@@ -819,7 +861,9 @@ int soup_multi_lora_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
   Args a = base_args(ids, ids_64, tokens_per_id, scales, tokens, adapters, rank, s, l);
   bf16* u = reinterpret_cast<bf16*>(s + l.u);
   cudaStream_t st = as_stream(stream);
-  if (tokens <= kFewTokens) {
+  // up to 128 tokens always; up to 256 where the 256-row tiles of the pair GEMM would
+  // leave more than half of the SMs idle
+  if (tokens <= kFewTile || (tokens <= kFewTokens && (n + 255) / 256 * 4 < num_sms())) {
     a.k = (int)k;
     a.u = u;
     if (int rc = cuda_status(launch_pdl(few_rank_kernel, dim3((unsigned)tokens, (a.rank + kFewWarps - 1) / kFewWarps),
@@ -831,7 +875,8 @@ int soup_multi_lora_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
     a.bias = static_cast<const bf16*>(bias);
     if (tokens <= 16) return few_product<16>(x, ldx, weight, ldw, lora_b, n, k, u, a, st);
     if (tokens <= 32) return few_product<32>(x, ldx, weight, ldw, lora_b, n, k, u, a, st);
-    return few_product<64>(x, ldx, weight, ldw, lora_b, n, k, u, a, st);
+    if (tokens <= 64) return few_product<64>(x, ldx, weight, ldw, lora_b, n, k, u, a, st);
+    return few_product<128>(x, ldx, weight, ldw, lora_b, n, k, u, a, st);
   }
   if (int rc = rank_product(x, ldx, k, lora_a, false, a, u, true, st)) return rc;
   return gemm_bf16_masked_k2(x, ldx, weight, ldw, false, u, a.rank_cols, lora_b, a.rank_cols, a.rank_cols, a.mask256,
@@ -857,7 +902,7 @@ int soup_multi_lora_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx
     return SOUP_ERR_INVALID;
   }
   if (!operand_ok(dy, lddy) || !operand_ok(weight, ldw) || (da && !operand_ok(x, ldx)) ||
-      (dx && !operand_ok(dx, lddx)) || !aligned16(lora_a) || !aligned16(lora_b)) {
+      (dx && !operand_ok(dx, lddx)) || !aligned16(lora_a) || !aligned16(lora_b) || !aligned16(da) || !aligned16(db)) {
     set_last_error("soup_multi_lora_bwd: operands need 16-byte aligned rows");
     return SOUP_ERR_UNSUPPORTED;
   }

@@ -54,6 +54,10 @@ LORA = [
     (33, 264, 1000, 5, 24, None, False),
     (64, 1536, 2048, 128, 32, None, False),
     (65, 1536, 2048, 64, 64, None, True),
+    (128, 392, 712, 12, 16, 3, False),
+    (200, 1536, 640, 31, 16, None, True),
+    (256, 264, 9600, 3, 8, 9, True),
+    (256, 264, 9344, 3, 8, 9, True),
     (127, 72, 88, 2, 4, 50, False),
     (129, 640, 512, 9, 16, 13, True),
     (300, 512, 264, 300, 8, 1, False),
