@@ -469,31 +469,26 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   if (!*abort_flag) {
     const uint32_t part_addr = smem_u32(part);
-    uint32_t peer[16];
+    uint32_t peer[8];
     if (ks > 1) {
 #pragma unroll
-      for (int p = 0; p < 16; ++p) peer[p] = p < ks ? cluster_addr(part_addr, p) : 0u;
+      for (int p = 0; p < 8; ++p) peer[p] = p < ks ? cluster_addr(part_addr, p) : 0u;
     }
-    // partials in rank order, eight of them in flight
+    // partials in rank order, all of them in flight
     auto reduce = [&](int off) {
       if (ks == 1) return *reinterpret_cast<const float4*>(part + off);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f), q[8];
 #pragma unroll
-      for (int p = 0; p < 16; p += 8) {
-        if (p >= ks) break;
-        float4 q[8];
+      for (int p = 0; p < 8; ++p)
+        if (p < ks) q[p] = ld_cluster_f4(peer[p] + off * 4);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (p + u < ks) q[u] = ld_cluster_f4(peer[p + u] + off * 4);
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (p + u < ks) {
-            sum.x += q[u].x;
-            sum.y += q[u].y;
-            sum.z += q[u].z;
-            sum.w += q[u].w;
-          }
-      }
+      for (int p = 0; p < 8; ++p)
+        if (p < ks) {
+          sum.x += q[p].x;
+          sum.y += q[p].y;
+          sum.z += q[p].z;
+          sum.w += q[p].w;
+        }
       return sum;
     };
     if (by_column) {
@@ -559,36 +554,58 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-// U of few tokens: a warp a (token, rank column), 16 bytes of x and of A's row a lane and
-// step. Bound by the latency of ids -> A -> sum, a third of the tile kernel's.
+// U of few tokens: `split` warps a (token, rank column), each its part of k, 16 bytes of x
+// and of A's row a lane and step, eight steps in flight. The projection's kernel streams the
+// weights meanwhile, so that each round trip waits behind those: with four steps in flight
+// and no split 8 tokens of 18944 features took 48 us beside the projection, 19 alone.
 constexpr int kFewWarps = 8;
+constexpr int kFewSteps = 4;
+constexpr int kFewFull = 4096;
 __global__ void __launch_bounds__(32 * kFewWarps) few_rank_kernel(const bf16* __restrict__ x, int64_t ldx,
-                                                                  const bf16* __restrict__ lora_a, const Args a) {
+                                                                  const bf16* __restrict__ lora_a, const Args a,
+                                                                  int split) {
+  __shared__ float parts[kFewWarps];
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x, j = blockIdx.y * kFewWarps + warp;
+  const int t = blockIdx.x, j = (blockIdx.y * kFewWarps + warp) / split;
   const int id = adapter_of(a, t);
+  float dot = 0.f;
   if (id >= 0 && j < a.rank) {
     const uint4* row = reinterpret_cast<const uint4*>(lora_a + ((int64_t)id * a.rank + j) * a.k);
     const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)t * ldx);
     uint64_t sum = 0;
-    const int parts = a.k / 8;
-#pragma unroll 4
-    for (int i = lane; i < parts; i += 32) {
-      const uint4 u = xr[i], v = row[i];
-      const uint32_t us[4] = {u.x, u.y, u.z, u.w}, vs[4] = {v.x, v.y, v.z, v.w};
+    const int all = a.k / 8, part = warp % split;
+    const int end = all * (part + 1) / split;
+    for (int i = all * part / split + lane; i - lane < end; i += 32 * kFewSteps) {
+      uint4 u[kFewSteps], v[kFewSteps];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        sum = f2_fma(f2_pack(__uint_as_float(us[q] << 16), __uint_as_float(us[q] & 0xffff0000u)),
-                     f2_pack(__uint_as_float(vs[q] << 16), __uint_as_float(vs[q] & 0xffff0000u)), sum);
+      for (int q = 0; q < kFewSteps; ++q) {
+        const bool in = i + 32 * q < end;
+        u[q] = in ? xr[i + 32 * q] : make_uint4(0, 0, 0, 0);
+        v[q] = in ? row[i + 32 * q] : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int q = 0; q < kFewSteps; ++q) {
+        const uint32_t us[4] = {u[q].x, u[q].y, u[q].z, u[q].w}, vs[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          sum = f2_fma(f2_pack(__uint_as_float(us[h] << 16), __uint_as_float(us[h] & 0xffff0000u)),
+                       f2_pack(__uint_as_float(vs[h] << 16), __uint_as_float(vs[h] & 0xffff0000u)), sum);
+      }
     }
     float lo, hi;
     f2_unpack(sum, lo, hi);
-    const float dot = warp_sum(lo + hi);
-    if (lane == 0)
-      a.u[(int64_t)t * a.rank_cols + id * a.rank + j] = __float2bfloat16_rn(dot * a.scales[id]);
+    dot = warp_sum(lo + hi);
   }
+  if (split > 1) {
+    if (lane == 0) parts[warp] = dot;
+    __syncthreads();
+    if (warp % split == 0)
+      for (int p = 1; p < split; ++p) dot += parts[warp + p];
+  }
+  if (id >= 0 && j < a.rank && warp % split == 0 && lane == 0)
+    a.u[(int64_t)t * a.rank_cols + id * a.rank + j] = __float2bfloat16_rn(dot * a.scales[id]);
   if (blockIdx.y != 0 || warp != 0) return;
   // the word of all tokens, and 0 in its blocks' columns of other adapters
   uint64_t word = 0;
@@ -647,7 +664,10 @@ int map2d(CUtensorMap* map, const void* ptr, int64_t inner, int64_t outer, int64
 }
 
 // `busy`: clusters of the grid that have work, as far as the host can tell. The k
-// range is split until one wave of two CTAs an SM is full, at least four k blocks each.
+// range is split until one wave of two CTAs an SM is full, at least four k blocks each;
+// into more than four parts only where each has sixteen blocks, eight at most: peers add up
+// and place slower than they save (8 tokens of 1536 columns: 8960 features 17.7 us split
+// four ways, 12.2 eight; 4096 x 4096 13.8 and 14.8).
 template <int MODE, bool B_MN, int NP>
 int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& ma2, const CUtensorMap& mb2, Args args,
            int k_blocks, int rank_blocks, int busy, cudaStream_t stream) {
@@ -656,7 +676,7 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& ma2,
   constexpr int kMost = 110 * 1024;  // two CTAs an SM
   static_assert(L::kBytesFor(kMaxTokens / 64) <= kMost, "shared memory of a CTA");
   static bool attr_done[64] = {false};
-  static int max_clusters[64][17] = {};  // by cluster size; -1: none fits
+  static int max_clusters[64][9] = {};  // by cluster size; -1: none fits
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cuda_status(cudaErrorInvalidDevice);
@@ -684,13 +704,12 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& ma2,
     if (!attr_done[dev]) {
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
       if (e != cudaSuccess) return cuda_status(e);
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-        cudaGetLastError();
       attr_done[dev] = true;
     }
   }
   int ks = 2 * sms / (busy > 0 ? busy : 1);
-  if (ks > 16) ks = 16;
+  const int most = k_blocks >= 128 ? 8 : k_blocks >= 80 ? k_blocks / 16 : 4;
+  if (ks > most) ks = most;
   if (ks > k_blocks / 4) ks = k_blocks / 4;
   if (ks < 1) ks = 1;
   for (; ks > 1; --ks) {
@@ -861,14 +880,19 @@ int soup_multi_lora_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
   Args a = base_args(ids, ids_64, tokens_per_id, scales, tokens, adapters, rank, s, l);
   bf16* u = reinterpret_cast<bf16*>(s + l.u);
   cudaStream_t st = as_stream(stream);
-  // up to 128 tokens always; up to 256 where the 256-row tiles of the pair GEMM would
-  // leave more than half of the SMs idle
-  if (tokens <= kFewTile || (tokens <= kFewTokens && (n + 255) / 256 * 4 < num_sms())) {
+  // up to 128 tokens always; up to 256 where the 256-row tiles of the pair GEMM would leave
+  // half of the SMs idle (256 tokens: 3584 -> 3584 features 24.5 us and 35.4 by that, 1536 ->
+  // 8960 21.3 and 23.9, 3584 -> 18944 46.4 and 40.1)
+  if (tokens <= kFewTile || (tokens <= kFewTokens && (n + 255) / 256 * 2 < num_sms())) {
     a.k = (int)k;
     a.u = u;
-    if (int rc = cuda_status(launch_pdl(few_rank_kernel, dim3((unsigned)tokens, (a.rank + kFewWarps - 1) / kFewWarps),
+    // warps a rank column: until one round of loads is all, or as many warps as the SMs hold
+    int split = 1;
+    while (split < kFewWarps && k > (int64_t)split * kFewSteps * 256 && tokens * a.rank * split < kFewFull) split *= 2;
+    const int columns = kFewWarps / split;
+    if (int rc = cuda_status(launch_pdl(few_rank_kernel, dim3((unsigned)tokens, (a.rank + columns - 1) / columns),
                                         dim3(32 * kFewWarps), 0, st, static_cast<const bf16*>(x), ldx,
-                                        static_cast<const bf16*>(lora_a), a)))
+                                        static_cast<const bf16*>(lora_a), a, split)))
       return rc;
     a.y = static_cast<bf16*>(y);
     a.ldy = ldy;
