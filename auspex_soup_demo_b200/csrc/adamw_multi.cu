@@ -38,6 +38,7 @@ constexpr int kBlock = 256;              // elements that share a scale
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kE4m3Max = 448.f;
+constexpr float kMostV = 3.3e38f;        // second moments past 32 bits stay at their end
 
 struct Tensor {
   void* p;
@@ -167,17 +168,28 @@ __device__ __forceinline__ uint64_t pair_of_codes(uint2 c, int i) {
   return f2_pack(v.x, v.y);
 }
 
-// Root and reciprocal to 2^-22, subnormals as 0: the IEEE forms cost more instructions
-// than all the rest.
-__device__ __forceinline__ float root_approx(float x) {
+// Reciprocal and reciprocal root to 2^-22, subnormals as 0: the IEEE forms cost more
+// instructions than all the rest.
+__device__ __forceinline__ float recip_root_approx(float x) {
   float y;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ float recip_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Square roots of a pair of finite numbers, rounded as exact ones are but for rare last bits:
+// one Newton step s + (x - s^2) / (2 sqrt(x)) from x times the approximate reciprocal root
+// (of x + 2^-126, which leaves 0 its root and numbers above 2^-102 as they are).
+__device__ __forceinline__ uint64_t root_pair(uint64_t x) {
+  float lo, hi;
+  f2_unpack(f2_add(x, f2_same(1.17549435e-38f)), lo, hi);
+  const uint64_t h = f2_pack(recip_root_approx(lo), recip_root_approx(hi));
+  const uint64_t s = f2_mul(x, h);
+  return f2_fma(f2_fma(s, s, f2_mul(x, f2_same(-1.f))), f2_mul(h, f2_same(-0.5f)), s);
 }
 
 // Scale of the warp's block and its codes. Values that are not finite are left out of
@@ -200,12 +212,17 @@ __device__ __forceinline__ uint2 to_codes(const uint64_t (&f)[4], float& scale) 
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]) <= 3.4028235e38f ? fabsf(v[i]) : 0.f);
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
   }
-  scale = top * (1.f / kE4m3Max);
+  scale = top / kE4m3Max;
   uint64_t y[4];
   if (scale >= 1.17549435e-38f) {  // warp-uniform
-    const uint64_t inv = f2_same(recip_approx(scale));
+    // quotients corrected by their remainder, as an exact division rounds them but for rare
+    // last bits: which of two codes a value between them takes is then that of the formula
+    const uint64_t inv = f2_same(recip_approx(scale)), minus = f2_same(-scale);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = f2_mul(f[i], inv);
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t q = f2_mul(f[i], inv);
+      y[i] = f2_fma(f2_fma(q, minus, f[i]), inv, q);
+    }
   } else {
     // no finite reciprocal: scaled up by 2^64 first (a block of zeros stays 0)
     const float inv = scale > 0.f ? 1.f / (scale * 1.8446744e19f) : 0.f;
@@ -376,11 +393,13 @@ __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_ke
       v[i] = v32.pair(i);
     }
     const uint64_t gi = f2_mul(g.pair(i), clip);
-    m[i] = f2_fma(c1, f2_fma(m[i], minus, gi), m[i]);
-    v[i] = f2_fma(f2_mul(c2, gi), gi, f2_mul(v[i], b2));
+    // each operation of the moments rounds once, as elementwise tensor operations do: an
+    // 8-bit state that lies between two codes then goes the same way
+    m[i] = f2_add(f2_mul(c1, f2_fma(m[i], minus, gi)), m[i]);
     float lo, hi;
-    f2_unpack(v[i], lo, hi);
-    root[i] = f2_pack(root_approx(lo), root_approx(hi));
+    f2_unpack(f2_add(f2_mul(v[i], b2), f2_mul(c2, f2_mul(gi, gi))), lo, hi);
+    v[i] = f2_pack(fminf(lo, kMostV), fminf(hi, kMostV));
+    root[i] = root_pair(v[i]);
     f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
     const uint64_t inv = f2_pack(recip_approx(lo), recip_approx(hi));
     p.set(i, f2_fma(f2_mul(m[i], step_size), inv, f2_mul(p.pair(i), decay)));

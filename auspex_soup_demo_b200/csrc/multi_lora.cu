@@ -388,30 +388,65 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ----------------------------------------------- MMA issuer ----
+    // ------------------------------------------------- MMA issuer ----
+    // (kModeGrad: the whole warp, which clears tokens; else one lane)
+    if (MODE == kModeGrad || lane == 0) {
       KWalk k = walk();
       int it = 0, kb;
       bool second;
       while (k.next(kb, second)) {
         const int s = it % L::kStages;
         const uint32_t ph = (it / L::kStages) & 1u;
-        if (!bounded_wait(full_bar(s), ph, abort_flag, err, kErrMma, wait_ns)) break;
-        tc_fence_after();
         const uint32_t a_addr = sbase + s * L::kStage;
         const uint32_t b_addr = a_addr + L::kABytes;
+        uint32_t out[2] = {0, 0};
+        if constexpr (MODE == kModeGrad) {
+          // tokens without an adapter of this rank block: their rows of x or dy, whose
+          // factors are 0, are cleared, or a NaN in a masked row would reach every sum
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const uint64_t ad = A_MN ? smem_desc_sw128(a_addr + kk * 2048, 8192, 1024)
-                                   : smem_desc_sw128(a_addr + kk * 32, 16, 1024);
-          const uint64_t bd = B_MN ? smem_desc_sw128(b_addr + kk * 2048, 8192, 1024)
-                                   : smem_desc_sw128(b_addr + kk * 32, 16, 1024);
-          tc_mma_bf16(tmem, ad, bd, kIdesc, (it > 0 || kk > 0) ? 1u : 0u);
+          for (int h = 0; h < 2; ++h) {
+            const int t = kb * 64 + h * 32 + lane;
+            out[h] = __ballot_sync(0xffffffffu,
+                                   t < a.tokens && !((adapter_bits(a, adapter_of(a, t)) >> rb) & 1));
+          }
+        }
+        bool ok = bounded_wait(full_bar(s), ph, abort_flag, err, kErrMma, wait_ns);
+        if constexpr (MODE == kModeGrad) {
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok && (out[0] | out[1])) {  // warp-uniform
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if ((out[h] >> lane) & 1) {
+                // a token is a row of 128 bytes in both boxes; swizzling stays within it
+                uint8_t* row = smem + s * L::kStage + (h * 32 + lane) * 128;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                  const int at = (c ^ (lane & 7)) * 16;
+                  *reinterpret_cast<uint4*>(row + at) = make_uint4(0, 0, 0, 0);
+                  *reinterpret_cast<uint4*>(row + 8192 + at) = make_uint4(0, 0, 0, 0);
+                }
+              }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint64_t ad = A_MN ? smem_desc_sw128(a_addr + kk * 2048, 8192, 1024)
+                                     : smem_desc_sw128(a_addr + kk * 32, 16, 1024);
+            const uint64_t bd = B_MN ? smem_desc_sw128(b_addr + kk * 2048, 8192, 1024)
+                                     : smem_desc_sw128(b_addr + kk * 32, 16, 1024);
+            tc_mma_bf16(tmem, ad, bd, kIdesc, (it > 0 || kk > 0) ? 1u : 0u);
+          }
+          tc_commit(empty_bar(s));
         }
         ++it;
-        tc_commit(empty_bar(s));
       }
-      if (it > 0) {
+      if (lane != 0) {
+      } else if (it > 0) {
         tc_commit(acc_bar);
         // the MMAs are done before TMEM can be freed, also when the epilogue
         // stopped waiting for them (bounded)

@@ -134,8 +134,14 @@ def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tenso
     adapters without tokens get zeros. K, N and adapters * rank must be multiples of
     8, adapters * rank at most 4096. Tokens of one adapter should follow one another,
     as requests do: the work of the adapters grows with the different ones among 256
-    consecutive tokens. Up to 64 tokens (the next tokens of many requests) take a form
+    consecutive tokens. Up to 256 tokens (the next tokens of many requests) take a form
     that streams the weight once through all SMs.
+
+    A token without an adapter may hold anything: it reaches its own row of y and of
+    x's gradient alone. Factors, also those that no token takes, have to be finite:
+    adapters are multiplied 64 columns at a time, with zeros where a token has another
+    adapter; and a row of x or of y's gradient that is not finite reaches the gradients
+    of the adapters that share 64 columns with its own.
     """
     fn = "multi_lora_linear"
     xs, ws, sa, sb = x.shape, weight.shape, lora_a.shape, lora_b.shape

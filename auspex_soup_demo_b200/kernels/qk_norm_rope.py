@@ -26,6 +26,7 @@ import torch
 from .. import _lib
 
 MAX_HEAD_DIM = 512
+MAX_AXES = 256
 
 # soup_qk_rope: sizes, types, table strides, six tensors' strides, eps
 _DESC = struct.Struct("=5q5q3q24qd")
@@ -162,6 +163,8 @@ def _check(fn: str, q, k, qw, kw, eps):
     d = qs[3]
     if d % 2 or not 0 < d <= MAX_HEAD_DIM:
         raise ValueError(f"{fn}: head_dim must be even and at most {MAX_HEAD_DIM}, got {d}")
+    if (qs[1] == 0) != (ks[1] == 0):
+        raise ValueError(f"{fn}: q and k must both have heads, got {qs[1]} and {ks[1]}")
     if not q.is_cuda or k.device != q.device:
         raise ValueError(f"{fn}: q and k must be on one CUDA device")
     if (qw is None) != (kw is None):
@@ -253,8 +256,8 @@ def apply_multi_axis_rope(q: torch.Tensor, k: torch.Tensor, position_ids: torch.
     axes = tuple(axes)
     if len(axes) != d // 2:
         raise ValueError(f"{fn}: {len(axes)} axes for {d // 2} frequencies")
-    if min(axes) < 0 or max(axes) >= shape[0]:
-        raise ValueError(f"{fn}: axes must be in [0, {shape[0]})")
+    if min(axes) < 0 or max(axes) >= min(shape[0], MAX_AXES):
+        raise ValueError(f"{fn}: axes must be in [0, {min(shape[0], MAX_AXES)})")
     if inv_freq.dtype is not torch.float32 or tuple(inv_freq.shape) != (d // 2,):
         raise ValueError(f"{fn}: inv_freq must be float32 [{d // 2}], got {inv_freq.dtype} {tuple(inv_freq.shape)}")
     if position_ids.device != q.device or inv_freq.device != q.device:

@@ -27,7 +27,7 @@ STATE_BLOCK = 256
 
 
 _grad, _dtype = operator.attrgetter("grad"), operator.attrgetter("dtype")
-_data_ptr, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_data_ptr, _is_contiguous, _get_device = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
 
 
 def _address(a: array.array) -> int:
@@ -61,7 +61,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     ``torch.optim.AdamW`` (every element, where the norm is clipped).
 
     The optimiser's steps share their workspace and states: steps of one optimiser
-    on several streams have to be ordered by the caller.
+    on several streams have to be ordered by the caller. Autograd does not see a
+    step's writes: a backward pass that needs the old values has to come before it.
     """
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -75,7 +76,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         self.grad_norm = None
         self._held = []
         self._step = None
-        self._squares = None
+        self._squares = []
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
     # -- set-up -----------------------------------------------------------------
@@ -103,7 +104,12 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     def _hold(self, params) -> _Held:
         held = _Held()
-        dev = self._step.device if self._step is not None else params[0].device
+        if self._step is not None:
+            dev = self._step.device
+        else:
+            dev = params[0].device if params else torch.device("cuda", torch.cuda.current_device())
+        if len(set(map(id, params))) != len(params):
+            raise ValueError("MultiTensorAdamW: a parameter is in the group twice")
         blocks, total = [], 0
         for p in params:
             _lib.dtype_code(p.dtype)
@@ -130,7 +136,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         held.v = torch.zeros(total, STATE_BLOCK, dtype=torch.uint8 if eight else dt, device=dev).view(dt)
         held.m_scale = torch.zeros(total, dtype=torch.float32, device=dev) if eight else None
         held.v_scale = torch.zeros(total, dtype=torch.float32, device=dev) if eight else None
-        if self._step is None:
+        if self._step is None and params:
             self._step = torch.zeros((), dtype=torch.float32, device=dev)
             self._coefs = torch.zeros(4, dtype=torch.float32, device=dev)
         if self.max_grad_norm is not None:
@@ -139,8 +145,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
             # one workspace of partial sums for the launches of every type of every group
             per = int(_lib.lib().soup_grad_square_workspace_bytes(1))
             need = int(_lib.lib().soup_grad_square_workspace_bytes(max(1, tensors))) + per * launches
-            if self._squares is None or self._squares.numel() < need:
-                self._squares = torch.empty(need, dtype=torch.uint8, device=dev)
+            if not self._squares or self._squares[-1].numel() < need:
+                # the smaller ones stay: a captured step may write them
+                self._squares.append(torch.empty(need, dtype=torch.uint8, device=dev))
             if self.grad_norm is None:
                 self.grad_norm = torch.zeros((), dtype=torch.float32, device=dev)
         for i, p in enumerate(params):
@@ -207,7 +214,7 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                     raise ValueError("MultiTensorAdamW: gradients must be dense")
                 grads = [g.detach().contiguous() for g in grads]
                 grad_ptrs = array.array("Q", map(_data_ptr, grads))
-            if set(map(_dtype, grads)) != {dtype} or grads[0].device != device:
+            if set(map(_dtype, grads)) != {dtype} or set(map(_get_device, grads)) != {device.index}:
                 raise ValueError(f"MultiTensorAdamW: gradients must be {dtype} on {device}, as their parameters")
             out.append((code, array.array("Q", map(_data_ptr, params)), grad_ptrs, sizes, blocks, grads))
         return out
@@ -218,6 +225,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if self._step is None:  # no parameters at all
+            return loss
         dev = self._step.device
         tables = [self._tables(h, dev) for h in self._held]
         launches = sum(map(len, tables))
@@ -227,10 +236,10 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         partials = ctypes.c_int(0)
         squares = None
         if self.max_grad_norm is not None:
-            squares = self._squares.data_ptr()
+            squares, nbytes = self._squares[-1].data_ptr(), self._squares[-1].numel()
             for code, _, g, sizes, _, _ in itertools.chain.from_iterable(tables):
                 _lib.call("soup_grad_square", dev, _address(g), _address(sizes), len(g), code, squares,
-                          self._squares.numel(), ctypes.byref(partials), stream)
+                          nbytes, ctypes.byref(partials), stream)
         done = 0
         for group, held, table in zip(self.param_groups, self._held, tables):
             b1, b2 = group["betas"]

@@ -295,3 +295,20 @@ def test_multi_adapter_linear_and_its_files(tmp_path):
         m.q_proj(torch.zeros(1, 16))
     with pytest.raises(ValueError, match="adapter ids"):
         m.ids.set(torch.zeros(2))
+
+
+def test_rotations_refuse_what_has_no_form():
+    """More axes than a byte counts, and heads of q or k alone."""
+    meta = _FakeCuda(torch.zeros(1, 2, 3, 8, dtype=BF, device="meta"))
+    pos = torch.zeros(300, 3, dtype=torch.int64, device="meta")
+    with pytest.raises(ValueError, match=r"axes must be in \[0, 256\)"):
+        kernels.apply_multi_axis_rope(meta, meta, pos, torch.ones(4, device="meta"), (0, 1, 2, 256))
+    none = _FakeCuda(torch.zeros(1, 0, 3, 8, dtype=BF, device="meta"))
+    with pytest.raises(ValueError, match="both have heads"):
+        qk_norm_rope._check("f", meta, none, None, None, 1e-6)
+
+
+def test_adamw_multi_refuses_a_parameter_twice():
+    p = torch.nn.Parameter(torch.zeros(4))
+    with pytest.warns(UserWarning), pytest.raises(ValueError, match="twice"):
+        MultiTensorAdamW([p, p])
