@@ -84,8 +84,8 @@ struct Smem {
   static constexpr int kBar = kStages * kStage;
   static constexpr int kNumBars = 2 * kStages + 1;  // full[S], empty[S], acc_full
   static constexpr int kMisc = kBar + kNumBars * 8;  // tmem, abort, words[8]
-  static constexpr int kBits = kMisc + 16 + 64;      // kModeGrad: one bit per token block
-  static constexpr int kBytesFor(int token_blocks) { return kBits + ((token_blocks + 31) / 32 + 1) * 4 + 1024; }
+  static constexpr int kBits = kMisc + 16 + 64;      // kModeGrad: two bits per token block
+  static constexpr int kBytesFor(int token_blocks) { return kBits + ((token_blocks + 31) / 32 + 1) * 8 + 1024; }
 };
 
 struct Args {
@@ -101,7 +101,8 @@ struct Args {
   int ids_64;
   int per;           // tokens of one id
   const float* scales;
-  uint64_t* mask64;  // words of 64-token blocks
+  uint64_t* mask64;  // words of 64-token blocks: rank blocks that any of their tokens has
+  uint64_t* all64;   // and that all of them have
   uint64_t* mask256; // words of 256-token tiles
   int write_masks;
   // outputs
@@ -166,6 +167,18 @@ __device__ __forceinline__ uint64_t warp_or64(uint64_t v) {
   const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)v);
   const uint32_t hi = __reduce_or_sync(0xffffffffu, (uint32_t)(v >> 32));
   return ((uint64_t)hi << 32) | lo;
+}
+// The words of 64 tokens, formed by a warp: rank blocks that any of them has, that all have.
+__device__ __forceinline__ uint64_t block_words(const Args& a, int t0, int lane, uint64_t& all) {
+  uint64_t any = 0, none = 0;
+#pragma unroll
+  for (int t = t0 + lane; t < t0 + 64; t += 32) {
+    const uint64_t b = adapter_bits(a, adapter_of(a, t));
+    any |= b;
+    none |= t < a.tokens ? ~b : 0;
+  }
+  all = ~warp_or64(none);
+  return warp_or64(any);
 }
 
 // The k blocks of a CTA: a run of blocks and (kModeFew) behind it its share of the rank
@@ -250,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   const int token_blocks = (a.tokens + 63) / 64;
-  const uint32_t used = MODE == kModeGrad ? L::kBits + ((token_blocks + 31) / 32 + 1) * 4 : L::kBits;
+  const uint32_t used = MODE == kModeGrad ? L::kBits + ((token_blocks + 31) / 32 + 1) * 8 : L::kBits;
   if ((uint32_t)(smem - smem_raw) + used > dynamic_smem()) {  // grid-uniform
     if (threadIdx.x == 0) atomicCAS(err, 0, kErrSmem);
     return;
@@ -265,6 +278,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
   uint64_t* words = reinterpret_cast<uint64_t*>(smem + L::kMisc + 16);
   uint32_t* bits = reinterpret_cast<uint32_t*>(smem + L::kBits);
+  uint32_t* mixed = bits + (token_blocks + 31) / 32 + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ks = a.ks;
@@ -281,17 +295,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   if constexpr (MODE == kModeRank) {
     // words of the 256 tokens around this tile, from the ids; cluster-uniform
     if (warp < 4) {
-      const int t0 = (mt >> 1) * 256 + warp * 64;
-      const uint64_t w =
-          warp_or64(adapter_bits(a, adapter_of(a, t0 + lane)) | adapter_bits(a, adapter_of(a, t0 + 32 + lane)));
-      if (lane == 0) words[warp] = w;
+      uint64_t all;
+      const uint64_t w = block_words(a, (mt >> 1) * 256 + warp * 64, lane, all);
+      if (lane == 0) {
+        words[warp] = w;
+        words[4 + warp] = all;
+      }
     }
     __syncthreads();
     const uint64_t here = words[(mt & 1) * 2] | words[(mt & 1) * 2 + 1];
     const uint64_t tile = words[0] | words[1] | words[2] | words[3];
     if (a.write_masks && rb == 0 && rank == 0 && threadIdx.x < 2) {
       const int blk = mt * 2 + threadIdx.x;
-      if (blk < token_blocks) a.mask64[blk] = words[(mt & 1) * 2 + threadIdx.x];
+      if (blk < token_blocks) {
+        a.mask64[blk] = words[(mt & 1) * 2 + threadIdx.x];
+        a.all64[blk] = words[4 + (mt & 1) * 2 + threadIdx.x];
+      }
       if (threadIdx.x == 0 && (mt & 1) == 0) a.mask256[mt >> 1] = tile;
     }
     if (!((tile >> rb) & 1)) return;
@@ -300,8 +319,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   if constexpr (MODE == kModeGrad) {
     for (int w = warp; w * 32 < token_blocks; w += kThreads / 32) {
       const int blk = w * 32 + lane;
-      const uint32_t b = __ballot_sync(0xffffffffu, blk < token_blocks && ((a.mask64[blk] >> rb) & 1));
-      if (lane == 0) bits[w] = b;
+      const uint64_t any = blk < token_blocks ? a.mask64[blk] : 0, all = blk < token_blocks ? a.all64[blk] : 0;
+      const uint32_t b = __ballot_sync(0xffffffffu, (any >> rb) & 1);
+      const uint32_t m = __ballot_sync(0xffffffffu, ((any & ~all) >> rb) & 1);
+      if (lane == 0) {
+        bits[w] = b;
+        mixed[w] = m;
+      }
     }
   }
   if (threadIdx.x == 0) {
@@ -400,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t a_addr = sbase + s * L::kStage;
         const uint32_t b_addr = a_addr + L::kABytes;
         uint32_t out[2] = {0, 0};
-        if constexpr (MODE == kModeGrad) {
+        if (MODE == kModeGrad && (mixed[kb >> 5] >> (kb & 31)) & 1) {
           // tokens without an adapter of this rank block: their rows of x or dy, whose
           // factors are 0, are cleared, or a NaN in a masked row would reach every sum
 #pragma unroll
@@ -645,9 +669,12 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rank_kernel(const bf16* __
   // the word of all tokens, and 0 in its blocks' columns of other adapters
   uint64_t word = 0;
   for (int b = 0; b * 64 < a.tokens; ++b) {
-    const uint64_t w = warp_or64(adapter_bits(a, adapter_of(a, b * 64 + lane)) |
-                                 adapter_bits(a, adapter_of(a, b * 64 + 32 + lane)));
-    if (t == 0 && lane == 0) a.mask64[b] = w;
+    uint64_t all;
+    const uint64_t w = block_words(a, b * 64, lane, all);
+    if (t == 0 && lane == 0) {
+      a.mask64[b] = w;
+      a.all64[b] = all;
+    }
     word |= w;
   }
   if (t == 0 && lane == 0) a.mask256[0] = word;
@@ -772,12 +799,13 @@ int launch(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& ma2,
 }
 
 struct Layout {
-  int64_t mask64, mask256, u, bytes;  // byte offsets into the state
+  int64_t mask64, all64, mask256, u, bytes;  // byte offsets into the state
 };
 Layout layout_of(int64_t tokens, int64_t rank_cols) {
   Layout l;
   l.mask64 = 0;
-  l.mask256 = ((tokens + 63) / 64 * 8 + 15) / 16 * 16;
+  l.all64 = (tokens + 63) / 64 * 8;
+  l.mask256 = (2 * l.all64 + 15) / 16 * 16;
   l.u = l.mask256 + ((tokens + 255) / 256 * 8 + 127) / 128 * 128;
   l.u = (l.u + 127) / 128 * 128;
   l.bytes = l.u + tokens * rank_cols * 2;
@@ -875,6 +903,7 @@ Args base_args(const void* ids, int ids_64, int64_t per, const float* scales, in
   a.per = (int)(per > tokens ? tokens : per);
   a.scales = scales;
   a.mask64 = reinterpret_cast<uint64_t*>(state + l.mask64);
+  a.all64 = reinterpret_cast<uint64_t*>(state + l.all64);
   a.mask256 = reinterpret_cast<uint64_t*>(state + l.mask256);
   return a;
 }

@@ -70,8 +70,8 @@ def test_multi_lora_c_arguments():
 
 @pytest.mark.parametrize("tokens,adapters,rank", [(1, 1, 8), (64, 3, 8), (65, 1, 64), (1000, 24, 8), (8192, 256, 16)])
 def test_multi_lora_state_layout(tokens, adapters, rank):
-    """Words of 64- and 256-token blocks, then U at a 128-byte boundary, none overlapping."""
-    m64 = (tokens + 63) // 64 * 8
+    """Two words of 64- and one of 256-token blocks, then U at a 128-byte boundary, none overlapping."""
+    m64 = (tokens + 63) // 64 * 8 * 2
     m256 = (m64 + 15) // 16 * 16
     u = m256 + ((tokens + 255) // 256 * 8 + 127) // 128 * 128
     u = (u + 127) // 128 * 128
