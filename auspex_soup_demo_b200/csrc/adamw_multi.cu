@@ -35,7 +35,7 @@ namespace soup {
 namespace {
 
 constexpr int kBlock = 256;              // elements that share a scale
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kE4m3Max = 448.f;
 constexpr float kMostV = 3.3e38f;        // second moments past 32 bits stay at their end
@@ -57,12 +57,15 @@ struct Table {
 // CTAs of the step's kernel on an SM (40 to 48 registers a thread). Each warp takes one
 // block and is done: CTAs then come in the order of memory. A grid of resident CTAs that
 // stride over the tensors, or walk a run of them each, drifts apart, and DRAM serves many
-// pages at a time: 8-bit states of 233 M bf16 elements take 407 us this way, 464 to 619
+// pages at a time: 8-bit states of 233 M bf16 elements took 407 us this way, 464 to 619
 // us with resident CTAs of every depth tried, with or without a ring of cp.async copies.
-__host__ __device__ constexpr int step_ctas(int es) { return es == 4 ? 5 : 6; }
+// With exactly rounded codes (root_pair, to_codes) it is 425 us, 5.5 TB/s (8 warps a CTA
+// 430, 16 453, 2 473); 100 M fp32 elements with 32-bit states 412 us, 6.8 TB/s.
+__host__ __device__ constexpr int step_ctas(int es) { return es == 4 ? 10 : 12; }
 
 struct Hyper {
   float one_minus_beta1, beta2, one_minus_beta2, eps, decay;  // decay: 1 - lr wd
+  float one;  // an argument, so that a * b + c written as (a * b) * one + c keeps its two roundings
 };
 
 // What a step's elements share, left by adamw_coef_kernel.
@@ -358,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_ke
   const float4 co = *reinterpret_cast<const float4*>(coefs);
   const uint64_t step_size = f2_same(-co.x), root_scale = f2_same(co.y), clip = f2_same(co.z);
   const uint64_t c1 = f2_same(h.one_minus_beta1), c2 = f2_same(h.one_minus_beta2), b2 = f2_same(h.beta2);
-  const uint64_t eps = f2_same(h.eps), decay = f2_same(h.decay), minus = f2_same(-1.f);
+  const uint64_t eps = f2_same(h.eps), decay = f2_same(h.decay), one = f2_same(h.one), minus = f2_same(-h.one);
   const Tensor& t = tab.t[ti];
   const int64_t e = (int64_t)(c - t.first) * kBlock + lane * 8;
   const int64_t rest = t.n - e;
@@ -393,11 +396,12 @@ __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_ke
       v[i] = v32.pair(i);
     }
     const uint64_t gi = f2_mul(g.pair(i), clip);
-    // each operation of the moments rounds once, as elementwise tensor operations do: an
-    // 8-bit state that lies between two codes then goes the same way
-    m[i] = f2_add(f2_mul(c1, f2_fma(m[i], minus, gi)), m[i]);
+    // each operation of the moments rounds by itself, as elementwise tensor operations do:
+    // what lies between two codes then goes the same way as there (one code off is a
+    // sixteenth of a moment, or twice a small root)
+    m[i] = f2_fma(f2_mul(c1, f2_fma(m[i], minus, gi)), one, m[i]);
     float lo, hi;
-    f2_unpack(f2_add(f2_mul(v[i], b2), f2_mul(c2, f2_mul(gi, gi))), lo, hi);
+    f2_unpack(f2_fma(f2_mul(v[i], b2), one, f2_mul(c2, f2_mul(gi, gi))), lo, hi);
     v[i] = f2_pack(fminf(lo, kMostV), fminf(hi, kMostV));
     root[i] = root_pair(v[i]);
     f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_ke
   }
 }
 
-constexpr int kSquareCtas = 6;              // of grad_square_kernel on an SM, each with a partial sum
+constexpr int kSquareCtas = 12;             // of grad_square_kernel on an SM, each with a partial sum
 constexpr int kSmall = 64, kLarge = 960;  // tensors of a launch: arguments of 2 and 30 KB
 
 inline int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
@@ -606,7 +610,7 @@ int soup_adamw_multi(void* const* params, const void* const* grads, const int64_
     return SOUP_ERR_INVALID;
   }
   const States s{exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale};
-  const Hyper h{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay)};
+  const Hyper h{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay), 1.f};
   cudaStream_t st = as_stream(stream);
   Coefs* co = reinterpret_cast<Coefs*>(coefs);
   if (int rc = cuda_status(launch_pdl(adamw_coef_kernel, dim3(1), dim3(kThreads), 0, st, lr, log(beta1), log(beta2),
