@@ -610,7 +610,8 @@ int soup_adamw_multi(void* const* params, const void* const* grads, const int64_
     return SOUP_ERR_INVALID;
   }
   const States s{exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale};
-  const Hyper h{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay), 1.f};
+  const Hyper h{(float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps, (float)(1.0 - lr * weight_decay),
+                1.f};
   cudaStream_t st = as_stream(stream);
   Coefs* co = reinterpret_cast<Coefs*>(coefs);
   if (int rc = cuda_status(launch_pdl(adamw_coef_kernel, dim3(1), dim3(kThreads), 0, st, lr, log(beta1), log(beta2),

@@ -24,13 +24,18 @@
 //
 // Few tokens (next tokens of many requests): the base product is W's bytes.
 // The same kernel then streams W as the 128-row operand against all tokens at once
-// (N = T rounded up, at most 128 a CTA), so that every SM takes part, with U and B's blocks behind; it starts
-// beside the kernel that forms U and waits for that one only before its rank blocks.
+// (N = T rounded up, at most 128 a CTA), so that every SM takes part, with U and B's
+// blocks behind; it starts beside the kernel that forms U and waits for that one only
+// before its rank blocks.
+//
+// 8192 tokens, 1536 -> 17920 features, 4 adapters of rank 16: U 17 us, y 322 (309 without
+// adapters), V 68 (dy's 294 MB at 4.3 TB/s), dx 330 (328), dA 17, dB 53 (5.5 TB/s). 48 tokens
+// and 64 adapters: 21 us for 55 MB of weights; 8 tokens of 18944 -> 3584 27 us, 5 TB/s.
 //
 // u and v are rounded to bf16 between the two products, as x, dy and the factors are.
 //
 //   warp 0     TMA producer (one lane)
-//   warp 1     TMEM allocator + MMA issuer (one lane)
+//   warp 1     TMEM allocator + MMA issuer (one lane; for gradients it also clears rows)
 //   warps 2-5  epilogue: tcgen05.ld of lane quarter (warp % 4), cluster reduction, stores
 //
 // Every mbarrier wait is bounded (soup_set_wait_limit_ns); on expiry the code goes to

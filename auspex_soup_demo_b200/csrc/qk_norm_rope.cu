@@ -16,12 +16,13 @@
 //
 // A row (token, head) is `lanes` threads of one warp, each with NE elements of the
 // first half and the matching NE of the second, so a rotation needs no exchange and a
-// norm needs log2(lanes) shuffles. A CTA walks a run of tokens; a thread keeps its
-// (head, elements) slot for all of them. Its rows arrive by cp.async in a ring of
-// shared memory of its own (nobody else reads them, so no barrier), several tokens
-// ahead, which keeps enough bytes in flight without the registers for them. Head dims
-// whose half is not a multiple of a vector, or rows that are not 16-byte aligned, take
-// a warp per row instead.
+// norm needs log2(lanes) shuffles. Forward: a thread takes the rows of two tokens and is
+// done. Backward: a CTA walks a run of tokens and a thread keeps its (head, elements) slot
+// for all of them, so that its share of dw stays in registers; its rows arrive by cp.async
+// in a ring of shared memory of its own (nobody else reads them, so no barrier), several
+// tokens ahead, which keeps enough bytes in flight without the registers for them. Head
+// dims whose half is not a multiple of a vector, or rows that are not 16-byte aligned,
+// take a warp per row instead.
 #include <stdio.h>
 
 #include <mutex>
@@ -353,7 +354,9 @@ __device__ __forceinline__ void give(uint32_t at, const T* src, uint32_t pitch) 
 
 // Forward (and, without weights and with sign -1, the backward of a rotation alone). A
 // thread takes one row's elements of P tokens; CTA (x, y) the tokens [x C P, ...) of all
-// its heads, C of them side by side. CTAs come in the order of memory.
+// its heads, C of them side by side. CTAs come in the order of memory: DRAM then serves
+// few pages at a time. 2 x 16001 tokens of 32/8 heads of 128 in bf16: 117 us, 5.6 TB/s;
+// 130 us with resident CTAs that walk runs of tokens behind rings of cp.async.
 template <typename T, int NE, int P, bool NORM, int SRC>
 __global__ void __launch_bounds__(kMaxThreads, fwd_ctas(NE * (int)sizeof(T))) qk_rope_fwd_kernel(
     HeadRows q, HeadRows k, const __grid_constant__ Angles ang, Shape sh) {
@@ -441,7 +444,8 @@ __global__ void __launch_bounds__(kMaxThreads, fwd_ctas(NE * (int)sizeof(T))) qk
 
 // Backward with norms. The thread's share of dw stays in its registers. The CTA joins
 // its rows of dw in the order of the heads and leaves one partial row [2][D] (q, k),
-// which dw_join_kernel sums in block order.
+// which dw_join_kernel sums in block order. 2 x 16001 tokens of 32/8 heads of 128 in
+// bf16: 207 us, 4.75 TB/s.
 template <typename T, int NE, int SRC>
 __global__ void __launch_bounds__(kMaxThreads, bwd_ctas(NE * (int)sizeof(T))) qk_norm_rope_bwd_kernel(
     HeadRows q, HeadRows k, const __grid_constant__ Angles ang, Shape sh, float* __restrict__ dw_part) {

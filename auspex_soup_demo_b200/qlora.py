@@ -1264,8 +1264,9 @@ class QLoRATrainer:
     def step(self, input_ids: torch.Tensor, labels: torch.Tensor, denominator: float, adapter_ids=None,
              position_ids=None):
         """One step. adapter_ids [B] or [B, S]: the adapter of each sequence or token, for a
-        model with several; position_ids [B, S] or [axes, B, S] where positions are not
-        0, 1, 2, ... (these two also in the other steps)."""
+        model with several (they stay the model's until others are given); position_ids
+        [B, S] or [axes, B, S] where positions are not 0, 1, 2, ... (these two also in the
+        other steps)."""
         self._begin_step()
         hidden = self._hidden(input_ids, adapter_ids, position_ids)
         loss, entropy, token_loss, correct = self.loss_fn.apply(
