@@ -428,26 +428,24 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t ph = (it / L::kStages) & 1u;
         const uint32_t a_addr = sbase + s * L::kStage;
         const uint32_t b_addr = a_addr + L::kABytes;
-        uint32_t out[2] = {0, 0};
-        if (MODE == kModeGrad && (mixed[kb >> 5] >> (kb & 31)) & 1) {
-          // tokens without an adapter of this rank block: their rows of x or dy, whose
-          // factors are 0, are cleared, or a NaN in a masked row would reach every sum
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t = kb * 64 + h * 32 + lane;
-            out[h] = __ballot_sync(0xffffffffu,
-                                   t < a.tokens && !((adapter_bits(a, adapter_of(a, t)) >> rb) & 1));
-          }
-        }
         bool ok = bounded_wait(full_bar(s), ph, abort_flag, err, kErrMma, wait_ns);
         if constexpr (MODE == kModeGrad) {
           ok = __all_sync(0xffffffffu, ok);
-          if (ok && (out[0] | out[1])) {  // warp-uniform
+          if (ok && (mixed[kb >> 5] >> (kb & 31)) & 1) {  // warp-uniform
+            // Tokens without an adapter of this rank block, whose row of U or V is 0: their
+            // rows of x or dy are cleared, or a NaN in a masked row would reach every sum. A
+            // token is a row of 128 bytes in each box; swizzling stays within it. (By the ids
+            // it would be a global load for each such block: dA of 2999 x 8960 28 us, 22 so.)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if ((out[h] >> lane) & 1) {
-                // a token is a row of 128 bytes in both boxes; swizzling stays within it
-                uint8_t* row = smem + s * L::kStage + (h * 32 + lane) * 128;
+            for (int h = 0; h < 2; ++h) {
+              uint8_t* row = smem + s * L::kStage + (h * 32 + lane) * 128;
+              uint32_t any = 0;
+#pragma unroll
+              for (int c = 0; c < 8; ++c) {
+                const uint4 q = *reinterpret_cast<const uint4*>(row + L::kABytes + (c ^ (lane & 7)) * 16);
+                any |= q.x | q.y | q.z | q.w;
+              }
+              if (any == 0) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                   const int at = (c ^ (lane & 7)) * 16;
@@ -455,6 +453,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                   *reinterpret_cast<uint4*>(row + 8192 + at) = make_uint4(0, 0, 0, 0);
                 }
               }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
