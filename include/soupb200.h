@@ -197,8 +197,10 @@ int soup_qk_norm_rope_bwd(const void* dq_out, const void* q, void* dq, const voi
  * state (soup_multi_lora_state_bytes, the caller's) holds the rank products and is what
  * the backward needs of the forward.
  * soup_multi_lora_bwd: dx [tokens, k] bf16, da and db (fp32 or bf16, laid out as lora_a
- * and lora_b; rows of adapters without tokens are 0), each where not NULL; x is read
- * for da alone. workspace for dx or da. Bitwise reproducible. */
+ * and lora_b, 16-byte aligned; rows of adapters without tokens are 0), each where not
+ * NULL; x is read for da alone. workspace for dx or da. Bitwise reproducible. What the
+ * rows of tokens without an adapter hold reaches no da or db; factors have to be finite,
+ * since 64 columns of adapters share a product. */
 size_t soup_multi_lora_state_bytes(int64_t tokens, int64_t adapters, int64_t rank);
 int soup_multi_lora_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* bias,
                         const void* lora_a, const void* lora_b, const float* scales, const void* ids, int ids_64,

@@ -57,6 +57,19 @@ def test_masked_rows_that_are_not_finite_reach_no_gradient(t, per, what):
         ref.check(name, pick(got), tuple(pick(v) for v in whole) if isinstance(whole, tuple) else pick(whole))
 
 
+@pytest.mark.parametrize("t,k,n,na,r", [(1, 8, 8, 1, 8), (17, 8, 24, 2, 4), (130, 16, 8, 8, 1), (300, 8, 8, 3, 8),
+                                        (257, 24, 40, 1, 64), (600, 8, 264, 40, 1)])
+def test_smallest_widths_and_ranks(t, k, n, na, r):
+    x, w, a, b, scale, dy = _lora(t, k, n, na, r, t + k)
+    ids = torch.arange(t, device=DEV) % (na + 1) - 1
+    leaves = [v.requires_grad_(True) for v in (x, a, b)]
+    y = kernels.multi_lora_linear(x, w, a, b, ids, scale)
+    grads = torch.autograd.grad(y, leaves, dy)
+    want = ref.multi_lora(x, w, a, b, ids, scale, None, dy)
+    for name, got in zip(("y", "dx", "da", "db"), (y, *grads)):
+        ref.check(name, got, want[name])
+
+
 @pytest.mark.parametrize("t", [8, 200, 1200])
 def test_bias_and_rows_at_any_address(t):
     k, n = 136, 9344 if t == 200 else 200
