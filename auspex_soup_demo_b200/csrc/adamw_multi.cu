@@ -38,7 +38,8 @@ constexpr int kBlock = 256;              // elements that share a scale
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kE4m3Max = 448.f;
-constexpr float kMostV = 3.3e38f;        // second moments past 32 bits stay at their end
+constexpr float kMostV = 3.3e38f;        // second moments past 32 bits stay at their end,
+constexpr float kMostRoot = 1.8e19f;     // with roots from here on
 
 struct Tensor {
   void* p;
@@ -197,11 +198,14 @@ __device__ __forceinline__ uint64_t root_pair(uint64_t x) {
 
 // Scale of the warp's block and its codes. Values that are not finite are left out of
 // the maximum (they must not wipe out the other 255): fmaxf passes NaN over, and a
-// maximum that is infinite, which no sound step has, is taken again without them. The
-// bits of numbers of 0 or more order as the numbers do, so one integer reduction of the
-// warp gives the maximum.
+// maximum that is infinite, which no sound step has, is taken again without them. Roots
+// are of moments that were held below kMostV, NaN too: beside a root that large, which no
+// sound step has either, those whose first moment is not finite become NaN and are left
+// out. (As a number it would be the block's largest, and the other 255 its smallest code,
+// beside which their steps are nothing.) The bits of numbers of 0 or more order as the
+// numbers do, so one integer reduction of the warp gives the maximum.
 template <bool ROOT>
-__device__ __forceinline__ uint2 to_codes(const uint64_t (&f)[4], float& scale) {
+__device__ __forceinline__ uint2 to_codes(uint64_t (&f)[4], const uint64_t (&first)[4], float& scale) {
   float v[8], top = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -209,7 +213,17 @@ __device__ __forceinline__ uint2 to_codes(const uint64_t (&f)[4], float& scale) 
     top = fmaxf(top, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
   }
   top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-  if (top > 3.4028235e38f) {  // warp-uniform
+  if (top >= (ROOT ? kMostRoot : __int_as_float(0x7f800000))) {  // warp-uniform
+    if constexpr (ROOT) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float lo, hi;
+        f2_unpack(first[i], lo, hi);
+        if (!(fabsf(lo) <= 3.4028235e38f)) v[2 * i] = __int_as_float(0x7fffffff);
+        if (!(fabsf(hi) <= 3.4028235e38f)) v[2 * i + 1] = __int_as_float(0x7fffffff);
+        f[i] = f2_pack(v[2 * i], v[2 * i + 1]);
+      }
+    }
     top = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]) <= 3.4028235e38f ? fabsf(v[i]) : 0.f);
@@ -425,8 +439,8 @@ __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_ke
   }
   if constexpr (EIGHT) {
     float sm, sv;
-    const uint2 cm = to_codes<false>(m, sm);
-    const uint2 cv = to_codes<true>(root, sv);
+    const uint2 cv = to_codes<true>(root, m, sv);
+    const uint2 cm = to_codes<false>(m, m, sm);
     __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.m) + at), cm);
     __stcs(reinterpret_cast<uint2*>(static_cast<uint8_t*>(st.v) + at), cv);
     if (lane == 0) {

@@ -1,0 +1,69 @@
+"""GPU: calls of the operators of a step with several adapters whose outcome their
+documentation promises: gradients that are not finite."""
+
+import math
+
+import pytest
+import torch
+
+from auspex_soup_demo_b200 import _lib
+from auspex_soup_demo_b200.optim import MultiTensorAdamW
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    yield
+    torch.cuda.synchronize()
+    assert _lib.device_error(torch.device("cuda:0")) == 0
+
+
+def _flat(opt):
+    """Parameters aside, what an optimiser holds of its one parameter: bytes of m and v, scales."""
+    st = opt.flat_state()
+    out = {k: st[k].view(torch.uint8).view(-1) if opt.state_bits == 8 else st[k].view(-1) for k in ("m", "v")}
+    return out, {k: st[k] for k in ("m_scale", "v_scale") if k in st}
+
+
+@pytest.mark.parametrize("what", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("clip", [None, 1.0])
+def test_gradients_that_are_not_finite_leave_their_neighbours(bits, dtype, what, clip):
+    """One step with such gradients, then two sound ones, beside a copy that sees 0 in their
+    places (everywhere, where a norm that is infinite scales all others to 0): every other
+    element's parameter and moments are the copy's, bit for bit, and it moves in each sound
+    step; in 8 bits the blocks' scales are the copy's too."""
+    if clip is not None and math.isnan(what):
+        pytest.skip("a norm that is not a number reaches every element")
+    n, bad = 600, [3, 300, 301, 599]
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    keep[bad] = False
+    g = torch.Generator(device=DEV).manual_seed(3)
+    start = (0.05 * torch.randn(n, generator=g, device=DEV)).to(dtype)
+    ps = [torch.nn.Parameter(start.clone()) for _ in range(2)]
+    opts = [MultiTensorAdamW([p], lr=1e-2, state_bits=bits, max_grad_norm=clip) for p in ps]
+    for step in range(3):
+        grad = (1.0 + 0.1 * torch.randn(n, generator=g, device=DEV)).to(dtype)
+        grad[bad] = 0.0
+        before = ps[0].detach().clone()
+        for p, o, first in zip(ps, opts, (True, False)):
+            p.grad = grad.clone()
+            if step == 0 and first:
+                p.grad[bad] = what
+            elif step == 0 and clip is not None:
+                p.grad.zero_()
+            o.step()
+        assert torch.equal(ps[0].detach()[keep], ps[1].detach()[keep])
+        assert not torch.isfinite(ps[0].detach()[~keep]).any()
+        (states, scales), (states2, scales2) = map(_flat, opts)
+        for k, s in states.items():
+            assert torch.equal(s[:n][keep], states2[k][:n][keep]), (step, k)
+            assert not s[n:].any()
+        for k, s in scales.items():
+            assert torch.equal(s, scales2[k]), (step, k)
+        if step > 0:
+            # gradients within a few tenths of 1 move an element by about lr
+            assert float((ps[0].detach() - before).abs()[keep].min()) >= 2e-3, step
