@@ -8,6 +8,7 @@ for the tensor's device.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 import threading
@@ -71,6 +72,7 @@ _SIGNATURES = {
     "soup_qk_norm_rope_bwd_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64, c_i64]),
     "soup_qk_norm_rope_bwd": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                       c_vp, c_vp, c_sz, c_vp]),
+    "soup_tensor_addresses": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, ctypes.POINTER(c_int)]),
     "soup_grad_square_workspace_bytes": (c_sz, [c_i64]),
     "soup_grad_square": (c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_sz, ctypes.POINTER(c_int), c_vp]),
     "soup_adamw_multi": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_d, c_d,
@@ -293,6 +295,44 @@ def set_stream_k(enabled: bool) -> None:
 
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+_table_reader = None
+
+
+def _reader():
+    """(soup_tensor_addresses bound with the interpreter's lock held, the function that
+    fills a DLPack table from a torch tensor)"""
+    global _table_reader
+    if _table_reader is None:
+        lib()  # built and loadable
+        fn = ctypes.PyDLL(LIB_PATH).soup_tensor_addresses
+        fn.restype, fn.argtypes = _SIGNATURES["soup_tensor_addresses"]
+        capsule = ctypes.pythonapi.PyCapsule_GetPointer
+        capsule.restype, capsule.argtypes = c_vp, [ctypes.py_object, ctypes.c_char_p]
+        api = capsule(torch.Tensor.__dlpack_c_exchange_api__, b"dlpack_exchange_api")
+        # DLPackExchangeAPI: version (two 32-bit numbers), an older interface, then five
+        # functions, of which the fourth fills a DLTensor that does not own anything
+        major = ctypes.cast(api, ctypes.POINTER(ctypes.c_uint32))[0]
+        read = ctypes.cast(api + 16, ctypes.POINTER(c_vp))[3]
+        if major != 1 or not read:
+            raise SoupLibraryError(f"torch's DLPack exchange interface has version {major} or cannot fill a DLTensor")
+        _table_reader = fn, read
+    return _table_reader
+
+
+def tensor_addresses(tensors, sizes: array.array, code: int, device: torch.device):
+    """The addresses (array of uint64) of tensors of these sizes (array of int64): dense, of
+    one type (its code) and on one device; or the index of the first that is not so. One
+    call for all of them: asking each of hundreds of tensors for its size, type, device
+    and layout from Python costs a step more than its kernels."""
+    fn, read = _reader()
+    objects = array.array("Q", map(id, tensors))
+    out, bad = array.array("Q", objects), c_int(0)
+    check("soup_tensor_addresses", fn(
+        read, objects.buffer_info()[0], sizes.buffer_info()[0], len(objects), code, 2 if device.type == "cuda" else 1,
+        device.index or 0, out.buffer_info()[0], ctypes.byref(bad)))
+    return out if bad.value < 0 else bad.value
 
 
 def dense(t: torch.Tensor) -> torch.Tensor:

@@ -458,6 +458,33 @@ __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_ke
   }
 }
 
+// What a DLPack exchange interface fills in for a tensor (DLTensor of DLPack 1).
+struct DlTensor {
+  void* data;
+  int32_t device_type, device;
+  int32_t ndim;
+  uint8_t type_code, type_bits;
+  uint16_t lanes;
+  const int64_t* shape;
+  const int64_t* strides;
+  uint64_t byte_offset;
+};
+constexpr int kDlFloat = 2, kDlBfloat = 4;
+
+// t is dense in the order of its axes and has n elements of that type on that device.
+bool dense_tensor(const DlTensor& t, int64_t n, int dtype, int device_type, int device) {
+  if (t.device_type != device_type || t.device != device || t.lanes != 1 ||
+      t.type_code != (dtype == SOUP_BF16 ? kDlBfloat : kDlFloat) || t.type_bits != (dtype == SOUP_F32 ? 32 : 16))
+    return false;
+  int64_t e = 1;
+  bool dense = true;
+  for (int d = t.ndim - 1; d >= 0; --d) {
+    if (t.shape[d] != 1 && t.strides && t.strides[d] != e) dense = false;
+    e *= t.shape[d];
+  }
+  return dense && e == n && t.data;
+}
+
 constexpr int kSquareCtas = 12;             // of grad_square_kernel on an SM, each with a partial sum
 constexpr int kSmall = 64, kLarge = 960;  // tensors of a launch: arguments of 2 and 30 KB
 
@@ -584,6 +611,26 @@ int step_run(const Args& a, const States& s, const Hyper& h, const Coefs* coefs,
 using namespace soup;
 
 extern "C" {
+
+int soup_tensor_addresses(const void* read, const uint64_t* objects, const int64_t* sizes, int count, int dtype,
+                          int device_type, int device, uint64_t* addresses, int* bad) {
+  if (!read || !objects || !sizes || count <= 0 || !addresses || !bad ||
+      (dtype != SOUP_F32 && dtype != SOUP_BF16 && dtype != SOUP_F16)) {
+    set_last_error("soup_tensor_addresses: bad arguments");
+    return SOUP_ERR_INVALID;
+  }
+  const auto fill = reinterpret_cast<int (*)(void*, DlTensor*)>(const_cast<void*>(read));
+  for (int i = 0; i < count; ++i) {
+    DlTensor t{};
+    if (fill(reinterpret_cast<void*>(objects[i]), &t) != 0 || !dense_tensor(t, sizes[i], dtype, device_type, device)) {
+      *bad = i;
+      return SOUP_OK;
+    }
+    addresses[i] = reinterpret_cast<uint64_t>(t.data) + t.byte_offset;
+  }
+  *bad = -1;
+  return SOUP_OK;
+}
 
 size_t soup_grad_square_workspace_bytes(int64_t tensors) {
   if (tensors <= 0) return 0;

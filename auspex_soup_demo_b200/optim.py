@@ -26,12 +26,22 @@ from . import _lib
 STATE_BLOCK = 256
 
 
-_grad, _dtype = operator.attrgetter("grad"), operator.attrgetter("dtype")
-_data_ptr, _is_contiguous, _get_device = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.get_device
+_grad = operator.attrgetter("grad")
 
 
 def _address(a: array.array) -> int:
     return a.buffer_info()[0]
+
+
+def _addresses(tensors, sizes, code: int, device):
+    """Addresses of tensors that are as a launch needs them, or None."""
+    try:
+        out = _lib.tensor_addresses(tensors, sizes, code, device)
+    except (_lib.SoupError, _lib.SoupLibraryError):
+        raise
+    except Exception:  # a tensor without an address, say a sparse one
+        return None
+    return None if isinstance(out, int) else out
 
 
 class _Held:
@@ -198,25 +208,28 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         type's parameters that have a gradient; the gradients are kept until the launch."""
         out = []
         for code, dtype, params, sizes, blocks in held.by_dtype:
-            # map over C methods: a step of hundreds of tensors is bound by these loops
             grads = list(map(_grad, params))
-            try:
-                grad_ptrs = array.array("Q", map(_data_ptr, grads))
-            except TypeError:  # parameters without a gradient
+            if any(g is None for g in grads):
                 keep = [i for i, g in enumerate(grads) if g is not None]
                 if not keep:
                     continue
                 params, grads = [params[i] for i in keep], [grads[i] for i in keep]
                 sizes, blocks = (array.array(t.typecode, [t[i] for i in keep]) for t in (sizes, blocks))
-                grad_ptrs = array.array("Q", map(_data_ptr, grads))
-            if not all(map(_is_contiguous, grads)):
+            # p.data = ... gives a parameter other memory, under a gradient that stays
+            grad_ptrs = _addresses(grads, sizes, code, device)
+            if grad_ptrs is None:
                 if any(g.layout is not torch.strided for g in grads):
                     raise ValueError("MultiTensorAdamW: gradients must be dense")
+                if any(g.dtype != dtype or g.device != device or g.numel() != n for g, n in zip(grads, sizes)):
+                    raise ValueError(f"MultiTensorAdamW: gradients must be {dtype} on {device} and of their parameters' "
+                                     "sizes")
                 grads = [g.detach().contiguous() for g in grads]
-                grad_ptrs = array.array("Q", map(_data_ptr, grads))
-            if set(map(_dtype, grads)) != {dtype} or set(map(_get_device, grads)) != {device.index}:
-                raise ValueError(f"MultiTensorAdamW: gradients must be {dtype} on {device}, as their parameters")
-            out.append((code, array.array("Q", map(_data_ptr, params)), grad_ptrs, sizes, blocks, grads))
+                grad_ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
+            ptrs = _addresses(params, sizes, code, device)
+            if ptrs is None:
+                raise ValueError(f"MultiTensorAdamW: parameters must stay {dtype} on {device}, contiguous and of the "
+                                 "sizes that the optimiser was made with")
+            out.append((code, ptrs, grad_ptrs, sizes, blocks, grads))
         return out
 
     def step(self, closure=None):

@@ -1,0 +1,91 @@
+"""CPU: what the operators of a step with several adapters check of tensors that changed
+between two calls."""
+
+import array
+import ctypes
+
+import pytest
+import torch
+
+from auspex_soup_demo_b200 import _lib, optim
+
+
+# --------------------------------------------------- tensors of an optimiser's step ----
+def _sizes(*n):
+    return array.array("q", n)
+
+
+def test_addresses_of_many_tensors():
+    """The compiled table of addresses against each tensor's own answers."""
+    cpu = torch.device("cpu")
+    base = torch.zeros(5000)
+    good = [base, base[3:50], torch.zeros(4, 5, 6), torch.zeros(7, 1, 3).expand(7, 1, 3), torch.zeros(()),
+            torch.nn.Parameter(torch.zeros(2, 2)), torch.zeros(4, 8, 2).transpose(0, 0), torch.zeros(6, 1).t()]
+    out = _lib.tensor_addresses(good, _sizes(*[t.numel() for t in good]), _lib.F32, cpu)
+    assert out.tolist() == [t.data_ptr() for t in good]
+    for dtype, code in ((torch.float16, _lib.F16), (torch.bfloat16, _lib.BF16)):
+        t = torch.zeros(9, dtype=dtype)
+        assert _lib.tensor_addresses([t], _sizes(9), code, cpu).tolist() == [t.data_ptr()]
+    for other in (torch.zeros(9), torch.zeros(11), torch.zeros(20)[::2], torch.zeros(5, 2).t(), torch.zeros(1).expand(10),
+                  torch.zeros(10, dtype=torch.bfloat16), torch.zeros(10, dtype=torch.float64),
+                  torch.zeros(10, dtype=torch.int32), torch.zeros(0)):
+        assert _lib.tensor_addresses([good[0], other], _sizes(5000, 10), _lib.F32, cpu) == 1, other
+    assert _lib.tensor_addresses([torch.zeros(9, dtype=torch.float16)], _sizes(9), _lib.BF16, cpu) == 0
+    # expected on a GPU, found on the host
+    assert _lib.tensor_addresses([base], _sizes(5000), _lib.F32, torch.device("cuda", 0)) == 0
+    with pytest.raises(Exception):
+        _lib.tensor_addresses([torch.zeros(3, 3).to_sparse()], _sizes(9), _lib.F32, cpu)
+
+
+def test_addresses_c_arguments():
+    lib, p, bad = _lib.lib(), ctypes.c_void_p(16), ctypes.c_int(0)
+    # never followed: validation fails first
+    for args in ((None, p, p, 1, 0, 1, 0, p), (p, None, p, 1, 0, 1, 0, p), (p, p, None, 1, 0, 1, 0, p),
+                 (p, p, p, 0, 0, 1, 0, p), (p, p, p, 1, 7, 1, 0, p), (p, p, p, 1, 0, 1, 0, None)):
+        assert lib.soup_tensor_addresses(*args, ctypes.byref(bad)) == _lib.SOUP_ERR_INVALID
+
+
+def _held(params):
+    h = optim._Held()
+    h.params, h.sizes = params, [p.numel() for p in params]
+    h.by_dtype = [(_lib.F32, torch.float32, params, _sizes(*h.sizes), array.array("i", range(len(params))))]
+    return h
+
+
+@pytest.mark.parametrize("change", [lambda p: torch.zeros(4), lambda p: torch.zeros(40), lambda p: torch.zeros(4, 2).t(),
+                                    lambda p: torch.zeros(2, 4, dtype=torch.bfloat16), lambda p: p[:, ::2],
+                                    lambda p: torch.zeros(2, 4).to_sparse()])
+def test_parameters_given_other_memory_are_refused(change):
+    """p.data = ... under a gradient that stays: nothing is launched over the old sizes."""
+    opt = object.__new__(optim.MultiTensorAdamW)
+    ps = [torch.nn.Parameter(torch.zeros(2, 4)) for _ in range(3)]
+    for p in ps:
+        p.grad = torch.ones(2, 4)
+    held, cpu = _held(ps), torch.device("cpu")
+    (_, addresses, grads, sizes, _, _), = opt._tables(held, cpu)
+    assert addresses.tolist() == [p.data_ptr() for p in ps] and grads.tolist() == [p.grad.data_ptr() for p in ps]
+    new = change(torch.zeros(2, 8))
+    try:
+        ps[1].data = new
+    except (RuntimeError, NotImplementedError, TypeError):
+        pytest.skip("torch refuses that itself")
+    with pytest.raises(ValueError, match="parameters must stay"):
+        opt._tables(held, cpu)
+    ps[1].grad = None  # then it has no part in the step
+    (_, addresses, _, sizes, _, _), = opt._tables(held, cpu)
+    assert addresses.tolist() == [ps[0].data_ptr(), ps[2].data_ptr()] and sizes.tolist() == [8, 8]
+
+
+def test_gradients_of_another_size_are_refused():
+    opt = object.__new__(optim.MultiTensorAdamW)
+    p = torch.nn.Parameter(torch.zeros(2, 4))
+    held = _held([p])
+    p.data = torch.zeros(4)
+    p.grad = torch.ones(4)
+    p.data = torch.zeros(2, 4)
+    with pytest.raises(ValueError, match="gradients must be"):
+        opt._tables(held, torch.device("cpu"))
+    p.grad = None
+    p.grad = torch.ones(4, 2).t()  # another order: copied
+    (_, _, grads, _, _, kept), = opt._tables(held, torch.device("cpu"))
+    assert kept[0].is_contiguous() and grads[0] == kept[0].data_ptr()

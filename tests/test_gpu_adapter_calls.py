@@ -1,5 +1,6 @@
 """GPU: calls of the operators of a step with several adapters whose outcome their
-documentation promises: gradients that are not finite."""
+documentation promises: gradients that are not finite, parameters that were given other
+memory."""
 
 import math
 
@@ -67,3 +68,24 @@ def test_gradients_that_are_not_finite_leave_their_neighbours(bits, dtype, what,
         if step > 0:
             # gradients within a few tenths of 1 move an element by about lr
             assert float((ps[0].detach() - before).abs()[keep].min()) >= 2e-3, step
+
+
+@pytest.mark.parametrize("change", [lambda p: p[:4].clone(), lambda p: p.cpu(), lambda p: p.bfloat16(),
+                                    lambda p: p.view(4, 2).t()])
+def test_parameters_given_other_memory_are_refused(change):
+    """Another size, place, type or layout under a gradient that stays; before anything is written."""
+    ps = [torch.nn.Parameter(torch.ones(8, device=DEV)) for _ in range(3)]
+    opt = MultiTensorAdamW(ps, lr=1e-2, max_grad_norm=1.0)
+    for p in ps:
+        p.grad = torch.ones(8, device=DEV)
+    opt.step()
+    before = [p.detach().clone() for p in ps]
+    old = ps[1].data
+    ps[1].data = change(ps[1].data)
+    with pytest.raises(ValueError, match="parameters must stay"):
+        opt.step()
+    assert torch.equal(ps[0], before[0]) and torch.equal(ps[2], before[2]) and torch.equal(old, before[1])
+    assert float(opt.flat_state()["step"]) == 1.0
+    ps[1].data = torch.zeros(8, device=DEV)  # other memory of the same form is the parameter's
+    opt.step()
+    assert ps[1].detach().all() and float(opt.flat_state()["step"]) == 2.0
