@@ -71,8 +71,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
     ``torch.optim.AdamW`` (every element, where the norm is clipped).
 
     The optimiser's steps share their workspace and states: steps of one optimiser
-    on several streams have to be ordered by the caller. Autograd does not see a
-    step's writes: a backward pass that needs the old values has to come before it.
+    on several streams have to be ordered by the caller. A backward pass that needs the
+    values before a step has to come before it; after it, it raises.
     """
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -204,8 +204,9 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     # -- step -------------------------------------------------------------------
     def _tables(self, held: _Held, device):
-        """(dtype code, parameter addresses, gradient addresses, sizes, blocks, gradients) of each
-        type's parameters that have a gradient; the gradients are kept until the launch."""
+        """(dtype code, parameter addresses, gradient addresses, sizes, blocks, gradients,
+        parameters) of each type's parameters that have a gradient; the gradients are kept until
+        the launch."""
         out = []
         for code, dtype, params, sizes, blocks in held.by_dtype:
             grads = list(map(_grad, params))
@@ -216,20 +217,22 @@ class MultiTensorAdamW(torch.optim.Optimizer):
                 params, grads = [params[i] for i in keep], [grads[i] for i in keep]
                 sizes, blocks = (array.array(t.typecode, [t[i] for i in keep]) for t in (sizes, blocks))
             # p.data = ... gives a parameter other memory, under a gradient that stays
-            grad_ptrs = _addresses(grads, sizes, code, device)
-            if grad_ptrs is None:
+            both = _addresses(grads + params, sizes + sizes, code, device)
+            if both is not None:
+                grad_ptrs, ptrs = both[:len(grads)], both[len(grads):]
+            else:
                 if any(g.layout is not torch.strided for g in grads):
                     raise ValueError("MultiTensorAdamW: gradients must be dense")
                 if any(g.dtype != dtype or g.device != device or g.numel() != n for g, n in zip(grads, sizes)):
                     raise ValueError(f"MultiTensorAdamW: gradients must be {dtype} on {device} and of their parameters' "
                                      "sizes")
+                ptrs = _addresses(params, sizes, code, device)
+                if ptrs is None:
+                    raise ValueError(f"MultiTensorAdamW: parameters must stay {dtype} on {device}, contiguous and of the "
+                                     "sizes that the optimiser was made with")
                 grads = [g.detach().contiguous() for g in grads]
                 grad_ptrs = array.array("Q", map(torch.Tensor.data_ptr, grads))
-            ptrs = _addresses(params, sizes, code, device)
-            if ptrs is None:
-                raise ValueError(f"MultiTensorAdamW: parameters must stay {dtype} on {device}, contiguous and of the "
-                                 "sizes that the optimiser was made with")
-            out.append((code, ptrs, grad_ptrs, sizes, blocks, grads))
+            out.append((code, ptrs, grad_ptrs, sizes, blocks, grads, params))
         return out
 
     def step(self, closure=None):
@@ -250,14 +253,15 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         squares = None
         if self.max_grad_norm is not None:
             squares, nbytes = self._squares[-1].data_ptr(), self._squares[-1].numel()
-            for code, _, g, sizes, _, _ in itertools.chain.from_iterable(tables):
+            for code, _, g, sizes, *_ in itertools.chain.from_iterable(tables):
                 _lib.call("soup_grad_square", dev, _address(g), _address(sizes), len(g), code, squares,
                           nbytes, ctypes.byref(partials), stream)
         done = 0
         for group, held, table in zip(self.param_groups, self._held, tables):
             b1, b2 = group["betas"]
-            for code, p, g, sizes, blocks, _ in table:
+            for code, p, g, sizes, blocks, _, params in table:
                 done += 1
+                torch.autograd.graph.increment_version(params)  # autograd sees no other sign of the writes
                 _lib.call("soup_adamw_multi", dev, _address(p), _address(g), _address(sizes), _address(blocks), len(p),
                           code, self.state_bits, held.m.data_ptr(), held.v.data_ptr(), _lib.ptr(held.m_scale),
                           _lib.ptr(held.v_scale), group["lr"], b1, b2, group["eps"], group["weight_decay"],

@@ -62,7 +62,7 @@ def test_parameters_given_other_memory_are_refused(change):
     for p in ps:
         p.grad = torch.ones(2, 4)
     held, cpu = _held(ps), torch.device("cpu")
-    (_, addresses, grads, sizes, _, _), = opt._tables(held, cpu)
+    (_, addresses, grads, sizes, *_), = opt._tables(held, cpu)
     assert addresses.tolist() == [p.data_ptr() for p in ps] and grads.tolist() == [p.grad.data_ptr() for p in ps]
     new = change(torch.zeros(2, 8))
     try:
@@ -72,7 +72,7 @@ def test_parameters_given_other_memory_are_refused(change):
     with pytest.raises(ValueError, match="parameters must stay"):
         opt._tables(held, cpu)
     ps[1].grad = None  # then it has no part in the step
-    (_, addresses, _, sizes, _, _), = opt._tables(held, cpu)
+    (_, addresses, _, sizes, *_), = opt._tables(held, cpu)
     assert addresses.tolist() == [ps[0].data_ptr(), ps[2].data_ptr()] and sizes.tolist() == [8, 8]
 
 
@@ -87,5 +87,5 @@ def test_gradients_of_another_size_are_refused():
         opt._tables(held, torch.device("cpu"))
     p.grad = None
     p.grad = torch.ones(4, 2).t()  # another order: copied
-    (_, _, grads, _, _, kept), = opt._tables(held, torch.device("cpu"))
+    (_, _, grads, _, _, kept, *_), = opt._tables(held, torch.device("cpu"))
     assert kept[0].is_contiguous() and grads[0] == kept[0].data_ptr()

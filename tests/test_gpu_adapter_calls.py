@@ -89,3 +89,17 @@ def test_parameters_given_other_memory_are_refused(change):
     ps[1].data = torch.zeros(8, device=DEV)  # other memory of the same form is the parameter's
     opt.step()
     assert ps[1].detach().all() and float(opt.flat_state()["step"]) == 2.0
+
+
+def test_steps_are_seen_by_autograd():
+    """A backward pass that needs the values before a step raises, as after torch's optimisers."""
+    w = torch.nn.Parameter(torch.ones(300, device=DEV))
+    unused = torch.nn.Parameter(torch.ones(8, device=DEV))
+    loss = (w * w).sum()
+    opt = MultiTensorAdamW([w, unused], lr=1e-2)
+    w.grad = torch.ones_like(w)
+    versions = w._version, unused._version
+    opt.step()
+    assert w._version > versions[0] and unused._version == versions[1]  # no gradient: not written
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
