@@ -186,14 +186,26 @@ __device__ __forceinline__ float recip_approx(float x) {
 }
 
 // Square roots of a pair of finite numbers, rounded as exact ones are but for rare last bits:
-// one Newton step s + (x - s^2) / (2 sqrt(x)) from x times the approximate reciprocal root
-// (of x + 2^-126, which leaves 0 its root and numbers above 2^-102 as they are).
+// one step of Newton's method, s + (x - s^2) / (2 sqrt(x)), from x times the approximate
+// reciprocal root (of x + 2^-126, which leaves 0 its root and numbers above 2^-102 as they
+// are; roots of smaller ones come out low, by kRootError at most).
+constexpr double kRootError = 2.1e-20;
 __device__ __forceinline__ uint64_t root_pair(uint64_t x) {
   float lo, hi;
   f2_unpack(f2_add(x, f2_same(1.17549435e-38f)), lo, hi);
   const uint64_t h = f2_pack(recip_root_approx(lo), recip_root_approx(hi));
   const uint64_t s = f2_mul(x, h);
   return f2_fma(f2_fma(s, s, f2_mul(x, f2_same(-1.f))), f2_mul(h, f2_same(-0.5f)), s);
+}
+
+// The same of every number: those below 2^-100 are scaled up by 2^64 first.
+__device__ __forceinline__ uint64_t root_pair_tiny(uint64_t x) {
+  constexpr float kLeast = 7.8886091e-31f;
+  float lo, hi, r0, r1, s0, s1;
+  f2_unpack(x, lo, hi);
+  f2_unpack(root_pair(x), r0, r1);
+  f2_unpack(f2_mul(root_pair(f2_mul(x, f2_same(1.8446744e19f))), f2_same(2.3283064e-10f)), s0, s1);
+  return f2_pack(lo < kLeast ? s0 : r0, hi < kLeast ? s1 : r1);
 }
 
 // Scale of the warp's block and its codes. Values that are not finite are left out of
@@ -361,8 +373,10 @@ __global__ void __launch_bounds__(kThreads) adamw_coef_kernel(double lr, double 
   if (raise) *step = (float)t;
 }
 
-// The step: a warp a block.
-template <typename T, bool EIGHT, int N>
+// The step: a warp a block. TINY: eps is so small that roots of second moments below
+// 2^-102 count beside it (see step_run). As a branch for each pair of elements it took the
+// other steps 24 of 418 us.
+template <typename T, bool EIGHT, bool TINY, int N>
 __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_kernel(const __grid_constant__ Table<N> tab,
                                                                                  States st, Hyper h,
                                                                                  const Coefs* __restrict__ coefs) {
@@ -417,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, step_ctas(sizeof(T))) adamw_multi_ke
     float lo, hi;
     f2_unpack(f2_fma(f2_mul(v[i], b2), one, f2_mul(c2, f2_mul(gi, gi))), lo, hi);
     v[i] = f2_pack(fminf(lo, kMostV), fminf(hi, kMostV));
-    root[i] = root_pair(v[i]);
+    root[i] = TINY ? root_pair_tiny(v[i]) : root_pair(v[i]);
     f2_unpack(f2_fma(root[i], root_scale, eps), lo, hi);
     const uint64_t inv = f2_pack(recip_approx(lo), recip_approx(hi));
     p.set(i, f2_fma(f2_mul(m[i], step_size), inv, f2_mul(p.pair(i), decay)));
@@ -554,12 +568,12 @@ int square_launch(const Args& a, int i0, int i1, double* partial, int* used, cud
   return launch_table(grad_square_kernel<T, N>, grid, st, tab, partial);
 }
 
-template <typename T, bool EIGHT, int N>
+template <typename T, bool EIGHT, bool TINY, int N>
 int step_launch(const Args& a, int i0, int i1, const States& s, const Hyper& h, const Coefs* coefs, cudaStream_t st) {
   Table<N> tab;
   fill_table(tab, a, i0, i1);
   const int grid = (tab.blocks + kWarps - 1) / kWarps;
-  return launch_table(adamw_multi_kernel<T, EIGHT, N>, grid, st, tab, s, h, coefs);
+  return launch_table(adamw_multi_kernel<T, EIGHT, TINY, N>, grid, st, tab, s, h, coefs);
 }
 
 int check_tensors(const char* fn, const Args& a, bool step) {
@@ -592,17 +606,27 @@ int square_run(const Args& a, double* partial, int cap, int* used, cudaStream_t 
   return SOUP_OK;
 }
 
-template <typename T, bool EIGHT>
+template <typename T, bool EIGHT, bool TINY>
 int step_run(const Args& a, const States& s, const Hyper& h, const Coefs* coefs, cudaStream_t st) {
   const int most = a.count <= kSmall ? kSmall : kLarge;
   for (int i0 = 0; i0 < a.count;) {
     const int i1 = launch_end(a, i0, most);
-    const int rc = most == kSmall ? step_launch<T, EIGHT, kSmall>(a, i0, i1, s, h, coefs, st)
-                                  : step_launch<T, EIGHT, kLarge>(a, i0, i1, s, h, coefs, st);
+    const int rc = most == kSmall ? step_launch<T, EIGHT, TINY, kSmall>(a, i0, i1, s, h, coefs, st)
+                                  : step_launch<T, EIGHT, TINY, kLarge>(a, i0, i1, s, h, coefs, st);
     if (rc) return rc;
     i0 = i1;
   }
   return SOUP_OK;
+}
+
+// Below 2^-102 root_pair's roots are low by kRootError at most, times 1 / sqrt(1 - b2) in the
+// denominator: less than a rounding of eps where eps is larger than this (1e-11 for b2 of
+// 0.999). Steps with a smaller eps take the roots of every number (442 us for 233 M bf16
+// elements, 418 without).
+template <typename T, bool EIGHT>
+int step_run(const Args& a, const States& s, const Hyper& h, double beta2, const Coefs* coefs, cudaStream_t st) {
+  const bool tiny = h.eps * 5.9604645e-8 < kRootError / sqrt(1.0 - beta2);
+  return tiny ? step_run<T, EIGHT, true>(a, s, h, coefs, st) : step_run<T, EIGHT, false>(a, s, h, coefs, st);
 }
 
 }  // namespace
@@ -679,7 +703,8 @@ int soup_adamw_multi(void* const* params, const void* const* grads, const int64_
                                       max_norm, static_cast<const double*>(grad_squares), partials, norm_out, step,
                                       last, co)))
     return rc;
-#define RUN(T) return state_bits == 8 ? step_run<T, true>(a, s, h, co, st) : step_run<T, false>(a, s, h, co, st)
+#define RUN(T) \
+  return state_bits == 8 ? step_run<T, true>(a, s, h, beta2, co, st) : step_run<T, false>(a, s, h, beta2, co, st)
   if (dtype == SOUP_F32) RUN(float);
   if (dtype == SOUP_BF16) RUN(__nv_bfloat16);
   RUN(__half);

@@ -1,12 +1,13 @@
 """GPU: calls of the operators of a step with several adapters whose outcome their
-documentation promises: gradients that are not finite, parameters that were given other
-memory."""
+documentation promises: gradients that are not finite, second moments near the smallest
+numbers, parameters that were given other memory."""
 
 import math
 
 import pytest
 import torch
 
+import adapter_step_reference as ref
 from auspex_soup_demo_b200 import _lib
 from auspex_soup_demo_b200.optim import MultiTensorAdamW
 
@@ -103,3 +104,36 @@ def test_steps_are_seen_by_autograd():
     assert w._version > versions[0] and unused._version == versions[1]  # no gradient: not written
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("eps", [1e-8, 4e-12, 3e-12, 1e-26])
+def test_second_moments_near_the_smallest_numbers(bits, eps):
+    """Gradients of 1e-21 to 1e-16, whose second moments are subnormal or close to it, and an
+    eps that is larger or smaller than their roots, against 64 bits: each of v's four
+    operations rounds by 2^-24 of its result or by 2^-150, half of the smallest number; the
+    rest are a dozen roundings of the update. Beside an eps of 3.5e-12 or more (for this
+    beta2) roots may be low by 2.1e-20, less than eps' own rounding."""
+    n, lr, betas = 256, 1e-3, (0.9, 0.99)
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = MultiTensorAdamW([p], lr=lr, betas=betas, eps=eps, state_bits=bits)
+    e, tiny = 2.0 ** -24, 2.0 ** -150
+    g = 10.0 ** torch.linspace(-21, -16, n, device=DEV)
+    p.grad = g.clone()
+    opt.step()
+    want, m, v, _ = ref.adamw(torch.zeros_like(g), g, torch.zeros_like(g), torch.zeros_like(g), 1, lr, betas, eps, 0.0)
+    slack = 8 * e * v + 4 * tiny
+    least, most = torch.sqrt((v - slack).clamp_(min=0.0)), torch.sqrt(v + slack)
+    step = lr / (1 - betas[0]) * m
+    small, large = (step / (r / math.sqrt(1 - betas[1]) + eps) for r in (most, least))
+    got = -p.detach().double()
+    assert (got >= (1 - 12 * e) * small).all() and (got <= (1 + 12 * e) * large).all()
+    st = opt.flat_state()
+    if bits == 32:
+        assert ((st["v"].double().view(-1) - v).abs() <= slack).all()
+    else:
+        low = 2.1e-20 if eps > 3.5e-12 else 0.0
+        root, scale = st["v"].float().double().view(-1) * st["v_scale"].double(), float(st["v_scale"])
+        assert abs(scale - float(torch.sqrt(v).max()) / 448) <= 8 * e * scale + low / 448
+        code = (2.0 ** -4 + 4 * e) * most + 2.0 ** -9 * scale  # half a step of 2^-4, or the smallest code
+        assert (root >= least - code - low).all() and (root <= most + code).all()
