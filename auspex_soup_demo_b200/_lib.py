@@ -14,6 +14,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libsoupb200.so")
 
@@ -224,6 +225,18 @@ def once_differentiable(backward):
         return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return run
+
+
+def differentiated(*tensors) -> bool:
+    """Whether a call on these tensors (or None) has to go through its autograd Function: a
+    gradient is wanted, or forward-mode derivatives may be (tangents do not show in
+    requires_grad), which the Function refuses."""
+    if forward_ad._current_level >= 0:
+        return True
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 def call(fn: str, device: torch.device, *args) -> None:

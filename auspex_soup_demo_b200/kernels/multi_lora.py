@@ -197,6 +197,6 @@ def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tenso
         # empty, connected to the states and the factors
         return x.new_zeros(*xs[:-1], n) + (x.sum() + lora_a[:, :0].sum() + lora_b[:0].sum()).to(x.dtype)
     ids = adapter_ids.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or lora_a.requires_grad or lora_b.requires_grad):
+    if _lib.differentiated(x, lora_a, lora_b):
         return MultiLoRAFunction.apply(x, weight, lora_a, lora_b, ids, scaling, bias, per)
     return _forward(x, weight, lora_a, lora_b, ids, scaling, bias, per)[0]

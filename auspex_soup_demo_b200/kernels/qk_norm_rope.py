@@ -189,8 +189,7 @@ def _apply(q, k, qw, kw, eps, a, c, axes):
     q, k = _head_rows(q), _head_rows(k)
     if qw is not None:
         qw, kw = qw.contiguous(), kw.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
-                                    (qw is not None and (qw.requires_grad or kw.requires_grad))):
+    if _lib.differentiated(q, k, qw, kw):
         return QKNormRoPEFunction.apply(q, k, qw, kw, eps, a, c, axes)
     return _forward(q, k, qw, kw, eps, a, c, axes)
 

@@ -1,14 +1,15 @@
 """GPU: calls of the operators of a step with several adapters whose outcome their
 documentation promises: gradients that are not finite, second moments near the smallest
-numbers, parameters that were given other memory."""
+numbers, parameters that were given other memory, tangents."""
 
 import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 import adapter_step_reference as ref
-from auspex_soup_demo_b200 import _lib
+from auspex_soup_demo_b200 import _lib, kernels
 from auspex_soup_demo_b200.optim import MultiTensorAdamW
 
 pytestmark = pytest.mark.gpu
@@ -137,3 +138,25 @@ def test_second_moments_near_the_smallest_numbers(bits, eps):
         assert abs(scale - float(torch.sqrt(v).max()) / 448) <= 8 * e * scale + low / 448
         code = (2.0 ** -4 + 4 * e) * most + 2.0 ** -9 * scale  # half a step of 2^-4, or the smallest code
         assert (root >= least - code - low).all() and (root <= most + code).all()
+
+
+def test_forward_mode_derivatives_are_refused():
+    """As the other operators': a tangent is refused, not dropped."""
+    x, w = torch.randn(10, 64, device=DEV).bfloat16(), torch.randn(32, 64, device=DEV).bfloat16()
+    a, b = torch.randn(2, 8, 64, device=DEV).bfloat16(), torch.randn(32, 2, 8, device=DEV).bfloat16()
+    ids = torch.zeros(10, dtype=torch.int64, device=DEV)
+    q, k = torch.randn(1, 2, 5, 8, device=DEV), torch.randn(1, 1, 5, 8, device=DEV)
+    nw, cos, sin = torch.ones(8, device=DEV), torch.rand(5, 8, device=DEV), torch.rand(5, 8, device=DEV)
+    pos, inv = torch.zeros(1, 5, dtype=torch.int64, device=DEV), torch.rand(4, device=DEV)
+    calls = [(lambda t: kernels.multi_lora_linear(t, w, a, b, ids), x),
+             (lambda t: kernels.multi_lora_linear(x, w, t, b, ids), a),
+             (lambda t: kernels.multi_lora_linear(x, w, a, t, ids), b),
+             (lambda t: kernels.apply_qk_norm_rope(t, k, nw, nw, cos, sin), q),
+             (lambda t: kernels.apply_qk_norm_rope(q, k, nw, t, cos, sin), nw),
+             (lambda t: kernels.apply_multi_axis_rope(q, t, pos, inv, (0,) * 4), k)]
+    for grad in (True, False):
+        for fn, t in calls:
+            with torch.set_grad_enabled(grad), fwad.dual_level():
+                with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
+                    fn(fwad.make_dual(t, torch.ones_like(t)))
+                fn(t)  # no tangent: nothing to refuse
