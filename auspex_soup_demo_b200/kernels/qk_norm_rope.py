@@ -70,6 +70,13 @@ def _head_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _out_like(t: torch.Tensor) -> torch.Tensor:
+    """An output in the order of t's axes, its rows contiguous (rows that overlap, as those of
+    a sliding view do, can have them in another order)."""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _source(a: torch.Tensor, c: torch.Tensor, axes):
     """(table dtype code, source, its three strides, axes) for the C calls: a and c are
     tables [B | 1, S, D] or [S, D], or positions [axes, B | 1, S] or [axes, S] and frequencies."""
@@ -83,7 +90,7 @@ def _source(a: torch.Tensor, c: torch.Tensor, axes):
 
 
 def _forward(q, k, qw, kw, eps, a, c, axes, inverse=0):
-    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    qo, ko = _out_like(q), _out_like(k)
     b, hq, s, d = q.shape
     code = _lib.dtype_code(q.dtype)
     tcode, src, ts, ax = _source(a, c, axes)
@@ -135,7 +142,7 @@ class QKNormRoPEFunction(torch.autograd.Function):
         _, _, need_q, need_k = ctx.needs_input_grad[:4]
         b, hq, s, d = qs
         hk = ks[1]
-        dq, dk = torch.empty_like(q), torch.empty_like(k)
+        dq, dk = _out_like(q), _out_like(k)
         dqw = torch.empty_like(qw) if need_q else None
         dkw = torch.empty_like(kw) if need_k else None
         nbytes, ws = 0, 0

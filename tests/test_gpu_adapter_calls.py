@@ -1,6 +1,7 @@
 """GPU: calls of the operators of a step with several adapters whose outcome their
 documentation promises: gradients that are not finite, second moments near the smallest
-numbers, parameters that were given other memory, tangents."""
+numbers, parameters that were given other memory, tangents, rows that
+overlap."""
 
 import math
 
@@ -160,3 +161,31 @@ def test_forward_mode_derivatives_are_refused():
                 with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward"):
                     fn(fwad.make_dual(t, torch.ones_like(t)))
                 fn(t)  # no tangent: nothing to refuse
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_that_overlap(dtype):
+    """Rows one element apart, and shared by all heads: any strides with a contiguous head dim
+    are allowed. Results and gradients (those of each row by itself) against 64 bits."""
+    b, h, s, d = 2, 3, 5, 8
+    buf = torch.randn(4000, device=DEV).to(dtype)
+    k = torch.randn(b, 1, s, d, device=DEV).to(dtype).requires_grad_(True)
+    w = (1 + torch.rand(d, device=DEV)).requires_grad_(True)
+    cos, sin = torch.rand(s, d, device=DEV), torch.rand(s, d, device=DEV)
+    pos, inv = torch.arange(s, device=DEV)[None], torch.rand(d // 2, device=DEV)
+    ang = (pos[0].double()[:, None] * inv.double())[None, None]
+    g = torch.randn(b, h, s, d, device=DEV).to(dtype)
+    tables = [t[None, None, :, :d // 2].double() for t in (cos, sin)]
+    for strides in ((500, 100, 1, 1), (500, 0, 1, 1), (0, 1, 0, 1), (1, 0, 0, 1)):
+        q = buf.as_strided((b, h, s, d), strides).requires_grad_(True)
+        for norm in (True, False):
+            if norm:
+                qo, ko = kernels.apply_qk_norm_rope(q, k, w, w, cos, sin)
+                want = ref.rotate(q, w, *tables, 1e-6, g)
+            else:
+                qo, ko = kernels.apply_multi_axis_rope(q, k, pos, inv, (0,) * (d // 2))
+                want = ref.rotate(q, None, ang.cos(), ang.sin(), 0.0, g, angle_error=2.0 ** -21)
+            (dq,) = torch.autograd.grad([qo, ko], [q], [g, torch.zeros_like(k)])
+            assert qo.stride(-1) == ko.stride(-1) == 1
+            ref.check("y", qo, want["y"])
+            ref.check("dx", dq, want["dx"])
