@@ -751,10 +751,8 @@ bool rows_ok(const HeadRows& t, bool grads, int64_t es) {
 }
 
 template <typename T>
-bool vectors_ok(const HeadRows& q, const HeadRows& k, const Angles& a, int dtype, int half, int ne, bool grads) {
-  if (ne == 0 || half % ne || half / ne > 32 || !rows_ok(q, grads, sizeof(T)) ||
-      !rows_ok(k, grads, sizeof(T)))
-    return false;
+bool vectors_ok(const HeadRows& q, const HeadRows& k, const Angles& a, int dtype, int ne, bool grads) {
+  if (ne == 0 || !rows_ok(q, grads, sizeof(T)) || !rows_ok(k, grads, sizeof(T))) return false;
   if (!a.cos) return true;
   const int64_t es = a.dtype == SOUP_F32 ? 4 : 2;
   return (a.dtype == dtype || a.dtype == SOUP_F32) && aligned16(a.cos) && aligned16(a.sin) && (a.tb * es) % 16 == 0 &&
@@ -802,10 +800,12 @@ cudaError_t fwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Sh
 template <typename T, int NE>
 cudaError_t fwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, bool norm, int src,
                        cudaStream_t st) {
-  if (norm && src == kTableT) return fwd_launch<T, NE, true, kTableT>(q, k, a, sh, st);
+  if constexpr (sizeof(T) == 2) {  // fp32 tables of fp32 rows are kTableF
+    if (norm && src == kTableT) return fwd_launch<T, NE, true, kTableT>(q, k, a, sh, st);
+    if (src == kTableT) return fwd_launch<T, NE, false, kTableT>(q, k, a, sh, st);
+  }
   if (norm && src == kTableF) return fwd_launch<T, NE, true, kTableF>(q, k, a, sh, st);
   if (norm) return fwd_launch<T, NE, true, kPositions>(q, k, a, sh, st);
-  if (src == kTableT) return fwd_launch<T, NE, false, kTableT>(q, k, a, sh, st);
   if (src == kTableF) return fwd_launch<T, NE, false, kTableF>(q, k, a, sh, st);
   return fwd_launch<T, NE, false, kPositions>(q, k, a, sh, st);
 }
@@ -827,7 +827,8 @@ cudaError_t bwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, Sh
 template <typename T, int NE>
 cudaError_t bwd_launch(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& sh, int src, float* part,
                        int* rows, cudaStream_t st) {
-  if (src == kTableT) return bwd_launch<T, NE, kTableT>(q, k, a, sh, part, rows, st);
+  if constexpr (sizeof(T) == 2)
+    if (src == kTableT) return bwd_launch<T, NE, kTableT>(q, k, a, sh, part, rows, st);
   if (src == kTableF) return bwd_launch<T, NE, kTableF>(q, k, a, sh, part, rows, st);
   return bwd_launch<T, NE, kPositions>(q, k, a, sh, part, rows, st);
 }
@@ -841,10 +842,11 @@ int run_fwd(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& 
             cudaStream_t st) {
   constexpr int NE = 16 / (int)sizeof(T);
   const int ne = row_ne(sh.half, sizeof(T));
-  if (vectors_ok<T>(q, k, a, dtype, sh.half, ne, false)) {
+  if (vectors_ok<T>(q, k, a, dtype, ne, false)) {
     const int src = source_of(a, dtype);
-    return cuda_status(ne == NE ? fwd_launch<T, NE>(q, k, a, sh, norm, src, st)
-                                : fwd_launch<T, 2 * NE>(q, k, a, sh, norm, src, st));
+    if constexpr (sizeof(T) == 4)  // (eight 16-bit elements reach every half of up to 256)
+      if (ne == 2 * NE) return cuda_status(fwd_launch<T, 2 * NE>(q, k, a, sh, norm, src, st));
+    return cuda_status(fwd_launch<T, NE>(q, k, a, sh, norm, src, st));
   }
   const int most = q.heads > k.heads ? q.heads : k.heads;
   const dim3 grid(any_blocks((int64_t)sh.batch * sh.seq, most), 2), block(32 * kAnyWarps);
@@ -863,10 +865,13 @@ int run_bwd(const HeadRows& q, const HeadRows& k, const Angles& a, const Shape& 
   int rows;
   cudaError_t e;
   const int ne = row_ne(sh.half, sizeof(T));
-  if (vectors_ok<T>(q, k, a, dtype, sh.half, ne, true)) {
+  if (vectors_ok<T>(q, k, a, dtype, ne, true)) {
     const int src = source_of(a, dtype);
-    e = ne == NE ? bwd_launch<T, NE>(q, k, a, sh, src, part, &rows, st)
-                 : bwd_launch<T, 2 * NE>(q, k, a, sh, src, part, &rows, st);
+    if constexpr (sizeof(T) == 4)
+      e = ne == NE ? bwd_launch<T, NE>(q, k, a, sh, src, part, &rows, st)
+                   : bwd_launch<T, 2 * NE>(q, k, a, sh, src, part, &rows, st);
+    else
+      e = bwd_launch<T, NE>(q, k, a, sh, src, part, &rows, st);
   } else {
     const int most = q.heads > k.heads ? q.heads : k.heads;
     rows = any_blocks((int64_t)sh.batch * sh.seq, most);
