@@ -70,11 +70,15 @@ def _head_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def _out_like(t: torch.Tensor) -> torch.Tensor:
-    """An output in the order of t's axes, its rows contiguous (rows that overlap, as those of
-    a sliding view do, can have them in another order)."""
+def _out_like(t: torch.Tensor):
+    """(output in the order of t's axes, its strides), its rows contiguous (of rows that
+    overlap, as those of a sliding view do, the axes' order can be another)."""
     out = torch.empty_like(t)
-    return out if out.stride(-1) == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    st = out.stride()
+    if st[3] != 1:
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        st = out.stride()
+    return out, st
 
 
 def _source(a: torch.Tensor, c: torch.Tensor, axes):
@@ -90,12 +94,12 @@ def _source(a: torch.Tensor, c: torch.Tensor, axes):
 
 
 def _forward(q, k, qw, kw, eps, a, c, axes, inverse=0):
-    qo, ko = _out_like(q), _out_like(k)
+    (qo, sq), (ko, sk) = _out_like(q), _out_like(k)
     b, hq, s, d = q.shape
     code = _lib.dtype_code(q.dtype)
     tcode, src, ts, ax = _source(a, c, axes)
     desc = _DESC.pack(b, s, d, hq, k.shape[1], code, code if qw is None else _lib.dtype_code(qw.dtype), tcode, src,
-                      inverse, *ts, *q.stride(), *qo.stride(), *k.stride(), *ko.stride(), *_NONE, *_NONE, eps)
+                      inverse, *ts, *q.stride(), *sq, *k.stride(), *sk, *_NONE, *_NONE, eps)
     _lib.call("soup_qk_norm_rope", q.device, q.data_ptr(), qo.data_ptr(), k.data_ptr(), ko.data_ptr(),
               0 if qw is None else qw.data_ptr(), 0 if kw is None else kw.data_ptr(), a.data_ptr(), c.data_ptr(), ax,
               desc, _lib.stream_of(q))
@@ -142,7 +146,7 @@ class QKNormRoPEFunction(torch.autograd.Function):
         _, _, need_q, need_k = ctx.needs_input_grad[:4]
         b, hq, s, d = qs
         hk = ks[1]
-        dq, dk = _out_like(q), _out_like(k)
+        (dq, sq), (dk, sk) = _out_like(q), _out_like(k)
         dqw = torch.empty_like(qw) if need_q else None
         dkw = torch.empty_like(kw) if need_k else None
         nbytes, ws = 0, 0
@@ -152,7 +156,7 @@ class QKNormRoPEFunction(torch.autograd.Function):
             ws = buf.data_ptr()
         tcode, src, ts, ax = _source(a, c, axes)
         desc = _DESC.pack(b, s, d, hq, hk, _lib.dtype_code(dt), _lib.dtype_code(qw.dtype), tcode, src, 0, *ts,
-                          *q.stride(), *dq.stride(), *k.stride(), *dk.stride(), *gq.stride(), *gk.stride(), eps)
+                          *q.stride(), *sq, *k.stride(), *sk, *gq.stride(), *gk.stride(), eps)
         _lib.call("soup_qk_norm_rope_bwd", dev, gq.data_ptr(), q.data_ptr(), dq.data_ptr(), gk.data_ptr(),
                   k.data_ptr(), dk.data_ptr(), qw.data_ptr(), kw.data_ptr(), _lib.ptr(dqw), _lib.ptr(dkw),
                   a.data_ptr(), c.data_ptr(), ax, desc, ws, nbytes, _lib.stream_of(q))
