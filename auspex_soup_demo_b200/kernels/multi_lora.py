@@ -10,7 +10,7 @@ once: csrc/multi_lora.cu.
 from __future__ import annotations
 
 import functools
-from typing import Optional, Union
+from typing import Callable, Optional, Union
 
 import torch
 
@@ -67,11 +67,12 @@ class MultiLoRAFunction(torch.autograd.Function):
     """See :func:`multi_lora_linear`; ``per``: tokens of one id."""
 
     @staticmethod
-    def forward(ctx, x, weight, lora_a, lora_b, ids, scaling, bias, per: int):
+    def forward(ctx, x, weight, lora_a, lora_b, ids, scaling, bias, per: int, weight_fn):
         y, x2, w, a16, b16, state = _forward(x, weight, lora_a, lora_b, ids, scaling, bias, per)
-        # x is needed for lora_a's gradient alone
-        ctx.save_for_backward(x2 if ctx.needs_input_grad[2] else None, w, a16, b16, ids, scaling, state)
-        ctx.meta = per, x.shape, lora_a.dtype, lora_b.dtype
+        # x is needed for lora_a's gradient alone, the weight for x's
+        ctx.save_for_backward(x2 if ctx.needs_input_grad[2] else None,
+                              w if ctx.needs_input_grad[0] and weight_fn is None else None, a16, b16, ids, scaling, state)
+        ctx.meta = per, x.shape, lora_a.dtype, lora_b.dtype, weight.shape, weight_fn
         return y
 
     @staticmethod
@@ -81,11 +82,13 @@ class MultiLoRAFunction(torch.autograd.Function):
         x2, w, a16, b16, ids, scaling, state = ctx.saved_tensors
         a16, b16, state = _lib.dense(a16), _lib.dense(b16), _lib.dense(state)
         ids, scaling = ids.contiguous(), scaling.contiguous()
-        per, shape, a_dtype, b_dtype = ctx.meta
-        n, k = w.shape
-        w = _rows(w, k)
-        na, r = a16.shape[0], a16.shape[1]
+        per, shape, a_dtype, b_dtype, (n, k), weight_fn = ctx.meta
         need_x, _, need_a, need_b = ctx.needs_input_grad[:4]
+        if need_x:
+            w = _rows(weight_fn() if w is None else w, k)
+        else:
+            w = a16.view(-1, k)  # not read
+        na, r = a16.shape[0], a16.shape[1]
         dy2 = _rows(dy, n)
         t = dy2.shape[0]
         dev = dy2.device
@@ -112,12 +115,13 @@ class MultiLoRAFunction(torch.autograd.Function):
             da = da.to(a_dtype)
         if db is not None and db.dtype is not b_dtype:
             db = db.to(b_dtype)
-        return dx, None, da, db, None, None, None, None
+        return dx, None, da, db, None, None, None, None, None
 
 
 def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                       adapter_ids: torch.Tensor, scaling: Union[float, torch.Tensor] = 1.0,
-                      bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      bias: Optional[torch.Tensor] = None,
+                      weight_fn: Optional[Callable[[], torch.Tensor]] = None) -> torch.Tensor:
     """``x W^T + bias`` plus, for each token, ``scaling * B (A x)`` of its own adapter.
 
     x [..., K] bfloat16; weight [N, K] and bias [N] bfloat16, frozen. lora_a
@@ -127,7 +131,8 @@ def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tenso
     for x [B, S, K], one for each sequence ([B]); an id outside [0, adapters), e.g. -1,
     takes the projection alone. scaling: a number, or float32 [adapters], constant.
     Adapters of smaller ranks are padded with zero rows and columns, whose gradients
-    are 0.
+    are 0. weight_fn: forms the same weight again; the backward pass then calls it, and the
+    weight is not kept for it (``qlora.KEEP_BASE_WEIGHTS``).
 
     Products accumulate in 32 bits; A x is rounded to bfloat16 before B. Differentiable
     with respect to x, lora_a and lora_b, once; gradients have their leaves' types, and
@@ -198,5 +203,5 @@ def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tenso
         return x.new_zeros(*xs[:-1], n) + (x.sum() + lora_a[:, :0].sum() + lora_b[:0].sum()).to(x.dtype)
     ids = adapter_ids.contiguous()
     if _lib.differentiated(x, lora_a, lora_b):
-        return MultiLoRAFunction.apply(x, weight, lora_a, lora_b, ids, scaling, bias, per)
+        return MultiLoRAFunction.apply(x, weight, lora_a, lora_b, ids, scaling, bias, per, weight_fn)
     return _forward(x, weight, lora_a, lora_b, ids, scaling, bias, per)[0]

@@ -10,6 +10,7 @@ adapter i as a PEFT directory.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Sequence, Union
 
@@ -56,6 +57,10 @@ class _MultiLoRABase(torch.nn.Module):
     def base_weight(self, dtype) -> torch.Tensor:
         raise NotImplementedError
 
+    def weight_again(self, dtype):
+        """What forms the base weight again in the backward pass; None: it is kept."""
+        return None
+
     def _apply(self, fn, *args, **kwargs):
         # model.to(bf16) casts buffers; the scales stay fp32
         scaling = self._buffers.pop("scaling")
@@ -72,7 +77,9 @@ class _MultiLoRABase(torch.nn.Module):
         ids = self.adapter_ids.ids
         if ids is None:
             raise ValueError("the batch's adapter ids are not set (AdapterIds.set, or the trainer's adapter_ids)")
-        return multi_lora_linear(x, self.base_weight(x.dtype), self.lora_A, self.lora_B, ids, self.scaling, self.bias)
+        args = x, self.base_weight(x.dtype), self.lora_A, self.lora_B, ids, self.scaling, self.bias
+        again = self.weight_again(x.dtype)
+        return multi_lora_linear(*args) if again is None else multi_lora_linear(*args, again)
 
 
 class MultiLoRANF4Linear(_MultiLoRABase):
@@ -92,6 +99,11 @@ class MultiLoRANF4Linear(_MultiLoRABase):
         from .qlora import nf4_dequantize
 
         return nf4_dequantize(self.packed, self.absmax, (self.out_features, self.in_features), dtype)
+
+    def weight_again(self, dtype):
+        from . import qlora
+
+        return None if qlora.KEEP_BASE_WEIGHTS else functools.partial(self.base_weight, dtype)
 
 
 class MultiLoRADenseLinear(_MultiLoRABase):

@@ -1,7 +1,7 @@
 """GPU: calls of the operators of a step with several adapters whose outcome their
 documentation promises: gradients that are not finite, second moments near the smallest
 numbers, parameters that were given other memory, tangents, rows that
-overlap."""
+overlap, base weights that are not kept."""
 
 import math
 
@@ -10,7 +10,8 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 import adapter_step_reference as ref
-from auspex_soup_demo_b200 import _lib, kernels
+from auspex_soup_demo_b200 import _lib, kernels, qlora
+from auspex_soup_demo_b200.multi_adapter import AdapterIds, MultiLoRANF4Linear
 from auspex_soup_demo_b200.optim import MultiTensorAdamW
 
 pytestmark = pytest.mark.gpu
@@ -189,3 +190,31 @@ def test_rows_that_overlap(dtype):
             assert qo.stride(-1) == ko.stride(-1) == 1
             ref.check("y", qo, want["y"])
             ref.check("dx", dq, want["dx"])
+
+
+@pytest.mark.parametrize("tokens", [9, 300])
+def test_base_weights_that_are_not_kept(tokens, monkeypatch):
+    """With KEEP_BASE_WEIGHTS off nothing of the dense weight's size stays between the passes of
+    an NF4 linear, and results and gradients are the same bits."""
+    ids = AdapterIds(3)
+    torch.manual_seed(0)
+    lin = MultiLoRANF4Linear(torch.nn.Linear(256, 192, device=DEV, dtype=torch.bfloat16), ids, r=8)
+    with torch.no_grad():
+        lin.lora_B.normal_(std=0.1)
+    x = torch.randn(1, tokens, 256, device=DEV, dtype=torch.bfloat16)
+    dy = torch.randn(1, tokens, 192, device=DEV, dtype=torch.bfloat16)
+    ids.set((torch.arange(tokens, device=DEV) % 4 - 1)[None])
+    runs = []
+    for keep in (True, False):
+        monkeypatch.setattr(qlora, "KEEP_BASE_WEIGHTS", keep)
+        for grad in (True, False):  # with and without x's gradient, which needs the weight
+            held = []
+            leaves = [lin.lora_A, lin.lora_B] + ([x.requires_grad_(True)] if grad else [])
+            x.requires_grad_(grad)
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: held.append(tuple(t.shape)) or t, lambda t: t):
+                y = lin(x)
+            assert ((192, 256) in held) == (keep and grad)
+            runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    for one, two in ((runs[0], runs[2]), (runs[1], runs[3]), (runs[0], runs[1])):
+        for a, b in zip(one, two):
+            assert torch.equal(a, b)
