@@ -33,6 +33,7 @@ class MultiAxisRotary(torch.nn.Module):
             raise ValueError("install_heads: a rotary embedding with a scaling factor has no form with several axes")
         self.register_buffer("inv_freq", inv_freq.to(torch.float32), persistent=False)
         self.axes = axes
+        self.positions = None  # [axes, B, S] of the model's call in progress
 
     def _apply(self, fn, *args, **kwargs):
         inv = self._buffers.pop("inv_freq")  # frequencies stay fp32 under model.to(bf16)
@@ -43,8 +44,23 @@ class MultiAxisRotary(torch.nn.Module):
             self._buffers["inv_freq"] = inv if moved.device == inv.device else inv.to(moved.device)
         return self
 
+    def take_positions(self, body, args, kwargs):
+        """Pre-hook of the model's body: positions of several axes go around it, straight to
+        :meth:`forward`. The body itself looks for packed sequences in its positions, and has
+        a form of that for [B, S] alone; without any it counts 0, 1, 2, ... of each row."""
+        self.positions = None
+        pos = kwargs.get("position_ids") if len(args) < 3 else args[2]
+        if pos is None or pos.dim() != 3:
+            return None
+        self.positions = pos
+        if len(args) >= 3:
+            return (*args[:2], None, *args[3:]), kwargs
+        return args, {**kwargs, "position_ids": None}
+
     def forward(self, x, position_ids):
         n = max(self.axes) + 1
+        if self.positions is not None:
+            position_ids, self.positions = self.positions, None
         if position_ids.dim() == 2:
             position_ids = position_ids.unsqueeze(0).expand(n, *position_ids.shape)
         elif position_ids.shape[0] < n:
@@ -85,7 +101,8 @@ def install_heads(model, qk_norm: bool = True, rope_sections: Optional[Sequence[
     """Give every attention layer of a Qwen2 causal-LM ``model`` norms of q and k for each
     head (weights 1; trained with ``train_norms``) and / or positions of several axes
     (``rope_sections``: frequencies of each axis, together half the head dim). Its
-    ``position_ids`` are then [B, S] or [axes, B, S]. CUDA models."""
+    ``position_ids`` are then [B, S] or [axes, B, S]; with the latter every row is one
+    sequence (a padding mask [B, S] is taken as ever). CUDA models."""
     from transformers.models.qwen2 import modeling_qwen2 as m
 
     from .kernels import rope_axes
@@ -99,7 +116,8 @@ def install_heads(model, qk_norm: bool = True, rope_sections: Optional[Sequence[
         half = model.model.rotary_emb.inv_freq.numel()
         if len(axes) != half:
             raise ValueError(f"install_heads: sections of {len(axes)} frequencies, the model has {half}")
-        model.model.rotary_emb = MultiAxisRotary(model.model.rotary_emb, axes)
+        rotary = model.model.rotary_emb = MultiAxisRotary(model.model.rotary_emb, axes)
+        model.model.register_forward_pre_hook(rotary.take_positions, with_kwargs=True)
     for layer in model.model.layers:
         attn = layer.self_attn
         attn.q_norm = attn.k_norm = None

@@ -1,5 +1,5 @@
 """CPU: what the operators of a step with several adapters check of tensors that changed
-between two calls."""
+between two calls, and calls of the model built of them (in plain torch)."""
 
 import array
 import ctypes
@@ -7,7 +7,8 @@ import ctypes
 import pytest
 import torch
 
-from auspex_soup_demo_b200 import _lib, optim
+import test_gpu_adapter_model as plain
+from auspex_soup_demo_b200 import _lib, kernels, optim, qlora
 
 
 # --------------------------------------------------- tensors of an optimiser's step ----
@@ -89,3 +90,63 @@ def test_gradients_of_another_size_are_refused():
     p.grad = torch.ones(4, 2).t()  # another order: copied
     (_, _, grads, _, _, kept, *_), = opt._tables(held, torch.device("cpu"))
     assert kept[0].is_contiguous() and grads[0] == kept[0].data_ptr()
+
+
+# -------------------------------------------------------------- the model itself ----
+def _model(monkeypatch, attention="sdpa", seed=0):
+    """A small model on the host, its operators in plain torch."""
+    monkeypatch.setattr(kernels, "multi_lora_linear", plain._plain_lora)
+    monkeypatch.setattr(kernels, "apply_multi_axis_rope", plain._plain_axes)
+    cfg = qlora.qwen2_1p5b_config(2, hidden_size=64, intermediate_size=96, num_attention_heads=2,
+                                  num_key_value_heads=1, vocab_size=100, head_dim=32)
+    cfg._attn_implementation = attention
+    m = qlora.build_qwen2_qlora(cfg, device="cpu", seed=seed, r=8, alpha=16, quantize=False, adapters=3, qk_norm=True,
+                                train_norms=True, rope_sections=(4, 6, 6), dtype=torch.float32)
+    g = torch.Generator().manual_seed(1)
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if "lora_B" in n:
+                p.copy_(0.1 * torch.randn(p.shape, generator=g))
+            if "_norm.weight" in n and "self_attn" in n:
+                p.copy_(1 + 0.2 * torch.randn(p.shape, generator=g))
+    return m
+
+
+def _batch(b, s=12, seed=3):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.randint(0, 100, (b, s), generator=g)
+    pos = torch.arange(s).expand(3, b, s).clone()
+    pos[1:, :, s // 2:] = torch.randint(0, 9, (2, b, s - s // 2), generator=g)
+    return ids, pos
+
+
+@pytest.mark.parametrize("attention", ["sdpa", "eager"])
+@pytest.mark.parametrize("b", [1, 2, 3])
+def test_positions_of_several_axes_in_a_call_of_the_model(b, attention, monkeypatch):
+    """model(ids, position_ids=[axes, B, S]) is the body with a prepared causal mask; a padded
+    batch's rows are those of the sequences alone."""
+    m = _model(monkeypatch, attention)
+    ids, pos = _batch(b)
+    m.adapter_ids.set(torch.arange(b))
+    with torch.no_grad():
+        got = m(ids, position_ids=pos).logits
+        assert not torch.allclose(got, m(ids).logits)  # the axes count
+        # the same positions on every axis, given as [B, S] and as [axes, B, S]
+        text = torch.arange(12).expand(b, 12)
+        one, two = m(ids, position_ids=text).logits, m(ids, position_ids=text.expand(3, b, 12)).logits
+        assert torch.equal(one, two) and torch.equal(one, m(ids).logits)
+        for i in range(b):
+            m.adapter_ids.set(torch.tensor([i]))
+            alone = m(ids[i:i + 1, :9], position_ids=pos[:, i:i + 1, :9]).logits
+            # the same sums in products of other row counts, 200 roundings of 2^-24 of numbers of a few units
+            assert float((got[i, :9] - alone[0]).abs().max()) <= 200 * 2.0 ** -24 * 8
+        mask = torch.ones(b, 12, dtype=torch.int64)
+        mask[:, 9:] = 0
+        m.adapter_ids.set(torch.arange(b))
+        padded = m(ids, attention_mask=mask, position_ids=pos).logits
+        assert float((padded[:, :9] - got[:, :9]).abs().max()) <= 200 * 2.0 ** -24 * 8
+        (last,) = m.model(ids, None, pos, return_dict=False)[:1]  # by place
+        assert torch.equal(m.lm_head(last), got)
+        with pytest.raises(ValueError, match="position_ids"):
+            m(ids, position_ids=pos[:2])
+        assert torch.equal(m(ids).logits, one)  # nothing of a refused call is left

@@ -1,7 +1,8 @@
 """GPU: calls of the operators of a step with several adapters whose outcome their
 documentation promises: gradients that are not finite, second moments near the smallest
 numbers, parameters that were given other memory, tangents, rows that
-overlap, base weights that are not kept."""
+overlap, base weights that are not kept,
+positions of several axes in a call of the model."""
 
 import math
 
@@ -10,6 +11,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 
 import adapter_step_reference as ref
+import test_gpu_adapter_model as model_tests
 from auspex_soup_demo_b200 import _lib, kernels, qlora
 from auspex_soup_demo_b200.multi_adapter import AdapterIds, MultiLoRANF4Linear
 from auspex_soup_demo_b200.optim import MultiTensorAdamW
@@ -218,3 +220,18 @@ def test_base_weights_that_are_not_kept(tokens, monkeypatch):
     for one, two in ((runs[0], runs[2]), (runs[1], runs[3]), (runs[0], runs[1])):
         for a, b in zip(one, two):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("attention", ["sdpa", "soup"])
+def test_positions_of_several_axes_in_a_call_of_the_model(attention):
+    """The model called with [axes, B, S] positions, beside its body with a prepared mask (no mask:
+    causal) as the trainer calls it: at most an attention kernel apart, 16 roundings of bf16."""
+    m = model_tests._model(attention=attention)
+    ids, _, pos = model_tests._batch()
+    m.adapter_ids.set(torch.tensor([0, 2, -1], device=DEV))
+    with torch.no_grad():
+        got = m(ids, position_ids=pos).logits
+        want = m.lm_head(m.model(input_ids=ids, attention_mask={"full_attention": None}, position_ids=pos)[0])
+        text = m(ids).logits
+    assert float((got - want).abs().max()) <= 16 * 2.0 ** -8 * float(want.abs().max())
+    assert not torch.equal(got, text)
