@@ -19,16 +19,52 @@ import torch
 
 class AdapterIds:
     """The adapter ids of the batch that a model is running: [B] or [B, S] integers on the
-    model's device, -1 for none. One object is shared by all of a model's linears."""
+    model's device, -1 for none. One object is shared by all of a model's linears.
+
+    The ids that hold for a call of the model are those set when it begins, or its
+    ``adapter_ids`` argument (:meth:`follow`). Its layers get them as an argument of
+    their own, so that a checkpointed layer that runs again in the backward pass takes
+    the ids of its forward pass, whatever was set since."""
 
     def __init__(self, adapters: int):
         self.adapters = adapters
         self.ids: Optional[torch.Tensor] = None
+        self._running = []  # the ids of the layers in progress
 
     def set(self, ids: Optional[torch.Tensor]) -> None:
+        self.ids = self._checked(ids)
+
+    @staticmethod
+    def _checked(ids: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
         if ids is not None and (ids.dim() not in (1, 2) or ids.dtype not in (torch.int64, torch.int32)):
             raise ValueError(f"adapter ids must be int64 or int32 [B] or [B, S], got {ids.dtype} {tuple(ids.shape)}")
-        self.ids = ids
+        return ids
+
+    def current(self) -> torch.Tensor:
+        """The ids of the layer in progress (outside one: those that are set)."""
+        ids = self._running[-1] if self._running else self.ids
+        if ids is None:
+            raise ValueError("the batch's adapter ids are not set (AdapterIds.set, or the trainer's adapter_ids)")
+        return ids
+
+    def follow(self, model) -> None:
+        """Hand the layers of a causal-LM ``model`` the ids of each of its calls."""
+        model.model.register_forward_pre_hook(self._begin, with_kwargs=True)
+        for layer in model.model.layers:
+            layer.register_forward_pre_hook(self._enter, with_kwargs=True)
+            layer.register_forward_hook(self._leave, always_call=True)
+
+    def _begin(self, body, args, kwargs):
+        ids = kwargs.get("adapter_ids")
+        return args, {**kwargs, "adapter_ids": self.ids if ids is None else self._checked(ids)}
+
+    def _enter(self, layer, args, kwargs):
+        self._running.append(kwargs.pop("adapter_ids", self.ids))
+        return args, kwargs
+
+    def _leave(self, layer, args, output):
+        if self._running:  # (another hook may have raised before _enter)
+            self._running.pop()
 
 
 class _MultiLoRABase(torch.nn.Module):
@@ -74,9 +110,7 @@ class _MultiLoRABase(torch.nn.Module):
     def forward(self, x):
         from .kernels import multi_lora_linear
 
-        ids = self.adapter_ids.ids
-        if ids is None:
-            raise ValueError("the batch's adapter ids are not set (AdapterIds.set, or the trainer's adapter_ids)")
+        ids = self.adapter_ids.current()
         args = x, self.base_weight(x.dtype), self.lora_A, self.lora_B, ids, self.scaling, self.bias
         again = self.weight_again(x.dtype)
         return multi_lora_linear(*args) if again is None else multi_lora_linear(*args, again)

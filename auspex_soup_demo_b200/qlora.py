@@ -1062,7 +1062,7 @@ def build_qwen2_qlora(config=None, device="cuda", seed: int = 0, r: int = 16, al
 
     adapters=n holds n adapters in every target linear (``multi_adapter``; alpha a
     number or one for each); the batch's ids are set through ``model.adapter_ids`` or
-    the trainer's ``adapter_ids``. qk_norm, train_norms, rope_sections and
+    given to a call, the model's or the trainer's, as ``adapter_ids``. qk_norm, train_norms, rope_sections and
     rope_interleaved: norms of queries and keys for each head and positions of several
     axes (:func:`.heads.install_heads`). CUDA, bf16.
     """
@@ -1097,6 +1097,8 @@ def build_qwen2_qlora(config=None, device="cuda", seed: int = 0, r: int = 16, al
                 lin = getattr(parent, name, None)
                 if isinstance(lin, torch.nn.Linear):
                     setattr(parent, name, wrap(lin, r, alpha))
+    if adapters is not None:
+        ids.follow(model)
     if qk_norm or rope_sections is not None:
         from .heads import install_heads
 

@@ -150,3 +150,55 @@ def test_positions_of_several_axes_in_a_call_of_the_model(b, attention, monkeypa
         with pytest.raises(ValueError, match="position_ids"):
             m(ids, position_ids=pos[:2])
         assert torch.equal(m(ids).logits, one)  # nothing of a refused call is left
+
+
+def _grads(m, hidden):
+    m.zero_grad()
+    hidden.square().sum().backward()
+    return [p.grad for p in m.parameters() if p.requires_grad]
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_layers_run_again_with_the_ids_of_their_forward(reentrant, monkeypatch):
+    """Two forward passes of different ids, and a call without a gradient, before the first
+    one's backward pass: gradients of each are those without checkpointing."""
+    m = _model(monkeypatch)
+    m.train()
+    (one, pos), (two, _) = _batch(2, seed=1), _batch(2, seed=2)
+    a, b, c = (torch.tensor(v) for v in ([0, 1], [2, -1], [1, 1]))
+
+    def run():
+        m.adapter_ids.set(a)
+        h1 = m.model(one, position_ids=pos)[0]
+        m.adapter_ids.set(b)
+        h2 = m.model(two)[0]
+        with torch.no_grad():
+            h3 = m.model(one, adapter_ids=c)[0]
+        assert m.adapter_ids.ids is b  # an argument holds for its call alone
+        return h3, _grads(m, h1), _grads(m, h2)
+
+    want = run()
+    m.enable_input_require_grads()
+    m.gradient_checkpointing_enable({"use_reentrant": reentrant})
+    got = run()
+    assert torch.equal(want[0], got[0])
+    for w, g in zip(want[1:], got[1:]):
+        for x, y in zip(w, g):
+            torch.testing.assert_close(x, y, rtol=1e-5, atol=1e-6 * float(x.abs().max() + 1e-3))
+    assert not m.adapter_ids._running
+
+
+def test_adapter_ids_of_a_call(monkeypatch):
+    m = _model(monkeypatch)
+    ids, pos = _batch(2)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="not set"):
+            m(ids)
+        with pytest.raises(ValueError, match="adapter ids"):
+            m(ids, adapter_ids=torch.zeros(2))
+        m.adapter_ids.set(torch.tensor([2, 2]))
+        one = m(ids).logits
+        assert torch.equal(one, m(ids, adapter_ids=torch.tensor([2, 2])).logits)
+        assert not torch.equal(one, m(ids, adapter_ids=torch.tensor([0, 2])).logits)
+        assert torch.equal(one, m(ids).logits)
+        assert not m.adapter_ids._running  # also after the refusals
