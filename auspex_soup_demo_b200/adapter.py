@@ -14,6 +14,11 @@ This module writes and reads that layout for models built by
   ``base_model.model.`` prefix of ``PeftModelForCausalLM``, adapter name removed),
   in the parameters' dtype (fp32 here, as PEFT keeps LoRA factors of 4-bit
   models);
+* beside them the other parameters that are trained (``requires_grad``: the norms of
+  queries and keys of ``heads.install_heads``, say) as ``base_model.model.P.<name>``,
+  their modules listed in the config's ``modules_to_save``, as PEFT does. A model
+  with several adapters has one of each for all adapters, and every adapter's file
+  holds it;
 * ``adapter_config.json``: the ``LoraConfig`` fields PEFT writes for a plain
   LoRA adapter (``peft_type`` LORA, ``task_type`` CAUSAL_LM, ``r``,
   ``lora_alpha``, ``target_modules``, ...).
@@ -47,6 +52,12 @@ def lora_modules(model) -> Dict[str, torch.nn.Module]:
     return out
 
 
+def trained_beside(model) -> Dict[str, torch.nn.Parameter]:
+    """Name -> parameter of what is trained and is no LoRA factor."""
+    factors = {id(p) for m in lora_modules(model).values() for p in (m.lora_A, m.lora_B)}
+    return {n: p for n, p in model.named_parameters() if p.requires_grad and id(p) not in factors}
+
+
 def _factors(mod, index: Optional[int]):
     """(A [r, in], B [out, r]) of a module; of adapter ``index`` where it holds several."""
     if mod.lora_A.dim() == 2:
@@ -66,13 +77,15 @@ def _scaling(mod, index: Optional[int]) -> float:
 
 
 def adapter_state_dict(model, index: Optional[int] = None) -> Dict[str, torch.Tensor]:
-    """PEFT-named LoRA tensors (CPU, contiguous, the parameters' dtype); ``index``: which
-    adapter of a model with several."""
+    """PEFT-named LoRA tensors and what is trained beside them (CPU, contiguous, the
+    parameters' dtype); ``index``: which adapter of a model with several."""
     sd = {}
     for path, mod in lora_modules(model).items():
         a, b = _factors(mod, index)
         sd[f"{_PREFIX}{path}.lora_A.weight"] = a.to("cpu").contiguous()
         sd[f"{_PREFIX}{path}.lora_B.weight"] = b.to("cpu").contiguous()
+    for name, p in trained_beside(model).items():
+        sd[_PREFIX + name] = p.detach().to("cpu").contiguous()
     return sd
 
 
@@ -91,6 +104,7 @@ def adapter_config(model, base_model_name_or_path: str, r: Optional[int] = None,
     if alpha.is_integer():
         alpha = int(alpha)
     targets = sorted({path.rsplit(".", 1)[-1] for path in mods})
+    beside = sorted({name.split(".")[-2] for name in trained_beside(model) if "." in name})
     return {
         "alpha_pattern": {},
         "base_model_name_or_path": base_model_name_or_path,
@@ -102,7 +116,7 @@ def adapter_config(model, base_model_name_or_path: str, r: Optional[int] = None,
         "layers_to_transform": None,
         "lora_alpha": alpha,
         "lora_dropout": float(lora_dropout),
-        "modules_to_save": None,
+        "modules_to_save": beside or None,
         "peft_type": "LORA",
         "r": r,
         "rank_pattern": {},
@@ -136,7 +150,9 @@ def load_adapter(model, directory: str, strict: bool = True, index: Optional[int
 
     Checks that r and lora_alpha match the wrapped modules (the scale is baked
     into each module) and, with ``strict``, that the file and the model hold
-    exactly the same set of LoRA tensors with the same shapes.
+    exactly the same set of LoRA tensors with the same shapes. Parameters that were
+    trained beside the factors are copied too, also where the model does not train
+    them; with ``strict`` those that it trains have to be there.
     """
     from safetensors.torch import load_file
 
@@ -148,11 +164,19 @@ def load_adapter(model, directory: str, strict: bool = True, index: Optional[int
         raise ValueError("rsLoRA / DoRA adapters are not supported")
     tensors = load_file(os.path.join(directory, ADAPTER_WEIGHTS))
     mods = lora_modules(model)
+    others = dict(model.named_parameters())
     seen = set()
     for key, value in tensors.items():
         m = _KEY.match(key)
         if m is None:
-            if strict:
+            name = key[len(_PREFIX):]
+            param = others.get(name) if key.startswith(_PREFIX) else None
+            if param is not None and name.split(".")[-2:-1] and name.split(".")[-2] in (cfg.get("modules_to_save") or ()):
+                if tuple(param.shape) != tuple(value.shape):
+                    raise ValueError(f"{key}: shape {tuple(value.shape)} vs model {tuple(param.shape)}")
+                param.detach().copy_(value.to(device=param.device, dtype=param.dtype))
+                seen.add(name)
+            elif strict:
                 raise KeyError(f"unexpected tensor in adapter: {key}")
             continue
         path, which = m.group(1), m.group(2)
@@ -170,6 +194,9 @@ def load_adapter(model, directory: str, strict: bool = True, index: Optional[int
         missing = [f"{p}.lora_{w}" for p in mods for w in "AB" if (p, w) not in seen]
         if missing:
             raise KeyError(f"adapter lacks {len(missing)} LoRA tensors, e.g. {missing[:3]}")
+        missing = [n for n in trained_beside(model) if n not in seen]
+        if missing:
+            raise KeyError(f"adapter lacks {len(missing)} parameters that the model trains, e.g. {missing[:3]}")
     for path, mod in mods.items():
         r = _factors(mod, index)[0].shape[0]
         if int(cfg.get("r", r)) != r:

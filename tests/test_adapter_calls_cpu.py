@@ -3,12 +3,13 @@ between two calls, and calls of the model built of them (in plain torch)."""
 
 import array
 import ctypes
+import json
 
 import pytest
 import torch
 
 import test_gpu_adapter_model as plain
-from auspex_soup_demo_b200 import _lib, kernels, optim, qlora
+from auspex_soup_demo_b200 import _lib, adapter, kernels, optim, qlora
 
 
 # --------------------------------------------------- tensors of an optimiser's step ----
@@ -202,3 +203,50 @@ def test_adapter_ids_of_a_call(monkeypatch):
         assert not torch.equal(one, m(ids, adapter_ids=torch.tensor([0, 2])).logits)
         assert torch.equal(one, m(ids).logits)
         assert not m.adapter_ids._running  # also after the refusals
+
+
+def test_norms_that_were_trained_are_in_the_adapters_file(tmp_path, monkeypatch):
+    """A step, saved and loaded into a fresh model: the same logits, also where the fresh model
+    does not train its norms; a file without them is refused where the model does."""
+    m = _model(monkeypatch)
+    ids, pos = _batch(2)
+    a = torch.tensor([1, 2])
+    m(ids, position_ids=pos, adapter_ids=a).logits.square().mean().backward()
+    norms = {n: p for n, p in m.named_parameters() if "q_norm" in n or "k_norm" in n}
+    assert len(norms) == 4
+    with torch.no_grad():
+        for p in m.parameters():
+            if p.grad is not None:
+                assert p.grad.any()
+                p.sub_(0.1 * p.grad / p.grad.norm())
+        want = m(ids, position_ids=pos, adapter_ids=a).logits
+    for i in (1, 2):
+        adapter.save_adapter(m, str(tmp_path / str(i)), index=i)
+    cfg = json.load(open(tmp_path / "1" / "adapter_config.json"))
+    assert cfg["modules_to_save"] == ["k_norm", "q_norm"]
+    listing = adapter.header_listing(str(tmp_path / "1" / "adapter_model.safetensors"))
+    assert listing["base_model.model.model.layers.1.self_attn.q_norm.weight"] == ["F32", [32]]
+    for trained in (True, False):
+        fresh = _model(monkeypatch)
+        for n, p in fresh.named_parameters():
+            if "q_norm" in n or "k_norm" in n:
+                p.requires_grad_(trained)
+        for i in (1, 2):
+            adapter.load_adapter(fresh, str(tmp_path / str(i)), index=i)
+        with torch.no_grad():
+            assert torch.equal(fresh(ids, position_ids=pos, adapter_ids=a).logits, want)
+        assert all(p.requires_grad == trained for n, p in fresh.named_parameters() if "q_norm" in n)
+        assert torch.equal(fresh.lm_head.weight, m.lm_head.weight)  # frozen, and in no file
+    for n, p in fresh.named_parameters():
+        if "_norm" in n:
+            p.requires_grad_(False)
+    adapter.save_adapter(fresh, str(tmp_path / "bare"), index=0)
+    assert json.load(open(tmp_path / "bare" / "adapter_config.json"))["modules_to_save"] is None
+    with pytest.raises(KeyError, match="parameters that the model trains"):
+        adapter.load_adapter(m, str(tmp_path / "bare"), index=0)
+    adapter.load_adapter(m, str(tmp_path / "bare"), strict=False, index=0)
+    # a model without such norms has no place for them
+    other = qlora.build_qwen2_qlora(m.config, device="cpu", r=8, alpha=16, quantize=False, adapters=3,
+                                    dtype=torch.float32)
+    with pytest.raises(KeyError, match="unexpected"):
+        adapter.load_adapter(other, str(tmp_path / "1"), index=1)
