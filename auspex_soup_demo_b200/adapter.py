@@ -152,7 +152,9 @@ def load_adapter(model, directory: str, strict: bool = True, index: Optional[int
     into each module) and, with ``strict``, that the file and the model hold
     exactly the same set of LoRA tensors with the same shapes. Parameters that were
     trained beside the factors are copied too, also where the model does not train
-    them; with ``strict`` those that it trains have to be there.
+    them; with ``strict`` those that it trains have to be there. A model with several
+    adapters takes finite factors alone: its adapters share products, so that those of
+    one that are not would reach the sequences of the others.
     """
     from safetensors.torch import load_file
 
@@ -185,6 +187,9 @@ def load_adapter(model, directory: str, strict: bool = True, index: Optional[int
             if strict:
                 raise KeyError(f"adapter tensor for a module the model does not wrap: {key}")
             continue
+        # (multiplied as bfloat16)
+        if mod.lora_A.dim() == 3 and not torch.isfinite(value.to(torch.bfloat16)).all():
+            raise ValueError(f"{key} is not finite: it would reach the model's other adapters")
         param = _factors(mod, index)[0 if which == "A" else 1]
         if tuple(param.shape) != tuple(value.shape):
             raise ValueError(f"{key}: shape {tuple(value.shape)} vs model {tuple(param.shape)}")

@@ -250,3 +250,18 @@ def test_norms_that_were_trained_are_in_the_adapters_file(tmp_path, monkeypatch)
                                     dtype=torch.float32)
     with pytest.raises(KeyError, match="unexpected"):
         adapter.load_adapter(other, str(tmp_path / "1"), index=1)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 3.4e38])  # the last one as bfloat16
+def test_factors_that_are_not_finite_stay_out_of_a_model_with_several_adapters(bad, tmp_path, monkeypatch):
+    m = _model(monkeypatch)
+    before = m.model.layers[0].mlp.up_proj.lora_B.detach().clone()
+    other = _model(monkeypatch, seed=1)
+    with torch.no_grad():
+        other.model.layers[0].mlp.up_proj.lora_B[3, 1, 2] = bad
+    adapter.save_adapter(other, str(tmp_path), index=1)
+    with pytest.raises(ValueError, match="not finite"):
+        adapter.load_adapter(m, str(tmp_path), index=1)
+    assert torch.equal(m.model.layers[0].mlp.up_proj.lora_B, before)
+    adapter.save_adapter(other, str(tmp_path), index=2)
+    adapter.load_adapter(m, str(tmp_path), index=2)
