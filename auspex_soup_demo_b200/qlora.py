@@ -1197,21 +1197,23 @@ class QLoRATrainer:
         on_cuda = self.params[0].is_cuda
         # AdamW (HF Trainer defaults: betas 0.9 / 0.999, eps 1e-8, weight decay 0).
         # "soup": one soup_adamw_flat launch over the flat buffers that also
-        # writes the 16-bit copies; "soup8": optim.MultiTensorAdamW with 8-bit
-        # moments (2 bytes a parameter instead of 8); "torch": torch.optim.AdamW;
-        # "auto": soup on CUDA, soup8 when max_grad_norm is given.
-        if optimizer not in ("auto", "soup", "soup8", "torch"):
-            raise ValueError(f"optimizer must be auto, soup, soup8 or torch, not {optimizer!r}")
+        # writes the 16-bit copies; "soup32" and "soup8": optim.MultiTensorAdamW, which
+        # can clip the gradients' norm, with fp32 or with 8-bit moments (2 bytes a
+        # parameter instead of 8); "torch": torch.optim.AdamW; "auto": soup on CUDA,
+        # soup32 when max_grad_norm is given.
+        if optimizer not in ("auto", "soup", "soup32", "soup8", "torch"):
+            raise ValueError(f"optimizer must be auto, soup, soup32, soup8 or torch, not {optimizer!r}")
         if optimizer == "auto" and on_cuda and max_grad_norm is not None:
-            optimizer = "soup8"
-        if max_grad_norm is not None and optimizer != "soup8":
-            raise ValueError("max_grad_norm needs optimizer='soup8' (on CUDA)")
+            optimizer = "soup32"
+        if max_grad_norm is not None and optimizer not in ("soup32", "soup8"):
+            raise ValueError("max_grad_norm needs optimizer='soup32' or 'soup8' (on CUDA)")
         self.lr, self.betas, self.eps, self.weight_decay = lr, (0.9, 0.999), 1e-8, weight_decay
-        if optimizer == "soup8":
+        if optimizer in ("soup32", "soup8"):
             from .optim import MultiTensorAdamW
 
             self.opt = MultiTensorAdamW(self.params, lr=lr, betas=self.betas, eps=self.eps,
-                                        weight_decay=weight_decay, state_bits=8, max_grad_norm=max_grad_norm)
+                                        weight_decay=weight_decay, state_bits=32 if optimizer == "soup32" else 8,
+                                        max_grad_norm=max_grad_norm)
         elif optimizer == "soup" or (optimizer == "auto" and on_cuda):
             if not on_cuda:
                 raise ValueError("optimizer='soup' needs CUDA parameters")

@@ -2,7 +2,7 @@
 documentation promises: gradients that are not finite, second moments near the smallest
 numbers, parameters that were given other memory, tangents, rows that
 overlap, base weights that are not kept,
-positions of several axes in a call of the model."""
+positions of several axes in a call of the model, the trainer's choice of moments."""
 
 import math
 
@@ -235,3 +235,30 @@ def test_positions_of_several_axes_in_a_call_of_the_model(attention):
         text = m(ids).logits
     assert float((got - want).abs().max()) <= 16 * 2.0 ** -8 * float(want.abs().max())
     assert not torch.equal(got, text)
+
+
+def _one_adapter():
+    cfg = qlora.qwen2_1p5b_config(1, hidden_size=256, intermediate_size=512, num_attention_heads=2,
+                                  num_key_value_heads=1, vocab_size=1000, head_dim=128)
+    return qlora.build_qwen2_qlora(cfg, device=DEV, r=8, alpha=16)
+
+
+def test_clipping_alone_does_not_choose_8_bit_moments():
+    """The trainer's own choice keeps fp32 moments; with a norm that clips nothing its steps are
+    those of the flat optimiser: 16 roundings of 2^-24 of a parameter and its update a step,
+    and an update is lr at most but for a few percent."""
+    ids, labels, _ = model_tests._batch()
+    den = float((labels != -100).sum())
+    trainers = [qlora.QLoRATrainer(_one_adapter(), max_grad_norm=1e9), qlora.QLoRATrainer(_one_adapter(), optimizer="soup"),
+                qlora.QLoRATrainer(_one_adapter(), optimizer="soup32", max_grad_norm=1e-3),
+                qlora.QLoRATrainer(_one_adapter(), optimizer="soup8", max_grad_norm=1e-3)]
+    assert [t.opt and t.opt.state_bits for t in trainers] == [32, None, 32, 8]
+    for t in trainers:
+        loss, _ = t.step(ids, labels, den)
+        assert torch.isfinite(loss)
+    one, two = (t.flat_param for t in trainers[:2])
+    assert float((one - two).abs().max()) <= 16 * 2.0 ** -24 * (float(two.abs().max()) + 2e-4)
+    assert float(trainers[0].opt.grad_norm) > 1e-3
+    for bad in ("soup", "torch"):
+        with pytest.raises(ValueError, match="soup32"):
+            qlora.QLoRATrainer(_one_adapter(), optimizer=bad, max_grad_norm=1.0)
