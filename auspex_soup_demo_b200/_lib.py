@@ -73,7 +73,7 @@ _SIGNATURES = {
     "soup_qk_norm_rope_bwd_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64, c_i64]),
     "soup_qk_norm_rope_bwd": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
                                       c_vp, c_vp, c_sz, c_vp]),
-    "soup_tensor_addresses": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp, ctypes.POINTER(c_int)]),
+    "soup_tensor_addresses": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_vp]),
     "soup_grad_square_workspace_bytes": (c_sz, [c_i64]),
     "soup_grad_square": (c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_sz, ctypes.POINTER(c_int), c_vp]),
     "soup_adamw_multi": (c_int, [c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_d, c_d,
@@ -314,8 +314,8 @@ _table_reader = None
 
 
 def _reader():
-    """(soup_tensor_addresses bound with the interpreter's lock held, the function that
-    fills a DLPack table from a torch tensor)"""
+    """(soup_tensor_addresses bound with the interpreter's lock held, its reader: the function
+    that fills a DLPack table from a torch tensor, PyList_GetItem, None)"""
     global _table_reader
     if _table_reader is None:
         lib()  # built and loadable
@@ -330,22 +330,26 @@ def _reader():
         read = ctypes.cast(api + 16, ctypes.POINTER(c_vp))[3]
         if major != 1 or not read:
             raise SoupLibraryError(f"torch's DLPack exchange interface has version {major} or cannot fill a DLTensor")
-        _table_reader = fn, read
+        item = ctypes.cast(ctypes.pythonapi.PyList_GetItem, c_vp).value
+        _table_reader = fn, (c_vp * 3)(read, item, id(None))
     return _table_reader
 
 
-def tensor_addresses(tensors, sizes: array.array, code: int, device: torch.device):
-    """The addresses (array of uint64) of tensors of these sizes (array of int64): dense, of
-    one type (its code) and on one device; or the index of the first that is not so. One
-    call for all of them: asking each of hundreds of tensors for its size, type, device
-    and layout from Python costs a step more than its kernels."""
-    fn, read = _reader()
-    objects = array.array("Q", map(id, tensors))
-    out, bad = array.array("Q", objects), c_int(0)
-    check("soup_tensor_addresses", fn(
-        read, objects.buffer_info()[0], sizes.buffer_info()[0], len(objects), code, 2 if device.type == "cuda" else 1,
-        device.index or 0, out.buffer_info()[0], ctypes.byref(bad)))
-    return out if bad.value < 0 else bad.value
+def tensor_addresses(tensors: list, sizes: array.array, code: int, device: torch.device):
+    """The addresses (array of 64-bit numbers) of a list of tensors of these sizes (array of
+    int64): dense, of one type (its code) and on one device; or the index of the first
+    that is not so, or is None. One call for all of them: asking each of hundreds of
+    tensors for its size, type, device and layout from Python costs a step more than its
+    kernels."""
+    fn, reader = _table_reader or _reader()
+    n, out = len(sizes), array.array("q", sizes)
+    if len(tensors) != n:
+        raise ValueError(f"{len(tensors)} tensors and {n} sizes")
+    status = fn(reader, id(tensors), sizes.buffer_info()[0], n, code, 2 if device.type == "cuda" else 1, device.index or 0,
+                out.buffer_info()[0])
+    if status > 0:
+        check("soup_tensor_addresses", status)
+    return out if status == 0 else -1 - status
 
 
 def dense(t: torch.Tensor) -> torch.Tensor:

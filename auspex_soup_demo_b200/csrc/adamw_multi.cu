@@ -636,23 +636,23 @@ using namespace soup;
 
 extern "C" {
 
-int soup_tensor_addresses(const void* read, const uint64_t* objects, const int64_t* sizes, int count, int dtype,
-                          int device_type, int device, uint64_t* addresses, int* bad) {
-  if (!read || !objects || !sizes || count <= 0 || !addresses || !bad ||
+int soup_tensor_addresses(void* const* reader, void* list, const int64_t* sizes, int count, int dtype, int device_type,
+                          int device, uint64_t* addresses) {
+  if (!reader || !reader[0] || !reader[1] || !list || !sizes || count <= 0 || !addresses ||
       (dtype != SOUP_F32 && dtype != SOUP_BF16 && dtype != SOUP_F16)) {
     set_last_error("soup_tensor_addresses: bad arguments");
     return SOUP_ERR_INVALID;
   }
-  const auto fill = reinterpret_cast<int (*)(void*, DlTensor*)>(const_cast<void*>(read));
+  const auto fill = reinterpret_cast<int (*)(void*, DlTensor*)>(reader[0]);
+  const auto item = reinterpret_cast<void* (*)(void*, intptr_t)>(reader[1]);
   for (int i = 0; i < count; ++i) {
+    void* object = item(list, i);
     DlTensor t{};
-    if (fill(reinterpret_cast<void*>(objects[i]), &t) != 0 || !dense_tensor(t, sizes[i], dtype, device_type, device)) {
-      *bad = i;
-      return SOUP_OK;
-    }
+    if (!object || object == reader[2] || fill(object, &t) != 0 ||
+        !dense_tensor(t, sizes[i], dtype, device_type, device))
+      return -1 - i;
     addresses[i] = reinterpret_cast<uint64_t>(t.data) + t.byte_offset;
   }
-  *bad = -1;
   return SOUP_OK;
 }
 

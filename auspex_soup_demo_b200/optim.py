@@ -210,14 +210,15 @@ class MultiTensorAdamW(torch.optim.Optimizer):
         out = []
         for code, dtype, params, sizes, blocks in held.by_dtype:
             grads = list(map(_grad, params))
-            if any(g is None for g in grads):
+            # p.data = ... gives a parameter other memory, under a gradient that stays
+            both = _addresses(grads + params, sizes + sizes, code, device)
+            if both is None and any(g is None for g in grads):
                 keep = [i for i, g in enumerate(grads) if g is not None]
                 if not keep:
                     continue
                 params, grads = [params[i] for i in keep], [grads[i] for i in keep]
                 sizes, blocks = (array.array(t.typecode, [t[i] for i in keep]) for t in (sizes, blocks))
-            # p.data = ... gives a parameter other memory, under a gradient that stays
-            both = _addresses(grads + params, sizes + sizes, code, device)
+                both = _addresses(grads + params, sizes + sizes, code, device)
             if both is not None:
                 grad_ptrs, ptrs = both[:len(grads)], both[len(grads):]
             else:

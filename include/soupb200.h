@@ -225,13 +225,13 @@ int soup_multi_lora_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx
  * min(1, max_norm / (sqrt(sum) + 1e-6)) and writes the norm to norm_out (may be NULL).
  * step (device fp32) counts completed steps and is raised by the call with last != 0;
  * coefs: four device floats, 16-byte aligned, of the optimiser's own. eps >= 1e-30.
- * soup_tensor_addresses (host work alone): the addresses of `count` Python tensors, read
- * through `read`, the dltensor_from_py_object_no_sync of their type's DLPack exchange
- * interface, called under the caller's interpreter lock. *bad is the first that is not
- * dense with sizes[i] elements of dtype on that device (DLPack's type: 1 host, 2 CUDA) or
- * that cannot be read, else -1. */
-int soup_tensor_addresses(const void* read, const uint64_t* objects, const int64_t* sizes, int count, int dtype,
-                          int device_type, int device, uint64_t* addresses, int* bad);
+ * soup_tensor_addresses (host work alone): the addresses of the `count` tensors of a Python
+ * list, read through reader[0], the dltensor_from_py_object_no_sync of their type's DLPack
+ * exchange interface, and reader[1], PyList_GetItem, called under the caller's interpreter
+ * lock; reader[2] is None. -1 - i for the first that is None, cannot be read or is not
+ * dense with sizes[i] elements of dtype on that device (DLPack's type: 1 host, 2 CUDA). */
+int soup_tensor_addresses(void* const* reader, void* list, const int64_t* sizes, int count, int dtype, int device_type,
+                          int device, uint64_t* addresses);
 size_t soup_grad_square_workspace_bytes(int64_t tensors);
 int soup_grad_square(const void* const* grads, const int64_t* sizes, int count, int dtype, void* workspace,
                      size_t workspace_bytes, int* partials, void* stream);

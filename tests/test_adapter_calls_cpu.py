@@ -33,6 +33,9 @@ def test_addresses_of_many_tensors():
                   torch.zeros(10, dtype=torch.int32), torch.zeros(0)):
         assert _lib.tensor_addresses([good[0], other], _sizes(5000, 10), _lib.F32, cpu) == 1, other
     assert _lib.tensor_addresses([torch.zeros(9, dtype=torch.float16)], _sizes(9), _lib.BF16, cpu) == 0
+    assert _lib.tensor_addresses([base, None], _sizes(5000, 1), _lib.F32, cpu) == 1
+    with pytest.raises(ValueError, match="sizes"):
+        _lib.tensor_addresses([base], _sizes(5000, 1), _lib.F32, cpu)
     # expected on a GPU, found on the host
     assert _lib.tensor_addresses([base], _sizes(5000), _lib.F32, torch.device("cuda", 0)) == 0
     with pytest.raises(Exception):
@@ -40,11 +43,12 @@ def test_addresses_of_many_tensors():
 
 
 def test_addresses_c_arguments():
-    lib, p, bad = _lib.lib(), ctypes.c_void_p(16), ctypes.c_int(0)
-    # never followed: validation fails first
-    for args in ((None, p, p, 1, 0, 1, 0, p), (p, None, p, 1, 0, 1, 0, p), (p, p, None, 1, 0, 1, 0, p),
-                 (p, p, p, 0, 0, 1, 0, p), (p, p, p, 1, 7, 1, 0, p), (p, p, p, 1, 0, 1, 0, None)):
-        assert lib.soup_tensor_addresses(*args, ctypes.byref(bad)) == _lib.SOUP_ERR_INVALID
+    lib, p = _lib.lib(), ctypes.c_void_p(16)  # never followed: validation fails first
+    r, half, empty = ((ctypes.c_void_p * 3)(*v) for v in ((16, 16, 16), (16, 0, 16), (0, 16, 16)))
+    for args in ((None, p, p, 1, 0, 1, 0, p), (half, p, p, 1, 0, 1, 0, p), (empty, p, p, 1, 0, 1, 0, p),
+                 (r, None, p, 1, 0, 1, 0, p), (r, p, None, 1, 0, 1, 0, p), (r, p, p, 0, 0, 1, 0, p),
+                 (r, p, p, 1, 7, 1, 0, p), (r, p, p, 1, 0, 1, 0, None)):
+        assert lib.soup_tensor_addresses(*args) == _lib.SOUP_ERR_INVALID
 
 
 def _held(params):
