@@ -60,8 +60,8 @@ struct Table {
 // stride over the tensors, or walk a run of them each, drifts apart, and DRAM serves many
 // pages at a time: 8-bit states of 233 M bf16 elements took 407 us this way, 464 to 619
 // us with resident CTAs of every depth tried, with or without a ring of cp.async copies.
-// With exactly rounded codes (root_pair, to_codes) it is 425 us, 5.5 TB/s (8 warps a CTA
-// 430, 16 453, 2 473); 100 M fp32 elements with 32-bit states 405 us, 6.9 TB/s.
+// With exactly rounded codes (root_pair, to_codes) it is 417 to 425 us, 5.6 TB/s (8 warps a
+// CTA 430, 16 453, 2 473); 100 M fp32 elements with 32-bit states 405 us, 6.9 TB/s.
 __host__ __device__ constexpr int step_ctas(int es) { return es == 4 ? 10 : 12; }
 
 struct Hyper {

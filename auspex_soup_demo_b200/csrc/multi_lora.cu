@@ -32,7 +32,14 @@
 // adapters), V 68 (dy's 294 MB at 4.3 TB/s), dx 330 (328), dA 17, dB 53 (5.5 TB/s). 48 tokens
 // and 64 adapters: 21 us for 55 MB of weights; 8 tokens of 18944 -> 3584 27 us, 5 TB/s.
 //
-// u and v are rounded to bf16 between the two products, as x, dy and the factors are.
+// u and v are rounded to bf16 between the two products: tcgen05 multiplies operands of one
+// type, and the factors are bf16. Beside the outputs' own rounding (0.00166 of the norm of
+// bf16 values) that is a second one of the same size in every term of dA and dB, 0.00235 by
+// the root of two and as measured, and a small part of y and dx (0.0017 to 0.0018). Held to
+// 16 bits, as a second set of rank columns for the remainders, u and v would take about what
+// twice the columns do: 8192 tokens trained 791 -> 811 us, 2999 ragged ones 193 -> 211, 48
+// tokens of as many adapters up to 17.5 -> 27 (with the factors' bytes doubled too). A step's
+// gradients, which the moments average, are not worth that.
 //
 //   warp 0     TMA producer (one lane)
 //   warp 1     TMEM allocator + MMA issuer (one lane; for gradients it also clears rows)
@@ -618,9 +625,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // U of few tokens: `split` warps a (token, rank column), each its part of k, 16 bytes of x
-// and of A's row a lane and step, eight steps in flight. The projection's kernel streams the
-// weights meanwhile, so that each round trip waits behind those: with four steps in flight
-// and no split 8 tokens of 18944 features took 48 us beside the projection, 19 alone.
+// and of A's row a lane and step, kFewSteps steps in flight. The projection's kernel streams
+// the weights meanwhile, so that each round trip waits behind those: a call of 8 tokens of
+// 18944 -> 3584 features took 53 us with one warp a column (48 of them in this kernel, which
+// takes 19 alone), 27 so.
 constexpr int kFewWarps = 8;
 constexpr int kFewSteps = 4;
 constexpr int kFewFull = 4096;

@@ -134,7 +134,9 @@ def multi_lora_linear(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tenso
     are 0. weight_fn: forms the same weight again; the backward pass then calls it, and the
     weight is not kept for it (``qlora.KEEP_BASE_WEIGHTS``).
 
-    Products accumulate in 32 bits; A x is rounded to bfloat16 before B. Differentiable
+    Products accumulate in 32 bits; A x is rounded to bfloat16 before B (and B^T dy before
+    A and x), which makes the rounding error of the factors' gradients 1.4 times that of
+    their type alone. Differentiable
     with respect to x, lora_a and lora_b, once; gradients have their leaves' types, and
     adapters without tokens get zeros. K, N and adapters * rank must be multiples of
     8, adapters * rank at most 4096. Tokens of one adapter should follow one another,
