@@ -84,8 +84,13 @@ class MultiLoRAFunction(torch.autograd.Function):
         ids, scaling = ids.contiguous(), scaling.contiguous()
         per, shape, a_dtype, b_dtype, (n, k), weight_fn = ctx.meta
         need_x, _, need_a, need_b = ctx.needs_input_grad[:4]
+        if need_x and w is None:
+            w = weight_fn()
+            if w.shape != (n, k) or w.dtype is not torch.bfloat16 or w.device != dy.device:
+                raise ValueError(f"multi_lora_linear: weight_fn formed {w.dtype} {tuple(w.shape)} on {w.device}, the "
+                                 f"forward's weight was bfloat16 {(n, k)} on {dy.device}")
         if need_x:
-            w = _rows(weight_fn() if w is None else w, k)
+            w = _rows(w, k)
         else:
             w = a16.view(-1, k)  # not read
         na, r = a16.shape[0], a16.shape[1]

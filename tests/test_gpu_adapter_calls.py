@@ -262,3 +262,17 @@ def test_clipping_alone_does_not_choose_8_bit_moments():
     for bad in ("soup", "torch"):
         with pytest.raises(ValueError, match="soup32"):
             qlora.QLoRATrainer(_one_adapter(), optimizer=bad, max_grad_norm=1.0)
+
+
+@pytest.mark.parametrize("again", [lambda w: w[:-8], lambda w: w[:, :-8], lambda w: w.float(), lambda w: w.cpu()])
+def test_a_weight_formed_again_is_checked(again):
+    x, w = torch.randn(20, 64, device=DEV).bfloat16().requires_grad_(True), torch.randn(32, 64, device=DEV).bfloat16()
+    a, b = torch.randn(2, 8, 64, device=DEV).bfloat16(), torch.randn(32, 2, 8, device=DEV).bfloat16()
+    ids = torch.zeros(20, dtype=torch.int64, device=DEV)
+    y = kernels.multi_lora_linear(x, w, a, b, ids, weight_fn=lambda: again(w))
+    with pytest.raises(ValueError, match="weight_fn"):
+        y.float().sum().backward()
+    y = kernels.multi_lora_linear(x, w, a, b, ids, weight_fn=lambda: w.t().contiguous().t())  # any strides
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    (want,) = torch.autograd.grad(kernels.multi_lora_linear(x, w, a, b, ids), x, torch.ones_like(y))
+    assert torch.equal(dx, want)
