@@ -10,6 +10,7 @@ attention layers of such a model RMS norms of q and k (``q_norm`` / ``k_norm``, 
 
 from __future__ import annotations
 
+import threading
 import types
 from typing import Optional, Sequence
 
@@ -33,7 +34,7 @@ class MultiAxisRotary(torch.nn.Module):
             raise ValueError("install_heads: a rotary embedding with a scaling factor has no form with several axes")
         self.register_buffer("inv_freq", inv_freq.to(torch.float32), persistent=False)
         self.axes = axes
-        self.positions = None  # [axes, B, S] of the model's call in progress
+        self.positions = {}  # thread -> [axes, B, S] of its call in progress
 
     def _apply(self, fn, *args, **kwargs):
         inv = self._buffers.pop("inv_freq")  # frequencies stay fp32 under model.to(bf16)
@@ -48,19 +49,19 @@ class MultiAxisRotary(torch.nn.Module):
         """Pre-hook of the model's body: positions of several axes go around it, straight to
         :meth:`forward`. The body itself looks for packed sequences in its positions, and has
         a form of that for [B, S] alone; without any it counts 0, 1, 2, ... of each row."""
-        self.positions = None
+        me = threading.get_ident()
+        self.positions.pop(me, None)
         pos = kwargs.get("position_ids") if len(args) < 3 else args[2]
         if pos is None or pos.dim() != 3:
             return None
-        self.positions = pos
+        self.positions[me] = pos
         if len(args) >= 3:
             return (*args[:2], None, *args[3:]), kwargs
         return args, {**kwargs, "position_ids": None}
 
     def forward(self, x, position_ids):
         n = max(self.axes) + 1
-        if self.positions is not None:
-            position_ids, self.positions = self.positions, None
+        position_ids = self.positions.pop(threading.get_ident(), position_ids)
         if position_ids.dim() == 2:
             position_ids = position_ids.unsqueeze(0).expand(n, *position_ids.shape)
         elif position_ids.shape[0] < n:

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import functools
 import math
+import threading
 from typing import Optional, Sequence, Union
 
 import torch
@@ -29,7 +30,7 @@ class AdapterIds:
     def __init__(self, adapters: int):
         self.adapters = adapters
         self.ids: Optional[torch.Tensor] = None
-        self._running = []  # the ids of the layers in progress
+        self._running = {}  # thread -> the ids of its layers in progress
 
     def set(self, ids: Optional[torch.Tensor]) -> None:
         self.ids = self._checked(ids)
@@ -42,7 +43,8 @@ class AdapterIds:
 
     def current(self) -> torch.Tensor:
         """The ids of the layer in progress (outside one: those that are set)."""
-        ids = self._running[-1] if self._running else self.ids
+        running = self._running.get(threading.get_ident())
+        ids = running[-1] if running else self.ids
         if ids is None:
             raise ValueError("the batch's adapter ids are not set (AdapterIds.set, or the trainer's adapter_ids)")
         return ids
@@ -59,12 +61,16 @@ class AdapterIds:
         return args, {**kwargs, "adapter_ids": self.ids if ids is None else self._checked(ids)}
 
     def _enter(self, layer, args, kwargs):
-        self._running.append(kwargs.pop("adapter_ids", self.ids))
+        self._running.setdefault(threading.get_ident(), []).append(kwargs.pop("adapter_ids", self.ids))
         return args, kwargs
 
     def _leave(self, layer, args, output):
-        if self._running:  # (another hook may have raised before _enter)
-            self._running.pop()
+        me = threading.get_ident()
+        running = self._running.get(me)
+        if running:  # (another hook may have raised before _enter)
+            running.pop()
+            if not running:
+                del self._running[me]
 
 
 class _MultiLoRABase(torch.nn.Module):

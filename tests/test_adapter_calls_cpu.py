@@ -4,6 +4,7 @@ between two calls, and calls of the model built of them (in plain torch)."""
 import array
 import ctypes
 import json
+import threading
 
 import pytest
 import torch
@@ -269,3 +270,42 @@ def test_factors_that_are_not_finite_stay_out_of_a_model_with_several_adapters(b
     assert torch.equal(m.model.layers[0].mlp.up_proj.lora_B, before)
     adapter.save_adapter(other, str(tmp_path), index=2)
     adapter.load_adapter(m, str(tmp_path), index=2)
+
+
+def test_two_calls_of_a_model_at_once(monkeypatch):
+    """Two threads, each with its own ids and positions: a call's are its own, whatever the
+    other one does between its layers."""
+    m = _model(monkeypatch)
+    (one, pos), (two, pos2) = _batch(2, seed=1), _batch(2, seed=2)
+    jobs = [(one, pos.flip(1), torch.tensor([0, 1])), (two, pos2, torch.tensor([2, -1]))]
+
+    def call(job):
+        with torch.no_grad():
+            return m(job[0], position_ids=job[1], adapter_ids=job[2]).logits
+
+    want = [call(j) for j in jobs]
+    # the layers and the rotary embedding of both calls in turn
+    turn = threading.Barrier(2, timeout=60)
+
+    def wait(*args):
+        turn.wait()
+
+    for mod in [m.model.rotary_emb, *m.model.layers, *(layer.self_attn.q_proj for layer in m.model.layers)]:
+        mod.register_forward_pre_hook(wait)
+    got = [None, None]
+
+    def run(i):
+        try:
+            got[i] = call(jobs[i])
+        except BaseException:
+            turn.abort()
+            raise
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for w, g in zip(want, got):
+        assert torch.equal(w, g)
+    assert not m.adapter_ids._running and not m.model.rotary_emb.positions
