@@ -201,7 +201,8 @@ def load_adapter(model, directory: str, strict: bool = True, index: Optional[int
             raise KeyError(f"adapter lacks {len(missing)} LoRA tensors, e.g. {missing[:3]}")
         missing = [n for n in trained_beside(model) if n not in seen]
         if missing:
-            raise KeyError(f"adapter lacks {len(missing)} parameters that the model trains, e.g. {missing[:3]}")
+            raise KeyError(f"adapter lacks {len(missing)} parameters that the model trains, e.g. {missing[:3]} "
+                           "(strict=False leaves them as they are)")
     for path, mod in mods.items():
         r = _factors(mod, index)[0].shape[0]
         if int(cfg.get("r", r)) != r:
