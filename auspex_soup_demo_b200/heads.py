@@ -10,8 +10,8 @@ attention layers of such a model RMS norms of q and k (``q_norm`` / ``k_norm``, 
 
 from __future__ import annotations
 
+import functools
 import threading
-import types
 from typing import Optional, Sequence
 
 import torch
@@ -129,5 +129,5 @@ def install_heads(model, qk_norm: bool = True, rope_sections: Optional[Sequence[
                 norm.weight.requires_grad_(train_norms)
                 setattr(attn, name, norm)
         attn.rope_axes = axes
-        attn.forward = types.MethodType(_attention_forward, attn)
+        attn.forward = functools.partial(_attention_forward, attn)  # (a bound method would not unpickle)
     return model

@@ -2,7 +2,9 @@
 between two calls, and calls of the model built of them (in plain torch)."""
 
 import array
+import copy
 import ctypes
+import io
 import json
 import threading
 
@@ -309,3 +311,22 @@ def test_two_calls_of_a_model_at_once(monkeypatch):
     for w, g in zip(want, got):
         assert torch.equal(w, g)
     assert not m.adapter_ids._running and not m.model.rotary_emb.positions
+
+
+def test_copies_of_a_model(monkeypatch):
+    """Deep copies and pickled models are models of their own, heads and adapters with them."""
+    m = _model(monkeypatch)
+    ids, pos = _batch(2)
+    m.adapter_ids.set(torch.tensor([0, 2]))
+    buf = io.BytesIO()
+    torch.save(m, buf)
+    buf.seek(0)
+    with torch.no_grad():
+        want = m(ids, position_ids=pos).logits
+        for other in (copy.deepcopy(m), torch.load(buf, weights_only=False)):
+            assert torch.equal(other(ids, position_ids=pos).logits, want)
+            other.adapter_ids.set(torch.tensor([1, 1]))
+            for p in other.model.layers[0].self_attn.q_norm.parameters():
+                p.mul_(2.0)
+            assert not torch.equal(other(ids, position_ids=pos).logits, want)
+            assert torch.equal(m(ids, position_ids=pos).logits, want)
