@@ -10,6 +10,7 @@ import threading
 
 import pytest
 import torch
+from transformers import DynamicCache
 
 import test_gpu_adapter_model as plain
 from auspex_soup_demo_b200 import _lib, adapter, kernels, optim, qlora
@@ -330,3 +331,18 @@ def test_copies_of_a_model(monkeypatch):
                 p.mul_(2.0)
             assert not torch.equal(other(ids, position_ids=pos).logits, want)
             assert torch.equal(m(ids, position_ids=pos).logits, want)
+
+
+@pytest.mark.parametrize("attention", ["sdpa", "eager"])
+def test_single_tokens_against_a_cache(attention, monkeypatch):
+    """A prompt, a token and a chunk of tokens against a cache, with positions of several axes:
+    the logits of the whole sequence (200 roundings of 2^-24 of numbers of a few units)."""
+    m = _model(monkeypatch, attention)
+    ids, pos = _batch(2)
+    m.adapter_ids.set(torch.tensor([0, 2]))
+    cache = DynamicCache(config=m.config)
+    with torch.no_grad():
+        want = m(ids, position_ids=pos).logits
+        got = [m(ids[:, a:b], position_ids=pos[..., a:b], past_key_values=cache, use_cache=True).logits
+               for a, b in ((0, 7), (7, 8), (8, 12))]
+    assert float((torch.cat(got, 1) - want).abs().max()) <= 200 * 2.0 ** -24 * 8
