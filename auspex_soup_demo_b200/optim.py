@@ -55,7 +55,8 @@ class MultiTensorAdamW(torch.optim.Optimizer):
 
     params: parameters or parameter groups (``lr``, ``betas``, ``eps`` and
     ``weight_decay`` per group) of float32, bfloat16 or float16, contiguous, all on
-    one device. Moments are kept for every parameter from the start:
+    one device; a step refuses those that have become anything else (``p.data = ...``).
+    Moments are kept for every parameter from the start:
 
     * ``state_bits=32``: two fp32 numbers an element;
     * ``state_bits=8``: two e4m3 numbers an element, m and the square root of v, with
